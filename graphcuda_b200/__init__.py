@@ -24,7 +24,8 @@ from .gcn import GCNConv, GCNConvFunction  # noqa: E402
 from .feed import PinnedFeed  # noqa: E402
 from .graphed import GraphedTrainStep  # noqa: E402
 from .losses import argmax_accuracy, log_softmax_nll_loss  # noqa: E402
-from .optim import FusedAdam, FusedSGD  # noqa: E402
+from .norm import RMSNorm, rms_norm, rms_norm_fp8  # noqa: E402
+from .optim import FusedAdam, FusedAdamW, FusedSGD, adamw_moments, adamw_step  # noqa: E402
 from .ops import gemm, get_default_precision, set_default_precision  # noqa: E402
 
 cpp_ext = _graphcuda

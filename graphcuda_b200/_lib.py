@@ -80,6 +80,14 @@ SIGNATURES = {
     "gc_adam_step_f32": (_int, [_int, _void, _void, _void, _void, _void, C.c_double, C.c_double, C.c_double,
                                 C.c_double, C.c_double, _void, _void]),
     "gc_sgd_step_f32": (_int, [_int, _void, _void, _void, C.c_double, C.c_double, _void]),
+    "gc_adamw_step": (_int, [_int, _void, _int, _void, _void, _void, _void, _void, _void, _void, _int, C.c_double,
+                             C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32, _void, _void]),
+    "gc_adamw_moments_f32": (_int, [_int, _void, _void, _void, _void, _void, _void, _void, _void]),
+    "gc_rms_norm_forward": (_int, [_void, _int, _i64, _void, _i64, _int, _f32p, _i64, _i64, C.c_double, _void, _int, _i64,
+                                   _void, _i64, _f32p, _f32p, _void]),
+    "gc_rms_norm_backward_workspace_bytes": (_size, [_i64, _i64]),
+    "gc_rms_norm_backward": (_int, [_void, _int, _i64, _void, _i64, _void, _i64, _void, _i64, _int, _f32p, _f32p, _i64,
+                                    _i64, _void, _int, _i64, _void, _i64, _f32p, _void, _size, _void]),
     "gc_coo_rows_to_rowptr": (_int, [_i64p, _i64, _i64, _i32p, _void]),
     "gc_narrow_i64_i32": (_int, [_i64p, _i32p, _i64, _void]),
     "gc_gcn_norm_f32": (_int, [_i64p, _i64p, _i64, _i64, _f32p, _f32p, _void]),
@@ -100,6 +108,10 @@ SPMM_MAX_BLOCKS = 16
 EPI_RELU = 1
 EPI_ACCUMULATE = 2
 EPI_TRANSPOSED_OUT = 4
+TYPE_F32 = 0
+TYPE_BF16 = 1
+TYPE_E4M3 = 2
+ADAMW_BLOCK = 256
 LAYER_RELU = 1
 LAYER_TRANSFORM_FIRST = 2
 PREC_AUTO = -1

@@ -38,11 +38,12 @@ SOURCES = [
     "gcn_layer.cu",
     "graph_build.cu",
     "loss.cu", "optim.cu",
+    "norm.cu", "adamw.cu",
 ]
 
 HOSTSRC = os.path.join(CSRC, "host")
 HOSTNAME = "_gc_host"
-HOST_SOURCES = ["core.cpp", "layer.cpp", "tail.cpp", "bind.cpp"]
+HOST_SOURCES = ["core.cpp", "layer.cpp", "tail.cpp", "block.cpp", "bind.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

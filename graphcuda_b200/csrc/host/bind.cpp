@@ -268,4 +268,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("argmax_accuracy", &argmax_accuracy, NoGil());
   m.def("adam_step", &adam_step, NoGil());
   m.def("sgd_step", &sgd_step, NoGil());
+
+  m.def("rms_norm", [](const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps,
+                       int64_t y_type) -> std::optional<std::pair<Tensor, Tensor>> {
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return rms_norm(x, weight, residual, eps, y_type);
+  }, NoGil());
+  m.def("rms_norm_fp8", &rms_norm_fp8, NoGil());
+  m.def("rms_norm_forward", [](const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps, int64_t y_type) {
+    const NormForward f = rms_norm_forward(x, weight, residual, eps, int(y_type), true);
+    return std::make_tuple(f.y, f.stream, norm_saved(f));
+  }, NoGil());
+  m.def("rms_norm_backward", [](const OptTensor& dy, const OptTensor& dstream, const Tensor& h, const OptTensor& residual,
+                                const Tensor& weight, const Tensor& rstd, int64_t y_type, int64_t x_type, bool had_residual,
+                                bool need_dx, bool need_dw) {
+    const NormGrads g = rms_norm_backward(dy, dstream, h, residual, weight, rstd, int(y_type), int(x_type), had_residual,
+                                          need_dx, need_dw);
+    return std::make_tuple(g.dx, g.dweight, g.dresidual);
+  }, NoGil());
+  m.def("adamw_step", &adamw_step, NoGil());
+  m.def("adamw_moments", &adamw_moments, NoGil());
 }

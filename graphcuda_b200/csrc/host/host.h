@@ -45,7 +45,9 @@ inline bool f32_on(const Tensor& t, const at::Device& dev) {
   X(gc_mask_mul_f32) X(gc_nll_workspace_bytes) X(gc_logsoftmax_nll_forward_f32) X(gc_logsoftmax_nll_backward_f32)   \
   X(gc_argmax_accuracy_masks_f32) X(gc_logsoftmax_nll_backward_pad_f32) X(gc_adam_step_f32) X(gc_sgd_step_f32) X(gc_csr_is_symmetric) X(gc_pad_rows_f32)                         \
   X(gc_edges_workspace_bytes) X(gc_edges_sort) X(gc_edges_to_csr) X(gc_degree_order_workspace_bytes)                \
-  X(gc_degree_order) X(gc_relu_bias_backward_workspace_bytes) X(gc_relu_bias_backward_f32)
+  X(gc_degree_order) X(gc_relu_bias_backward_workspace_bytes) X(gc_relu_bias_backward_f32)                          \
+  X(gc_rms_norm_forward) X(gc_rms_norm_backward_workspace_bytes) X(gc_rms_norm_backward) X(gc_adamw_step)           \
+  X(gc_adamw_moments_f32)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
   GC_HOST_FUNCTIONS(X)
@@ -182,4 +184,29 @@ std::pair<Tensor, Tensor> argmax_accuracy(const Tensor& logits, const OptTensor&
 void adam_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
                const std::vector<Tensor>& v, double lr, double b1, double b2, double eps, double wd, const Tensor& state);
 void sgd_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, double lr, double wd);
+
+// ------------------------------------------------------------------ between the graph layers (block.cpp)
+struct NormForward {
+  Tensor y, stream, rstd, scale;  // stream: only where there is a residual
+  Tensor x, residual, weight;     // as the kernels took them
+};
+NormForward rms_norm_forward(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps, int y_type,
+                             bool want_rstd);
+std::vector<Tensor> norm_saved(const NormForward& f);
+struct NormGrads {
+  Tensor dx, dresidual, dweight;
+};
+NormGrads rms_norm_backward(const OptTensor& dy, const OptTensor& dstream, const Tensor& h, const OptTensor& residual,
+                            const Tensor& weight, const Tensor& rstd, int y_type, int x_type, bool had_residual,
+                            bool need_dx, bool need_dw);
+std::pair<Tensor, Tensor> rms_norm(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps,
+                                   int64_t y_type);
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                                                double eps);
+void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
+                const std::vector<Tensor>& v, const Tensor& state, const std::vector<Tensor>& masters,
+                const std::vector<Tensor>& m_scales, const std::vector<Tensor>& v_scales, double lr, double b1, double b2,
+                double eps, double wd, int64_t seed);
+void adamw_moments(const std::vector<Tensor>& m, const std::vector<Tensor>& v, const std::vector<Tensor>& m_scales,
+                   const std::vector<Tensor>& v_scales, const std::vector<Tensor>& m_out, const std::vector<Tensor>& v_out);
 }  // namespace gch

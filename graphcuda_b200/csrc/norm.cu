@@ -1,0 +1,594 @@
+// Root-mean-square norm with the residual's addition, forward and backward.
+//
+//   h = x + r,  c = 1 / sqrt(mean(h^2) + eps),  y = h c w           (the new residual stream is h)
+//   dh = c (dy w - hat mean(dy w hat)) + dstream,  hat = h c,  dx = dr = dh,  dw = sum over the rows of dy hat
+//
+// and, for y in 8 bits, one scale per row: s = max|y| / 448, q = e4m3(y / s).
+//
+// Bound by memory: every element is read once and written once and a handful of operations is done on it.  A row is
+// held in the registers of a group of 8, 32 or 256 threads between the pass that sums its squares and the pass that
+// scales it, 8 consecutive elements (16 or 32 bytes) per thread and load; rows whose pitch or base does not allow that
+// are read element by element, in the same kernels with one element per load.  Rows of more than 8192 elements are
+// read twice instead.  Sums and statistics are fp32; h enters the statistics, y and the gradients unrounded, also where
+// the stream that is stored has 16 bits (the backward pass then adds x and r again: from a stream rounded to bf16 the
+// weight gradient would be off by 2e-3).
+//
+// dw: a thread keeps the same columns for all rows of its group and sums them in registers; groups are added through
+// shared memory, CTAs by a second kernel, both in a fixed order.
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxHeld = 8192;  // widest row that is held in registers
+
+using bf16 = __nv_bfloat16;
+
+// N consecutive elements, or one
+template <int VEC>
+__device__ __forceinline__ void load(const float* p, float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void load(const bf16* p, float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[2 * k] = __uint_as_float(w[k] << 16);
+      v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+    }
+  } else {
+    v[0] = __bfloat162float(*p);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_f32(float* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *p = v[0];
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_bf16(bf16* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+    uint4 o;
+    uint32_t* w = &o.x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+      w[k] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+    *reinterpret_cast<uint4*>(p) = o;
+  } else {
+    *p = __float2bfloat16_rn(v[0]);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 8) {
+    uint16_t h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      h[k] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * k], v[2 * k + 1]), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint2*>(p) = make_uint2(uint32_t(h[0]) | uint32_t(h[1]) << 16, uint32_t(h[2]) | uint32_t(h[3]) << 16);
+  } else {
+    *p = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_as(void* base, int type, int64_t at, const float (&v)[VEC]) {
+  if (type == GC_TYPE_F32) store_f32<VEC>(static_cast<float*>(base) + at, v);
+  else if (type == GC_TYPE_BF16) store_bf16<VEC>(static_cast<bf16*>(base) + at, v);
+  else store_e4m3<VEC>(static_cast<uint8_t*>(base) + at, v);
+}
+
+struct Sum {
+  using T = float;
+  static __device__ T of(T a, T b) { return a + b; }
+};
+// The largest of |v| by its bits: a NaN is above infinity and stays.
+struct MaxBits {
+  using T = uint32_t;
+  static __device__ T of(T a, T b) { return max(a, b); }
+};
+// Over a group of G threads; every thread gets the result.  `sm`: one word per warp, for groups of whole CTAs.
+template <int G, class Op>
+__device__ __forceinline__ typename Op::T reduce(typename Op::T v, typename Op::T* sm) {
+  constexpr int kIn = G < 32 ? G : 32;
+#pragma unroll
+  for (int d = kIn / 2; d > 0; d /= 2) v = Op::of(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+  if constexpr (G > 32) {
+    static_assert(G == kThreads, "a group is part of a warp, a warp, or the CTA");
+    __syncthreads();  // the words' readers of the last reduction are done
+    if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = sm[0];
+#pragma unroll
+    for (int w = 1; w < G / 32; ++w) v = Op::of(v, sm[w]);
+  }
+  return v;
+}
+
+// The scale of a row in 8 bits and what its elements are multiplied by.  A row whose scale would be subnormal is stored
+// as zeros; one with a NaN has a NaN for its scale, one with an infinity an infinity.
+__device__ __forceinline__ float2 scale_of(uint32_t top_bits) {
+  const float s = __uint_as_float(top_bits) * (1.0f / 448.0f);
+  if (s < 1.17549435e-38f) return make_float2(0.f, 0.f);
+  return make_float2(s, 1.0f / s);
+}
+
+struct Forward {
+  const void* x;
+  const void* r;  // null: no residual
+  const float* w;
+  void* y;
+  void* stream_out;  // null: not written
+  float* rstd;       // null: not written
+  float* scale;      // for y in 8 bits
+  int64_t ldx, ldr, ldy, lds;
+  int64_t M;
+  int N, y_type;
+  float eps;
+};
+
+// A row per group of G threads, held in ITEMS vectors of VEC elements per thread.
+template <class TX, class TS, int G, int VEC, int ITEMS>
+__global__ void __launch_bounds__(kThreads)
+rms_norm_kernel(Forward f) {
+  __shared__ float sum_s[kThreads / 32];
+  __shared__ uint32_t top_s[kThreads / 32];
+  const int in_group = threadIdx.x % G;
+  const int64_t row = int64_t(blockIdx.x) * (kThreads / G) + threadIdx.x / G;
+  const bool live = row < f.M;  // groups of the last CTA may have none, and take part in the shuffles
+  const TX* x = static_cast<const TX*>(f.x) + row * f.ldx;
+  const TS* r = f.r ? static_cast<const TS*>(f.r) + row * f.ldr : nullptr;
+  float h[ITEMS][VEC], add[ITEMS][VEC];
+  auto column = [&](int i) { return (i * G + in_group) * VEC; };
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const bool ok = live && column(i) < f.N;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) h[i][k] = add[i][k] = 0.f;
+    if (ok) load<VEC>(x + column(i), h[i]);
+    if (ok && r) load<VEC>(r + column(i), add[i]);
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      if (r) h[i][k] += add[i][k];
+      s += h[i][k] * h[i][k];
+    }
+  if (f.stream_out && live) {
+    TS* out = static_cast<TS*>(f.stream_out) + row * f.lds;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (column(i) < f.N) {
+        if constexpr (sizeof(TS) == 4) store_f32<VEC>(out + column(i), h[i]);
+        else store_bf16<VEC>(out + column(i), h[i]);
+      }
+  }
+  s = reduce<G, Sum>(s, sum_s);
+  const float c = rsqrtf(s / float(f.N) + f.eps);
+  if (f.rstd && live && in_group == 0) f.rstd[row] = c;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+    if (column(i) < f.N) {
+      float w[VEC];
+      load<VEC>(f.w + column(i), w);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * c * w[k];
+    }
+  if (f.y_type == GC_TYPE_E4M3) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (column(i) < f.N) top = max(top, __float_as_uint(h[i][k]) & 0x7FFFFFFFu);
+    const float2 sc = scale_of(reduce<G, MaxBits>(top, top_s));
+    if (live && in_group == 0) f.scale[row] = sc.x;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[i][k] *= sc.y;
+  }
+  if (live)
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (column(i) < f.N) store_as<VEC>(f.y, f.y_type, row * f.ldy + column(i), h[i]);
+}
+
+// Rows of more than kMaxHeld elements: a CTA reads the row for its sum, and again to scale it (three times in 8 bits).
+template <class TX, class TS>
+__global__ void __launch_bounds__(kThreads)
+rms_norm_long_kernel(Forward f) {
+  __shared__ float sum_s[kThreads / 32];
+  __shared__ uint32_t top_s[kThreads / 32];
+  const int64_t row = blockIdx.x;
+  const TX* x = static_cast<const TX*>(f.x) + row * f.ldx;
+  const TS* r = f.r ? static_cast<const TS*>(f.r) + row * f.ldr : nullptr;
+  auto at = [&](int n) {
+    float v[1], a[1] = {0.f};
+    load<1>(x + n, v);
+    if (r) load<1>(r + n, a);
+    return r ? v[0] + a[0] : v[0];
+  };
+  float s = 0.f;
+  for (int n = threadIdx.x; n < f.N; n += kThreads) {
+    const float h[1] = {at(n)};
+    s += h[0] * h[0];
+  }
+  s = reduce<kThreads, Sum>(s, sum_s);
+  const float c = rsqrtf(s / float(f.N) + f.eps);
+  if (f.rstd && threadIdx.x == 0) f.rstd[row] = c;
+  float up = 1.f;
+  if (f.y_type == GC_TYPE_E4M3) {
+    uint32_t top = 0;
+    for (int n = threadIdx.x; n < f.N; n += kThreads) top = max(top, __float_as_uint(at(n) * c * f.w[n]) & 0x7FFFFFFFu);
+    const float2 sc = scale_of(reduce<kThreads, MaxBits>(top, top_s));
+    if (threadIdx.x == 0) f.scale[row] = sc.x;
+    up = sc.y;
+  }
+  for (int n = threadIdx.x; n < f.N; n += kThreads) {
+    const float h[1] = {at(n)};  // before the stream is written, which may be the residual itself
+    if (f.stream_out) {
+      if constexpr (sizeof(TS) == 4) store_f32<1>(static_cast<float*>(f.stream_out) + row * f.lds + n, h);
+      else store_bf16<1>(static_cast<bf16*>(f.stream_out) + row * f.lds + n, h);
+    }
+    float y[1] = {h[0] * c * f.w[n]};
+    if (f.y_type == GC_TYPE_E4M3) y[0] *= up;
+    store_as<1>(f.y, f.y_type, row * f.ldy + n, y);
+  }
+}
+
+struct Backward {
+  const void* dy;
+  const void* dstream;  // null: none; of h's type
+  const void* h;        // the stream, or x where the stream's rounding would show
+  const void* r;        // then the residual; null: none
+  const float* w;
+  const float* rstd;
+  void* dx;    // null: not wanted
+  void* dres;  // null: dx serves
+  float* dw;   // partial sums [CTA][N], or the gradient itself when there is one CTA; null: not wanted
+  int64_t lddy, ldds, ldh, ldr, lddx, lddr;
+  int64_t M;
+  int N, dx_type;
+};
+
+// RES: r is there.  Rows are dealt to the groups of a grid of at most some CTAs per SM.
+template <class TH, bool RES, class TY, int G, int VEC, int ITEMS>
+__global__ void __launch_bounds__(kThreads)
+rms_norm_backward_kernel(Backward b) {
+  constexpr int kGroups = kThreads / G;
+  __shared__ float sum_s[kThreads / 32];
+  __shared__ float dw_s[G < kThreads ? kThreads * VEC : 1];
+  const int in_group = threadIdx.x % G, group = threadIdx.x / G;
+  auto column = [&](int i) { return (i * G + in_group) * VEC; };
+  float dw[ITEMS][VEC];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) dw[i][k] = 0.f;
+  const int64_t step = int64_t(gridDim.x) * kGroups;
+  for (int64_t first = int64_t(blockIdx.x) * kGroups; first < b.M; first += step) {  // the same count for all of a CTA
+    const int64_t row = first + group;
+    const bool live = row < b.M;
+    float h[ITEMS][VEC], g[ITEMS][VEC], ds[ITEMS][VEC];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int n = column(i);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) h[i][k] = g[i][k] = ds[i][k] = 0.f;
+      if (live && n < b.N) {
+        load<VEC>(static_cast<const TH*>(b.h) + row * b.ldh + n, h[i]);
+        load<VEC>(static_cast<const TY*>(b.dy) + row * b.lddy + n, g[i]);
+        if (b.dstream) load<VEC>(static_cast<const TH*>(b.dstream) + row * b.ldds + n, ds[i]);
+        if constexpr (RES) {
+          float r[VEC];
+          load<VEC>(static_cast<const TH*>(b.r) + row * b.ldr + n, r);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) h[i][k] += r[k];
+        }
+      }
+    }
+    const float c = live ? b.rstd[row] : 0.f;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      float w[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) w[k] = 0.f;
+      if (column(i) < b.N) load<VEC>(b.w + column(i), w);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float hat = h[i][k] * c;
+        dw[i][k] += g[i][k] * hat;
+        g[i][k] *= w[k];
+        s += g[i][k] * hat;
+        h[i][k] = hat;
+      }
+    }
+    s = reduce<G, Sum>(s, sum_s);
+    const float mean = s / float(b.N);
+    if (live && b.dx)
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        if (column(i) < b.N) {
+          float d[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) d[k] = c * (g[i][k] - h[i][k] * mean) + ds[i][k];
+          store_as<VEC>(b.dx, b.dx_type, row * b.lddx + column(i), d);
+          if (b.dres) store_as<VEC>(b.dres, sizeof(TH) == 4 ? GC_TYPE_F32 : GC_TYPE_BF16, row * b.lddr + column(i), d);
+        }
+  }
+  if (!b.dw) return;
+  float* out = b.dw + int64_t(blockIdx.x) * b.N;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    if constexpr (G < kThreads) {  // the CTA's groups, in their order
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) dw_s[(group * VEC + k) * G + in_group] = dw[i][k];
+      __syncthreads();
+      for (int e = threadIdx.x; e < G * VEC; e += kThreads) {  // element e: vector e % G, place e / G
+        float t = 0.f;
+#pragma unroll 8
+        for (int q = 0; q < kGroups; ++q) t += dw_s[q * VEC * G + e];
+        const int n = (i * G + e % G) * VEC + e / G;
+        if (n < b.N) out[n] = t;
+      }
+    } else if (column(i) < b.N) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) out[column(i) + k] = dw[i][k];
+    }
+  }
+}
+
+// dw = the sum of the CTAs' partial rows: 32 columns per CTA, 8 rows side by side, added in a fixed order.
+__global__ void __launch_bounds__(kThreads)
+rms_norm_dw_kernel(const float* __restrict__ partial, int parts, int N, float* __restrict__ dw) {
+  __shared__ float sm[8][32];
+  const int n = blockIdx.x * 32 + threadIdx.x % 32, q = threadIdx.x / 32;
+  float s = 0.f;
+  if (n < N) {
+#pragma unroll 8
+    for (int p = q; p < parts; p += 8) s += partial[int64_t(p) * N + n];
+  }
+  sm[q][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (q == 0 && n < N) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += sm[k][threadIdx.x];
+    dw[n] = s;
+  }
+}
+
+// Rows of more than kMaxHeld elements, read twice; the weight gradient by columns in a kernel of its own.
+template <class TH, bool RES, class TY>
+__global__ void __launch_bounds__(kThreads)
+rms_norm_backward_long_kernel(Backward b) {
+  __shared__ float sum_s[kThreads / 32];
+  const int64_t row = blockIdx.x;
+  const float c = b.rstd[row];
+  auto at = [&](int n, float& hat, float& g) {
+    float v[1], r[1] = {0.f};
+    load<1>(static_cast<const TH*>(b.h) + row * b.ldh + n, v);
+    if constexpr (RES) load<1>(static_cast<const TH*>(b.r) + row * b.ldr + n, r);
+    hat = (RES ? v[0] + r[0] : v[0]) * c;
+    load<1>(static_cast<const TY*>(b.dy) + row * b.lddy + n, v);
+    g = v[0] * b.w[n];
+  };
+  float s = 0.f, hat, g;
+  for (int n = threadIdx.x; n < b.N; n += kThreads) {
+    at(n, hat, g);
+    s += g * hat;
+  }
+  const float mean = reduce<kThreads, Sum>(s, sum_s) / float(b.N);
+  for (int n = threadIdx.x; n < b.N; n += kThreads) {
+    at(n, hat, g);
+    float d[1] = {0.f};
+    if (b.dstream) load<1>(static_cast<const TH*>(b.dstream) + row * b.ldds + n, d);
+    d[0] += c * (g - hat * mean);
+    store_as<1>(b.dx, b.dx_type, row * b.lddx + n, d);
+    if (b.dres) store_as<1>(b.dres, sizeof(TH) == 4 ? GC_TYPE_F32 : GC_TYPE_BF16, row * b.lddr + n, d);
+  }
+}
+template <class TH, bool RES, class TY>
+__global__ void __launch_bounds__(kThreads)
+rms_norm_dw_long_kernel(Backward b) {
+  const int n = blockIdx.x * kThreads + threadIdx.x;
+  if (n >= b.N) return;
+  const int64_t per = (b.M + gridDim.y - 1) / gridDim.y;
+  float s = 0.f;
+  for (int64_t row = blockIdx.y * per; row < min(b.M, (blockIdx.y + 1) * per); ++row) {
+    float v[1], r[1] = {0.f}, g[1];
+    load<1>(static_cast<const TH*>(b.h) + row * b.ldh + n, v);
+    if constexpr (RES) load<1>(static_cast<const TH*>(b.r) + row * b.ldr + n, r);
+    load<1>(static_cast<const TY*>(b.dy) + row * b.lddy + n, g);
+    s += g[0] * ((RES ? v[0] + r[0] : v[0]) * b.rstd[row]);
+  }
+  b.dw[int64_t(blockIdx.y) * b.N + n] = s;
+}
+
+// ------------------------------------------------------------------ host
+bool known(int type, bool eight) { return type == GC_TYPE_F32 || type == GC_TYPE_BF16 || (eight && type == GC_TYPE_E4M3); }
+size_t size_of(int type) { return type == GC_TYPE_F32 ? 4 : type == GC_TYPE_BF16 ? 2 : 1; }
+
+// Whether rows of this matrix can be read 8 elements at a time in accesses of 16 bytes (8 for 8-bit elements).
+bool vector_rows(const void* p, int type, int64_t ld) {
+  if (!p) return true;
+  const size_t unit = type == GC_TYPE_E4M3 ? 8 : 16;
+  return reinterpret_cast<uintptr_t>(p) % unit == 0 && size_t(ld) * size_of(type) % unit == 0;
+}
+
+// The group that holds a row, and how many vectors each of its threads has.  Smallest that fits: a row of 64 elements
+// takes 8 threads of a warp, one of up to 1024 a warp, beyond that the CTA.
+template <class F>
+void with_shape(bool vec, int N, F&& go) {
+#define GC_SHAPE(G, V, I) go(std::integral_constant<int, G>{}, std::integral_constant<int, V>{}, std::integral_constant<int, I>{})
+  if (vec) {
+    if (N <= 64) GC_SHAPE(8, 8, 1);
+    else if (N <= 256) GC_SHAPE(32, 8, 1);
+    else if (N <= 512) GC_SHAPE(32, 8, 2);
+    else if (N <= 1024) GC_SHAPE(32, 8, 4);
+    else if (N <= 2048) GC_SHAPE(256, 8, 1);
+    else if (N <= 4096) GC_SHAPE(256, 8, 2);
+    else GC_SHAPE(256, 8, 4);
+  } else {
+    if (N <= 64) GC_SHAPE(8, 1, 8);
+    else if (N <= 256) GC_SHAPE(32, 1, 8);
+    else if (N <= 1024) GC_SHAPE(32, 1, 32);
+    else if (N <= 2048) GC_SHAPE(256, 1, 8);
+    else GC_SHAPE(256, 1, 32);
+  }
+#undef GC_SHAPE
+}
+
+template <class TX, class TS>
+int launch_forward(const Forward& f, bool vec, cudaStream_t st) {
+  if (f.N > kMaxHeld) {
+    if (f.M > 0x7FFFFFFF) return gc::fail(GC_ERR_UNSUPPORTED, "gc_rms_norm_forward: too many rows");
+    rms_norm_long_kernel<TX, TS><<<unsigned(f.M), kThreads, 0, st>>>(f);
+  } else {
+    int64_t blocks = 0;
+    with_shape(vec, f.N, [&](auto g, auto v, auto items) {
+      constexpr int G = decltype(g)::value;
+      blocks = gc::ceil_div(f.M, kThreads / G);
+      if (blocks <= 0x7FFFFFFF)
+        rms_norm_kernel<TX, TS, G, decltype(v)::value, decltype(items)::value><<<unsigned(blocks), kThreads, 0, st>>>(f);
+    });
+    if (blocks > 0x7FFFFFFF) return gc::fail(GC_ERR_UNSUPPORTED, "gc_rms_norm_forward: too many rows");
+  }
+  return gc::check_launch("gc_rms_norm_forward");
+}
+
+// CTAs that a backward launch deals its rows to: some per SM, so that the weight gradient has that many partial rows.
+int64_t backward_ctas(int64_t M, int64_t N) {
+  if (N > kMaxHeld) return std::min<int64_t>(gc::ceil_div(M, 64), 64);
+  const int groups = N <= 64 ? 32 : N <= 1024 ? 8 : 1;
+  return std::min<int64_t>(gc::ceil_div(M, groups), gc::kNumSMs * 4);
+}
+
+template <class TH, bool RES, class TY>
+int launch_backward(Backward b, bool vec, float* dw, float* partial, cudaStream_t st) {
+  const int64_t ctas = backward_ctas(b.M, b.N);
+  b.dw = !dw ? nullptr : ctas == 1 ? dw : partial;
+  int launches = 0;
+  if (b.N > kMaxHeld) {
+    if (b.M > 0x7FFFFFFF) return gc::fail(GC_ERR_UNSUPPORTED, "gc_rms_norm_backward: too many rows");
+    if (b.dx) {
+      rms_norm_backward_long_kernel<TH, RES, TY><<<unsigned(b.M), kThreads, 0, st>>>(b);
+      ++launches;
+    }
+    if (dw) {
+      rms_norm_dw_long_kernel<TH, RES, TY><<<dim3(unsigned(gc::ceil_div(b.N, kThreads)), unsigned(ctas)), kThreads, 0, st>>>(b);
+      ++launches;
+    }
+  } else {
+    with_shape(vec, b.N, [&](auto g, auto v, auto items) {
+      rms_norm_backward_kernel<TH, RES, TY, decltype(g)::value, decltype(v)::value, decltype(items)::value>
+          <<<unsigned(ctas), kThreads, 0, st>>>(b);
+    });
+    ++launches;
+  }
+  if (dw && ctas > 1) {
+    rms_norm_dw_kernel<<<unsigned(gc::ceil_div(b.N, 32)), kThreads, 0, st>>>(partial, int(ctas), b.N, dw);
+    ++launches;
+  }
+  return gc::check_launch("gc_rms_norm_backward", launches);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gc_rms_norm_forward(const void* x, int x_type, int64_t ldx, const void* residual, int64_t ldr, int stream_type,
+                        const float* weight, int64_t M, int64_t N, double eps, void* y, int y_type, int64_t ldy,
+                        void* stream_out, int64_t lds, float* rstd, float* scale, void* stream) {
+  GC_REQUIRE(M >= 0 && N >= 0, "gc_rms_norm_forward: negative size");
+  GC_REQUIRE(known(x_type, false) && known(stream_type, false) && known(y_type, true), "gc_rms_norm_forward: unknown type");
+  GC_REQUIRE(x_type == stream_type || (residual && x_type == GC_TYPE_BF16),
+             "gc_rms_norm_forward: x has the stream's type, or is bf16 beside an fp32 stream");
+  if (M == 0 || N == 0) return GC_OK;
+  GC_REQUIRE(N < (int64_t(1) << 31) - 8192, "gc_rms_norm_forward: rows of 2^31 elements and more are not served");
+  GC_REQUIRE(x && weight && y, "gc_rms_norm_forward: null pointer");
+  GC_REQUIRE(y_type != GC_TYPE_E4M3 || scale, "gc_rms_norm_forward: 8-bit rows need room for their scales");
+  GC_REQUIRE(ldx >= N && ldy >= N && (!residual || ldr >= N) && (!stream_out || lds >= N),
+             "gc_rms_norm_forward: leading dimension below the row length");
+  Forward f{x, residual, weight, y, stream_out, rstd, scale, ldx, ldr, ldy, lds, M, int(N), y_type, float(eps)};
+  const bool vec = N % 8 == 0 && vector_rows(x, x_type, ldx) && vector_rows(residual, stream_type, ldr) &&
+                   vector_rows(y, y_type, ldy) && vector_rows(stream_out, stream_type, lds) && gc::aligned16(weight);
+  const cudaStream_t st = gc::as_stream(stream);
+  if (x_type == GC_TYPE_F32) return launch_forward<float, float>(f, vec, st);
+  if (stream_type == GC_TYPE_F32) return launch_forward<bf16, float>(f, vec, st);
+  return launch_forward<bf16, bf16>(f, vec, st);
+}
+
+size_t gc_rms_norm_backward_workspace_bytes(int64_t M, int64_t N) {
+  if (M <= 0 || N <= 0) return 0;
+  const int64_t ctas = backward_ctas(M, N);
+  return ctas > 1 ? size_t(ctas) * size_t(N) * sizeof(float) : 0;
+}
+
+int gc_rms_norm_backward(const void* dy, int dy_type, int64_t lddy, const void* dstream, int64_t ldds, const void* h,
+                         int64_t ldh, const void* residual, int64_t ldr, int stream_type, const float* weight,
+                         const float* rstd, int64_t M, int64_t N, void* dx, int dx_type, int64_t lddx, void* dresidual,
+                         int64_t lddr, float* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  GC_REQUIRE(M >= 0 && N >= 0, "gc_rms_norm_backward: negative size");
+  GC_REQUIRE(known(dy_type, false) && known(stream_type, false) && known(dx_type, false),
+             "gc_rms_norm_backward: unknown type");
+  const cudaStream_t st = gc::as_stream(stream);
+  if (N == 0) return GC_OK;
+  GC_REQUIRE(N < (int64_t(1) << 31) - 8192, "gc_rms_norm_backward: rows of 2^31 elements and more are not served");
+  if (M == 0) {
+    if (dweight && cudaMemsetAsync(dweight, 0, size_t(N) * sizeof(float), st) != cudaSuccess)
+      return gc::fail(GC_ERR_CUDA, "gc_rms_norm_backward: %s", cudaGetErrorString(cudaGetLastError()));
+    return GC_OK;
+  }
+  GC_REQUIRE(dy && h && weight && rstd, "gc_rms_norm_backward: null pointer");
+  GC_REQUIRE(!residual || stream_type == GC_TYPE_BF16,
+             "gc_rms_norm_backward: an fp32 stream is exact, and taken instead of x and the residual");
+  GC_REQUIRE(dx || !dresidual, "gc_rms_norm_backward: dresidual alone is what dx of that type would be");
+  GC_REQUIRE(lddy >= N && ldh >= N && (!dstream || ldds >= N) && (!residual || ldr >= N) && (!dx || lddx >= N) &&
+                 (!dresidual || lddr >= N),
+             "gc_rms_norm_backward: leading dimension below the row length");
+  if (!dx && !dweight) return GC_OK;
+  const size_t need = dweight ? gc_rms_norm_backward_workspace_bytes(M, N) : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return gc::fail(GC_ERR_WORKSPACE, "gc_rms_norm_backward: workspace missing or smaller than its query says");
+  GC_REQUIRE(!need || reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "gc_rms_norm_backward: workspace is not aligned");
+  Backward b{dy, dstream, h, residual, weight, rstd, dx, dresidual, nullptr, lddy, ldds, ldh, ldr, lddx, lddr, M, int(N),
+             dx_type};
+  const bool vec = N % 8 == 0 && vector_rows(dy, dy_type, lddy) && vector_rows(dstream, stream_type, ldds) &&
+                   vector_rows(h, stream_type, ldh) && vector_rows(residual, stream_type, ldr) &&
+                   vector_rows(dx, dx_type, lddx) && vector_rows(dresidual, stream_type, lddr) && gc::aligned16(weight);
+  float* partial = static_cast<float*>(workspace);
+  const bool y32 = dy_type == GC_TYPE_F32;
+  if (stream_type == GC_TYPE_F32)
+    return y32 ? launch_backward<float, false, float>(b, vec, dweight, partial, st)
+               : launch_backward<float, false, bf16>(b, vec, dweight, partial, st);
+  if (residual)
+    return y32 ? launch_backward<bf16, true, float>(b, vec, dweight, partial, st)
+               : launch_backward<bf16, true, bf16>(b, vec, dweight, partial, st);
+  return y32 ? launch_backward<bf16, false, float>(b, vec, dweight, partial, st)
+             : launch_backward<bf16, false, bf16>(b, vec, dweight, partial, st);
+}
+
+}  // extern "C"

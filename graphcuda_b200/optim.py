@@ -3,7 +3,7 @@
 
 ``FusedAdam`` follows ``torch.optim.Adam`` (amsgrad / maximize off) and
 ``FusedSGD`` the momentum-free ``torch.optim.SGD`` the reference's script
-builds; both update every parameter of the model with one kernel
+builds (``FusedAdamW``, for deeper models, has its own notes below); both update every parameter of the model with one kernel
 (``gc_adam_step_f32`` / ``gc_sgd_step_f32``).  The Adam step count lives on the
 device, so ``step()`` can be recorded in a CUDA graph and replayed
 (graphed.GraphedTrainStep); ``lr`` is read on the host when the launch is
@@ -89,3 +89,126 @@ class FusedSGD(torch.optim.Optimizer):
                     chunk = ps[i:i + _MAX]
                     _lib.host.sgd_step(chunk, [p.grad for p in chunk], group["lr"], group["weight_decay"])
         return loss
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, masters=None, scales=None, seed: int = 0) -> None:
+    """One AdamW step over lists of tensors, in place; one launch per 440 tensors.
+
+    ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
+    ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)``.
+
+    ``params`` and ``grads`` are all float32, or all bfloat16 beside float32 ``masters``, which take the update.
+    ``exp_avgs`` and ``exp_avg_sqs`` are float32; or uint8 (zeros at the start) with ``scales = (of exp_avgs, of
+    exp_avg_sqs)``, float32 tensors of ceil(size / 256) elements each: 8 bits per value, rounded at random by a hash of
+    (seed, step, position in the list, element).  ``step`` is a CUDA int64 tensor of two elements, zeros at the start; the
+    kernel counts in it, so the call can be recorded in a CUDA graph."""
+    of_m, of_v = scales if scales is not None else ((), ())
+    _lib.host.adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, masters or (), of_m, of_v, lr, betas[0], betas[1], eps,
+                         weight_decay, seed & 0xFFFFFFFF)
+
+
+def adamw_moments(exp_avgs, exp_avg_sqs, scales, out=None):
+    """The values that moments in 8 bits stand for: two lists of float32 tensors (``out``, where given)."""
+    if out is None:
+        out = tuple([torch.empty(t.shape, dtype=torch.float32, device=t.device) for t in ts] for ts in (exp_avgs, exp_avg_sqs))
+    _lib.host.adamw_moments(exp_avgs, exp_avg_sqs, scales[0], scales[1], out[0], out[1])
+    return out
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW (``torch.optim.AdamW``, amsgrad and maximize off) for any number of tensors in one launch.
+
+    Float32 parameters are updated as they are; bfloat16 ones beside a float32 master in the optimizer's state.
+    ``state_bits=8`` holds both moments in 8 bits with a float32 scale per 256 elements (see ``adamw_step``): 2 bytes per
+    parameter instead of 8.  Tensors of 256 elements and fewer keep 32 bits: there is nothing to save in them."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 state_bits: int = 32, seed: int = 0):
+        if lr < 0 or eps < 0 or not 0 <= betas[0] < 1 or not 0 <= betas[1] < 1 or weight_decay < 0:
+            raise ValueError("FusedAdamW: invalid hyper-parameter")
+        if state_bits not in (8, 32):
+            raise ValueError("FusedAdamW: state_bits must be 8 or 32")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, seed=seed))
+
+    def _new_state(self, p, bits):
+        st, n = {}, p.numel()
+        kind = torch.uint8 if bits == 8 and n > _lib.ADAMW_BLOCK else torch.float32
+        for name in ("exp_avg", "exp_avg_sq"):
+            st[name] = torch.zeros(p.shape, dtype=kind, device=p.device)
+            if kind == torch.uint8:
+                st[name + "_scale"] = torch.zeros(-(-n // _lib.ADAMW_BLOCK), dtype=torch.float32, device=p.device)
+        if p.dtype == torch.bfloat16:
+            st["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format)
+        return st
+
+    def _together(self, group):
+        """The group's parameters that have a gradient, as lists that one launch updates: of one device and type, and of one
+        step count -- parameters that have always been updated together share the tensor that holds it."""
+        fresh, launches, members = {}, {}, {}
+        for p in group["params"]:
+            st = self.state[p] if p.grad is not None else self.state.get(p)
+            if p.grad is not None and not st:
+                st.update(self._new_state(p, group["state_bits"]))
+                key = (p.device, p.dtype, st["exp_avg"].dtype)
+                if key not in fresh:
+                    fresh[key] = torch.zeros(2, dtype=torch.int64, device=p.device)
+                st["step"] = fresh[key]
+            if not st:
+                continue
+            members[id(st["step"])] = members.get(id(st["step"]), 0) + 1
+            if p.grad is not None:
+                launches.setdefault(id(st["step"]), []).append(p)
+        for key, ps in launches.items():
+            if len(ps) < members[key]:  # the others keep the old count
+                step = self.state[ps[0]]["step"].clone()
+                for p in ps:
+                    self.state[p]["step"] = step
+        return launches.values()
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for ps in self._together(group):
+                st = [self.state[p] for p in ps]
+                of = lambda name: [x[name] for x in st]  # noqa: E731
+                eight = st[0]["exp_avg"].dtype == torch.uint8
+                adamw_step(ps, [p.grad for p in ps], of("exp_avg"), of("exp_avg_sq"), st[0]["step"], lr=group["lr"],
+                           betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                           masters=of("master") if "master" in st[0] else None,
+                           scales=(of("exp_avg_scale"), of("exp_avg_sq_scale")) if eight else None, seed=group["seed"])
+        return loss
+
+    def moments(self, p):
+        """(exp_avg, exp_avg_sq) of a parameter as float32 tensors, whatever they are held in."""
+        st = self.state[p]
+        if st["exp_avg"].dtype != torch.uint8:
+            return st["exp_avg"], st["exp_avg_sq"]
+        m, v = adamw_moments([st["exp_avg"]], [st["exp_avg_sq"]], ([st["exp_avg_scale"]], [st["exp_avg_sq_scale"]]))
+        return m[0], v[0]
+
+    def steps_taken(self) -> int:
+        """Reads the largest step count back (synchronises)."""
+        return max((int(st["step"][0].item()) for st in self.state.values()), default=0)
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # The base class casts states to the parameter's type: here their types are their own.
+        saved = {i: st for i, st in state_dict["state"].items()}
+        order = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        shared = {}
+        for i, p in zip(order, params):
+            if i not in saved:
+                continue
+            st = {k: v.detach().to(p.device, copy=True) for k, v in saved[i].items()}
+            # Equal counts are shared again, within what one launch updates.
+            group = next(n for n, g in enumerate(self.param_groups) if any(q is p for q in g["params"]))
+            key = (group, p.device, p.dtype, st["exp_avg"].dtype, int(st["step"][0].item()))
+            st["step"] = shared.setdefault(key, st["step"])
+            self.state[p] = st

@@ -10,8 +10,8 @@
  * GC_ERR_* code; gc_last_error() gives a thread-local message for the last
  * failure on the calling thread.
  *
- * All matrices are row-major fp32.  "ld" is the distance in elements between
- * consecutive rows.
+ * All matrices are row-major, and fp32 where nothing else is said.  "ld" is the
+ * distance in elements between consecutive rows.
  *
  * Each declaration cites the reference interface (path within the GraphCUDA
  * project : lines) whose work it takes over.
@@ -32,6 +32,11 @@ extern "C" {
 #define GC_ERR_CUDA (-3)         /* a CUDA runtime / driver call or kernel launch failed */
 #define GC_ERR_WORKSPACE (-4)    /* workspace pointer null or too small */
 #define GC_ERR_DEVICE_FLAG (-5)  /* a kernel reported a bounded wait that ran out (read back by gc_gemm_check_flag) */
+
+/* Element types where an entry point takes several. */
+#define GC_TYPE_F32 0
+#define GC_TYPE_BF16 1
+#define GC_TYPE_E4M3 2 /* 8 bits: sign, 4 of exponent (bias 7), 3 of mantissa; largest value 448 */
 
 /* ---- library ---------------------------------------------------------- */
 
@@ -425,6 +430,59 @@ int gc_adam_step_f32(int n_tensors, float* const* params, const float* const* gr
                      void* state, void* stream);
 int gc_sgd_step_f32(int n_tensors, float* const* params, const float* const* grads, const int64_t* sizes,
                     double lr, double weight_decay, void* stream);
+
+/*
+ * AdamW (decay decoupled from the gradient) for every tensor of a model; no counterpart in the reference.  The arrays
+ * are HOST arrays of any number of device pointers / element counts, read during the call, tensors contiguous:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * param_type: GC_TYPE_F32, or GC_TYPE_BF16 for parameters and gradients in bf16 beside fp32 masters, which take the update
+ * and are rounded into the parameters (masters is not read for GC_TYPE_F32).
+ * state_bits 32: exp_avg and exp_avg_sq are fp32 (the scales are not read).  8: they are bytes, in blocks of
+ * GC_ADAMW_BLOCK elements of a tensor with an fp32 scale each (ceil(size / GC_ADAMW_BLOCK) per tensor): e4m3, and the
+ * upper byte of a positive fp16 number without its sign bit; all zero at the start.  Their values are rounded up or
+ * down at random by a hash of (seed, step, tensor, element), the same on every run.  A block that has met a NaN or an
+ * infinity keeps one for its scale.
+ * state: 16 bytes of device memory as for gc_adam_step_f32.  One launch per 440 tensors.
+ */
+#define GC_ADAMW_BLOCK 256
+int gc_adamw_step(int n_tensors, void* const* params, int param_type, const void* const* grads, float* const* masters,
+                  void* const* exp_avg, void* const* exp_avg_sq, float* const* exp_avg_scales,
+                  float* const* exp_avg_sq_scales, const int64_t* sizes, int state_bits,
+                  double lr, double beta1, double beta2, double eps, double weight_decay, uint32_t seed,
+                  void* state, void* stream);
+/* The values that moments in 8 bits stand for, as fp32 tensors. */
+int gc_adamw_moments_f32(int n_tensors, const uint8_t* const* exp_avg, const uint8_t* const* exp_avg_sq,
+                         const float* const* exp_avg_scales, const float* const* exp_avg_sq_scales,
+                         const int64_t* sizes, float* const* exp_avg_out, float* const* exp_avg_sq_out, void* stream);
+
+/* ---- root-mean-square norm ------------------------------------------------ */
+
+/*
+ * h = x + residual (x where residual is null), rows of N elements;  y = h / sqrt(mean(h^2) + eps) * weight.
+ * No counterpart in the reference: what a stack of more layers than its two needs between them.
+ * Types: x and the stream (residual in, h out) both fp32 or both bf16, or x in bf16 beside an fp32 stream; y fp32,
+ * bf16 or e4m3; weight fp32.  In 8 bits y = e4m3(value / scale[row]) with scale[row] = max |value| / 448 (0 for a row
+ * of zeros).  h enters y unrounded.  stream_out (h, may be the residual's own memory) and rstd (1 / the root, for the
+ * backward pass) may be null.
+ */
+int gc_rms_norm_forward(const void* x, int x_type, int64_t ldx, const void* residual, int64_t ldr, int stream_type,
+                        const float* weight, int64_t M, int64_t N, double eps,
+                        void* y, int y_type, int64_t ldy, void* stream_out, int64_t lds, float* rstd, float* scale,
+                        void* stream);
+/*
+ * dx = dresidual = rstd (dy weight - hat mean(dy weight hat)) + dstream, hat = h rstd;  dweight = sum over rows of
+ * dy hat.  dstream (gradient of h through its other uses, of the stream's type) may be null.  h: the fp32 stream, or
+ * x where it was rounded to bf16, with `residual` beside it (then h + residual is formed again, unrounded; null where
+ * there was none).  dx has x's type; dresidual (the stream's type) is for streams of another type than x's, null
+ * otherwise.  dx or dweight may be null (not computed).  Sums in a fixed order.
+ */
+size_t gc_rms_norm_backward_workspace_bytes(int64_t M, int64_t N);
+int gc_rms_norm_backward(const void* dy, int dy_type, int64_t lddy, const void* dstream, int64_t ldds,
+                         const void* h, int64_t ldh, const void* residual, int64_t ldr, int stream_type,
+                         const float* weight, const float* rstd, int64_t M, int64_t N,
+                         void* dx, int dx_type, int64_t lddx, void* dresidual, int64_t lddr, float* dweight,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- adjacency construction (reference tests/gcn/graphcuda_impl.py:27-38) - */
 
