@@ -20,6 +20,7 @@ from ._graphcuda import (gemm_cublas, matmul1, matmul2, matmul3, matmul4,  # noq
                          spmm_cusparse)
 from .adjacency import (CSRAdjacency, DenseAdjacency, as_adjacency, degree_order, gcn_norm,  # noqa: E402
                         normalized_adjacency)
+from .ffn import GatedFFN, gated_ffn, gated_ffn_fp8, quantize_weight_fp8  # noqa: E402
 from .gcn import GCNConv, GCNConvFunction  # noqa: E402
 from .feed import PinnedFeed  # noqa: E402
 from .graphed import GraphedTrainStep  # noqa: E402

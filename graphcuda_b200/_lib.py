@@ -88,6 +88,15 @@ SIGNATURES = {
     "gc_rms_norm_backward_workspace_bytes": (_size, [_i64, _i64]),
     "gc_rms_norm_backward": (_int, [_void, _int, _i64, _void, _i64, _void, _i64, _void, _i64, _int, _f32p, _f32p, _i64,
                                     _i64, _void, _int, _i64, _void, _i64, _f32p, _void, _size, _void]),
+    "gc_gated_ffn_hidden_pitch": (_i64, [_i64]),
+    "gc_gated_ffn_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _int]),
+    "gc_gated_ffn_forward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _i64, _i64, _i64, _i64, _int, _void, _i64,
+                                         _void, _void, _void, _size, _void]),
+    "gc_gated_ffn_backward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _void, _i64, _void, _void, _i64, _i64, _i64,
+                                          _i64, _int, _void, _i64, _void, _i64, _void, _i64, _void, _size, _void]),
+    "gc_gated_ffn_e4m3_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
+    "gc_gated_ffn_forward_e4m3": (_int, [_void, _i64, _f32p, _void, _i64, _f32p, _void, _i64, _i64, _i64, _i64, _i64, _int,
+                                         _void, _i64, _void, _size, _void]),
     "gc_coo_rows_to_rowptr": (_int, [_i64p, _i64, _i64, _i32p, _void]),
     "gc_narrow_i64_i32": (_int, [_i64p, _i32p, _i64, _void]),
     "gc_gcn_norm_f32": (_int, [_i64p, _i64p, _i64, _i64, _f32p, _f32p, _void]),
@@ -112,6 +121,9 @@ TYPE_F32 = 0
 TYPE_BF16 = 1
 TYPE_E4M3 = 2
 ADAMW_BLOCK = 256
+ACT_SILU = 0
+ACT_GELU = 1
+ACT_RELU = 2
 LAYER_RELU = 1
 LAYER_TRANSFORM_FIRST = 2
 PREC_AUTO = -1

@@ -38,7 +38,7 @@ SOURCES = [
     "gcn_layer.cu",
     "graph_build.cu",
     "loss.cu", "optim.cu",
-    "norm.cu", "adamw.cu",
+    "norm.cu", "adamw.cu", "ffn.cu",
 ]
 
 HOSTSRC = os.path.join(CSRC, "host")

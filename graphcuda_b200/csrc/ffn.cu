@@ -1,0 +1,974 @@
+// Gated feed-forward block on the 5th-generation tensor cores, forward and backward, bf16 (or e4m3 into the first product).
+//
+//   forward    G = X Wg, U = X Wu, A = act(G) * U, Y = A Wo                   [Wg | Wu] is one matrix, D x 2H
+//   backward   dA = dY Wo^T, dU = dA act(G), dG = dA U act'(G)
+//              dX = [dG | dU] [Wg | Wu]^T, d[Wg | Wu] = X^T [dG | dU], dWo = A^T dY
+//
+// One kernel, three epilogues:
+//   Gated      the accumulators of a tile hold as many columns of G as of U (the same ones), so the epilogue has both and stores A
+//              alone; for a backward pass G and U are stored beside it
+//   GatedBack  the accumulator is a tile of dA, which is never stored: the epilogue reads G and U and stores dG and dU
+//   Plain      a bf16 product: Y, dX and the weight gradients
+// Operands are read where they lie: K-major or MN-major tiles (matrices whose rows run along the product's K or across it),
+// so nothing is transposed in memory.  Sums are fp32 in TMEM.  A, G, U, dG and dU are rounded to bf16 where they are stored
+// between kernels: they are the next product's operands, which the tensor core takes in 16 bits; every one adds a
+// relative 2^-9 at random, as the output's own rounding does.
+//
+// CTA = 12 warps, persistent over tiles of 128 x BN accumulators (or a pair of CTAs over 256 x BN):
+//   warp 0       TMA producer (one lane)
+//   warp 1       MMA issuer (one lane)
+//   warp 2       TMEM allocator
+//   warps 4-11   epilogue: two warps per TMEM lane quarter, one for the even 64-column chunks, one for the odd ones; a
+//                chunk leaves through a swizzled 32 x 64 tile in shared memory and one TMA store
+// Two accumulators in TMEM let the epilogue of a tile overlap the main loop of the next.  Products with few tiles and a
+// long K are split along K into fp32 parts that a second kernel adds in a fixed order.
+//
+// Every wait on a barrier is bounded, as in the other tensor-core kernel: a wait that ran out raises the device's error
+// word, all roles leave, copies in flight are drained and TMEM is released.
+#include "common.cuh"
+#include "gemm_internal.cuh"
+#include "tcgen05.cuh"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+namespace {
+
+using namespace gc::tc;
+using bf16 = __nv_bfloat16;
+
+constexpr int BM = 128;
+constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;
+constexpr int kTileBytes = 32 * 128;  // what a warp stores at once: 32 rows of 128 bytes
+constexpr int kBuffers = 2;           // of them per warp
+
+enum Kind { kPlain, kGated, kGatedBack };
+
+template <int BN, bool PAIR>
+struct Cfg {
+  static constexpr int BNC = PAIR ? BN / 2 : BN;  // rows of B that a CTA holds
+  static constexpr int kABytes = BM * 128, kBBytes = BNC * 128;  // a stage has 128 bytes of K
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStaging = kEpiWarps * kBuffers * kTileBytes;
+  static constexpr int kStages = std::min(8, (227 * 1024 - 1024 - 512 - kStaging) / kStageBytes);
+  static constexpr int kSmemBytes = kStages * kStageBytes + kStaging + 512 /*barriers*/ + 1024 /*alignment slack*/;
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static_assert(kSmemBytes <= 227 * 1024 && kStages >= 3, "shared memory budget");
+  static_assert(kTmemCols >= 32 && kTmemCols <= 512, "two accumulators in TMEM");
+};
+
+struct Params {
+  int M, N, K;  // of the product; Gated: N = H, the columns of G and of U
+  int b_up;     // Gated: where U's columns start in B
+  int act;
+  int save;         // Gated: G and U are stored
+  const float* sa;  // e4m3: scales of A's rows and B's columns
+  const float* sb;
+  bf16* C;  // Plain: the output, for rows that TMA cannot store
+  int64_t ldc;
+  int tma_store;
+  // columns of the product -> the c_cols columns of C: those from `gap_from` on move down by `gap`, over the ones in between
+  int gap_from, gap, c_cols;
+  int splits, kb_per_split;
+  int* word;  // the device's error word
+};
+
+// One MMA of 32 bytes of K.
+template <bool PAIR, bool F8>
+__device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+#define GC_UMMA(GROUP, KIND)                                                                    \
+  asm volatile(                                                                                 \
+      "{\n\t.reg .pred p;\n\t"                                                                  \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                               \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)                                       \
+      : "memory")
+  if constexpr (PAIR && F8) GC_UMMA("2", "f8f6f4");
+  else if constexpr (PAIR) GC_UMMA("2", "f16");
+  else if constexpr (F8) GC_UMMA("1", "f8f6f4");
+  else GC_UMMA("1", "f16");
+#undef GC_UMMA
+}
+
+// Instruction descriptor, fp32 accumulation.  Operand formats: kind::f16 1 = bf16; kind::f8f6f4 0 = e4m3.
+__host__ __device__ constexpr uint32_t make_idesc(int bm, int bn, bool a_mn, bool b_mn, bool f8) {
+  return (1u << 4) | (uint32_t(f8 ? 0 : 1) << 7) | (uint32_t(f8 ? 0 : 1) << 10) | (uint32_t(a_mn) << 15) |
+         (uint32_t(b_mn) << 16) | (uint32_t(bn >> 3) << 17) | (uint32_t(bm >> 4) << 24);
+}
+
+// Tiles in shared memory are rows of 128 bytes under the 128-byte swizzle (16-byte atoms).  K-major: a row is 128 bytes of K
+// of one index, 8-row groups 1024 bytes apart, one MMA takes 32 bytes of every row.  MN-major (bf16): a row is 64
+// consecutive indices at one k, 8-k groups 1024 bytes apart, 64-index blocks 64 rows (8192 bytes) apart, one MMA
+// takes 16 rows.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, bool mn_major) {
+  return mn_major ? smem_desc(saddr, 64 * 128, 1024, 2u) : smem_desc(saddr, 0, 1024, 2u);
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y),
+               "r"(z), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// At most N of this thread's stores still read shared memory.
+template <int N>
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// Waits for a copy in flight whatever else has failed (bounded): it must have landed before the CTA may exit.
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    if (mbar_test(bar, parity)) break;
+    __nanosleep(64);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// act(g) and, for the backward pass, its derivative.
+template <int ACT>
+__device__ __forceinline__ float activate(float g, float& slope) {
+  if constexpr (ACT == GC_ACT_SILU) {
+    const float s = __fdividef(1.f, 1.f + __expf(-g));
+    slope = s + g * s * (1.f - s);
+    return g * s;
+  } else if constexpr (ACT == GC_ACT_GELU) {
+    const float cdf = 0.5f + 0.5f * erff(g * 0.70710678118654752f);
+    slope = cdf + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
+    return g * cdf;
+  } else {
+    slope = g > 0.f ? 1.f : 0.f;
+    return g <= 0.f ? 0.f : g;  // a NaN stays
+  }
+}
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
+  if (act == GC_ACT_SILU) f(std::integral_constant<int, GC_ACT_SILU>{});
+  else if (act == GC_ACT_GELU) f(std::integral_constant<int, GC_ACT_GELU>{});
+  else f(std::integral_constant<int, GC_ACT_RELU>{});
+}
+
+// The 16-byte unit `j` of a lane's row in a warp's swizzled tile.
+__device__ __forceinline__ uint4* unit(uint8_t* tile, int row, int j) {
+  return reinterpret_cast<uint4*>(tile + row * 128 + ((j ^ (row & 7)) << 4));
+}
+
+// Where a column of the product goes (see Params); one that is dropped goes beyond the last.
+__device__ __forceinline__ int out_column(int n, int gap_from, int gap) {
+  return n < gap_from ? n : n < gap_from + gap ? 0x7FFFFFFF : n - gap;
+}
+
+struct Maps {
+  CUtensorMap a, b;
+  CUtensorMap out;      // Plain: C, or the fp32 parts; Gated: A; GatedBack: dG
+  CUtensorMap out2;     // Gated: G; GatedBack: dU
+  CUtensorMap out3;     // Gated: U
+  CUtensorMap in1, in2;  // GatedBack: G, U
+};
+
+// A_MN / B_MN: the operand is MN-major.  F8: e4m3 operands (K-major).  PAIR: two CTAs of a cluster work on a tile of 256 rows,
+// each with its 128 rows of A and half of B's (Gated: rank 0 has G's columns, rank 1 U's).
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  using C_ = Cfg<BN, PAIR>;
+  constexpr int S = C_::kStages, BNC = C_::BNC;
+  constexpr int KE = F8 ? 128 : 64;  // K elements per stage
+  constexpr int TM = PAIR ? 2 * BM : BM;
+  constexpr int NT = KIND == kGated ? BN / 2 : BN;  // output columns of a tile
+  static_assert(!F8 || (!A_MN && !B_MN && KIND == kGated), "e4m3 operands are K-major");
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
+  const int first_item = PAIR ? int(blockIdx.x / 2) : int(blockIdx.x);
+  const int item_step = PAIR ? int(gridDim.x / 2) : int(gridDim.x);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  auto sA = [&](int s) { return base + s * C_::kStageBytes; };
+  auto sB = [&](int s) { return base + s * C_::kStageBytes + C_::kABytes; };
+  constexpr int kStagingAt = S * C_::kStageBytes;
+  const uint32_t bars = base + kStagingAt + C_::kStaging;
+  auto bar_full = [&](int s) { return bars + 8 * s; };
+  auto bar_empty = [&](int s) { return bars + 8 * (S + s); };
+  auto bar_tfull = [&](int b) { return bars + 8 * (2 * S + b); };
+  auto bar_tempty = [&](int b) { return bars + 8 * (2 * S + 2 + b); };
+  auto bar_in = [&](int w) { return bars + 8 * (2 * S + 4 + w); };  // GatedBack: a warp's G and U have landed
+  static_assert(8 * (2 * S + 4 + kEpiWarps) <= 512, "room for the barriers");
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_s;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int tiles_n = (p.N + NT - 1) / NT;
+  const int tiles_m = (p.M + TM - 1) / TM;
+  const int nkb_total = (p.K + KE - 1) / KE;
+  const int splits = KIND == kPlain ? p.splits : 1;
+  const int kb_per = splits > 1 ? p.kb_per_split : nkb_total;
+  const int num_items = tiles_m * tiles_n * splits;  // (split, m, n), n fastest
+  auto item_coords = [&](int item, int& m0, int& n0, int& kb0, int& kb1, int& split) {
+    const int t = item % (tiles_m * tiles_n);
+    split = item / (tiles_m * tiles_n);
+    m0 = (t / tiles_n) * TM + int(rank) * BM;  // first row of this CTA's half
+    n0 = (t % tiles_n) * NT;
+    kb0 = split * kb_per;
+    kb1 = min(nkb_total, kb0 + kb_per);
+  };
+
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    for (int s = 0; s < S; ++s) {
+      mbar_init(bar_full(s), 1);
+      mbar_init(bar_empty(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_tfull(b), 1);
+      mbar_init(bar_tempty(b), kEpiWarps * (PAIR ? 2 : 1));
+    }
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(bar_in(w), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  if (PAIR) {
+    __syncthreads();
+    cluster_sync_all();  // both CTAs' barriers exist before either is signalled
+  }
+  if (warp == 2) tmem_alloc<PAIR>(smem_u32(&tmem_base_s), C_::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+  volatile int* abort_p = &abort_s;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int item = first_item; item < num_items && ok; item += item_step) {
+        int m0, n0, kb0, kb1, split;
+        item_coords(item, m0, n0, kb0, kb1, split);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(bar_empty(s), ((it / S) & 1u) ^ 1u, abort_p)) { ok = false; break; }
+          // a pair's copies are all counted at the leader
+          if (!PAIR) mbar_expect_tx(bar_full(s), C_::kStageBytes);
+          else if (rank == 0) mbar_expect_tx(bar_full(s), 2 * C_::kStageBytes);
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+            if (PAIR) tma_load_2d_leader(dst, map, x, y, bar_full(s));
+            else tma_load_2d(dst, map, x, y, bar_full(s));
+          };
+          if (A_MN) {
+#pragma unroll
+            for (int c = 0; c < BM / 64; ++c) load(sA(s) + c * (64 * 128), &maps.a, m0 + c * 64, kb * KE);
+          } else {
+            load(sA(s), &maps.a, kb * KE, m0);
+          }
+          // B's rows n of this CTA: Gated takes the tile's columns of G, then the same of U
+          auto load_b = [&](int at, int n, int rows) {
+            if (B_MN) {
+              for (int c = 0; c < rows / 64; ++c) load(sB(s) + (at + c * 64) * 128, &maps.b, n + c * 64, kb * KE);
+            } else {
+              load(sB(s) + at * 128, &maps.b, kb * KE, n);
+            }
+          };
+          if (KIND == kGated && PAIR) {
+            load_b(0, (rank ? p.b_up : 0) + n0, BNC);
+          } else if (KIND == kGated) {
+            load_b(0, n0, BN / 2);
+            load_b(BN / 2, p.b_up + n0, BN / 2);
+          } else {
+            load_b(0, n0 + int(rank) * BNC, BNC);
+          }
+        }
+      }
+      // every copy issued must have landed before the CTA may exit (counted at the leader, for whom the peer waits)
+      const uint32_t pending = PAIR && rank != 0 ? 0u : it < uint32_t(S) ? it : uint32_t(S);
+      for (uint32_t j = 0; j < pending; ++j) {
+        const uint32_t q = it - 1 - j;
+        drain(bar_full(q % S), (q / S) & 1u);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = make_idesc(TM, BN, A_MN, B_MN, F8);
+      constexpr uint32_t kAStep = A_MN ? 16 * 128 : 32, kBStep = B_MN ? 16 * 128 : 32;  // bytes per MMA
+      uint32_t it = 0, tcount = 0;
+      bool ok = true;
+      for (int item = first_item; item < num_items && ok; item += item_step, ++tcount) {
+        int m0, n0, kb0, kb1, split;
+        item_coords(item, m0, n0, kb0, kb1, split);
+        const int b = tcount & 1;
+        if (!mbar_wait(bar_tempty(b), ((tcount >> 1) & 1u) ^ 1u, abort_p)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + uint32_t(b * BN);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(bar_full(s), (it / S) & 1u, abort_p)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t da = operand_desc(sA(s), A_MN), db = operand_desc(sB(s), B_MN);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma<PAIR, F8>(d_tmem, da + ((k * kAStep) >> 4), db + ((k * kBStep) >> 4), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          umma_commit<PAIR>(bar_empty(s));  // frees the stage once these MMAs have read it
+        }
+        if (ok) umma_commit<PAIR>(bar_tfull(b));
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp % 4;             // TMEM lane quarter
+    const int grp = (warp - 4) / 4;     // parity of the 64-column chunks
+    uint8_t* tiles = smem + kStagingAt + (warp - 4) * (kBuffers * kTileBytes);
+    const uint32_t tiles_u = smem_u32(tiles);
+    int buf = 0;
+    // The next of the warp's tiles, once the store that read it last has done so.
+    auto acquire = [&]() {
+      if (lane == 0) store_wait_read<kBuffers - 1>();
+      __syncwarp();
+      const int b = buf;
+      buf = (buf + 1) % kBuffers;
+      return b;
+    };
+    // Hands a tile to the TMA store.
+    auto put = [&](const CUtensorMap* map, int b, int x, int y) {
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(map, tiles_u + b * kTileBytes, x, y);
+        store_commit();
+      }
+    };
+    uint32_t tcount = 0, loads = 0;
+    bool ok = true;
+    for (int item = first_item; item < num_items && ok; item += item_step, ++tcount) {
+      int m0, n0, kb0, kb1, split;
+      item_coords(item, m0, n0, kb0, kb1, split);
+      const int b = tcount & 1;
+      const int row0 = m0 + q * 32;  // first of the warp's rows
+      const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * BN);
+      bool have_in = false;  // GatedBack: the first chunk's G and U are on their way while the tile is being computed
+      auto request = [&](int col) {
+        if (lane == 0) {
+          store_wait_read<0>();
+          mbar_expect_tx(bar_in(warp - 4), 2 * kTileBytes);
+          tma_load_2d(tiles_u, &maps.in1, col, row0, bar_in(warp - 4));
+          tma_load_2d(tiles_u + kTileBytes, &maps.in2, col, row0, bar_in(warp - 4));
+        }
+      };
+      if (KIND == kGatedBack && n0 + grp * 64 < p.N && row0 < p.M) {
+        request(n0 + grp * 64);
+        have_in = true;
+      }
+      if (!mbar_wait(bar_tfull(b), (tcount >> 1) & 1u, abort_p)) ok = false;
+      if (ok) tc_fence_after();
+      if constexpr (KIND == kGatedBack) {
+        for (int c = grp; c < NT / 64; c += 2) {
+          const int col = n0 + c * 64;
+          if (col >= p.N || row0 >= p.M) break;
+          if (!have_in) {
+            if (!ok) break;
+            request(col);
+          }
+          have_in = false;
+          if (!mbar_wait(bar_in(warp - 4), loads & 1u, abort_p)) {
+            drain(bar_in(warp - 4), loads & 1u);
+            ok = false;
+          }
+          ++loads;
+          if (!ok) break;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            uint32_t acc[32];
+            tmem_ld32(taddr + uint32_t(c * 64 + half * 32), acc);
+            tmem_ld_wait();
+            with_activation(p.act, [&](auto act) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint4* gp = unit(tiles, lane, half * 4 + j);
+                uint4* up = unit(tiles + kTileBytes, lane, half * 4 + j);
+                uint4 g4 = *gp, u4 = *up;
+                uint32_t* gw = &g4.x;
+                uint32_t* uw = &u4.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float d0 = __uint_as_float(acc[j * 8 + 2 * e]), d1 = __uint_as_float(acc[j * 8 + 2 * e + 1]);
+                  float s0, s1;
+                  const float a0 = activate<decltype(act)::value>(low(gw[e]), s0);
+                  const float a1 = activate<decltype(act)::value>(high(gw[e]), s1);
+                  gw[e] = pack2(d0 * low(uw[e]) * s0, d1 * high(uw[e]) * s1);
+                  uw[e] = pack2(d0 * a0, d1 * a1);
+                }
+                *gp = g4;
+                *up = u4;
+              }
+            });
+          }
+          put(&maps.out, 0, col, row0);
+          put(&maps.out2, 1, col, row0);
+        }
+      } else if (ok && KIND == kGated) {
+        const float sa = F8 ? p.sa[min(row0 + lane, p.M - 1)] : 1.f;
+        for (int c = grp; c < NT / 64; c += 2) {
+          const int col = n0 + c * 64;
+          if (col >= p.N || row0 >= p.M) break;
+          const int ba = acquire();
+          uint32_t hold_g[32], hold_u[32];  // packed, 64 columns each, where they are stored too
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t g[32], u[32];
+            tmem_ld32(taddr + uint32_t(c * 64 + half * 32), g);
+            tmem_ld32(taddr + uint32_t(NT + c * 64 + half * 32), u);
+            tmem_ld_wait();
+            if (F8) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int n = min(col + half * 32 + j, p.N - 1);
+                g[j] = __float_as_uint(__uint_as_float(g[j]) * (sa * __ldg(p.sb + n)));
+                u[j] = __float_as_uint(__uint_as_float(u[j]) * (sa * __ldg(p.sb + p.b_up + n)));
+              }
+            }
+            if (!F8 && p.save) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                hold_g[half * 16 + j] = pack2(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1]));
+                hold_u[half * 16 + j] = pack2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+              }
+            }
+            with_activation(p.act, [&](auto act) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint4 o;
+                uint32_t* w = &o.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int i = j * 8 + 2 * e;
+                  float unused;
+                  w[e] = pack2(activate<decltype(act)::value>(__uint_as_float(g[i]), unused) * __uint_as_float(u[i]),
+                               activate<decltype(act)::value>(__uint_as_float(g[i + 1]), unused) * __uint_as_float(u[i + 1]));
+                }
+                *unit(tiles + ba * kTileBytes, lane, half * 4 + j) = o;
+              }
+            });
+          }
+          put(&maps.out, ba, col, row0);
+          if (!F8 && p.save) {
+            const int bg = acquire();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *unit(tiles + bg * kTileBytes, lane, j) =
+                  make_uint4(hold_g[4 * j], hold_g[4 * j + 1], hold_g[4 * j + 2], hold_g[4 * j + 3]);
+            put(&maps.out2, bg, col, row0);
+            const int bu = acquire();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *unit(tiles + bu * kTileBytes, lane, j) =
+                  make_uint4(hold_u[4 * j], hold_u[4 * j + 1], hold_u[4 * j + 2], hold_u[4 * j + 3]);
+            put(&maps.out3, bu, col, row0);
+          }
+        }
+      } else if (ok && splits > 1) {
+        // fp32 parts, 32 columns at a time
+        for (int c = grp; c < NT / 32; c += 2) {
+          const int col = n0 + c * 32;
+          if (col >= p.N || row0 >= p.M) break;
+          uint32_t acc[32];
+          tmem_ld32(taddr + uint32_t(c * 32), acc);
+          const int bo = acquire();
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *unit(tiles + bo * kTileBytes, lane, j) = make_uint4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&maps.out, tiles_u + bo * kTileBytes, col, row0, split);
+            store_commit();
+          }
+        }
+      } else if (ok) {
+        for (int c = grp; c < NT / 64; c += 2) {
+          const int col = n0 + c * 64;
+          if (col >= p.N || row0 >= p.M) break;
+          const int bo = acquire();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t acc[32];
+            tmem_ld32(taddr + uint32_t(c * 64 + half * 32), acc);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint4 o;
+              uint32_t* w = &o.x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack2(__uint_as_float(acc[j * 8 + 2 * e]), __uint_as_float(acc[j * 8 + 2 * e + 1]));
+              *unit(tiles + bo * kTileBytes, lane, half * 4 + j) = o;
+            }
+          }
+          if (p.tma_store) {
+            put(&maps.out, bo, col, row0);
+          } else {
+            // rows of an odd pitch: two neighbouring columns per lane, row by row
+            __syncwarp();
+            const int rows = min(32, p.M - row0);
+            for (int r = 0; r < rows; ++r) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(
+                  reinterpret_cast<const uint8_t*>(unit(tiles + bo * kTileBytes, r, lane / 4)) + (lane % 4) * 4);
+              bf16* out = p.C + int64_t(row0 + r) * p.ldc;
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int n = out_column(col + 2 * lane + e, p.gap_from, p.gap);
+                if (n < p.c_cols) out[n] = __ushort_as_bfloat16(uint16_t(e ? w >> 16 : w));
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_leader(bar_tempty(b));
+        else mbar_arrive(bar_tempty(b));
+      }
+    }
+    if (lane == 0) store_wait_all();  // shared memory is read until then
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync_all();  // the peer's MMAs read this CTA's shared memory and write its TMEM until here
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc<PAIR>(tmem_base, C_::kTmemCols);
+  if (threadIdx.x == 0 && abort_s) atomicExch(p.word, 1);
+}
+
+// C (bf16) = the sum of the fp32 parts [split][M][pitch] in their order, four columns per thread.
+__global__ void __launch_bounds__(256)
+ffn_sum_kernel(const float* __restrict__ parts, int splits, int M, int pitch, bf16* __restrict__ C, int64_t ldc, int c_cols,
+               int gap_from, int gap) {
+  const int64_t quads = int64_t(M) * (pitch / 4);
+  const bool vec = gap == 0 && c_cols % 4 == 0 && ldc % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 8 == 0;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < quads; i += int64_t(gridDim.x) * 256) {
+    const int64_t m = i / (pitch / 4);
+    const int n = int(i % (pitch / 4)) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(parts + (int64_t(z) * M + m) * pitch + n));
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    if (vec) {
+      *reinterpret_cast<uint2*>(C + m * ldc + n) = make_uint2(pack2(s.x, s.y), pack2(s.z, s.w));
+    } else {
+      const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = out_column(n + e, gap_from, gap);
+        if (c < c_cols) C[m * ldc + c] = __float2bfloat16_rn(v[e]);
+      }
+    }
+  }
+}
+
+// dst[r, c] = src[r, c] for c < cols, 0 up to the pitch ldd: rows that TMA can read.
+template <class T>
+__global__ void __launch_bounds__(256)
+repitch_kernel(const T* __restrict__ src, int64_t lds, T* __restrict__ dst, int64_t ldd, int64_t rows, int cols, int width) {
+  const int64_t total = rows * width;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const int64_t r = i / width;
+    const int c = int(i % width);
+    dst[r * ldd + c] = c < cols ? src[r * lds + c] : T(0);
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct Matrix {  // row-major, `size` bytes per element
+  const void* p;
+  int64_t rows, cols, ld;
+  int size;
+};
+
+int make_map(CUtensorMap* map, const Matrix& m, int box_cols, int box_rows, int64_t planes = 0) {
+  EncodeFn enc = get_encode();
+  if (!enc) return gc::fail(GC_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  const cuuint64_t dims[3] = {cuuint64_t(m.cols), cuuint64_t(m.rows), cuuint64_t(planes)};
+  const cuuint64_t strides[2] = {cuuint64_t(m.ld) * m.size, cuuint64_t(m.ld) * m.size * m.rows};
+  const cuuint32_t box[3] = {cuuint32_t(box_cols), cuuint32_t(box_rows), 1u};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type = m.size == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : m.size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUresult r = enc(map, type, planes ? 3 : 2, const_cast<void*>(m.p), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return gc::fail(GC_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
+  return GC_OK;
+}
+
+inline int64_t up8(int64_t x) { return (x + 7) & ~int64_t(7); }
+inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// A launch's tile: accumulator columns, and whether CTAs work in pairs.
+struct Tile {
+  int bn;
+  bool pair;
+};
+// Pairs of CTAs on 256 x 256 where that gives every pair a tile; 128 x 128 below, and 128 x 64 where even those are fewer
+// than the SMs (a product with few rows is bound by reading B, which more CTAs do faster).
+Tile pick_tile(Kind kind, int64_t M, int64_t N, int64_t splits_possible) {
+  const int64_t n_acc = kind == kGated ? 2 * N : N;
+  const int64_t big = gc::ceil_div(M, 256) * gc::ceil_div(n_acc, 256) * splits_possible;
+  if (M > BM && n_acc > 128 && big >= gc::kNumSMs / 2) return {256, true};
+  if (kind == kGated) return {128, false};
+  const int64_t mid = gc::ceil_div(M, BM) * gc::ceil_div(n_acc, 128) * splits_possible;
+  return {n_acc > 64 && mid >= gc::kNumSMs ? 128 : 64, false};
+}
+// Plain products with fewer tiles than CTAs and a long K are cut along K.
+struct Split {
+  Tile tile;
+  int splits, per;
+};
+Split plan_plain(int64_t M, int64_t N, int64_t K) {
+  const int64_t nkb = gc::ceil_div(K, 64);
+  Split s;
+  s.tile = pick_tile(kPlain, M, N, std::max<int64_t>(1, nkb / 8));
+  const int64_t tm = s.tile.pair ? 256 : BM, units = s.tile.pair ? gc::kNumSMs / 2 : gc::kNumSMs;
+  const int64_t tiles = gc::ceil_div(M, tm) * gc::ceil_div(N, s.tile.bn);
+  int64_t splits = 1;
+  if (tiles * 2 <= units && nkb >= 8) splits = std::min<int64_t>(units / tiles, nkb / 4);
+  s.per = int(gc::ceil_div(nkb, std::max<int64_t>(1, splits)));
+  s.splits = int(gc::ceil_div(nkb, s.per));
+  return s;
+}
+inline int64_t part_pitch(int64_t N) { return (N + 3) & ~int64_t(3); }
+size_t plain_workspace(int64_t M, int64_t N, int64_t K) {
+  const Split s = plan_plain(M, N, K);
+  return s.splits > 1 ? align256(size_t(s.splits) * size_t(M) * size_t(part_pitch(N)) * 4) : 0;
+}
+
+int error_word(int** word) {
+  static int* cached[64] = {};  // by device; the address does not change
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return gc::fail(GC_ERR_CUDA, "no current device");
+  if (dev < 64 && cached[dev]) {
+    *word = cached[dev];
+    return GC_OK;
+  }
+  int32_t* w = nullptr;
+  const int rc = gc::wait_error_word(&w);
+  if (rc != GC_OK) return rc;
+  if (dev < 64) cached[dev] = w;
+  *word = w;
+  return GC_OK;
+}
+
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR>
+int launch_kernel(const Maps& maps, const Params& p, cudaStream_t st) {
+  using C_ = Cfg<BN, PAIR>;
+  auto kern = ffn_kernel<KIND, BN, A_MN, B_MN, F8, PAIR>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::kSmemBytes);
+  if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  constexpr int kCtas = PAIR ? 2 : 1;
+  constexpr int NT = KIND == kGated ? BN / 2 : BN;
+  const int64_t items = gc::ceil_div(p.M, BM * kCtas) * gc::ceil_div(p.N, NT) * (KIND == kPlain ? p.splits : 1);
+  if (items > 0x7FFFFFFF) return gc::fail(GC_ERR_UNSUPPORTED, "gated feed-forward: too many tiles");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>(items, gc::kNumSMs / kCtas)) * kCtas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C_::kSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kern, maps, p);
+  return gc::check_launch("ffn_kernel");
+}
+template <int KIND, bool A_MN, bool B_MN, bool F8>
+int launch_tile(const Tile& t, const Maps& maps, const Params& p, cudaStream_t st) {
+  if (t.pair) return launch_kernel<KIND, 256, A_MN, B_MN, F8, true>(maps, p, st);
+  if constexpr (KIND != kGated)
+    if (t.bn == 64) return launch_kernel<KIND, 64, A_MN, B_MN, F8, false>(maps, p, st);
+  return launch_kernel<KIND, 128, A_MN, B_MN, F8, false>(maps, p, st);
+}
+
+// The maps of the operands.  A and B: matrices as they lie; K-major ones have K in their rows.
+int operand_maps(Maps& maps, const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int b_rows) {
+  const int ke = 128 / A.size;  // K elements of a stage
+  int rc = a_mn ? make_map(&maps.a, A, 64, 64) : make_map(&maps.a, A, ke, BM);
+  if (rc == GC_OK) rc = b_mn ? make_map(&maps.b, B, 64, 64) : make_map(&maps.b, B, ke, b_rows);
+  return rc;
+}
+
+// C (M x N, bf16) = A B, fp32 sums.
+int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int64_t N, int64_t K, bf16* C, int64_t ldc,
+          int64_t gap_from, int64_t gap, void* workspace, cudaStream_t st) {
+  if (M == 0 || N == 0) return GC_OK;
+  const Split s = plan_plain(M, N, K);
+  Maps maps;
+  Params p{};
+  p.M = int(M); p.N = int(N); p.K = int(K);
+  p.C = C; p.ldc = ldc;
+  p.gap_from = gap ? int(gap_from) : int(N);
+  p.gap = int(gap);
+  p.c_cols = int(N - 2 * gap);  // [G | U] with the pads behind both
+  p.splits = s.splits; p.kb_per_split = s.per;
+  p.tma_store = gap == 0 && ldc % 8 == 0 && gc::aligned16(C);
+  int rc = error_word(&p.word);
+  if (rc == GC_OK) rc = operand_maps(maps, A, a_mn, B, b_mn, s.tile.pair ? s.tile.bn / 2 : s.tile.bn);
+  const int64_t pitch = part_pitch(N);
+  if (rc == GC_OK && s.splits > 1) rc = make_map(&maps.out, Matrix{workspace, M, N, pitch, 4}, 32, 32, s.splits);
+  else if (rc == GC_OK && p.tma_store) rc = make_map(&maps.out, Matrix{C, M, N, ldc, 2}, 64, 32);
+  if (rc != GC_OK) return rc;
+  if (a_mn) rc = launch_tile<kPlain, true, true, false>(s.tile, maps, p, st);
+  else if (b_mn) rc = launch_tile<kPlain, false, true, false>(s.tile, maps, p, st);
+  else rc = launch_tile<kPlain, false, false, false>(s.tile, maps, p, st);
+  if (rc != GC_OK || s.splits == 1) return rc;
+  const int64_t quads = M * (pitch / 4);
+  ffn_sum_kernel<<<unsigned(std::min<int64_t>(gc::ceil_div(quads, 256), gc::kNumSMs * 8)), 256, 0, st>>>(
+      static_cast<const float*>(workspace), s.splits, int(M), int(pitch), C, ldc, p.c_cols, p.gap_from, p.gap);
+  return gc::check_launch("ffn_sum_kernel");
+}
+
+// A matrix that TMA can read: itself, or a copy with a pitch of 16 bytes in the workspace, which moves on.
+bool readable(const Matrix& m) { return gc::aligned16(m.p) && m.ld * m.size % 16 == 0; }
+int64_t readable_ld(const Matrix& m) { return (m.cols * m.size + 15) / 16 * 16 / m.size; }
+size_t copy_bytes(const Matrix& m) { return readable(m) ? 0 : align256(size_t(m.rows) * size_t(readable_ld(m)) * m.size); }
+template <class T>
+int repitch(const Matrix& m, void* dst, int64_t ldd, int64_t width, cudaStream_t st) {
+  const int64_t total = m.rows * width;
+  repitch_kernel<T><<<unsigned(std::min<int64_t>(gc::ceil_div(total, 256), gc::kNumSMs * 16)), 256, 0, st>>>(
+      static_cast<const T*>(m.p), m.ld, static_cast<T*>(dst), ldd, m.rows, int(m.cols), int(width));
+  return gc::check_launch("repitch_kernel");
+}
+int make_readable(Matrix& m, char*& ws, cudaStream_t st) {
+  if (readable(m)) return GC_OK;
+  const size_t bytes = copy_bytes(m);
+  const int64_t ld = readable_ld(m);
+  const int rc = m.size == 2 ? repitch<uint16_t>(m, ws, ld, ld, st) : repitch<uint8_t>(m, ws, ld, ld, st);
+  m.p = ws;
+  m.ld = ld;
+  ws += bytes;
+  return rc;
+}
+// [Wg | Wu]: where H is not a multiple of 8, U's columns are moved to the next one, and the columns between are zeros -- as are
+// then those of G, U, A and their gradients.
+size_t gate_up_bytes(const Matrix& w, int64_t H) {
+  return H % 8 == 0 ? copy_bytes(w) : align256(size_t(w.rows) * size_t(2 * up8(H)) * 2);
+}
+int make_gate_up(Matrix& w, int64_t H, char*& ws, cudaStream_t st) {
+  if (H % 8 == 0) return make_readable(w, ws, st);
+  const int64_t hp = up8(H);
+  uint16_t* to = reinterpret_cast<uint16_t*>(ws);
+  Matrix gate{w.p, w.rows, H, w.ld, 2}, up{static_cast<const uint16_t*>(w.p) + H, w.rows, H, w.ld, 2};
+  int rc = repitch<uint16_t>(gate, to, 2 * hp, hp, st);
+  if (rc == GC_OK) rc = repitch<uint16_t>(up, to + hp, 2 * hp, hp, st);
+  ws += gate_up_bytes(w, H);
+  w = Matrix{to, w.rows, 2 * hp, 2 * hp, 2};
+  return rc;
+}
+
+bool sizes_ok(int64_t M, int64_t D, int64_t H, int64_t O) {
+  const int64_t top = (int64_t(1) << 31) - 512;  // coordinates and tile counts are 32-bit
+  return M <= top && D <= top && 2 * up8(H) <= top && O <= top;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t gc_gated_ffn_hidden_pitch(int64_t H) { return up8(std::max<int64_t>(H, 0)); }
+
+size_t gc_gated_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O, int backward) {
+  if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, D, H, O)) return 0;
+  const int64_t hp = up8(H);
+  // copies of every operand, should none be readable in place
+  size_t b = align256(size_t(M) * up8(D) * 2) + align256(size_t(D) * 2 * hp * 2) + align256(size_t(H) * up8(O) * 2);
+  if (!backward) return b + align256(size_t(M) * hp * 2) + plain_workspace(M, O, H);
+  b += align256(size_t(M) * up8(O) * 2) + align256(size_t(M) * 2 * hp * 2);  // dY, dG | dU
+  return b + std::max({plain_workspace(M, D, 2 * hp), plain_workspace(D, 2 * hp, M), plain_workspace(H, O, M)});
+}
+
+int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin, const uint16_t* Wout,
+                              int64_t ldwout, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy,
+                              uint16_t* hidden, uint16_t* gate_up, void* workspace, size_t workspace_bytes, void* stream) {
+  GC_REQUIRE(M >= 0 && D >= 0 && H >= 0 && O >= 0, "gc_gated_ffn_forward_bf16: negative size");
+  GC_REQUIRE(act >= GC_ACT_SILU && act <= GC_ACT_RELU, "gc_gated_ffn_forward_bf16: unknown activation");
+  GC_REQUIRE(ldx >= D && ldwin >= 2 * H && ldwout >= O && ldy >= O,
+             "gc_gated_ffn_forward_bf16: leading dimension below the row length");
+  if (!sizes_ok(M, D, H, O)) return gc::fail(GC_ERR_UNSUPPORTED, "gc_gated_ffn_forward_bf16: a size beyond 2^31");
+  const cudaStream_t st = gc::as_stream(stream);
+  if (M == 0 || O == 0) return GC_OK;
+  GC_REQUIRE(Y, "gc_gated_ffn_forward_bf16: null pointer");
+  const int64_t hp = up8(H);
+  if (D == 0 || H == 0) {  // G = U = 0, or no hidden columns: Y = 0
+    cudaError_t e = cudaMemset2DAsync(Y, size_t(ldy) * 2, 0, size_t(O) * 2, size_t(M), st);
+    if (e == cudaSuccess && hidden && H) e = cudaMemsetAsync(hidden, 0, size_t(M) * hp * 2, st);
+    if (e == cudaSuccess && gate_up && H) e = cudaMemsetAsync(gate_up, 0, size_t(M) * hp * 4, st);
+    return e == cudaSuccess ? GC_OK : gc::fail(GC_ERR_CUDA, "gc_gated_ffn_forward_bf16: %s", cudaGetErrorString(e));
+  }
+  GC_REQUIRE(X && Win && Wout, "gc_gated_ffn_forward_bf16: null pointer");
+  GC_REQUIRE(gc::aligned16(hidden) && gc::aligned16(gate_up), "gc_gated_ffn_forward_bf16: saved matrices must be 16-byte aligned");
+  if (!workspace || workspace_bytes < gc_gated_ffn_workspace_bytes(M, D, H, O, 0))
+    return gc::fail(GC_ERR_WORKSPACE, "gc_gated_ffn_forward_bf16: workspace missing or smaller than its query says");
+  GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_bf16: workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  Matrix x{X, M, D, ldx, 2}, win{Win, D, 2 * H, ldwin, 2}, wout{Wout, H, O, ldwout, 2};
+  int rc = make_readable(x, ws, st);
+  if (rc == GC_OK) rc = make_gate_up(win, H, ws, st);
+  if (rc == GC_OK) rc = make_readable(wout, ws, st);
+  if (rc != GC_OK) return rc;
+  if (!hidden) {
+    hidden = reinterpret_cast<uint16_t*>(ws);
+    ws += align256(size_t(M) * hp * 2);
+  }
+  const Tile t = pick_tile(kGated, M, hp, 1);
+  Maps maps;
+  Params p{};
+  p.M = int(M); p.N = int(hp); p.K = int(D);
+  p.b_up = int(hp);
+  p.act = act;
+  p.save = gate_up != nullptr;
+  rc = error_word(&p.word);
+  if (rc == GC_OK) rc = operand_maps(maps, x, false, win, true, 0);
+  if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, hp, hp, 2}, 64, 32);
+  if (rc == GC_OK && gate_up) rc = make_map(&maps.out2, Matrix{gate_up, M, hp, 2 * hp, 2}, 64, 32);
+  if (rc == GC_OK && gate_up) rc = make_map(&maps.out3, Matrix{gate_up + hp, M, hp, 2 * hp, 2}, 64, 32);
+  if (rc == GC_OK) rc = launch_tile<kGated, false, true, false>(t, maps, p, st);
+  if (rc != GC_OK) return rc;
+  return plain(Matrix{hidden, M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
+}
+
+int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* Win,
+                               int64_t ldwin, const uint16_t* Wout, int64_t ldwout, const uint16_t* hidden,
+                               const uint16_t* gate_up, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* dX,
+                               int64_t lddx, uint16_t* dWin, int64_t lddwin, uint16_t* dWout, int64_t lddwout,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  GC_REQUIRE(M >= 0 && D >= 0 && H >= 0 && O >= 0, "gc_gated_ffn_backward_bf16: negative size");
+  GC_REQUIRE(act >= GC_ACT_SILU && act <= GC_ACT_RELU, "gc_gated_ffn_backward_bf16: unknown activation");
+  GC_REQUIRE(lddy >= O && ldx >= D && ldwin >= 2 * H && ldwout >= O && (!dX || lddx >= D) && (!dWin || lddwin >= 2 * H) &&
+                 (!dWout || lddwout >= O),
+             "gc_gated_ffn_backward_bf16: leading dimension below the row length");
+  if (!sizes_ok(M, D, H, O)) return gc::fail(GC_ERR_UNSUPPORTED, "gc_gated_ffn_backward_bf16: a size beyond 2^31");
+  const cudaStream_t st = gc::as_stream(stream);
+  const int64_t hp = up8(H);
+  if (M == 0 || D == 0 || H == 0 || O == 0) {  // sums of nothing
+    cudaError_t e = cudaSuccess;
+    auto zero = [&](uint16_t* p, int64_t ld, int64_t rows, int64_t cols) {
+      if (p && rows && cols && e == cudaSuccess) e = cudaMemset2DAsync(p, size_t(ld) * 2, 0, size_t(cols) * 2, size_t(rows), st);
+    };
+    zero(dX, lddx, M, D);
+    zero(dWin, lddwin, D, 2 * H);
+    zero(dWout, lddwout, H, O);
+    return e == cudaSuccess ? GC_OK : gc::fail(GC_ERR_CUDA, "gc_gated_ffn_backward_bf16: %s", cudaGetErrorString(e));
+  }
+  if (!dX && !dWin && !dWout) return GC_OK;
+  GC_REQUIRE(dY && X && Win && Wout && hidden && gate_up, "gc_gated_ffn_backward_bf16: null pointer");
+  GC_REQUIRE(gc::aligned16(hidden) && gc::aligned16(gate_up), "gc_gated_ffn_backward_bf16: saved matrices must be 16-byte aligned");
+  if (!workspace || workspace_bytes < gc_gated_ffn_workspace_bytes(M, D, H, O, 1))
+    return gc::fail(GC_ERR_WORKSPACE, "gc_gated_ffn_backward_bf16: workspace missing or smaller than its query says");
+  GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_backward_bf16: workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  Matrix dy{dY, M, O, lddy, 2}, x{X, M, D, ldx, 2}, win{Win, D, 2 * H, ldwin, 2}, wout{Wout, H, O, ldwout, 2};
+  int rc = make_readable(dy, ws, st);
+  if (rc == GC_OK && dWin) rc = make_readable(x, ws, st);
+  if (rc == GC_OK && dX) rc = make_gate_up(win, H, ws, st);
+  if (rc == GC_OK && (dX || dWin)) rc = make_readable(wout, ws, st);
+  if (rc != GC_OK) return rc;
+  const Matrix dgu{ws, M, 2 * hp, 2 * hp, 2};
+  if (dX || dWin) {
+    uint16_t* out = reinterpret_cast<uint16_t*>(ws);
+    ws += align256(size_t(M) * 2 * hp * 2);
+    const Tile t = pick_tile(kGatedBack, M, hp, 1);
+    Maps maps;
+    Params p{};
+    p.M = int(M); p.N = int(hp); p.K = int(O);
+    p.act = act;
+    rc = error_word(&p.word);
+    if (rc == GC_OK) rc = operand_maps(maps, dy, false, wout, false, t.pair ? t.bn / 2 : t.bn);
+    if (rc == GC_OK) rc = make_map(&maps.in1, Matrix{gate_up, M, hp, 2 * hp, 2}, 64, 32);
+    if (rc == GC_OK) rc = make_map(&maps.in2, Matrix{gate_up + hp, M, hp, 2 * hp, 2}, 64, 32);
+    if (rc == GC_OK) rc = make_map(&maps.out, Matrix{out, M, hp, 2 * hp, 2}, 64, 32);
+    if (rc == GC_OK) rc = make_map(&maps.out2, Matrix{out + hp, M, hp, 2 * hp, 2}, 64, 32);
+    if (rc == GC_OK) rc = launch_tile<kGatedBack, false, false, false>(t, maps, p, st);
+    if (rc != GC_OK) return rc;
+  }
+  if (dX) rc = plain(dgu, false, win, false, M, D, 2 * hp, reinterpret_cast<bf16*>(dX), lddx, 0, 0, ws, st);
+  if (rc == GC_OK && dWin)
+    rc = plain(x, true, dgu, true, D, 2 * hp, M, reinterpret_cast<bf16*>(dWin), lddwin, H, hp - H, ws, st);
+  if (rc == GC_OK && dWout)
+    rc = plain(Matrix{hidden, M, H, hp, 2}, true, dy, true, H, O, M, reinterpret_cast<bf16*>(dWout), lddwout, 0, 0, ws, st);
+  return rc;
+}
+
+size_t gc_gated_ffn_e4m3_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O) {
+  if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, D, H, O)) return 0;
+  const int64_t d16 = (D + 15) / 16 * 16;
+  return align256(size_t(M) * d16) + align256(size_t(2 * H) * d16) + align256(size_t(H) * up8(O) * 2) +
+         align256(size_t(M) * up8(H) * 2) + plain_workspace(M, O, H);
+}
+
+int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_scale, const uint8_t* W8, int64_t ldw,
+                              const float* w_scale, const uint16_t* Wout, int64_t ldwout, int64_t M, int64_t D, int64_t H,
+                              int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  GC_REQUIRE(M >= 0 && D >= 0 && H >= 0 && O >= 0, "gc_gated_ffn_forward_e4m3: negative size");
+  GC_REQUIRE(act >= GC_ACT_SILU && act <= GC_ACT_RELU, "gc_gated_ffn_forward_e4m3: unknown activation");
+  GC_REQUIRE(ldx >= D && ldw >= D && ldwout >= O && ldy >= O,
+             "gc_gated_ffn_forward_e4m3: leading dimension below the row length");
+  if (!sizes_ok(M, D, H, O)) return gc::fail(GC_ERR_UNSUPPORTED, "gc_gated_ffn_forward_e4m3: a size beyond 2^31");
+  const cudaStream_t st = gc::as_stream(stream);
+  if (M == 0 || O == 0) return GC_OK;
+  GC_REQUIRE(Y, "gc_gated_ffn_forward_e4m3: null pointer");
+  if (D == 0 || H == 0) {
+    const cudaError_t e = cudaMemset2DAsync(Y, size_t(ldy) * 2, 0, size_t(O) * 2, size_t(M), st);
+    return e == cudaSuccess ? GC_OK : gc::fail(GC_ERR_CUDA, "gc_gated_ffn_forward_e4m3: %s", cudaGetErrorString(e));
+  }
+  GC_REQUIRE(X8 && x_scale && W8 && w_scale && Wout, "gc_gated_ffn_forward_e4m3: null pointer");
+  if (!workspace || workspace_bytes < gc_gated_ffn_e4m3_workspace_bytes(M, D, H, O))
+    return gc::fail(GC_ERR_WORKSPACE, "gc_gated_ffn_forward_e4m3: workspace missing or smaller than its query says");
+  GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_e4m3: workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  Matrix x{X8, M, D, ldx, 1}, w{W8, 2 * H, D, ldw, 1}, wout{Wout, H, O, ldwout, 2};
+  int rc = make_readable(x, ws, st);
+  if (rc == GC_OK) rc = make_readable(w, ws, st);
+  if (rc == GC_OK) rc = make_readable(wout, ws, st);
+  if (rc != GC_OK) return rc;
+  const int64_t hp = up8(H);
+  uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);
+  ws += align256(size_t(M) * hp * 2);
+  const Tile t = pick_tile(kGated, M, H, 1);
+  Maps maps;
+  Params p{};
+  p.M = int(M); p.N = int(H); p.K = int(D);
+  p.b_up = int(H);  // rows of W8: no alignment to keep
+  p.act = act;
+  p.sa = x_scale;
+  p.sb = w_scale;
+  rc = error_word(&p.word);
+  if (rc == GC_OK) rc = operand_maps(maps, x, false, w, false, t.bn / 2);
+  if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 64, 32);
+  if (rc == GC_OK) rc = launch_tile<kGated, false, false, true>(t, maps, p, st);
+  if (rc != GC_OK) return rc;
+  return plain(Matrix{hidden, M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
+}
+
+}  // extern "C"

@@ -286,6 +286,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                           need_dx, need_dw);
     return std::make_tuple(g.dx, g.dweight, g.dresidual);
   }, NoGil());
+  m.def("gated_ffn", [](const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act) -> OptTensor {
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return gated_ffn(x, w_in, w_out, act);
+  }, NoGil());
+  m.def("gated_ffn_forward", [](const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act) {
+    const FfnForward f = gated_ffn_forward(x, w_in, w_out, int(act), true);
+    return std::make_tuple(f.y, std::vector<Tensor>{f.x, f.w_in, f.w_out, f.hidden, f.gate_up});
+  }, NoGil());
+  m.def("gated_ffn_backward", [](const Tensor& dy, const Tensor& x, const Tensor& w_in, const Tensor& w_out,
+                                 const Tensor& hidden, const Tensor& gate_up, int64_t act, bool dx, bool dw_in, bool dw_out) {
+    const FfnGrads g = gated_ffn_backward(dy, x, w_in, w_out, hidden, gate_up, int(act), dx, dw_in, dw_out);
+    return std::make_tuple(g.dx, g.dw_in, g.dw_out);
+  }, NoGil());
+  m.def("gated_ffn_fp8", &gated_ffn_fp8, NoGil());
   m.def("adamw_step", &adamw_step, NoGil());
   m.def("adamw_moments", &adamw_moments, NoGil());
 }

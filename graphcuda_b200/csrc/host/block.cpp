@@ -150,6 +150,124 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& w
   return {f.y, f.scale, f.stream};
 }
 
+// ------------------------------------------------------------------ gated feed-forward block
+namespace {
+struct FfnSizes {
+  int64_t M, D, H, O, pitch;
+};
+const uint16_t* bits(const Tensor& t) { return static_cast<const uint16_t*>(t.const_data_ptr()); }
+uint16_t* bits_mut(const Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
+bool bf16_matrix(const Tensor& t, const at::Device& dev) {
+  return t.dim() == 2 && t.device() == dev && t.scalar_type() == at::kBFloat16;
+}
+FfnSizes ffn_sizes(const Tensor& x, const Tensor& w_in, const Tensor& w_out) {
+  require(x.is_cuda() && bf16_matrix(x, x.device()), "gated_ffn: x must be a bfloat16 CUDA matrix");
+  require(bf16_matrix(w_in, x.device()) && w_in.size(0) == x.size(1) && w_in.size(1) % 2 == 0,
+          "gated_ffn: w_in must be bfloat16 [in, 2 * hidden] on x's device");
+  require(bf16_matrix(w_out, x.device()) && w_out.size(0) == w_in.size(1) / 2,
+          "gated_ffn: w_out must be bfloat16 [hidden, out] on x's device");
+  return {x.size(0), x.size(1), w_out.size(0), w_out.size(1), abi.gc_gated_ffn_hidden_pitch(w_out.size(0))};
+}
+}  // namespace
+
+FfnForward gated_ffn_forward(const Tensor& xin, const Tensor& w_in, const Tensor& w_out, int act, bool save) {
+  const FfnSizes n = ffn_sizes(xin, w_in, w_out);
+  const at::Device dev = xin.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  FfnForward f;
+  f.x = row_major(xin);
+  f.w_in = row_major(w_in);
+  f.w_out = row_major(w_out);
+  f.y = empty_like_rows(n.M, n.O, at::kBFloat16, dev);
+  if (save) {
+    f.hidden = empty_like_rows(n.M, n.pitch, at::kBFloat16, dev);
+    f.gate_up = empty_like_rows(n.M, 2 * n.pitch, at::kBFloat16, dev);
+  }
+  const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 0), dev);
+  check(abi.gc_gated_ffn_forward_bf16(bits(f.x), ld_of(f.x), bits(f.w_in), ld_of(f.w_in), bits(f.w_out), ld_of(f.w_out),
+                                      n.M, n.D, n.H, n.O, act, bits_mut(f.y), std::max<int64_t>(n.O, 1),
+                                      save ? bits_mut(f.hidden) : nullptr, save ? bits_mut(f.gate_up) : nullptr, ws.ptr,
+                                      ws.bytes, stream_of(dev)),
+        "gc_gated_ffn_forward_bf16");
+  return f;
+}
+
+FfnGrads gated_ffn_backward(const Tensor& dy_in, const Tensor& x, const Tensor& w_in, const Tensor& w_out,
+                            const Tensor& hidden, const Tensor& gate_up, int act, bool need_dx, bool need_dw_in,
+                            bool need_dw_out) {
+  const FfnSizes n = ffn_sizes(x, w_in, w_out);
+  const at::Device dev = x.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor dy = row_major(dy_in);
+  FfnGrads g;
+  if (need_dx) g.dx = empty_like_rows(n.M, n.D, at::kBFloat16, dev);
+  if (need_dw_in) g.dw_in = empty_like_rows(n.D, 2 * n.H, at::kBFloat16, dev);
+  if (need_dw_out) g.dw_out = empty_like_rows(n.H, n.O, at::kBFloat16, dev);
+  const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 1), dev);
+  check(abi.gc_gated_ffn_backward_bf16(
+            bits(dy), ld_of(dy), bits(x), ld_of(x), bits(w_in), ld_of(w_in), bits(w_out), ld_of(w_out), bits(hidden),
+            bits(gate_up), n.M, n.D, n.H, n.O, act, need_dx ? bits_mut(g.dx) : nullptr, std::max<int64_t>(n.D, 1),
+            need_dw_in ? bits_mut(g.dw_in) : nullptr, std::max<int64_t>(2 * n.H, 1),
+            need_dw_out ? bits_mut(g.dw_out) : nullptr, std::max<int64_t>(n.O, 1), ws.ptr, ws.bytes, stream_of(dev)),
+        "gc_gated_ffn_backward_bf16");
+  return g;
+}
+
+namespace {
+struct FfnFunction : torch::autograd::Function<FfnFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act) {
+    const FfnForward f = gated_ffn_forward(x, w_in, w_out, int(act), true);
+    ctx->save_for_backward({f.x, f.w_in, f.w_out, f.hidden, f.gate_up});
+    ctx->saved_data["act"] = act;
+    return f.y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("gated_ffn");
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const FfnGrads g = gated_ffn_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4],
+                                          int(ctx->saved_data["act"].toInt()), ctx->needs_input_grad(0),
+                                          ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+    return {g.dx, g.dw_in, g.dw_out, Tensor()};
+  }
+};
+}  // namespace
+
+Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act) {
+  if (!recorded({&x, &w_in, &w_out})) return gated_ffn_forward(x, w_in, w_out, int(act), false).y;
+  return FfnFunction::apply(x, w_in, w_out, act);
+}
+
+Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Tensor& w_out,
+                     int64_t act) {
+  require(x8.is_cuda() && x8.dim() == 2 && x8.scalar_type() == at::kFloat8_e4m3fn,
+          "gated_ffn_fp8: x8 must be a float8_e4m3fn CUDA matrix");
+  const at::Device dev = x8.device();
+  const int64_t M = x8.size(0), D = x8.size(1);
+  require(w8.dim() == 2 && w8.device() == dev && w8.scalar_type() == at::kFloat8_e4m3fn && w8.size(1) == D &&
+              w8.size(0) % 2 == 0,
+          "gated_ffn_fp8: w8 must be float8_e4m3fn [2 * hidden, in] on x8's device");
+  const int64_t H = w8.size(0) / 2;
+  require(f32_on(x_scale, dev) && x_scale.dim() == 1 && x_scale.size(0) == M && f32_on(w_scale, dev) &&
+              w_scale.dim() == 1 && w_scale.size(0) == 2 * H,
+          "gated_ffn_fp8: float32 scales expected, one per row of x8 and of w8, on their device");
+  require(bf16_matrix(w_out, dev) && w_out.size(0) == H, "gated_ffn_fp8: w_out must be bfloat16 [hidden, out] on x8's device");
+  if (recorded({&w_out, &x_scale, &w_scale}))
+    raise("gated_ffn_fp8 has no gradient: call it under torch.no_grad(), or gated_ffn for training");
+  const int64_t O = w_out.size(1);
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor x = row_major(x8), w = row_major(w8), wo = row_major(w_out);
+  const Tensor sx = x_scale.contiguous(), sw = w_scale.contiguous();
+  Tensor y = empty_like_rows(M, O, at::kBFloat16, dev);
+  const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_e4m3_workspace_bytes(M, D, H, O), dev);
+  check(abi.gc_gated_ffn_forward_e4m3(static_cast<const uint8_t*>(x.const_data_ptr()), ld_of(x), sx.const_data_ptr<float>(),
+                                      static_cast<const uint8_t*>(w.const_data_ptr()), ld_of(w), sw.const_data_ptr<float>(),
+                                      bits(wo), ld_of(wo), M, D, H, O, int(act), bits_mut(y), std::max<int64_t>(O, 1),
+                                      ws.ptr, ws.bytes, stream_of(dev)),
+        "gc_gated_ffn_forward_e4m3");
+  return y;
+}
+
 // ------------------------------------------------------------------ AdamW
 namespace {
 bool part(const Tensor& t, at::ScalarType type, const at::Device& dev, int64_t n) {
