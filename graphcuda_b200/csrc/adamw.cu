@@ -18,10 +18,8 @@
 // m and v are computed with one rounding per operation, as the formula reads, so that the codes depend on nothing else;
 // the parameters are updated from the moments before they are rounded to 8 bits.
 //
-// Bound by memory: 28 bytes per parameter (32 bits), 16 and a sixteenth (8 bits).  A CTA takes chunks of 2048
-// elements, a warp 256 of them, a thread two runs of 4: accesses of 16 bytes (4 for codes), of which every thread has all in
-// flight before it uses the first.  The list of tensors travels in the launch's parameters: nothing is kept on the device that
-// could go stale, and a launch can be recorded.
+// The list of tensors travels in the launch's parameters: nothing is kept on the device that could go stale, and a launch
+// can be recorded.
 #include "common.cuh"
 
 #include <cuda_bf16.h>
@@ -36,26 +34,27 @@ constexpr int kThreads = 256;
 constexpr int kBlock = GC_ADAMW_BLOCK;          // elements that share a scale: one warp, 8 per lane
 constexpr int kChunk = kThreads / 32 * kBlock;  // elements of a CTA's pass
 static_assert(kBlock == 256, "a warp holds a block, 8 elements per lane");
-// Tensors of one launch: launch parameters hold up to 32,764 bytes, and most models need far fewer.
-constexpr int kFew = 48, kMany = 440;
 
 using bf16 = __nv_bfloat16;
 
-template <int MAX>
+// What an entry of the list points at: gradient, moments, fp32 parameter; beside bf16 parameters those; scales of 8-bit
+// moments.  Launch parameters hold up to 32,764 bytes; most models need far fewer than fit.
+enum Role { kG, kM, kV, kMaster };
+template <int BITS, bool MIXED>
+struct Layout {
+  [[maybe_unused]] static constexpr int kP16 = 4, kMs = 4 + MIXED, kVs = 5 + MIXED;
+  static constexpr int kArrays = 4 + MIXED + (BITS == 8 ? 2 : 0);
+  static constexpr int kMany = 31000 / (8 * kArrays + 13);
+};
+constexpr int kFew = 48;
+template <int ARRAYS, int MAX>
 struct List {
-  void* p[MAX];        // bf16 or fp32 parameters
-  float* master[MAX];  // fp32 parameters (p itself where it is fp32)
-  const void* g[MAX];
-  void* m[MAX];
-  void* v[MAX];
-  float* ms[MAX];  // scales, 8 bits
-  float* vs[MAX];
+  void* at[ARRAYS][MAX];
   int64_t n[MAX];
   int32_t first_chunk[MAX + 1];  // prefix sum of ceil(n / kChunk)
   uint8_t vec[MAX];              // every array is aligned for vector accesses
   int count, first_tensor;       // first_tensor: tensors of earlier launches of the same step
 };
-static_assert(sizeof(List<kMany>) <= 32000, "launch parameters");
 
 struct Hyper {
   double lr, beta1, beta2;
@@ -71,31 +70,55 @@ __device__ __forceinline__ uint32_t mix(uint32_t x) {
   return x ^ (x >> 16);
 }
 
-// The four elements from `at` on; beyond n: zeros.
-template <class T>
-__device__ __forceinline__ void load4(const T* base, int64_t at, int64_t n, bool vec, T (&v)[4]) {
+// Four elements from `at` on.  FAST: all of them exist, in one access; else those beyond n are zeros.
+template <bool FAST, class T>
+__device__ __forceinline__ void load4(const void* base, int64_t at, int64_t n, T (&v)[4]) {
   struct alignas(4 * sizeof(T)) V { T v[4]; };
-  if (vec && at + 4 <= n) {
-    const V t = *reinterpret_cast<const V*>(base + at);
+  const T* p = static_cast<const T*>(base) + at;
+  if constexpr (FAST) {
+    const V t = *reinterpret_cast<const V*>(p);
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = t.v[k];
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = at + k < n ? base[at + k] : T(0.f);
+    for (int k = 0; k < 4; ++k) v[k] = at + k < n ? p[k] : T(0.f);
   }
 }
-template <class T>
-__device__ __forceinline__ void store4(T* base, int64_t at, int64_t n, bool vec, const T (&v)[4]) {
+template <bool FAST, class T>
+__device__ __forceinline__ void store4(void* base, int64_t at, int64_t n, const T (&v)[4]) {
   struct alignas(4 * sizeof(T)) V { T v[4]; };
-  if (vec && at + 4 <= n) {
+  T* p = static_cast<T*>(base) + at;
+  if constexpr (FAST) {
     V t;
 #pragma unroll
     for (int k = 0; k < 4; ++k) t.v[k] = v[k];
-    *reinterpret_cast<V*>(base + at) = t;
+    *reinterpret_cast<V*>(p) = t;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (at + k < n) base[at + k] = v[k];
+      if (at + k < n) p[k] = v[k];
+  }
+}
+// Four codes as one word.
+template <bool FAST>
+__device__ __forceinline__ uint32_t load_codes(const void* base, int64_t at, int64_t n) {
+  const uint8_t* p = static_cast<const uint8_t*>(base) + at;
+  if constexpr (FAST) return *reinterpret_cast<const uint32_t*>(p);
+  uint32_t w = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (at + k < n) w |= uint32_t(p[k]) << (8 * k);
+  return w;
+}
+template <bool FAST>
+__device__ __forceinline__ void store_codes(void* base, int64_t at, int64_t n, const uint32_t (&q)[4]) {
+  uint8_t* p = static_cast<uint8_t*>(base) + at;
+  if constexpr (FAST) {
+    *reinterpret_cast<uint32_t*>(p) = (q[0] | q[1] << 8) | (q[2] << 16 | q[3] << 24);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at + k < n) p[k] = uint8_t(q[k]);
   }
 }
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -109,34 +132,42 @@ __device__ __forceinline__ float2 scale_of(uint32_t top_bits, float top_code) {
   return make_float2(s, __frcp_rn(s));
 }
 // t >= 0 to a code of 3 bits of mantissa and an exponent of bias BIAS: u (16 bits) is added below the last kept bit and
-// the rest cut off.  Below the smallest normal number the grid is even, and the sum is formed in units of it.
+// the rest cut off.  Below the smallest normal number the grid is even, and the sum is formed in units of it.  Floats and
+// integers are taken from each other's bits here: conversion instructions run at an eighth of the rate.
 template <int BIAS>
 __device__ __forceinline__ uint32_t round_code(float t, uint32_t u) {
   constexpr float kLowest = BIAS == 7 ? 0x1p-6f : 0x1p-14f, kUnits = BIAS == 7 ? 0x1p9f : 0x1p17f;
   const uint32_t high = ((__float_as_uint(t) + (u << 4)) >> 20) - ((127u - BIAS) << 3);
-  const uint32_t low = uint32_t(__fadd_rn(t * kUnits, float(u) * 0x1p-16f));  // towards zero
+  const float fraction = __uint_as_float(0x3F800000u | (u << 7)) - 1.0f;  // u / 2^16
+  const uint32_t low = __float_as_uint(__fadd_rd(__fmaf_rn(t, kUnits, fraction), 0x1p23f)) & 0xFFu;  // towards zero
   return t < kLowest ? low : high;
 }
 
-// e4m3 and second-moment codes, four at a time
-__device__ __forceinline__ void decode_m(const uint8_t (&q)[4], float s, float (&x)[4]) {
+// Four codes of a word as values.
+__device__ __forceinline__ void decode_m(uint32_t q, float s, float (&x)[4]) {
 #pragma unroll
   for (int k = 0; k < 4; k += 2) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(uint16_t(q[k] | q[k + 1] << 8), __NV_E4M3);
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(uint16_t(q >> (8 * k)), __NV_E4M3);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
     x[k] = __fmul_rn(f.x, s);
     x[k + 1] = __fmul_rn(f.y, s);
   }
 }
-__device__ __forceinline__ void decode_v(const uint8_t (&q)[4], float s, float (&x)[4]) {
+__device__ __forceinline__ void decode_v(uint32_t q, float s, float (&x)[4]) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) x[k] = __fmul_rn(__half2float(__ushort_as_half(uint16_t(q[k] << 7))), s);
+  for (int k = 0; k < 4; k += 2) {
+    const uint32_t w = __byte_perm(q, 0, k ? 0x4342 : 0x4140) << 7;  // two fp16 numbers
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    x[k] = __fmul_rn(f.x, s);
+    x[k + 1] = __fmul_rn(f.y, s);
+  }
 }
 
-// The tensor that a chunk belongs to: the last whose first chunk is not beyond it.
-template <int MAX>
-__device__ __forceinline__ int tensor_of(const List<MAX>& tl, int chunk) {
-  int lo = 0, hi = tl.count;
+// The tensor that a chunk belongs to, the last whose first chunk is not beyond it; k is that of an earlier chunk.
+template <class L>
+__device__ __forceinline__ int tensor_of(const L& tl, int chunk, int k) {
+  if (chunk < tl.first_chunk[k + 1]) return k;
+  int lo = k + 1, hi = tl.count;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (tl.first_chunk[mid] <= chunk) lo = mid;
@@ -145,131 +176,28 @@ __device__ __forceinline__ int tensor_of(const List<MAX>& tl, int chunk) {
   return lo;
 }
 
+// The step's scalars, by two threads while the CTA's first loads are on their way, in double, as Python would form them.
+struct Scalars {
+  float step_size, inv_bc2;
+  uint32_t key;
+};
+__device__ __forceinline__ void form_scalars(const Hyper& hp, unsigned long long step, Scalars& out) {
+  const int warp = threadIdx.x / 32;
+  if (threadIdx.x % 32 != 0 || warp >= 2) return;
+  const double rest = 1.0 - pow(warp ? hp.beta2 : hp.beta1, double(step + 1ull));
+  if (warp) {
+    out.inv_bc2 = float(1.0 / sqrt(rest));
+  } else {
+    out.step_size = float(hp.lr / rest);
+    out.key = mix(hp.seed + uint32_t(step + 1ull) * 0x9E3779B9u);
+  }
+}
 // state[0] = steps taken so far (read by every CTA before it counts itself in state[1]); of the step's last launch the
 // CTA that arrives last writes the new count and clears the counter.
-// BITS: of the moments.  TP: of the parameters and gradients.
-template <int BITS, class TP, int MAX>
-__global__ void __launch_bounds__(kThreads)
-adamw_kernel(const __grid_constant__ List<MAX> tl, const __grid_constant__ Hyper hp,
-             unsigned long long* __restrict__ state) {
-  __shared__ float consts_s[2];
-  __shared__ uint32_t key_s;
-  constexpr bool kMixed = sizeof(TP) == 2;
-  using TM = std::conditional_t<BITS == 8, uint8_t, float>;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int total = tl.first_chunk[tl.count];
-
-  float pv[2][4];
-  TP gv[2][4];
-  TM mv[2][4], vv[2][4];
-  float ms = 0.f, vs = 0.f;
-  int k = 0;
-  int64_t block = 0, n = 0;
-  bool vec = false;
-  auto load = [&](int chunk) {
-    k = tensor_of(tl, chunk);
-    n = tl.n[k];
-    vec = tl.vec[k];
-    block = int64_t(chunk - tl.first_chunk[k]) * (kChunk / kBlock) + warp;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t at = block * kBlock + j * 128 + lane * 4;
-      load4(static_cast<const float*>(tl.master[k]), at, n, vec, pv[j]);
-      load4(static_cast<const TP*>(tl.g[k]), at, n, vec, gv[j]);
-      load4(static_cast<const TM*>(tl.m[k]), at, n, vec, mv[j]);
-      load4(static_cast<const TM*>(tl.v[k]), at, n, vec, vv[j]);
-    }
-    if (BITS == 8 && block * kBlock < n) {
-      ms = tl.ms[k][block];
-      vs = tl.vs[k][block];
-    }
-  };
-
-  int chunk = blockIdx.x;
-  unsigned long long step = 0;
-  if (lane == 0 && warp < 2) step = *reinterpret_cast<volatile unsigned long long*>(state);
-  if (chunk < total) load(chunk);
-  if (lane == 0 && warp < 2) {
-    // the scalars in double, as Python would form them
-    const double rest = 1.0 - pow(warp ? hp.beta2 : hp.beta1, double(step + 1ull));
-    consts_s[warp] = float(warp ? 1.0 / sqrt(rest) : hp.lr / rest);
-    if (warp == 0) key_s = mix(hp.seed + uint32_t(step + 1ull) * 0x9E3779B9u);
-  }
-  __syncthreads();
-  const float step_size = consts_s[0], inv_bc2 = consts_s[1];
-  const uint32_t step_key = key_s;
-
-  while (chunk < total) {
-    const int64_t at0 = block * kBlock + lane * 4;
-    if (block * kBlock < n) {  // uniform in the warp
-      float m[2][4], v[2][4];
-      if constexpr (BITS == 8) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          decode_m(mv[j], ms, m[j]);
-          decode_v(vv[j], vs, v[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) m[j][e] = mv[j][e], v[j][e] = vv[j][e];
-      }
-      uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float g = to_f32(gv[j][e]);
-          m[j][e] = __fadd_rn(__fmul_rn(m[j][e], hp.b1), __fmul_rn(g, hp.w1));
-          v[j][e] = __fadd_rn(__fmul_rn(v[j][e], hp.b2), __fmul_rn(__fmul_rn(g, g), hp.w2));
-          pv[j][e] = pv[j][e] * hp.keep - step_size * (m[j][e] / (sqrtf(v[j][e]) * inv_bc2 + hp.eps));
-          if (BITS == 8) {  // elements beyond the tensor: zeros
-            const bool in = at0 + j * 128 + e < n;
-            top_m = max(top_m, in ? __float_as_uint(m[j][e]) & 0x7FFFFFFFu : 0u);
-            top_v = max(top_v, in ? __float_as_uint(v[j][e]) & 0x7FFFFFFFu : 0u);
-          }
-        }
-        const int64_t at = at0 + j * 128;
-        store4(tl.master[k], at, n, vec, pv[j]);
-        if constexpr (kMixed) {
-          bf16 p16[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) p16[e] = __float2bfloat16_rn(pv[j][e]);
-          store4(static_cast<bf16*>(tl.p[k]), at, n, vec, p16);
-        }
-        if constexpr (BITS == 32) {
-          store4(static_cast<float*>(tl.m[k]), at, n, vec, m[j]);
-          store4(static_cast<float*>(tl.v[k]), at, n, vec, v[j]);
-        }
-      }
-      if constexpr (BITS == 8) {
-        const float2 sm = scale_of(__reduce_max_sync(0xFFFFFFFFu, top_m), 1.0f / 448.0f);
-        const float2 sv = scale_of(__reduce_max_sync(0xFFFFFFFFu, top_v), 1.0f / 61440.0f);
-        if (lane == 0) {
-          tl.ms[k][block] = sm.x;
-          tl.vs[k][block] = sv.x;
-        }
-        const uint32_t key = mix(step_key + uint32_t(tl.first_tensor + k));
-        const uint32_t least = sv.x > 0.f ? 1u : 0u;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint8_t qm[4], qv[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t r = mix(key + uint32_t(at0 + j * 128 + e));
-            const float tm = __fmul_rn(m[j][e], sm.y), tv = __fmul_rn(v[j][e], sv.y);
-            qm[e] = uint8_t(min(round_code<7>(fabsf(tm), r & 0xFFFFu), 0x7Eu) | (__float_as_uint(tm) >> 31 << 7));
-            qv[e] = uint8_t(max(min(round_code<15>(tv, r >> 16), 0xF7u), least));
-          }
-          store4(static_cast<uint8_t*>(tl.m[k]), at0 + j * 128, n, vec, qm);
-          store4(static_cast<uint8_t*>(tl.v[k]), at0 + j * 128, n, vec, qv);
-        }
-      }
-    }
-    chunk += gridDim.x;
-    if (chunk < total) load(chunk);
-  }
+__device__ __forceinline__ unsigned long long read_step(const unsigned long long* state) {
+  return *reinterpret_cast<const volatile unsigned long long*>(state);
+}
+__device__ __forceinline__ void count_step(const Hyper& hp, unsigned long long step, unsigned long long* state) {
   if (!hp.advance) return;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -282,50 +210,218 @@ adamw_kernel(const __grid_constant__ List<MAX> tl, const __grid_constant__ Hyper
   }
 }
 
-// The values of 8-bit moments.  p, g: where the first and second moments go.
+// One element: moments as the formula reads, one rounding per operation; the parameter from them.  The quotient may be off
+// by 2^-21 of the update (approximate root and division: the exact ones take half of an element's instructions).
+__device__ __forceinline__ void update(const Hyper& hp, const Scalars& sc, float g, float& m, float& v, float& p) {
+  m = __fadd_rn(__fmul_rn(m, hp.b1), __fmul_rn(g, hp.w1));
+  v = __fadd_rn(__fmul_rn(v, hp.b2), __fmul_rn(__fmul_rn(g, g), hp.w2));
+  float root;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
+  p = p * hp.keep - sc.step_size * __fdividef(m, root * sc.inv_bc2 + hp.eps);
+}
+
+// Moments of 32 bits.  Bound by memory: 28 bytes per parameter.  A thread takes 4 elements of a pass, all of whose loads are
+// under way before the first is used.
+template <class TP, int MAX>
+__global__ void __launch_bounds__(kThreads, 6)
+adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, MAX> tl, const __grid_constant__ Hyper hp,
+             unsigned long long* __restrict__ state) {
+  constexpr bool kMixed = sizeof(TP) == 2;
+  __shared__ Scalars sc_s;
+  const int total = 2 * tl.first_chunk[tl.count];  // half a chunk per pass
+  float pv[4], mv[4], vv[4];
+  TP gv[4];
+  int k = 0;
+  int64_t at = 0, n = 0;
+  bool fast = false;
+  auto load = [&](int pass) {
+    k = tensor_of(tl, pass / 2, k);
+    n = tl.n[k];
+    at = int64_t(pass - 2 * tl.first_chunk[k]) * (kChunk / 2) + threadIdx.x * 4;
+    fast = tl.vec[k] && at + 4 <= n;
+    auto all = [&](auto f) {
+      constexpr bool F = decltype(f)::value;
+      load4<F>(tl.at[kMaster][k], at, n, pv);
+      load4<F>(tl.at[kG][k], at, n, gv);
+      load4<F>(tl.at[kM][k], at, n, mv);
+      load4<F>(tl.at[kV][k], at, n, vv);
+    };
+    if (fast) all(std::true_type{});
+    else all(std::false_type{});
+  };
+  int pass = blockIdx.x;
+  unsigned long long step = read_step(state);
+  if (pass < total) load(pass);
+  form_scalars(hp, step, sc_s);
+  __syncthreads();
+  const Scalars sc = sc_s;
+  while (pass < total) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) update(hp, sc, to_f32(gv[e]), mv[e], vv[e], pv[e]);
+    auto all = [&](auto f) {
+      constexpr bool F = decltype(f)::value;
+      store4<F>(tl.at[kMaster][k], at, n, pv);
+      store4<F>(tl.at[kM][k], at, n, mv);
+      store4<F>(tl.at[kV][k], at, n, vv);
+      if constexpr (kMixed) {
+        const bf16 p16[4] = {__float2bfloat16_rn(pv[0]), __float2bfloat16_rn(pv[1]), __float2bfloat16_rn(pv[2]),
+                             __float2bfloat16_rn(pv[3])};
+        store4<F>(tl.at[Layout<32, kMixed>::kP16][k], at, n, p16);
+      }
+    };
+    if (fast) all(std::true_type{});
+    else all(std::false_type{});
+    pass += gridDim.x;
+    if (pass < total) load(pass);
+  }
+  count_step(hp, step, state);
+}
+
+// Moments of 8 bits.  A warp takes a block of 256 elements, a lane two runs of 4.
+template <class TP, int MAX>
+__global__ void __launch_bounds__(kThreads, 3)
+adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArrays, MAX> tl,
+                  const __grid_constant__ Hyper hp, unsigned long long* __restrict__ state) {
+  constexpr bool kMixed = sizeof(TP) == 2;
+  using L = Layout<8, kMixed>;
+  __shared__ Scalars sc_s;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int total = tl.first_chunk[tl.count];
+  float pv[2][4];
+  TP gv[2][4];
+  uint32_t mq[2], vq[2];
+  float ms = 0.f, vs = 0.f;
+  int k = 0;
+  int64_t at = 0, n = 0;
+  bool fast = false;
+  auto load = [&](int chunk) {
+    k = tensor_of(tl, chunk, k);
+    n = tl.n[k];
+    const int64_t block = int64_t(chunk - tl.first_chunk[k]) * (kChunk / kBlock) + warp;
+    at = block * kBlock + lane * 4;
+    fast = tl.vec[k] && (block + 1) * kBlock <= n;
+    auto all = [&](auto f) {
+      constexpr bool F = decltype(f)::value;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        load4<F>(tl.at[kMaster][k], at + j * 128, n, pv[j]);
+        load4<F>(tl.at[kG][k], at + j * 128, n, gv[j]);
+        mq[j] = load_codes<F>(tl.at[kM][k], at + j * 128, n);
+        vq[j] = load_codes<F>(tl.at[kV][k], at + j * 128, n);
+      }
+      if (F || block * kBlock < n) {
+        ms = static_cast<const float*>(tl.at[L::kMs][k])[block];
+        vs = static_cast<const float*>(tl.at[L::kVs][k])[block];
+      }
+    };
+    if (fast) all(std::true_type{});
+    else all(std::false_type{});
+  };
+  int chunk = blockIdx.x;
+  const unsigned long long step = read_step(state);
+  if (chunk < total) load(chunk);
+  form_scalars(hp, step, sc_s);
+  __syncthreads();
+  const Scalars sc = sc_s;
+  while (chunk < total) {
+    auto all = [&](auto f) {
+      constexpr bool F = decltype(f)::value;
+      float m[2][4], v[2][4];
+      uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        decode_m(mq[j], ms, m[j]);
+        decode_v(vq[j], vs, v[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          update(hp, sc, to_f32(gv[j][e]), m[j][e], v[j][e], pv[j][e]);
+          if (!F && at + j * 128 + e >= n) m[j][e] = v[j][e] = 0.f;  // beyond the tensor
+          top_m = max(top_m, __float_as_uint(m[j][e]) & 0x7FFFFFFFu);  // a NaN is above infinity and stays
+          top_v = max(top_v, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
+        }
+        store4<F>(tl.at[kMaster][k], at + j * 128, n, pv[j]);
+        if constexpr (kMixed) {
+          const bf16 p16[4] = {__float2bfloat16_rn(pv[j][0]), __float2bfloat16_rn(pv[j][1]), __float2bfloat16_rn(pv[j][2]),
+                               __float2bfloat16_rn(pv[j][3])};
+          store4<F>(tl.at[L::kP16][k], at + j * 128, n, p16);
+        }
+      }
+      const float2 sm = scale_of(__reduce_max_sync(0xFFFFFFFFu, top_m), 1.0f / 448.0f);
+      const float2 sv = scale_of(__reduce_max_sync(0xFFFFFFFFu, top_v), 1.0f / 61440.0f);
+      if (lane == 0) {
+        static_cast<float*>(tl.at[L::kMs][k])[at / kBlock] = sm.x;
+        static_cast<float*>(tl.at[L::kVs][k])[at / kBlock] = sv.x;
+      }
+      const uint32_t key = mix(sc.key + uint32_t(tl.first_tensor + k)) + uint32_t(at);
+      const uint32_t least = sv.x > 0.f ? 1u : 0u;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t qm[4], qv[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t r = mix(key + uint32_t(j * 128 + e));
+          const float tm = __fmul_rn(m[j][e], sm.y), tv = __fmul_rn(v[j][e], sv.y);
+          qm[e] = min(round_code<7>(fabsf(tm), r & 0xFFFFu), 0x7Eu) | (__float_as_uint(tm) >> 31 << 7);
+          qv[e] = max(min(round_code<15>(tv, r >> 16), 0xF7u), least);
+        }
+        store_codes<F>(tl.at[kM][k], at + j * 128, n, qm);
+        store_codes<F>(tl.at[kV][k], at + j * 128, n, qv);
+      }
+    };
+    if (fast) all(std::true_type{});
+    else if (at - lane * 4 < n) all(std::false_type{});  // uniform in the warp
+    chunk += gridDim.x;
+    if (chunk < total) load(chunk);
+  }
+  count_step(hp, step, state);
+}
+
+// The values of 8-bit moments, into the fp32 tensors at kG (first) and kMaster (second); scales as for 8 bits and fp32
+// parameters.  A chunk per CTA.
 template <int MAX>
 __global__ void __launch_bounds__(kThreads)
-adamw_moments_kernel(const __grid_constant__ List<MAX> tl, int total) {
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  for (int chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
-    const int k = tensor_of(tl, chunk);
-    const int64_t n = tl.n[k], block = int64_t(chunk - tl.first_chunk[k]) * (kChunk / kBlock) + warp;
-    const bool vec = tl.vec[k];
-    if (block * kBlock >= n) continue;
-    const float ms = tl.ms[k][block], vs = tl.vs[k][block];
-    uint8_t qm[2][4], qv[2][4];
+adamw_moments_kernel(const __grid_constant__ List<Layout<8, false>::kArrays, MAX> tl) {
+  using L = Layout<8, false>;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, chunk = blockIdx.x;
+  const int k = tensor_of(tl, chunk, 0);
+  const int64_t n = tl.n[k], block = int64_t(chunk - tl.first_chunk[k]) * (kChunk / kBlock) + warp;
+  if (block * kBlock >= n) return;
+  const int64_t at = block * kBlock + lane * 4;
+  auto all = [&](auto f) {
+    constexpr bool F = decltype(f)::value;
+    uint32_t qm[2], qv[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      load4(static_cast<const uint8_t*>(tl.m[k]), block * kBlock + j * 128 + lane * 4, n, vec, qm[j]);
-      load4(static_cast<const uint8_t*>(tl.v[k]), block * kBlock + j * 128 + lane * 4, n, vec, qv[j]);
+      qm[j] = load_codes<F>(tl.at[kM][k], at + j * 128, n);
+      qv[j] = load_codes<F>(tl.at[kV][k], at + j * 128, n);
     }
+    const float ms = static_cast<const float*>(tl.at[L::kMs][k])[block];
+    const float vs = static_cast<const float*>(tl.at[L::kVs][k])[block];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       float m[4], v[4];
       decode_m(qm[j], ms, m);
       decode_v(qv[j], vs, v);
-      store4(static_cast<float*>(tl.p[k]), block * kBlock + j * 128 + lane * 4, n, vec, m);
-      store4(tl.master[k], block * kBlock + j * 128 + lane * 4, n, vec, v);
+      store4<F>(tl.at[kG][k], at + j * 128, n, m);
+      store4<F>(tl.at[kMaster][k], at + j * 128, n, v);
     }
-  }
+  };
+  if (tl.vec[k] && (block + 1) * kBlock <= n) all(std::true_type{});
+  else all(std::false_type{});
 }
 
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
-// Fills the list with tensors from `from` on, as many as fit; returns the first that does not.
+// Host arrays in the order of a layout, the bytes that four elements of each take (0: scales, which have no say in whether
+// accesses are vectors), and the sizes.
 struct Arrays {
-  void* const* p;
-  float* const* master;
-  const void* const* g;
-  void* const* m;
-  void* const* v;
-  float* const* ms;
-  float* const* vs;
+  const void* const* at[7];
+  int unit[7];
   const int64_t* n;
-  int p_size, m_size;  // bytes of an element
 };
-template <int MAX>
-int fill(List<MAX>& tl, const Arrays& a, int from, int n_tensors) {
+// Fills the list with tensors from `from` on, as many as fit; returns the first that does not.
+template <int ARRAYS, int MAX>
+int fill(List<ARRAYS, MAX>& tl, const Arrays& a, int from, int n_tensors) {
   tl.count = 0;
   tl.first_tensor = from;
   tl.first_chunk[0] = 0;
@@ -333,55 +429,57 @@ int fill(List<MAX>& tl, const Arrays& a, int from, int n_tensors) {
   for (; i < n_tensors && tl.count < MAX; ++i) {
     const int k = tl.count;
     const int64_t chunks = gc::ceil_div(a.n[i], kChunk);
-    if (int64_t(tl.first_chunk[k]) + chunks > 0x40000000) break;
-    tl.p[k] = a.p[i];
-    tl.master[k] = a.master ? a.master[i] : static_cast<float*>(a.p[i]);
-    tl.g[k] = a.g ? a.g[i] : nullptr;
-    tl.m[k] = a.m[i];
-    tl.v[k] = a.v[i];
-    tl.ms[k] = a.ms ? a.ms[i] : nullptr;
-    tl.vs[k] = a.vs ? a.vs[i] : nullptr;
+    if (int64_t(tl.first_chunk[k]) + chunks > 0x3F000000) break;
+    bool vec = true;
+    for (int r = 0; r < ARRAYS; ++r) {
+      tl.at[r][k] = const_cast<void*>(a.at[r][i]);
+      vec = vec && (a.unit[r] == 0 || aligned(a.at[r][i], a.unit[r]));
+    }
     tl.n[k] = a.n[i];
-    tl.vec[k] = aligned(tl.p[k], 4 * a.p_size) && aligned(tl.g[k], 4 * a.p_size) && aligned(tl.master[k], 16) &&
-                aligned(tl.m[k], 4 * a.m_size) && aligned(tl.v[k], 4 * a.m_size);
+    tl.vec[k] = vec;
     tl.first_chunk[k + 1] = tl.first_chunk[k] + int32_t(chunks);
     ++tl.count;
   }
   return i;
 }
 
-template <int MAX, int BITS, class TP>
-void launch(const List<MAX>& tl, const Hyper& hp, void* state, cudaStream_t st) {
-  const int total = tl.first_chunk[tl.count];
-  const int blocks = std::max(1, std::min(total, gc::kNumSMs * (BITS == 8 ? 4 : 4)));
-  adamw_kernel<BITS, TP, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, static_cast<unsigned long long*>(state));
-}
-template <int MAX>
-int step(const Arrays& a, int n_tensors, int bits, Hyper hp, void* state, cudaStream_t st) {
+template <int BITS, class TP, int MAX>
+int step_lists(const Arrays& a, int n_tensors, Hyper hp, void* state, cudaStream_t st) {
+  constexpr int kArrays = Layout<BITS, sizeof(TP) == 2>::kArrays;
+  static_assert(sizeof(List<kArrays, MAX>) + sizeof(Hyper) <= 32000, "launch parameters");
+  unsigned long long* count = static_cast<unsigned long long*>(state);
   int from = 0, launches = 0;
   do {
-    List<MAX> tl;
+    List<kArrays, MAX> tl;
     const int next = fill(tl, a, from, n_tensors);
     if (next == from && n_tensors > 0) return gc::fail(GC_ERR_UNSUPPORTED, "gc_adamw_step: tensor %d is too large", from);
     hp.advance = next >= n_tensors;
-    if (bits == 8) a.p_size == 2 ? launch<MAX, 8, bf16>(tl, hp, state, st) : launch<MAX, 8, float>(tl, hp, state, st);
-    else a.p_size == 2 ? launch<MAX, 32, bf16>(tl, hp, state, st) : launch<MAX, 32, float>(tl, hp, state, st);
+    const int passes = tl.first_chunk[tl.count] * (BITS == 8 ? 1 : 2);
+    // as many CTAs as the SMs hold, each over many passes; an empty model still counts the step
+    const int blocks = std::max(1, std::min(passes, gc::kNumSMs * (BITS == 8 ? 3 : 6)));
+    if constexpr (BITS == 8) adamw_8bit_kernel<TP, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
+    else adamw_kernel<TP, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
     ++launches;
     from = next;
   } while (from < n_tensors);
   return gc::check_launch("gc_adamw_step", launches);
 }
+template <int BITS, class TP>
+int step(const Arrays& a, int n_tensors, const Hyper& hp, void* state, cudaStream_t st) {
+  return n_tensors <= kFew ? step_lists<BITS, TP, kFew>(a, n_tensors, hp, state, st)
+                           : step_lists<BITS, TP, Layout<BITS, sizeof(TP) == 2>::kMany>(a, n_tensors, hp, state, st);
+}
 template <int MAX>
 int moments(const Arrays& a, int n_tensors, cudaStream_t st) {
   int launches = 0;
   for (int from = 0; from < n_tensors;) {
-    List<MAX> tl;
+    List<Layout<8, false>::kArrays, MAX> tl;
     const int next = fill(tl, a, from, n_tensors);
     if (next == from) return gc::fail(GC_ERR_UNSUPPORTED, "gc_adamw_moments_f32: tensor %d is too large", from);
     from = next;
     const int total = tl.first_chunk[tl.count];
     if (total == 0) continue;
-    adamw_moments_kernel<MAX><<<std::min(total, gc::kNumSMs * 8), kThreads, 0, st>>>(tl, total);
+    adamw_moments_kernel<MAX><<<total, kThreads, 0, st>>>(tl);
     ++launches;
   }
   return launches ? gc::check_launch("gc_adamw_moments_f32", launches) : GC_OK;
@@ -411,11 +509,18 @@ int gc_adamw_step(int n_tensors, void* const* params, int param_type, const void
   }
   Hyper hp{lr, beta1, beta2, float(beta1), float(1.0 - beta1), float(beta2), float(1.0 - beta2), float(eps),
            float(1.0 - lr * weight_decay), seed, 0};
-  const Arrays a{params, mixed ? masters : nullptr, grads, exp_avg, exp_avg_sq, eight ? exp_avg_scales : nullptr,
-                 eight ? exp_avg_sq_scales : nullptr, sizes, mixed ? 2 : 4, eight ? 1 : 4};
+  const auto list = [](auto p) { return reinterpret_cast<const void* const*>(p); };
+  const int tp = mixed ? 8 : 16, tm = eight ? 4 : 16;
+  Arrays a{{grads, list(exp_avg), list(exp_avg_sq), mixed ? list(masters) : list(params)}, {tp, tm, tm, 16}, sizes};
+  int r = kMaster + 1;
+  if (mixed) a.unit[r] = tp, a.at[r++] = list(params);
+  if (eight) {
+    a.at[r++] = list(exp_avg_scales);
+    a.at[r++] = list(exp_avg_sq_scales);
+  }
   const cudaStream_t st = gc::as_stream(stream);
-  return n_tensors <= kFew ? step<kFew>(a, n_tensors, state_bits, hp, state, st)
-                           : step<kMany>(a, n_tensors, state_bits, hp, state, st);
+  if (eight) return mixed ? step<8, bf16>(a, n_tensors, hp, state, st) : step<8, float>(a, n_tensors, hp, state, st);
+  return mixed ? step<32, bf16>(a, n_tensors, hp, state, st) : step<32, float>(a, n_tensors, hp, state, st);
 }
 
 int gc_adamw_moments_f32(int n_tensors, const uint8_t* const* exp_avg, const uint8_t* const* exp_avg_sq,
@@ -431,12 +536,13 @@ int gc_adamw_moments_f32(int n_tensors, const uint8_t* const* exp_avg, const uin
                                  exp_avg_out[i] && exp_avg_sq_out[i]),
                "gc_adamw_moments_f32: null pointer in tensor %d", i);
   }
-  const Arrays a{reinterpret_cast<void* const*>(exp_avg_out), exp_avg_sq_out, nullptr,
-                 const_cast<void* const*>(reinterpret_cast<const void* const*>(exp_avg)),
-                 const_cast<void* const*>(reinterpret_cast<const void* const*>(exp_avg_sq)),
-                 const_cast<float* const*>(exp_avg_scales), const_cast<float* const*>(exp_avg_sq_scales), sizes, 4, 1};
+  const auto list = [](auto p) { return reinterpret_cast<const void* const*>(p); };
+  const Arrays a{{list(exp_avg_out), list(exp_avg), list(exp_avg_sq), list(exp_avg_sq_out), list(exp_avg_scales),
+                  list(exp_avg_sq_scales)},
+                 {16, 4, 4, 16},
+                 sizes};
   const cudaStream_t st = gc::as_stream(stream);
-  return n_tensors <= kFew ? moments<kFew>(a, n_tensors, st) : moments<kMany>(a, n_tensors, st);
+  return n_tensors <= kFew ? moments<kFew>(a, n_tensors, st) : moments<Layout<8, false>::kMany>(a, n_tensors, st);
 }
 
 }  // extern "C"

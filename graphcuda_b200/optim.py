@@ -93,7 +93,7 @@ class FusedSGD(torch.optim.Optimizer):
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, masters=None, scales=None, seed: int = 0) -> None:
-    """One AdamW step over lists of tensors, in place; one launch per 440 tensors.
+    """One AdamW step over lists of tensors, in place; one launch for up to 449 tensors.
 
     ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
     ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)``.
