@@ -88,12 +88,12 @@ SIGNATURES = {
     "gc_rms_norm_backward_workspace_bytes": (_size, [_i64, _i64]),
     "gc_rms_norm_backward": (_int, [_void, _int, _i64, _void, _i64, _void, _i64, _void, _i64, _int, _f32p, _f32p, _i64,
                                     _i64, _void, _int, _i64, _void, _i64, _f32p, _void, _size, _void]),
-    "gc_gated_ffn_hidden_pitch": (_i64, [_i64]),
+    "gc_gated_ffn_saved_bytes": (_size, [_i64, _i64]),
     "gc_gated_ffn_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _int]),
     "gc_gated_ffn_forward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _i64, _i64, _i64, _i64, _int, _void, _i64,
-                                         _void, _void, _void, _size, _void]),
-    "gc_gated_ffn_backward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _void, _i64, _void, _void, _i64, _i64, _i64,
-                                          _i64, _int, _void, _i64, _void, _i64, _void, _i64, _void, _size, _void]),
+                                         _void, _void, _size, _void]),
+    "gc_gated_ffn_backward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _void, _i64, _void, _i64, _i64, _i64, _i64, _int,
+                                          _void, _i64, _void, _i64, _void, _i64, _void, _size, _void]),
     "gc_gated_ffn_e4m3_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
     "gc_gated_ffn_forward_e4m3": (_int, [_void, _i64, _f32p, _void, _i64, _f32p, _void, _i64, _i64, _i64, _i64, _i64, _int,
                                          _void, _i64, _void, _size, _void]),

@@ -10,18 +10,21 @@
 //   GatedBack  the accumulator is a tile of dA, which is never stored: the epilogue reads G and U and stores dG and dU
 //   Plain      a bf16 product: Y, dX and the weight gradients
 // Operands are read where they lie: K-major or MN-major tiles (matrices whose rows run along the product's K or across it),
-// so nothing is transposed in memory.  Sums are fp32 in TMEM.  A, G, U, dG and dU are rounded to bf16 where they are stored
-// between kernels: they are the next product's operands, which the tensor core takes in 16 bits; every one adds a
-// relative 2^-9 at random, as the output's own rounding does.
+// so nothing is transposed in memory.  Sums are fp32 in TMEM.  A, dG and dU are rounded to bf16 where they are stored
+// between kernels: they are the next product's operands, which the tensor core takes in 16 bits; that adds as much noise
+// as the output's own rounding does.  G and U are no operands, and three times their rounding on top would show in dX and
+// dWin: they are kept as fp16 numbers with an exponent for every 32 columns of a row, eight times as exact in as many bits.
 //
-// CTA = 12 warps, persistent over tiles of 128 x BN accumulators (or a pair of CTAs over 256 x BN):
+// CTA = 20 warps, persistent over tiles of 128 x BN accumulators (or a pair of CTAs over 256 x BN):
 //   warp 0       TMA producer (one lane)
 //   warp 1       MMA issuer (one lane)
 //   warp 2       TMEM allocator
-//   warps 4-11   epilogue: two warps per TMEM lane quarter, one for the even 64-column chunks, one for the odd ones; a
-//                chunk leaves through a swizzled 32 x 64 tile in shared memory and one TMA store
-// Two accumulators in TMEM let the epilogue of a tile overlap the main loop of the next.  Products with few tiles and a
-// long K are split along K into fp32 parts that a second kernel adds in a fixed order.
+//   warps 4-19   epilogue: four warps per TMEM lane quarter, which take the 32-column chunks of a tile in turn; a
+//                chunk leaves through a swizzled 32 x 32 tile in shared memory and one TMA store
+// Two accumulators in TMEM let the epilogue of a tile overlap the main loop of the next.  The epilogues are chains of
+// dependent loads and special functions: with 8 warps on chunks of 64 columns they, not memory or the tensor cores, set the
+// time of products with a short K.  Products with few tiles and a long K are split along K into fp32 parts that a second
+// kernel adds in a fixed order.
 //
 // Every wait on a barrier is bounded, as in the other tensor-core kernel: a wait that ran out raises the device's error
 // word, all roles leave, copies in flight are drained and TMEM is released.
@@ -30,6 +33,7 @@
 #include "tcgen05.cuh"
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 
@@ -39,10 +43,10 @@ using namespace gc::tc;
 using bf16 = __nv_bfloat16;
 
 constexpr int BM = 128;
-constexpr int kThreads = 384;
-constexpr int kEpiWarps = 8;
-constexpr int kTileBytes = 32 * 128;  // what a warp stores at once: 32 rows of 128 bytes
-constexpr int kBuffers = 2;           // of them per warp
+constexpr int kEpiWarps = 16, kEpiGroups = kEpiWarps / 4;
+constexpr int kThreads = 128 + 32 * kEpiWarps;
+constexpr int kTileBytes = 32 * 64;  // what a warp stores at once: 32 rows of 64 bytes
+constexpr int kBuffers = 2;          // of them per warp
 
 enum Kind { kPlain, kGated, kGatedBack };
 
@@ -63,7 +67,7 @@ struct Params {
   int M, N, K;  // of the product; Gated: N = H, the columns of G and of U
   int b_up;     // Gated: where U's columns start in B
   int act;
-  int save;         // Gated: G and U are stored
+  int8_t* exps;     // G's and U's exponents, [2][ceil(N / 32)][M] (Gated: null where G and U are not stored)
   const float* sa;  // e4m3: scales of A's rows and B's columns
   const float* sb;
   bf16* C;  // Plain: the output, for rows that TMA cannot store
@@ -160,9 +164,40 @@ __device__ __forceinline__ void with_activation(int act, F&& f) {
   else f(std::integral_constant<int, GC_ACT_RELU>{});
 }
 
-// The 16-byte unit `j` of a lane's row in a warp's swizzled tile.
+// The 16-byte unit `j` of a row in a warp's swizzled tile.
 __device__ __forceinline__ uint4* unit(uint8_t* tile, int row, int j) {
-  return reinterpret_cast<uint4*>(tile + row * 128 + ((j ^ (row & 7)) << 4));
+  return reinterpret_cast<uint4*>(tile + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+}
+
+// 32 values to fp16 with a common power of two, which is returned: 0 unless the largest would overflow or fall below 2^-10,
+// where fp16 begins to lose bits; then it brings the largest to 2^14.
+__device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t (&out)[16]) {
+  __half2 top = __float2half2_rn(0.f);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+    top = __hmax2(top, __habs2(h));
+    out[j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const uint32_t t = *reinterpret_cast<const uint32_t*>(&top), most = max(t & 0xFFFFu, t >> 16);
+  if (most >= 0x1400u && most < 0x7C00u) return 0;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) bits = max(bits, v[j] & 0x7FFFFFFFu);
+  if (bits == 0 || bits >= 0x7F800000u) return 0;  // zeros; an infinity or a NaN, with which the row is lost
+  const int e = max(int(bits >> 23) - 127 - 14, -126);
+  // two factors: 2^-e alone may not be a number
+  const float a = __uint_as_float(uint32_t(127 - e / 2) << 23), b = __uint_as_float(uint32_t(127 - (e - e / 2)) << 23);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]) * a * b, __uint_as_float(v[2 * j + 1]) * a * b);
+    out[j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return e;
+}
+__device__ __forceinline__ float2 unpack_fp16(uint32_t w, float scale) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return make_float2(f.x * scale, f.y * scale);
 }
 
 // Where a column of the product goes (see Params); one that is dropped goes beyond the last.
@@ -328,8 +363,8 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp % 4;             // TMEM lane quarter
-    const int grp = (warp - 4) / 4;     // parity of the 64-column chunks
+    const int q = warp % 4;          // TMEM lane quarter
+    const int grp = (warp - 4) / 4;  // which of the 32-column chunks: grp, grp + 4, ..
     uint8_t* tiles = smem + kStagingAt + (warp - 4) * (kBuffers * kTileBytes);
     const uint32_t tiles_u = smem_u32(tiles);
     int buf = 0;
@@ -350,15 +385,24 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
         store_commit();
       }
     };
+    auto put_words = [&](const CUtensorMap* map, const uint32_t (&w)[16], int x, int y) {
+      const int b = acquire();
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *unit(tiles + b * kTileBytes, lane, j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      put(map, b, x, y);
+    };
     uint32_t tcount = 0, loads = 0;
     bool ok = true;
     for (int item = first_item; item < num_items && ok; item += item_step, ++tcount) {
       int m0, n0, kb0, kb1, split;
       item_coords(item, m0, n0, kb0, kb1, split);
       const int b = tcount & 1;
-      const int row0 = m0 + q * 32;  // first of the warp's rows
+      const int row0 = m0 + q * 32, row = row0 + lane;  // the warp's first row, the lane's
       const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * BN);
-      bool have_in = false;  // GatedBack: the first chunk's G and U are on their way while the tile is being computed
+      const int chunks_m = (p.N + 31) / 32;  // Gated, GatedBack: rows of a table of exponents
+      // GatedBack: G and U of a chunk; those of the first are on their way while the tile is being computed
+      bool have_in = false;
       auto request = [&](int col) {
         if (lane == 0) {
           store_wait_read<0>();
@@ -367,173 +411,125 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           tma_load_2d(tiles_u + kTileBytes, &maps.in2, col, row0, bar_in(warp - 4));
         }
       };
-      if (KIND == kGatedBack && n0 + grp * 64 < p.N && row0 < p.M) {
-        request(n0 + grp * 64);
+      if (KIND == kGatedBack && n0 + grp * 32 < p.N && row0 < p.M) {
+        request(n0 + grp * 32);
         have_in = true;
       }
       if (!mbar_wait(bar_tfull(b), (tcount >> 1) & 1u, abort_p)) ok = false;
       if (ok) tc_fence_after();
-      if constexpr (KIND == kGatedBack) {
-        for (int c = grp; c < NT / 64; c += 2) {
-          const int col = n0 + c * 64;
-          if (col >= p.N || row0 >= p.M) break;
-          if (!have_in) {
-            if (!ok) break;
-            request(col);
-          }
+      for (int c = grp; c < NT / 32 && (ok || have_in); c += kEpiGroups) {
+        const int col = n0 + c * 32;
+        if (col >= p.N || row0 >= p.M) break;
+        if constexpr (KIND == kGatedBack) {
+          if (!have_in) request(col);
           have_in = false;
+          const int64_t at = int64_t(col / 32) * p.M + min(row, p.M - 1);
+          const float sg = __uint_as_float(uint32_t(127 + p.exps[at]) << 23);
+          const float su = __uint_as_float(uint32_t(127 + p.exps[at + int64_t(chunks_m) * p.M]) << 23);
+          uint32_t acc[32];
+          if (ok) tmem_ld32(taddr + uint32_t(c * 32), acc);
           if (!mbar_wait(bar_in(warp - 4), loads & 1u, abort_p)) {
             drain(bar_in(warp - 4), loads & 1u);
             ok = false;
           }
           ++loads;
           if (!ok) break;
-#pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            uint32_t acc[32];
-            tmem_ld32(taddr + uint32_t(c * 64 + half * 32), acc);
-            tmem_ld_wait();
-            with_activation(p.act, [&](auto act) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint4* gp = unit(tiles, lane, half * 4 + j);
-                uint4* up = unit(tiles + kTileBytes, lane, half * 4 + j);
-                uint4 g4 = *gp, u4 = *up;
-                uint32_t* gw = &g4.x;
-                uint32_t* uw = &u4.x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float d0 = __uint_as_float(acc[j * 8 + 2 * e]), d1 = __uint_as_float(acc[j * 8 + 2 * e + 1]);
-                  float s0, s1;
-                  const float a0 = activate<decltype(act)::value>(low(gw[e]), s0);
-                  const float a1 = activate<decltype(act)::value>(high(gw[e]), s1);
-                  gw[e] = pack2(d0 * low(uw[e]) * s0, d1 * high(uw[e]) * s1);
-                  uw[e] = pack2(d0 * a0, d1 * a1);
-                }
-                *gp = g4;
-                *up = u4;
-              }
-            });
-          }
-          put(&maps.out, 0, col, row0);
-          put(&maps.out2, 1, col, row0);
-        }
-      } else if (ok && KIND == kGated) {
-        const float sa = F8 ? p.sa[min(row0 + lane, p.M - 1)] : 1.f;
-        for (int c = grp; c < NT / 64; c += 2) {
-          const int col = n0 + c * 64;
-          if (col >= p.N || row0 >= p.M) break;
-          const int ba = acquire();
-          uint32_t hold_g[32], hold_u[32];  // packed, 64 columns each, where they are stored too
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t g[32], u[32];
-            tmem_ld32(taddr + uint32_t(c * 64 + half * 32), g);
-            tmem_ld32(taddr + uint32_t(NT + c * 64 + half * 32), u);
-            tmem_ld_wait();
-            if (F8) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int n = min(col + half * 32 + j, p.N - 1);
-                g[j] = __float_as_uint(__uint_as_float(g[j]) * (sa * __ldg(p.sb + n)));
-                u[j] = __float_as_uint(__uint_as_float(u[j]) * (sa * __ldg(p.sb + p.b_up + n)));
-              }
-            }
-            if (!F8 && p.save) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                hold_g[half * 16 + j] = pack2(__uint_as_float(g[2 * j]), __uint_as_float(g[2 * j + 1]));
-                hold_u[half * 16 + j] = pack2(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
-              }
-            }
-            with_activation(p.act, [&](auto act) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint4 o;
-                uint32_t* w = &o.x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const int i = j * 8 + 2 * e;
-                  float unused;
-                  w[e] = pack2(activate<decltype(act)::value>(__uint_as_float(g[i]), unused) * __uint_as_float(u[i]),
-                               activate<decltype(act)::value>(__uint_as_float(g[i + 1]), unused) * __uint_as_float(u[i + 1]));
-                }
-                *unit(tiles + ba * kTileBytes, lane, half * 4 + j) = o;
-              }
-            });
-          }
-          put(&maps.out, ba, col, row0);
-          if (!F8 && p.save) {
-            const int bg = acquire();
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *unit(tiles + bg * kTileBytes, lane, j) =
-                  make_uint4(hold_g[4 * j], hold_g[4 * j + 1], hold_g[4 * j + 2], hold_g[4 * j + 3]);
-            put(&maps.out2, bg, col, row0);
-            const int bu = acquire();
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *unit(tiles + bu * kTileBytes, lane, j) =
-                  make_uint4(hold_u[4 * j], hold_u[4 * j + 1], hold_u[4 * j + 2], hold_u[4 * j + 3]);
-            put(&maps.out3, bu, col, row0);
-          }
-        }
-      } else if (ok && splits > 1) {
-        // fp32 parts, 32 columns at a time
-        for (int c = grp; c < NT / 32; c += 2) {
-          const int col = n0 + c * 32;
-          if (col >= p.N || row0 >= p.M) break;
-          uint32_t acc[32];
-          tmem_ld32(taddr + uint32_t(c * 32), acc);
-          const int bo = acquire();
           tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *unit(tiles + bo * kTileBytes, lane, j) = make_uint4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_3d(&maps.out, tiles_u + bo * kTileBytes, col, row0, split);
-            store_commit();
-          }
-        }
-      } else if (ok) {
-        for (int c = grp; c < NT / 64; c += 2) {
-          const int col = n0 + c * 64;
-          if (col >= p.N || row0 >= p.M) break;
-          const int bo = acquire();
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t acc[32];
-            tmem_ld32(taddr + uint32_t(c * 64 + half * 32), acc);
-            tmem_ld_wait();
+          with_activation(p.act, [&](auto act) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              uint4 o;
-              uint32_t* w = &o.x;
+              uint4* gp = unit(tiles, lane, j);
+              uint4* up = unit(tiles + kTileBytes, lane, j);
+              uint4 g4 = *gp, u4 = *up;
+              uint32_t* gw = &g4.x;
+              uint32_t* uw = &u4.x;
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = pack2(__uint_as_float(acc[j * 8 + 2 * e]), __uint_as_float(acc[j * 8 + 2 * e + 1]));
-              *unit(tiles + bo * kTileBytes, lane, half * 4 + j) = o;
+              for (int e = 0; e < 4; ++e) {
+                const float d0 = __uint_as_float(acc[j * 8 + 2 * e]), d1 = __uint_as_float(acc[j * 8 + 2 * e + 1]);
+                const float2 g = unpack_fp16(gw[e], sg), u = unpack_fp16(uw[e], su);
+                float s0, s1;
+                const float a0 = activate<decltype(act)::value>(g.x, s0);
+                const float a1 = activate<decltype(act)::value>(g.y, s1);
+                gw[e] = pack2(d0 * u.x * s0, d1 * u.y * s1);
+                uw[e] = pack2(d0 * a0, d1 * a1);
+              }
+              *gp = g4;
+              *up = u4;
+            }
+          });
+          put(&maps.out, 0, col, row0);
+          put(&maps.out2, 1, col, row0);
+        } else if constexpr (KIND == kGated) {
+          uint32_t g[32], u[32], w[16];
+          tmem_ld32(taddr + uint32_t(c * 32), g);
+          tmem_ld32(taddr + uint32_t(NT + c * 32), u);
+          tmem_ld_wait();
+          if (F8) {
+            const float sa = p.sa[min(row, p.M - 1)];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int n = min(col + j, p.N - 1);
+              g[j] = __float_as_uint(__uint_as_float(g[j]) * (sa * __ldg(p.sb + n)));
+              u[j] = __float_as_uint(__uint_as_float(u[j]) * (sa * __ldg(p.sb + p.b_up + n)));
             }
           }
-          if (p.tma_store) {
-            put(&maps.out, bo, col, row0);
-          } else {
-            // rows of an odd pitch: two neighbouring columns per lane, row by row
-            __syncwarp();
-            const int rows = min(32, p.M - row0);
-            for (int r = 0; r < rows; ++r) {
-              const uint32_t w = *reinterpret_cast<const uint32_t*>(
-                  reinterpret_cast<const uint8_t*>(unit(tiles + bo * kTileBytes, r, lane / 4)) + (lane % 4) * 4);
-              bf16* out = p.C + int64_t(row0 + r) * p.ldc;
+          if (!F8 && p.exps) {
+            const int64_t at = int64_t(col / 32) * p.M + row;
+            const int eg = pack_fp16(g, w);
+            if (row < p.M) p.exps[at] = int8_t(eg);
+            put_words(&maps.out2, w, col, row0);
+            const int eu = pack_fp16(u, w);
+            if (row < p.M) p.exps[at + int64_t(chunks_m) * p.M] = int8_t(eu);
+            put_words(&maps.out3, w, col, row0);
+          }
+          with_activation(p.act, [&](auto act) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int n = out_column(col + 2 * lane + e, p.gap_from, p.gap);
-                if (n < p.c_cols) out[n] = __ushort_as_bfloat16(uint16_t(e ? w >> 16 : w));
-              }
+            for (int j = 0; j < 16; ++j) {
+              float unused;
+              w[j] = pack2(activate<decltype(act)::value>(__uint_as_float(g[2 * j]), unused) * __uint_as_float(u[2 * j]),
+                           activate<decltype(act)::value>(__uint_as_float(g[2 * j + 1]), unused) * __uint_as_float(u[2 * j + 1]));
             }
+          });
+          put_words(&maps.out, w, col, row0);
+        } else if (splits > 1) {
+          // fp32 parts, 16 columns to a tile
+          uint32_t acc[32];
+          tmem_ld32(taddr + uint32_t(c * 32), acc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int bo = acquire();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int i = half * 16 + 4 * j;
+              *unit(tiles + bo * kTileBytes, lane, j) = make_uint4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+            }
+            fence_async_smem();
             __syncwarp();
+            if (lane == 0) {
+              if (col + half * 16 < p.N) tma_store_3d(&maps.out, tiles_u + bo * kTileBytes, col + half * 16, row0, split);
+              store_commit();
+            }
+          }
+        } else {
+          uint32_t acc[32], w[16];
+          tmem_ld32(taddr + uint32_t(c * 32), acc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = pack2(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
+          if (p.tma_store) {
+            put_words(&maps.out, w, col, row0);
+          } else {
+            // rows of an odd pitch: a row at a time, a column per lane
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *unit(tiles, lane, j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            __syncwarp();
+            const int n = out_column(col + lane, p.gap_from, p.gap), rows = min(32, p.M - row0);
+            if (n < p.c_cols)
+              for (int r = 0; r < rows; ++r)
+                p.C[int64_t(row0 + r) * p.ldc + n] =
+                    reinterpret_cast<const bf16*>(unit(tiles, r, lane / 8))[lane % 8];
           }
         }
       }
@@ -603,6 +599,7 @@ struct Matrix {  // row-major, `size` bytes per element
   int size;
 };
 
+// Boxes of 128 bytes x box_rows are operands; the epilogues' are of 64 bytes.
 int make_map(CUtensorMap* map, const Matrix& m, int box_cols, int box_rows, int64_t planes = 0) {
   EncodeFn enc = get_encode();
   if (!enc) return gc::fail(GC_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
@@ -614,8 +611,9 @@ int make_map(CUtensorMap* map, const Matrix& m, int box_cols, int box_rows, int6
                                    : m.size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT8;
   const CUresult r = enc(map, type, planes ? 3 : 2, const_cast<void*>(m.p), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_cols * m.size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return gc::fail(GC_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
   return GC_OK;
 }
@@ -735,8 +733,8 @@ int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int
   int rc = error_word(&p.word);
   if (rc == GC_OK) rc = operand_maps(maps, A, a_mn, B, b_mn, s.tile.pair ? s.tile.bn / 2 : s.tile.bn);
   const int64_t pitch = part_pitch(N);
-  if (rc == GC_OK && s.splits > 1) rc = make_map(&maps.out, Matrix{workspace, M, N, pitch, 4}, 32, 32, s.splits);
-  else if (rc == GC_OK && p.tma_store) rc = make_map(&maps.out, Matrix{C, M, N, ldc, 2}, 64, 32);
+  if (rc == GC_OK && s.splits > 1) rc = make_map(&maps.out, Matrix{workspace, M, N, pitch, 4}, 16, 32, s.splits);
+  else if (rc == GC_OK && p.tma_store) rc = make_map(&maps.out, Matrix{C, M, N, ldc, 2}, 32, 32);
   if (rc != GC_OK) return rc;
   if (a_mn) rc = launch_tile<kPlain, true, true, false>(s.tile, maps, p, st);
   else if (b_mn) rc = launch_tile<kPlain, false, true, false>(s.tile, maps, p, st);
@@ -786,6 +784,23 @@ int make_gate_up(Matrix& w, int64_t H, char*& ws, cudaStream_t st) {
   return rc;
 }
 
+// What a forward pass leaves for the backward pass, in one buffer.
+struct Saved {
+  uint16_t* hidden;   // M x P, P = up8(H)
+  uint16_t* gate_up;  // M x 2P: G and U as fp16 numbers
+  int8_t* exps;       // and their exponents
+};
+Saved saved_at(void* p, int64_t M, int64_t H) {
+  const int64_t hp = up8(H);
+  char* c = static_cast<char*>(p);
+  Saved s;
+  s.hidden = reinterpret_cast<uint16_t*>(c);
+  c += align256(size_t(M) * hp * 2);
+  s.gate_up = reinterpret_cast<uint16_t*>(c);
+  s.exps = reinterpret_cast<int8_t*>(c + align256(size_t(M) * hp * 4));
+  return s;
+}
+
 bool sizes_ok(int64_t M, int64_t D, int64_t H, int64_t O) {
   const int64_t top = (int64_t(1) << 31) - 512;  // coordinates and tile counts are 32-bit
   return M <= top && D <= top && 2 * up8(H) <= top && O <= top;
@@ -795,7 +810,11 @@ bool sizes_ok(int64_t M, int64_t D, int64_t H, int64_t O) {
 
 extern "C" {
 
-int64_t gc_gated_ffn_hidden_pitch(int64_t H) { return up8(std::max<int64_t>(H, 0)); }
+size_t gc_gated_ffn_saved_bytes(int64_t M, int64_t H) {
+  if (M <= 0 || H <= 0) return 0;
+  const int64_t hp = up8(H);
+  return align256(size_t(M) * hp * 2) + align256(size_t(M) * hp * 4) + align256(2 * size_t(gc::ceil_div(hp, 32)) * size_t(M));
+}
 
 size_t gc_gated_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O, int backward) {
   if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, D, H, O)) return 0;
@@ -809,7 +828,7 @@ size_t gc_gated_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O, 
 
 int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin, const uint16_t* Wout,
                               int64_t ldwout, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy,
-                              uint16_t* hidden, uint16_t* gate_up, void* workspace, size_t workspace_bytes, void* stream) {
+                              void* saved, void* workspace, size_t workspace_bytes, void* stream) {
   GC_REQUIRE(M >= 0 && D >= 0 && H >= 0 && O >= 0, "gc_gated_ffn_forward_bf16: negative size");
   GC_REQUIRE(act >= GC_ACT_SILU && act <= GC_ACT_RELU, "gc_gated_ffn_forward_bf16: unknown activation");
   GC_REQUIRE(ldx >= D && ldwin >= 2 * H && ldwout >= O && ldy >= O,
@@ -820,13 +839,11 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   GC_REQUIRE(Y, "gc_gated_ffn_forward_bf16: null pointer");
   const int64_t hp = up8(H);
   if (D == 0 || H == 0) {  // G = U = 0, or no hidden columns: Y = 0
-    cudaError_t e = cudaMemset2DAsync(Y, size_t(ldy) * 2, 0, size_t(O) * 2, size_t(M), st);
-    if (e == cudaSuccess && hidden && H) e = cudaMemsetAsync(hidden, 0, size_t(M) * hp * 2, st);
-    if (e == cudaSuccess && gate_up && H) e = cudaMemsetAsync(gate_up, 0, size_t(M) * hp * 4, st);
+    const cudaError_t e = cudaMemset2DAsync(Y, size_t(ldy) * 2, 0, size_t(O) * 2, size_t(M), st);
     return e == cudaSuccess ? GC_OK : gc::fail(GC_ERR_CUDA, "gc_gated_ffn_forward_bf16: %s", cudaGetErrorString(e));
   }
   GC_REQUIRE(X && Win && Wout, "gc_gated_ffn_forward_bf16: null pointer");
-  GC_REQUIRE(gc::aligned16(hidden) && gc::aligned16(gate_up), "gc_gated_ffn_forward_bf16: saved matrices must be 16-byte aligned");
+  GC_REQUIRE(gc::aligned16(saved), "gc_gated_ffn_forward_bf16: the saved buffer must be 16-byte aligned");
   if (!workspace || workspace_bytes < gc_gated_ffn_workspace_bytes(M, D, H, O, 0))
     return gc::fail(GC_ERR_WORKSPACE, "gc_gated_ffn_forward_bf16: workspace missing or smaller than its query says");
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_bf16: workspace must be 16-byte aligned");
@@ -836,8 +853,12 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   if (rc == GC_OK) rc = make_gate_up(win, H, ws, st);
   if (rc == GC_OK) rc = make_readable(wout, ws, st);
   if (rc != GC_OK) return rc;
-  if (!hidden) {
-    hidden = reinterpret_cast<uint16_t*>(ws);
+  uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);
+  Saved keep{};
+  if (saved) {
+    keep = saved_at(saved, M, H);
+    hidden = keep.hidden;
+  } else {
     ws += align256(size_t(M) * hp * 2);
   }
   const Tile t = pick_tile(kGated, M, hp, 1);
@@ -846,20 +867,20 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   p.M = int(M); p.N = int(hp); p.K = int(D);
   p.b_up = int(hp);
   p.act = act;
-  p.save = gate_up != nullptr;
+  p.exps = keep.exps;
   rc = error_word(&p.word);
   if (rc == GC_OK) rc = operand_maps(maps, x, false, win, true, 0);
-  if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, hp, hp, 2}, 64, 32);
-  if (rc == GC_OK && gate_up) rc = make_map(&maps.out2, Matrix{gate_up, M, hp, 2 * hp, 2}, 64, 32);
-  if (rc == GC_OK && gate_up) rc = make_map(&maps.out3, Matrix{gate_up + hp, M, hp, 2 * hp, 2}, 64, 32);
+  if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, hp, hp, 2}, 32, 32);
+  if (rc == GC_OK && saved) rc = make_map(&maps.out2, Matrix{keep.gate_up, M, hp, 2 * hp, 2}, 32, 32);
+  if (rc == GC_OK && saved) rc = make_map(&maps.out3, Matrix{keep.gate_up + hp, M, hp, 2 * hp, 2}, 32, 32);
   if (rc == GC_OK) rc = launch_tile<kGated, false, true, false>(t, maps, p, st);
   if (rc != GC_OK) return rc;
   return plain(Matrix{hidden, M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
 }
 
 int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* Win,
-                               int64_t ldwin, const uint16_t* Wout, int64_t ldwout, const uint16_t* hidden,
-                               const uint16_t* gate_up, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* dX,
+                               int64_t ldwin, const uint16_t* Wout, int64_t ldwout, const void* saved,
+                               int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* dX,
                                int64_t lddx, uint16_t* dWin, int64_t lddwin, uint16_t* dWout, int64_t lddwout,
                                void* workspace, size_t workspace_bytes, void* stream) {
   GC_REQUIRE(M >= 0 && D >= 0 && H >= 0 && O >= 0, "gc_gated_ffn_backward_bf16: negative size");
@@ -881,8 +902,8 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
     return e == cudaSuccess ? GC_OK : gc::fail(GC_ERR_CUDA, "gc_gated_ffn_backward_bf16: %s", cudaGetErrorString(e));
   }
   if (!dX && !dWin && !dWout) return GC_OK;
-  GC_REQUIRE(dY && X && Win && Wout && hidden && gate_up, "gc_gated_ffn_backward_bf16: null pointer");
-  GC_REQUIRE(gc::aligned16(hidden) && gc::aligned16(gate_up), "gc_gated_ffn_backward_bf16: saved matrices must be 16-byte aligned");
+  GC_REQUIRE(dY && X && Win && Wout && saved, "gc_gated_ffn_backward_bf16: null pointer");
+  GC_REQUIRE(gc::aligned16(saved), "gc_gated_ffn_backward_bf16: the saved buffer must be 16-byte aligned");
   if (!workspace || workspace_bytes < gc_gated_ffn_workspace_bytes(M, D, H, O, 1))
     return gc::fail(GC_ERR_WORKSPACE, "gc_gated_ffn_backward_bf16: workspace missing or smaller than its query says");
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_backward_bf16: workspace must be 16-byte aligned");
@@ -893,6 +914,7 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
   if (rc == GC_OK && dX) rc = make_gate_up(win, H, ws, st);
   if (rc == GC_OK && (dX || dWin)) rc = make_readable(wout, ws, st);
   if (rc != GC_OK) return rc;
+  const Saved kept = saved_at(const_cast<void*>(saved), M, H);
   const Matrix dgu{ws, M, 2 * hp, 2 * hp, 2};
   if (dX || dWin) {
     uint16_t* out = reinterpret_cast<uint16_t*>(ws);
@@ -902,12 +924,13 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
     Params p{};
     p.M = int(M); p.N = int(hp); p.K = int(O);
     p.act = act;
+    p.exps = kept.exps;
     rc = error_word(&p.word);
     if (rc == GC_OK) rc = operand_maps(maps, dy, false, wout, false, t.pair ? t.bn / 2 : t.bn);
-    if (rc == GC_OK) rc = make_map(&maps.in1, Matrix{gate_up, M, hp, 2 * hp, 2}, 64, 32);
-    if (rc == GC_OK) rc = make_map(&maps.in2, Matrix{gate_up + hp, M, hp, 2 * hp, 2}, 64, 32);
-    if (rc == GC_OK) rc = make_map(&maps.out, Matrix{out, M, hp, 2 * hp, 2}, 64, 32);
-    if (rc == GC_OK) rc = make_map(&maps.out2, Matrix{out + hp, M, hp, 2 * hp, 2}, 64, 32);
+    if (rc == GC_OK) rc = make_map(&maps.in1, Matrix{kept.gate_up, M, hp, 2 * hp, 2}, 32, 32);
+    if (rc == GC_OK) rc = make_map(&maps.in2, Matrix{kept.gate_up + hp, M, hp, 2 * hp, 2}, 32, 32);
+    if (rc == GC_OK) rc = make_map(&maps.out, Matrix{out, M, hp, 2 * hp, 2}, 32, 32);
+    if (rc == GC_OK) rc = make_map(&maps.out2, Matrix{out + hp, M, hp, 2 * hp, 2}, 32, 32);
     if (rc == GC_OK) rc = launch_tile<kGatedBack, false, false, false>(t, maps, p, st);
     if (rc != GC_OK) return rc;
   }
@@ -915,7 +938,7 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
   if (rc == GC_OK && dWin)
     rc = plain(x, true, dgu, true, D, 2 * hp, M, reinterpret_cast<bf16*>(dWin), lddwin, H, hp - H, ws, st);
   if (rc == GC_OK && dWout)
-    rc = plain(Matrix{hidden, M, H, hp, 2}, true, dy, true, H, O, M, reinterpret_cast<bf16*>(dWout), lddwout, 0, 0, ws, st);
+    rc = plain(Matrix{kept.hidden, M, H, hp, 2}, true, dy, true, H, O, M, reinterpret_cast<bf16*>(dWout), lddwout, 0, 0, ws, st);
   return rc;
 }
 
@@ -965,7 +988,7 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   p.sb = w_scale;
   rc = error_word(&p.word);
   if (rc == GC_OK) rc = operand_maps(maps, x, false, w, false, t.bn / 2);
-  if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 64, 32);
+  if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 32, 32);
   if (rc == GC_OK) rc = launch_tile<kGated, false, false, true>(t, maps, p, st);
   if (rc != GC_OK) return rc;
   return plain(Matrix{hidden, M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);

@@ -292,11 +292,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   }, NoGil());
   m.def("gated_ffn_forward", [](const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act) {
     const FfnForward f = gated_ffn_forward(x, w_in, w_out, int(act), true);
-    return std::make_tuple(f.y, std::vector<Tensor>{f.x, f.w_in, f.w_out, f.hidden, f.gate_up});
+    return std::make_tuple(f.y, std::vector<Tensor>{f.x, f.w_in, f.w_out, f.saved});
   }, NoGil());
   m.def("gated_ffn_backward", [](const Tensor& dy, const Tensor& x, const Tensor& w_in, const Tensor& w_out,
-                                 const Tensor& hidden, const Tensor& gate_up, int64_t act, bool dx, bool dw_in, bool dw_out) {
-    const FfnGrads g = gated_ffn_backward(dy, x, w_in, w_out, hidden, gate_up, int(act), dx, dw_in, dw_out);
+                                 const Tensor& saved, int64_t act, bool dx, bool dw_in, bool dw_out) {
+    const FfnGrads g = gated_ffn_backward(dy, x, w_in, w_out, saved, int(act), dx, dw_in, dw_out);
     return std::make_tuple(g.dx, g.dw_in, g.dw_out);
   }, NoGil());
   m.def("gated_ffn_fp8", &gated_ffn_fp8, NoGil());

@@ -153,7 +153,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& w
 // ------------------------------------------------------------------ gated feed-forward block
 namespace {
 struct FfnSizes {
-  int64_t M, D, H, O, pitch;
+  int64_t M, D, H, O;
 };
 const uint16_t* bits(const Tensor& t) { return static_cast<const uint16_t*>(t.const_data_ptr()); }
 uint16_t* bits_mut(const Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
@@ -166,7 +166,7 @@ FfnSizes ffn_sizes(const Tensor& x, const Tensor& w_in, const Tensor& w_out) {
           "gated_ffn: w_in must be bfloat16 [in, 2 * hidden] on x's device");
   require(bf16_matrix(w_out, x.device()) && w_out.size(0) == w_in.size(1) / 2,
           "gated_ffn: w_out must be bfloat16 [hidden, out] on x's device");
-  return {x.size(0), x.size(1), w_out.size(0), w_out.size(1), abi.gc_gated_ffn_hidden_pitch(w_out.size(0))};
+  return {x.size(0), x.size(1), w_out.size(0), w_out.size(1)};
 }
 }  // namespace
 
@@ -179,22 +179,18 @@ FfnForward gated_ffn_forward(const Tensor& xin, const Tensor& w_in, const Tensor
   f.w_in = row_major(w_in);
   f.w_out = row_major(w_out);
   f.y = empty_like_rows(n.M, n.O, at::kBFloat16, dev);
-  if (save) {
-    f.hidden = empty_like_rows(n.M, n.pitch, at::kBFloat16, dev);
-    f.gate_up = empty_like_rows(n.M, 2 * n.pitch, at::kBFloat16, dev);
-  }
+  if (save)
+    f.saved = at::empty({int64_t(abi.gc_gated_ffn_saved_bytes(n.M, n.H))}, at::TensorOptions().dtype(at::kByte).device(dev));
   const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 0), dev);
   check(abi.gc_gated_ffn_forward_bf16(bits(f.x), ld_of(f.x), bits(f.w_in), ld_of(f.w_in), bits(f.w_out), ld_of(f.w_out),
                                       n.M, n.D, n.H, n.O, act, bits_mut(f.y), std::max<int64_t>(n.O, 1),
-                                      save ? bits_mut(f.hidden) : nullptr, save ? bits_mut(f.gate_up) : nullptr, ws.ptr,
-                                      ws.bytes, stream_of(dev)),
+                                      save ? f.saved.data_ptr() : nullptr, ws.ptr, ws.bytes, stream_of(dev)),
         "gc_gated_ffn_forward_bf16");
   return f;
 }
 
 FfnGrads gated_ffn_backward(const Tensor& dy_in, const Tensor& x, const Tensor& w_in, const Tensor& w_out,
-                            const Tensor& hidden, const Tensor& gate_up, int act, bool need_dx, bool need_dw_in,
-                            bool need_dw_out) {
+                            const Tensor& saved, int act, bool need_dx, bool need_dw_in, bool need_dw_out) {
   const FfnSizes n = ffn_sizes(x, w_in, w_out);
   const at::Device dev = x.device();
   const c10::cuda::CUDAGuard guard(dev);
@@ -205,8 +201,8 @@ FfnGrads gated_ffn_backward(const Tensor& dy_in, const Tensor& x, const Tensor& 
   if (need_dw_out) g.dw_out = empty_like_rows(n.H, n.O, at::kBFloat16, dev);
   const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 1), dev);
   check(abi.gc_gated_ffn_backward_bf16(
-            bits(dy), ld_of(dy), bits(x), ld_of(x), bits(w_in), ld_of(w_in), bits(w_out), ld_of(w_out), bits(hidden),
-            bits(gate_up), n.M, n.D, n.H, n.O, act, need_dx ? bits_mut(g.dx) : nullptr, std::max<int64_t>(n.D, 1),
+            bits(dy), ld_of(dy), bits(x), ld_of(x), bits(w_in), ld_of(w_in), bits(w_out), ld_of(w_out),
+            saved.const_data_ptr(), n.M, n.D, n.H, n.O, act, need_dx ? bits_mut(g.dx) : nullptr, std::max<int64_t>(n.D, 1),
             need_dw_in ? bits_mut(g.dw_in) : nullptr, std::max<int64_t>(2 * n.H, 1),
             need_dw_out ? bits_mut(g.dw_out) : nullptr, std::max<int64_t>(n.O, 1), ws.ptr, ws.bytes, stream_of(dev)),
         "gc_gated_ffn_backward_bf16");
@@ -217,7 +213,7 @@ namespace {
 struct FfnFunction : torch::autograd::Function<FfnFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act) {
     const FfnForward f = gated_ffn_forward(x, w_in, w_out, int(act), true);
-    ctx->save_for_backward({f.x, f.w_in, f.w_out, f.hidden, f.gate_up});
+    ctx->save_for_backward({f.x, f.w_in, f.w_out, f.saved});
     ctx->saved_data["act"] = act;
     return f.y;
   }
@@ -225,7 +221,7 @@ struct FfnFunction : torch::autograd::Function<FfnFunction> {
     once("gated_ffn");
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const FfnGrads g = gated_ffn_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4],
+    const FfnGrads g = gated_ffn_backward(grads[0], saved[0], saved[1], saved[2], saved[3],
                                           int(ctx->saved_data["act"].toInt()), ctx->needs_input_grad(0),
                                           ctx->needs_input_grad(1), ctx->needs_input_grad(2));
     return {g.dx, g.dw_in, g.dw_out, Tensor()};

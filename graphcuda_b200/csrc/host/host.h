@@ -47,7 +47,7 @@ inline bool f32_on(const Tensor& t, const at::Device& dev) {
   X(gc_edges_workspace_bytes) X(gc_edges_sort) X(gc_edges_to_csr) X(gc_degree_order_workspace_bytes)                \
   X(gc_degree_order) X(gc_relu_bias_backward_workspace_bytes) X(gc_relu_bias_backward_f32)                          \
   X(gc_rms_norm_forward) X(gc_rms_norm_backward_workspace_bytes) X(gc_rms_norm_backward) X(gc_adamw_step)           \
-  X(gc_adamw_moments_f32) X(gc_gated_ffn_hidden_pitch) X(gc_gated_ffn_workspace_bytes)                              \
+  X(gc_adamw_moments_f32) X(gc_gated_ffn_saved_bytes) X(gc_gated_ffn_workspace_bytes)                              \
   X(gc_gated_ffn_forward_bf16) X(gc_gated_ffn_backward_bf16) X(gc_gated_ffn_e4m3_workspace_bytes)                   \
   X(gc_gated_ffn_forward_e4m3)
 struct Abi {
@@ -206,16 +206,15 @@ std::pair<Tensor, Tensor> rms_norm(const Tensor& x, const Tensor& weight, const 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& residual,
                                                 double eps);
 struct FfnForward {
-  Tensor y, hidden, gate_up;  // the last two: for a backward pass
-  Tensor x, w_in, w_out;      // as the kernels took them
+  Tensor y, saved;        // saved: for a backward pass
+  Tensor x, w_in, w_out;  // as the kernels took them
 };
 FfnForward gated_ffn_forward(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int act, bool save);
 struct FfnGrads {
   Tensor dx, dw_in, dw_out;
 };
 FfnGrads gated_ffn_backward(const Tensor& dy, const Tensor& x, const Tensor& w_in, const Tensor& w_out,
-                            const Tensor& hidden, const Tensor& gate_up, int act, bool need_dx, bool need_dw_in,
-                            bool need_dw_out);
+                            const Tensor& saved, int act, bool need_dx, bool need_dw_in, bool need_dw_out);
 Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act);
 Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Tensor& w_out,
                      int64_t act);

@@ -491,24 +491,24 @@ int gc_rms_norm_backward(const void* dy, int dy_type, int64_t lddy, const void* 
  * two aggregations.  X is M x D, Win = [Wg | Wu] is D x 2H, Wout is H x O, all bf16 (bit patterns) with fp32 sums; the
  * activation's product is rounded to bf16 on its way into the second product.  Rows whose pitch is not a multiple of 16 bytes, and
  * an H that is not a multiple of 8, are copied to such in the workspace.
- * For a backward pass the forward call leaves `hidden` (M x P) and gate_up (M x 2P: X Wg, X Wu from column P on), P =
- * gc_gated_ffn_hidden_pitch(H), 16-byte aligned, pad columns zero; both may be null without one.
- * backward: with dA = dY Wo^T,  dX = [dA Wu-part act' | dA act] Win^T,  dWin = X^T [...],  dWout = hidden^T dY.
- * dX, dWin and dWout may be null (not computed).  Sums along K in a fixed order.
+ * saved: gc_gated_ffn_saved_bytes(M, H) bytes, 16-byte aligned, that the forward call fills for the backward call (6 M H
+ * bytes and a little: the activation's product, X Wg and X Wu); null where there will be none.
+ * backward, with G = X Wg, U = X Wu, dA = dY Wo^T:  [dG | dU] = [dA U act'(G) | dA act(G)],  dX = [dG | dU] Win^T,
+ * dWin = X^T [dG | dU],  dWout = (act(G) U)^T dY.  dX, dWin and dWout may be null (not computed).  Sums along K in a fixed order.
  * A wait that ran out is told by gc_gemm_error_word's word.
  */
 #define GC_ACT_SILU 0 /* g / (1 + exp(-g)) */
 #define GC_ACT_GELU 1 /* g (1 + erf(g / sqrt 2)) / 2 */
 #define GC_ACT_RELU 2
-int64_t gc_gated_ffn_hidden_pitch(int64_t H);
+size_t gc_gated_ffn_saved_bytes(int64_t M, int64_t H);
 size_t gc_gated_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O, int backward);
 int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin,
                               const uint16_t* Wout, int64_t ldwout, int64_t M, int64_t D, int64_t H, int64_t O, int act,
-                              uint16_t* Y, int64_t ldy, uint16_t* hidden, uint16_t* gate_up,
+                              uint16_t* Y, int64_t ldy, void* saved,
                               void* workspace, size_t workspace_bytes, void* stream);
 int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx,
                                const uint16_t* Win, int64_t ldwin, const uint16_t* Wout, int64_t ldwout,
-                               const uint16_t* hidden, const uint16_t* gate_up,
+                               const void* saved,
                                int64_t M, int64_t D, int64_t H, int64_t O, int act,
                                uint16_t* dX, int64_t lddx, uint16_t* dWin, int64_t lddwin,
                                uint16_t* dWout, int64_t lddwout, void* workspace, size_t workspace_bytes, void* stream);
