@@ -16,11 +16,17 @@
 // dWin: they are kept as fp16 numbers with an exponent for every 32 columns of a row, eight times as exact in as many bits.
 //
 // CTA = 20 warps, persistent over tiles of 128 x BN accumulators (or a pair of CTAs over 256 x BN):
-//   warp 0       TMA producer (one lane)
+//   warp 0       TMA producer of A (one lane)
 //   warp 1       MMA issuer (one lane)
 //   warp 2       TMEM allocator
-//   warps 4-19   epilogue: four warps per TMEM lane quarter, which take the 32-column chunks of a tile in turn; a
-//                chunk leaves through a swizzled 32 x 32 tile in shared memory and one TMA store
+//   warp 3       TMA producer of B (one lane)
+// The three single lanes share their schedulers with the epilogue, so an instruction takes them some eight clocks and a k-block only
+// 512: what they do per k-block and per tile is kept to a minimum (stages and coordinates are counted on, never divided;
+// one producer for both operands and divisions per tile left the tensor cores idle half of the time at K = 256).
+//   warps 4-19   epilogue: four warps per TMEM lane quarter, which take the 32-column chunks of a tile in turn; a chunk
+//                leaves through swizzled 32 x 32 tiles in shared memory and TMA stores.  (Two warps to a tile of 64
+//                columns, with a barrier between them: 265 us instead of 241 for A, G and U of 169,343 rows at K =
+//                256, H = 1024; half of the warps on every other tile: 259.)
 // Two accumulators in TMEM let the epilogue of a tile overlap the main loop of the next.  The epilogues are chains of
 // dependent loads and special functions: with 8 warps on chunks of 64 columns they, not memory or the tensor cores, set the
 // time of products with a short K.  Products with few tiles and a long K are split along K into fp32 parts that a second
@@ -45,21 +51,27 @@ using bf16 = __nv_bfloat16;
 constexpr int BM = 128;
 constexpr int kEpiWarps = 16, kEpiGroups = kEpiWarps / 4;
 constexpr int kThreads = 128 + 32 * kEpiWarps;
-constexpr int kTileBytes = 32 * 64;  // what a warp stores at once: 32 rows of 64 bytes
-constexpr int kBuffers = 2;          // of them per warp
+constexpr int kTileBytes = 32 * 64;  // what an epilogue warp stores at once: 32 rows of 64 bytes
+constexpr int kResident = 4;         // k-blocks of A that stay in shared memory, where that is all of K
 
 enum Kind { kPlain, kGated, kGatedBack };
 
-template <int BN, bool PAIR>
+// RES: A stays in shared memory while the CTA goes through all columns of its rows, and only B is loaded for every tile.
+template <int KIND, int BN, bool F8, bool PAIR, bool RES>
 struct Cfg {
   static constexpr int BNC = PAIR ? BN / 2 : BN;  // rows of B that a CTA holds
-  static constexpr int kABytes = BM * 128, kBBytes = BNC * 128;  // a stage has 128 bytes of K
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStaging = kEpiWarps * kBuffers * kTileBytes;
-  static constexpr int kStages = std::min(8, (227 * 1024 - 1024 - 512 - kStaging) / kStageBytes);
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStaging + 512 /*barriers*/ + 1024 /*alignment slack*/;
+  static constexpr int kABytes = BM * 128, kBBytes = BNC * 128;  // of a k-block: 128 bytes of K
+  static constexpr int kStageBytes = (RES ? 0 : kABytes) + kBBytes;
+  static constexpr int kHeldBytes = RES ? kResident * kABytes : 0;
+  // tiles in shared memory per epilogue warp: two, filled in turn; GatedBack works in place on a tile of G and one of U, and
+  // with a short K, where memory is the limit, on two pairs in turn
+  static constexpr int kTiles = KIND == kGatedBack && RES ? 4 : 2;
+  static constexpr int kScaleBytes = F8 ? kEpiWarps * 64 * 4 : 0;  // of a warp's columns of G and of U
+  static constexpr int kStaging = kEpiWarps * kTiles * kTileBytes + kScaleBytes;
+  static constexpr int kStages = std::min(8, (227 * 1024 - 1024 - 512 - kStaging - kHeldBytes) / kStageBytes);
+  static constexpr int kSmemBytes = kHeldBytes + kStages * kStageBytes + kStaging + 512 /*barriers*/ + 1024 /*alignment*/;
   static constexpr uint32_t kTmemCols = 2 * BN;
-  static_assert(kSmemBytes <= 227 * 1024 && kStages >= 3, "shared memory budget");
+  static_assert(kSmemBytes <= 227 * 1024 && kStages >= 2, "shared memory budget");
   static_assert(kTmemCols >= 32 && kTmemCols <= 512, "two accumulators in TMEM");
 };
 
@@ -126,6 +138,26 @@ template <int N>
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// Waits for a phase of a barrier, bounded.  The thread sleeps in the barrier unit between tries (a microsecond at most): twenty
+// warps that poll take issue slots from the lanes that feed the tensor cores, and power from all.  Returns false when the CTA is
+// aborting (this wait or another ran out).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_s) {
+  constexpr uint32_t kTries = 1u << 21;
+  for (uint32_t i = 0; i < kTries; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (*abort_s) return false;
+  }
+  *abort_s = 1;
+  return false;
+}
 // Waits for a copy in flight whatever else has failed (bounded): it must have landed before the CTA may exit.
 __device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < kWaitLimit; ++i) {
@@ -138,23 +170,72 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&t);
 }
-__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// 2^x and 1 / x to 2^-22, one instruction each; results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two floats at a time: the packed instructions do both in one issue slot.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ explicit F2(uint64_t x) : v(x) {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ F2(uint32_t a, uint32_t b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ F2 both(float x) { return F2(x, x); }
+template <class F>
+__device__ __forceinline__ F2 each(F2 a, F&& f) {
+  float x, y;
+  a.get(x, y);
+  return F2(f(x), f(y));
+}
+__device__ __forceinline__ uint32_t pack2(F2 a) {
+  float x, y;
+  a.get(x, y);
+  return pack2(x, y);
+}
 
 // act(g) and, for the backward pass, its derivative.
 template <int ACT>
-__device__ __forceinline__ float activate(float g, float& slope) {
+__device__ __forceinline__ F2 activate(F2 g, F2& slope) {
   if constexpr (ACT == GC_ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
-    slope = s + g * s * (1.f - s);
-    return g * s;
+    const F2 e = each(g * both(-1.4426950408889634f), [](float x) { return exp2_approx(x); });
+    const F2 s = each(e + both(1.f), [](float x) { return rcp_approx(x); });
+    const F2 a = g * s;
+    slope = fma2(a, fma2(s, both(-1.f), both(1.f)), s);
+    return a;
   } else if constexpr (ACT == GC_ACT_GELU) {
-    const float cdf = 0.5f + 0.5f * erff(g * 0.70710678118654752f);
-    slope = cdf + g * __expf(-0.5f * g * g) * 0.39894228040143268f;
+    const F2 cdf = fma2(each(g * both(0.70710678118654752f), [](float x) { return erff(x); }), both(0.5f), both(0.5f));
+    const F2 pdf = each(g * g * both(-0.72134752044448170f), [](float x) { return exp2_approx(x); });
+    slope = fma2(g * pdf, both(0.39894228040143268f), cdf);
     return g * cdf;
   } else {
-    slope = g > 0.f ? 1.f : 0.f;
-    return g <= 0.f ? 0.f : g;  // a NaN stays
+    slope = each(g, [](float x) { return x > 0.f ? 1.f : 0.f; });
+    return each(g, [](float x) { return x <= 0.f ? 0.f : x; });  // a NaN stays
   }
 }
 template <class F>
@@ -164,22 +245,51 @@ __device__ __forceinline__ void with_activation(int act, F&& f) {
   else f(std::integral_constant<int, GC_ACT_RELU>{});
 }
 
-// The 16-byte unit `j` of a row in a warp's swizzled tile.
-__device__ __forceinline__ uint4* unit(uint8_t* tile, int row, int j) {
-  return reinterpret_cast<uint4*>(tile + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+// A tile in shared memory: 32 rows of 64 bytes, their 16-byte units swizzled as TMA does it.  row_at is the address of unit
+// 0 of a row; unit j is where its bits 4 and 5 are XORed with j.
+__device__ __forceinline__ uint32_t row_at(uint32_t tile, int row) { return tile + row * 64 + (((row >> 1) & 3) << 4); }
+__device__ __forceinline__ void store_unit(uint32_t lane_at, int j, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(lane_at ^ (j << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 load_unit(uint32_t lane_at, int j) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(lane_at ^ (j << 4))
+               : "memory");
+  return v;
 }
 
-// 32 values to fp16 with a common power of two, which is returned: 0 unless the largest would overflow or fall below 2^-10,
-// where fp16 begins to lose bits; then it brings the largest to 2^14.
-__device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t (&out)[16]) {
-  __half2 top = __float2half2_rn(0.f);
+__device__ __forceinline__ uint16_t load_column(uint32_t tile, int row, int column) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"((row_at(tile, row) ^ (column / 8 << 4)) + column % 8 * 2) : "memory");
+  return v;
+}
+
+// Eight floats from shared memory, the same for all lanes.
+__device__ __forceinline__ void load_8(uint32_t at, F2 (&v)[4]) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-    top = __hmax2(top, __habs2(h));
-    out[j] = *reinterpret_cast<const uint32_t*>(&h);
+  for (int j = 0; j < 2; ++j)
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[2 * j].v), "=l"(v[2 * j + 1].v) : "r"(at + 16 * j) : "memory");
+}
+
+// 32 values to a row of a tile as fp16 with a common power of two, which is returned: 0 unless the largest would overflow or
+// fall below 2^-10, where fp16 begins to lose bits; then it brings the largest to 2^14.
+__device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t lane_at) {
+  __half2 top[2] = {__float2half2_rn(0.f), __float2half2_rn(0.f)};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __half2 h = __floats2half2_rn(__uint_as_float(v[j * 8 + 2 * e]), __uint_as_float(v[j * 8 + 2 * e + 1]));
+      top[e & 1] = __hmax2(top[e & 1], __habs2(h));
+      w[e] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    store_unit(lane_at, j, w[0], w[1], w[2], w[3]);
   }
-  const uint32_t t = *reinterpret_cast<const uint32_t*>(&top), most = max(t & 0xFFFFu, t >> 16);
+  top[0] = __hmax2(top[0], top[1]);
+  const uint32_t t = *reinterpret_cast<const uint32_t*>(&top[0]), most = max(t & 0xFFFFu, t >> 16);
   if (most >= 0x1400u && most < 0x7C00u) return 0;
   uint32_t bits = 0;
 #pragma unroll
@@ -189,15 +299,21 @@ __device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t (&out
   // two factors: 2^-e alone may not be a number
   const float a = __uint_as_float(uint32_t(127 - e / 2) << 23), b = __uint_as_float(uint32_t(127 - (e - e / 2)) << 23);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]) * a * b, __uint_as_float(v[2 * j + 1]) * a * b);
-    out[j] = *reinterpret_cast<const uint32_t*>(&h);
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = j * 8 + 2 * k;
+      const __half2 h = __floats2half2_rn(__uint_as_float(v[i]) * a * b, __uint_as_float(v[i + 1]) * a * b);
+      w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    store_unit(lane_at, j, w[0], w[1], w[2], w[3]);
   }
   return e;
 }
-__device__ __forceinline__ float2 unpack_fp16(uint32_t w, float scale) {
+__device__ __forceinline__ F2 unpack_fp16(uint32_t w, F2 scale) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return make_float2(f.x * scale, f.y * scale);
+  return F2(f.x, f.y) * scale;
 }
 
 // Where a column of the product goes (see Params); one that is dropped goes beyond the last.
@@ -214,33 +330,35 @@ struct Maps {
 };
 
 // A_MN / B_MN: the operand is MN-major.  F8: e4m3 operands (K-major).  PAIR: two CTAs of a cluster work on a tile of 256 rows,
-// each with its 128 rows of A and half of B's (Gated: rank 0 has G's columns, rank 1 U's).
-template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR>
+// each with its 128 rows of A and half of B's (Gated: rank 0 has G's columns, rank 1 U's).  RES: see Cfg.
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES>
 __global__ void __launch_bounds__(kThreads, 1)
 ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
-  using C_ = Cfg<BN, PAIR>;
+  using C_ = Cfg<KIND, BN, F8, PAIR, RES>;
   constexpr int S = C_::kStages, BNC = C_::BNC;
-  constexpr int KE = F8 ? 128 : 64;  // K elements per stage
+  constexpr int KE = F8 ? 128 : 64;  // K elements per k-block
   constexpr int TM = PAIR ? 2 * BM : BM;
   constexpr int NT = KIND == kGated ? BN / 2 : BN;  // output columns of a tile
   static_assert(!F8 || (!A_MN && !B_MN && KIND == kGated), "e4m3 operands are K-major");
+  static_assert(!RES || (!A_MN && KIND != kPlain), "A is held K-major, for short products");
   const uint32_t rank = PAIR ? cluster_rank() : 0;
-  const int first_item = PAIR ? int(blockIdx.x / 2) : int(blockIdx.x);
-  const int item_step = PAIR ? int(gridDim.x / 2) : int(gridDim.x);
+  const int unit = PAIR ? int(blockIdx.x / 2) : int(blockIdx.x), units = PAIR ? int(gridDim.x / 2) : int(gridDim.x);
   extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t base = (raw + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (base - raw);
-  auto sA = [&](int s) { return base + s * C_::kStageBytes; };
-  auto sB = [&](int s) { return base + s * C_::kStageBytes + C_::kABytes; };
-  constexpr int kStagingAt = S * C_::kStageBytes;
-  const uint32_t bars = base + kStagingAt + C_::kStaging;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  auto sHeld = [&](int kb) { return base + kb * C_::kABytes; };
+  auto sA = [&](int s) { return base + C_::kHeldBytes + s * C_::kStageBytes; };
+  auto sB = [&](int s) { return sA(s) + (RES ? 0 : C_::kABytes); };
+  const uint32_t staging = base + C_::kHeldBytes + S * C_::kStageBytes;
+  const uint32_t bars = staging + C_::kStaging;
   auto bar_full = [&](int s) { return bars + 8 * s; };
   auto bar_empty = [&](int s) { return bars + 8 * (S + s); };
   auto bar_tfull = [&](int b) { return bars + 8 * (2 * S + b); };
   auto bar_tempty = [&](int b) { return bars + 8 * (2 * S + 2 + b); };
-  auto bar_in = [&](int w) { return bars + 8 * (2 * S + 4 + w); };  // GatedBack: a warp's G and U have landed
-  static_assert(8 * (2 * S + 4 + kEpiWarps) <= 512, "room for the barriers");
+  auto bar_afull = [&](int kb) { return bars + 8 * (2 * S + 4 + kb); };  // RES: a k-block of A
+  auto bar_aempty = [&](int kb) { return bars + 8 * (2 * S + 4 + kResident + kb); };
+  auto bar_in = [&](int i) { return bars + 8 * (2 * S + 4 + 2 * kResident + i); };  // GatedBack: G and U have landed
+  constexpr int kPlaces = KIND == kGatedBack ? C_::kTiles / 2 : 1;  // for a tile of G and one of U, per warp
+  static_assert(8 * (2 * S + 4 + 2 * kResident + kPlaces * kEpiWarps) <= 512, "room for the barriers");
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
 
@@ -251,26 +369,46 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
   const int splits = KIND == kPlain ? p.splits : 1;
   const int kb_per = splits > 1 ? p.kb_per_split : nkb_total;
   const int num_items = tiles_m * tiles_n * splits;  // (split, m, n), n fastest
-  auto item_coords = [&](int item, int& m0, int& n0, int& kb0, int& kb1, int& split) {
-    const int t = item % (tiles_m * tiles_n);
-    split = item / (tiles_m * tiles_n);
-    m0 = (t / tiles_n) * TM + int(rank) * BM;  // first row of this CTA's half
-    n0 = (t % tiles_n) * NT;
-    kb0 = split * kb_per;
-    kb1 = min(nkb_total, kb0 + kb_per);
+  // This CTA's items: every units-th, or (RES) a run of them, so that A changes once per row of tiles.
+  const int first_item = RES ? int(int64_t(num_items) * unit / units) : unit;
+  const int my_tiles = RES ? int(int64_t(num_items) * (unit + 1) / units) - first_item
+                           : unit < num_items ? (num_items - unit + units - 1) / units : 0;
+  // Tile t = from, from + by, .. of this CTA, in coordinates that are divided once and counted on from there.
+  struct Tile {
+    int t, m, n, split, by, dm, dn, ds;
   };
+  auto tile_at = [&](int from, int by) {
+    const int item = first_item + from * (RES ? 1 : units), step = by * (RES ? 1 : units), i = item % (tiles_m * tiles_n),
+              j = step % (tiles_m * tiles_n);
+    return Tile{from, i / tiles_n, i % tiles_n, item / (tiles_m * tiles_n), by, j / tiles_n, j % tiles_n, step / (tiles_m * tiles_n)};
+  };
+  auto next = [&](Tile& x) {
+    x.t += x.by;
+    x.n += x.dn;
+    x.m += x.dm;
+    x.split += x.ds;
+    if (x.n >= tiles_n) x.n -= tiles_n, ++x.m;
+    if (x.m >= tiles_m) x.m -= tiles_m, ++x.split;
+  };
+  auto row_of = [&](const Tile& x) { return x.m * TM + int(rank) * BM; };  // first row of this CTA's half
+  auto first_kb = [&](const Tile& x) { return x.split * kb_per; };
+  auto last_kb = [&](const Tile& x) { return min(nkb_total, x.split * kb_per + kb_per); };
 
   if (threadIdx.x == 0) {
     abort_s = 0;
     for (int s = 0; s < S; ++s) {
-      mbar_init(bar_full(s), 1);
+      mbar_init(bar_full(s), RES ? 1 : 2);  // B's producer, and A's
       mbar_init(bar_empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar_tfull(b), 1);
       mbar_init(bar_tempty(b), kEpiWarps * (PAIR ? 2 : 1));
     }
-    for (int w = 0; w < kEpiWarps; ++w) mbar_init(bar_in(w), 1);
+    for (int kb = 0; kb < kResident; ++kb) {
+      mbar_init(bar_afull(kb), 1);
+      mbar_init(bar_aempty(kb), 1);
+    }
+    for (int i = 0; i < kPlaces * kEpiWarps; ++i) mbar_init(bar_in(i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
@@ -285,261 +423,329 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
   const uint32_t tmem_base = tmem_base_s;
   volatile int* abort_p = &abort_s;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int item = first_item; item < num_items && ok; item += item_step) {
-        int m0, n0, kb0, kb1, split;
-        item_coords(item, m0, n0, kb0, kb1, split);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(bar_empty(s), ((it / S) & 1u) ^ 1u, abort_p)) { ok = false; break; }
-          // a pair's copies are all counted at the leader
-          if (!PAIR) mbar_expect_tx(bar_full(s), C_::kStageBytes);
-          else if (rank == 0) mbar_expect_tx(bar_full(s), 2 * C_::kStageBytes);
-          auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
-            if (PAIR) tma_load_2d_leader(dst, map, x, y, bar_full(s));
-            else tma_load_2d(dst, map, x, y, bar_full(s));
-          };
-          if (A_MN) {
-#pragma unroll
-            for (int c = 0; c < BM / 64; ++c) load(sA(s) + c * (64 * 128), &maps.a, m0 + c * 64, kb * KE);
-          } else {
-            load(sA(s), &maps.a, kb * KE, m0);
-          }
-          // B's rows n of this CTA: Gated takes the tile's columns of G, then the same of U
-          auto load_b = [&](int at, int n, int rows) {
-            if (B_MN) {
-              for (int c = 0; c < rows / 64; ++c) load(sB(s) + (at + c * 64) * 128, &maps.b, n + c * 64, kb * KE);
-            } else {
-              load(sB(s) + at * 128, &maps.b, kb * KE, n);
-            }
-          };
-          if (KIND == kGated && PAIR) {
-            load_b(0, (rank ? p.b_up : 0) + n0, BNC);
-          } else if (KIND == kGated) {
-            load_b(0, n0, BN / 2);
-            load_b(BN / 2, p.b_up + n0, BN / 2);
-          } else {
-            load_b(0, n0 + int(rank) * BNC, BNC);
-          }
+  if ((warp == 0 || warp == 3) && lane == 0) {
+    // ------------------------------------------------------------ TMA producers: A, B
+    const bool is_a = warp == 0;
+    // a pair's copies are all counted at the leader
+    auto expect = [&](uint32_t bar, uint32_t bytes) {
+      if (!PAIR) mbar_expect_tx(bar, bytes);
+      else if (rank == 0) mbar_expect_tx(bar, 2 * bytes);
+    };
+    auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+      if (PAIR) tma_load_2d_leader(dst, map, x, y, bar);
+      else tma_load_2d(dst, map, x, y, bar);
+    };
+    bool ok = true;
+    if (RES && is_a) {
+      uint32_t rows = 0, held = 0;  // whole A's fetched; k-blocks of the one that is being fetched
+      for (Tile x = tile_at(0, 1); x.t < my_tiles && ok; next(x)) {
+        if (x.t > 0 && x.n > 0) continue;  // the A of the tile before
+        for (int kb = 0; kb < nkb_total; ++kb) {
+          if (!wait(bar_aempty(kb), (rows & 1u) ^ 1u, abort_p)) { ok = false; break; }
+          expect(bar_afull(kb), C_::kABytes);
+          load(sHeld(kb), &maps.a, kb * KE, row_of(x), bar_afull(kb));
+          ++held;
         }
+        if (ok) ++rows, held = 0;
       }
       // every copy issued must have landed before the CTA may exit (counted at the leader, for whom the peer waits)
-      const uint32_t pending = PAIR && rank != 0 ? 0u : it < uint32_t(S) ? it : uint32_t(S);
-      for (uint32_t j = 0; j < pending; ++j) {
-        const uint32_t q = it - 1 - j;
-        drain(bar_full(q % S), (q / S) & 1u);
+      for (uint32_t kb = 0; kb < uint32_t(nkb_total) && (!PAIR || rank == 0); ++kb) {
+        const uint32_t fetched = rows + (kb < held ? 1u : 0u);
+        if (fetched) drain(bar_afull(kb), (fetched - 1) & 1u);
       }
+    } else {
+      uint32_t s = 0, phase = 0, issued = 0;
+      for (Tile x = tile_at(0, 1); x.t < my_tiles && ok; next(x)) {
+        const int m0 = row_of(x), kb1 = last_kb(x);
+        // Gated takes the tile's columns of G, then the same of U
+        const int n0 = KIND == kGated ? x.n * NT + (PAIR && rank ? p.b_up : 0) : x.n * NT + int(rank) * BNC;
+        for (int kb = first_kb(x); kb < kb1; ++kb) {
+          if (!wait(bar_empty(s), phase ^ 1u, abort_p)) { ok = false; break; }
+          const uint32_t bar = bar_full(s);
+          if (is_a) {
+            expect(bar, C_::kABytes);
+            if (A_MN) {
+#pragma unroll
+              for (int c = 0; c < BM / 64; ++c) load(sA(s) + c * (64 * 128), &maps.a, m0 + c * 64, kb * KE, bar);
+            } else {
+              load(sA(s), &maps.a, kb * KE, m0, bar);
+            }
+          } else {
+            expect(bar, C_::kBBytes);
+            constexpr int kRows = KIND == kGated && !PAIR ? BNC / 2 : BNC;
+#pragma unroll
+            for (int part = 0; part < BNC / kRows; ++part) {
+              const int n = n0 + part * p.b_up;
+              const uint32_t dst = sB(s) + part * kRows * 128;
+              if (B_MN) {
+#pragma unroll
+                for (int c = 0; c < kRows / 64; ++c) load(dst + c * (64 * 128), &maps.b, n + c * 64, kb * KE, bar);
+              } else {
+                load(dst, &maps.b, kb * KE, n, bar);
+              }
+            }
+          }
+          ++issued;
+          if (++s == uint32_t(S)) s = 0, phase ^= 1u;
+        }
+      }
+      if (!PAIR || rank == 0)
+        for (uint32_t j = 0; j < issued && j < uint32_t(S); ++j) {  // as above
+          if (s == 0) phase ^= 1u;
+          s = s == 0 ? S - 1 : s - 1;
+          drain(bar_full(s), phase);
+        }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc = make_idesc(TM, BN, A_MN, B_MN, F8);
       constexpr uint32_t kAStep = A_MN ? 16 * 128 : 32, kBStep = B_MN ? 16 * 128 : 32;  // bytes per MMA
-      uint32_t it = 0, tcount = 0;
+      const uint64_t da0 = operand_desc(RES ? sHeld(0) : sA(0), A_MN), db0 = operand_desc(sB(0), B_MN);
+      uint32_t s = 0, phase = 0, rows = 0;
       bool ok = true;
-      for (int item = first_item; item < num_items && ok; item += item_step, ++tcount) {
-        int m0, n0, kb0, kb1, split;
-        item_coords(item, m0, n0, kb0, kb1, split);
-        const int b = tcount & 1;
-        if (!mbar_wait(bar_tempty(b), ((tcount >> 1) & 1u) ^ 1u, abort_p)) { ok = false; break; }
+      for (Tile x = tile_at(0, 1); x.t < my_tiles && ok;) {
+        const int b = x.t & 1, kb0 = first_kb(x), kb1 = last_kb(x);
+        const uint32_t turn = (x.t >> 1) & 1u;
+        const bool new_a = RES && (x.t == 0 || x.n == 0);
+        next(x);
+        const bool last_of_a = RES && (x.t >= my_tiles || x.n == 0);
+        if (!wait(bar_tempty(b), turn ^ 1u, abort_p)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + uint32_t(b * BN);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(bar_full(s), (it / S) & 1u, abort_p)) { ok = false; break; }
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (new_a && !wait(bar_afull(kb), rows & 1u, abort_p)) { ok = false; break; }
+          if (!wait(bar_full(s), phase, abort_p)) { ok = false; break; }
           tc_fence_after();
-          const uint64_t da = operand_desc(sA(s), A_MN), db = operand_desc(sB(s), B_MN);
+          const uint64_t da = da0 + (RES ? uint32_t(kb) * (C_::kABytes >> 4) : s * (C_::kStageBytes >> 4));
+          const uint64_t db = db0 + s * (C_::kStageBytes >> 4);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma<PAIR, F8>(d_tmem, da + ((k * kAStep) >> 4), db + ((k * kBStep) >> 4), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
           umma_commit<PAIR>(bar_empty(s));  // frees the stage once these MMAs have read it
+          if (last_of_a) umma_commit<PAIR>(bar_aempty(kb));
+          if (++s == uint32_t(S)) s = 0, phase ^= 1u;
         }
+        if (new_a) ++rows;
         if (ok) umma_commit<PAIR>(bar_tfull(b));
       }
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp % 4;          // TMEM lane quarter
+    const int q = warp % 4;  // TMEM lane quarter
     const int grp = (warp - 4) / 4;  // which of the 32-column chunks: grp, grp + 4, ..
-    uint8_t* tiles = smem + kStagingAt + (warp - 4) * (kBuffers * kTileBytes);
-    const uint32_t tiles_u = smem_u32(tiles);
-    int buf = 0;
+    const uint32_t tiles = staging + (warp - 4) * (C_::kTiles * kTileBytes);
+    const uint32_t lane_at = row_at(tiles, lane);
+    const int64_t exps_u = int64_t((p.N + 31) / 32) * p.M;  // from G's table of exponents to U's
+    uint32_t buf = 0;  // byte offset of the tile that was filled last
+    bool ok = true;
+    // The same answer for all of a warp.
+    auto wait_warp = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity, abort_p)) != 0; };
     // The next of the warp's tiles, once the store that read it last has done so.
     auto acquire = [&]() {
-      if (lane == 0) store_wait_read<kBuffers - 1>();
+      if (lane == 0) store_wait_read<1>();
       __syncwarp();
-      const int b = buf;
-      buf = (buf + 1) % kBuffers;
-      return b;
+      buf ^= kTileBytes;
+      return buf;
     };
-    // Hands a tile to the TMA store.
-    auto put = [&](const CUtensorMap* map, int b, int x, int y) {
+    // Hands a filled tile to the TMA store.
+    auto put = [&](const CUtensorMap* map, uint32_t at, int col, int row) {
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
-        tma_store_2d(map, tiles_u + b * kTileBytes, x, y);
+        tma_store_2d(map, tiles + at, col, row);
         store_commit();
       }
     };
-    auto put_words = [&](const CUtensorMap* map, const uint32_t (&w)[16], int x, int y) {
-      const int b = acquire();
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *unit(tiles + b * kTileBytes, lane, j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-      put(map, b, x, y);
+
+    // GatedBack: the warp's chunks in their order, and the copies of G and U for them.
+    Tile ahead = tile_at(0, 1);
+    int ahead_c = grp;
+    auto find_chunk = [&]() {  // the next that exists, from there on
+      for (; ahead.t < my_tiles; next(ahead), ahead_c = grp)
+        if (row_of(ahead) + q * 32 < p.M && ahead_c < NT / 32 && ahead.n * NT + ahead_c * 32 < p.N) return true;
+      return false;
     };
-    uint32_t tcount = 0, loads = 0;
-    bool ok = true;
-    for (int item = first_item; item < num_items && ok; item += item_step, ++tcount) {
-      int m0, n0, kb0, kb1, split;
-      item_coords(item, m0, n0, kb0, kb1, split);
-      const int b = tcount & 1;
-      const int row0 = m0 + q * 32, row = row0 + lane;  // the warp's first row, the lane's
-      const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * BN);
-      const int chunks_m = (p.N + 31) / 32;  // Gated, GatedBack: rows of a table of exponents
-      // GatedBack: G and U of a chunk; those of the first are on their way while the tile is being computed
-      bool have_in = false;
-      auto request = [&](int col) {
-        if (lane == 0) {
-          store_wait_read<0>();
-          mbar_expect_tx(bar_in(warp - 4), 2 * kTileBytes);
-          tma_load_2d(tiles_u, &maps.in1, col, row0, bar_in(warp - 4));
-          tma_load_2d(tiles_u + kTileBytes, &maps.in2, col, row0, bar_in(warp - 4));
-        }
-      };
-      if (KIND == kGatedBack && n0 + grp * 32 < p.N && row0 < p.M) {
-        request(n0 + grp * 32);
-        have_in = true;
+    uint32_t asked = 0, used = 0;  // copies
+    auto request = [&]() {
+      if (lane == 0) {
+        const int col = ahead.n * NT + ahead_c * 32, row = row_of(ahead) + q * 32;
+        const uint32_t at = asked % kPlaces, bar = bar_in((warp - 4) * kPlaces + at), dst = tiles + at * 2 * kTileBytes;
+        store_wait_read<0>();  // what was put from these tiles has left them
+        mbar_expect_tx(bar, 2 * kTileBytes);
+        tma_load_2d(dst, &maps.in1, col, row, bar);
+        tma_load_2d(dst + kTileBytes, &maps.in2, col, row, bar);
       }
-      if (!mbar_wait(bar_tfull(b), (tcount >> 1) & 1u, abort_p)) ok = false;
-      if (ok) tc_fence_after();
-      for (int c = grp; c < NT / 32 && (ok || have_in); c += kEpiGroups) {
+      ++asked;
+      ahead_c += kEpiGroups;
+    };
+    if (KIND == kGatedBack && find_chunk()) request();
+
+    for (Tile x = tile_at(0, 1); x.t < my_tiles && ok; next(x)) {
+      const int b = x.t & 1, n0 = x.n * NT;
+      const int row0 = row_of(x) + q * 32, row = row0 + lane;  // the warp's first row, the lane's
+      const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * BN);
+      if (!wait_warp(bar_tfull(b), (x.t >> 1) & 1u)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // Gives the accumulator back as soon as the warp's last chunk is in registers.
+      bool held = true;
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_leader(bar_tempty(b));
+          else mbar_arrive(bar_tempty(b));
+        }
+        held = false;
+      };
+      auto loaded = [&](int c) {
+        tmem_ld_wait();
+        if (c + kEpiGroups >= NT / 32 || n0 + (c + kEpiGroups) * 32 >= p.N) release();
+      };
+      for (int c = grp; c < NT / 32; c += kEpiGroups) {
         const int col = n0 + c * 32;
         if (col >= p.N || row0 >= p.M) break;
+        const uint32_t acc_at = taddr + uint32_t(c * 32);
         if constexpr (KIND == kGatedBack) {
-          if (!have_in) request(col);
-          have_in = false;
+          // the next chunk's copies go out before this one is worked on, where there are tiles for them
+          if (kPlaces > 1 && find_chunk()) request();
           const int64_t at = int64_t(col / 32) * p.M + min(row, p.M - 1);
           const float sg = __uint_as_float(uint32_t(127 + p.exps[at]) << 23);
-          const float su = __uint_as_float(uint32_t(127 + p.exps[at + int64_t(chunks_m) * p.M]) << 23);
+          const float su = __uint_as_float(uint32_t(127 + p.exps[at + exps_u]) << 23);
+          const uint32_t place = used % kPlaces, at_g = lane_at + place * 2 * kTileBytes, at_u = at_g + kTileBytes;
           uint32_t acc[32];
-          if (ok) tmem_ld32(taddr + uint32_t(c * 32), acc);
-          if (!mbar_wait(bar_in(warp - 4), loads & 1u, abort_p)) {
-            drain(bar_in(warp - 4), loads & 1u);
+          tmem_ld32(acc_at, acc);
+          if (!wait_warp(bar_in((warp - 4) * kPlaces + place), (used / kPlaces) & 1u)) {
             ok = false;
+            break;
           }
-          ++loads;
-          if (!ok) break;
-          tmem_ld_wait();
+          ++used;
+          loaded(c);
           with_activation(p.act, [&](auto act) {
+            const F2 fg = both(sg), fu = both(su);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              uint4* gp = unit(tiles, lane, j);
-              uint4* up = unit(tiles + kTileBytes, lane, j);
-              uint4 g4 = *gp, u4 = *up;
+              uint4 g4 = load_unit(at_g, j), u4 = load_unit(at_u, j);
               uint32_t* gw = &g4.x;
               uint32_t* uw = &u4.x;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float d0 = __uint_as_float(acc[j * 8 + 2 * e]), d1 = __uint_as_float(acc[j * 8 + 2 * e + 1]);
-                const float2 g = unpack_fp16(gw[e], sg), u = unpack_fp16(uw[e], su);
-                float s0, s1;
-                const float a0 = activate<decltype(act)::value>(g.x, s0);
-                const float a1 = activate<decltype(act)::value>(g.y, s1);
-                gw[e] = pack2(d0 * u.x * s0, d1 * u.y * s1);
-                uw[e] = pack2(d0 * a0, d1 * a1);
+                const F2 d(acc[j * 8 + 2 * e], acc[j * 8 + 2 * e + 1]);
+                const F2 u = unpack_fp16(uw[e], fu);
+                F2 slope;
+                const F2 a = activate<decltype(act)::value>(unpack_fp16(gw[e], fg), slope);
+                gw[e] = pack2(d * u * slope);
+                uw[e] = pack2(d * a);
               }
-              *gp = g4;
-              *up = u4;
+              store_unit(at_g, j, g4.x, g4.y, g4.z, g4.w);
+              store_unit(at_u, j, u4.x, u4.y, u4.z, u4.w);
             }
           });
-          put(&maps.out, 0, col, row0);
-          put(&maps.out2, 1, col, row0);
-        } else if constexpr (KIND == kGated) {
-          uint32_t g[32], u[32], w[16];
-          tmem_ld32(taddr + uint32_t(c * 32), g);
-          tmem_ld32(taddr + uint32_t(NT + c * 32), u);
-          tmem_ld_wait();
-          if (F8) {
-            const float sa = p.sa[min(row, p.M - 1)];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int n = min(col + j, p.N - 1);
-              g[j] = __float_as_uint(__uint_as_float(g[j]) * (sa * __ldg(p.sb + n)));
-              u[j] = __float_as_uint(__uint_as_float(u[j]) * (sa * __ldg(p.sb + p.b_up + n)));
-            }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&maps.out, tiles + place * 2 * kTileBytes, col, row0);
+            tma_store_2d(&maps.out2, tiles + place * 2 * kTileBytes + kTileBytes, col, row0);
+            store_commit();
           }
+          if (kPlaces == 1 && find_chunk()) request();
+        } else if constexpr (KIND == kGated) {
+          const float sa = F8 ? p.sa[min(row, p.M - 1)] : 1.f;
+          const uint32_t scales = staging + C_::kStaging - C_::kScaleBytes + (warp - 4) * 256;
+          if (F8) {
+            const int n = min(col + lane, p.N - 1);
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + 4 * lane), "f"(__ldg(p.sb + n)) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + 128 + 4 * lane), "f"(__ldg(p.sb + p.b_up + n)) : "memory");
+          }
+          uint32_t g[32], u[32];
+          tmem_ld32(acc_at, g);
+          tmem_ld32(acc_at + uint32_t(NT), u);
+          loaded(c);
           if (!F8 && p.exps) {
             const int64_t at = int64_t(col / 32) * p.M + row;
-            const int eg = pack_fp16(g, w);
-            if (row < p.M) p.exps[at] = int8_t(eg);
-            put_words(&maps.out2, w, col, row0);
-            const int eu = pack_fp16(u, w);
-            if (row < p.M) p.exps[at + int64_t(chunks_m) * p.M] = int8_t(eu);
-            put_words(&maps.out3, w, col, row0);
+            const uint32_t bg = acquire();
+            const int eg = pack_fp16(g, lane_at + bg);
+            put(&maps.out2, bg, col, row0);
+            const uint32_t bu = acquire();
+            const int eu = pack_fp16(u, lane_at + bu);
+            put(&maps.out3, bu, col, row0);
+            if (row < p.M) {
+              p.exps[at] = int8_t(eg);
+              p.exps[at + exps_u] = int8_t(eu);
+            }
           }
+          const uint32_t bo = acquire();
+          if (F8) __syncwarp();  // the scales are written
           with_activation(p.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float unused;
-              w[j] = pack2(activate<decltype(act)::value>(__uint_as_float(g[2 * j]), unused) * __uint_as_float(u[2 * j]),
-                           activate<decltype(act)::value>(__uint_as_float(g[2 * j + 1]), unused) * __uint_as_float(u[2 * j + 1]));
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+              F2 sg[4], su[4];
+              if (F8) {
+                load_8(scales + 32 * j, sg);
+                load_8(scales + 128 + 32 * j, su);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int i = j * 8 + 2 * e;
+                F2 vg(g[i], g[i + 1]), vu(u[i], u[i + 1]), unused;
+                if (F8) vg = vg * (both(sa) * sg[e]), vu = vu * (both(sa) * su[e]);
+                w[e] = pack2(activate<decltype(act)::value>(vg, unused) * vu);
+              }
+              store_unit(lane_at + bo, j, w[0], w[1], w[2], w[3]);
             }
           });
-          put_words(&maps.out, w, col, row0);
-        } else if (splits > 1) {
-          // fp32 parts, 16 columns to a tile
+          put(&maps.out, bo, col, row0);
+        } else {
           uint32_t acc[32];
-          tmem_ld32(taddr + uint32_t(c * 32), acc);
-          tmem_ld_wait();
+          tmem_ld32(acc_at, acc);
+          loaded(c);
+          if (splits > 1) {
+            // fp32 parts, 16 columns to a tile
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int bo = acquire();
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t bo = acquire();
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int i = half * 16 + 4 * j;
+                store_unit(lane_at + bo, j, acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+              }
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (col + half * 16 < p.N) tma_store_3d(&maps.out, tiles + bo, col + half * 16, row0, x.split);
+                store_commit();
+              }
+            }
+          } else {
+            const uint32_t bo = acquire();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int i = half * 16 + 4 * j;
-              *unit(tiles + bo * kTileBytes, lane, j) = make_uint4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (col + half * 16 < p.N) tma_store_3d(&maps.out, tiles_u + bo * kTileBytes, col + half * 16, row0, split);
-              store_commit();
-            }
-          }
-        } else {
-          uint32_t acc[32], w[16];
-          tmem_ld32(taddr + uint32_t(c * 32), acc);
-          tmem_ld_wait();
+              uint32_t w[4];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = pack2(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
-          if (p.tma_store) {
-            put_words(&maps.out, w, col, row0);
-          } else {
-            // rows of an odd pitch: a row at a time, a column per lane
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) *unit(tiles, lane, j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-            __syncwarp();
-            const int n = out_column(col + lane, p.gap_from, p.gap), rows = min(32, p.M - row0);
-            if (n < p.c_cols)
-              for (int r = 0; r < rows; ++r)
-                p.C[int64_t(row0 + r) * p.ldc + n] =
-                    reinterpret_cast<const bf16*>(unit(tiles, r, lane / 8))[lane % 8];
+              for (int e = 0; e < 4; ++e) w[e] = pack2(F2(acc[j * 8 + 2 * e], acc[j * 8 + 2 * e + 1]));
+              store_unit(lane_at + bo, j, w[0], w[1], w[2], w[3]);
+            }
+            if (p.tma_store) {
+              put(&maps.out, bo, col, row0);
+            } else {
+              // rows of an odd pitch: a row at a time, a column per lane
+              __syncwarp();
+              const int n = out_column(col + lane, p.gap_from, p.gap), rows = min(32, p.M - row0);
+              if (n < p.c_cols)
+                for (int r = 0; r < rows; ++r)
+                  p.C[int64_t(row0 + r) * p.ldc + n] = __ushort_as_bfloat16(load_column(tiles + bo, r, lane));
+            }
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (PAIR) mbar_arrive_leader(bar_tempty(b));
-        else mbar_arrive(bar_tempty(b));
-      }
+      if (held) release();
     }
+    if (KIND == kGatedBack && lane == 0)  // copies that were asked for and not waited for have to land all the same
+      for (; used != asked; ++used) drain(bar_in((warp - 4) * kPlaces + used % kPlaces), (used / kPlaces) & 1u);
     if (lane == 0) store_wait_all();  // shared memory is read until then
   }
 
@@ -599,7 +805,7 @@ struct Matrix {  // row-major, `size` bytes per element
   int size;
 };
 
-// Boxes of 128 bytes x box_rows are operands; the epilogues' are of 64 bytes.
+// Boxes with rows of 128 bytes are operands; the epilogues' have 64.
 int make_map(CUtensorMap* map, const Matrix& m, int box_cols, int box_rows, int64_t planes = 0) {
   EncodeFn enc = get_encode();
   if (!enc) return gc::fail(GC_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
@@ -675,10 +881,10 @@ int error_word(int** word) {
   return GC_OK;
 }
 
-template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR>
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES>
 int launch_kernel(const Maps& maps, const Params& p, cudaStream_t st) {
-  using C_ = Cfg<BN, PAIR>;
-  auto kern = ffn_kernel<KIND, BN, A_MN, B_MN, F8, PAIR>;
+  using C_ = Cfg<KIND, BN, F8, PAIR, RES>;
+  auto kern = ffn_kernel<KIND, BN, A_MN, B_MN, F8, PAIR, RES>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::kSmemBytes);
   if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   constexpr int kCtas = PAIR ? 2 : 1;
@@ -702,10 +908,13 @@ int launch_kernel(const Maps& maps, const Params& p, cudaStream_t st) {
 }
 template <int KIND, bool A_MN, bool B_MN, bool F8>
 int launch_tile(const Tile& t, const Maps& maps, const Params& p, cudaStream_t st) {
-  if (t.pair) return launch_kernel<KIND, 256, A_MN, B_MN, F8, true>(maps, p, st);
+  if constexpr (KIND != kPlain)
+    if (t.pair && gc::ceil_div(p.K, F8 ? 128 : 64) <= kResident)
+      return launch_kernel<KIND, 256, A_MN, B_MN, F8, true, true>(maps, p, st);
+  if (t.pair) return launch_kernel<KIND, 256, A_MN, B_MN, F8, true, false>(maps, p, st);
   if constexpr (KIND != kGated)
-    if (t.bn == 64) return launch_kernel<KIND, 64, A_MN, B_MN, F8, false>(maps, p, st);
-  return launch_kernel<KIND, 128, A_MN, B_MN, F8, false>(maps, p, st);
+    if (t.bn == 64) return launch_kernel<KIND, 64, A_MN, B_MN, F8, false, false>(maps, p, st);
+  return launch_kernel<KIND, 128, A_MN, B_MN, F8, false, false>(maps, p, st);
 }
 
 // The maps of the operands.  A and B: matrices as they lie; K-major ones have K in their rows.
