@@ -38,7 +38,7 @@ SOURCES = [
     "gcn_layer.cu",
     "graph_build.cu",
     "loss.cu", "optim.cu",
-    "norm.cu", "adamw.cu", "ffn.cu",
+    "norm.cu", "adamw.cu", "ffn.cu", "ffn_rows.cu",
 ]
 
 HOSTSRC = os.path.join(CSRC, "host")

@@ -35,6 +35,7 @@
 // Every wait on a barrier is bounded, as in the other tensor-core kernel: a wait that ran out raises the device's error
 // word, all roles leave, copies in flight are drained and TMEM is released.
 #include "common.cuh"
+#include "ffn_internal.cuh"
 #include "gemm_internal.cuh"
 #include "tcgen05.cuh"
 
@@ -46,6 +47,7 @@
 namespace {
 
 using namespace gc::tc;
+using namespace gc::ffn;
 using bf16 = __nv_bfloat16;
 
 constexpr int BM = 128;
@@ -77,6 +79,7 @@ struct Cfg {
 
 struct Params {
   int M, N, K;  // of the product; Gated: N = H, the columns of G and of U
+  int a_bytes;  // of a k-block of A that are loaded: fewer than a tile's where M is below its rows
   int b_up;     // Gated: where U's columns start in B
   int act;
   int8_t* exps;     // G's and U's exponents, [2][ceil(N / 32)][M] (Gated: null where G and U are not stored)
@@ -171,78 +174,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&t);
 }
 
-// 2^x and 1 / x to 2^-22, one instruction each; results below 2^-126 are zero.
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// Two floats at a time: the packed instructions do both in one issue slot.
-struct F2 {
-  uint64_t v;
-  __device__ __forceinline__ F2() {}
-  __device__ __forceinline__ explicit F2(uint64_t x) : v(x) {}
-  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ F2(uint32_t a, uint32_t b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(a), "r"(b)); }
-  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
-  F2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
-  F2 d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
-__device__ __forceinline__ F2 both(float x) { return F2(x, x); }
-template <class F>
-__device__ __forceinline__ F2 each(F2 a, F&& f) {
-  float x, y;
-  a.get(x, y);
-  return F2(f(x), f(y));
-}
 __device__ __forceinline__ uint32_t pack2(F2 a) {
   float x, y;
   a.get(x, y);
   return pack2(x, y);
-}
-
-// act(g) and, for the backward pass, its derivative.
-template <int ACT>
-__device__ __forceinline__ F2 activate(F2 g, F2& slope) {
-  if constexpr (ACT == GC_ACT_SILU) {
-    const F2 e = each(g * both(-1.4426950408889634f), [](float x) { return exp2_approx(x); });
-    const F2 s = each(e + both(1.f), [](float x) { return rcp_approx(x); });
-    const F2 a = g * s;
-    slope = fma2(a, fma2(s, both(-1.f), both(1.f)), s);
-    return a;
-  } else if constexpr (ACT == GC_ACT_GELU) {
-    const F2 cdf = fma2(each(g * both(0.70710678118654752f), [](float x) { return erff(x); }), both(0.5f), both(0.5f));
-    const F2 pdf = each(g * g * both(-0.72134752044448170f), [](float x) { return exp2_approx(x); });
-    slope = fma2(g * pdf, both(0.39894228040143268f), cdf);
-    return g * cdf;
-  } else {
-    slope = each(g, [](float x) { return x > 0.f ? 1.f : 0.f; });
-    return each(g, [](float x) { return x <= 0.f ? 0.f : x; });  // a NaN stays
-  }
-}
-template <class F>
-__device__ __forceinline__ void with_activation(int act, F&& f) {
-  if (act == GC_ACT_SILU) f(std::integral_constant<int, GC_ACT_SILU>{});
-  else if (act == GC_ACT_GELU) f(std::integral_constant<int, GC_ACT_GELU>{});
-  else f(std::integral_constant<int, GC_ACT_RELU>{});
 }
 
 // A tile in shared memory: 32 rows of 64 bytes, their 16-byte units swizzled as TMA does it.  row_at is the address of unit
@@ -273,8 +208,7 @@ __device__ __forceinline__ void load_8(uint32_t at, F2 (&v)[4]) {
     asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[2 * j].v), "=l"(v[2 * j + 1].v) : "r"(at + 16 * j) : "memory");
 }
 
-// 32 values to a row of a tile as fp16 with a common power of two, which is returned: 0 unless the largest would overflow or
-// fall below 2^-10, where fp16 begins to lose bits; then it brings the largest to 2^14.
+// 32 values to a row of a tile as fp16 with a common power of two, which is returned.
 __device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t lane_at) {
   __half2 top[2] = {__float2half2_rn(0.f), __float2half2_rn(0.f)};
 #pragma unroll
@@ -290,21 +224,19 @@ __device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t lane_
   }
   top[0] = __hmax2(top[0], top[1]);
   const uint32_t t = *reinterpret_cast<const uint32_t*>(&top[0]), most = max(t & 0xFFFFu, t >> 16);
-  if (most >= 0x1400u && most < 0x7C00u) return 0;
+  if (fits_fp16(most)) return 0;
   uint32_t bits = 0;
 #pragma unroll
   for (int j = 0; j < 32; ++j) bits = max(bits, v[j] & 0x7FFFFFFFu);
-  if (bits == 0 || bits >= 0x7F800000u) return 0;  // zeros; an infinity or a NaN, with which the row is lost
-  const int e = max(int(bits >> 23) - 127 - 14, -126);
-  // two factors: 2^-e alone may not be a number
-  const float a = __uint_as_float(uint32_t(127 - e / 2) << 23), b = __uint_as_float(uint32_t(127 - (e - e / 2)) << 23);
+  const int e = shared_exponent(bits);
+  const float2 f = unscale(e);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     uint32_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = j * 8 + 2 * k;
-      const __half2 h = __floats2half2_rn(__uint_as_float(v[i]) * a * b, __uint_as_float(v[i + 1]) * a * b);
+      const __half2 h = __floats2half2_rn(__uint_as_float(v[i]) * f.x * f.y, __uint_as_float(v[i + 1]) * f.x * f.y);
       w[k] = *reinterpret_cast<const uint32_t*>(&h);
     }
     store_unit(lane_at, j, w[0], w[1], w[2], w[3]);
@@ -463,7 +395,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           if (!wait(bar_empty(s), phase ^ 1u, abort_p)) { ok = false; break; }
           const uint32_t bar = bar_full(s);
           if (is_a) {
-            expect(bar, C_::kABytes);
+            expect(bar, p.a_bytes);
             if (A_MN) {
 #pragma unroll
               for (int c = 0; c < BM / 64; ++c) load(sA(s) + c * (64 * 128), &maps.a, m0 + c * 64, kb * KE, bar);
@@ -918,9 +850,13 @@ int launch_tile(const Tile& t, const Maps& maps, const Params& p, cudaStream_t s
 }
 
 // The maps of the operands.  A and B: matrices as they lie; K-major ones have K in their rows.
-int operand_maps(Maps& maps, const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int b_rows) {
+int operand_maps(Maps& maps, Params& p, const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int b_rows) {
   const int ke = 128 / A.size;  // K elements of a stage
-  int rc = a_mn ? make_map(&maps.a, A, 64, 64) : make_map(&maps.a, A, ke, BM);
+  // Of a tile that M does not fill only the rows that exist are loaded: the TMA unit takes as long for a row of zeros, and
+  // what the others hold stays in accumulators that nobody reads.
+  const int rows = int(std::min<int64_t>(BM, (A.rows + 7) / 8 * 8));
+  p.a_bytes = (a_mn ? BM : rows) * 128;
+  int rc = a_mn ? make_map(&maps.a, A, 64, 64) : make_map(&maps.a, A, ke, rows);
   if (rc == GC_OK) rc = b_mn ? make_map(&maps.b, B, 64, 64) : make_map(&maps.b, B, ke, b_rows);
   return rc;
 }
@@ -940,7 +876,7 @@ int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int
   p.splits = s.splits; p.kb_per_split = s.per;
   p.tma_store = gap == 0 && ldc % 8 == 0 && gc::aligned16(C);
   int rc = error_word(&p.word);
-  if (rc == GC_OK) rc = operand_maps(maps, A, a_mn, B, b_mn, s.tile.pair ? s.tile.bn / 2 : s.tile.bn);
+  if (rc == GC_OK) rc = operand_maps(maps, p, A, a_mn, B, b_mn, s.tile.pair ? s.tile.bn / 2 : s.tile.bn);
   const int64_t pitch = part_pitch(N);
   if (rc == GC_OK && s.splits > 1) rc = make_map(&maps.out, Matrix{workspace, M, N, pitch, 4}, 16, 32, s.splits);
   else if (rc == GC_OK && p.tma_store) rc = make_map(&maps.out, Matrix{C, M, N, ldc, 2}, 32, 32);
@@ -993,12 +929,6 @@ int make_gate_up(Matrix& w, int64_t H, char*& ws, cudaStream_t st) {
   return rc;
 }
 
-// What a forward pass leaves for the backward pass, in one buffer.
-struct Saved {
-  uint16_t* hidden;   // M x P, P = up8(H)
-  uint16_t* gate_up;  // M x 2P: G and U as fp16 numbers
-  int8_t* exps;       // and their exponents
-};
 Saved saved_at(void* p, int64_t M, int64_t H) {
   const int64_t hp = up8(H);
   char* c = static_cast<char*>(p);
@@ -1008,6 +938,13 @@ Saved saved_at(void* p, int64_t M, int64_t H) {
   s.gate_up = reinterpret_cast<uint16_t*>(c);
   s.exps = reinterpret_cast<int8_t*>(c + align256(size_t(M) * hp * 4));
   return s;
+}
+
+// Whether a forward pass takes the form for few rows.  Measured against this file's, us: weights of 100 MB 27 / 38 at one row
+// (both from memory), 30 / 29 at two, 34 / 29 at four; of 1.5 MB 7 / 13 at one, 10 / 13 at eight; of 4 MB at odd widths, which
+// this file's would copy first, 13 / 29 at one, 17 / 29 at eight.
+bool few_rows(int64_t M, int64_t D, int64_t H, int64_t O, bool in_place) {
+  return M == 1 || (M <= kFewRows && (!in_place || 2 * (2 * D * H + H * O) <= (int64_t(16) << 20)));
 }
 
 bool sizes_ok(int64_t M, int64_t D, int64_t H, int64_t O) {
@@ -1058,6 +995,12 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_bf16: workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Matrix x{X, M, D, ldx, 2}, win{Win, D, 2 * H, ldwin, 2}, wout{Wout, H, O, ldwout, 2};
+  if (few_rows(M, D, H, O, readable(win) && H % 8 == 0 && readable(wout))) {
+    const Saved keep = saved ? saved_at(saved, M, H) : Saved{};
+    const Rows r{X, Win, Wout, nullptr, nullptr, saved ? keep.hidden : reinterpret_cast<uint16_t*>(ws), Y, ldx, ldwin, ldwout,
+                 hp, ldy, int(M), int(D), int(H), int(O), act, keep};
+    return forward_few_rows(r, false, st);
+  }
   int rc = make_readable(x, ws, st);
   if (rc == GC_OK) rc = make_gate_up(win, H, ws, st);
   if (rc == GC_OK) rc = make_readable(wout, ws, st);
@@ -1078,7 +1021,7 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   p.act = act;
   p.exps = keep.exps;
   rc = error_word(&p.word);
-  if (rc == GC_OK) rc = operand_maps(maps, x, false, win, true, 0);
+  if (rc == GC_OK) rc = operand_maps(maps, p, x, false, win, true, 0);
   if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, hp, hp, 2}, 32, 32);
   if (rc == GC_OK && saved) rc = make_map(&maps.out2, Matrix{keep.gate_up, M, hp, 2 * hp, 2}, 32, 32);
   if (rc == GC_OK && saved) rc = make_map(&maps.out3, Matrix{keep.gate_up + hp, M, hp, 2 * hp, 2}, 32, 32);
@@ -1135,7 +1078,7 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
     p.act = act;
     p.exps = kept.exps;
     rc = error_word(&p.word);
-    if (rc == GC_OK) rc = operand_maps(maps, dy, false, wout, false, t.pair ? t.bn / 2 : t.bn);
+    if (rc == GC_OK) rc = operand_maps(maps, p, dy, false, wout, false, t.pair ? t.bn / 2 : t.bn);
     if (rc == GC_OK) rc = make_map(&maps.in1, Matrix{kept.gate_up, M, hp, 2 * hp, 2}, 32, 32);
     if (rc == GC_OK) rc = make_map(&maps.in2, Matrix{kept.gate_up + hp, M, hp, 2 * hp, 2}, 32, 32);
     if (rc == GC_OK) rc = make_map(&maps.out, Matrix{out, M, hp, 2 * hp, 2}, 32, 32);
@@ -1180,6 +1123,11 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_e4m3: workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Matrix x{X8, M, D, ldx, 1}, w{W8, 2 * H, D, ldw, 1}, wout{Wout, H, O, ldwout, 2};
+  if (few_rows(M, D, H, O, readable(w) && readable(wout))) {
+    const Rows r{X8, W8, Wout, x_scale, w_scale, reinterpret_cast<uint16_t*>(ws), Y, ldx, ldw, ldwout, up8(H), ldy, int(M), int(D),
+                 int(H), int(O), act, Saved{}};
+    return forward_few_rows(r, true, st);
+  }
   int rc = make_readable(x, ws, st);
   if (rc == GC_OK) rc = make_readable(w, ws, st);
   if (rc == GC_OK) rc = make_readable(wout, ws, st);
@@ -1196,7 +1144,7 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   p.sa = x_scale;
   p.sb = w_scale;
   rc = error_word(&p.word);
-  if (rc == GC_OK) rc = operand_maps(maps, x, false, w, false, t.bn / 2);
+  if (rc == GC_OK) rc = operand_maps(maps, p, x, false, w, false, t.bn / 2);
   if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 32, 32);
   if (rc == GC_OK) rc = launch_tile<kGated, false, false, true>(t, maps, p, st);
   if (rc != GC_OK) return rc;
