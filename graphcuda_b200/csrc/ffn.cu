@@ -718,15 +718,42 @@ ffn_sum_kernel(const float* __restrict__ parts, int splits, int M, int pitch, bf
   }
 }
 
-// dst[r, c] = src[r, c] for c < cols, 0 up to the pitch ldd: rows that TMA can read.
-template <class T>
+// Copies of matrices whose rows TMA cannot read, all of a call in one launch: dst[r, c] = src[r, c] for c < cols, 0 up to
+// `width`, a multiple of 4 bytes in rows that are 4-byte aligned.  A warp takes rows in turn, a lane a word of the copy.
+struct Copies {
+  static constexpr int kMost = 6;
+  struct Job {
+    const void* src;
+    void* dst;
+    int64_t lds, ldd, rows;
+    int cols, width, size;  // size: bytes of an element, 1 or 2
+  } job[kMost];
+  int first_block[kMost + 1];  // prefix sum of the CTAs that a job gets
+  int count;
+};
 __global__ void __launch_bounds__(256)
-repitch_kernel(const T* __restrict__ src, int64_t lds, T* __restrict__ dst, int64_t ldd, int64_t rows, int cols, int width) {
-  const int64_t total = rows * width;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-    const int64_t r = i / width;
-    const int c = int(i % width);
-    dst[r * ldd + c] = c < cols ? src[r * lds + c] : T(0);
+repitch_kernel(const __grid_constant__ Copies c) {
+  int j = 0;
+  while (j + 1 < c.count && int(blockIdx.x) >= c.first_block[j + 1]) ++j;
+  const Copies::Job& job = c.job[j];
+  const int lane = threadIdx.x % 32, blocks = c.first_block[j + 1] - c.first_block[j];
+  const int per = 4 / job.size;  // elements of a word
+  for (int64_t r = int64_t(blockIdx.x - c.first_block[j]) * 8 + threadIdx.x / 32; r < job.rows; r += int64_t(blocks) * 8) {
+    const uint8_t* src = static_cast<const uint8_t*>(job.src) + r * job.lds * job.size;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(job.dst) + r * job.ldd * job.size);
+    for (int w = lane; w < job.width / per; w += 32) {
+      uint32_t word = 0;
+      if (job.size == 2) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (2 * w + e < job.cols) word |= uint32_t(reinterpret_cast<const uint16_t*>(src)[2 * w + e]) << (16 * e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * w + e < job.cols) word |= uint32_t(src[4 * w + e]) << (8 * e);
+      }
+      dst[w] = word;
+    }
   }
 }
 
@@ -774,7 +801,9 @@ Tile pick_tile(Kind kind, int64_t M, int64_t N, int64_t splits_possible) {
   const int64_t mid = gc::ceil_div(M, BM) * gc::ceil_div(n_acc, 128) * splits_possible;
   return {n_acc > 64 && mid >= gc::kNumSMs ? 128 : 64, false};
 }
-// Plain products with fewer tiles than CTAs and a long K are cut along K.
+// Plain products with at most half as many tiles as CTAs and a long K are cut along K, into at least 4 k-blocks each.  The
+// launch that adds the parts costs 2 to 3 us, as much as some ten k-blocks: from 16 k-blocks on (steps of seven sizes, 40 x
+// 1024 to 9000 x 300: from 8 on 1 to 5 % slower on the small ones, from 24 or 32 on and into 8 the same or up to 5 %).
 struct Split {
   Tile tile;
   int splits, per;
@@ -786,7 +815,7 @@ Split plan_plain(int64_t M, int64_t N, int64_t K) {
   const int64_t tm = s.tile.pair ? 256 : BM, units = s.tile.pair ? gc::kNumSMs / 2 : gc::kNumSMs;
   const int64_t tiles = gc::ceil_div(M, tm) * gc::ceil_div(N, s.tile.bn);
   int64_t splits = 1;
-  if (tiles * 2 <= units && nkb >= 8) splits = std::min<int64_t>(units / tiles, nkb / 4);
+  if (tiles * 2 <= units && nkb >= 16) splits = std::min<int64_t>(units / tiles, nkb / 4);
   s.per = int(gc::ceil_div(nkb, std::max<int64_t>(1, splits)));
   s.splits = int(gc::ceil_div(nkb, s.per));
   return s;
@@ -895,38 +924,40 @@ int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int
 bool readable(const Matrix& m) { return gc::aligned16(m.p) && m.ld * m.size % 16 == 0; }
 int64_t readable_ld(const Matrix& m) { return (m.cols * m.size + 15) / 16 * 16 / m.size; }
 size_t copy_bytes(const Matrix& m) { return readable(m) ? 0 : align256(size_t(m.rows) * size_t(readable_ld(m)) * m.size); }
-template <class T>
-int repitch(const Matrix& m, void* dst, int64_t ldd, int64_t width, cudaStream_t st) {
-  const int64_t total = m.rows * width;
-  repitch_kernel<T><<<unsigned(std::min<int64_t>(gc::ceil_div(total, 256), gc::kNumSMs * 16)), 256, 0, st>>>(
-      static_cast<const T*>(m.p), m.ld, static_cast<T*>(dst), ldd, m.rows, int(m.cols), int(width));
-  return gc::check_launch("repitch_kernel");
+void add_copy(Copies& c, const Matrix& m, void* dst, int64_t ldd, int64_t width) {
+  const int j = c.count++;
+  c.job[j] = {m.p, dst, m.ld, ldd, m.rows, int(m.cols), int(width), m.size};
+  const int64_t blocks = std::min<int64_t>(gc::ceil_div(m.rows, 8), gc::kNumSMs * 8);
+  c.first_block[0] = 0;
+  c.first_block[j + 1] = c.first_block[j] + int(blocks);
 }
-int make_readable(Matrix& m, char*& ws, cudaStream_t st) {
-  if (readable(m)) return GC_OK;
+void make_readable(Matrix& m, char*& ws, Copies& c) {
+  if (readable(m)) return;
   const size_t bytes = copy_bytes(m);
   const int64_t ld = readable_ld(m);
-  const int rc = m.size == 2 ? repitch<uint16_t>(m, ws, ld, ld, st) : repitch<uint8_t>(m, ws, ld, ld, st);
+  add_copy(c, m, ws, ld, ld);
   m.p = ws;
   m.ld = ld;
   ws += bytes;
-  return rc;
 }
 // [Wg | Wu]: where H is not a multiple of 8, U's columns are moved to the next one, and the columns between are zeros -- as are
 // then those of G, U, A and their gradients.
 size_t gate_up_bytes(const Matrix& w, int64_t H) {
   return H % 8 == 0 ? copy_bytes(w) : align256(size_t(w.rows) * size_t(2 * up8(H)) * 2);
 }
-int make_gate_up(Matrix& w, int64_t H, char*& ws, cudaStream_t st) {
-  if (H % 8 == 0) return make_readable(w, ws, st);
+void make_gate_up(Matrix& w, int64_t H, char*& ws, Copies& c) {
+  if (H % 8 == 0) return make_readable(w, ws, c);
   const int64_t hp = up8(H);
   uint16_t* to = reinterpret_cast<uint16_t*>(ws);
-  Matrix gate{w.p, w.rows, H, w.ld, 2}, up{static_cast<const uint16_t*>(w.p) + H, w.rows, H, w.ld, 2};
-  int rc = repitch<uint16_t>(gate, to, 2 * hp, hp, st);
-  if (rc == GC_OK) rc = repitch<uint16_t>(up, to + hp, 2 * hp, hp, st);
+  add_copy(c, Matrix{w.p, w.rows, H, w.ld, 2}, to, 2 * hp, hp);
+  add_copy(c, Matrix{static_cast<const uint16_t*>(w.p) + H, w.rows, H, w.ld, 2}, to + hp, 2 * hp, hp);
   ws += gate_up_bytes(w, H);
   w = Matrix{to, w.rows, 2 * hp, 2 * hp, 2};
-  return rc;
+}
+int run_copies(const Copies& c, cudaStream_t st) {
+  if (c.count == 0) return GC_OK;
+  repitch_kernel<<<unsigned(c.first_block[c.count]), 256, 0, st>>>(c);
+  return gc::check_launch("repitch_kernel");
 }
 
 Saved saved_at(void* p, int64_t M, int64_t H) {
@@ -946,6 +977,9 @@ Saved saved_at(void* p, int64_t M, int64_t H) {
 bool few_rows(int64_t M, int64_t D, int64_t H, int64_t O, bool in_place) {
   return M == 1 || (M <= kFewRows && (!in_place || 2 * (2 * D * H + H * O) <= (int64_t(16) << 20)));
 }
+
+// Room for the product between the two launches: fp32 in the form for few rows.
+size_t hidden_bytes(int64_t M, int64_t hp) { return align256(size_t(M) * hp * (M <= kFewRows ? 4 : 2)); }
 
 bool sizes_ok(int64_t M, int64_t D, int64_t H, int64_t O) {
   const int64_t top = (int64_t(1) << 31) - 512;  // coordinates and tile counts are 32-bit
@@ -967,7 +1001,7 @@ size_t gc_gated_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O, 
   const int64_t hp = up8(H);
   // copies of every operand, should none be readable in place
   size_t b = align256(size_t(M) * up8(D) * 2) + align256(size_t(D) * 2 * hp * 2) + align256(size_t(H) * up8(O) * 2);
-  if (!backward) return b + align256(size_t(M) * hp * 2) + plain_workspace(M, O, H);
+  if (!backward) return b + hidden_bytes(M, hp) + plain_workspace(M, O, H);
   b += align256(size_t(M) * up8(O) * 2) + align256(size_t(M) * 2 * hp * 2);  // dY, dG | dU
   return b + std::max({plain_workspace(M, D, 2 * hp), plain_workspace(D, 2 * hp, M), plain_workspace(H, O, M)});
 }
@@ -997,13 +1031,15 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   Matrix x{X, M, D, ldx, 2}, win{Win, D, 2 * H, ldwin, 2}, wout{Wout, H, O, ldwout, 2};
   if (few_rows(M, D, H, O, readable(win) && H % 8 == 0 && readable(wout))) {
     const Saved keep = saved ? saved_at(saved, M, H) : Saved{};
-    const Rows r{X, Win, Wout, nullptr, nullptr, saved ? keep.hidden : reinterpret_cast<uint16_t*>(ws), Y, ldx, ldwin, ldwout,
+    const Rows r{X, Win, Wout, nullptr, nullptr, reinterpret_cast<float*>(ws), Y, ldx, ldwin, ldwout,
                  hp, ldy, int(M), int(D), int(H), int(O), act, keep};
     return forward_few_rows(r, false, st);
   }
-  int rc = make_readable(x, ws, st);
-  if (rc == GC_OK) rc = make_gate_up(win, H, ws, st);
-  if (rc == GC_OK) rc = make_readable(wout, ws, st);
+  Copies copies{};
+  make_readable(x, ws, copies);
+  make_gate_up(win, H, ws, copies);
+  make_readable(wout, ws, copies);
+  int rc = run_copies(copies, st);
   if (rc != GC_OK) return rc;
   uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);
   Saved keep{};
@@ -1061,10 +1097,12 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_backward_bf16: workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Matrix dy{dY, M, O, lddy, 2}, x{X, M, D, ldx, 2}, win{Win, D, 2 * H, ldwin, 2}, wout{Wout, H, O, ldwout, 2};
-  int rc = make_readable(dy, ws, st);
-  if (rc == GC_OK && dWin) rc = make_readable(x, ws, st);
-  if (rc == GC_OK && dX) rc = make_gate_up(win, H, ws, st);
-  if (rc == GC_OK && (dX || dWin)) rc = make_readable(wout, ws, st);
+  Copies copies{};
+  make_readable(dy, ws, copies);
+  if (dWin) make_readable(x, ws, copies);
+  if (dX) make_gate_up(win, H, ws, copies);
+  if (dX || dWin) make_readable(wout, ws, copies);
+  int rc = run_copies(copies, st);
   if (rc != GC_OK) return rc;
   const Saved kept = saved_at(const_cast<void*>(saved), M, H);
   const Matrix dgu{ws, M, 2 * hp, 2 * hp, 2};
@@ -1098,7 +1136,7 @@ size_t gc_gated_ffn_e4m3_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_
   if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, D, H, O)) return 0;
   const int64_t d16 = (D + 15) / 16 * 16;
   return align256(size_t(M) * d16) + align256(size_t(2 * H) * d16) + align256(size_t(H) * up8(O) * 2) +
-         align256(size_t(M) * up8(H) * 2) + plain_workspace(M, O, H);
+         hidden_bytes(M, up8(H)) + plain_workspace(M, O, H);
 }
 
 int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_scale, const uint8_t* W8, int64_t ldw,
@@ -1124,13 +1162,15 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   char* ws = static_cast<char*>(workspace);
   Matrix x{X8, M, D, ldx, 1}, w{W8, 2 * H, D, ldw, 1}, wout{Wout, H, O, ldwout, 2};
   if (few_rows(M, D, H, O, readable(w) && readable(wout))) {
-    const Rows r{X8, W8, Wout, x_scale, w_scale, reinterpret_cast<uint16_t*>(ws), Y, ldx, ldw, ldwout, up8(H), ldy, int(M), int(D),
+    const Rows r{X8, W8, Wout, x_scale, w_scale, reinterpret_cast<float*>(ws), Y, ldx, ldw, ldwout, up8(H), ldy, int(M), int(D),
                  int(H), int(O), act, Saved{}};
     return forward_few_rows(r, true, st);
   }
-  int rc = make_readable(x, ws, st);
-  if (rc == GC_OK) rc = make_readable(w, ws, st);
-  if (rc == GC_OK) rc = make_readable(wout, ws, st);
+  Copies copies{};
+  make_readable(x, ws, copies);
+  make_readable(w, ws, copies);
+  make_readable(wout, ws, copies);
+  int rc = run_copies(copies, st);
   if (rc != GC_OK) return rc;
   const int64_t hp = up8(H);
   uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);

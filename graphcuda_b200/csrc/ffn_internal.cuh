@@ -105,7 +105,7 @@ struct Rows {
   const uint16_t* w_out;  // H x O
   const float* x_scale;
   const float* w_scale;
-  uint16_t* hidden;  // M x H scratch, pitch `ldh`
+  float* hidden;     // M x H scratch, pitch `ldh` = P
   uint16_t* y;
   int64_t ldx, ldw, ldwout, ldh, ldy;
   int M, D, H, O, act;

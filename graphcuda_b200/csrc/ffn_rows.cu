@@ -1,7 +1,7 @@
 // The gated feed-forward block for a few rows: what a server runs for single vertices.
 //
 // Bound by memory: with up to 8 rows every weight is read once and used for a handful of multiply-adds, so the products run on
-// CUDA cores, in fp32, with as many loads in flight as the SMs hold; a tile of the tensor cores would be empty.  Two
+// CUDA cores, in fp32 (the product between the launches too: it is small, and no tensor core asks for 16 bits), with as many loads in flight as the SMs hold; a tile of the tensor cores would be empty.  Two
 // launches: G, U and their product; then Y.  The second starts while the first still runs, brings its weights into the L2, which do
 // not depend on it, and waits.
 //
@@ -63,11 +63,12 @@ __device__ __forceinline__ float gated(float g, float u, int act) {
   return a * u;
 }
 
-// out (M x N) = x W, or (GATED) act(x Wg) * (x Wu) with W = [Wg | Wu].  VEC: rows of W in 16-byte accesses, N a multiple of 8.
+// GATED: hidden (M x N, fp32) = act(x Wg) * (x Wu) with W = [Wg | Wu], x in bf16, and what `keep` asks for; else out (M x N, bf16)
+// = hidden W.  VEC: rows of W in 16-byte accesses, N a multiple of 8.
 template <bool GATED, int MR, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-ffn_rows_kernel(const bf16* __restrict__ x, int64_t ldx, const bf16* __restrict__ w, int64_t ldw, bf16* __restrict__ out,
-                int64_t ldo, int M, int K, int N, int act, int ctas, int x_vec, Saved keep) {
+ffn_rows_kernel(const std::conditional_t<GATED, bf16, float>* __restrict__ x, int64_t ldx, const bf16* __restrict__ w,
+                int64_t ldw, std::conditional_t<GATED, float, bf16>* __restrict__ out, int64_t ldo, int M, int K, int N, int act, int ctas, int x_vec, Saved keep) {
   constexpr int kLanes = GATED ? 16 : 8;   // to a row of W
   constexpr int kSubs = 32 / kLanes;       // blocks of 8 rows that a warp reads at once
   constexpr int kWidth = GATED ? 2 * kCols : kCols;
@@ -97,7 +98,8 @@ ffn_rows_kernel(const bf16* __restrict__ x, int64_t ldx, const bf16* __restrict_
 #pragma unroll 1
   for (int b = b_from + warp * kSubs + lane / kLanes; b < b_to; b += kWarps * kSubs) {
     const int k0 = b * 8;
-    uint4 wv[8], xv[MR];
+    uint4 wv[8];
+    float xv[MR][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int k = k0 + i;
@@ -113,15 +115,23 @@ ffn_rows_kernel(const bf16* __restrict__ x, int64_t ldx, const bf16* __restrict_
     }
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
-      const bf16* row = x + int64_t(min(m, M - 1)) * ldx + k0;
+      const auto* row = x + int64_t(min(m, M - 1)) * ldx + k0;
       if (x_vec && k0 + 8 <= K) {
-        xv[m] = *reinterpret_cast<const uint4*>(row);
-      } else {
-        xv[m] = make_uint4(0, 0, 0, 0);
-        uint32_t* words = &xv[m].x;
+        if constexpr (GATED) {
+          const uint4 t = *reinterpret_cast<const uint4*>(row);
+          const uint32_t words[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (k0 + e < K) words[e / 2] |= uint32_t(__bfloat16_as_ushort(row[e])) << (e % 2 * 16);
+          for (int e = 0; e < 8; ++e) xv[m][e] = __uint_as_float(e % 2 ? words[e / 2] & 0xFFFF0000u : words[e / 2] << 16);
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 t = *reinterpret_cast<const float4*>(row + 4 * h);
+            xv[m][4 * h] = t.x, xv[m][4 * h + 1] = t.y, xv[m][4 * h + 2] = t.z, xv[m][4 * h + 3] = t.w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) xv[m][e] = k0 + e < K ? float(row[e]) : 0.f;
       }
     }
 #pragma unroll
@@ -132,8 +142,7 @@ ffn_rows_kernel(const bf16* __restrict__ x, int64_t ldx, const bf16* __restrict_
       for (int j = 0; j < 4; ++j) v[j] = F2(words[j] << 16, words[j] & 0xFFFF0000u);
 #pragma unroll
       for (int m = 0; m < MR; ++m) {
-        const uint32_t pair = (&xv[m].x)[i / 2];
-        const F2 xm = both(__uint_as_float(i % 2 ? pair & 0xFFFF0000u : pair << 16));
+        const F2 xm = both(xv[m][i]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[m][j] = fma2(xm, v[j], acc[m][j]);
       }
@@ -173,7 +182,15 @@ ffn_rows_kernel(const bf16* __restrict__ x, int64_t ldx, const bf16* __restrict_
       if (GATED) u += ctas > 1 ? peer_load(&part_s[m][kCols + c], r) : part_s[m][kCols + c];
     }
     const int col = col0 + c;
-    if (m < M && col < N) out[int64_t(m) * ldo + col] = __float2bfloat16_rn(GATED ? gated(a, u, act) : a);
+    if (m < M && col < N) {
+      if constexpr (GATED) {
+        const float h = gated(a, u, act);
+        out[int64_t(m) * ldo + col] = h;
+        if (keep.hidden) reinterpret_cast<bf16*>(keep.hidden)[int64_t(m) * ldo + col] = __float2bfloat16_rn(h);
+      } else {
+        out[int64_t(m) * ldo + col] = __float2bfloat16_rn(a);
+      }
+    }
     if (GATED && keep.gate_up && m < M) {  // a warp has 32 columns of one row
       const int pitch = (N + 7) / 8 * 8;
       if (col >= N) a = u = 0.f;  // the pad columns take part in the backward pass as zeros
@@ -194,12 +211,12 @@ ffn_rows_kernel(const bf16* __restrict__ x, int64_t ldx, const bf16* __restrict_
   if (ctas > 1) cluster_sync();  // a CTA's shared memory is read by the others until here
 }
 
-// hidden (M x H) = act(G) U from e4m3 operands, K along the rows of both: a warp per column.
+// hidden (M x H, fp32) = act(G) U from e4m3 operands, K along the rows of both: a warp per column.
 template <int MR, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 ffn_rows_e4m3_kernel(const uint8_t* __restrict__ x, int64_t ldx, const float* __restrict__ x_scale,
-                     const uint8_t* __restrict__ w, int64_t ldw, const float* __restrict__ w_scale, bf16* __restrict__ out,
-                     int64_t ldo, int M, int K, int H, int act) {
+                     const uint8_t* __restrict__ w, int64_t ldw, const float* __restrict__ w_scale,
+                     float* __restrict__ out, int64_t ldo, int M, int K, int H, int act) {
   const int lane = threadIdx.x % 32, h = int(blockIdx.x) * kWarps + threadIdx.x / 32;
   let_next_begin();
   if (h >= H) return;
@@ -258,7 +275,7 @@ ffn_rows_e4m3_kernel(const uint8_t* __restrict__ x, int64_t ldx, const float* __
     }
     if (lane == 0 && m < M) {
       const float sx = x_scale[m];
-      out[int64_t(m) * ldo + h] = __float2bfloat16_rn(gated(s[0] * (sx * w_scale[h]), s[1] * (sx * w_scale[H + h]), act));
+      out[int64_t(m) * ldo + h] = gated(s[0] * (sx * w_scale[h]), s[1] * (sx * w_scale[H + h]), act);
     }
   }
 }
@@ -273,8 +290,13 @@ int cluster_of(int N, int K) {
   return c;
 }
 
+template <bool GATED>
+using In = std::conditional_t<GATED, bf16, float>;
+template <bool GATED>
+using Out = std::conditional_t<GATED, float, bf16>;
+
 template <bool GATED, int MR, bool VEC>
-int launch_rows(const bf16* x, int64_t ldx, const bf16* w, int64_t ldw, bf16* out, int64_t ldo, int M, int K, int N, int act,
+int launch_rows(const In<GATED>* x, int64_t ldx, const bf16* w, int64_t ldw, Out<GATED>* out, int64_t ldo, int M, int K, int N, int act,
                 const Saved& keep, cudaStream_t st) {
   const int ctas = cluster_of(N, K);
   const int64_t blocks = gc::ceil_div(N, kCols) * ctas;
@@ -295,11 +317,11 @@ int launch_rows(const bf16* x, int64_t ldx, const bf16* w, int64_t ldw, bf16* ou
     at[cfg.numAttrs].val.clusterDim.y = 1;
     at[cfg.numAttrs++].val.clusterDim.z = 1;
   }
-  cudaLaunchKernelEx(&cfg, ffn_rows_kernel<GATED, MR, VEC>, x, ldx, w, ldw, out, ldo, M, K, N, act, ctas, int(aligned_rows(x, ldx * 2)), keep);
+  cudaLaunchKernelEx(&cfg, ffn_rows_kernel<GATED, MR, VEC>, x, ldx, w, ldw, out, ldo, M, K, N, act, ctas, int(aligned_rows(x, ldx * int64_t(sizeof(*x)))), keep);
   return gc::check_launch("ffn_rows_kernel");
 }
 template <bool GATED, bool VEC>
-int rows_of(const bf16* x, int64_t ldx, const bf16* w, int64_t ldw, bf16* out, int64_t ldo, int M, int K, int N, int act,
+int rows_of(const In<GATED>* x, int64_t ldx, const bf16* w, int64_t ldw, Out<GATED>* out, int64_t ldo, int M, int K, int N, int act,
             const Saved& keep, cudaStream_t st) {
   if (M == 1) return launch_rows<GATED, 1, VEC>(x, ldx, w, ldw, out, ldo, M, K, N, act, keep, st);
   if (M == 2) return launch_rows<GATED, 2, VEC>(x, ldx, w, ldw, out, ldo, M, K, N, act, keep, st);
@@ -307,7 +329,7 @@ int rows_of(const bf16* x, int64_t ldx, const bf16* w, int64_t ldw, bf16* out, i
   return launch_rows<GATED, 8, VEC>(x, ldx, w, ldw, out, ldo, M, K, N, act, keep, st);
 }
 template <bool GATED>
-int product(const bf16* x, int64_t ldx, const bf16* w, int64_t ldw, bf16* out, int64_t ldo, int M, int K, int N, int act,
+int product(const In<GATED>* x, int64_t ldx, const bf16* w, int64_t ldw, Out<GATED>* out, int64_t ldo, int M, int K, int N, int act,
             const Saved& keep, cudaStream_t st) {
   return N % 8 == 0 && aligned_rows(w, ldw * 2) ? rows_of<GATED, true>(x, ldx, w, ldw, out, ldo, M, K, N, act, keep, st)
                                                 : rows_of<GATED, false>(x, ldx, w, ldw, out, ldo, M, K, N, act, keep, st);
@@ -316,11 +338,10 @@ template <int MR>
 int product_e4m3(const Rows& r, cudaStream_t st) {
   const unsigned blocks = unsigned(gc::ceil_div(r.H, kWarps));
   const uint8_t *x = static_cast<const uint8_t*>(r.x), *w = static_cast<const uint8_t*>(r.w);
-  bf16* out = reinterpret_cast<bf16*>(r.hidden);
   if (r.D % 16 == 0 && aligned_rows(x, r.ldx) && aligned_rows(w, r.ldw))
-    ffn_rows_e4m3_kernel<MR, true><<<blocks, kThreads, 0, st>>>(x, r.ldx, r.x_scale, w, r.ldw, r.w_scale, out, r.ldh, r.M, r.D, r.H, r.act);
+    ffn_rows_e4m3_kernel<MR, true><<<blocks, kThreads, 0, st>>>(x, r.ldx, r.x_scale, w, r.ldw, r.w_scale, r.hidden, r.ldh, r.M, r.D, r.H, r.act);
   else
-    ffn_rows_e4m3_kernel<MR, false><<<blocks, kThreads, 0, st>>>(x, r.ldx, r.x_scale, w, r.ldw, r.w_scale, out, r.ldh, r.M, r.D, r.H, r.act);
+    ffn_rows_e4m3_kernel<MR, false><<<blocks, kThreads, 0, st>>>(x, r.ldx, r.x_scale, w, r.ldw, r.w_scale, r.hidden, r.ldh, r.M, r.D, r.H, r.act);
   return gc::check_launch("ffn_rows_e4m3_kernel");
 }
 
@@ -330,15 +351,14 @@ namespace gc {
 namespace ffn {
 
 int forward_few_rows(const Rows& r, bool e4m3, cudaStream_t st) {
-  bf16* hidden = reinterpret_cast<bf16*>(r.hidden);
   int rc;
   if (e4m3)
     rc = r.M == 1 ? product_e4m3<1>(r, st) : r.M == 2 ? product_e4m3<2>(r, st) : r.M <= 4 ? product_e4m3<4>(r, st) : product_e4m3<8>(r, st);
   else
-    rc = product<true>(static_cast<const bf16*>(r.x), r.ldx, static_cast<const bf16*>(r.w), r.ldw, hidden, r.ldh, r.M, r.D, r.H,
+    rc = product<true>(static_cast<const bf16*>(r.x), r.ldx, static_cast<const bf16*>(r.w), r.ldw, r.hidden, r.ldh, r.M, r.D, r.H,
                        r.act, r.saved, st);
   if (rc != GC_OK) return rc;
-  return product<false>(hidden, r.ldh, reinterpret_cast<const bf16*>(r.w_out), r.ldwout, reinterpret_cast<bf16*>(r.y), r.ldy,
+  return product<false>(r.hidden, r.ldh, reinterpret_cast<const bf16*>(r.w_out), r.ldwout, reinterpret_cast<bf16*>(r.y), r.ldy,
                         r.M, r.H, r.O, r.act, Saved{}, st);
 }
 
