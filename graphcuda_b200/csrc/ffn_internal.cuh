@@ -61,8 +61,24 @@ __device__ __forceinline__ F2 activate(F2 g, F2& slope) {
     slope = fma2(a, fma2(s, both(-1.f), both(1.f)), s);
     return a;
   } else if constexpr (ACT == GC_ACT_GELU) {
-    const F2 cdf = fma2(each(g * both(0.70710678118654752f), [](float x) { return erff(x); }), both(0.5f), both(0.5f));
-    const F2 pdf = each(g * g * both(-0.72134752044448170f), [](float x) { return exp2_approx(x); });
+    // The normal distribution's tail beyond |g| is e^(-g^2/2) / 2 times erfcx(|g| / sqrt 2), and for erfcx a polynomial in t =
+    // 1 / (1 + 0.44 x) was fitted here, the relative error made even over 0 <= x <= 13: 6e-6, in the far tail too, where 1 + erf would
+    // cancel.  The exponential is the one that the derivative needs.  (With erff the epilogue of the backward product set
+    // its time: tensor cores 59 % active at K = 2048.)
+    const F2 x = each(g, [](float v) { return fabsf(v); }) * both(0.70710678118654752f);
+    const F2 t = each(fma2(x, both(0.44f), both(1.f)), [](float v) { return rcp_approx(v); });
+    const F2 pdf = each(g * g * both(-0.72134752044448170f), [](float v) { return exp2_approx(v); });
+    F2 q = both(-0.14544761f);
+    q = fma2(q, t, both(0.34884202f));
+    q = fma2(q, t, both(0.04260680f));
+    q = fma2(q, t, both(0.26268032f));
+    q = fma2(q, t, both(0.24277152f));
+    q = fma2(q, t, both(0.24854454f));
+    q = q * (t * (pdf * both(0.5f)));
+    float g0, g1, q0, q1;
+    g.get(g0, g1);
+    q.get(q0, q1);
+    const F2 cdf(g0 < 0.f ? q0 : 1.f - q0, g1 < 0.f ? q1 : 1.f - q1);
     slope = fma2(g * pdf, both(0.39894228040143268f), cdf);
     return g * cdf;
   } else {
