@@ -227,7 +227,7 @@ __device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t lane_
   if (fits_fp16(most)) return 0;
   uint32_t bits = 0;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) bits = max(bits, v[j] & 0x7FFFFFFFu);
+  for (int j = 0; j < 32; ++j) bits = max(bits, finite_bits(v[j]));
   const int e = shared_exponent(bits);
   const float2 f = unscale(e);
 #pragma unroll
@@ -616,6 +616,11 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           loaded(c);
           if (!F8 && p.exps) {
             const int64_t at = int64_t(col / 32) * p.M + row;
+            if (col + 32 > p.N) {  // what lies beyond has no say in the exponents
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (col + i >= p.N) g[i] = u[i] = 0;
+            }
             const uint32_t bg = acquire();
             const int eg = pack_fp16(g, lane_at + bg);
             put(&maps.out2, bg, col, row0);

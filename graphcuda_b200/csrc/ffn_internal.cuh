@@ -100,10 +100,12 @@ struct Saved {
   uint16_t* gate_up;  // M x 2P
   int8_t* exps;       // [2][ceil(P / 32)][M]
 };
+// A magnitude as a float's bits; 0 for an infinity or a NaN, which any exponent keeps and which has no say in its neighbours'.
+__device__ __forceinline__ uint32_t finite_bits(uint32_t v) { return (v & 0x7FFFFFFFu) < 0x7F800000u ? v & 0x7FFFFFFFu : 0u; }
 // The exponent that 32 values with the largest magnitude `bits` (as a float's) take where `most`, the largest fp16 number they
 // would be, overflows or falls below 2^-10, from where fp16 loses bits: it brings the largest to 2^14.  0 where it does not.
 __device__ __forceinline__ int shared_exponent(uint32_t bits) {
-  if (bits == 0 || bits >= 0x7F800000u) return 0;  // zeros; an infinity or a NaN, with which the row is lost
+  if (bits == 0) return 0;
   return max(int(bits >> 23) - 127 - 14, -126);
 }
 __device__ __forceinline__ bool fits_fp16(uint32_t most) { return most >= 0x1400u && most < 0x7C00u; }

@@ -49,7 +49,7 @@ __device__ __forceinline__ int pack_fp16(float v, __half& out) {
   out = __float2half_rn(v);
   const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, uint32_t(__half_as_ushort(out)) & 0x7FFFu);
   if (fits_fp16(most)) return 0;
-  const int e = shared_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu));
+  const int e = shared_exponent(__reduce_max_sync(0xFFFFFFFFu, finite_bits(__float_as_uint(v))));
   const float2 f = unscale(e);
   out = __float2half_rn(v * f.x * f.y);
   return e;
