@@ -84,6 +84,8 @@ __device__ __forceinline__ void load4(const void* base, int64_t at, int64_t n, T
     for (int k = 0; k < 4; ++k) v[k] = at + k < n ? p[k] : T(0.f);
   }
 }
+// Stores that the L2 gives up first: nothing is read again before the next step (82 M parameters in 394 us, with plain stores
+// 402).
 template <bool FAST, class T>
 __device__ __forceinline__ void store4(void* base, int64_t at, int64_t n, const T (&v)[4]) {
   struct alignas(4 * sizeof(T)) V { T v[4]; };
@@ -92,7 +94,9 @@ __device__ __forceinline__ void store4(void* base, int64_t at, int64_t n, const 
     V t;
 #pragma unroll
     for (int k = 0; k < 4; ++k) t.v[k] = v[k];
-    *reinterpret_cast<V*>(p) = t;
+    using W = std::conditional_t<sizeof(V) == 16, uint4, uint2>;
+    static_assert(sizeof(V) == sizeof(W), "four elements of 4 or 2 bytes");
+    __stcs(reinterpret_cast<W*>(p), *reinterpret_cast<const W*>(&t));
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -110,11 +114,12 @@ __device__ __forceinline__ uint32_t load_codes(const void* base, int64_t at, int
     if (at + k < n) w |= uint32_t(p[k]) << (8 * k);
   return w;
 }
+// (the lowest bytes of q)
 template <bool FAST>
 __device__ __forceinline__ void store_codes(void* base, int64_t at, int64_t n, const uint32_t (&q)[4]) {
   uint8_t* p = static_cast<uint8_t*>(base) + at;
   if constexpr (FAST) {
-    *reinterpret_cast<uint32_t*>(p) = (q[0] | q[1] << 8) | (q[2] << 16 | q[3] << 24);
+    *reinterpret_cast<uint32_t*>(p) = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -131,16 +136,24 @@ __device__ __forceinline__ float2 scale_of(uint32_t top_bits, float top_code) {
   if (s < 1.17549435e-38f) return make_float2(0.f, 0.f);
   return make_float2(s, __frcp_rn(s));
 }
-// t >= 0 to a code of 3 bits of mantissa and an exponent of bias BIAS: u (16 bits) is added below the last kept bit and
-// the rest cut off.  Below the smallest normal number the grid is even, and the sum is formed in units of it.  Floats and
-// integers are taken from each other's bits here: conversion instructions run at an eighth of the rate.
+// To a code of 3 bits of mantissa and an exponent of bias BIAS: u (16 bits) is added below the last kept bit and the rest
+// cut off.  Floats and integers are taken from each other's bits here: conversion instructions run at an eighth of the rate.
+// Normal numbers: the result, of either sign, is in bits 20 to 26 (30), with the sign in bit 31.  None rounds up beyond the largest
+// code: what is left of the largest value's own mantissa is an error of 3 units at most, and 16 would carry.
+template <int BIAS>
+__device__ __forceinline__ uint32_t round_normal(float t, uint32_t u_by_16) {
+  return __float_as_uint(t) + u_by_16 - ((127u - BIAS) << 23);
+}
+// Any t >= 0.  Below the smallest normal number the grid is even, and the sum is formed in units of it.
+template <int BIAS>
+constexpr float kLowest = BIAS == 7 ? 0x1p-6f : 0x1p-14f;
 template <int BIAS>
 __device__ __forceinline__ uint32_t round_code(float t, uint32_t u) {
-  constexpr float kLowest = BIAS == 7 ? 0x1p-6f : 0x1p-14f, kUnits = BIAS == 7 ? 0x1p9f : 0x1p17f;
-  const uint32_t high = ((__float_as_uint(t) + (u << 4)) >> 20) - ((127u - BIAS) << 3);
+  constexpr float kUnits = BIAS == 7 ? 0x1p9f : 0x1p17f;
+  const uint32_t high = round_normal<BIAS>(t, u << 4) >> 20;
   const float fraction = __uint_as_float(0x3F800000u | (u << 7)) - 1.0f;  // u / 2^16
   const uint32_t low = __float_as_uint(__fadd_rd(__fmaf_rn(t, kUnits, fraction), 0x1p23f)) & 0xFFu;  // towards zero
-  return t < kLowest ? low : high;
+  return t < kLowest<BIAS> ? low : high;
 }
 
 // Four codes of a word as values.
@@ -211,17 +224,21 @@ __device__ __forceinline__ void count_step(const Hyper& hp, unsigned long long s
 }
 
 // One element: moments as the formula reads, one rounding per operation; the parameter from them.  The quotient may be off
-// by 2^-21 of the update (approximate root and division: the exact ones take half of an element's instructions).
+// by 2^-21 of the update (approximate root and division: the exact ones take half of an element's instructions).  What is
+// added to v, the smallest normal number, is a root of 1.1e-19: it stands for the subnormal ones, which the fast
+// instructions take for zero.
 __device__ __forceinline__ void update(const Hyper& hp, const Scalars& sc, float g, float& m, float& v, float& p) {
   m = __fadd_rn(__fmul_rn(m, hp.b1), __fmul_rn(g, hp.w1));
   v = __fadd_rn(__fmul_rn(v, hp.b2), __fmul_rn(__fmul_rn(g, g), hp.w2));
   float root;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
-  p = p * hp.keep - sc.step_size * __fdividef(m, root * sc.inv_bc2 + hp.eps);
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v + 1.17549435e-38f));
+  float inverse;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(root * sc.inv_bc2 + hp.eps));
+  p = p * hp.keep - sc.step_size * (m * inverse);
 }
 
-// Moments of 32 bits.  Bound by memory: 28 bytes per parameter.  A thread takes 4 elements of a pass, all of whose loads are
-// under way before the first is used.
+// Moments of 32 bits.  Bound by memory: 28 bytes per parameter (82 M of them in 394 us, 5.8 TB/s).  A thread takes 4 elements of
+// a pass, all of whose loads are under way before the first is used; 6 CTAs per SM.
 template <class TP, int MAX>
 __global__ void __launch_bounds__(kThreads, 6)
 adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, MAX> tl, const __grid_constant__ Hyper hp,
@@ -277,9 +294,11 @@ adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, 
   count_step(hp, step, state);
 }
 
-// Moments of 8 bits.  A warp takes a block of 256 elements, a lane two runs of 4.
+// Moments of 8 bits.  A warp takes a block of 256 elements, a lane two runs of 4.  16 bytes per mixed parameter, of which 218 M
+// take 667 us (5.2 TB/s): some 60 instructions to an element share the issue slots with the loads.  4 CTAs per SM hide more of
+// these than 3 (694 us) and than 2 that read a chunk ahead (764).
 template <class TP, int MAX>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
 adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArrays, MAX> tl,
                   const __grid_constant__ Hyper hp, unsigned long long* __restrict__ state) {
   constexpr bool kMixed = sizeof(TP) == 2;
@@ -337,7 +356,7 @@ adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArra
           update(hp, sc, to_f32(gv[j][e]), m[j][e], v[j][e], pv[j][e]);
           if (!F && at + j * 128 + e >= n) m[j][e] = v[j][e] = 0.f;  // beyond the tensor
           top_m = max(top_m, __float_as_uint(m[j][e]) & 0x7FFFFFFFu);  // a NaN is above infinity and stays
-          top_v = max(top_v, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
+          top_v = max(top_v, __float_as_uint(v[j][e]));  // never negative
         }
         store4<F>(tl.at[kMaster][k], at + j * 128, n, pv[j]);
         if constexpr (kMixed) {
@@ -353,16 +372,35 @@ adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArra
         static_cast<float*>(tl.at[L::kVs][k])[at / kBlock] = sv.x;
       }
       const uint32_t key = mix(sc.key + uint32_t(tl.first_tensor + k)) + uint32_t(at);
+      bool normal = true;  // of nearly all blocks: no value below the smallest normal code, no NaN
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          m[j][e] = __fmul_rn(m[j][e], sm.y);
+          v[j][e] = __fmul_rn(v[j][e], sv.y);
+          normal = normal && fabsf(m[j][e]) >= kLowest<7> && v[j][e] >= kLowest<15>;
+        }
+      const bool all_normal = __all_sync(0xFFFFFFFFu, normal);
       const uint32_t least = sv.x > 0.f ? 1u : 0u;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint32_t qm[4], qv[4];
+        if (all_normal) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t r = mix(key + uint32_t(j * 128 + e));
-          const float tm = __fmul_rn(m[j][e], sm.y), tv = __fmul_rn(v[j][e], sv.y);
-          qm[e] = min(round_code<7>(fabsf(tm), r & 0xFFFFu), 0x7Eu) | (__float_as_uint(tm) >> 31 << 7);
-          qv[e] = max(min(round_code<15>(tv, r >> 16), 0xF7u), least);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t r = mix(key + uint32_t(j * 128 + e));
+            const uint32_t c = round_normal<7>(m[j][e], (r << 4) & 0xFFFF0u);
+            qm[e] = ((c >> 20) & 0x7Fu) | ((c >> 24) & 0x80u);
+            qv[e] = round_normal<15>(v[j][e], (r >> 12) & 0xFFFF0u) >> 20;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t r = mix(key + uint32_t(j * 128 + e));
+            qm[e] = min(round_code<7>(fabsf(m[j][e]), r & 0xFFFFu), 0x7Eu) | (__float_as_uint(m[j][e]) >> 31 << 7);
+            qv[e] = max(min(round_code<15>(v[j][e], r >> 16), 0xF7u), least);
+          }
         }
         store_codes<F>(tl.at[kM][k], at + j * 128, n, qm);
         store_codes<F>(tl.at[kV][k], at + j * 128, n, qv);
@@ -456,7 +494,7 @@ int step_lists(const Arrays& a, int n_tensors, Hyper hp, void* state, cudaStream
     hp.advance = next >= n_tensors;
     const int passes = tl.first_chunk[tl.count] * (BITS == 8 ? 1 : 2);
     // as many CTAs as the SMs hold, each over many passes; an empty model still counts the step
-    const int blocks = std::max(1, std::min(passes, gc::kNumSMs * (BITS == 8 ? 3 : 6)));
+    const int blocks = std::max(1, std::min(passes, gc::kNumSMs * (BITS == 8 ? 4 : 6)));
     if constexpr (BITS == 8) adamw_8bit_kernel<TP, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
     else adamw_kernel<TP, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
     ++launches;
