@@ -1,9 +1,10 @@
 // The gated feed-forward block for a few rows: what a server runs for single vertices.
 //
 // Bound by memory: with up to 8 rows every weight is read once and used for a handful of multiply-adds, so the products run on
-// CUDA cores, in fp32 (the product between the launches too: it is small, and no tensor core asks for 16 bits), with as many loads in flight as the SMs hold; a tile of the tensor cores would be empty.  Two
-// launches: G, U and their product; then Y.  The second starts while the first still runs, brings its weights into the L2, which do
-// not depend on it, and waits.
+// CUDA cores, in fp32 (the product between the launches too: it is small, and no tensor core asks for 16 bits), with as many
+// loads in flight as the SMs hold; a tile of the tensor cores would be empty.  Two launches: G, U and their product; then Y.
+// The second starts while the first still runs, brings its weights into the L2, which do not depend on it, and waits.
+// One row through 2048 -> 8192 -> 2048, 100 MB of weights that are not in the L2: 23.6 us by the call, 4.3 TB/s.
 //
 // Weights with K down the rows (bf16): a CTA has 64 output columns (of G and of U), its warps take blocks of 8 rows in turn, and a
 // lane holds 8 columns of 8 rows: 16-byte loads, whole 128-byte lines per row, and the 8 values of x in one load too.

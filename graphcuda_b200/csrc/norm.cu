@@ -10,9 +10,12 @@
 // scales it, 8 consecutive elements (16 or 32 bytes) per thread and load; rows whose length, pitch or base do not allow that
 // are read 4 elements at a time, or element by element, in the same kernels.  A group that has several rows reads the next
 // one before it works on this one, where registers allow: without that a row's loads, its sum and its stores follow each
-// other, and wide rows came to 4.3 TB/s.  Rows of more than 8192 elements are read twice instead.  Sums and statistics are fp32; h enters the statistics, y and the gradients unrounded, also where
-// the stream that is stored has 16 bits (the backward pass then adds x and r again: from a stream rounded to bf16 the
-// weight gradient would be off by 2e-3).
+// other, and wide rows came to 4.3 TB/s.  Rows of more than 8192 elements are read twice instead.  Sums and statistics are
+// fp32; h enters the statistics, y and the gradients unrounded, also where the stream that is stored has 16 bits (the backward
+// pass then adds x and r again: from a stream rounded to bf16 the weight gradient would be off by 2e-3).
+//
+// 169,343 x 256, bf16 beside an fp32 stream: forward 75 us (6.9 TB/s), backward 111 (6.2 TB/s; reading ahead by asynchronous copies
+// into shared memory 157, vectors of 4 that lie side by side in fp32 too 115).  8192 x 4096 to 8 bits: 39 us (6.0 TB/s).
 //
 // dw: a thread keeps the same columns for all rows of its group and sums them in registers; groups are added through
 // shared memory, CTAs by a second kernel, both in a fixed order.

@@ -39,9 +39,10 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activati
     """``(act(x @ Wg) * (x @ Wu)) @ w_out`` with ``w_in = [Wg | Wu]``, all bfloat16.
 
     ``x`` is [rows, in], ``w_in`` [in, 2 * hidden], ``w_out`` [hidden, out] (in x out, like GCNConv's weights).  Sums are
-    float32; the hidden row is rounded to bfloat16 before the second product, and for the backward pass so are ``x @ w_in`` and
-    its gradient.  ``activation``: "silu", "gelu" (with erf) or "relu".  Widths that are multiples of 8 are read in place,
-    others through padded copies."""
+    float32.  The hidden row is rounded to bfloat16 before the second product, and so is the gradient of ``x @ w_in`` in the
+    backward pass; ``x @ w_in`` itself is kept for it to 11 bits, with an exponent for every 32 columns of a row.
+    ``activation``: "silu", "gelu" (with erf) or "relu".  Widths that are multiples of 8 are read in place, others through
+    padded copies."""
     act = _act(activation)
     y = _lib.host.gated_ffn(x, w_in, w_out, act)
     return y if y is not None else _TracedFFN.apply(x, w_in, w_out, act)

@@ -443,7 +443,7 @@ int gc_sgd_step_f32(int n_tensors, float* const* params, const float* const* gra
  * upper byte of a positive fp16 number without its sign bit; all zero at the start.  Their values are rounded up or
  * down at random by a hash of (seed, step, tensor, element), the same on every run.  A block that has met a NaN or an
  * infinity keeps one for its scale.
- * state: 16 bytes of device memory as for gc_adam_step_f32.  One launch per 449 tensors (689 in fp32 alone).
+ * state: 16 bytes of device memory as for gc_adam_step_f32.  One launch per 449 tensors (688 in fp32 alone).
  */
 #define GC_ADAMW_BLOCK 256
 int gc_adamw_step(int n_tensors, void* const* params, int param_type, const void* const* grads, float* const* masters,
