@@ -39,6 +39,12 @@
 //   epilogue's chains.  The e4m3 first product: 149, epilogue.
 //   8192 x 2048 -> 8192 -> 2048, GELU: 375, 206, 231, 402, 341, 204 = 1190 to 1610 TFLOP/s: the tensor cores, under the power limit.
 //
+// Up to 64 rows (kStacked) the roundings of A, dG and dU, few and dominated by the largest values, do not average out, and rows
+// cost nothing there, the tiles having 128: those matrices are stored with what their rounding left as as many rows more,
+// [hi; lo].  Products over their rows' columns (Y, dX) have twice the rows, whose fp32 halves are added on the way to the
+// output; products along their rows (the weight gradients) take the other operand twice.  (Relative errors of the outputs of a step
+// of 3 rows, 25 -> 68 -> 2336: 1.6e-3, which is the output's own rounding, against 2.8e-3.)
+//
 // Every wait on a barrier is bounded, as in the other tensor-core kernel: a wait that ran out raises the device's error
 // word, all roles leave, copies in flight are drained and TMEM is released.
 #include "common.cuh"
@@ -92,9 +98,9 @@ struct Params {
   int8_t* exps;     // G's and U's exponents, [2][ceil(N / 32)][M] (Gated: null where G and U are not stored)
   const float* sa;  // e4m3: scales of A's rows and B's columns
   const float* sb;
-  bf16* C;  // Plain: the output, for rows that TMA cannot store
+  bf16* C;  // Plain: the output, for rows that TMA cannot store; else what the rounding of A, or of dG | dU, left; or null
   int64_t ldc;
-  int tma_store;
+  int tma_store, parts;  // parts: Plain stores fp32 parts
   // columns of the product -> the c_cols columns of C: those from `gap_from` on move down by `gap`, over the ones in between
   int gap_from, gap, c_cols;
   int splits, kb_per_split;
@@ -186,6 +192,14 @@ __device__ __forceinline__ uint32_t pack2(F2 a) {
   a.get(x, y);
   return pack2(x, y);
 }
+// What that left of a, rounded in its turn; nothing where it is not finite.
+__device__ __forceinline__ uint32_t pack_rest(F2 a, uint32_t packed) {
+  float x, y;
+  a.get(x, y);
+  const uint32_t lo = packed << 16, hi = packed & 0xFFFF0000u;
+  return pack2((lo & 0x7F800000u) == 0x7F800000u ? 0.f : x - __uint_as_float(lo),
+               (hi & 0x7F800000u) == 0x7F800000u ? 0.f : y - __uint_as_float(hi));
+}
 
 // A tile in shared memory: 32 rows of 64 bytes, their 16-byte units swizzled as TMA does it.  row_at is the address of unit
 // 0 of a row; unit j is where its bits 4 and 5 are XORed with j.
@@ -269,8 +283,9 @@ struct Maps {
 };
 
 // A_MN / B_MN: the operand is MN-major.  F8: e4m3 operands (K-major).  PAIR: two CTAs of a cluster work on a tile of 256 rows,
-// each with its 128 rows of A and half of B's (Gated: rank 0 has G's columns, rank 1 U's).  RES: see Cfg.
-template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES>
+// each with its 128 rows of A and half of B's (Gated: rank 0 has G's columns, rank 1 U's).  RES: see Cfg.  LO: what roundings left is
+// stored too.
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES, bool LO>
 __global__ void __launch_bounds__(kThreads, 1)
 ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C_ = Cfg<KIND, BN, F8, PAIR, RES>;
@@ -588,14 +603,25 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
               uint4 g4 = load_unit(at_g, j), u4 = load_unit(at_u, j);
               uint32_t* gw = &g4.x;
               uint32_t* uw = &u4.x;
+              uint32_t rest_g[4], rest_u[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const F2 d(acc[j * 8 + 2 * e], acc[j * 8 + 2 * e + 1]);
                 const F2 u = unpack_fp16(uw[e], fu);
                 F2 slope;
                 const F2 a = activate<decltype(act)::value>(unpack_fp16(gw[e], fg), slope);
-                gw[e] = pack2(d * u * slope);
-                uw[e] = pack2(d * a);
+                const F2 dg = d * u * slope, du = d * a;
+                gw[e] = pack2(dg);
+                uw[e] = pack2(du);
+                if (LO) {
+                  rest_g[e] = pack_rest(dg, gw[e]);
+                  rest_u[e] = pack_rest(du, uw[e]);
+                }
+              }
+              if (LO && row < p.M && col + 8 * j < p.N) {
+                bf16* to = p.C + row * p.ldc + col + 8 * j;
+                *reinterpret_cast<uint4*>(to) = make_uint4(rest_g[0], rest_g[1], rest_g[2], rest_g[3]);
+                *reinterpret_cast<uint4*>(to + p.N) = make_uint4(rest_u[0], rest_u[1], rest_u[2], rest_u[3]);
               }
               store_unit(at_g, j, g4.x, g4.y, g4.z, g4.w);
               store_unit(at_u, j, u4.x, u4.y, u4.z, u4.w);
@@ -644,7 +670,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           with_activation(p.act, [&](auto act) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              uint32_t w[4];
+              uint32_t w[4], rest[4];
               F2 sg[4], su[4];
               if (F8) {
                 load_8(scales + 32 * j, sg);
@@ -655,8 +681,12 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
                 const int i = j * 8 + 2 * e;
                 F2 vg(g[i], g[i + 1]), vu(u[i], u[i + 1]), unused;
                 if (F8) vg = vg * (both(sa) * sg[e]), vu = vu * (both(sa) * su[e]);
-                w[e] = pack2(activate<decltype(act)::value>(vg, unused) * vu);
+                const F2 a = activate<decltype(act)::value>(vg, unused) * vu;
+                w[e] = pack2(a);
+                if (LO) rest[e] = pack_rest(a, w[e]);
               }
+              if (LO && row < p.M && col + 8 * j < p.N)
+                *reinterpret_cast<uint4*>(p.C + row * p.ldc + col + 8 * j) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
               store_unit(lane_at + bo, j, w[0], w[1], w[2], w[3]);
             }
           });
@@ -665,7 +695,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           uint32_t acc[32];
           tmem_ld32(acc_at, acc);
           loaded(c);
-          if (splits > 1) {
+          if (p.parts) {
             // fp32 parts, 16 columns to a tile
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -749,9 +779,10 @@ ffn_sum_kernel(const float* __restrict__ parts, int splits, int M, int pitch, bf
 }
 
 // Copies of matrices whose rows TMA cannot read, all of a call in one launch: dst[r, c] = src[r, c] for c < cols, 0 up to
-// `width`, a multiple of 4 bytes in rows that are 4-byte aligned.  A warp takes rows in turn, a lane a word of the copy.
+// `width`, a multiple of 4 bytes in rows that are 4-byte aligned.  A warp takes runs of kRun words of a row in turn, a lane a
+// word of the copy (whole rows: 15 us for 16 of 2048 columns, four times).
 struct Copies {
-  static constexpr int kMost = 6;
+  static constexpr int kMost = 7, kRun = 128;
   struct Job {
     const void* src;
     void* dst;
@@ -768,10 +799,14 @@ repitch_kernel(const __grid_constant__ Copies c) {
   const Copies::Job& job = c.job[j];
   const int lane = threadIdx.x % 32, blocks = c.first_block[j + 1] - c.first_block[j];
   const int per = 4 / job.size;  // elements of a word
-  for (int64_t r = int64_t(blockIdx.x - c.first_block[j]) * 8 + threadIdx.x / 32; r < job.rows; r += int64_t(blocks) * 8) {
+  const int words = job.width / per, runs = (words + Copies::kRun - 1) / Copies::kRun;
+  for (int64_t i = int64_t(blockIdx.x - c.first_block[j]) * 8 + threadIdx.x / 32; i < job.rows * runs; i += int64_t(blocks) * 8) {
+    const int64_t r = i / runs;
+    const int from = int(i - r * runs) * Copies::kRun, to = min(words, from + Copies::kRun);
     const uint8_t* src = static_cast<const uint8_t*>(job.src) + r * job.lds * job.size;
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(job.dst) + r * job.ldd * job.size);
-    for (int w = lane; w < job.width / per; w += 32) {
+#pragma unroll 4
+    for (int w = from + lane; w < to; w += 32) {
       uint32_t word = 0;
       if (job.size == 2) {
 #pragma unroll
@@ -851,9 +886,13 @@ Split plan_plain(int64_t M, int64_t N, int64_t K) {
   return s;
 }
 inline int64_t part_pitch(int64_t N) { return (N + 3) & ~int64_t(3); }
-size_t plain_workspace(int64_t M, int64_t N, int64_t K) {
+// Rows of which A, dG and dU are kept in two bf16 numbers each, [hi; lo].
+constexpr int64_t kStacked = BM / 2;
+int64_t stack(int64_t M) { return M <= kStacked ? 2 : 1; }
+size_t plain_workspace(int64_t M, int64_t N, int64_t K, int64_t halves = 1) {
+  M *= halves;
   const Split s = plan_plain(M, N, K);
-  return s.splits > 1 ? align256(size_t(s.splits) * size_t(M) * size_t(part_pitch(N)) * 4) : 0;
+  return s.splits > 1 || halves > 1 ? align256(size_t(s.splits) * size_t(M) * size_t(part_pitch(N)) * 4) : 0;
 }
 
 int error_word(int** word) {
@@ -872,10 +911,10 @@ int error_word(int** word) {
   return GC_OK;
 }
 
-template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES>
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES, bool LO = false>
 int launch_kernel(const Maps& maps, const Params& p, cudaStream_t st) {
   using C_ = Cfg<KIND, BN, F8, PAIR, RES>;
-  auto kern = ffn_kernel<KIND, BN, A_MN, B_MN, F8, PAIR, RES>;
+  auto kern = ffn_kernel<KIND, BN, A_MN, B_MN, F8, PAIR, RES, LO>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::kSmemBytes);
   if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   constexpr int kCtas = PAIR ? 2 : 1;
@@ -903,9 +942,17 @@ int launch_tile(const Tile& t, const Maps& maps, const Params& p, cudaStream_t s
     if (t.pair && gc::ceil_div(p.K, F8 ? 128 : 64) <= kResident)
       return launch_kernel<KIND, 256, A_MN, B_MN, F8, true, true>(maps, p, st);
   if (t.pair) return launch_kernel<KIND, 256, A_MN, B_MN, F8, true, false>(maps, p, st);
-  if constexpr (KIND != kGated)
-    if (t.bn == 64) return launch_kernel<KIND, 64, A_MN, B_MN, F8, false, false>(maps, p, st);
-  return launch_kernel<KIND, 128, A_MN, B_MN, F8, false, false>(maps, p, st);
+  auto single = [&](auto bn, auto lo) {
+    return launch_kernel<KIND, decltype(bn)::value, A_MN, B_MN, F8, false, false, decltype(lo)::value>(maps, p, st);
+  };
+  auto width = [&](auto lo) {
+    if constexpr (KIND != kGated)
+      if (t.bn == 64) return single(std::integral_constant<int, 64>{}, lo);
+    return single(std::integral_constant<int, 128>{}, lo);
+  };
+  if constexpr (KIND != kPlain)
+    if (p.C) return width(std::true_type{});
+  return width(std::false_type{});
 }
 
 // The maps of the operands.  A and B: matrices as they lie; K-major ones have K in their rows.
@@ -920,10 +967,12 @@ int operand_maps(Maps& maps, Params& p, const Matrix& A, bool a_mn, const Matrix
   return rc;
 }
 
-// C (M x N, bf16) = A B, fp32 sums.
+// C (M x N, bf16) = A B, fp32 sums; `halves`: A has that many times M rows, and M apart are added.
 int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int64_t N, int64_t K, bf16* C, int64_t ldc,
-          int64_t gap_from, int64_t gap, void* workspace, cudaStream_t st) {
+          int64_t gap_from, int64_t gap, void* workspace, cudaStream_t st, int64_t halves = 1) {
   if (M == 0 || N == 0) return GC_OK;
+  const int64_t out_rows = M;
+  M *= halves;
   const Split s = plan_plain(M, N, K);
   Maps maps;
   Params p{};
@@ -933,20 +982,21 @@ int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int
   p.gap = int(gap);
   p.c_cols = int(N - 2 * gap);  // [G | U] with the pads behind both
   p.splits = s.splits; p.kb_per_split = s.per;
+  p.parts = s.splits > 1 || halves > 1;
   p.tma_store = gap == 0 && ldc % 8 == 0 && gc::aligned16(C);
   int rc = error_word(&p.word);
   if (rc == GC_OK) rc = operand_maps(maps, p, A, a_mn, B, b_mn, s.tile.pair ? s.tile.bn / 2 : s.tile.bn);
   const int64_t pitch = part_pitch(N);
-  if (rc == GC_OK && s.splits > 1) rc = make_map(&maps.out, Matrix{workspace, M, N, pitch, 4}, 16, 32, s.splits);
+  if (rc == GC_OK && p.parts) rc = make_map(&maps.out, Matrix{workspace, M, N, pitch, 4}, 16, 32, s.splits);
   else if (rc == GC_OK && p.tma_store) rc = make_map(&maps.out, Matrix{C, M, N, ldc, 2}, 32, 32);
   if (rc != GC_OK) return rc;
   if (a_mn) rc = launch_tile<kPlain, true, true, false>(s.tile, maps, p, st);
   else if (b_mn) rc = launch_tile<kPlain, false, true, false>(s.tile, maps, p, st);
   else rc = launch_tile<kPlain, false, false, false>(s.tile, maps, p, st);
-  if (rc != GC_OK || s.splits == 1) return rc;
-  const int64_t quads = M * (pitch / 4);
+  if (rc != GC_OK || !p.parts) return rc;
+  const int64_t quads = out_rows * (pitch / 4);
   ffn_sum_kernel<<<unsigned(std::min<int64_t>(gc::ceil_div(quads, 256), gc::kNumSMs * 8)), 256, 0, st>>>(
-      static_cast<const float*>(workspace), s.splits, int(M), int(pitch), C, ldc, p.c_cols, p.gap_from, p.gap);
+      static_cast<const float*>(workspace), int(s.splits * halves), int(out_rows), int(pitch), C, ldc, p.c_cols, p.gap_from, p.gap);
   return gc::check_launch("ffn_sum_kernel");
 }
 
@@ -957,7 +1007,8 @@ size_t copy_bytes(const Matrix& m) { return readable(m) ? 0 : align256(size_t(m.
 void add_copy(Copies& c, const Matrix& m, void* dst, int64_t ldd, int64_t width) {
   const int j = c.count++;
   c.job[j] = {m.p, dst, m.ld, ldd, m.rows, int(m.cols), int(width), m.size};
-  const int64_t blocks = std::min<int64_t>(gc::ceil_div(m.rows, 8), gc::kNumSMs * 8);
+  const int64_t runs = gc::ceil_div(width * m.size / 4, Copies::kRun);
+  const int64_t blocks = std::min<int64_t>(gc::ceil_div(m.rows * runs, 8), gc::kNumSMs * 8);
   c.first_block[0] = 0;
   c.first_block[j + 1] = c.first_block[j] + int(blocks);
 }
@@ -969,6 +1020,14 @@ void make_readable(Matrix& m, char*& ws, Copies& c) {
   m.p = ws;
   m.ld = ld;
   ws += bytes;
+}
+// A copy of m on top of itself.
+Matrix stacked(const Matrix& m, char*& ws, Copies& c) {
+  const int64_t ld = readable_ld(m);
+  const Matrix two{ws, 2 * m.rows, m.cols, ld, m.size};
+  for (int i = 0; i < 2; ++i) add_copy(c, m, ws + i * m.rows * ld * m.size, ld, ld);
+  ws += align256(size_t(two.rows) * size_t(ld) * m.size);
+  return two;
 }
 // [Wg | Wu]: where H is not a multiple of 8, U's columns are moved to the next one, and the columns between are zeros -- as are
 // then those of G, U, A and their gradients.
@@ -995,7 +1054,7 @@ Saved saved_at(void* p, int64_t M, int64_t H) {
   char* c = static_cast<char*>(p);
   Saved s;
   s.hidden = reinterpret_cast<uint16_t*>(c);
-  c += align256(size_t(M) * hp * 2);
+  c += align256(size_t(stack(M) * M) * hp * 2);
   s.gate_up = reinterpret_cast<uint16_t*>(c);
   s.exps = reinterpret_cast<int8_t*>(c + align256(size_t(M) * hp * 4));
   return s;
@@ -1008,8 +1067,9 @@ bool few_rows(int64_t M, int64_t D, int64_t H, int64_t O, bool in_place) {
   return M == 1 || (M <= kFewRows && (!in_place || 2 * (2 * D * H + H * O) <= (int64_t(16) << 20)));
 }
 
-// Room for the product between the two launches: fp32 in the form for few rows.
-size_t hidden_bytes(int64_t M, int64_t hp) { return align256(size_t(M) * hp * (M <= kFewRows ? 4 : 2)); }
+// Room for the product between the two launches: fp32, or [hi; lo], up to kStacked rows.
+size_t hidden_bytes(int64_t M, int64_t hp) { return align256(size_t(stack(M) * M) * hp * 2); }
+static_assert(kFewRows <= kStacked, "the form for few rows has room for fp32");
 
 bool sizes_ok(int64_t M, int64_t D, int64_t H, int64_t O) {
   const int64_t top = (int64_t(1) << 31) - 512;  // coordinates and tile counts are 32-bit
@@ -1023,17 +1083,18 @@ extern "C" {
 size_t gc_gated_ffn_saved_bytes(int64_t M, int64_t H) {
   if (M <= 0 || H <= 0) return 0;
   const int64_t hp = up8(H);
-  return align256(size_t(M) * hp * 2) + align256(size_t(M) * hp * 4) + align256(2 * size_t(gc::ceil_div(hp, 32)) * size_t(M));
+  return align256(size_t(stack(M) * M) * hp * 2) + align256(size_t(M) * hp * 4) + align256(2 * size_t(gc::ceil_div(hp, 32)) * size_t(M));
 }
 
 size_t gc_gated_ffn_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O, int backward) {
   if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, D, H, O)) return 0;
   const int64_t hp = up8(H);
   // copies of every operand, should none be readable in place
-  size_t b = align256(size_t(M) * up8(D) * 2) + align256(size_t(D) * 2 * hp * 2) + align256(size_t(H) * up8(O) * 2);
-  if (!backward) return b + hidden_bytes(M, hp) + plain_workspace(M, O, H);
-  b += align256(size_t(M) * up8(O) * 2) + align256(size_t(M) * 2 * hp * 2);  // dY, dG | dU
-  return b + std::max({plain_workspace(M, D, 2 * hp), plain_workspace(D, 2 * hp, M), plain_workspace(H, O, M)});
+  const int64_t halves = stack(M), rows = halves * M;
+  size_t b = align256(size_t(rows) * up8(D) * 2) + align256(size_t(D) * 2 * hp * 2) + align256(size_t(H) * up8(O) * 2);
+  if (!backward) return b + hidden_bytes(M, hp) + plain_workspace(M, O, H, halves);
+  b += align256(size_t(rows) * up8(O) * 2) + align256(size_t(rows) * 2 * hp * 2);  // dY, dG | dU
+  return b + std::max({plain_workspace(M, D, 2 * hp, halves), plain_workspace(D, 2 * hp, rows), plain_workspace(H, O, rows)});
 }
 
 int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin, const uint16_t* Wout,
@@ -1077,8 +1138,9 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
     keep = saved_at(saved, M, H);
     hidden = keep.hidden;
   } else {
-    ws += align256(size_t(M) * hp * 2);
+    ws += hidden_bytes(M, hp);
   }
+  const int64_t halves = stack(M);
   const Tile t = pick_tile(kGated, M, hp, 1);
   Maps maps;
   Params p{};
@@ -1086,6 +1148,8 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   p.b_up = int(hp);
   p.act = act;
   p.exps = keep.exps;
+  p.C = halves > 1 ? reinterpret_cast<bf16*>(hidden) + M * hp : nullptr;
+  p.ldc = hp;
   rc = error_word(&p.word);
   if (rc == GC_OK) rc = operand_maps(maps, p, x, false, win, true, 0);
   if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, hp, hp, 2}, 32, 32);
@@ -1093,7 +1157,7 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   if (rc == GC_OK && saved) rc = make_map(&maps.out3, Matrix{keep.gate_up + hp, M, hp, 2 * hp, 2}, 32, 32);
   if (rc == GC_OK) rc = launch_tile<kGated, false, true, false>(t, maps, p, st);
   if (rc != GC_OK) return rc;
-  return plain(Matrix{hidden, M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
+  return plain(Matrix{hidden, halves * M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st, halves);
 }
 
 int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* Win,
@@ -1128,23 +1192,34 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
   char* ws = static_cast<char*>(workspace);
   Matrix dy{dY, M, O, lddy, 2}, x{X, M, D, ldx, 2}, win{Win, D, 2 * H, ldwin, 2}, wout{Wout, H, O, ldwout, 2};
   Copies copies{};
-  make_readable(dy, ws, copies);
-  if (dWin) make_readable(x, ws, copies);
+  const int64_t halves = stack(M), rows = halves * M;
+  Matrix dy_rows = dy;  // as the weight gradients take it and x
+  if (halves > 1) {
+    dy_rows = stacked(dy, ws, copies);
+    dy = Matrix{dy_rows.p, M, O, dy_rows.ld, 2};
+    if (dWin) x = stacked(x, ws, copies);
+  } else {
+    make_readable(dy, ws, copies);
+    dy_rows = dy;
+    if (dWin) make_readable(x, ws, copies);
+  }
   if (dX) make_gate_up(win, H, ws, copies);
   if (dX || dWin) make_readable(wout, ws, copies);
   int rc = run_copies(copies, st);
   if (rc != GC_OK) return rc;
   const Saved kept = saved_at(const_cast<void*>(saved), M, H);
-  const Matrix dgu{ws, M, 2 * hp, 2 * hp, 2};
+  const Matrix dgu{ws, rows, 2 * hp, 2 * hp, 2};
   if (dX || dWin) {
     uint16_t* out = reinterpret_cast<uint16_t*>(ws);
-    ws += align256(size_t(M) * 2 * hp * 2);
+    ws += align256(size_t(rows) * 2 * hp * 2);
     const Tile t = pick_tile(kGatedBack, M, hp, 1);
     Maps maps;
     Params p{};
     p.M = int(M); p.N = int(hp); p.K = int(O);
     p.act = act;
     p.exps = kept.exps;
+    p.C = halves > 1 ? reinterpret_cast<bf16*>(out) + M * 2 * hp : nullptr;
+    p.ldc = 2 * hp;
     rc = error_word(&p.word);
     if (rc == GC_OK) rc = operand_maps(maps, p, dy, false, wout, false, t.pair ? t.bn / 2 : t.bn);
     if (rc == GC_OK) rc = make_map(&maps.in1, Matrix{kept.gate_up, M, hp, 2 * hp, 2}, 32, 32);
@@ -1154,11 +1229,11 @@ int gc_gated_ffn_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t*
     if (rc == GC_OK) rc = launch_tile<kGatedBack, false, false, false>(t, maps, p, st);
     if (rc != GC_OK) return rc;
   }
-  if (dX) rc = plain(dgu, false, win, false, M, D, 2 * hp, reinterpret_cast<bf16*>(dX), lddx, 0, 0, ws, st);
+  if (dX) rc = plain(dgu, false, win, false, M, D, 2 * hp, reinterpret_cast<bf16*>(dX), lddx, 0, 0, ws, st, halves);
   if (rc == GC_OK && dWin)
-    rc = plain(x, true, dgu, true, D, 2 * hp, M, reinterpret_cast<bf16*>(dWin), lddwin, H, hp - H, ws, st);
+    rc = plain(x, true, dgu, true, D, 2 * hp, rows, reinterpret_cast<bf16*>(dWin), lddwin, H, hp - H, ws, st);
   if (rc == GC_OK && dWout)
-    rc = plain(Matrix{kept.hidden, M, H, hp, 2}, true, dy, true, H, O, M, reinterpret_cast<bf16*>(dWout), lddwout, 0, 0, ws, st);
+    rc = plain(Matrix{kept.hidden, rows, H, hp, 2}, true, dy_rows, true, H, O, rows, reinterpret_cast<bf16*>(dWout), lddwout, 0, 0, ws, st);
   return rc;
 }
 
@@ -1166,7 +1241,7 @@ size_t gc_gated_ffn_e4m3_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_
   if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, D, H, O)) return 0;
   const int64_t d16 = (D + 15) / 16 * 16;
   return align256(size_t(M) * d16) + align256(size_t(2 * H) * d16) + align256(size_t(H) * up8(O) * 2) +
-         hidden_bytes(M, up8(H)) + plain_workspace(M, O, H);
+         hidden_bytes(M, up8(H)) + plain_workspace(M, O, H, stack(M));
 }
 
 int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_scale, const uint8_t* W8, int64_t ldw,
@@ -1204,7 +1279,8 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   if (rc != GC_OK) return rc;
   const int64_t hp = up8(H);
   uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);
-  ws += align256(size_t(M) * hp * 2);
+  ws += hidden_bytes(M, hp);
+  const int64_t halves = stack(M);
   const Tile t = pick_tile(kGated, M, H, 1);
   Maps maps;
   Params p{};
@@ -1213,12 +1289,14 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   p.act = act;
   p.sa = x_scale;
   p.sb = w_scale;
+  p.C = halves > 1 ? reinterpret_cast<bf16*>(hidden) + M * hp : nullptr;
+  p.ldc = hp;
   rc = error_word(&p.word);
   if (rc == GC_OK) rc = operand_maps(maps, p, x, false, w, false, t.bn / 2);
   if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 32, 32);
   if (rc == GC_OK) rc = launch_tile<kGated, false, false, true>(t, maps, p, st);
   if (rc != GC_OK) return rc;
-  return plain(Matrix{hidden, M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
+  return plain(Matrix{hidden, halves * M, H, hp, 2}, false, wout, true, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st, halves);
 }
 
 }  // extern "C"

@@ -96,7 +96,7 @@ __device__ __forceinline__ void with_activation(int act, F&& f) {
 // What a forward pass leaves for the backward pass, in one buffer: G and U are kept as fp16 numbers with an exponent for every
 // 32 columns of a row: eight times as exact as bf16 in as many bits, over the same range.
 struct Saved {
-  uint16_t* hidden;   // M x P bf16, P = H rounded up to a multiple of 8
+  uint16_t* hidden;   // M x P bf16, P = H rounded up to a multiple of 8; for few rows what its rounding left follows, M x P
   uint16_t* gate_up;  // M x 2P
   int8_t* exps;       // [2][ceil(P / 32)][M]
 };

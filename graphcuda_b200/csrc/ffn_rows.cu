@@ -187,7 +187,12 @@ ffn_rows_kernel(const std::conditional_t<GATED, bf16, float>* __restrict__ x, in
       if constexpr (GATED) {
         const float h = gated(a, u, act);
         out[int64_t(m) * ldo + col] = h;
-        if (keep.hidden) reinterpret_cast<bf16*>(keep.hidden)[int64_t(m) * ldo + col] = __float2bfloat16_rn(h);
+        if (keep.hidden) {  // [hi; lo]; nothing is left of what is not finite
+          bf16* at = reinterpret_cast<bf16*>(keep.hidden) + int64_t(m) * ldo + col;
+          const bf16 hi = __float2bfloat16_rn(h);
+          at[0] = hi;
+          at[int64_t(M) * ldo] = __float2bfloat16_rn(isfinite(__bfloat162float(hi)) ? h - __bfloat162float(hi) : 0.f);
+        }
       } else {
         out[int64_t(m) * ldo + col] = __float2bfloat16_rn(a);
       }

@@ -492,7 +492,8 @@ int gc_rms_norm_backward(const void* dy, int dy_type, int64_t lddy, const void* 
  * activation's product is rounded to bf16 on its way into the second product.  Rows whose pitch is not a multiple of 16 bytes, and
  * an H that is not a multiple of 8, are copied to such in the workspace.
  * saved: gc_gated_ffn_saved_bytes(M, H) bytes, 16-byte aligned, that the forward call fills for the backward call (6 M H
- * bytes and a little: the activation's product, X Wg and X Wu); null where there will be none.
+ * bytes and a little: the activation's product, X Wg and X Wu; 8 M H up to 64 rows, where the product is kept in two numbers, as
+ * few values' roundings do not average out); null where there will be none.
  * backward, with G = X Wg, U = X Wu, dA = dY Wo^T:  [dG | dU] = [dA U act'(G) | dA act(G)],  dX = [dG | dU] Win^T,
  * dWin = X^T [dG | dU],  dWout = (act(G) U)^T dY.  dX, dWin and dWout may be null (not computed).  Sums along K in a fixed order.
  * A wait that ran out is told by gc_gemm_error_word's word.

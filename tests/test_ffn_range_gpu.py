@@ -67,6 +67,31 @@ def test_magnitudes_far_from_one(cuda, shape, power):
     ops.check_gemm_flag(cuda)
 
 
+@pytest.mark.parametrize("m", [1, 3, 9, 33, 64])
+@pytest.mark.parametrize("shape", [(25, 68, 2336), (128, 76, 1416), (264, 1032, 40), (2048, 1111, 513)], ids=str)
+def test_few_rows_round_their_outputs_alone(cuda, m, shape):
+    """Up to 64 rows, A and the gradients of G and U are kept to 16 bits and more (two bf16 numbers): the outputs' own rounding is
+    left, and, of gradients, what G and U are off by, 2^-12 of the largest of 32 columns."""
+    d, h, o = shape
+    t = [v.bfloat16() for v in (_randn(m, d), _randn(d, 2 * h, seed=1) / d ** 0.5, _randn(h, o, seed=2) / h ** 0.5, _randn(m, o, seed=3))]
+    x, w_in, w_out, dy = (v.double() for v in t)
+    g, u = x @ w_in[:, :h], x @ w_in[:, h:]
+    a, slope = g.clamp(min=0), (g > 0).double()
+    hid, da = a * u, dy @ w_out.t()
+    dgu = torch.cat((da * u * slope, da * a), 1)
+    pad = -h % 32
+    top = lambda v: torch.nn.functional.pad(v.abs(), (0, pad)).view(m, -1, 32).amax(2).repeat_interleave(32, 1)[:, :h]  # noqa: E731
+    e = torch.cat((da.abs() * top(u) * slope, da.abs() * top(g)), 1) / 8
+    either = torch.cat((da * u * (g.abs() < top(g) * 2.0 ** -15), torch.zeros_like(da)), 1).abs()
+    ref = (hid @ w_out, dgu @ w_in.t(), x.t() @ dgu, hid.t() @ dy)
+    # two bf16 numbers: 2^-17 of the value; fp32 sums add as much
+    parts = (hid.abs() @ w_out.abs(), dgu.abs() @ w_in.abs().t(), x.abs().t() @ dgu.abs(), hid.abs().t() @ dy.abs())
+    noise = (0.0, (e.square() @ w_in.square().t()).sqrt(), (x.square().t() @ e.square()).sqrt(), 0.0)
+    loose = (0.0, either @ w_in.abs().t(), x.abs().t() @ either, 0.0)
+    tol = [U * (r.abs() + 3.5 * n) + 2.0 ** -16 * p + o + 1e-37 for r, n, p, o in zip(ref, noise, parts, loose)]
+    _check(_gradients(*t), ref, tol)
+
+
 @pytest.mark.parametrize("m", [1, 6, 200])
 @pytest.mark.parametrize("h", [40, 100, 1032])
 @pytest.mark.parametrize("value", [float("inf"), float("nan"), 2.0 ** 120])
