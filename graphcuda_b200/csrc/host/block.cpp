@@ -160,6 +160,17 @@ uint16_t* bits_mut(const Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()
 bool bf16_matrix(const Tensor& t, const at::Device& dev) {
   return t.dim() == 2 && t.device() == dev && t.scalar_type() == at::kBFloat16;
 }
+// Beyond a few megabytes the workspace holds matrices of the size of activations (700 MB at 169,343 rows of 1024): the call's own
+// memory then, which the next layer can have when the call has ended.
+Scratch ffn_workspace(size_t bytes, const at::Device& dev) {
+  constexpr size_t kKept = size_t(32) << 20;
+  if (bytes <= kKept) return scratch(kGemm, bytes, dev);
+  Scratch s;
+  s.keep = at::empty({int64_t(bytes)}, at::TensorOptions().dtype(at::kByte).device(dev));
+  s.ptr = s.keep.data_ptr();
+  s.bytes = bytes;
+  return s;
+}
 FfnSizes ffn_sizes(const Tensor& x, const Tensor& w_in, const Tensor& w_out) {
   require(x.is_cuda() && bf16_matrix(x, x.device()), "gated_ffn: x must be a bfloat16 CUDA matrix");
   require(bf16_matrix(w_in, x.device()) && w_in.size(0) == x.size(1) && w_in.size(1) % 2 == 0,
@@ -181,7 +192,7 @@ FfnForward gated_ffn_forward(const Tensor& xin, const Tensor& w_in, const Tensor
   f.y = empty_like_rows(n.M, n.O, at::kBFloat16, dev);
   if (save)
     f.saved = at::empty({int64_t(abi.gc_gated_ffn_saved_bytes(n.M, n.H))}, at::TensorOptions().dtype(at::kByte).device(dev));
-  const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 0), dev);
+  const Scratch ws = ffn_workspace(abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 0), dev);
   check(abi.gc_gated_ffn_forward_bf16(bits(f.x), ld_of(f.x), bits(f.w_in), ld_of(f.w_in), bits(f.w_out), ld_of(f.w_out),
                                       n.M, n.D, n.H, n.O, act, bits_mut(f.y), std::max<int64_t>(n.O, 1),
                                       save ? f.saved.data_ptr() : nullptr, ws.ptr, ws.bytes, stream_of(dev)),
@@ -199,7 +210,7 @@ FfnGrads gated_ffn_backward(const Tensor& dy_in, const Tensor& x, const Tensor& 
   if (need_dx) g.dx = empty_like_rows(n.M, n.D, at::kBFloat16, dev);
   if (need_dw_in) g.dw_in = empty_like_rows(n.D, 2 * n.H, at::kBFloat16, dev);
   if (need_dw_out) g.dw_out = empty_like_rows(n.H, n.O, at::kBFloat16, dev);
-  const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 1), dev);
+  const Scratch ws = ffn_workspace(abi.gc_gated_ffn_workspace_bytes(n.M, n.D, n.H, n.O, 1), dev);
   check(abi.gc_gated_ffn_backward_bf16(
             bits(dy), ld_of(dy), bits(x), ld_of(x), bits(w_in), ld_of(w_in), bits(w_out), ld_of(w_out),
             saved.const_data_ptr(), n.M, n.D, n.H, n.O, act, need_dx ? bits_mut(g.dx) : nullptr, std::max<int64_t>(n.D, 1),
@@ -255,7 +266,7 @@ Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, 
   const Tensor x = row_major(x8), w = row_major(w8), wo = row_major(w_out);
   const Tensor sx = x_scale.contiguous(), sw = w_scale.contiguous();
   Tensor y = empty_like_rows(M, O, at::kBFloat16, dev);
-  const Scratch ws = scratch(kGemm, abi.gc_gated_ffn_e4m3_workspace_bytes(M, D, H, O), dev);
+  const Scratch ws = ffn_workspace(abi.gc_gated_ffn_e4m3_workspace_bytes(M, D, H, O), dev);
   check(abi.gc_gated_ffn_forward_e4m3(static_cast<const uint8_t*>(x.const_data_ptr()), ld_of(x), sx.const_data_ptr<float>(),
                                       static_cast<const uint8_t*>(w.const_data_ptr()), ld_of(w), sw.const_data_ptr<float>(),
                                       bits(wo), ld_of(wo), M, D, H, O, int(act), bits_mut(y), std::max<int64_t>(O, 1),

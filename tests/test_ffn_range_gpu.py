@@ -172,6 +172,15 @@ def test_offsets_beyond_32_bits(cuda, give_memory_back):
         assert float((a - b).detach().float().abs().max()) <= 2.0 ** -7 * float(b.detach().float().abs().max())
 
 
+def test_large_workspaces_go_back(cuda):
+    """What a call needs between its kernels is not held when it has ended, nor is what it kept for a backward pass that is over."""
+    t = [v.bfloat16() for v in (_randn(60_000, 64), _randn(64, 1024, seed=1) / 8, _randn(512, 64, seed=2) / 16, _randn(60_000, 64, seed=3))]
+    before = torch.cuda.memory_allocated()
+    got = _gradients(*t)
+    del got
+    assert torch.cuda.memory_allocated() - before < 64 << 20
+
+
 def test_buffers_are_as_large_as_asked_for(cuda):
     """Nothing is written behind what is kept and behind the workspace."""
     from graphcuda_b200 import _lib
