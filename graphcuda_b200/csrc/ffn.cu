@@ -1060,11 +1060,17 @@ Saved saved_at(void* p, int64_t M, int64_t H) {
   return s;
 }
 
-// Whether a forward pass takes the form for few rows.  Measured against this file's, us: weights of 100 MB 27 / 38 at one row
-// (both from memory), 30 / 29 at two, 34 / 29 at four; of 1.5 MB 7 / 13 at one, 10 / 13 at eight; of 4 MB at odd widths, which
-// this file's would copy first, 13 / 29 at one, 17 / 29 at eight.
-bool few_rows(int64_t M, int64_t D, int64_t H, int64_t O, bool in_place) {
-  return M == 1 || (M <= kFewRows && (!in_place || 2 * (2 * D * H + H * O) <= (int64_t(16) << 20)));
+// Whether a forward pass takes the form for few rows, of which its time depends as on the weights' bytes, while this file's
+// hardly depends on the rows.  Measured, that form / this file's, us by the call:
+//   bf16 in place      12 MB  10 / 21 at two rows, 12 / 21 at four, 31 / 21 at eight;   3 MB  19 / 19 at eight
+//                      48 MB  21 / 31            , 25 / 31        , 70 / 31         ;  96 MB  33 / 35, 39 / 36, 94 / 36
+//   odd widths, which  12 MB  16 / 33            , 19 / 33        , 47 / 33         ;   4 MB  20 / 29 at eight
+//   this file copies   47 MB  55 / 66            , 58 / 66        , 176 / 66
+//   e4m3               12 MB  10 / 19            , 10 / 19        , 19 / 19         ;   6 MB  14 / 18 at eight
+//                      48 MB  14 / 27            , 19 / 27        , 39 / 27         ;  96 MB  24 / 32, 30 / 32, 62 / 32
+bool few_rows(int64_t M, int64_t D, int64_t H, int64_t O, bool bf16_in_place) {
+  const double weights = 2.0 * double(H) * (2.0 * double(D) + double(O)), mb = 1 << 20;
+  return M <= 2 || (M <= 4 && weights <= 64 * mb) || (M <= kFewRows && weights <= (bf16_in_place ? 3 : 6) * mb);
 }
 
 // Room for the product between the two launches: fp32, or [hi; lo], up to kStacked rows.
@@ -1266,7 +1272,7 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_e4m3: workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Matrix x{X8, M, D, ldx, 1}, w{W8, 2 * H, D, ldw, 1}, wout{Wout, H, O, ldwout, 2};
-  if (few_rows(M, D, H, O, readable(w) && readable(wout))) {
+  if (few_rows(M, D, H, O, false)) {
     const Rows r{X8, W8, Wout, x_scale, w_scale, reinterpret_cast<float*>(ws), Y, ldx, ldw, ldwout, up8(H), ldy, int(M), int(D),
                  int(H), int(O), act, Saved{}};
     return forward_few_rows(r, true, st);
