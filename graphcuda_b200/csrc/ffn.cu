@@ -56,6 +56,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace {
 
@@ -896,17 +897,14 @@ size_t plain_workspace(int64_t M, int64_t N, int64_t K, int64_t halves = 1) {
 }
 
 int error_word(int** word) {
-  static int* cached[64] = {};  // by device; the address does not change
+  static std::atomic<int*> cached[64] = {};  // by device; the address does not change
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return gc::fail(GC_ERR_CUDA, "no current device");
-  if (dev < 64 && cached[dev]) {
-    *word = cached[dev];
-    return GC_OK;
-  }
+  if (dev < 64 && (*word = cached[dev].load(std::memory_order_relaxed))) return GC_OK;
   int32_t* w = nullptr;
   const int rc = gc::wait_error_word(&w);
   if (rc != GC_OK) return rc;
-  if (dev < 64) cached[dev] = w;
+  if (dev < 64) cached[dev].store(w, std::memory_order_relaxed);
   *word = w;
   return GC_OK;
 }
