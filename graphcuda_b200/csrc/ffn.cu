@@ -230,7 +230,8 @@ __device__ __forceinline__ void load_8(uint32_t at, F2 (&v)[4]) {
     asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v[2 * j].v), "=l"(v[2 * j + 1].v) : "r"(at + 16 * j) : "memory");
 }
 
-// 32 values to a row of a tile as fp16 with a common power of two, which is returned.
+// 32 values to a row of a tile as fp16 with a common power of two, which is returned.  SIGN: see stay_positive.
+template <bool SIGN>
 __device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t lane_at) {
   __half2 top[2] = {__float2half2_rn(0.f), __float2half2_rn(0.f)};
 #pragma unroll
@@ -238,7 +239,8 @@ __device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t lane_
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const __half2 h = __floats2half2_rn(__uint_as_float(v[j * 8 + 2 * e]), __uint_as_float(v[j * 8 + 2 * e + 1]));
+      const float x = __uint_as_float(v[j * 8 + 2 * e]), y = __uint_as_float(v[j * 8 + 2 * e + 1]);
+      const __half2 h = SIGN ? __floats2half2_rn(stay_positive(x), stay_positive(y)) : __floats2half2_rn(x, y);
       top[e & 1] = __hmax2(top[e & 1], __habs2(h));
       w[e] = *reinterpret_cast<const uint32_t*>(&h);
     }
@@ -258,7 +260,8 @@ __device__ __forceinline__ int pack_fp16(const uint32_t (&v)[32], uint32_t lane_
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = j * 8 + 2 * k;
-      const __half2 h = __floats2half2_rn(__uint_as_float(v[i]) * f.x * f.y, __uint_as_float(v[i + 1]) * f.x * f.y);
+      const float x = __uint_as_float(v[i]) * f.x * f.y, y = __uint_as_float(v[i + 1]) * f.x * f.y;
+      const __half2 h = SIGN ? __floats2half2_rn(stay_positive(x), stay_positive(y)) : __floats2half2_rn(x, y);
       w[k] = *reinterpret_cast<const uint32_t*>(&h);
     }
     store_unit(lane_at, j, w[0], w[1], w[2], w[3]);
@@ -656,10 +659,10 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
                 if (col + i >= p.N) g[i] = u[i] = 0;
             }
             const uint32_t bg = acquire();
-            const int eg = pack_fp16(g, lane_at + bg);
+            const int eg = p.act == GC_ACT_RELU ? pack_fp16<true>(g, lane_at + bg) : pack_fp16<false>(g, lane_at + bg);
             put(&maps.out2, bg, col, row0);
             const uint32_t bu = acquire();
-            const int eu = pack_fp16(u, lane_at + bu);
+            const int eu = pack_fp16<false>(u, lane_at + bu);
             put(&maps.out3, bu, col, row0);
             if (row < p.M) {
               p.exps[at] = int8_t(eg);

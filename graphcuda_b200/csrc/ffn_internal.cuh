@@ -109,6 +109,9 @@ __device__ __forceinline__ int shared_exponent(uint32_t bits) {
   return max(int(bits >> 23) - 127 - 14, -126);
 }
 __device__ __forceinline__ bool fits_fp16(uint32_t most) { return most >= 0x1400u && most < 0x7C00u; }
+// What is positive stays so: the smallest fp16 number stands for less.  relu's slope hangs on it, and a value of G below 2^-25
+// beside one above 2^-10 would come back as zero.
+__device__ __forceinline__ float stay_positive(float v) { return v > 0.f ? fmaxf(v, 0x1p-24f) : v; }
 // 2^-e as two factors: alone it may not be a number.
 __device__ __forceinline__ float2 unscale(int e) {
   return make_float2(__uint_as_float(uint32_t(127 - e / 2) << 23), __uint_as_float(uint32_t(127 - (e - e / 2)) << 23));

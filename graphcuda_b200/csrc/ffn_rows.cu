@@ -45,14 +45,15 @@ __device__ __forceinline__ float peer_load(const float* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
   return v;
 }
-// One value per lane to fp16 with a power of two for the warp, which is returned.
-__device__ __forceinline__ int pack_fp16(float v, __half& out) {
-  out = __float2half_rn(v);
+// One value per lane to fp16 with a power of two for the warp, which is returned.  sign: see stay_positive.
+__device__ __forceinline__ int pack_fp16(float v, bool sign, __half& out) {
+  out = __float2half_rn(sign ? stay_positive(v) : v);
   const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, uint32_t(__half_as_ushort(out)) & 0x7FFFu);
   if (fits_fp16(most)) return 0;
   const int e = shared_exponent(__reduce_max_sync(0xFFFFFFFFu, finite_bits(__float_as_uint(v))));
   const float2 f = unscale(e);
-  out = __float2half_rn(v * f.x * f.y);
+  v = v * f.x * f.y;
+  out = __float2half_rn(sign ? stay_positive(v) : v);
   return e;
 }
 __device__ __forceinline__ float gated(float g, float u, int act) {
@@ -201,7 +202,7 @@ ffn_rows_kernel(const std::conditional_t<GATED, bf16, float>* __restrict__ x, in
       const int pitch = (N + 7) / 8 * 8;
       if (col >= N) a = u = 0.f;  // the pad columns take part in the backward pass as zeros
       __half hg, hu;
-      const int eg = pack_fp16(a, hg), eu = pack_fp16(u, hu);
+      const int eg = pack_fp16(a, act == GC_ACT_RELU, hg), eu = pack_fp16(u, false, hu);
       if (col < pitch) {
         __half* row = reinterpret_cast<__half*>(keep.gate_up) + int64_t(m) * 2 * pitch;
         row[col] = hg;

@@ -172,6 +172,30 @@ def test_offsets_beyond_32_bits(cuda, give_memory_back):
         assert float((a - b).detach().float().abs().max()) <= 2.0 ** -7 * float(b.detach().float().abs().max())
 
 
+@pytest.mark.parametrize("m", [1, 6, 9, 200, 3000])
+@pytest.mark.parametrize("scale", [0, 20, -20])
+def test_relu_of_next_to_nothing(cuda, m, scale):
+    """A G of 2^-30 beside ones about 1 (times a power of two) is positive, one of zero and one below are not: their gradients are
+    those of relu all the same."""
+    d, h, o = 64, 96, 64
+    x, w_in, w_out = _randn(m, d), _randn(d, 2 * h, seed=1) / 8, _randn(h, o, seed=2) / 8
+    x[:, 0] = 1.0
+    for column, value in ((1, 2.0 ** -30), (34, -2.0 ** -30), (70, 0.0), (95, 2.0 ** -40)):
+        w_in[:, column] = 0.0
+        w_in[0, column] = value
+    w_in[:, :h] *= 2.0 ** scale
+    t = [v.bfloat16() for v in (x, w_in, w_out, _randn(m, o, seed=3))]
+    got = _gradients(*t)
+    x, w_in, w_out, dy = (v.double() for v in t)
+    g, u, da = x @ w_in[:, :h], x @ w_in[:, h:], dy @ w_out.t()
+    dg = da * u * (g > 0)
+    tol = U * ((x.t() @ dg).abs() + 3.5 * (x.square().t() @ (dg * 1.2).square()).sqrt()) + 1e-37
+    cols = [1, 34, 70, 95]
+    over = (got[2][:, cols].double() - (x.t() @ dg)[:, cols]).abs() - tol[:, cols]
+    assert float(over.max()) <= 0
+    assert bool((got[2][:, [34, 70]] == 0).all()) and bool((got[2][:, [1, 95]] != 0).any())
+
+
 def test_large_workspaces_go_back(cuda):
     """What a call needs between its kernels is not held when it has ended, nor is what it kept for a backward pass that is over."""
     t = [v.bfloat16() for v in (_randn(60_000, 64), _randn(64, 1024, seed=1) / 8, _randn(512, 64, seed=2) / 16, _randn(60_000, 64, seed=3))]
