@@ -274,7 +274,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     if (torch::jit::tracer::isTracing()) return std::nullopt;
     return rms_norm(x, weight, residual, eps, y_type);
   }, NoGil());
-  m.def("rms_norm_fp8", &rms_norm_fp8, NoGil());
+  m.def("rms_norm_fp8", [](const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                           double eps) -> std::optional<std::tuple<Tensor, Tensor, Tensor>> {
+    refuse_norm_fp8_gradient(x, weight, residual);
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return rms_norm_fp8(x, weight, residual, eps);
+  }, NoGil());
+  m.def("rms_norm_fp8_forward", &rms_norm_fp8, NoGil());
   m.def("rms_norm_forward", [](const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps, int64_t y_type) {
     const NormForward f = rms_norm_forward(x, weight, residual, eps, int(y_type), true);
     return std::make_tuple(f.y, f.stream, norm_saved(f));
@@ -299,7 +305,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     const FfnGrads g = gated_ffn_backward(dy, x, w_in, w_out, saved, int(act), dx, dw_in, dw_out);
     return std::make_tuple(g.dx, g.dw_in, g.dw_out);
   }, NoGil());
-  m.def("gated_ffn_fp8", &gated_ffn_fp8, NoGil());
+  m.def("gated_ffn_fp8", [](const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale,
+                            const Tensor& w_out, int64_t act) -> OptTensor {
+    refuse_ffn_fp8_gradient(x_scale, w_scale, w_out);
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return gated_ffn_fp8(x8, x_scale, w8, w_scale, w_out, act);
+  }, NoGil());
+  m.def("gated_ffn_fp8_forward", &gated_ffn_fp8, NoGil());
   m.def("adamw_step", &adamw_step, NoGil());
   m.def("adamw_moments", &adamw_moments, NoGil());
 }

@@ -144,10 +144,13 @@ std::pair<Tensor, Tensor> rms_norm(const Tensor& x, const Tensor& weight, const 
 }
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& residual, double eps) {
-  if (recorded({&x, &weight, residual ? &*residual : nullptr}))
-    raise("rms_norm_fp8 has no gradient: call it under torch.no_grad(), or rms_norm for training");
   const NormForward f = rms_norm_forward(x, weight, residual, eps, GC_TYPE_E4M3, false);
   return {f.y, f.scale, f.stream};
+}
+
+void refuse_norm_fp8_gradient(const Tensor& x, const Tensor& weight, const OptTensor& residual) {
+  if (recorded({&x, &weight, residual ? &*residual : nullptr}))
+    raise("rms_norm_fp8 has no gradient: call it under torch.no_grad(), or rms_norm for training");
 }
 
 // ------------------------------------------------------------------ gated feed-forward block
@@ -259,8 +262,6 @@ Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, 
               w_scale.dim() == 1 && w_scale.size(0) == 2 * H,
           "gated_ffn_fp8: float32 scales expected, one per row of x8 and of w8, on their device");
   require(bf16_matrix(w_out, dev) && w_out.size(0) == H, "gated_ffn_fp8: w_out must be bfloat16 [hidden, out] on x8's device");
-  if (recorded({&w_out, &x_scale, &w_scale}))
-    raise("gated_ffn_fp8 has no gradient: call it under torch.no_grad(), or gated_ffn for training");
   const int64_t O = w_out.size(1);
   const c10::cuda::CUDAGuard guard(dev);
   const Tensor x = row_major(x8), w = row_major(w8), wo = row_major(w_out);
@@ -273,6 +274,11 @@ Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, 
                                       ws.ptr, ws.bytes, stream_of(dev)),
         "gc_gated_ffn_forward_e4m3");
   return y;
+}
+
+void refuse_ffn_fp8_gradient(const Tensor& x_scale, const Tensor& w_scale, const Tensor& w_out) {
+  if (recorded({&w_out, &x_scale, &w_scale}))
+    raise("gated_ffn_fp8 has no gradient: call it under torch.no_grad(), or gated_ffn for training");
 }
 
 // ------------------------------------------------------------------ AdamW

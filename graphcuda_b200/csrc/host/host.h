@@ -205,6 +205,7 @@ std::pair<Tensor, Tensor> rms_norm(const Tensor& x, const Tensor& weight, const 
                                    int64_t y_type);
 std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x, const Tensor& weight, const OptTensor& residual,
                                                 double eps);
+void refuse_norm_fp8_gradient(const Tensor& x, const Tensor& weight, const OptTensor& residual);
 struct FfnForward {
   Tensor y, saved;        // saved: for a backward pass
   Tensor x, w_in, w_out;  // as the kernels took them
@@ -218,6 +219,7 @@ FfnGrads gated_ffn_backward(const Tensor& dy, const Tensor& x, const Tensor& w_i
 Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act);
 Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Tensor& w_out,
                      int64_t act);
+void refuse_ffn_fp8_gradient(const Tensor& x_scale, const Tensor& w_scale, const Tensor& w_out);
 void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
                 const std::vector<Tensor>& v, const Tensor& state, const std::vector<Tensor>& masters,
                 const std::vector<Tensor>& m_scales, const std::vector<Tensor>& v_scales, double lr, double b1, double b2,

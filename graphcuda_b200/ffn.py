@@ -35,6 +35,18 @@ class _TracedFFN(torch.autograd.Function):
         return _lib.host.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.act, *ctx.needs_input_grad[:3]) + (None,)
 
 
+class _TracedFFNFp8(torch.autograd.Function):
+    """The block with its first product in 8 bits inside torch.jit.trace."""
+
+    @staticmethod
+    def forward(ctx, x8, x_scale, w8, w_scale, w_out, act):
+        return _lib.host.gated_ffn_fp8_forward(x8, x_scale, w8, w_scale, w_out, act)
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError("gated_ffn_fp8 has no gradient: call it under torch.no_grad(), or gated_ffn for training")
+
+
 def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """``(act(x @ Wg) * (x @ Wu)) @ w_out`` with ``w_in = [Wg | Wu]``, all bfloat16.
 
@@ -62,7 +74,9 @@ def gated_ffn_fp8(x8: torch.Tensor, x_scale: torch.Tensor, w_in8: torch.Tensor, 
                   w_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """The block for serving, its first product in 8 bits: ``x8, x_scale`` as ``rms_norm_fp8`` leaves them,
     ``w_in8, w_in_scale`` from ``quantize_weight_fp8``; ``w_out`` and the result are bfloat16."""
-    return _lib.host.gated_ffn_fp8(x8, x_scale, w_in8, w_in_scale, w_out, _act(activation))
+    act = _act(activation)
+    y = _lib.host.gated_ffn_fp8(x8, x_scale, w_in8, w_in_scale, w_out, act)
+    return y if y is not None else _TracedFFNFp8.apply(x8, x_scale, w_in8, w_in_scale, w_out, act)
 
 
 class GatedFFN(torch.nn.Module):

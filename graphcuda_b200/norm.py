@@ -31,6 +31,19 @@ class _TracedNorm(torch.autograd.Function):
         return dx if need[0] else None, dw, dr if need[2] else None, None, None
 
 
+class _TracedNormFp8(torch.autograd.Function):
+    """The norm with 8-bit rows inside torch.jit.trace."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, scale, stream = _lib.host.rms_norm_fp8_forward(x, weight, residual, eps)
+        return (y, scale) if residual is None else (y, scale, stream)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad(), or rms_norm for training")
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
              out_dtype: Optional[torch.dtype] = None):
     """``y = h / sqrt(mean(h^2) + eps) * weight`` over the rows of ``h = x + residual``.
@@ -53,8 +66,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
 
     ``y8`` is float8_e4m3fn and stands for ``y8 * scale[:, None]``; a row's scale is its largest |value| / 448 (zero for a
     row of zeros; not finite for a row that holds a NaN or an infinity).  The operand of ``gated_ffn_fp8``."""
-    y, scale, stream = _lib.host.rms_norm_fp8(x, weight, residual, eps)
-    return (y, scale) if residual is None else (y, scale, stream)
+    got = _lib.host.rms_norm_fp8(x, weight, residual, eps)
+    if got is None:
+        return _TracedNormFp8.apply(x, weight, residual, eps)
+    return got[:2] if residual is None else got
 
 
 class RMSNorm(torch.nn.Module):

@@ -1,0 +1,86 @@
+"""The 8-bit forms as a server has them: inside a trace, frozen beside a model that trains on, and without a gradient."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _poison(*like):
+    """What fresh memory holds from here on."""
+    junk = [torch.full((t.numel() * t.element_size() // 4 + 64,), float("nan"), device=t.device) for t in like for _ in range(4)]
+    del junk
+
+
+class _Traced(torch.nn.Module):
+    """Norm and block with a residual that is no input of the trace."""
+
+    def __init__(self, norm, ffn, residual):
+        super().__init__()
+        self.norm, self.ffn, self.residual = norm, ffn, residual
+
+    def forward(self, x):
+        got = self.norm.fp8(x, self.residual)
+        return (self.ffn(got[0], got[1]), *got)
+
+
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("rows", [1, 7, 300])
+def test_traced_eight_bit_forms_run_on_new_inputs(cuda, rows, add):
+    import graphcuda_b200 as gc
+    torch.manual_seed(0)
+    norm, ffn = gc.RMSNorm(96).to(cuda), gc.GatedFFN(96, 160, 40).to(cuda).for_serving()
+    xs = [torch.randn(rows, 96, device=cuda).bfloat16() for _ in range(3)]
+    model = _Traced(norm, ffn, torch.randn(rows, 96, device=cuda) if add else None)
+    with torch.no_grad():
+        traced = torch.jit.trace(model, (xs[0],), check_trace=False)
+        for x in xs:
+            expect = model(x)
+            _poison(*expect)
+            got = traced(x)
+            assert len(got) == len(expect) == (4 if add else 3)
+            assert all(a.dtype == b.dtype and torch.equal(a.float(), b.float()) for a, b in zip(got, expect))
+
+
+def test_a_trace_has_no_gradient_either(cuda):
+    """What raises outside of a trace raises while it is taken."""
+    import graphcuda_b200 as gc
+    x, w = torch.randn(4, 32, device=cuda), torch.ones(32, device=cuda, requires_grad=True)
+    w8, ws = gc.quantize_weight_fp8(torch.randn(32, 48, device=cuda))
+    w_out = torch.randn(24, 16, device=cuda).bfloat16().requires_grad_()
+    x8, xs = gc.rms_norm_fp8(x, w.detach())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.jit.trace(lambda t: gc.rms_norm_fp8(t, w)[1], (x,), check_trace=False)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.jit.trace(lambda s: gc.gated_ffn_fp8(x8, s, w8, ws, w_out), (xs,), check_trace=False)
+
+
+def _setup(cuda, seed=0):
+    from graphcuda_b200 import normalized_adjacency, synth
+    from graphcuda_b200.models import ResidualGCN
+    n, f, classes = 400, 40, 5
+    edges = synth.symmetrize(synth.preferential_attachment_edges(n, 4 * n, seed))
+    adj = normalized_adjacency(edges.to(cuda), n, symmetric=True)
+    torch.manual_seed(seed)
+    model = ResidualGCN(f, 48, 3, classes, hidden=80).to(cuda)
+    return adj, model, torch.randn(n, f, device=cuda), torch.randint(0, classes, (n,), device=cuda)
+
+
+def test_traced_served_model_runs_on_new_inputs(cuda):
+    adj, model, X, _ = _setup(cuda)
+    served = model.for_serving()
+
+    class Answer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.model = served
+
+        def forward(self, x):
+            return self.model(x, adj, log_softmax=False)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(Answer(), (X,), check_trace=False)
+        for seed in range(3):
+            x = torch.randn(X.shape, generator=torch.Generator().manual_seed(seed)).to(cuda)
+            expect = served(x, adj, log_softmax=False)
+            _poison(expect, x)
+            assert torch.equal(traced(x), expect)
