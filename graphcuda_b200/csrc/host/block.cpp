@@ -342,6 +342,8 @@ void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, cons
                           vv.data(), mss.data(), vss.data(), n.data(), eight ? 8 : 32, lr, b1, b2, eps, wd, uint32_t(seed),
                           state.data_ptr(), stream_of(dev)),
         "gc_adamw_step");
+  for (const auto* list : {&p, &m, &v, &masters, &ms, &vs}) written(*list);
+  written(state);
 }
 
 void adamw_moments(const std::vector<Tensor>& m, const std::vector<Tensor>& v, const std::vector<Tensor>& ms,
@@ -374,6 +376,8 @@ void adamw_moments(const std::vector<Tensor>& m, const std::vector<Tensor>& v, c
   check(abi.gc_adamw_moments_f32(int(count), mm.data(), vv.data(), mss.data(), vss.data(), n.data(), mo.data(), vo.data(),
                                  stream_of(dev)),
         "gc_adamw_moments_f32");
+  written(m_out);
+  written(v_out);
 }
 
 }  // namespace gch

@@ -77,6 +77,15 @@ struct Scratch {
 Scratch scratch(Tag tag, size_t bytes, const at::Device& dev);
 void scratch_clear();
 
+// For every tensor of the caller's that a kernel has written: autograd checks its version where it was saved for a backward pass
+// (tensors of inference mode have none).
+inline void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+inline void written(const std::vector<Tensor>& ts) {
+  for (const Tensor& t : ts) written(t);
+}
+
 inline void* stream_of(const at::Device& dev) { return at::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
 // A row-major matrix as the kernels take it, or the transpose of one (trans: rows x cols is a view of a cols x rows

@@ -185,6 +185,8 @@ void adam_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const
   check(abi.gc_adam_step_f32(int(p.size()), l.p.data(), l.g.data(), l.m.data(), l.v.data(), l.n.data(), lr, b1, b2,
                              eps, wd, state.data_ptr(), stream_of(dev)),
         "gc_adam_step_f32");
+  for (const auto* list : {&p, &m, &v}) written(*list);
+  written(state);
 }
 
 void sgd_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, double lr, double wd) {
@@ -194,6 +196,7 @@ void sgd_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, double
   const c10::cuda::CUDAGuard guard(dev);
   check(abi.gc_sgd_step_f32(int(p.size()), l.p.data(), l.g.data(), l.n.data(), lr, wd, stream_of(dev)),
         "gc_sgd_step_f32");
+  written(p);
 }
 
 }  // namespace gch
