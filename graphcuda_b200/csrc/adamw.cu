@@ -4,7 +4,9 @@
 //   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 //
 // Parameters are fp32, or bf16 beside an fp32 master that takes the update (a bf16 weight of 1 does not move by less
-// than 4e-3).
+// than 4e-3).  A bf16 parameter that may have been changed between steps by others is read too (FOLLOW): where it is not what
+// the last step left, its master's rounding, the master takes its value.  2 bytes more per parameter (218 M of them: 1112 us instead
+// of 1052 with moments of 32 bits, 777 instead of 650 with 8), which a list whose owner changes masters alone does not need.
 //
 // Moments in 8 bits: blocks of 256 elements of a tensor share an fp32 scale per moment.  The first is e4m3 (largest
 // value 448); the second, which is never negative, has the upper byte of a positive fp16 number without its sign: 5
@@ -223,6 +225,21 @@ __device__ __forceinline__ void count_step(const Hyper& hp, unsigned long long s
   }
 }
 
+// Masters of four parameters: their own values, or the parameters' where those are no longer what was rounded from them (compared two
+// at a time, and nearly always equal).
+__device__ __forceinline__ void follow(float (&master)[4], const bf16 (&p)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; k += 2) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(master[k], master[k + 1]);
+    const uint32_t left = *reinterpret_cast<const uint32_t*>(&t);
+    const uint32_t now = __bfloat16_as_ushort(p[k]) | uint32_t(__bfloat16_as_ushort(p[k + 1])) << 16;
+    if (left != now) {
+      if ((left ^ now) & 0xFFFFu) master[k] = __bfloat162float(p[k]);
+      if ((left ^ now) >> 16) master[k + 1] = __bfloat162float(p[k + 1]);
+    }
+  }
+}
+
 // One element: moments as the formula reads, one rounding per operation; the parameter from them.  The quotient may be off
 // by 2^-21 of the update (approximate root and division: the exact ones take half of an element's instructions).  What is
 // added to v, the smallest normal number, is a root of 1.1e-19: it stands for the subnormal ones, which the fast
@@ -239,7 +256,7 @@ __device__ __forceinline__ void update(const Hyper& hp, const Scalars& sc, float
 
 // Moments of 32 bits.  Bound by memory: 28 bytes per parameter (82 M of them in 394 us, 5.8 TB/s).  A thread takes 4 elements of
 // a pass, all of whose loads are under way before the first is used; 6 CTAs per SM.
-template <class TP, int MAX>
+template <class TP, bool FOLLOW, int MAX>
 __global__ void __launch_bounds__(kThreads, 6)
 adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, MAX> tl, const __grid_constant__ Hyper hp,
              unsigned long long* __restrict__ state) {
@@ -248,6 +265,7 @@ adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, 
   const int total = 2 * tl.first_chunk[tl.count];  // half a chunk per pass
   float pv[4], mv[4], vv[4];
   TP gv[4];
+  [[maybe_unused]] bf16 old[4];
   int k = 0;
   int64_t at = 0, n = 0;
   bool fast = false;
@@ -262,6 +280,7 @@ adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, 
       load4<F>(tl.at[kG][k], at, n, gv);
       load4<F>(tl.at[kM][k], at, n, mv);
       load4<F>(tl.at[kV][k], at, n, vv);
+      if constexpr (FOLLOW) load4<F>(tl.at[Layout<32, kMixed>::kP16][k], at, n, old);
     };
     if (fast) all(std::true_type{});
     else all(std::false_type{});
@@ -273,6 +292,7 @@ adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, 
   __syncthreads();
   const Scalars sc = sc_s;
   while (pass < total) {
+    if constexpr (FOLLOW) follow(pv, old);
 #pragma unroll
     for (int e = 0; e < 4; ++e) update(hp, sc, to_f32(gv[e]), mv[e], vv[e], pv[e]);
     auto all = [&](auto f) {
@@ -297,7 +317,7 @@ adamw_kernel(const __grid_constant__ List<Layout<32, sizeof(TP) == 2>::kArrays, 
 // Moments of 8 bits.  A warp takes a block of 256 elements, a lane two runs of 4.  16 bytes per mixed parameter, of which 218 M
 // take 667 us (5.2 TB/s): some 60 instructions to an element share the issue slots with the loads.  4 CTAs per SM hide more of
 // these than 3 (694 us) and than 2 that read a chunk ahead (764).
-template <class TP, int MAX>
+template <class TP, bool FOLLOW, int MAX>
 __global__ void __launch_bounds__(kThreads, 4)
 adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArrays, MAX> tl,
                   const __grid_constant__ Hyper hp, unsigned long long* __restrict__ state) {
@@ -308,6 +328,7 @@ adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArra
   const int total = tl.first_chunk[tl.count];
   float pv[2][4];
   TP gv[2][4];
+  [[maybe_unused]] bf16 old[2][4];
   uint32_t mq[2], vq[2];
   float ms = 0.f, vs = 0.f;
   int k = 0;
@@ -327,6 +348,7 @@ adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArra
         load4<F>(tl.at[kG][k], at + j * 128, n, gv[j]);
         mq[j] = load_codes<F>(tl.at[kM][k], at + j * 128, n);
         vq[j] = load_codes<F>(tl.at[kV][k], at + j * 128, n);
+        if constexpr (FOLLOW) load4<F>(tl.at[L::kP16][k], at + j * 128, n, old[j]);
       }
       if (F || block * kBlock < n) {
         ms = static_cast<const float*>(tl.at[L::kMs][k])[block];
@@ -351,6 +373,7 @@ adamw_8bit_kernel(const __grid_constant__ List<Layout<8, sizeof(TP) == 2>::kArra
       for (int j = 0; j < 2; ++j) {
         decode_m(mq[j], ms, m[j]);
         decode_v(vq[j], vs, v[j]);
+        if constexpr (FOLLOW) follow(pv[j], old[j]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           update(hp, sc, to_f32(gv[j][e]), m[j][e], v[j][e], pv[j][e]);
@@ -481,7 +504,7 @@ int fill(List<ARRAYS, MAX>& tl, const Arrays& a, int from, int n_tensors) {
   return i;
 }
 
-template <int BITS, class TP, int MAX>
+template <int BITS, class TP, bool FOLLOW, int MAX>
 int step_lists(const Arrays& a, int n_tensors, Hyper hp, void* state, cudaStream_t st) {
   constexpr int kArrays = Layout<BITS, sizeof(TP) == 2>::kArrays;
   static_assert(sizeof(List<kArrays, MAX>) + sizeof(Hyper) <= 32000, "launch parameters");
@@ -495,17 +518,17 @@ int step_lists(const Arrays& a, int n_tensors, Hyper hp, void* state, cudaStream
     const int passes = tl.first_chunk[tl.count] * (BITS == 8 ? 1 : 2);
     // as many CTAs as the SMs hold, each over many passes; an empty model still counts the step
     const int blocks = std::max(1, std::min(passes, gc::kNumSMs * (BITS == 8 ? 4 : 6)));
-    if constexpr (BITS == 8) adamw_8bit_kernel<TP, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
-    else adamw_kernel<TP, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
+    if constexpr (BITS == 8) adamw_8bit_kernel<TP, FOLLOW, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
+    else adamw_kernel<TP, FOLLOW, MAX><<<blocks, kThreads, 0, st>>>(tl, hp, count);
     ++launches;
     from = next;
   } while (from < n_tensors);
   return gc::check_launch("gc_adamw_step", launches);
 }
-template <int BITS, class TP>
+template <int BITS, class TP, bool FOLLOW>
 int step(const Arrays& a, int n_tensors, const Hyper& hp, void* state, cudaStream_t st) {
-  return n_tensors <= kFew ? step_lists<BITS, TP, kFew>(a, n_tensors, hp, state, st)
-                           : step_lists<BITS, TP, Layout<BITS, sizeof(TP) == 2>::kMany>(a, n_tensors, hp, state, st);
+  return n_tensors <= kFew ? step_lists<BITS, TP, FOLLOW, kFew>(a, n_tensors, hp, state, st)
+                           : step_lists<BITS, TP, FOLLOW, Layout<BITS, sizeof(TP) == 2>::kMany>(a, n_tensors, hp, state, st);
 }
 template <int MAX>
 int moments(const Arrays& a, int n_tensors, cudaStream_t st) {
@@ -533,9 +556,10 @@ int gc_adamw_step(int n_tensors, void* const* params, int param_type, const void
                   double beta2, double eps, double weight_decay, uint32_t seed, void* state, void* stream) {
   GC_REQUIRE(state, "gc_adamw_step: null state");
   GC_REQUIRE(n_tensors >= 0, "gc_adamw_step: negative number of tensors");
-  GC_REQUIRE(param_type == GC_TYPE_F32 || param_type == GC_TYPE_BF16, "gc_adamw_step: parameters are fp32 or bf16");
+  GC_REQUIRE(param_type == GC_TYPE_F32 || param_type == GC_TYPE_BF16 || param_type == (GC_TYPE_BF16 | GC_ADAMW_FOLLOW),
+             "gc_adamw_step: parameters are fp32 or bf16, and those beside masters may be followed");
   GC_REQUIRE(state_bits == 8 || state_bits == 32, "gc_adamw_step: moments have 8 or 32 bits");
-  const bool mixed = param_type == GC_TYPE_BF16, eight = state_bits == 8;
+  const bool mixed = param_type != GC_TYPE_F32, eight = state_bits == 8, followed = param_type & GC_ADAMW_FOLLOW;
   GC_REQUIRE(n_tensors == 0 || (params && grads && exp_avg && exp_avg_sq && sizes), "gc_adamw_step: null list");
   GC_REQUIRE(n_tensors == 0 || !mixed || masters, "gc_adamw_step: bf16 parameters need fp32 masters");
   GC_REQUIRE(n_tensors == 0 || !eight || (exp_avg_scales && exp_avg_sq_scales), "gc_adamw_step: 8-bit moments need scales");
@@ -557,8 +581,9 @@ int gc_adamw_step(int n_tensors, void* const* params, int param_type, const void
     a.at[r++] = list(exp_avg_sq_scales);
   }
   const cudaStream_t st = gc::as_stream(stream);
-  if (eight) return mixed ? step<8, bf16>(a, n_tensors, hp, state, st) : step<8, float>(a, n_tensors, hp, state, st);
-  return mixed ? step<32, bf16>(a, n_tensors, hp, state, st) : step<32, float>(a, n_tensors, hp, state, st);
+  if (followed) return eight ? step<8, bf16, true>(a, n_tensors, hp, state, st) : step<32, bf16, true>(a, n_tensors, hp, state, st);
+  if (mixed) return eight ? step<8, bf16, false>(a, n_tensors, hp, state, st) : step<32, bf16, false>(a, n_tensors, hp, state, st);
+  return eight ? step<8, float, false>(a, n_tensors, hp, state, st) : step<32, float, false>(a, n_tensors, hp, state, st);
 }
 
 int gc_adamw_moments_f32(int n_tensors, const uint8_t* const* exp_avg, const uint8_t* const* exp_avg_sq,

@@ -292,7 +292,7 @@ int64_t blocks_of(int64_t n) { return (n + GC_ADAMW_BLOCK - 1) / GC_ADAMW_BLOCK;
 void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
                 const std::vector<Tensor>& v, const Tensor& state, const std::vector<Tensor>& masters,
                 const std::vector<Tensor>& ms, const std::vector<Tensor>& vs, double lr, double b1, double b2, double eps,
-                double wd, int64_t seed) {
+                double wd, int64_t seed, bool follow) {
   const size_t count = p.size();
   require(state.is_cuda() && state.scalar_type() == at::kLong && state.is_contiguous() && state.numel() >= 2,
           "adamw_step: step must be a CUDA int64 tensor of two elements, zeros before the first step");
@@ -300,6 +300,7 @@ void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, cons
   const at::Device dev = state.device();
   const bool mixed = count && p[0].scalar_type() == at::kBFloat16, eight = count && m[0].scalar_type() == at::kByte;
   require(masters.size() == (mixed ? count : 0), "adamw_step: bfloat16 parameters need float32 masters, float32 ones take none");
+  require(!follow || !count || mixed, "adamw_step: float32 parameters have no masters that could follow them");
   require(ms.size() == (eight ? count : 0) && vs.size() == ms.size(),
           "adamw_step: moments in 8 bits need their scales, moments in 32 bits have none");
   require(lr >= 0 && eps >= 0 && wd >= 0 && b1 >= 0 && b1 < 1 && b2 >= 0 && b2 < 1, "adamw_step: invalid hyper-parameter");
@@ -338,7 +339,7 @@ void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, cons
     }
   }
   const c10::cuda::CUDAGuard guard(dev);
-  check(abi.gc_adamw_step(int(count), pp.data(), mixed ? GC_TYPE_BF16 : GC_TYPE_F32, gg.data(), mas.data(), mm.data(),
+  check(abi.gc_adamw_step(int(count), pp.data(), !mixed ? GC_TYPE_F32 : follow ? GC_TYPE_BF16 | GC_ADAMW_FOLLOW : GC_TYPE_BF16, gg.data(), mas.data(), mm.data(),
                           vv.data(), mss.data(), vss.data(), n.data(), eight ? 8 : 32, lr, b1, b2, eps, wd, uint32_t(seed),
                           state.data_ptr(), stream_of(dev)),
         "gc_adamw_step");

@@ -232,7 +232,7 @@ void refuse_ffn_fp8_gradient(const Tensor& x_scale, const Tensor& w_scale, const
 void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
                 const std::vector<Tensor>& v, const Tensor& state, const std::vector<Tensor>& masters,
                 const std::vector<Tensor>& m_scales, const std::vector<Tensor>& v_scales, double lr, double b1, double b2,
-                double eps, double wd, int64_t seed);
+                double eps, double wd, int64_t seed, bool follow);
 void adamw_moments(const std::vector<Tensor>& m, const std::vector<Tensor>& v, const std::vector<Tensor>& m_scales,
                    const std::vector<Tensor>& v_scales, const std::vector<Tensor>& m_out, const std::vector<Tensor>& v_out);
 }  // namespace gch

@@ -92,20 +92,22 @@ class FusedSGD(torch.optim.Optimizer):
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
-               weight_decay: float = 1e-2, masters=None, scales=None, seed: int = 0) -> None:
+               weight_decay: float = 1e-2, masters=None, scales=None, seed: int = 0, follow: bool = False) -> None:
     """One AdamW step over lists of tensors, in place; one launch for up to 449 tensors.
 
     ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
     ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)``.
 
-    ``params`` and ``grads`` are all float32, or all bfloat16 beside float32 ``masters``, which take the update.
+    ``params`` and ``grads`` are all float32, or all bfloat16 beside float32 ``masters``, which take the update: a parameter is
+    its master's rounding, whatever it held before.  ``follow=True``: one that is not has been changed by others since the last
+    step, and its master takes its value first.
     ``exp_avgs`` and ``exp_avg_sqs`` are float32; or uint8 (zeros at the start) with ``scales = (of exp_avgs, of
     exp_avg_sqs)``, float32 tensors of ceil(size / 256) elements each: 8 bits per value, rounded at random by a hash of
     (seed, step, position in the list, element).  ``step`` is a CUDA int64 tensor of two elements, zeros at the start; the
     kernel counts in it, so the call can be recorded in a CUDA graph."""
     of_m, of_v = scales if scales is not None else ((), ())
     _lib.host.adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, masters or (), of_m, of_v, lr, betas[0], betas[1], eps,
-                         weight_decay, seed & 0xFFFFFFFF)
+                         weight_decay, seed & 0xFFFFFFFF, follow)
 
 
 def adamw_moments(exp_avgs, exp_avg_sqs, scales, out=None):
@@ -119,7 +121,8 @@ def adamw_moments(exp_avgs, exp_avg_sqs, scales, out=None):
 class FusedAdamW(torch.optim.Optimizer):
     """AdamW (``torch.optim.AdamW``, amsgrad and maximize off) for any number of tensors in one launch.
 
-    Float32 parameters are updated as they are; bfloat16 ones beside a float32 master in the optimizer's state.
+    Float32 parameters are updated as they are; bfloat16 ones beside a float32 master in the optimizer's state, which follows a
+    parameter that others have changed between steps (a state dict loaded, a copy, weights clipped; recorded or not).
     ``state_bits=8`` holds both moments in 8 bits with a float32 scale per 256 elements (see ``adamw_step``): 2 bytes per
     parameter instead of 8.  Tensors of 256 elements and fewer keep 32 bits: there is nothing to save in them."""
 
@@ -180,7 +183,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 eight = st[0]["exp_avg"].dtype == torch.uint8
                 adamw_step(ps, [p.grad for p in ps], of("exp_avg"), of("exp_avg_sq"), st[0]["step"], lr=group["lr"],
                            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                           masters=of("master") if "master" in st[0] else None,
+                           masters=of("master") if "master" in st[0] else None, follow="master" in st[0],
                            scales=(of("exp_avg_scale"), of("exp_avg_sq_scale")) if eight else None, seed=group["seed"])
         return loss
 

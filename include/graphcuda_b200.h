@@ -437,7 +437,8 @@ int gc_sgd_step_f32(int n_tensors, float* const* params, const float* const* gra
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * param_type: GC_TYPE_F32, or GC_TYPE_BF16 for parameters and gradients in bf16 beside fp32 masters, which take the update
- * and are rounded into the parameters (masters is not read for GC_TYPE_F32).
+ * and are rounded into the parameters (masters is not read for GC_TYPE_F32); GC_TYPE_BF16 | GC_ADAMW_FOLLOW: a parameter
+ * that is not its master's rounding has been changed since the last step, and its master takes its value first.
  * state_bits 32: exp_avg and exp_avg_sq are fp32 (the scales are not read).  8: they are bytes, in blocks of
  * GC_ADAMW_BLOCK elements of a tensor with an fp32 scale each (ceil(size / GC_ADAMW_BLOCK) per tensor): e4m3, and the
  * upper byte of a positive fp16 number without its sign bit; all zero at the start.  Their values are rounded up or
@@ -446,6 +447,7 @@ int gc_sgd_step_f32(int n_tensors, float* const* params, const float* const* gra
  * state: 16 bytes of device memory as for gc_adam_step_f32.  One launch per 449 tensors (688 in fp32 alone).
  */
 #define GC_ADAMW_BLOCK 256
+#define GC_ADAMW_FOLLOW 256
 int gc_adamw_step(int n_tensors, void* const* params, int param_type, const void* const* grads, float* const* masters,
                   void* const* exp_avg, void* const* exp_avg_sq, float* const* exp_avg_scales,
                   float* const* exp_avg_sq_scales, const int64_t* sizes, int state_bits,

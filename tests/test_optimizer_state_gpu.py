@@ -65,3 +65,98 @@ def test_everything_a_step_writes_has_a_new_version(cuda):
         step = torch.zeros(2, dtype=torch.int64, device=cuda)
         gc.adamw_step([p], [g], [m], [v], step, lr=0.1)
         assert int(step[0]) == 1 and bool((p < 0).all())
+
+
+# ---- masters
+SIZES = [(700,), (33,), (65, 64), (4097,)]
+
+
+def _change(p, new, how):
+    if how == "copy_":
+        with torch.no_grad():
+            p.copy_(new)
+    elif how == "data":
+        p.data.copy_(new)
+    elif how == "swap":
+        p.data = new.clone()
+    else:  # one element of seven: the others keep what their masters have beyond bfloat16
+        p.data.view(-1)[::7] = new.view(-1)[::7]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["copy_", "data", "swap", "some"])
+def test_a_parameter_changed_between_steps_stays_changed(cuda, bits, how):
+    """As with torch.optim: the next step starts from the value that the parameter has.  Beside it, an optimizer whose masters
+    are changed by hand."""
+    import graphcuda_b200 as gc
+    sets = [[torch.nn.Parameter(_randn(s, i, torch.bfloat16)) for i, s in enumerate(SIZES)] for _ in range(2)]
+    opts = [gc.FusedAdamW(ps, **HYPER, state_bits=bits, seed=5) for ps in sets]
+
+    def step(t):
+        for ps, opt in zip(sets, opts):
+            for i, p in enumerate(ps):
+                p.grad = _randn(p.shape, 10 * t + i, torch.bfloat16)
+            opt.step()
+
+    for t in range(3):
+        step(t)
+    for i, (p, q) in enumerate(zip(*sets)):
+        master = opts[1].state[q]["master"]
+        assert not torch.equal(master, q.detach().float())  # there is something to keep
+        new = _randn(p.shape, 100 + i, torch.bfloat16)
+        _change(p, new, how)
+        changed = p.detach().view(torch.int16) != q.detach().view(torch.int16)
+        assert changed.any()
+        master.copy_(torch.where(changed, p.detach().float(), master))
+        q.data.copy_(p.detach())
+    for t in range(3, 5):
+        step(t)
+    for p, q in zip(*sets):
+        assert torch.equal(p, q)
+        assert all(torch.equal(opts[0].state[p][k], opts[1].state[q][k]) for k in opts[0].state[p])
+
+
+def test_loaded_weights_stay_in_a_run_that_is_recorded(cuda):
+    """A state dict loaded between replays of a recorded step."""
+    import graphcuda_b200 as gc
+    lin = gc.GatedFFN(32, 40, 24).to(cuda)
+    for i, p in enumerate(lin.parameters()):
+        p.grad = _randn(p.shape, i, torch.bfloat16)
+    start = {k: v.clone() for k, v in lin.state_dict().items()}
+    opt = gc.FusedAdamW(lin.parameters(), lr=1e-2, weight_decay=0.0)
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(20):
+        graph.replay()
+    far = {k: (v.float() - start[k].float()).abs().max().item() for k, v in lin.state_dict().items()}
+    assert min(far.values()) > 0.1
+    lin.load_state_dict(start)
+    graph.replay()
+    for k, v in lin.state_dict().items():  # one step of a constant gradient: the learning rate, and bfloat16's rounding
+        assert float((v.float() - start[k].float()).abs().max()) < 0.011 + float(start[k].abs().max()) * 2.0 ** -8
+
+
+def test_lists_with_masters_take_the_masters_word(cuda):
+    """adamw_step on lists: the masters are the parameters, whatever the bfloat16 tensors hold -- unless they are to follow."""
+    import graphcuda_b200 as gc
+    for follow in (False, True):
+        master, g = _randn(900, 0), _randn(900, 1, torch.bfloat16)
+        p = torch.full((900,), 3.0, dtype=torch.bfloat16, device=cuda)
+        m, v = torch.zeros(900, device=cuda), torch.zeros(900, device=cuda)
+        step = torch.zeros(2, dtype=torch.int64, device=cuda)
+        expect = torch.full_like(master, 3.0) if follow else master.clone()
+        gc.adamw_step([p], [g], [m], [v], step, masters=[master], **(dict(follow=True) if follow else {}), **HYPER)
+        m2, v2, step2 = torch.zeros(900, device=cuda), torch.zeros(900, device=cuda), torch.zeros(2, dtype=torch.int64, device=cuda)
+        gc.adamw_step([expect], [g.float()], [m2], [v2], step2, **HYPER)
+        assert torch.equal(master, expect) and torch.equal(p, expect.bfloat16())
+
+
+def test_following_takes_masters(cuda):
+    import graphcuda_b200 as gc
+    p, step = torch.zeros(300, device=cuda), torch.zeros(2, dtype=torch.int64, device=cuda)
+    with pytest.raises(RuntimeError, match="masters"):
+        gc.adamw_step([p], [p], [p.clone()], [p.clone()], step, lr=0.1, follow=True)
+    assert not step.any()
