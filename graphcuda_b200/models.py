@@ -3,6 +3,7 @@
 with ReLU on all but the last, ``log_softmax`` on top."""
 from __future__ import annotations
 
+import copy
 from typing import Optional, Sequence
 
 import torch
@@ -109,21 +110,35 @@ class ResidualGCN(torch.nn.Module):
         return ServedResidualGCN(self)
 
 
+def _frozen(module: torch.nn.Module) -> torch.nn.Module:
+    return copy.deepcopy(module).requires_grad_(False)
+
+
+class ServedBlock(ResidualBlock):
+    """``ResidualBlock`` with its feed-forward block in 8 bits: weights of their own, those that the block had."""
+
+    def __init__(self, block: ResidualBlock):
+        torch.nn.Module.__init__(self)
+        self.norm_conv, self.conv, self.norm_ffn = (_frozen(m) for m in (block.norm_conv, block.conv, block.norm_ffn))
+        self.ffn = block.ffn.for_serving()
+
+    def forward(self, y, h, adj):
+        a, h = self.aggregate(y, h, adj)
+        n8, scale, h = self.norm_ffn.fp8(a, h)
+        return self.ffn(n8, scale), h
+
+
 class ServedResidualGCN(ResidualGCN):
     """``ResidualGCN`` for inference: the norm in front of a feed-forward block writes 8 bits and a scale per row, which the
-    block multiplies with weights laid out in 8 bits once.  Shares the other parameters with the model it is made of."""
+    block multiplies with weights laid out in 8 bits once.  All of its weights are copies: the source may train on, or go."""
 
     def __init__(self, model: ResidualGCN):
         torch.nn.Module.__init__(self)
-        self.conv_in, self.blocks, self.norm_out, self.conv_out = model.conv_in, model.blocks, model.norm_out, model.conv_out
-        self.served = torch.nn.ModuleList([block.ffn.for_serving() for block in model.blocks])
+        self.conv_in, self.norm_out, self.conv_out = (_frozen(m) for m in (model.conv_in, model.norm_out, model.conv_out))
+        self.blocks = torch.nn.ModuleList([ServedBlock(block) for block in model.blocks])
 
-    def _blocks(self, y, h, adj):
-        for block, ffn in zip(self.blocks, self.served):
-            a, h = block.aggregate(y, h, adj)
-            n8, scale, h = block.norm_ffn.fp8(a, h)
-            y = ffn(n8, scale)
-        return y, h
+    def for_serving(self) -> "ServedResidualGCN":
+        return self
 
     @torch.no_grad()
     def forward(self, x, adj, log_softmax: bool = True):

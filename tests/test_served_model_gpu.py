@@ -84,3 +84,37 @@ def test_traced_served_model_runs_on_new_inputs(cuda):
             expect = served(x, adj, log_softmax=False)
             _poison(expect, x)
             assert torch.equal(traced(x), expect)
+
+
+def test_served_model_is_that_of_its_moment(cuda):
+    """The source trains on: the served model answers as it did."""
+    from graphcuda_b200 import FusedAdamW, log_softmax_nll_loss
+    adj, model, X, y = _setup(cuda, seed=1)
+    opt = FusedAdamW(model.parameters(), lr=1e-2)
+    served = model.for_serving()
+    before = served(X, adj, log_softmax=False)
+    for _ in range(3):
+        opt.zero_grad(set_to_none=True)
+        log_softmax_nll_loss(model(X, adj, log_softmax=False), y, scale=1.0 / len(y)).backward()
+        opt.step()
+    assert torch.equal(served(X, adj, log_softmax=False), before)
+    later = model.for_serving()(X, adj, log_softmax=False)
+    assert not torch.equal(later, before)
+    # nor does what is done to the served model reach its source
+    kept = [p.detach().clone() for p in model.parameters()]
+    for t in (*served.parameters(), *served.buffers()):
+        t.data.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(kept, model.parameters()))
+    assert not any(p.requires_grad for p in served.parameters())
+
+
+def test_served_model_holds_one_set_of_weights(cuda):
+    """Smaller than its source, by half of the first products' weights: nothing is kept that no call reads."""
+    _, model, _, _ = _setup(cuda)
+    served = model.for_serving()
+    size = lambda m: sum(t.numel() * t.element_size() for t in (*m.parameters(), *m.buffers()))  # noqa: E731
+    w_in = sum(b.ffn.w_in.numel() for b in model.blocks)
+    scales = sum(b.ffn.w_in.size(1) * 4 for b in model.blocks)
+    assert size(served) == size(model) - w_in + scales
+    again = served.for_serving()
+    assert all(torch.equal(a.float(), b.float()) for a, b in zip(again.state_dict().values(), served.state_dict().values()))
