@@ -307,7 +307,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   }, NoGil());
   m.def("gated_ffn_fp8", [](const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale,
                             const Tensor& w_out, int64_t act) -> OptTensor {
-    refuse_ffn_fp8_gradient(x_scale, w_scale, w_out);
+    refuse_ffn_fp8_gradient({&x8, &x_scale, &w8, &w_scale, &w_out});
     if (torch::jit::tracer::isTracing()) return std::nullopt;
     return gated_ffn_fp8(x8, x_scale, w8, w_scale, w_out, act);
   }, NoGil());

@@ -276,8 +276,8 @@ Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, 
   return y;
 }
 
-void refuse_ffn_fp8_gradient(const Tensor& x_scale, const Tensor& w_scale, const Tensor& w_out) {
-  if (recorded({&w_out, &x_scale, &w_scale}))
+void refuse_ffn_fp8_gradient(std::initializer_list<const Tensor*> inputs) {
+  if (recorded(inputs))
     raise("gated_ffn_fp8 has no gradient: call it under torch.no_grad(), or gated_ffn for training");
 }
 

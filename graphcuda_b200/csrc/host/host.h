@@ -228,7 +228,7 @@ FfnGrads gated_ffn_backward(const Tensor& dy, const Tensor& x, const Tensor& w_i
 Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64_t act);
 Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Tensor& w_out,
                      int64_t act);
-void refuse_ffn_fp8_gradient(const Tensor& x_scale, const Tensor& w_scale, const Tensor& w_out);
+void refuse_ffn_fp8_gradient(std::initializer_list<const Tensor*> inputs);
 void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
                 const std::vector<Tensor>& v, const Tensor& state, const std::vector<Tensor>& masters,
                 const std::vector<Tensor>& m_scales, const std::vector<Tensor>& v_scales, double lr, double b1, double b2,

@@ -118,3 +118,19 @@ def test_served_model_holds_one_set_of_weights(cuda):
     assert size(served) == size(model) - w_in + scales
     again = served.for_serving()
     assert all(torch.equal(a.float(), b.float()) for a, b in zip(again.state_dict().values(), served.state_dict().values()))
+
+
+def test_an_eight_bit_operand_with_a_gradient_is_refused(cuda):
+    """A cast to 8 bits is differentiable to torch: the block would drop what comes back."""
+    import graphcuda_b200 as gc
+    x = torch.randn(4, 32, device=cuda, requires_grad=True)
+    w = torch.randn(32, 48, device=cuda, requires_grad=True)
+    w8, ws = gc.quantize_weight_fp8(w)
+    w_out, ones = torch.randn(24, 16, device=cuda).bfloat16(), torch.ones(4, device=cuda)
+    x8, wx8 = x.to(torch.float8_e4m3fn), w.t().to(torch.float8_e4m3fn)
+    assert x8.requires_grad and wx8.requires_grad and not w8.requires_grad
+    for a, b in ((x8, w8), (x8.detach(), wx8)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            gc.gated_ffn_fp8(a, ones, b, ws, w_out)
+        with torch.no_grad():
+            gc.gated_ffn_fp8(a, ones, b, ws, w_out)
