@@ -67,7 +67,9 @@ def quantize_weight_fp8(w: torch.Tensor):
         raise RuntimeError("quantize_weight_fp8: a matrix of floating-point weights expected")
     wt = w.detach().float().t()
     scale = wt.abs().amax(1) / 448.0 if w.size(0) else wt.new_zeros(wt.size(0))
-    return (wt / torch.where(scale > 0, scale, 1.0)[:, None]).contiguous().to(torch.float8_e4m3fn), scale
+    # of a scale that is subnormal, and so rounded coarsely, there may be more than 448 in the largest value, which has no code
+    q = (wt / torch.where(scale > 0, scale, 1.0)[:, None]).clamp(-448.0, 448.0)
+    return q.contiguous().to(torch.float8_e4m3fn), scale
 
 
 def gated_ffn_fp8(x8: torch.Tensor, x_scale: torch.Tensor, w_in8: torch.Tensor, w_in_scale: torch.Tensor,
