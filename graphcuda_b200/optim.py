@@ -135,7 +135,15 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
                                       state_bits=state_bits, seed=seed))
 
+    @staticmethod
+    def _not_recorded(device):
+        """What is made while a stream is captured is made again, as it was, at every replay."""
+        if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: take one step with the gradients of the recorded one before it is recorded "
+                               "(states and step counts must exist by then)")
+
     def _new_state(self, p, bits):
+        self._not_recorded(p.device)
         st, n = {}, p.numel()
         kind = torch.uint8 if bits == 8 and n > _lib.ADAMW_BLOCK else torch.float32
         for name in ("exp_avg", "exp_avg_sq"):
@@ -165,6 +173,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 launches.setdefault(id(st["step"]), []).append(p)
         for key, ps in launches.items():
             if len(ps) < members[key]:  # the others keep the old count
+                self._not_recorded(ps[0].device)
                 step = self.state[ps[0]]["step"].clone()
                 for p in ps:
                     self.state[p]["step"] = step

@@ -160,3 +160,46 @@ def test_following_takes_masters(cuda):
     with pytest.raises(RuntimeError, match="masters"):
         gc.adamw_step([p], [p], [p.clone()], [p.clone()], step, lr=0.1, follow=True)
     assert not step.any()
+
+
+# ---- recording
+def test_a_first_step_is_not_recorded(cuda):
+    """States made while a stream is captured would be zeros again at every replay."""
+    import graphcuda_b200 as gc
+    p, x = torch.nn.Parameter(_randn(500, 0)), torch.zeros(1, device=cuda)
+    p.grad = _randn(500, 1)
+    opt = gc.FusedAdamW([p], lr=0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="before it is recorded"):
+            opt.step()
+    assert not opt.state[p]
+    opt.step()
+    assert opt.steps_taken() == 1
+
+
+def test_a_count_that_parts_is_not_recorded(cuda):
+    """Parameters that have always been updated together share a count; a copy of it made while a stream is captured would be
+    the same count again at every replay."""
+    import graphcuda_b200 as gc
+    p, q, x = torch.nn.Parameter(_randn(500, 0)), torch.nn.Parameter(_randn(400, 1)), torch.zeros(1, device=cuda)
+    p.grad, q.grad = _randn(500, 2), _randn(400, 3)
+    opt = gc.FusedAdamW([p, q], lr=0.1)
+    opt.step()
+    q.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="before it is recorded"):
+            opt.step()
+    opt.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+    assert int(opt.state[p]["step"][0]) == 5 and int(opt.state[q]["step"][0]) == 1
