@@ -185,6 +185,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        number = 0  # of the 8-bit list within the step: each rounds by random bits of its own
         for group in self.param_groups:
             for ps in self._together(group):
                 st = [self.state[p] for p in ps]
@@ -193,7 +194,9 @@ class FusedAdamW(torch.optim.Optimizer):
                 adamw_step(ps, [p.grad for p in ps], of("exp_avg"), of("exp_avg_sq"), st[0]["step"], lr=group["lr"],
                            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                            masters=of("master") if "master" in st[0] else None, follow="master" in st[0],
-                           scales=(of("exp_avg_scale"), of("exp_avg_sq_scale")) if eight else None, seed=group["seed"])
+                           scales=(of("exp_avg_scale"), of("exp_avg_sq_scale")) if eight else None,
+                           seed=group["seed"] + number * 0x632BE5AB)
+                number += eight
         return loss
 
     def moments(self, p):

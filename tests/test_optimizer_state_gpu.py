@@ -203,3 +203,28 @@ def test_a_count_that_parts_is_not_recorded(cuda):
     for _ in range(3):
         graph.replay()
     assert int(opt.state[p]["step"][0]) == 5 and int(opt.state[q]["step"][0]) == 1
+
+
+# ---- random bits
+def test_lists_round_by_bits_of_their_own(cuda):
+    """Equal tensors and gradients in different groups, and in one group beside others: rounded differently, the first as a call
+    on a list alone."""
+    import graphcuda_b200 as gc
+    n = 2048
+    ps = [torch.nn.Parameter(_randn(n, 0)) for _ in range(3)]
+    opt = gc.FusedAdamW([dict(params=[p]) for p in ps], **HYPER, state_bits=8, seed=11)
+    codes = [[torch.zeros(n, dtype=torch.uint8, device=cuda)] for _ in range(2)]
+    scales = [[torch.zeros(n // 256, device=cuda)] for _ in range(2)]
+    step, alone = torch.zeros(2, dtype=torch.int64, device=cuda), ps[0].detach().clone()
+    g = _randn(n, 1)
+    for _ in range(2):
+        for p in ps:
+            p.grad = g.clone()
+        opt.step()
+        gc.adamw_step([alone], [g], *codes, step, scales=scales, seed=11, **HYPER)
+    st = [opt.state[p] for p in ps]
+    assert torch.equal(st[0]["exp_avg"], codes[0][0]) and torch.equal(st[0]["exp_avg_sq"], codes[1][0])
+    for i in range(3):
+        for j in range(i):
+            for k in ("exp_avg", "exp_avg_sq"):
+                assert float((st[i][k] != st[j][k]).float().mean()) > 0.2
