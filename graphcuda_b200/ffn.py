@@ -32,6 +32,8 @@ class _TracedFFN(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_ffn has no second derivative (create_graph)")
         return _lib.host.gated_ffn_backward(dy, *ctx.saved_tensors, ctx.act, *ctx.needs_input_grad[:3]) + (None,)
 
 

@@ -24,6 +24,8 @@ class _TracedNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dstream=None):
+        if torch.is_grad_enabled():
+            raise RuntimeError("rms_norm has no second derivative (create_graph)")
         y_type, x_type, add = ctx.call
         need = ctx.needs_input_grad
         dx, dw, dr = _lib.host.rms_norm_backward(dy, dstream, *ctx.saved_tensors, y_type, x_type, add, need[0] or need[2],
