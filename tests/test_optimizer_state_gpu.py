@@ -228,3 +228,28 @@ def test_lists_round_by_bits_of_their_own(cuda):
         for j in range(i):
             for k in ("exp_avg", "exp_avg_sq"):
                 assert float((st[i][k] != st[j][k]).float().mean()) > 0.2
+
+
+# ---- more elements than the CTAs of a launch take in one pass
+def test_8_bit_codes_of_a_large_tensor(cuda):
+    """Chunks that a CTA comes to in its second and third pass, and the tensor behind: the codes of the formula."""
+    import graphcuda_b200 as gc
+    from test_adamw_gpu import _blocks, _host_step
+    from test_adamw_gpu import HYPER as hyper
+    sizes = (148 * 4 * 2048 * 2 + 777, 5000)
+    gs = [_randn(n, i) for i, n in enumerate(sizes)]
+    ps = [torch.zeros(n, device=cuda) for n in sizes]
+    codes = [[torch.zeros(n, dtype=torch.uint8, device=cuda) for n in sizes] for _ in range(2)]
+    scales = [[torch.zeros(-(-n // 256), device=cuda) for n in sizes] for _ in range(2)]
+    step = torch.zeros(2, dtype=torch.int64, device=cuda)
+    host = [(np.zeros_like(_blocks(g.cpu().numpy())),) * 2 for g in gs]
+    for t in (1, 2):
+        gc.adamw_step(ps, gs, *codes, step, scales=scales, seed=3, **hyper)
+        for i, n in enumerate(sizes):
+            qm, qv, ms, vs, m, v = _host_step(gs[i].cpu().numpy(), *host[i], 3, t, i)
+            m.reshape(-1)[n:] = 0
+            v.reshape(-1)[n:] = 0
+            host[i] = m, v
+            assert np.array_equal(scales[0][i].cpu().numpy(), ms[:, 0]) and np.array_equal(scales[1][i].cpu().numpy(), vs[:, 0])
+            assert np.array_equal(codes[0][i].cpu().numpy(), qm.reshape(-1)[:n])
+            assert np.array_equal(codes[1][i].cpu().numpy(), qv.reshape(-1)[:n])
