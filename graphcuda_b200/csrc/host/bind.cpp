@@ -265,7 +265,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return std::make_tuple(f.loss, f.Z, f.labels, f.ws, f.masked);
   }, NoGil());
   m.def("nll_backward", &nll_backward, NoGil());
-  m.def("argmax_accuracy", &argmax_accuracy, NoGil());
+  m.def("argmax_accuracy", [](const Tensor& logits, const OptTensor& labels, const std::optional<std::vector<Tensor>>& masks,
+                              bool want_pred) -> std::optional<std::pair<Tensor, Tensor>> {
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return argmax_accuracy(logits, labels, masks, want_pred);
+  }, NoGil());
+  m.def("argmax_accuracy_forward", &argmax_accuracy, NoGil());
   m.def("adam_step", &adam_step, NoGil());
   m.def("sgd_step", &sgd_step, NoGil());
 

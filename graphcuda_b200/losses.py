@@ -24,6 +24,21 @@ class _TracedLoss(torch.autograd.Function):
         return _lib.host.nll_backward(grad_loss, *ctx.saved_tensors, *ctx.call), None, None, None
 
 
+class _TracedAccuracy(torch.autograd.Function):
+    """Predictions and counts inside torch.jit.trace: those of them that are asked for."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, want_pred, selected, *masks):
+        got = _lib.host.argmax_accuracy_forward(logits, labels, list(masks) if selected else None, want_pred)
+        got = tuple(t for t in got if t is not None)
+        ctx.mark_non_differentiable(*got)
+        return got
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return (None,) * len(ctx.needs_input_grad)
+
+
 def log_softmax_nll_loss(logits: torch.Tensor, labels: torch.Tensor, row_mask: Optional[torch.Tensor] = None,
                          scale: Optional[float] = None) -> torch.Tensor:
     """``F.nll_loss(torch.log_softmax(logits, 1)[row_mask], labels[row_mask])`` in one
@@ -49,4 +64,8 @@ def argmax_accuracy(logits: torch.Tensor, labels: Optional[torch.Tensor] = None,
     Nothing is read back to the host: ``counts[:, 0] / counts[:, 1]`` are the accuracies."""
     if masks is not None:
         masks = [masks] if isinstance(masks, torch.Tensor) and masks.dim() == 1 else list(masks)
-    return _lib.host.argmax_accuracy(logits, labels, masks, want_pred)
+    got = _lib.host.argmax_accuracy(logits, labels, masks, want_pred)
+    if got is not None:
+        return got
+    got = _TracedAccuracy.apply(logits, labels, want_pred, masks is not None, *(masks or ()))
+    return got[0] if want_pred else None, got[-1] if labels is not None else None
