@@ -1069,9 +1069,17 @@ Saved saved_at(void* p, int64_t M, int64_t H) {
 //   this file copies   47 MB  55 / 66            , 58 / 66        , 176 / 66
 //   e4m3               12 MB  10 / 19            , 10 / 19        , 19 / 19         ;   6 MB  14 / 18 at eight
 //                      48 MB  14 / 27            , 19 / 27        , 39 / 27         ;  96 MB  24 / 32, 30 / 32, 62 / 32
-bool few_rows(int64_t M, int64_t D, int64_t H, int64_t O, bool bf16_in_place) {
+//   e4m3 in rows that  3 MB  12 / 25 at one row, 17 / 25 at two, 14 / 25 at four, 21 / 25 at eight;   6 MB  41 / 28 at eight
+//   16-byte accesses   12 MB  17 / 29           , 21 / 29       , 29 / 29       , 64 / 29
+//   cannot take        24 MB  23 / 35           , 33 / 35       , 46 / 35       ;  47 MB  31 / 43, 40 / 44, 56 / 44
+//                      96 MB  72 / 61           , 107 / 61      (with H and O odd too 24 MB 33 / 39, 45 / 39; 47 MB 43 / 54, 53 / 54)
+// (weights of e4m3 counted at two bytes here.)
+enum class Reading { kBf16InPlace, kOther, kOddE4m3 };
+bool few_rows(int64_t M, int64_t D, int64_t H, int64_t O, Reading how) {
   const double weights = 2.0 * double(H) * (2.0 * double(D) + double(O)), mb = 1 << 20;
-  return M <= 2 || (M <= 4 && weights <= 64 * mb) || (M <= kFewRows && weights <= (bf16_in_place ? 3 : 6) * mb);
+  if (how == Reading::kOddE4m3)
+    return M <= kFewRows && weights <= (M == 1 ? 64 : M == 2 ? 16 : M <= 4 ? 6 : 3) * mb;
+  return M <= 2 || (M <= 4 && weights <= 64 * mb) || (M <= kFewRows && weights <= (how == Reading::kBf16InPlace ? 3 : 6) * mb);
 }
 
 // Room for the product between the two launches: fp32, or [hi; lo], up to kStacked rows.
@@ -1127,7 +1135,7 @@ int gc_gated_ffn_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* Wi
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_bf16: workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Matrix x{X, M, D, ldx, 2}, win{Win, D, 2 * H, ldwin, 2}, wout{Wout, H, O, ldwout, 2};
-  if (few_rows(M, D, H, O, readable(win) && H % 8 == 0 && readable(wout))) {
+  if (few_rows(M, D, H, O, readable(win) && H % 8 == 0 && readable(wout) ? Reading::kBf16InPlace : Reading::kOther)) {
     const Saved keep = saved ? saved_at(saved, M, H) : Saved{};
     const Rows r{X, Win, Wout, nullptr, nullptr, reinterpret_cast<float*>(ws), Y, ldx, ldwin, ldwout,
                  hp, ldy, int(M), int(D), int(H), int(O), act, keep};
@@ -1273,7 +1281,7 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
   GC_REQUIRE(gc::aligned16(workspace), "gc_gated_ffn_forward_e4m3: workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
   Matrix x{X8, M, D, ldx, 1}, w{W8, 2 * H, D, ldw, 1}, wout{Wout, H, O, ldwout, 2};
-  if (few_rows(M, D, H, O, false)) {
+  if (few_rows(M, D, H, O, D % 16 == 0 && readable(x) && readable(w) ? Reading::kOther : Reading::kOddE4m3)) {
     const Rows r{X8, W8, Wout, x_scale, w_scale, reinterpret_cast<float*>(ws), Y, ldx, ldw, ldwout, up8(H), ldy, int(M), int(D),
                  int(H), int(O), act, Saved{}};
     return forward_few_rows(r, true, st);
