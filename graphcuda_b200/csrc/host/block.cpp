@@ -116,6 +116,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
                                double eps, int64_t y_type) {
     const NormForward f = rms_norm_forward(x, weight, residual, eps, int(y_type), true);
     ctx->save_for_backward(norm_saved(f));
+    ctx->set_materialize_grads(false);  // an output that nobody uses has no gradient, not one of zeros
     ctx->saved_data["types"] = y_type | int64_t(type_of(x)) << 2 | int64_t(f.stream.defined()) << 4;
     if (!f.stream.defined()) return {f.y};
     return {f.y, f.stream};

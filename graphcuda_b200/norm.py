@@ -19,6 +19,7 @@ class _TracedNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps, y_type):
         y, stream, saved = _lib.host.rms_norm_forward(x, weight, residual, eps, y_type)
         ctx.save_for_backward(*saved)
+        ctx.set_materialize_grads(False)
         ctx.call = y_type, _TYPES[x.dtype], residual is not None
         return y if residual is None else (y, stream)
 
