@@ -10,8 +10,8 @@
 //
 // Moments in 8 bits: blocks of 256 elements of a tensor share an fp32 scale per moment.  The first is e4m3 (largest
 // value 448); the second, which is never negative, has the upper byte of a positive fp16 number without its sign: 5
-// bits of exponent, 3 of mantissa, largest value 61440.  Both keep 3 to 6 % at most over a range of 2^17 in |m| and in
-// sqrt(v).  With beta2 = 0.999 an average moves by a thousandth of itself in a step, which rounding to nearest would
+// bits of exponent, 3 of mantissa, largest value 61440.  A rounding, up or down, moves m by less than 12.5 % over a range of 2^14.8
+// and sqrt(v) by less than 6.3 % over one of 2^15; below those the codes are evenly spaced.  With beta2 = 0.999 an average moves by a thousandth of itself in a step, which rounding to nearest would
 // lose for good, so values are rounded up or down at random in proportion to the distance; 16 random bits each, from a
 // hash of (seed, step, tensor, element), so that a run can be repeated.  A second moment never falls to zero in a block
 // that holds anything: its smallest code stands for 2^-33 of the block's largest value, and |m| / sqrt(v) stays bounded

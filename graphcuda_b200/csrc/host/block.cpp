@@ -1,4 +1,5 @@
-// What stands between the graph layers of a deep model: the norm of the residual stream, and AdamW over its tensors.
+// What stands between the graph layers of a deep model: the norm of the residual stream and the gated feed-forward block, each with its
+// autograd node and its 8-bit form, and AdamW over the model's tensors.
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <vector>

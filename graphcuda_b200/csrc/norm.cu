@@ -133,7 +133,9 @@ __device__ __forceinline__ typename Op::T reduce(typename Op::T v, typename Op::
   return v;
 }
 
-// The scale of a row in 8 bits and what its elements are multiplied by.  A row whose scale would be subnormal is stored
+// The scale of a row in 8 bits and what its elements are multiplied by: products with rounded reciprocals, which put no more codes on
+// the wrong side of a boundary than a quotient's own rounding (28 against 25 of the 34 M of 8192 x 4096, PyTorch's quotients 28), where
+// dividing every element takes 60 us instead of 41.  A row whose scale would be subnormal is stored
 // as zeros; one with a NaN has a NaN for its scale, one with an infinity an infinity.
 __device__ __forceinline__ float2 scale_of(uint32_t top_bits) {
   const float s = __uint_as_float(top_bits) * (1.0f / 448.0f);

@@ -53,8 +53,11 @@ def gated_ffn(x: torch.Tensor, w_in: torch.Tensor, w_out: torch.Tensor, activati
     """``(act(x @ Wg) * (x @ Wu)) @ w_out`` with ``w_in = [Wg | Wu]``, all bfloat16.
 
     ``x`` is [rows, in], ``w_in`` [in, 2 * hidden], ``w_out`` [hidden, out] (in x out, like GCNConv's weights).  Sums are
-    float32.  The hidden row is rounded to bfloat16 before the second product, and so is the gradient of ``x @ w_in`` in the
-    backward pass; ``x @ w_in`` itself is kept for it to 11 bits, with an exponent for every 32 columns of a row.
+    float32.  Of more than 64 rows the hidden row is rounded to bfloat16 before the second product, and so is the gradient of
+    ``x @ w_in`` in the backward pass: results are off by 2.4e-3 (relative, root mean square), of which the output's own rounding is
+    1.7e-3.  Of 64 rows and fewer both are kept to 16 bits and more, and only the output's rounding shows; so a row's result in a
+    large call differs from that in a small one by as much.  ``x @ w_in`` itself is kept for the backward pass to 11 bits, with an
+    exponent for every 32 columns of a row.
     ``activation``: "silu", "gelu" (with erf) or "relu".  Widths that are multiples of 8 are read in place, others through
     padded copies."""
     act = _act(activation)
@@ -77,7 +80,8 @@ def quantize_weight_fp8(w: torch.Tensor):
 def gated_ffn_fp8(x8: torch.Tensor, x_scale: torch.Tensor, w_in8: torch.Tensor, w_in_scale: torch.Tensor,
                   w_out: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """The block for serving, its first product in 8 bits: ``x8, x_scale`` as ``rms_norm_fp8`` leaves them,
-    ``w_in8, w_in_scale`` from ``quantize_weight_fp8``; ``w_out`` and the result are bfloat16."""
+    ``w_in8, w_in_scale`` from ``quantize_weight_fp8``; ``w_out`` and the result are bfloat16, and the hidden row between the
+    products is rounded as in ``gated_ffn``."""
     act = _act(activation)
     y = _lib.host.gated_ffn_fp8(x8, x_scale, w_in8, w_in_scale, w_out, act)
     return y if y is not None else _TracedFFNFp8.apply(x8, x_scale, w_in8, w_in_scale, w_out, act)

@@ -93,7 +93,7 @@ class FusedSGD(torch.optim.Optimizer):
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, masters=None, scales=None, seed: int = 0, follow: bool = False) -> None:
-    """One AdamW step over lists of tensors, in place; one launch for up to 449 tensors.
+    """One AdamW step over lists of tensors, in place; one launch for up to 449 tensors (688 in float32 alone).
 
     ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
     ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)``.
@@ -119,12 +119,16 @@ def adamw_moments(exp_avgs, exp_avg_sqs, scales, out=None):
 
 
 class FusedAdamW(torch.optim.Optimizer):
-    """AdamW (``torch.optim.AdamW``, amsgrad and maximize off) for any number of tensors in one launch.
+    """AdamW (``torch.optim.AdamW``, amsgrad and maximize off) for any number of tensors, up to 449 to a launch (688 in float32 alone).
 
     Float32 parameters are updated as they are; bfloat16 ones beside a float32 master in the optimizer's state, which follows a
     parameter that others have changed between steps (a state dict loaded, a copy, weights clipped; recorded or not).
     ``state_bits=8`` holds both moments in 8 bits with a float32 scale per 256 elements (see ``adamw_step``): 2 bytes per
-    parameter instead of 8.  Tensors of 256 elements and fewer keep 32 bits: there is nothing to save in them."""
+    parameter instead of 8.  Tensors of 256 elements and fewer keep 32 bits: there is nothing to save in them.
+
+    The lists are gathered in Python on every step, about a microsecond per tensor (480 tensors: 445 us to issue, whatever their
+    size); recorded in a CUDA graph a step takes what its kernels take.  States are made at the first step, and a count of its
+    own when a parameter has no gradient in some step: both before a step is recorded."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
                  state_bits: int = 32, seed: int = 0):
