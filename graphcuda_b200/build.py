@@ -37,7 +37,7 @@ SOURCES = [
     "elementwise.cu",
     "gcn_layer.cu",
     "graph_build.cu",
-    "loss.cu", "optim.cu",
+    "loss.cu", "distill.cu", "optim.cu",
     "norm.cu", "adamw.cu", "ffn.cu", "ffn_rows.cu",
 ]
 

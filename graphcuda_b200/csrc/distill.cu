@@ -1,0 +1,508 @@
+// Distillation loss of a student's logits against a teacher's top logits, and its gradient with respect to the student's.
+//
+//   p_j = softmax over the entries of a row's list of t_j / T        q_c = softmax over all C classes of z_c / T
+//   loss = scale T^2 sum over selected rows of sum_j p_j (log p_j - log q_{i_j})
+//   dZ[r, c] = g scale T (q_c - sum of p_j over the entries with i_j = c)      for rows that count, 0 otherwise
+//
+// An entry whose index is no class, or whose logit is -inf, is none; a row without entries does not count.  The logits are read
+// once forward (a running maximum and sum) and once backward, where the row's four statistics are at hand; probabilities
+// come from one exponential each, and nothing but dZ is written.  Sums and statistics are fp32.  With u = (z - max) log2(e) / T the
+// subtraction comes before the product, so that a row filled with the type's lowest value does not overflow.
+//
+// G threads take a row: 8 up to 256 classes (a row is few vectors, and what a row costs beside them is shared by fewer), a warp up to
+// 4096, a CTA of 512 above; with fewer rows than SMs a CTA takes a part of a row (kParts) and another launch puts the parts
+// together.  Rows may start anywhere: what lies before the first and behind the last 16-byte vector is read by itself.
+#include "common.cuh"
+#include "ffn_internal.cuh"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+namespace {
+
+using gc::ffn::both;
+using gc::ffn::each;
+using gc::ffn::exp2_approx;
+using gc::ffn::F2;
+using gc::ffn::fma2;
+
+constexpr int kBlocks = gc::kNumSMs * 8;  // partial sums of the loss
+constexpr int kMaxParts = 16;             // of a row
+constexpr int kMaxList = 1024;            // entries of a list
+constexpr int kWide = 512;                // threads of a CTA that takes a row, or a part of one
+constexpr int kShortList = 32;            // entries up to which 8 threads take a row
+constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
+
+struct Problem {
+  const void* z;
+  const void* top;
+  const void* index;
+  const uint8_t* mask;  // null: all rows
+  int64_t ldz, ldt, ldi, M;
+  int C, k, parts;
+  bool top16, index64;
+  float a;  // log2(e) / T
+};
+
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ------------------------------------------------------------------ groups of threads
+// Reductions over the G threads of a row; all of them get the result.  For a CTA `sh` holds a word per warp.
+template <int G, class F>
+__device__ __forceinline__ float over_group(float v, float* sh, F&& f) {
+#pragma unroll
+  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if constexpr (G > 32) {
+    __syncthreads();  // the words' last readers are done
+    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < G / 32; ++w) v = f(v, sh[w]);
+  }
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v, float* sh) {
+  return over_group<G>(v, sh, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float* sh) {
+  return over_group<G>(v, sh, [](float a, float b) { return a + b; });
+}
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (G > 32) __syncthreads();
+  else if constexpr (G == 32) __syncwarp();
+  else __syncwarp(((1u << G) - 1) << (threadIdx.x % 32 / G * G));
+}
+
+// ------------------------------------------------------------------ logits
+template <class T>
+__device__ __forceinline__ float as_float(T v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else return __bfloat162float(v);
+}
+// A vector of 16 bytes as pairs of floats.
+template <class T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T), P = N / 2;
+};
+template <class T>
+__device__ __forceinline__ void unpack(const uint4& v, F2 (&f)[Vec<T>::P]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (sizeof(T) == 4) {
+    f[0] = F2(w[0], w[1]);
+    f[1] = F2(w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = F2(w[i] << 16, w[i] & 0xFFFF0000u);
+  }
+}
+template <class T>
+__device__ __forceinline__ float vec_max(const uint4& v) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  } else {
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const float2 m = __bfloat1622float2(__hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])));
+    return fmaxf(m.x, m.y);
+  }
+}
+template <class T>
+__device__ __forceinline__ uint4 nothing() {  // a vector of -inf
+  const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+  return make_uint4(w, w, w, w);
+}
+// Elements before the first 16-byte boundary at or behind p.
+template <class T>
+__device__ __forceinline__ int before_vectors(const T* p, int n) {
+  return min(n, int((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(T)));
+}
+
+// A maximum m and the sum of 2^((z - m) a), of nothing at first.  (Of a row of -inf the sum is zero; of one with +inf or a NaN, a NaN.)
+struct Running {
+  float m = -INFINITY, s = 0.f;
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+  __device__ __forceinline__ void raise(float to, float a) {
+    if (to > m) {
+      s *= exp2_approx((m - to) * a);
+      m = to;
+    }
+  }
+};
+
+template <class T, int G>
+__device__ __forceinline__ Running scan(const T* __restrict__ z, int n, int rank, float a) {
+  constexpr int U = G == 8 ? 2 : 4;
+  Running r;
+  const int head = before_vectors(z, n), vectors = (n - head) / Vec<T>::N, tail = head + vectors * Vec<T>::N;
+  const uint4* v = reinterpret_cast<const uint4*>(z + head);
+  // what no vector holds, fewer than 8 elements at either end
+  float ends[2] = {-INFINITY, -INFINITY};
+  if (rank < head) ends[0] = as_float(z[rank]);
+  if (rank < n - tail) ends[1] = as_float(z[tail + rank]);
+  for (int i = rank; i < vectors; i += G * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = i + u * G < vectors ? __ldg(v + i + u * G) : nothing<T>();
+    float top = vec_max<T>(w[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) top = fmaxf(top, vec_max<T>(w[u]));
+    r.raise(top, a);
+    const F2 base = both(-r.base()), scale = both(a);
+    F2 sum = both(0.f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      F2 f[Vec<T>::P];
+      unpack<T>(w[u], f);
+#pragma unroll
+      for (int e = 0; e < Vec<T>::P; ++e) sum = sum + each((f[e] + base) * scale, [](float x) { return exp2_approx(x); });
+    }
+    float x, y;
+    sum.get(x, y);
+    r.s += x + y;
+  }
+  r.raise(fmaxf(ends[0], ends[1]), a);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r.s += exp2_approx((ends[i] - r.base()) * a);
+  return r;
+}
+// The group's threads together.
+template <int G>
+__device__ __forceinline__ Running combined(Running r, float a, float* sh) {
+  Running all;
+  all.m = group_max<G>(r.m, sh);
+  all.s = group_sum<G>(r.m == -INFINITY ? r.s : r.s * exp2_approx((r.m - all.m) * a), sh);
+  return all;
+}
+
+// ------------------------------------------------------------------ lists
+struct Entry {
+  float t;
+  int c;  // below zero: none
+};
+__device__ __forceinline__ Entry entry(const Problem& p, int64_t r, int j) {
+  const int64_t at = r * p.ldi + j;
+  const int64_t c = p.index64 ? __ldg(static_cast<const int64_t*>(p.index) + at) : __ldg(static_cast<const int32_t*>(p.index) + at);
+  const int64_t ta = r * p.ldt + j;
+  Entry e;
+  e.t = p.top16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.top)[ta]) : __ldg(static_cast<const float*>(p.top) + ta);
+  e.c = c >= 0 && c < p.C && e.t != -INFINITY ? int(c) : -1;
+  return e;
+}
+
+// Of a row: the student's maximum and the logarithm (base 2) of its sum, and the teacher's.  A row that does not count has +inf
+// for the last, which no other has.
+struct Stats {
+  float zm, zl, tm, tl;
+};
+
+// The parts of a row's columns begin at multiples of this.
+__device__ __host__ __forceinline__ int part_columns(int C, int parts) { return ((C + parts - 1) / parts + 63) / 64 * 64; }
+
+// Part `blockIdx.x` of row `blockIdx.y`.
+template <class T>
+__global__ void __launch_bounds__(kWide)
+distill_part_kernel(const __grid_constant__ Problem p, float2* __restrict__ out) {
+  __shared__ float sh[kWide / 32];
+  const int64_t r = blockIdx.y;
+  if (p.mask && !p.mask[r]) return;
+  const int width = part_columns(p.C, p.parts), from = min(p.C, int(blockIdx.x) * width), n = min(width, p.C - from);
+  const Running x = combined<kWide>(scan<T, kWide>(static_cast<const T*>(p.z) + r * p.ldz + from, n, threadIdx.x, p.a), p.a, sh);
+  if (threadIdx.x == 0) out[r * p.parts + blockIdx.x] = make_float2(x.m, x.s);
+}
+
+// G threads per row; the block's sum of losses goes to partials.  from_parts: what the kernel above left, or null.
+template <class T, int G>
+__global__ void __launch_bounds__(G > 32 ? G : 256)
+distill_forward_kernel(const __grid_constant__ Problem p, const float2* __restrict__ from_parts, Stats* __restrict__ stats,
+                       float* __restrict__ partials) {
+  constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G;  // rows of a CTA at a time
+  __shared__ float sh[32];
+  const int rank = threadIdx.x % G;
+  float loss = 0.f;
+  for (int64_t r0 = int64_t(blockIdx.x) * R; r0 < p.M; r0 += int64_t(gridDim.x) * R) {  // the same for all of a CTA
+    const int64_t mine = r0 + threadIdx.x / G, r = min(mine, p.M - 1);
+    const bool chosen = mine < p.M && (!p.mask || p.mask[r]);
+    const T* z = static_cast<const T*>(p.z) + r * p.ldz;
+    // the list: its largest logit
+    float tm = -INFINITY;
+    bool any = false;
+    for (int j = rank; chosen && j < p.k; j += G) {
+      const Entry e = entry(p, r, j);
+      if (e.c >= 0) tm = fmaxf(tm, e.t), any = true;
+    }
+    tm = group_max<G>(tm, sh);
+    any = group_max<G>(any ? 1.f : 0.f, sh) > 0.f;
+    const bool counts = chosen && any;
+    if (G > 32 && !counts) {
+      if (threadIdx.x == 0) stats[r] = {0.f, 0.f, 0.f, INFINITY};
+      continue;
+    }
+    Running x;
+    if (counts) {
+      if (from_parts) {
+        for (int i = rank; i < p.parts; i += G) {
+          const float2 part = from_parts[r * p.parts + i];
+          x.raise(part.x, p.a);
+          x.s += part.x == -INFINITY ? part.y : part.y * exp2_approx((part.x - x.m) * p.a);
+        }
+      } else {
+        x = scan<T, G>(z, p.C, rank, p.a);
+      }
+    }
+    x = combined<G>(x, p.a, sh);
+    // sum of the list's exponentials, and of their products with what the logarithms differ by
+    float s = 0.f, d = 0.f;
+    for (int j = rank; counts && j < p.k; j += G) {
+      const Entry e = entry(p, r, j);
+      if (e.c < 0) continue;
+      const float w = exp2_approx((e.t - tm) * p.a);
+      s += w;
+      if (!(w == 0.f)) d += w * (((e.t - tm) - (as_float(z[e.c]) - x.m)) * p.a);
+    }
+    s = group_sum<G>(s, sh);
+    d = group_sum<G>(d, sh);
+    if (rank == 0 && mine < p.M) {
+      const Stats st = {x.m, log2_approx(x.s), tm, counts ? log2_approx(s) : INFINITY};
+      stats[r] = counts ? st : Stats{0.f, 0.f, 0.f, INFINITY};
+      if (counts) loss += kLn2 * (d / s - st.tl + st.zl);
+    }
+  }
+  loss = over_group<(G > 32 ? G : 256)>(loss, sh, [](float a, float b) { return a + b; });
+  if (threadIdx.x == 0) partials[blockIdx.x] = loss;
+}
+
+__global__ void __launch_bounds__(256)
+distill_sum_kernel(const float* __restrict__ partials, int n, float scale, float* __restrict__ loss) {
+  __shared__ double sh[256];
+  double a = 0.;
+  for (int i = threadIdx.x; i < n; i += 256) a += partials[i];
+  sh[threadIdx.x] = a;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (threadIdx.x < o) sh[threadIdx.x] += sh[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *loss = float(sh[0] * scale);
+}
+
+// ------------------------------------------------------------------ gradient
+template <class T>
+__device__ __forceinline__ uint4 pack(const F2 (&f)[Vec<T>::P]) {
+  uint32_t w[4];
+  float x, y;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f[i].get(x, y);
+      w[2 * i] = __float_as_uint(x);
+      w[2 * i + 1] = __float_as_uint(y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i].get(x, y);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <class T>
+__device__ __forceinline__ T rounded(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else return __float2bfloat16_rn(v);
+}
+
+// G threads per row, or per part of one (G = kWide).  Rows are taken from the last to the first: the forward pass, which has mostly
+// just run, left the last ones in the L2.  `pad`: columns of zeros behind a row of dZ.
+template <class T, int G>
+__global__ void __launch_bounds__(G > 32 ? G : 256)
+distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restrict__ stats, const float* __restrict__ grad, float factor,
+                        T* __restrict__ dz, int64_t lddz, int pad) {
+  constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G, U = G == 8 ? 2 : 4;
+  extern __shared__ __align__(16) uint8_t lists[];  // of each of the CTA's rows: the entries' classes, then their probabilities
+  const int rank = threadIdx.x % G, kp = (p.k + 3) / 4 * 4;
+  int* cls = reinterpret_cast<int*>(lists) + (threadIdx.x / G) * 2 * kp;
+  float* prob = reinterpret_cast<float*>(cls + kp);
+  const float g = factor * __ldg(grad);
+  const int width = p.parts > 1 ? part_columns(p.C, p.parts) : p.C;
+  const int64_t items = p.M * p.parts;
+  for (int64_t i0 = int64_t(blockIdx.x) * R; i0 < items; i0 += int64_t(gridDim.x) * R) {
+    const int64_t item = items - 1 - (i0 + threadIdx.x / G);
+    group_sync<G>();  // the lists of the row before are read
+    if (item < 0) continue;  // only in groups of a warp or less, whose other rows exist
+    const int64_t r = item / p.parts;
+    const int from = min(p.C, int(item - r * p.parts) * width), n = min(width, p.C - from);
+    const bool last = int(item - r * p.parts) == p.parts - 1;
+    const T* z = static_cast<const T*>(p.z) + r * p.ldz + from;
+    T* d = dz + r * lddz + from;
+    const Stats st = stats[r];
+    const bool counts = !(st.tl == INFINITY);
+    if (last && rank < pad) dz[r * lddz + p.C + rank] = rounded<T>(0.f);
+    if (counts)
+      for (int j = rank; j < kp; j += G) {
+        Entry e{0.f, -1};
+        if (j < p.k) e = entry(p, r, j);
+        cls[j] = e.c;
+        prob[j] = e.c < 0 ? 0.f : exp2_approx((e.t - st.tm) * p.a - st.tl);
+      }
+    auto one = [&](float v) { return g * exp2_approx((v - st.zm) * p.a - st.zl); };
+    const int head = before_vectors(d, n);
+    const bool vectors_fit = (reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(d)) % 16 == 0;
+    const int vectors = vectors_fit ? (n - head) / Vec<T>::N : 0, tail = vectors_fit ? head + vectors * Vec<T>::N : head;
+    if (rank < head) d[rank] = rounded<T>(counts ? one(as_float(z[rank])) : 0.f);
+    for (int c = tail + rank; c < n; c += G) d[c] = rounded<T>(counts ? one(as_float(z[c])) : 0.f);
+    const uint4* v = reinterpret_cast<const uint4*>(z + head);
+    uint4* to = reinterpret_cast<uint4*>(d + head);
+    const F2 m = both(-st.zm), a = both(p.a), l = both(-st.zl), gg = both(g);
+    for (int i = rank; i < vectors; i += G * U) {
+      uint4 w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = counts && i + u * G < vectors ? __ldg(v + i + u * G) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        F2 f[Vec<T>::P];
+        unpack<T>(w[u], f);
+#pragma unroll
+        for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e] + m, a, l), [](float x) { return exp2_approx(x); }) * gg;
+        if (i + u * G < vectors) __stcs(to + i + u * G, counts ? pack<T>(f) : make_uint4(0, 0, 0, 0));
+      }
+    }
+    group_sync<G>();  // the lists, and the columns that the entries below write again
+    if (!counts) continue;
+    for (int j = rank; j < p.k; j += G) {
+      const int c = cls[j];
+      if (c < from || c >= from + n) continue;
+      float sum = 0.f;  // an index may stand in the list more than once: all of its entries write the same
+      for (int i = 0; i < kp; i += 4) {
+        const int4 ci = *reinterpret_cast<const int4*>(cls + i);
+        const float4 pi = *reinterpret_cast<const float4*>(prob + i);
+        sum += (ci.x == c ? pi.x : 0.f) + (ci.y == c ? pi.y : 0.f) + (ci.z == c ? pi.z : 0.f) + (ci.w == c ? pi.w : 0.f);
+      }
+      d[c - from] = rounded<T>(g * (exp2_approx((as_float(z[c - from]) - st.zm) * p.a - st.zl) - sum));
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+int threads_per_row(int64_t C, int64_t k) { return C > 4096 ? kWide : C <= 256 && k <= kShortList ? 8 : 32; }
+// Rows above 8192 columns of which there are fewer than SMs are cut, into parts of 4096 or more.
+int parts_of(int64_t M, int64_t C) {
+  if (M >= gc::kNumSMs || C <= 8192) return 1;
+  return int(std::max<int64_t>(1, std::min<int64_t>({2 * gc::kNumSMs / std::max<int64_t>(M, 1), C / 4096, kMaxParts})));
+}
+unsigned grid_of(int64_t M, int G) {
+  const int rows = G > 32 ? 1 : 256 / G;
+  return unsigned(std::min<int64_t>(gc::ceil_div(M, rows), kBlocks));
+}
+
+int fill(Problem& p, const char* what, const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt,
+         const void* index, int index_bits, int64_t ldi, int64_t M, int64_t C, int64_t k, float temperature) {
+  GC_REQUIRE(M >= 0 && C >= 1 && k >= 0, "%s: bad size", what);
+  GC_REQUIRE((type == GC_TYPE_F32 || type == GC_TYPE_BF16) && (top_type == GC_TYPE_F32 || top_type == GC_TYPE_BF16),
+             "%s: logits are float32 or bfloat16", what);
+  GC_REQUIRE(index_bits == 32 || index_bits == 64, "%s: indices have 32 or 64 bits", what);
+  GC_REQUIRE(temperature > 0.f && temperature < INFINITY && kLog2e / temperature < INFINITY,
+             "%s: the temperature must be positive and finite, and so its reciprocal", what);
+  GC_REQUIRE(ldz >= C && ldt >= k && ldi >= k, "%s: leading dimension below the row length", what);
+  if (C > (1 << 30) || k > kMaxList) return gc::fail(GC_ERR_UNSUPPORTED, "%s: more than %d entries to a list, or too many classes", what, kMaxList);
+  GC_REQUIRE(M == 0 || (Z && (k == 0 || (top && index))), "%s: null pointer", what);
+  p = Problem{Z, top, index, nullptr, ldz, ldt, ldi, M, int(C), int(k), parts_of(M, C), top_type == GC_TYPE_BF16, index_bits == 64,
+              kLog2e / temperature};
+  return GC_OK;
+}
+template <class F>
+void with_group(int G, F&& f) {
+  if (G == 8) f(std::integral_constant<int, 8>{});
+  else if (G == 32) f(std::integral_constant<int, 32>{});
+  else f(std::integral_constant<int, kWide>{});
+}
+template <class F>
+void with_type(int type, F&& f) {
+  if (type == GC_TYPE_F32) f(float{});
+  else f(__nv_bfloat16{});
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gc_distill_workspace_bytes(int64_t M, int64_t C) {
+  if (M < 0 || C < 1) return 0;
+  return size_t(kBlocks) * sizeof(float) + (parts_of(M, C) > 1 ? size_t(M) * kMaxParts * sizeof(float2) : 0);
+}
+
+int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
+                       int index_bits, int64_t ldi, const uint8_t* row_mask, int64_t M, int64_t C, int64_t k, float temperature,
+                       float scale, float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+  Problem p;
+  const int rc = fill(p, "gc_distill_forward", Z, type, ldz, top, top_type, ldt, index, index_bits, ldi, M, C, k, temperature);
+  if (rc != GC_OK) return rc;
+  GC_REQUIRE(loss && (M == 0 || stats), "gc_distill_forward: null pointer");
+  GC_REQUIRE(gc::aligned16(stats), "gc_distill_forward: the statistics must be 16-byte aligned");
+  const cudaStream_t st = gc::as_stream(stream);
+  if (M == 0) {
+    const cudaError_t e = cudaMemsetAsync(loss, 0, sizeof(float), st);
+    return e == cudaSuccess ? GC_OK : gc::fail(GC_ERR_CUDA, "gc_distill_forward: %s", cudaGetErrorString(e));
+  }
+  if (!workspace || workspace_bytes < gc_distill_workspace_bytes(M, C))
+    return gc::fail(GC_ERR_WORKSPACE, "gc_distill_forward: workspace missing or smaller than its query says");
+  GC_REQUIRE(gc::aligned16(workspace), "gc_distill_forward: workspace must be 16-byte aligned");
+  p.mask = row_mask;
+  float* partials = static_cast<float*>(workspace);
+  float2* parts = p.parts > 1 ? reinterpret_cast<float2*>(partials + kBlocks) : nullptr;
+  const int G = parts ? 32 : threads_per_row(C, k);
+  const unsigned grid = grid_of(M, G);
+  with_type(type, [&](auto t) {
+    using T = decltype(t);
+    if (parts) distill_part_kernel<T><<<dim3(unsigned(p.parts), unsigned(M)), kWide, 0, st>>>(p, parts);
+    with_group(G, [&](auto gt) {
+      constexpr int kG = decltype(gt)::value;
+      distill_forward_kernel<T, kG><<<grid, kG > 32 ? kG : 256, 0, st>>>(p, parts, reinterpret_cast<Stats*>(stats), partials);
+    });
+  });
+  distill_sum_kernel<<<1, 256, 0, st>>>(partials, int(grid), scale * temperature * temperature, loss);
+  return gc::check_launch("gc_distill_forward", parts ? 3 : 2);
+}
+
+int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
+                        int index_bits, int64_t ldi, const float* stats, int64_t M, int64_t C, int64_t k, float temperature,
+                        float scale, const float* grad_loss, void* dZ, int64_t lddz, int64_t pad, void* stream) {
+  Problem p;
+  const int rc = fill(p, "gc_distill_backward", Z, type, ldz, top, top_type, ldt, index, index_bits, ldi, M, C, k, temperature);
+  if (rc != GC_OK) return rc;
+  GC_REQUIRE(pad >= 0 && pad < 8 && lddz >= C + pad, "gc_distill_backward: leading dimension below the row length");
+  if (M == 0) return GC_OK;
+  GC_REQUIRE(stats && grad_loss && dZ, "gc_distill_backward: null pointer");
+  GC_REQUIRE(gc::aligned16(stats), "gc_distill_backward: the statistics must be 16-byte aligned");
+  const int G = threads_per_row(C, k);
+  const int rows = G > 32 ? 1 : 256 / G, kp = int((k + 3) / 4 * 4);
+  const size_t smem = size_t(rows) * 2 * kp * 4;
+  const unsigned grid = unsigned(std::min<int64_t>(gc::ceil_div(M * p.parts, rows), int64_t(1) << 30));
+  int bad = GC_OK;
+  with_type(type, [&](auto t) {
+    using T = decltype(t);
+    with_group(G, [&](auto gt) {
+      constexpr int kG = decltype(gt)::value;
+      auto kern = distill_backward_kernel<T, kG>;
+      if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (e != cudaSuccess) bad = gc::fail(GC_ERR_CUDA, "gc_distill_backward: %s", cudaGetErrorString(e));
+      }
+      if (bad == GC_OK)
+        kern<<<grid, kG > 32 ? kG : 256, smem, gc::as_stream(stream)>>>(p, reinterpret_cast<const Stats*>(stats), grad_loss,
+                                                                         scale * temperature, static_cast<T*>(dZ), lddz, int(pad));
+    });
+  });
+  return bad != GC_OK ? bad : gc::check_launch("gc_distill_backward");
+}
+
+}  // extern "C"

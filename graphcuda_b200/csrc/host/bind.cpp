@@ -265,6 +265,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return std::make_tuple(f.loss, f.Z, f.labels, f.ws, f.masked);
   }, NoGil());
   m.def("nll_backward", &nll_backward, NoGil());
+  m.def("distill_loss", [](const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
+                           double scale) -> OptTensor {
+    require(!recorded({&top}), "distill_loss has no gradient for the teacher: pass its logits detached");
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return distill_loss(Z, top, index, row_mask, temperature, scale);
+  }, NoGil());
+  m.def("distill_forward", [](const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
+                              double scale) {
+    const DistillForward f = distill_forward(Z, top, index, row_mask, temperature, scale);
+    return std::make_tuple(f.loss, std::vector<Tensor>{f.Z, f.top, f.index, f.stats});
+  }, NoGil());
+  m.def("distill_backward", &distill_backward, NoGil());
   m.def("argmax_accuracy", [](const Tensor& logits, const OptTensor& labels, const std::optional<std::vector<Tensor>>& masks,
                               bool want_pred) -> std::optional<std::pair<Tensor, Tensor>> {
     if (torch::jit::tracer::isTracing()) return std::nullopt;

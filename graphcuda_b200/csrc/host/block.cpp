@@ -18,20 +18,19 @@ int type_of(const Tensor& t) {
 }
 bool f32_or_bf16(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
 bool dual(const Tensor& t) { return t._fw_grad(0).defined(); }
-// Whether a call has to become a node of the graph: a gradient may be asked for, or a tangent has to be refused.
+Tensor empty_like_rows(int64_t rows, int64_t cols, at::ScalarType type, const at::Device& dev) {
+  return at::empty({rows, cols}, at::TensorOptions().dtype(type).device(dev));
+}
+}  // namespace
+
 bool recorded(std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
     if (t && t->defined() && ((c10::GradMode::is_enabled() && t->requires_grad()) || dual(*t))) return true;
   return false;
 }
-// Backward passes here are kernels, which autograd cannot differentiate again.
 void once(const char* what) {
   if (c10::GradMode::is_enabled()) raise(std::string(what) + " has no second derivative (create_graph)");
 }
-Tensor empty_like_rows(int64_t rows, int64_t cols, at::ScalarType type, const at::Device& dev) {
-  return at::empty({rows, cols}, at::TensorOptions().dtype(type).device(dev));
-}
-}  // namespace
 
 // ------------------------------------------------------------------ norm
 NormForward rms_norm_forward(const Tensor& xin, const Tensor& weight, const OptTensor& residual, double eps, int y_type,

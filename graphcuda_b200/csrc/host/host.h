@@ -49,7 +49,7 @@ inline bool f32_on(const Tensor& t, const at::Device& dev) {
   X(gc_rms_norm_forward) X(gc_rms_norm_backward_workspace_bytes) X(gc_rms_norm_backward) X(gc_adamw_step)           \
   X(gc_adamw_moments_f32) X(gc_gated_ffn_saved_bytes) X(gc_gated_ffn_workspace_bytes)                              \
   X(gc_gated_ffn_forward_bf16) X(gc_gated_ffn_backward_bf16) X(gc_gated_ffn_e4m3_workspace_bytes)                   \
-  X(gc_gated_ffn_forward_e4m3)
+  X(gc_gated_ffn_forward_e4m3) X(gc_distill_workspace_bytes) X(gc_distill_forward) X(gc_distill_backward)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
   GC_HOST_FUNCTIONS(X)
@@ -156,6 +156,11 @@ std::tuple<Tensor, Tensor, Tensor> degree_order(const Tensor& edge_index, int64_
 std::tuple<Tensor, Tensor, Tensor> edges_to_csr(const Tensor& edge_index, int64_t n, bool self_loops,
                                                 const OptTensor& relabel);
 
+// Whether a call has to become a node of the graph: a gradient may be asked for, or a tangent has to be refused.
+bool recorded(std::initializer_list<const Tensor*> inputs);
+// Backward passes here are kernels, which autograd cannot differentiate again.
+void once(const char* what);
+
 // ------------------------------------------------------------------ layer, loss, optimizers (layer.cpp, tail.cpp)
 struct Forward {
   Tensor Y, mask, inter;  // inter: A X when the aggregation came first, undefined otherwise
@@ -190,6 +195,17 @@ NllForward nll_forward(const Tensor& Z, const Tensor& labels, const OptTensor& r
 Tensor nll_backward(const Tensor& grad, const Tensor& Z, const Tensor& labels, const Tensor& ws, bool masked,
                     double scale);
 Tensor nll_loss(const Tensor& Z, const Tensor& labels, const OptTensor& row_mask, double scale);
+
+// The distillation loss, and what its backward pass needs.
+struct DistillForward {
+  Tensor loss, Z, top, index, stats;  // as the kernels took them
+};
+DistillForward distill_forward(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
+                               double scale);
+Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats,
+                        double temperature, double scale);
+Tensor distill_loss(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
+                    double scale);
 std::pair<Tensor, Tensor> argmax_accuracy(const Tensor& logits, const OptTensor& labels,
                                           const std::optional<std::vector<Tensor>>& masks, bool want_pred);
 void adam_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,

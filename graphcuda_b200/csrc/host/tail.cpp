@@ -99,6 +99,104 @@ Tensor nll_loss(const Tensor& Z, const Tensor& labels, const OptTensor& row_mask
   return NllFunction::apply(Z, labels, row_mask, scale);
 }
 
+// ------------------------------------------------------------------ distillation
+namespace {
+bool f32_or_bf16(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+int type_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? GC_TYPE_F32 : GC_TYPE_BF16; }
+int bits_of(const Tensor& index) { return index.scalar_type() == at::kLong ? 64 : 32; }
+}  // namespace
+
+DistillForward distill_forward(const Tensor& Zin, const Tensor& top, const Tensor& index, const OptTensor& row_mask,
+                               double temperature, double scale) {
+  require(Zin.dim() == 2 && Zin.is_cuda() && f32_or_bf16(Zin), "distill_loss: logits must be a float32 or bfloat16 CUDA matrix");
+  const at::Device dev = Zin.device();
+  const int64_t M = Zin.size(0), C = Zin.size(1);
+  require(C >= 1, "distill_loss: logits have no classes");
+  require(top.dim() == 2 && top.device() == dev && f32_or_bf16(top) && top.size(0) == M,
+          "distill_loss: top_logits must be a float32 or bfloat16 matrix with a row per row of the logits, on their device");
+  require(index.device() == dev && (index.scalar_type() == at::kLong || index.scalar_type() == at::kInt) &&
+              index.sizes() == top.sizes(),
+          "distill_loss: top_index must be int64 or int32 of top_logits' shape, on its device");
+  require(top.size(1) <= 1024, "distill_loss: at most 1024 entries to a row");
+  Tensor mask8;
+  if (row_mask && row_mask->defined()) {
+    require(row_mask->device() == dev && row_mask->numel() == M,
+            "distill_loss: row_mask must have one entry per row, on the logits' device");
+    require(row_mask->scalar_type() == at::kBool || row_mask->scalar_type() == at::kByte,
+            "distill_loss: row_mask must be bool or uint8");
+    mask8 = row_mask->contiguous();
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  DistillForward f;
+  f.Z = row_major(Zin);
+  f.top = row_major(top);
+  f.index = row_major(index);
+  const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
+  f.stats = at::empty({M, 4}, f32);
+  f.loss = at::empty({}, f32);
+  const Scratch ws = scratch(kSpmm, abi.gc_distill_workspace_bytes(M, C), dev);
+  check(abi.gc_distill_forward(f.Z.const_data_ptr(), type_of(f.Z), ld_of(f.Z), f.top.const_data_ptr(), type_of(f.top), ld_of(f.top),
+                               f.index.const_data_ptr(), bits_of(f.index), ld_of(f.index),
+                               mask8.defined() ? static_cast<const uint8_t*>(mask8.data_ptr()) : nullptr, M, C, top.size(1),
+                               float(temperature), float(scale), f.loss.data_ptr<float>(), f.stats.data_ptr<float>(), ws.ptr,
+                               ws.bytes, stream_of(dev)),
+        "gc_distill_forward");
+  return f;
+}
+
+Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats,
+                        double temperature, double scale) {
+  const int64_t M = Z.size(0), C = Z.size(1), ldz = ld_of(Z);
+  const at::Device dev = Z.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  // Rows of the gradient start as many bytes behind a 16-byte boundary as the logits' own, so that both go in vectors.  Where the
+  // logits are a view of a matrix padded to 16-byte rows (an odd class count), its pad columns become zero, so that the layer below
+  // can aggregate it without re-padding a copy (as in nll_backward).
+  const int64_t vec = 16 / Z.element_size(), lddz = std::max<int64_t>(C, 1) + (ldz - C) % vec;
+  Tensor buf = at::empty({M, lddz}, Z.options());
+  int64_t pad = 0;
+  if (M > 1 && C < lddz && ldz == lddz && lddz % 4 == 0 && lddz <= C + 3 && Z.scalar_type() == at::kFloat &&
+      reinterpret_cast<uintptr_t>(Z.data_ptr()) % 16 == 0) {
+    pad = lddz - C;
+    register_zero_padded(buf);
+  }
+  const Tensor dZ = lddz == C ? buf : buf.narrow(1, 0, C);
+  const Tensor g = grad.to(at::kFloat).contiguous();
+  check(abi.gc_distill_backward(Z.const_data_ptr(), type_of(Z), ldz, top.const_data_ptr(), type_of(top), ld_of(top),
+                                index.const_data_ptr(), bits_of(index), ld_of(index), stats.const_data_ptr<float>(), M, C, top.size(1),
+                                float(temperature), float(scale), g.const_data_ptr<float>(), buf.data_ptr(), lddz, pad,
+                                stream_of(dev)),
+        "gc_distill_backward");
+  return dZ;
+}
+
+namespace {
+struct DistillFunction : torch::autograd::Function<DistillFunction> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& Z, const Tensor& top, const Tensor& index,
+                        const OptTensor& row_mask, double temperature, double scale) {
+    const DistillForward f = distill_forward(Z, top, index, row_mask, temperature, scale);
+    ctx->save_for_backward({f.Z, f.top, f.index, f.stats});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["scale"] = scale;
+    return f.loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    once("distill_loss");
+    const auto saved = ctx->get_saved_variables();
+    return {distill_backward(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["temperature"].toDouble(),
+                             ctx->saved_data["scale"].toDouble()),
+            Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+}  // namespace
+
+Tensor distill_loss(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
+                    double scale) {
+  if (!recorded({&Z, &top})) return distill_forward(Z, top, index, row_mask, temperature, scale).loss;
+  return DistillFunction::apply(Z, top, index, row_mask, temperature, scale);
+}
+
+// ------------------------------------------------------------------ evaluation
 std::pair<Tensor, Tensor> argmax_accuracy(const Tensor& logits, const OptTensor& labels_in,
                                           const std::optional<std::vector<Tensor>>& masks, bool want_pred) {
   require(logits.is_cuda() && logits.dim() == 2 && logits.scalar_type() == at::kFloat,

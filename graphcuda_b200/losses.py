@@ -24,6 +24,23 @@ class _TracedLoss(torch.autograd.Function):
         return _lib.host.nll_backward(grad_loss, *ctx.saved_tensors, *ctx.call), None, None, None
 
 
+class _TracedDistillation(torch.autograd.Function):
+    """The distillation loss inside torch.jit.trace."""
+
+    @staticmethod
+    def forward(ctx, logits, top_logits, top_index, row_mask, temperature, scale):
+        loss, saved = _lib.host.distill_forward(logits, top_logits, top_index, row_mask, temperature, scale)
+        ctx.save_for_backward(*saved)
+        ctx.call = temperature, scale
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad_loss):
+        if torch.is_grad_enabled():
+            raise RuntimeError("distill_loss has no second derivative (create_graph)")
+        return (_lib.host.distill_backward(grad_loss, *ctx.saved_tensors, *ctx.call),) + (None,) * 5
+
+
 class _TracedAccuracy(torch.autograd.Function):
     """Predictions and counts inside torch.jit.trace: those of them that are asked for."""
 
@@ -51,6 +68,28 @@ def log_softmax_nll_loss(logits: torch.Tensor, labels: torch.Tensor, row_mask: O
         scale = 1.0 / max(cnt, 1)
     loss = _lib.host.nll_loss(logits, labels, row_mask, scale)
     return loss if loss is not None else _TracedLoss.apply(logits, labels, row_mask, scale)
+
+
+def distill_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_index: torch.Tensor,
+                 row_mask: Optional[torch.Tensor] = None, temperature: float = 1.0, *,
+                 scale: Optional[float] = None) -> torch.Tensor:
+    """Divergence of a small model's answers from a large one's, of which the largest logits were kept:
+    ``scale * temperature**2 * sum over rows of KL(p || q)`` with ``p`` the softmax of ``top_logits / temperature`` over a row's
+    entries and ``q`` the softmax of ``logits / temperature`` over all classes.
+
+    ``logits`` is [rows, classes], ``top_logits`` and ``top_index`` (int64 or int32) are [rows, k] with k up to 1024, as
+    ``teacher_logits.topk(k)`` returns them; logits are float32 or bfloat16, and so is the gradient.  An entry whose index is
+    outside [0, classes) (-1, where a row has fewer) or whose logit is -inf is none; a row without entries, or that
+    ``row_mask`` (bool or uint8) leaves out, adds nothing and gets a gradient of zeros.  ``scale`` defaults to 1 / (number of rows
+    that ``row_mask`` selects), as in ``log_softmax_nll_loss``.  The factor temperature**2 keeps the gradient's size (it
+    has one 1 / temperature of the student's and one of the teacher's slope).  The teacher has no gradient."""
+    if scale is None:
+        cnt = int(row_mask.sum().item()) if row_mask is not None else logits.size(0)
+        scale = 1.0 / max(cnt, 1)
+    loss = _lib.host.distill_loss(logits, top_logits, top_index, row_mask, temperature, scale)
+    if loss is not None:
+        return loss
+    return _TracedDistillation.apply(logits, top_logits, top_index, row_mask, temperature, scale)
 
 
 def argmax_accuracy(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, masks=None, *,

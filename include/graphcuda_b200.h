@@ -390,6 +390,26 @@ int gc_logsoftmax_nll_backward_pad_f32(const float* Z, int64_t ldz, const int64_
                                    float* dZ, int64_t lddz, const void* workspace, void* stream);
 
 /*
+ * Distillation: the loss of a student's logits Z [M, C] against the teacher's `k` top logits of every row, top[M, k] with their
+ * classes index[M, k].  Per row r that counts, with p = softmax of top / temperature over the row's entries and q = softmax of
+ * Z / temperature over all classes,
+ *   loss += scale * temperature^2 * sum_j p_j (log p_j - log q[index_j])
+ *   dZ[r, c] = grad_loss * scale * temperature * (q_c - sum of p_j over the entries with index_j == c)
+ * An entry whose index is outside [0, C) or whose logit is -inf is none; an index may stand in a row more than once.  A row
+ * without entries, or with row_mask[r] == 0, does not count: it adds nothing, whatever it holds, and its dZ is zero.
+ *   type, top_type: GC_TYPE_F32 or GC_TYPE_BF16 (dZ has Z's).  index_bits: 64 or 32.  k: at most 1024.
+ *   stats: M x 4 floats, 16-byte aligned, which the backward call reads.  loss, grad_loss: one device float each.
+ *   pad: columns behind a row of dZ that are its own and become zero (less than 8).
+ */
+size_t gc_distill_workspace_bytes(int64_t M, int64_t C);
+int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
+                       int index_bits, int64_t ldi, const uint8_t* row_mask, int64_t M, int64_t C, int64_t k, float temperature,
+                       float scale, float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
+                        int index_bits, int64_t ldi, const float* stats, int64_t M, int64_t C, int64_t k, float temperature,
+                        float scale, const float* grad_loss, void* dZ, int64_t lddz, int64_t pad, void* stream);
+
+/*
  * Evaluation tail of the reference's script (tests/gcn/graphcuda_impl.py:63-68:
  * out.argmax(dim=1), then (pred[mask] == y[mask]).sum() / mask.sum() for the
  * train / validation / test selections) in one pass over Z.
