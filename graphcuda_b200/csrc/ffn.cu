@@ -1093,6 +1093,56 @@ bool sizes_ok(int64_t M, int64_t D, int64_t H, int64_t O) {
 
 }  // namespace
 
+namespace gc {
+namespace ffn {
+
+size_t rows_workspace(int64_t M, int64_t K, int64_t N) { return align256(size_t(M) * up8(K) * 2) + plain_workspace(M, N, K); }
+int rows_times(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, int64_t M, int64_t K, int64_t N, uint16_t* Y,
+               int64_t ldy, void* workspace, cudaStream_t st) {
+  char* ws = static_cast<char*>(workspace);
+  Matrix x{X, M, K, ldx, 2};
+  Copies copies{};
+  make_readable(x, ws, copies);
+  const int rc = run_copies(copies, st);
+  if (rc != GC_OK) return rc;
+  return plain(x, false, Matrix{W, N, K, ldw, 2}, false, M, N, K, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
+}
+
+size_t block_workspace(int64_t M, int64_t D, int64_t H, int64_t O) {
+  const int64_t halves = stack(M);
+  return align256(size_t(M) * up8(D) * 2) + hidden_bytes(M, up8(H)) + plain_workspace(M, O, H, halves);
+}
+int block_times(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin, const uint16_t* Wout, int64_t ldwout, int64_t M,
+                int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace, cudaStream_t st) {
+  char* ws = static_cast<char*>(workspace);
+  Matrix x{X, M, D, ldx, 2};
+  Copies copies{};
+  make_readable(x, ws, copies);
+  int rc = run_copies(copies, st);
+  if (rc != GC_OK) return rc;
+  const int64_t hp = up8(H), halves = stack(M);
+  uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);
+  ws += hidden_bytes(M, hp);
+  const Tile t = pick_tile(kGated, M, H, 1);
+  Maps maps;
+  Params p{};
+  p.M = int(M); p.N = int(H); p.K = int(D);
+  p.b_up = int(H);  // rows of Win: no alignment to keep
+  p.act = act;
+  p.C = halves > 1 ? reinterpret_cast<bf16*>(hidden) + M * hp : nullptr;
+  p.ldc = hp;
+  rc = error_word(&p.word);
+  if (rc == GC_OK) rc = operand_maps(maps, p, x, false, Matrix{Win, 2 * H, D, ldwin, 2}, false, t.bn / 2);
+  if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 32, 32);
+  if (rc == GC_OK) rc = launch_tile<kGated, false, false, false>(t, maps, p, st);
+  if (rc != GC_OK) return rc;
+  return plain(Matrix{hidden, halves * M, H, hp, 2}, false, Matrix{Wout, O, H, ldwout, 2}, false, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0,
+               0, ws, st, halves);
+}
+
+}  // namespace ffn
+}  // namespace gc
+
 extern "C" {
 
 size_t gc_gated_ffn_saved_bytes(int64_t M, int64_t H) {

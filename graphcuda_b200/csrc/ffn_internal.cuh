@@ -134,5 +134,14 @@ struct Rows {
 };
 int forward_few_rows(const Rows& r, bool e4m3, cudaStream_t st);
 
+// On the tensor cores, with weights whose inputs run along their rows (16-byte aligned ones): Y (M x N) = X W^T with W N x K, and the
+// block with Win 2H x D and Wout O x H.  All bf16; X and Y may lie as they like.
+size_t rows_workspace(int64_t M, int64_t K, int64_t N);
+int rows_times(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, int64_t M, int64_t K, int64_t N, uint16_t* Y,
+               int64_t ldy, void* workspace, cudaStream_t st);
+size_t block_workspace(int64_t M, int64_t D, int64_t H, int64_t O);
+int block_times(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin, const uint16_t* Wout, int64_t ldwout, int64_t M,
+                int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace, cudaStream_t st);
+
 }  // namespace ffn
 }  // namespace gc

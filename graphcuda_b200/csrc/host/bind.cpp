@@ -329,6 +329,28 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return gated_ffn_fp8(x8, x_scale, w8, w_scale, w_out, act);
   }, NoGil());
   m.def("gated_ffn_fp8_forward", &gated_ffn_fp8, NoGil());
+  const auto linear4 = [](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
+                          int64_t n) { return linear_int4(x, Int4{codes, scale, zero, group, k, n}); };
+  const auto block4 = [](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
+                         int64_t n, const Tensor& codes_out, const Tensor& scale_out, const OptTensor& zero_out, int64_t group_out,
+                         int64_t k_out, int64_t n_out, int64_t act) {
+    return gated_ffn_int4(x, Int4{codes, scale, zero, group, k, n}, Int4{codes_out, scale_out, zero_out, group_out, k_out, n_out}, act);
+  };
+  m.def("linear_int4", [linear4](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
+                                 int64_t n) -> OptTensor {
+    if (recorded({&x})) raise("linear_int4 has no gradient: call it under torch.no_grad()");
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return linear4(x, codes, scale, zero, group, k, n);
+  }, NoGil());
+  m.def("linear_int4_forward", linear4, NoGil());
+  m.def("gated_ffn_int4", [block4](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
+                                   int64_t n, const Tensor& codes_out, const Tensor& scale_out, const OptTensor& zero_out,
+                                   int64_t group_out, int64_t k_out, int64_t n_out, int64_t act) -> OptTensor {
+    if (recorded({&x})) raise("gated_ffn_int4 has no gradient: call it under torch.no_grad(), or gated_ffn for training");
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return block4(x, codes, scale, zero, group, k, n, codes_out, scale_out, zero_out, group_out, k_out, n_out, act);
+  }, NoGil());
+  m.def("gated_ffn_int4_forward", block4, NoGil());
   m.def("adamw_step", &adamw_step, NoGil());
   m.def("adamw_moments", &adamw_moments, NoGil());
 }

@@ -49,7 +49,8 @@ inline bool f32_on(const Tensor& t, const at::Device& dev) {
   X(gc_rms_norm_forward) X(gc_rms_norm_backward_workspace_bytes) X(gc_rms_norm_backward) X(gc_adamw_step)           \
   X(gc_adamw_moments_f32) X(gc_gated_ffn_saved_bytes) X(gc_gated_ffn_workspace_bytes)                              \
   X(gc_gated_ffn_forward_bf16) X(gc_gated_ffn_backward_bf16) X(gc_gated_ffn_e4m3_workspace_bytes)                   \
-  X(gc_gated_ffn_forward_e4m3) X(gc_distill_workspace_bytes) X(gc_distill_forward) X(gc_distill_backward)
+  X(gc_gated_ffn_forward_e4m3) X(gc_distill_workspace_bytes) X(gc_distill_forward) X(gc_distill_backward)             \
+  X(gc_linear_int4_workspace_bytes) X(gc_linear_int4_bf16) X(gc_gated_ffn_int4_workspace_bytes) X(gc_gated_ffn_int4_bf16)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
   GC_HOST_FUNCTIONS(X)
@@ -245,6 +246,16 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_in, const Tensor& w_out, int64
 Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, const Tensor& w_scale, const Tensor& w_out,
                      int64_t act);
 void refuse_ffn_fp8_gradient(std::initializer_list<const Tensor*> inputs);
+// Scratch for the tensor-core products: kept up to a few megabytes, the call's own memory beyond.
+Scratch product_workspace(size_t bytes, const at::Device& dev);
+// A weight of 4 bits as it was laid out (int4.cpp).
+struct Int4 {
+  const Tensor &codes, &scale;
+  const OptTensor& zero;
+  int64_t group, k, n;
+};
+Tensor linear_int4(const Tensor& x, const Int4& w);
+Tensor gated_ffn_int4(const Tensor& x, const Int4& w_in, const Int4& w_out, int64_t act);
 void adamw_step(const std::vector<Tensor>& p, const std::vector<Tensor>& g, const std::vector<Tensor>& m,
                 const std::vector<Tensor>& v, const Tensor& state, const std::vector<Tensor>& masters,
                 const std::vector<Tensor>& m_scales, const std::vector<Tensor>& v_scales, double lr, double b1, double b2,

@@ -100,9 +100,15 @@ class GatedFFN(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return gated_ffn(x, self.w_in, self.w_out, self.activation)
 
-    def for_serving(self) -> "GatedFFNFp8":
-        """The block with its first product in 8 bits; its weights are those of this moment."""
-        return GatedFFNFp8(self)
+    def for_serving(self, bits: int = 8):
+        """The block with its first product in 8 bits (``GatedFFNFp8``), or with both weights in 4 (``int4.GatedFFNInt4``); its
+        weights are those of this moment."""
+        if bits == 8:
+            return GatedFFNFp8(self)
+        if bits != 4:
+            raise ValueError(f"bits must be 4 or 8, got {bits}")
+        from .int4 import GatedFFNInt4
+        return GatedFFNInt4(self)
 
 
 class GatedFFNFp8(torch.nn.Module):

@@ -105,9 +105,10 @@ class ResidualGCN(torch.nn.Module):
         """As ``GCN.evaluate``: ``(pred, counts)``."""
         return argmax_accuracy(self.forward(x, adj, log_softmax=False), labels, masks)
 
-    def for_serving(self) -> "ServedResidualGCN":
-        """The model with the first product of every feed-forward block in 8 bits, its weights those of this moment."""
-        return ServedResidualGCN(self)
+    def for_serving(self, bits: int = 8) -> "ServedResidualGCN":
+        """The model with the first product of every feed-forward block in 8 bits, or with all weights of these blocks in 4; its
+        weights are those of this moment."""
+        return ServedResidualGCN(self, bits)
 
 
 def _frozen(module: torch.nn.Module) -> torch.nn.Module:
@@ -115,29 +116,36 @@ def _frozen(module: torch.nn.Module) -> torch.nn.Module:
 
 
 class ServedBlock(ResidualBlock):
-    """``ResidualBlock`` with its feed-forward block in 8 bits: weights of their own, those that the block had."""
+    """``ResidualBlock`` with its feed-forward block in 8 or 4 bits: weights of their own, those that the block had."""
 
-    def __init__(self, block: ResidualBlock):
+    def __init__(self, block: ResidualBlock, bits: int = 8):
         torch.nn.Module.__init__(self)
         self.norm_conv, self.conv, self.norm_ffn = (_frozen(m) for m in (block.norm_conv, block.conv, block.norm_ffn))
-        self.ffn = block.ffn.for_serving()
+        self.ffn = block.ffn.for_serving(bits)
+        self.bits = bits
 
     def forward(self, y, h, adj):
+        if self.bits == 4:
+            return super().forward(y, h, adj)
         a, h = self.aggregate(y, h, adj)
         n8, scale, h = self.norm_ffn.fp8(a, h)
         return self.ffn(n8, scale), h
 
 
 class ServedResidualGCN(ResidualGCN):
-    """``ResidualGCN`` for inference: the norm in front of a feed-forward block writes 8 bits and a scale per row, which the
-    block multiplies with weights laid out in 8 bits once.  All of its weights are copies: the source may train on, or go."""
+    """``ResidualGCN`` for inference.  ``bits=8``: the norm in front of a feed-forward block writes 8 bits and a scale per row, which
+    the block multiplies with weights laid out in 8 bits once.  ``bits=4``: both weights of every feed-forward block have 4 bits.
+    All of its weights are copies: the source may train on, or go."""
 
-    def __init__(self, model: ResidualGCN):
+    def __init__(self, model: ResidualGCN, bits: int = 8):
         torch.nn.Module.__init__(self)
+        self.bits = bits
         self.conv_in, self.norm_out, self.conv_out = (_frozen(m) for m in (model.conv_in, model.norm_out, model.conv_out))
-        self.blocks = torch.nn.ModuleList([ServedBlock(block) for block in model.blocks])
+        self.blocks = torch.nn.ModuleList([ServedBlock(block, bits) for block in model.blocks])
 
-    def for_serving(self) -> "ServedResidualGCN":
+    def for_serving(self, bits: Optional[int] = None) -> "ServedResidualGCN":
+        if bits not in (None, self.bits):
+            raise RuntimeError(f"the model serves in {self.bits} bits: ask the one that it was made of")
         return self
 
     @torch.no_grad()
