@@ -24,6 +24,7 @@ from .ffn import GatedFFN, gated_ffn, gated_ffn_fp8, quantize_weight_fp8  # noqa
 from .gcn import GCNConv, GCNConvFunction  # noqa: E402
 from .feed import PinnedFeed  # noqa: E402
 from .graphed import GraphedTrainStep  # noqa: E402
+from .grouped import GroupedLinear, grouped_linear  # noqa: E402
 from .int4 import Int4Weight, gated_ffn_int4, linear_int4, quantize_weight_int4  # noqa: E402
 from .losses import argmax_accuracy, distill_loss, log_softmax_nll_loss  # noqa: E402
 from .norm import RMSNorm, rms_norm, rms_norm_fp8  # noqa: E402

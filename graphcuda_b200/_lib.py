@@ -73,6 +73,10 @@ SIGNATURES = {
                                              _void]),
     "gc_logsoftmax_nll_backward_f32": (_int, [_f32p, _i64, _i64p, _void, _i64, _i64, C.c_float, _f32p, _f32p, _i64,
                                               _void, _void]),
+    "gc_grouped_linear_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _int]),
+    "gc_grouped_linear_forward_bf16": (_int, [_void, _i64, _void, _i64, _i32p, _i64, _i64, _i64, _i64, _void, _i64, _void, _size, _void]),
+    "gc_grouped_linear_backward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _i32p, _i64, _i64, _i64, _i64, _void, _i64, _void,
+                                               _void, _size, _void]),
     "gc_linear_int4_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "gc_linear_int4_bf16": (_int, [_void, _i64, _void, _void, _void, _int, _i64, _i64, _i64, _void, _i64, _void, _size, _void]),
     "gc_gated_ffn_int4_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),

@@ -38,12 +38,12 @@ SOURCES = [
     "gcn_layer.cu",
     "graph_build.cu",
     "loss.cu", "distill.cu", "optim.cu",
-    "norm.cu", "adamw.cu", "ffn.cu", "ffn_rows.cu", "int4.cu",
+    "norm.cu", "adamw.cu", "ffn.cu", "ffn_rows.cu", "int4.cu", "grouped.cu",
 ]
 
 HOSTSRC = os.path.join(CSRC, "host")
 HOSTNAME = "_gc_host"
-HOST_SOURCES = ["core.cpp", "layer.cpp", "tail.cpp", "block.cpp", "int4.cpp", "bind.cpp"]
+HOST_SOURCES = ["core.cpp", "layer.cpp", "tail.cpp", "block.cpp", "int4.cpp", "grouped.cpp", "bind.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -329,6 +329,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return gated_ffn_fp8(x8, x_scale, w8, w_scale, w_out, act);
   }, NoGil());
   m.def("gated_ffn_fp8_forward", &gated_ffn_fp8, NoGil());
+  m.def("grouped_linear", [](const Tensor& x, const Tensor& w, const Tensor& offsets) -> OptTensor {
+    if (torch::jit::tracer::isTracing()) return std::nullopt;
+    return grouped_linear(x, w, offsets);
+  }, NoGil());
+  m.def("grouped_linear_forward", [](const Tensor& x, const Tensor& w, const Tensor& offsets) {
+    const GroupedForward f = grouped_linear_forward(x, w, offsets);
+    return std::make_tuple(f.y, std::vector<Tensor>{f.x, f.w, f.offsets});
+  }, NoGil());
+  m.def("grouped_linear_backward", &grouped_linear_backward, NoGil());
   const auto linear4 = [](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
                           int64_t n) { return linear_int4(x, Int4{codes, scale, zero, group, k, n}); };
   const auto block4 = [](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,

@@ -50,6 +50,7 @@ inline bool f32_on(const Tensor& t, const at::Device& dev) {
   X(gc_adamw_moments_f32) X(gc_gated_ffn_saved_bytes) X(gc_gated_ffn_workspace_bytes)                              \
   X(gc_gated_ffn_forward_bf16) X(gc_gated_ffn_backward_bf16) X(gc_gated_ffn_e4m3_workspace_bytes)                   \
   X(gc_gated_ffn_forward_e4m3) X(gc_distill_workspace_bytes) X(gc_distill_forward) X(gc_distill_backward)             \
+  X(gc_grouped_linear_workspace_bytes) X(gc_grouped_linear_forward_bf16) X(gc_grouped_linear_backward_bf16)         \
   X(gc_linear_int4_workspace_bytes) X(gc_linear_int4_bf16) X(gc_gated_ffn_int4_workspace_bytes) X(gc_gated_ffn_int4_bf16)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
@@ -248,6 +249,14 @@ Tensor gated_ffn_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, 
 void refuse_ffn_fp8_gradient(std::initializer_list<const Tensor*> inputs);
 // Scratch for the tensor-core products: kept up to a few megabytes, the call's own memory beyond.
 Scratch product_workspace(size_t bytes, const at::Device& dev);
+// Rows by group times a weight per group (grouped.cpp): y, and the operands as the kernels took them.
+struct GroupedForward {
+  Tensor y, x, w, offsets;
+};
+GroupedForward grouped_linear_forward(const Tensor& x, const Tensor& w, const Tensor& offsets);
+std::pair<Tensor, Tensor> grouped_linear_backward(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& offsets, bool need_dx,
+                                                  bool need_dw);
+Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets);
 // A weight of 4 bits as it was laid out (int4.cpp).
 struct Int4 {
   const Tensor &codes, &scale;

@@ -546,6 +546,22 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
                               uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Rows sorted by group times a weight per group, all bf16 with fp32 sums: W is G matrices K x N, one below the other (ldw elements
+ * from row to row), and rows offsets[g] to offsets[g + 1] - 1 of X (M x K) belong to group g; offsets, G + 1 of them, lie on the
+ * device.  Groups may be empty; rows before offsets[0] and from offsets[G] on belong to none, and what they get is zeros.  Offsets that are
+ * outside [0, M] or decrease are read as the nearest that do not.
+ *   forward    Y[r] = X[r] W[g]
+ *   backward   dX[r] = dY[r] W[g]^T and dW[g] = X_g^T dY_g (dW contiguous; either may be null)
+ */
+size_t gc_grouped_linear_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int backward);
+int gc_grouped_linear_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, const int32_t* offsets, int64_t M,
+                                   int64_t K, int64_t N, int64_t G, uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+int gc_grouped_linear_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw,
+                                    const int32_t* offsets, int64_t M, int64_t K, int64_t N, int64_t G, uint16_t* dX, int64_t lddx,
+                                    uint16_t* dW, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Products with weights of 4 bits, for serving: Y (M x N, bf16) = X (M x K, bf16) W with
  *   W[k, n] = (code - zero) * scale
  * of an input's group of 32, 64 or 128 (`group`) and an output: codes and zero points 0 to 15 (zero null: 8), scales bf16.  Laid out,
