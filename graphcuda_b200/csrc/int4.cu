@@ -9,8 +9,8 @@
 // product that waits for memory gains nothing from its rate.)  Codes are laid out so that a lane's 16 bytes are what it
 // multiplies: see gc_linear_int4_bf16 in the header.
 //
-// A CTA's 8 warps are wn blocks of outputs times wk interleaved shares of the 128-input chunks; where the outputs alone do not
-// fill the GPU, a cluster of CTAs shares the chunks too.  Sums meet in a fixed order.  In the block, the hidden row between the
+// A CTA has 16 or 32 outputs, whose chunks of 128 inputs its warps take in turn; where the outputs alone do not fill the GPU, those of a
+// cluster do.  Sums meet in a fixed order.  In the block, the hidden row between the
 // two launches goes as two bf16 numbers, hi and lo, in twice the rows of X; the second launch starts while the first runs, and its
 // first codes are in registers when it has ended.
 //
@@ -18,6 +18,7 @@
 // cores has to be), 2.5 bytes of traffic per weight, and the tensor-core product of the gated block runs on them.
 #include "common.cuh"
 #include "ffn_internal.cuh"
+#include "tiles.cuh"
 
 #include <cuda_bf16.h>
 
@@ -28,7 +29,7 @@ namespace {
 using namespace gc::ffn;
 using bf16 = __nv_bfloat16;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMostThreads = 256;
 constexpr int kChunk = 128;       // inputs of a chunk
 constexpr int kTile = 1024;       // bytes of 16 outputs' codes of a chunk
 constexpr int kMostColumns = 64;  // rows of X (of hi and lo: twice) that a launch takes
@@ -64,8 +65,8 @@ __device__ __forceinline__ void unpack(uint32_t w, __nv_bfloat162 zero, uint32_t
     o[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-__device__ __forceinline__ __nv_bfloat162 zero_pair(uint32_t zero) {
-  const uint32_t t = (0x4300u + zero) * 0x10001u;
+__device__ __forceinline__ __nv_bfloat162 zero_pair(uint32_t zeros, int byte) {
+  const uint32_t t = __byte_perm(zeros, 0x43u, 0x4040u + 0x0101u * byte);
   return *reinterpret_cast<const __nv_bfloat162*>(&t);
 }
 __device__ __forceinline__ float gated(float g, float u, int act) {
@@ -78,7 +79,7 @@ __device__ __forceinline__ float gated(float g, float u, int act) {
 }
 
 struct Params {
-  const uint16_t* x;
+  const uint16_t* x;  // rows in 16-byte accesses, zeros up to the next multiple of 8 inputs
   const uint8_t* codes;
   const uint16_t* scale;
   const uint8_t* zero;  // null: 8
@@ -86,10 +87,9 @@ struct Params {
   int64_t ldx, ldo;
   int rows, out_rows;  // of X; of the output: half of them where X is hi and lo
   int K, N;            // N: outputs, of either half of a gated product
-  int wn, ctas;
+  int ctas;            // of a cluster
   int act;
-  int x_vec;   // rows of X in 16-byte accesses
-  int wait;    // X comes from the launch before
+  int wait;  // X comes from the launch before
 };
 
 // Of one chunk what a lane needs: codes of its outputs lane / 4 and lane / 4 + 8 of MT blocks, and their groups' scales and zero
@@ -101,18 +101,17 @@ struct Fetched {
   uint32_t zero[MT][2];
 };
 
-// NT: 8 rows of X each.  MT: blocks of 16 outputs of a warp (GATED: the same ones of G and of U).  GPC: groups in a chunk.
-template <int NT, int MT, bool GATED, int GPC>
-__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1)
+// NT: 8 rows of X each.  MT: blocks of 16 outputs of a CTA (GATED: the same ones of G and of U).  GPC: groups in a chunk.  DEPTH: chunks
+// that a warp has on their way to its registers.  The CTA's warps, and those of the cluster's other CTAs, take chunks in turn.
+template <int NT, int MT, bool GATED, int GPC, int DEPTH>
+__global__ void __launch_bounds__(kMostThreads, NT == 1 ? 2 : 1)
 int4_rows_kernel(const __grid_constant__ Params p) {
-  extern __shared__ float sums[];  // [wk][wn * MT * 16][NT * 8]
-  constexpr int kCols = NT * 8;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
+  extern __shared__ float sums[];  // [warp][MT * 16][NT * 8]
+  constexpr int kCols = NT * 8, kOuts = MT * 16, kBlocks = 4 / GPC;  // kBlocks: 32s of inputs in a group
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, g = lane / 4, t = lane % 4;
   const uint32_t rank = p.ctas > 1 ? cluster_rank() : 0;
-  const int wn = p.wn, wk = kWarps / wn, my_n = warp % wn, my_k = warp / wn;
   const int chunks = (p.K + kChunk - 1) / kChunk, total_n = GATED ? 2 * p.N : p.N;
-  const int out0 = int(blockIdx.x / p.ctas) * wn * (GATED ? 1 : MT) * 16;  // the CTA's first output
-  const int n0 = out0 + my_n * (GATED ? 1 : MT) * 16;
+  const int out0 = int(blockIdx.x / p.ctas) * (GATED ? 16 : kOuts);  // the CTA's first output
   // where the lane's outputs begin, which need not begin a block (U's of a gated product); the second of two lies `codes_on` and
   // `groups_on` behind the first
   const uint8_t* codes_at[MT];
@@ -121,7 +120,7 @@ int4_rows_kernel(const __grid_constant__ Params p) {
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     auto place = [&](int h, int64_t& codes, int64_t& groups) {
-      const int n = min(n0 + h * 8 + g + (GATED ? m * p.N : m * 16), total_n - 1);
+      const int n = min(out0 + h * 8 + g + (GATED ? m * p.N : m * 16), total_n - 1);
       const int64_t tile = int64_t(n / 16) * chunks;
       codes = tile * kTile + n % 16 * 64 + t * 16;
       groups = (tile * 16 + n % 16) * GPC;
@@ -156,18 +155,12 @@ int4_rows_kernel(const __grid_constant__ Params p) {
       }
     return f;
   };
-  // eight inputs of a row of X
-  auto fetch_x = [&](int nt, int k) {
-    const int r = nt * 8 + g;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r >= p.rows) return v;
-    const uint16_t* row = p.x + int64_t(r) * p.ldx + k;
-    if (p.x_vec && k + 8 <= p.K) return *reinterpret_cast<const uint4*>(row);
-    uint32_t* w = &v.x;
+  const uint16_t* x_at[NT];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k + e < p.K) w[e / 2] |= uint32_t(row[e]) << (e % 2 * 16);
-    return v;
+  for (int n = 0; n < NT; ++n) x_at[n] = n * 8 + g < p.rows ? p.x + int64_t(n * 8 + g) * p.ldx + t * 8 : nullptr;
+  const int x_end = p.K - t * 8;  // of what may be read from x_at on
+  auto fetch_x = [&](int n, int k) {  // eight inputs
+    return x_at[n] && k < x_end ? __ldg(reinterpret_cast<const uint4*>(x_at[n] + k)) : make_uint4(0, 0, 0, 0);
   };
 
   float tot[MT][NT][4], acc[MT][NT][4];
@@ -177,71 +170,96 @@ int4_rows_kernel(const __grid_constant__ Params p) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) tot[m][n][e] = 0.f;
-  const int step = p.ctas * wk, first = int(rank) * wk + my_k;
-  Fetched<MT, GPC> now, ahead;
-  if (first < chunks) now = fetch(first);
+  const int step = p.ctas * warps;
+  int c = int(rank) * warps + warp;
+  Fetched<MT, GPC> ring[DEPTH];
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (c + d * step < chunks) ring[d] = fetch(c + d * step);
   if (GATED) let_next_begin();
   if (p.wait) wait_for_last();
-  for (int c = first; c < chunks; c += step) {
-    if (c + step < chunks) ahead = fetch(c + step);
+  // X of a chunk: for up to 16 rows all at once, and of up to 8 rows a chunk ahead
+  constexpr bool kWhole = NT <= 2, kAhead = NT == 1;
+  uint4 xs[kWhole ? NT : 1][4], xn[kAhead ? NT : 1][4];
+  auto fetch_chunk = [&](uint4 (&to)[kWhole ? NT : 1][4], int at) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // 32 inputs
-      constexpr int kBlocks = 4 / GPC;
-      if (j % kBlocks == 0) {
+    for (int n = 0; n < (kWhole ? NT : 1); ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[n][j] = fetch_x(n, at * kChunk + j * 32);
+  };
+  if constexpr (kAhead)
+    if (c < chunks) fetch_chunk(xs, c);
+  for (; c < chunks;) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d, c += step) {
+      if (c >= chunks) break;
+      const Fetched<MT, GPC>& now = ring[d];
+      if constexpr (kAhead) fetch_chunk(xn, c + step);  // beyond the last: nothing is read
+      else if constexpr (kWhole) fetch_chunk(xs, c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // 32 inputs
+        if (j % kBlocks == 0) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
+        }
+        uint4 xj[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (kWhole) xj[n] = xs[n][j];
+          else xj[n] = fetch_x(n, c * kChunk + j * 32);
+        }
+        uint32_t a[MT][2][4];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int h = 0; h < 2; ++h) unpack((&now.codes[m][h].x)[j], zero_pair(now.zero[m][h], j / kBlocks), a[m][h]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-      }
-      uint32_t a[MT][2][4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+          for (int m = 0; m < MT; ++m) {
+            mma(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], xj[n].x, xj[n].y);
+            mma(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], xj[n].z, xj[n].w);
+          }
+        if (j % kBlocks == kBlocks - 1) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          unpack((&now.codes[m][h].x)[j], zero_pair(now.zero[m][h] >> (8 * (j / kBlocks)) & 0xFFu), a[m][h]);
+          for (int m = 0; m < MT; ++m) {
+            auto scale = [&](int h) {
+              const uint32_t w = now.scale[m][h][j / kBlocks / 2];
+              return __uint_as_float(j / kBlocks % 2 ? w & 0xFFFF0000u : w << 16);
+            };
+            const float s0 = scale(0), s1 = scale(1);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint4 x = fetch_x(n, c * kChunk + j * 32 + t * 8);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          mma(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x.x, x.y);
-          mma(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], x.z, x.w);
-        }
-      }
-      if (j % kBlocks == kBlocks - 1) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          auto scale = [&](int h) {
-            const uint32_t w = now.scale[m][h][j / kBlocks / 2];
-            return __uint_as_float(j / kBlocks % 2 ? w & 0xFFFF0000u : w << 16);
-          };
-          const float s0 = scale(0), s1 = scale(1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            tot[m][n][0] = fmaf(s0, acc[m][n][0], tot[m][n][0]);
-            tot[m][n][1] = fmaf(s0, acc[m][n][1], tot[m][n][1]);
-            tot[m][n][2] = fmaf(s1, acc[m][n][2], tot[m][n][2]);
-            tot[m][n][3] = fmaf(s1, acc[m][n][3], tot[m][n][3]);
+            for (int n = 0; n < NT; ++n) {
+              tot[m][n][0] = fmaf(s0, acc[m][n][0], tot[m][n][0]);
+              tot[m][n][1] = fmaf(s0, acc[m][n][1], tot[m][n][1]);
+              tot[m][n][2] = fmaf(s1, acc[m][n][2], tot[m][n][2]);
+              tot[m][n][3] = fmaf(s1, acc[m][n][3], tot[m][n][3]);
+            }
           }
         }
       }
+      if (c + DEPTH * step < chunks) ring[d] = fetch(c + DEPTH * step);
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xs[0][j] = xn[0][j];
+      }
     }
-    now = ahead;
   }
-  const int outs = wn * MT * 16;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        sums[(my_k * outs + (my_n * MT + m) * 16 + g + e / 2 * 8) * kCols + n * 8 + 2 * t + e % 2] = tot[m][n][e];
+        sums[(warp * kOuts + m * 16 + g + e / 2 * 8) * kCols + n * 8 + 2 * t + e % 2] = tot[m][n][e];
   __syncthreads();
-  for (int i = threadIdx.x; i < outs * kCols; i += kThreads) {
+  for (int i = threadIdx.x; i < kOuts * kCols; i += blockDim.x) {
     float s = sums[i];
-    for (int w = 1; w < wk; ++w) s += sums[w * outs * kCols + i];
+    for (int w = 1; w < warps; ++w) s += sums[w * kOuts * kCols + i];
     sums[i] = s;
   }
   if (p.ctas > 1) cluster_sync();
@@ -255,18 +273,18 @@ int4_rows_kernel(const __grid_constant__ Params p) {
       }
     return s;
   };
-  const int width = GATED ? wn * 16 : outs;  // outputs of the CTA, which the cluster shares out among its CTAs
-  for (int i = int(rank) * kThreads + threadIdx.x; i < width * p.out_rows; i += p.ctas * kThreads) {
-    const int r = i / width, o = i % width, n = out0 + o;
-    if (n >= p.N) continue;
+  constexpr int kWidth = GATED ? 16 : kOuts;  // outputs of the CTA, which the cluster shares out among its CTAs
+  for (int i = int(rank) * blockDim.x + threadIdx.x; i < kWidth * p.out_rows; i += p.ctas * blockDim.x) {
+    const int r = i / kWidth, o = i % kWidth, n = out0 + o;
     bf16* to = reinterpret_cast<bf16*>(p.out) + r * p.ldo + n;
     if constexpr (GATED) {
-      const int place = o / 16 * 32 + o % 16;
-      const float h = gated(whole(place, r), whole(place + 16, r), p.act);
+      const float h = n < p.N ? gated(whole(o, r), whole(o + 16, r), p.act) : 0.f;
       const bf16 hi = __float2bfloat16_rn(h);
-      to[0] = hi;  // nothing is left of what is not finite
-      to[p.out_rows * p.ldo] = __float2bfloat16_rn(isfinite(__bfloat162float(hi)) ? h - __bfloat162float(hi) : 0.f);
-    } else {
+      if (n < (p.N + 7) / 8 * 8) {  // zeros up to there
+        to[0] = hi;
+        to[p.out_rows * p.ldo] = __float2bfloat16_rn(isfinite(__bfloat162float(hi)) ? h - __bfloat162float(hi) : 0.f);  // of inf nothing is left
+      }
+    } else if (n < p.N) {
       to[0] = __float2bfloat16_rn(whole(o, r));
     }
   }
@@ -288,7 +306,7 @@ int4_unpack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict
     const int64_t at = (tile * 16 + n % 16) * gpc + j * gpc / 4;
     const float s = __uint_as_float(uint32_t(__ldg(scale + at)) << 16);
     uint32_t o[4];
-    unpack(word, zero_pair(zero ? __ldg(zero + at) : 8), o);
+    unpack(word, zero_pair(zero ? __ldg(zero + at) : 8, 0), o);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const __nv_bfloat162 v = __floats2bfloat162_rn(s * __uint_as_float(o[e] << 16), s * __uint_as_float(o[e] & 0xFFFF0000u));
@@ -305,30 +323,27 @@ struct Weights {
   const uint8_t* zero;
   int group;
 };
-inline int64_t up8(int64_t x) { return (x + 7) & ~int64_t(7); }
-inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+using gc::tiles::align256;
+using gc::tiles::up8;
 
-template <int NT, int MT, bool GATED, int GPC>
+template <int NT, int MT, bool GATED, int GPC, int DEPTH>
 int launch_rows(Params p, cudaStream_t st) {
-  const int64_t blocks_n = gc::ceil_div(p.N, 16 * (GATED ? 1 : MT));
+  const int64_t blocks = gc::ceil_div(p.N, GATED ? 16 : 16 * MT);
   const int chunks = int(gc::ceil_div(p.K, kChunk));
-  // Blocks of outputs in a CTA read the same X, which then comes from the L1.
-  p.wn = NT == 1 ? (p.rows > 2 ? 2 : 1) : 4;
-  while (p.wn > 1 && gc::ceil_div(blocks_n, p.wn) < gc::kNumSMs) p.wn /= 2;
-  const int wk = kWarps / p.wn;
-  const int64_t ctas = gc::ceil_div(blocks_n, p.wn);
+  const int warps = chunks >= 32 ? 8 : 4;
+  // All warps at once, 16 to an SM
   p.ctas = 1;
-  while (p.ctas < 8 && ctas * p.ctas < 2 * gc::kNumSMs && 2 * p.ctas * wk <= chunks) p.ctas *= 2;
-  if (ctas * p.ctas > 0x7FFFFFFF) return gc::fail(GC_ERR_UNSUPPORTED, "4-bit product: too many outputs");
-  const size_t smem = size_t(kWarps) * MT * 16 * NT * 8 * sizeof(float);
-  auto kern = int4_rows_kernel<NT, MT, GATED, GPC>;
+  while (p.ctas < 8 && blocks * 2 * p.ctas * warps <= 16 * gc::kNumSMs && 2 * p.ctas * warps <= chunks) p.ctas *= 2;
+  if (blocks * p.ctas > 0x7FFFFFFF) return gc::fail(GC_ERR_UNSUPPORTED, "4-bit product: too many outputs");
+  const size_t smem = size_t(warps) * MT * 16 * NT * 8 * sizeof(float);
+  auto kern = int4_rows_kernel<NT, MT, GATED, GPC, DEPTH>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(ctas * p.ctas));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(unsigned(blocks * p.ctas));
+  cfg.blockDim = dim3(unsigned(32 * warps));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -351,17 +366,30 @@ int product(const Weights& w, Params p, cudaStream_t st) {
   p.codes = w.codes;
   p.scale = w.scale;
   p.zero = w.zero;
-  p.x_vec = gc::aligned16(p.x) && p.ldx % 8 == 0;
   auto sized = [&](auto gpc) {
     constexpr int kGpc = decltype(gpc)::value;
-    if (p.rows <= 8) return launch_rows<1, GATED ? 2 : 1, GATED, kGpc>(p, st);
-    if (p.rows <= 16) return launch_rows<2, GATED ? 2 : 1, GATED, kGpc>(p, st);
-    if (p.rows <= 32) return launch_rows<4, 2, GATED, kGpc>(p, st);
-    return launch_rows<8, 2, GATED, kGpc>(p, st);
+    if (p.rows <= 8) return launch_rows<1, GATED ? 2 : 1, GATED, kGpc, GATED ? 2 : 4>(p, st);
+    if (p.rows <= 16) return launch_rows<2, 2, GATED, kGpc, 2>(p, st);
+    if (p.rows <= 32) return launch_rows<4, 2, GATED, kGpc, 2>(p, st);
+    return launch_rows<8, 2, GATED, kGpc, 1>(p, st);
   };
   return w.group == 32    ? sized(std::integral_constant<int, 4>{})
          : w.group == 64 ? sized(std::integral_constant<int, 2>{})
                          : sized(std::integral_constant<int, 1>{});
+}
+// X as the kernel takes it: itself, or a copy in the workspace.
+bool rows_ready(const uint16_t* X, int64_t ldx, int64_t K) { return gc::aligned16(X) && ldx % 8 == 0 && K % 8 == 0; }
+size_t rows_bytes(int64_t M, int64_t K) { return align256(size_t(M) * up8(K) * 2); }
+int ready_rows(Params& p, const uint16_t* X, int64_t ldx, int64_t M, int64_t K, char*& ws, cudaStream_t st) {
+  p.x = X;
+  p.ldx = ldx;
+  if (rows_ready(X, ldx, K)) return GC_OK;
+  gc::tiles::Copies copies{};
+  gc::tiles::add_copy(copies, gc::tiles::Matrix{X, M, K, ldx, 2}, ws, up8(K), up8(K));
+  p.x = reinterpret_cast<const uint16_t*>(ws);
+  p.ldx = up8(K);
+  ws += rows_bytes(M, K);
+  return gc::tiles::run_copies(copies, st);
 }
 int unpack_to(const Weights& w, int64_t K, int64_t N, void* to, cudaStream_t st) {
   const int64_t pieces = N * gc::ceil_div(K, kChunk) * 16;
@@ -392,7 +420,8 @@ constexpr int64_t kLinearRows = kMostColumns, kBlockRows = kMostColumns / 2;
 extern "C" {
 
 size_t gc_linear_int4_workspace_bytes(int64_t M, int64_t K, int64_t N) {
-  if (M <= 0 || K <= 0 || N <= 0 || !sizes_ok(M, K, N) || M <= kLinearRows) return 0;
+  if (M <= 0 || K <= 0 || N <= 0 || !sizes_ok(M, K, N)) return 0;
+  if (M <= kLinearRows) return rows_bytes(M, K);
   return unpacked_bytes(K, N) + gc::ffn::rows_workspace(M, K, N);
 }
 
@@ -410,17 +439,19 @@ int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes, co
   const Weights w{codes, scale, zero, group};
   int rc = weights_ok(w, "gc_linear_int4_bf16");
   if (rc != GC_OK) return rc;
+  if (!workspace || workspace_bytes < gc_linear_int4_workspace_bytes(M, K, N))
+    return gc::fail(GC_ERR_WORKSPACE, "gc_linear_int4_bf16: workspace missing or smaller than its query says");
+  GC_REQUIRE(gc::aligned16(workspace), "gc_linear_int4_bf16: workspace must be 16-byte aligned");
   if (M <= kLinearRows) {
     Params p{};
-    p.x = X; p.ldx = ldx;
+    char* ws = static_cast<char*>(workspace);
+    rc = ready_rows(p, X, ldx, M, K, ws, st);
+    if (rc != GC_OK) return rc;
     p.out = Y; p.ldo = ldy;
     p.rows = p.out_rows = int(M);
     p.K = int(K); p.N = int(N);
     return product<false>(w, p, st);
   }
-  if (!workspace || workspace_bytes < gc_linear_int4_workspace_bytes(M, K, N))
-    return gc::fail(GC_ERR_WORKSPACE, "gc_linear_int4_bf16: workspace missing or smaller than its query says");
-  GC_REQUIRE(gc::aligned16(workspace), "gc_linear_int4_bf16: workspace must be 16-byte aligned");
   rc = unpack_to(w, K, N, workspace, st);
   if (rc != GC_OK) return rc;
   return gc::ffn::rows_times(X, ldx, static_cast<const uint16_t*>(workspace), up8(K), M, K, N, Y, ldy,
@@ -429,7 +460,7 @@ int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes, co
 
 size_t gc_gated_ffn_int4_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O) {
   if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, std::max(D, H), O) || !sizes_ok(2 * H, 0, 0)) return 0;
-  if (M <= kBlockRows) return align256(size_t(2 * M) * up8(H) * 2);
+  if (M <= kBlockRows) return rows_bytes(M, D) + rows_bytes(2 * M, H);
   return unpacked_bytes(D, 2 * H) + unpacked_bytes(H, O) + gc::ffn::block_workspace(M, D, H, O);
 }
 
@@ -456,7 +487,8 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes_
   char* ws = static_cast<char*>(workspace);
   if (M <= kBlockRows) {
     Params p{};
-    p.x = X; p.ldx = ldx;
+    rc = ready_rows(p, X, ldx, M, D, ws, st);
+    if (rc != GC_OK) return rc;
     p.out = reinterpret_cast<uint16_t*>(ws); p.ldo = up8(H);
     p.rows = p.out_rows = int(M);
     p.K = int(D); p.N = int(H);
