@@ -51,10 +51,15 @@ __device__ __forceinline__ float peer_load(const float* p, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
   return v;
 }
+// c = A B, or c + A B.
+template <bool FIRST>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  float d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = FIRST ? 0.f : c[i];
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 // Eight codes as four pairs of bf16 numbers less `zero`, a pair of 128 + zero point: 0x4300 is 128 and its last bits count ones.
 __device__ __forceinline__ void unpack(uint32_t w, __nv_bfloat162 zero, uint32_t (&o)[4]) {
@@ -90,6 +95,8 @@ struct Params {
   int ctas;            // of a cluster
   int act;
   int wait;  // X comes from the launch before
+  const uint8_t* next;  // gated: the codes of the launch behind
+  int64_t next_bytes;
 };
 
 // Of one chunk what a lane needs: codes of its outputs lane / 4 and lane / 4 + 8 of MT blocks, and their groups' scales and zero
@@ -112,55 +119,73 @@ int4_rows_kernel(const __grid_constant__ Params p) {
   const uint32_t rank = p.ctas > 1 ? cluster_rank() : 0;
   const int chunks = (p.K + kChunk - 1) / kChunk, total_n = GATED ? 2 * p.N : p.N;
   const int out0 = int(blockIdx.x / p.ctas) * (GATED ? 16 : kOuts);  // the CTA's first output
-  // where the lane's outputs begin, which need not begin a block (U's of a gated product); the second of two lies `codes_on` and
-  // `groups_on` behind the first
+  // Where the lane's outputs begin: rows g and g + 8 of a block, but for U's of a gated product, which need not begin one.  The
+  // second lies `codes_on` and `groups_on` behind the first.
+  constexpr int kCodesOn = 8 * 64, kGroupsOn = 8 * GPC;
+  const int step = p.ctas * warps;
   const uint8_t* codes_at[MT];
-  int64_t group_at[MT];
-  int codes_on[MT], groups_on[MT];
+  const uint16_t* scale_at[MT];
+  const uint8_t* zero_at[MT];
+  int codes_on = kCodesOn, groups_on = kGroupsOn;  // U's
+  int c = int(rank) * warps + warp;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    auto place = [&](int h, int64_t& codes, int64_t& groups) {
-      const int n = min(out0 + h * 8 + g + (GATED ? m * p.N : m * 16), total_n - 1);
-      const int64_t tile = int64_t(n / 16) * chunks;
+    auto place = [&](int n, int64_t& codes, int64_t& groups) {
+      const int64_t tile = int64_t(n / 16) * chunks + c;
       codes = tile * kTile + n % 16 * 64 + t * 16;
       groups = (tile * 16 + n % 16) * GPC;
     };
-    int64_t c0, c1, g0, g1;
-    place(0, c0, g0);
-    place(1, c1, g1);
-    codes_at[m] = p.codes + c0;
-    group_at[m] = g0;
-    codes_on[m] = int(c1 - c0);
-    groups_on[m] = int(g1 - g0);
+    int64_t codes, groups;
+    if (GATED && m == 1) {
+      const int n0 = min(out0 + g + p.N, total_n - 1), n1 = min(out0 + 8 + g + p.N, total_n - 1);
+      int64_t codes1, groups1;
+      place(n0, codes, groups);
+      place(n1, codes1, groups1);
+      codes_on = int(codes1 - codes);
+      groups_on = int(groups1 - groups);
+    } else {
+      place(min(out0 / 16 + m, (total_n - 1) / 16) * 16 + g, codes, groups);
+    }
+    codes_at[m] = p.codes + codes;
+    scale_at[m] = p.scale + groups;
+    zero_at[m] = p.zero ? p.zero + groups : nullptr;
   }
-  auto fetch = [&](int c) {
+  // The next chunk of the warp's.
+  auto fetch = [&]() {
     Fetched<MT, GPC> f;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m) {
+      const bool any = GATED && m == 1;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        f.codes[m][h] = __ldcs(reinterpret_cast<const uint4*>(codes_at[m] + int64_t(c) * kTile + (h ? codes_on[m] : 0)));
-        const int64_t at = group_at[m] + int64_t(c) * (16 * GPC) + (h ? groups_on[m] : 0);
+        f.codes[m][h] = __ldcs(reinterpret_cast<const uint4*>(codes_at[m] + (h == 0 ? 0 : any ? codes_on : kCodesOn)));
+        const uint16_t* scale = scale_at[m] + (h == 0 ? 0 : any ? groups_on : kGroupsOn);
+        const uint8_t* zero = zero_at[m] + (h == 0 ? 0 : any ? groups_on : kGroupsOn);
         if constexpr (GPC == 4) {
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(p.scale + at));
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(scale));
           f.scale[m][h][0] = v.x, f.scale[m][h][1] = v.y;
-          f.zero[m][h] = p.zero ? __ldg(reinterpret_cast<const uint32_t*>(p.zero + at)) : 0x08080808u;
+          f.zero[m][h] = p.zero ? __ldg(reinterpret_cast<const uint32_t*>(zero)) : 0x08080808u;
         } else if constexpr (GPC == 2) {
-          f.scale[m][h][0] = __ldg(reinterpret_cast<const uint32_t*>(p.scale + at));
-          f.zero[m][h] = p.zero ? __ldg(reinterpret_cast<const uint16_t*>(p.zero + at)) : 0x0808u;
+          f.scale[m][h][0] = __ldg(reinterpret_cast<const uint32_t*>(scale));
+          f.zero[m][h] = p.zero ? __ldg(reinterpret_cast<const uint16_t*>(zero)) : 0x0808u;
         } else {
-          f.scale[m][h][0] = __ldg(p.scale + at);
-          f.zero[m][h] = p.zero ? __ldg(p.zero + at) : 8;
+          f.scale[m][h][0] = __ldg(scale);
+          f.zero[m][h] = p.zero ? __ldg(zero) : 8;
         }
       }
+      codes_at[m] += int64_t(step) * kTile;
+      scale_at[m] += int64_t(step) * 16 * GPC;
+      zero_at[m] += int64_t(step) * 16 * GPC;
+    }
     return f;
   };
+  // Eight inputs of a row of X.  What columns beyond the last row hold, nobody reads: they take that row's once more.
   const uint16_t* x_at[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) x_at[n] = n * 8 + g < p.rows ? p.x + int64_t(n * 8 + g) * p.ldx + t * 8 : nullptr;
-  const int x_end = p.K - t * 8;  // of what may be read from x_at on
-  auto fetch_x = [&](int n, int k) {  // eight inputs
-    return x_at[n] && k < x_end ? __ldg(reinterpret_cast<const uint4*>(x_at[n] + k)) : make_uint4(0, 0, 0, 0);
+  for (int n = 0; n < NT; ++n) x_at[n] = p.x + int64_t(min(n * 8 + g, p.rows - 1)) * p.ldx + t * 8;
+  auto fetch_x = [&](int n, int k, bool all) {  // all: of the chunk, or some beyond the last input, where zeros go
+    if (all || k + t * 8 < p.K) return __ldg(reinterpret_cast<const uint4*>(x_at[n] + k));
+    return make_uint4(0, 0, 0, 0);
   };
 
   float tot[MT][NT][4], acc[MT][NT][4];
@@ -170,22 +195,32 @@ int4_rows_kernel(const __grid_constant__ Params p) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) tot[m][n][e] = 0.f;
-  const int step = p.ctas * warps;
-  int c = int(rank) * warps + warp;
   Fetched<MT, GPC> ring[DEPTH];
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
-    if (c + d * step < chunks) ring[d] = fetch(c + d * step);
-  if (GATED) let_next_begin();
+    if (c + d * step < chunks) ring[d] = fetch();
+  if (GATED) {
+    let_next_begin();
+    // the next launch's codes, a line per thread, on their way to the L2
+    for (int64_t at = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * 128; at < p.next_bytes; at += int64_t(gridDim.x) * blockDim.x * 128)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.next + at));
+  }
   if (p.wait) wait_for_last();
   // X of a chunk: for up to 16 rows all at once, and of up to 8 rows a chunk ahead
   constexpr bool kWhole = NT <= 2, kAhead = NT == 1;
   uint4 xs[kWhole ? NT : 1][4], xn[kAhead ? NT : 1][4];
   auto fetch_chunk = [&](uint4 (&to)[kWhole ? NT : 1][4], int at) {
+    if ((at + 1) * kChunk <= p.K) {
 #pragma unroll
-    for (int n = 0; n < (kWhole ? NT : 1); ++n)
+      for (int n = 0; n < (kWhole ? NT : 1); ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) to[n][j] = fetch_x(n, at * kChunk + j * 32);
+        for (int j = 0; j < 4; ++j) to[n][j] = fetch_x(n, at * kChunk + j * 32, true);
+    } else {
+#pragma unroll
+      for (int n = 0; n < (kWhole ? NT : 1); ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[n][j] = fetch_x(n, at * kChunk + j * 32, false);
+    }
   };
   if constexpr (kAhead)
     if (c < chunks) fetch_chunk(xs, c);
@@ -194,23 +229,19 @@ int4_rows_kernel(const __grid_constant__ Params p) {
     for (int d = 0; d < DEPTH; ++d, c += step) {
       if (c >= chunks) break;
       const Fetched<MT, GPC>& now = ring[d];
-      if constexpr (kAhead) fetch_chunk(xn, c + step);  // beyond the last: nothing is read
-      else if constexpr (kWhole) fetch_chunk(xs, c);
+      if constexpr (kAhead) {
+        if (c + step < chunks) fetch_chunk(xn, c + step);
+      } else if constexpr (kWhole) {
+        fetch_chunk(xs, c);
+      }
+      const bool all = (c + 1) * kChunk <= p.K;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {  // 32 inputs
-        if (j % kBlocks == 0) {
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.f;
-        }
         uint4 xj[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           if constexpr (kWhole) xj[n] = xs[n][j];
-          else xj[n] = fetch_x(n, c * kChunk + j * 32);
+          else xj[n] = fetch_x(n, c * kChunk + j * 32, all);
         }
         uint32_t a[MT][2][4];
 #pragma unroll
@@ -221,8 +252,9 @@ int4_rows_kernel(const __grid_constant__ Params p) {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            mma(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], xj[n].x, xj[n].y);
-            mma(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], xj[n].z, xj[n].w);
+            if (j % kBlocks == 0) mma<true>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], xj[n].x, xj[n].y);
+            else mma<false>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], xj[n].x, xj[n].y);
+            mma<false>(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], xj[n].z, xj[n].w);
           }
         if (j % kBlocks == kBlocks - 1) {
 #pragma unroll
@@ -242,7 +274,7 @@ int4_rows_kernel(const __grid_constant__ Params p) {
           }
         }
       }
-      if (c + DEPTH * step < chunks) ring[d] = fetch(c + DEPTH * step);
+      if (c + DEPTH * step < chunks) ring[d] = fetch();
       if constexpr (kAhead) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) xs[0][j] = xn[0][j];
@@ -493,6 +525,8 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes_
     p.rows = p.out_rows = int(M);
     p.K = int(D); p.N = int(H);
     p.act = act;
+    p.next = codes_out;
+    p.next_bytes = gc::ceil_div(O, 16) * gc::ceil_div(H, kChunk) * kTile;
     rc = product<true>(in, p, st);
     if (rc != GC_OK) return rc;
     Params q{};
