@@ -78,10 +78,10 @@ SIGNATURES = {
     "gc_grouped_linear_backward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _i32p, _i64, _i64, _i64, _i64, _void, _i64, _void,
                                                _void, _size, _void]),
     "gc_linear_int4_workspace_bytes": (_size, [_i64, _i64, _i64]),
-    "gc_linear_int4_bf16": (_int, [_void, _i64, _void, _void, _void, _int, _i64, _i64, _i64, _void, _i64, _void, _size, _void]),
+    "gc_linear_int4_bf16": (_int, [_void, _i64, _void, _int, _int, _i64, _i64, _i64, _void, _i64, _void, _size, _void]),
     "gc_gated_ffn_int4_workspace_bytes": (_size, [_i64, _i64, _i64, _i64]),
-    "gc_gated_ffn_int4_bf16": (_int, [_void, _i64, _void, _void, _void, _int, _void, _void, _void, _int, _i64, _i64, _i64, _i64, _int,
-                                      _void, _i64, _void, _size, _void]),
+    "gc_gated_ffn_int4_bf16": (_int, [_void, _i64, _void, _int, _int, _void, _int, _int, _i64, _i64, _i64, _i64, _int, _void, _i64, _void,
+                                      _size, _void]),
     "gc_distill_workspace_bytes": (_size, [_i64, _i64]),
     "gc_distill_forward": (_int, [_void, _int, _i64, _void, _int, _i64, _void, _int, _i64, _void, _i64, _i64, _i64, C.c_float,
                                   C.c_float, _f32p, _f32p, _void, _size, _void]),

@@ -338,26 +338,25 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return std::make_tuple(f.y, std::vector<Tensor>{f.x, f.w, f.offsets});
   }, NoGil());
   m.def("grouped_linear_backward", &grouped_linear_backward, NoGil());
-  const auto linear4 = [](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
-                          int64_t n) { return linear_int4(x, Int4{codes, scale, zero, group, k, n}); };
-  const auto block4 = [](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
-                         int64_t n, const Tensor& codes_out, const Tensor& scale_out, const OptTensor& zero_out, int64_t group_out,
-                         int64_t k_out, int64_t n_out, int64_t act) {
-    return gated_ffn_int4(x, Int4{codes, scale, zero, group, k, n}, Int4{codes_out, scale_out, zero_out, group_out, k_out, n_out}, act);
+  const auto linear4 = [](const Tensor& x, const Tensor& records, bool zeros, int64_t group, int64_t k, int64_t n) {
+    return linear_int4(x, Int4{records, zeros, group, k, n});
   };
-  m.def("linear_int4", [linear4](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
-                                 int64_t n) -> OptTensor {
+  const auto block4 = [](const Tensor& x, const Tensor& records, bool zeros, int64_t group, int64_t k, int64_t n, const Tensor& records_out,
+                         bool zeros_out, int64_t group_out, int64_t k_out, int64_t n_out, int64_t act) {
+    return gated_ffn_int4(x, Int4{records, zeros, group, k, n}, Int4{records_out, zeros_out, group_out, k_out, n_out}, act);
+  };
+  m.def("linear_int4", [linear4](const Tensor& x, const Tensor& records, bool zeros, int64_t group, int64_t k, int64_t n) -> OptTensor {
     if (recorded({&x})) raise("linear_int4 has no gradient: call it under torch.no_grad()");
     if (torch::jit::tracer::isTracing()) return std::nullopt;
-    return linear4(x, codes, scale, zero, group, k, n);
+    return linear4(x, records, zeros, group, k, n);
   }, NoGil());
   m.def("linear_int4_forward", linear4, NoGil());
-  m.def("gated_ffn_int4", [block4](const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& zero, int64_t group, int64_t k,
-                                   int64_t n, const Tensor& codes_out, const Tensor& scale_out, const OptTensor& zero_out,
-                                   int64_t group_out, int64_t k_out, int64_t n_out, int64_t act) -> OptTensor {
+  m.def("gated_ffn_int4", [block4](const Tensor& x, const Tensor& records, bool zeros, int64_t group, int64_t k, int64_t n,
+                                   const Tensor& records_out, bool zeros_out, int64_t group_out, int64_t k_out, int64_t n_out,
+                                   int64_t act) -> OptTensor {
     if (recorded({&x})) raise("gated_ffn_int4 has no gradient: call it under torch.no_grad(), or gated_ffn for training");
     if (torch::jit::tracer::isTracing()) return std::nullopt;
-    return block4(x, codes, scale, zero, group, k, n, codes_out, scale_out, zero_out, group_out, k_out, n_out, act);
+    return block4(x, records, zeros, group, k, n, records_out, zeros_out, group_out, k_out, n_out, act);
   }, NoGil());
   m.def("gated_ffn_int4_forward", block4, NoGil());
   m.def("adamw_step", &adamw_step, NoGil());

@@ -259,8 +259,8 @@ std::pair<Tensor, Tensor> grouped_linear_backward(const Tensor& dy, const Tensor
 Tensor grouped_linear(const Tensor& x, const Tensor& w, const Tensor& offsets);
 // A weight of 4 bits as it was laid out (int4.cpp).
 struct Int4 {
-  const Tensor &codes, &scale;
-  const OptTensor& zero;
+  const Tensor& records;
+  bool zeros;
   int64_t group, k, n;
 };
 Tensor linear_int4(const Tensor& x, const Int4& w);

@@ -5,21 +5,14 @@ namespace gch {
 
 namespace {
 const uint16_t* bits(const Tensor& t) { return static_cast<const uint16_t*>(t.const_data_ptr()); }
-const uint8_t* bytes(const OptTensor& t) {
-  return t && t->defined() ? static_cast<const uint8_t*>(t->const_data_ptr()) : nullptr;
-}
-// The buffers are what the kernels read, up to their ends: their sizes have to be those of the weight.
+const uint8_t* records(const Int4& w) { return static_cast<const uint8_t*>(w.records.const_data_ptr()); }
+// The buffer is what the kernels read, up to its end: its size has to be the weight's.
 void check_weight(const Int4& w, const at::Device& dev) {
-  require(w.k >= 0 && w.n >= 0 && (w.group == 32 || w.group == 64 || w.group == 128),
-          "Int4Weight: a group is 32, 64 or 128 inputs");
-  const int64_t tiles = (w.n + 15) / 16 * ((w.k + 127) / 128), groups = tiles * 16 * (128 / w.group);
-  require(w.codes.device() == dev && w.codes.scalar_type() == at::kByte && w.codes.is_contiguous() && w.codes.numel() == tiles * 1024,
-          "Int4Weight: codes must be what Int4Weight.from_codes lays out, on x's device");
-  require(w.scale.device() == dev && w.scale.scalar_type() == at::kBFloat16 && w.scale.is_contiguous() && w.scale.numel() == groups,
-          "Int4Weight: scale must be bfloat16 as Int4Weight.from_codes lays it out, on x's device");
-  require(!w.zero || !w.zero->defined() ||
-              (w.zero->device() == dev && w.zero->scalar_type() == at::kByte && w.zero->is_contiguous() && w.zero->numel() == groups),
-          "Int4Weight: zero must be uint8 as Int4Weight.from_codes lays it out, on x's device");
+  require(w.k >= 0 && w.n >= 0 && (w.group == 32 || w.group == 64 || w.group == 128), "Int4Weight: a group is 32, 64 or 128 inputs");
+  const int64_t groups = 16 * (128 / w.group), record = 1024 + groups * (w.zeros ? 3 : 2);
+  require(w.records.device() == dev && w.records.scalar_type() == at::kByte && w.records.is_contiguous() &&
+              w.records.numel() == (w.n + 15) / 16 * ((w.k + 127) / 128) * record,
+          "Int4Weight: records must be what Int4Weight.from_codes lays out, on x's device");
 }
 }  // namespace
 
@@ -33,7 +26,7 @@ Tensor linear_int4(const Tensor& xin, const Int4& w) {
   const int64_t M = x.size(0);
   Tensor y = at::empty({M, w.n}, x.options());
   const Scratch ws = product_workspace(abi.gc_linear_int4_workspace_bytes(M, w.k, w.n), dev);
-  check(abi.gc_linear_int4_bf16(bits(x), ld_of(x), bytes(w.codes), bits(w.scale), bytes(w.zero), int(w.group), M, w.k, w.n,
+  check(abi.gc_linear_int4_bf16(bits(x), ld_of(x), records(w), int(w.group), w.zeros, M, w.k, w.n,
                                 static_cast<uint16_t*>(y.data_ptr()), std::max<int64_t>(w.n, 1), ws.ptr, ws.bytes, stream_of(dev)),
         "gc_linear_int4_bf16");
   return y;
@@ -51,8 +44,8 @@ Tensor gated_ffn_int4(const Tensor& xin, const Int4& w_in, const Int4& w_out, in
   const int64_t M = x.size(0), O = w_out.n;
   Tensor y = at::empty({M, O}, x.options());
   const Scratch ws = product_workspace(abi.gc_gated_ffn_int4_workspace_bytes(M, w_in.k, w_out.k, O), dev);
-  check(abi.gc_gated_ffn_int4_bf16(bits(x), ld_of(x), bytes(w_in.codes), bits(w_in.scale), bytes(w_in.zero), int(w_in.group),
-                                   bytes(w_out.codes), bits(w_out.scale), bytes(w_out.zero), int(w_out.group), M, w_in.k, w_out.k, O,
+  check(abi.gc_gated_ffn_int4_bf16(bits(x), ld_of(x), records(w_in), int(w_in.group), w_in.zeros, records(w_out), int(w_out.group),
+                                   w_out.zeros, M, w_in.k, w_out.k, O,
                                    int(act), static_cast<uint16_t*>(y.data_ptr()), std::max<int64_t>(O, 1), ws.ptr, ws.bytes,
                                    stream_of(dev)),
         "gc_gated_ffn_int4_bf16");

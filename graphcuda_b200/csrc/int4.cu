@@ -2,15 +2,17 @@
 //
 //   W[k, n] = (code[k, n] - zero[k / group, n]) * scale[k / group, n]      codes 0 to 15, zero 8 where none is given, scale bf16
 //
-// Up to kFewRows rows every code is read once and the time is that of reading them.  A warp turns 16 outputs x 32 inputs of codes into
-// the bf16 operand of mma.sync -- code - zero is a whole number below 16 and exact there -- multiplies it by up to 64 rows of X, and
+// Up to 32 rows (16 in the block) every code is read once and the time is that of reading them.  A warp turns 16 outputs x 32 inputs of codes into
+// the bf16 operand of mma.sync -- code - zero is a whole number below 16 and exact there -- multiplies it by up to 32 rows of X, and
 // adds the fp32 sums of a group times its scale to the outputs' fp32 sums: no weight is ever rounded.  (The 5th-generation tensor
 // core takes its operands from shared memory and TMEM, through which every unpacked weight would have to go first; a
-// product that waits for memory gains nothing from its rate.)  Codes are laid out so that a lane's 16 bytes are what it
-// multiplies: see gc_linear_int4_bf16 in the header.
+// product that waits for memory gains nothing from its rate.)
 //
-// A CTA has 16 or 32 outputs, whose chunks of 128 inputs its warps take in turn; where the outputs alone do not fill the GPU, those of a
-// cluster do.  Sums meet in a fixed order.  In the block, the hidden row between the
+// Weights are records: of 16 outputs and 128 inputs the codes, scales and zero points (see gc_linear_int4_bf16 in the header), laid out so
+// that a lane's 16 bytes are what it multiplies.  A warp has a ring of records in shared memory, which one lane keeps filled
+// with bulk copies: some 100 KB have to be on their way to an SM at any time (64 KB in registers, as loads of 16 warps: 4.0 TB/s
+// without any arithmetic), and no instructions are spent on them.  A CTA takes 16 or 32 outputs at a time, whose records its warps take in
+// turn; where the outputs alone do not fill the GPU, those of a cluster do.  Sums meet in a fixed order.  In the block, the hidden row between the
 // two launches goes as two bf16 numbers, hi and lo, in twice the rows of X; the second launch starts while the first runs, and its
 // first codes are in registers when it has ended.
 //
@@ -27,18 +29,16 @@
 namespace {
 
 using namespace gc::ffn;
+using namespace gc::tc;
+using gc::tiles::align256;
+using gc::tiles::drain;
+using gc::tiles::up8;
 using bf16 = __nv_bfloat16;
 
 constexpr int kMostThreads = 256;
 constexpr int kChunk = 128;       // inputs of a chunk
-constexpr int kTile = 1024;       // bytes of 16 outputs' codes of a chunk
-constexpr int kMostColumns = 64;  // rows of X (of hi and lo: twice) that a launch takes
+constexpr int kMostColumns = 32;  // rows of X (of hi and lo: twice) that a launch takes
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
@@ -61,18 +61,69 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
-// Eight codes as four pairs of bf16 numbers less `zero`, a pair of 128 + zero point: 0x4300 is 128 and its last bits count ones.
+// Waits for a copy, a bounded time (tries of a microsecond at most); the same answer for all of a warp.
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
+  uint32_t tries = 1u << 21;
+  bool done;
+  do {
+    uint32_t now;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(now)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    done = now != 0;
+  } while (!done && --tries);
+  return __all_sync(0xFFFFFFFFu, done);
+}
+// Eight codes as four pairs of bf16 numbers less their zero points; 0x4300 is 128 and its last bits count ones, and `zero` is a pair of
+// -(128 + zero point).  (A multiply-add, by one: a subtraction would go to the pipe of the shifts and masks, which is the busy one.)
 __device__ __forceinline__ void unpack(uint32_t w, __nv_bfloat162 zero, uint32_t (&o)[4]) {
+  const __nv_bfloat162 one = __float2bfloat162_rn(1.f);
+  uint32_t mask;
+  asm("mov.b32 %0, 0x000F000F;" : "=r"(mask));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t t = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), zero);
+    uint32_t t;  // (w >> 4 i & mask) | 128s, in one instruction but for the shift: the mask waits in a register
+    asm("lop3.b32 %0, %1, %2, 0x43004300, 0xEA;" : "=r"(t) : "r"(w >> (4 * i)), "r"(mask));
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&t), one, zero);
     o[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
 }
 __device__ __forceinline__ __nv_bfloat162 zero_pair(uint32_t zeros, int byte) {
-  const uint32_t t = __byte_perm(zeros, 0x43u, 0x4040u + 0x0101u * byte);
+  const uint32_t t = __byte_perm(zeros, 0xC3u, 0x4040u + 0x0101u * byte);
   return *reinterpret_cast<const __nv_bfloat162*>(&t);
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ uint4 shared_16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 shared_8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t shared_4(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t shared_2(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t shared_1(uint32_t at) {
+  uint16_t v;
+  asm volatile("{\n\t.reg .u8 b;\n\tld.shared.u8 b, [%1];\n\tcvt.u16.u8 %0, b;\n\t}" : "=h"(v) : "r"(at) : "memory");
+  return v;
 }
 __device__ __forceinline__ float gated(float g, float u, int act) {
   float a = 0.f, unused;
@@ -83,110 +134,114 @@ __device__ __forceinline__ float gated(float g, float u, int act) {
   return a * u;
 }
 
+// A record: 64 bytes of codes for each of 16 outputs, their scales, their zero points.
+constexpr int kScales = 16 * 64;
+constexpr int kRun = 2;  // records that are fetched, waited for and given back together: of a block of outputs they follow each other
+__host__ __device__ constexpr int zeros_at(int gpc) { return kScales + 16 * gpc * 2; }
+__host__ __device__ constexpr int record_bytes(int gpc, bool zeros) { return zeros_at(gpc) + (zeros ? 16 * gpc : 0); }
+
 struct Params {
   const uint16_t* x;  // rows in 16-byte accesses, zeros up to the next multiple of 8 inputs
-  const uint8_t* codes;
-  const uint16_t* scale;
-  const uint8_t* zero;  // null: 8
+  const uint8_t* w;   // records
   uint16_t* out;
   int64_t ldx, ldo;
   int rows, out_rows;  // of X; of the output: half of them where X is hi and lo
   int K, N;            // N: outputs, of either half of a gated product
   int ctas;            // of a cluster
+  int ring;            // places in a warp's ring
   int act;
   int wait;  // X comes from the launch before
-  const uint8_t* next;  // gated: the codes of the launch behind
+  const uint8_t* next;  // gated: the records of the launch behind
   int64_t next_bytes;
+  int* word;  // the device's error word
 };
 
-// Of one chunk what a lane needs: codes of its outputs lane / 4 and lane / 4 + 8 of MT blocks, and their groups' scales and zero
-// points, packed as they lie.
-template <int MT, int GPC>
-struct Fetched {
-  uint4 codes[MT][2];
-  uint32_t scale[MT][2][GPC == 4 ? 2 : 1];
-  uint32_t zero[MT][2];
-};
-
-// NT: 8 rows of X each.  MT: blocks of 16 outputs of a CTA (GATED: the same ones of G and of U).  GPC: groups in a chunk.  DEPTH: chunks
-// that a warp has on their way to its registers.  The CTA's warps, and those of the cluster's other CTAs, take chunks in turn.
-template <int NT, int MT, bool GATED, int GPC, int DEPTH>
-__global__ void __launch_bounds__(kMostThreads, NT == 1 ? 2 : 1)
+// NT: 8 rows of X each.  MT: blocks of 16 outputs that a CTA takes at a time (GATED: the same ones of G and of U, whose outputs lie in two
+// blocks where SPLIT).  GPC: groups in a record.  ZEROS: whether records have zero points.
+template <int NT, int MT, bool GATED, bool SPLIT, int GPC, bool ZEROS>
+__global__ void __launch_bounds__(kMostThreads, NT == 1 ? (MT == 1 ? 3 : 2) : NT == 2 ? 2 : 1)
 int4_rows_kernel(const __grid_constant__ Params p) {
-  extern __shared__ float sums[];  // [warp][MT * 16][NT * 8]
+  extern __shared__ __align__(128) uint8_t shared[];  // sums of two turns, [warp][MT * 16][NT * 8]; barriers; rings
   constexpr int kCols = NT * 8, kOuts = MT * 16, kBlocks = 4 / GPC;  // kBlocks: 32s of inputs in a group
+  constexpr int kWidth = GATED ? 16 : kOuts;                         // outputs at a time
+  constexpr int kRecord = record_bytes(GPC, ZEROS), kCopies = SPLIT ? 3 : MT, kPlace = kCopies * kRun * kRecord;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32, g = lane / 4, t = lane % 4;
-  const uint32_t rank = p.ctas > 1 ? cluster_rank() : 0;
-  const int chunks = (p.K + kChunk - 1) / kChunk, total_n = GATED ? 2 * p.N : p.N;
-  const int out0 = int(blockIdx.x / p.ctas) * (GATED ? 16 : kOuts);  // the CTA's first output
-  // Where the lane's outputs begin: rows g and g + 8 of a block, but for U's of a gated product, which need not begin one.  The
-  // second lies `codes_on` and `groups_on` behind the first.
-  constexpr int kCodesOn = 8 * 64, kGroupsOn = 8 * GPC;
-  const int step = p.ctas * warps;
-  const uint8_t* codes_at[MT];
-  const uint16_t* scale_at[MT];
-  const uint8_t* zero_at[MT];
-  int codes_on = kCodesOn, groups_on = kGroupsOn;  // U's
-  int c = int(rank) * warps + warp;
+  const int rank = blockIdx.y;  // in the cluster
+  const int chunks = (p.K + kChunk - 1) / kChunk;
+  const int step = p.ctas * warps * kRun, first = (rank * warps + warp) * kRun;
+  float* const sums_of_two = reinterpret_cast<float*>(shared);
+  const uint32_t bars = smem_u32(shared) + 2 * warps * kOuts * kCols * 4 + warp * p.ring * 8;
+  const uint32_t ring = smem_u32(shared) + 2 * warps * kOuts * kCols * 4 + (warps * p.ring * 8 + 127) / 128 * 128 + warp * p.ring * kPlace;
+
+  // One lane fetches: the run of records from `ahead` on of the outputs from ahead_out on.
+  int ahead_out = blockIdx.x * kWidth, ahead = first;
+  const uint8_t* from[kCopies];
+  auto begin = [&]() {
+    const int last_block = ((GATED ? 2 * p.N : p.N) + 15) / 16 - 1;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    auto place = [&](int n, int64_t& codes, int64_t& groups) {
-      const int64_t tile = int64_t(n / 16) * chunks + c;
-      codes = tile * kTile + n % 16 * 64 + t * 16;
-      groups = (tile * 16 + n % 16) * GPC;
-    };
-    int64_t codes, groups;
-    if (GATED && m == 1) {
-      const int n0 = min(out0 + g + p.N, total_n - 1), n1 = min(out0 + 8 + g + p.N, total_n - 1);
-      int64_t codes1, groups1;
-      place(n0, codes, groups);
-      place(n1, codes1, groups1);
-      codes_on = int(codes1 - codes);
-      groups_on = int(groups1 - groups);
-    } else {
-      place(min(out0 / 16 + m, (total_n - 1) / 16) * 16 + g, codes, groups);
+    for (int i = 0; i < kCopies; ++i) {
+      const int b = GATED && i > 0 ? (ahead_out + p.N) / 16 + i - 1 : ahead_out / 16 + i;
+      from[i] = p.w + (int64_t(min(b, last_block)) * chunks + first) * kRecord;
     }
-    codes_at[m] = p.codes + codes;
-    scale_at[m] = p.scale + groups;
-    zero_at[m] = p.zero ? p.zero + groups : nullptr;
+  };
+  auto fetch = [&](uint32_t bar, uint32_t to) {
+    if (ahead >= chunks) {  // on to the CTA's next outputs
+      ahead_out += gridDim.x * kWidth;
+      ahead = first;
+      begin();
+    }
+    if (ahead_out >= p.N) return false;
+    const uint32_t bytes = min(kRun, chunks - ahead) * kRecord;
+    mbar_expect_tx(bar, kCopies * bytes);
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      bulk_load(to + i * (kRun * kRecord), from[i], bytes, bar);
+      from[i] += step * kRecord;
+    }
+    ahead += step;
+    return true;
+  };
+  int on_their_way = 0;  // copies, as lane 0 counts them
+  if (lane == 0 && first < chunks) {
+    for (int i = 0; i < p.ring; ++i) mbar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+    begin();
+    while (on_their_way < p.ring && fetch(bars + 8 * on_their_way, ring + on_their_way * kPlace)) ++on_their_way;
   }
-  // The next chunk of the warp's.
-  auto fetch = [&]() {
-    Fetched<MT, GPC> f;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const bool any = GATED && m == 1;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f.codes[m][h] = __ldcs(reinterpret_cast<const uint4*>(codes_at[m] + (h == 0 ? 0 : any ? codes_on : kCodesOn)));
-        const uint16_t* scale = scale_at[m] + (h == 0 ? 0 : any ? groups_on : kGroupsOn);
-        const uint8_t* zero = zero_at[m] + (h == 0 ? 0 : any ? groups_on : kGroupsOn);
-        if constexpr (GPC == 4) {
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(scale));
-          f.scale[m][h][0] = v.x, f.scale[m][h][1] = v.y;
-          f.zero[m][h] = p.zero ? __ldg(reinterpret_cast<const uint32_t*>(zero)) : 0x08080808u;
-        } else if constexpr (GPC == 2) {
-          f.scale[m][h][0] = __ldg(reinterpret_cast<const uint32_t*>(scale));
-          f.zero[m][h] = p.zero ? __ldg(reinterpret_cast<const uint16_t*>(zero)) : 0x0808u;
-        } else {
-          f.scale[m][h][0] = __ldg(scale);
-          f.zero[m][h] = p.zero ? __ldg(zero) : 8;
-        }
-      }
-      codes_at[m] += int64_t(step) * kTile;
-      scale_at[m] += int64_t(step) * 16 * GPC;
-      zero_at[m] += int64_t(step) * 16 * GPC;
-    }
-    return f;
+  __syncwarp();
+  uint32_t bar = bars, place = ring, parity = 0;  // what is used next, and the phase of its barrier
+  const uint32_t bar_end = bars + 8 * p.ring;
+  // Where in a place the lane's outputs lie, rows g and g + 8 of a block: its codes 16 bytes a lane, then 16 bytes a lane.  But for U's
+  // where they lie in two blocks.
+  auto row_of = [&](int h) { return g + h * 8 + p.N % 16; };
+  auto of_row = [&](int row) { return row / 16 * (kRun * kRecord); };
+  auto codes_at = [&](int m, int h) {
+    if (SPLIT && m == 1) return (kRun * kRecord) + of_row(row_of(h)) + row_of(h) % 16 * 64 + t * 16;
+    return m * (kRun * kRecord) + lane * 16 + h * 512;
+  };
+  auto groups_at = [&](int m, int h, int bytes) {  // `bytes` for each of the output's groups
+    if (SPLIT && m == 1) return (kRun * kRecord) + of_row(row_of(h)) + row_of(h) % 16 * (GPC * bytes);
+    return m * (kRun * kRecord) + (g + h * 8) * (GPC * bytes);
   };
   // Eight inputs of a row of X.  What columns beyond the last row hold, nobody reads: they take that row's once more.
   const uint16_t* x_at[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) x_at[n] = p.x + int64_t(min(n * 8 + g, p.rows - 1)) * p.ldx + t * 8;
-  auto fetch_x = [&](int n, int k, bool all) {  // all: of the chunk, or some beyond the last input, where zeros go
-    if (all || k + t * 8 < p.K) return __ldg(reinterpret_cast<const uint4*>(x_at[n] + k));
+  auto fetch_x = [&](int n, int c, int j, bool all) {  // all: of the chunk, or some beyond the last input, where zeros go
+    if (all || c * kChunk + j * 32 + t * 8 < p.K) return __ldg(reinterpret_cast<const uint4*>(x_at[n] + c * kChunk + j * 32));
     return make_uint4(0, 0, 0, 0);
   };
+  constexpr bool kWhole = NT <= 2;  // X of a chunk at once
+
+  if (GATED) {
+    let_next_begin();
+    // the next launch's records, a line per thread, on their way to the L2
+    for (int64_t i = ((int64_t(blockIdx.x) * p.ctas + rank) * blockDim.x + threadIdx.x) * 128; i < p.next_bytes;
+         i += int64_t(gridDim.x) * p.ctas * blockDim.x * 128)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.next + i));
+  }
+  if (p.wait) wait_for_last();
 
   float tot[MT][NT][4], acc[MT][NT][4];
 #pragma unroll
@@ -195,150 +250,168 @@ int4_rows_kernel(const __grid_constant__ Params p) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) tot[m][n][e] = 0.f;
-  Fetched<MT, GPC> ring[DEPTH];
+  float* sums = sums_of_two;
+  bool ok = true;
+  for (int out0 = blockIdx.x * kWidth; out0 < p.N; out0 += gridDim.x * kWidth) {
+    for (int c0 = first; c0 < chunks; c0 += step) {
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d)
-    if (c + d * step < chunks) ring[d] = fetch();
-  if (GATED) {
-    let_next_begin();
-    // the next launch's codes, a line per thread, on their way to the L2
-    for (int64_t at = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) * 128; at < p.next_bytes; at += int64_t(gridDim.x) * blockDim.x * 128)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.next + at));
-  }
-  if (p.wait) wait_for_last();
-  // X of a chunk: for up to 16 rows all at once, and of up to 8 rows a chunk ahead
-  constexpr bool kWhole = NT <= 2, kAhead = NT == 1;
-  uint4 xs[kWhole ? NT : 1][4], xn[kAhead ? NT : 1][4];
-  auto fetch_chunk = [&](uint4 (&to)[kWhole ? NT : 1][4], int at) {
-    if ((at + 1) * kChunk <= p.K) {
+      for (int u = 0; u < kRun; ++u) {
+        const int c = c0 + u;
+        if (u > 0 && c >= chunks) break;
+        const bool all = (c + 1) * kChunk <= p.K;
+        uint4 xs[NT][kWhole ? 4 : 1];
+        if constexpr (kWhole) {
+          if (all) {
 #pragma unroll
-      for (int n = 0; n < (kWhole ? NT : 1); ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) to[n][j] = fetch_x(n, at * kChunk + j * 32, true);
-    } else {
+              for (int j = 0; j < 4; ++j) xs[n][j] = fetch_x(n, c, j, true);
+          } else {
 #pragma unroll
-      for (int n = 0; n < (kWhole ? NT : 1); ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) to[n][j] = fetch_x(n, at * kChunk + j * 32, false);
-    }
-  };
-  if constexpr (kAhead)
-    if (c < chunks) fetch_chunk(xs, c);
-  for (; c < chunks;) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d, c += step) {
-      if (c >= chunks) break;
-      const Fetched<MT, GPC>& now = ring[d];
-      if constexpr (kAhead) {
-        if (c + step < chunks) fetch_chunk(xn, c + step);
-      } else if constexpr (kWhole) {
-        fetch_chunk(xs, c);
-      }
-      const bool all = (c + 1) * kChunk <= p.K;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {  // 32 inputs
-        uint4 xj[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if constexpr (kWhole) xj[n] = xs[n][j];
-          else xj[n] = fetch_x(n, c * kChunk + j * 32, all);
+              for (int j = 0; j < 4; ++j) xs[n][j] = fetch_x(n, c, j, false);
+          }
         }
-        uint32_t a[MT][2][4];
+        if (u == 0 && ok) ok = arrived(bar, parity);
+        uint4 codes[MT][2];
+        uint32_t scale[MT][2][GPC == 4 ? 2 : 1], zero[MT][2];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) unpack((&now.codes[m][h].x)[j], zero_pair(now.zero[m][h], j / kBlocks), a[m][h]);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            if (j % kBlocks == 0) mma<true>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], xj[n].x, xj[n].y);
-            else mma<false>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], xj[n].x, xj[n].y);
-            mma<false>(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], xj[n].z, xj[n].w);
+          for (int h = 0; h < 2; ++h) {
+            codes[m][h] = shared_16(place + u * kRecord + codes_at(m, h));
+            const uint32_t s = place + u * kRecord + kScales + groups_at(m, h, 2), z = place + u * kRecord + zeros_at(GPC) + groups_at(m, h, 1);
+            if constexpr (GPC == 4) {
+              const uint2 v = shared_8(s);
+              scale[m][h][0] = v.x, scale[m][h][1] = v.y;
+            } else {
+              scale[m][h][0] = GPC == 2 ? shared_4(s) : shared_2(s);
+            }
+            zero[m][h] = !ZEROS ? 0x08080808u : GPC == 4 ? shared_4(z) : GPC == 2 ? shared_2(z) : shared_1(z);
           }
-        if (j % kBlocks == kBlocks - 1) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            auto scale = [&](int h) {
-              const uint32_t w = now.scale[m][h][j / kBlocks / 2];
-              return __uint_as_float(j / kBlocks % 2 ? w & 0xFFFF0000u : w << 16);
-            };
-            const float s0 = scale(0), s1 = scale(1);
+        for (int j = 0; j < 4; ++j) {  // 32 inputs
+          if constexpr (!kWhole)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              tot[m][n][0] = fmaf(s0, acc[m][n][0], tot[m][n][0]);
-              tot[m][n][1] = fmaf(s0, acc[m][n][1], tot[m][n][1]);
-              tot[m][n][2] = fmaf(s1, acc[m][n][2], tot[m][n][2]);
-              tot[m][n][3] = fmaf(s1, acc[m][n][3], tot[m][n][3]);
+            for (int n = 0; n < NT; ++n) xs[n][0] = fetch_x(n, c, j, all);
+          auto x = [&](int n) { return xs[n][kWhole ? j : 0]; };
+          uint32_t a[MT][2][4];
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) unpack((&codes[m][h].x)[j], zero_pair(zero[m][h], j / kBlocks), a[m][h]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              if (j % kBlocks == 0) mma<true>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x(n).x, x(n).y);
+              else mma<false>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x(n).x, x(n).y);
+              mma<false>(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], x(n).z, x(n).w);
+            }
+          if (j % kBlocks == kBlocks - 1) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              auto value = [&](int h) {
+                const uint32_t w = scale[m][h][j / kBlocks / 2];
+                return __uint_as_float(j / kBlocks % 2 ? w & 0xFFFF0000u : w << 16);
+              };
+              const float s0 = value(0), s1 = value(1);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                tot[m][n][0] = fmaf(s0, acc[m][n][0], tot[m][n][0]);
+                tot[m][n][1] = fmaf(s0, acc[m][n][1], tot[m][n][1]);
+                tot[m][n][2] = fmaf(s1, acc[m][n][2], tot[m][n][2]);
+                tot[m][n][3] = fmaf(s1, acc[m][n][3], tot[m][n][3]);
+              }
             }
           }
         }
       }
-      if (c + DEPTH * step < chunks) ring[d] = fetch();
-      if constexpr (kAhead) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) xs[0][j] = xn[0][j];
+      __syncwarp();  // all have read
+      if (ok) {
+        if (lane == 0 && !fetch(bar, place)) --on_their_way;
+        bar += 8;
+        place += kPlace;
+        if (bar == bar_end) bar = bars, place = ring, parity ^= 1;
       }
     }
-  }
+    // ---- the outputs' sums: over the warps, over the cluster, of hi and lo
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        sums[(warp * kOuts + m * 16 + g + e / 2 * 8) * kCols + n * 8 + 2 * t + e % 2] = tot[m][n][e];
-  __syncthreads();
-  for (int i = threadIdx.x; i < kOuts * kCols; i += blockDim.x) {
-    float s = sums[i];
-    for (int w = 1; w < warps; ++w) s += sums[w * kOuts * kCols + i];
-    sums[i] = s;
-  }
-  if (p.ctas > 1) cluster_sync();
-  else __syncthreads();
-  auto whole = [&](int out, int row) {  // over the cluster; hi and lo
-    float s = 0.f;
-    for (int r = row; r < p.rows; r += p.out_rows)
-      for (int q = 0; q < p.ctas; ++q) {
+        for (int h = 0; h < 2; ++h) {
+          float2* to = reinterpret_cast<float2*>(sums + (warp * kOuts + m * 16 + g + h * 8) * kCols + n * 8 + 2 * t);
+          *to = make_float2(tot[m][n][2 * h], tot[m][n][2 * h + 1]);
+          tot[m][n][2 * h] = tot[m][n][2 * h + 1] = 0.f;
+        }
+    __syncthreads();
+    if (p.ctas > 1) {
+      for (int i = threadIdx.x; i < kOuts * kCols; i += blockDim.x) {
+        float s = sums[i];
+        for (int w = 1; w < warps; ++w) s += sums[w * kOuts * kCols + i];
+        sums[i] = s;
+      }
+      cluster_sync();
+    }
+    auto whole = [&](int out, int row) {
+      float s = 0.f;
+      for (int r = row; r < p.rows; r += p.out_rows) {
         const float* v = sums + out * kCols + r;
-        s += p.ctas > 1 ? peer_load(v, q) : *v;
+        if (p.ctas > 1)
+          for (int q = 0; q < p.ctas; ++q) s += peer_load(v, q);
+        else
+          for (int w = 0; w < warps; ++w) s += v[w * kOuts * kCols];
       }
-    return s;
-  };
-  constexpr int kWidth = GATED ? 16 : kOuts;  // outputs of the CTA, which the cluster shares out among its CTAs
-  for (int i = int(rank) * blockDim.x + threadIdx.x; i < kWidth * p.out_rows; i += p.ctas * blockDim.x) {
-    const int r = i / kWidth, o = i % kWidth, n = out0 + o;
-    bf16* to = reinterpret_cast<bf16*>(p.out) + r * p.ldo + n;
-    if constexpr (GATED) {
-      const float h = n < p.N ? gated(whole(o, r), whole(o + 16, r), p.act) : 0.f;
-      const bf16 hi = __float2bfloat16_rn(h);
-      if (n < (p.N + 7) / 8 * 8) {  // zeros up to there
-        to[0] = hi;
-        to[p.out_rows * p.ldo] = __float2bfloat16_rn(isfinite(__bfloat162float(hi)) ? h - __bfloat162float(hi) : 0.f);  // of inf nothing is left
+      return s;
+    };
+    // a cluster shares the outputs out among its CTAs
+    for (int i = rank * blockDim.x + threadIdx.x; i < kWidth * p.out_rows; i += p.ctas * blockDim.x) {
+      const int r = i / kWidth, o = i % kWidth, n = out0 + o;
+      bf16* to = reinterpret_cast<bf16*>(p.out) + r * p.ldo + n;
+      if constexpr (GATED) {
+        const float h = n < p.N ? gated(whole(o, r), whole(o + 16, r), p.act) : 0.f;
+        const bf16 hi = __float2bfloat16_rn(h);
+        if (n < (p.N + 7) / 8 * 8) {  // zeros up to there
+          to[0] = hi;
+          to[p.out_rows * p.ldo] = __float2bfloat16_rn(isfinite(__bfloat162float(hi)) ? h - __bfloat162float(hi) : 0.f);  // of inf nothing is left
+        }
+      } else if (n < p.N) {
+        to[0] = __float2bfloat16_rn(whole(o, r));
       }
-    } else if (n < p.N) {
-      to[0] = __float2bfloat16_rn(whole(o, r));
     }
+    if (p.ctas > 1) cluster_sync();  // a CTA's shared memory is read by the others until here
+    // the other half of the shared memory: the one before's readers have all come past the barrier since
+    sums = sums == sums_of_two ? sums_of_two + warps * kOuts * kCols : sums_of_two;
   }
-  if (p.ctas > 1) cluster_sync();  // a CTA's shared memory is read by the others until here
+  // what was fetched has all been waited for, unless a wait ran out
+  if (!ok && lane == 0) {
+    for (; on_their_way > 0; --on_their_way) {
+      drain(bar, parity);
+      bar += 8;
+      if (bar == bar_end) bar = bars, parity ^= 1;
+    }
+    atomicExch(p.word, 1);
+  }
 }
 
 // Weights as bf16, an output's inputs in a row: eight of them per thread.
 __global__ void __launch_bounds__(256)
-int4_unpack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scale, const uint8_t* __restrict__ zero, int K, int N,
-                   int gpc, uint16_t* __restrict__ w, int64_t ldw) {
-  const int chunks = (K + kChunk - 1) / kChunk;
+int4_unpack_kernel(const uint8_t* __restrict__ records, int zeros, int K, int N, int gpc, uint16_t* __restrict__ w, int64_t ldw) {
+  const int chunks = (K + kChunk - 1) / kChunk, size = record_bytes(gpc, zeros != 0);
   const int64_t total = int64_t(N) * chunks * 16;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
     const int piece = int(i % 16), j = piece / 4, t = piece % 4;
     const int c = int(i / 16 % chunks), n = int(i / 16 / chunks), k = c * kChunk + piece * 8;
     if (k >= K) continue;
-    const int64_t tile = int64_t(n / 16) * chunks + c;
-    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(codes + tile * kTile + n % 16 * 64 + t * 16) + j);
-    const int64_t at = (tile * 16 + n % 16) * gpc + j * gpc / 4;
-    const float s = __uint_as_float(uint32_t(__ldg(scale + at)) << 16);
+    const uint8_t* r = records + (int64_t(n / 16) * chunks + c) * size;
+    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(r + n % 16 * 64 + t * 16) + j);
+    const int group = n % 16 * gpc + j * gpc / 4;
+    const float s = __uint_as_float(uint32_t(__ldg(reinterpret_cast<const uint16_t*>(r + kScales) + group)) << 16);
     uint32_t o[4];
-    unpack(word, zero_pair(zero ? __ldg(zero + at) : 8, 0), o);
+    unpack(word, zero_pair(zeros ? __ldg(r + zeros_at(gpc) + group) : 8, 0), o);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const __nv_bfloat162 v = __floats2bfloat162_rn(s * __uint_as_float(o[e] << 16), s * __uint_as_float(o[e] & 0xFFFF0000u));
@@ -350,31 +423,37 @@ int4_unpack_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict
 
 // ------------------------------------------------------------------ host
 struct Weights {
-  const uint8_t* codes;
-  const uint16_t* scale;
-  const uint8_t* zero;
-  int group;
+  const uint8_t* records;
+  int group, zeros;
+  int gpc() const { return kChunk / group; }
+  int64_t bytes(int64_t K, int64_t N) const { return gc::ceil_div(N, 16) * gc::ceil_div(K, kChunk) * record_bytes(gpc(), zeros); }
 };
-using gc::tiles::align256;
-using gc::tiles::up8;
 
-template <int NT, int MT, bool GATED, int GPC, int DEPTH>
+template <int NT, int MT, bool GATED, bool SPLIT, int GPC, bool ZEROS>
 int launch_rows(Params p, cudaStream_t st) {
   const int64_t blocks = gc::ceil_div(p.N, GATED ? 16 : 16 * MT);
-  const int chunks = int(gc::ceil_div(p.K, kChunk));
-  const int warps = chunks >= 32 ? 8 : 4;
-  // All warps at once, 16 to an SM
+  const int runs = int(gc::ceil_div(gc::ceil_div(p.K, kChunk), kRun));
+  const int warps = runs >= 16 ? 8 : 4, per_sm = NT == 1 && MT == 1 ? 24 : NT <= 2 ? 16 : 8;
+  // All warps at once: outputs beyond those follow in the same CTAs.
+  const int64_t slots = per_sm / warps * gc::kNumSMs;
   p.ctas = 1;
-  while (p.ctas < 8 && blocks * 2 * p.ctas * warps <= 16 * gc::kNumSMs && 2 * p.ctas * warps <= chunks) p.ctas *= 2;
-  if (blocks * p.ctas > 0x7FFFFFFF) return gc::fail(GC_ERR_UNSUPPORTED, "4-bit product: too many outputs");
-  const size_t smem = size_t(warps) * MT * 16 * NT * 8 * sizeof(float);
-  auto kern = int4_rows_kernel<NT, MT, GATED, GPC, DEPTH>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  }
+  while (p.ctas < 8 && blocks * 2 * p.ctas <= slots && 2 * p.ctas * warps <= runs) p.ctas *= 2;
+  const int64_t ctas = std::min(blocks, slots);
+  // As many places in a ring as a warp has runs of records, up to what the SM's shared memory holds.
+  constexpr int kPlace = (SPLIT ? 3 : MT) * kRun * record_bytes(GPC, ZEROS);
+  const int64_t mine = gc::ceil_div(runs, p.ctas * warps) * gc::ceil_div(blocks, ctas);
+  const int sums = 2 * warps * MT * 16 * NT * 8 * int(sizeof(float));
+  const int room = (220 * 1024 / (per_sm / warps) - 1024 - 256 - sums) / warps;
+  static_assert((220 * 1024 / (NT == 1 && MT == 1 ? 6 : NT <= 2 ? 4 : 2) - 1280) / 4 - 2 * MT * 16 * NT * 8 * 4 >= kPlace + 8, "room for a place");
+  p.ring = int(std::min<int64_t>({mine, 16, room / (kPlace + 8)}));
+  const int smem = sums + (warps * p.ring * 8 + 127) / 128 * 128 + warps * p.ring * kPlace;
+  auto kern = int4_rows_kernel<NT, MT, GATED, SPLIT, GPC, ZEROS>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  const int rc = gc::tiles::error_word(&p.word);
+  if (rc != GC_OK) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(blocks * p.ctas));
+  cfg.gridDim = dim3(unsigned(ctas), unsigned(p.ctas));
   cfg.blockDim = dim3(unsigned(32 * warps));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -386,28 +465,39 @@ int launch_rows(Params p, cudaStream_t st) {
   }
   if (p.ctas > 1) {
     at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[cfg.numAttrs].val.clusterDim.x = unsigned(p.ctas);
-    at[cfg.numAttrs].val.clusterDim.y = 1;
+    at[cfg.numAttrs].val.clusterDim.x = 1;
+    at[cfg.numAttrs].val.clusterDim.y = unsigned(p.ctas);
     at[cfg.numAttrs++].val.clusterDim.z = 1;
   }
   cudaLaunchKernelEx(&cfg, kern, p);
   return gc::check_launch("int4_rows_kernel");
 }
+// Records from which on a warp takes two blocks of outputs at a time, with half of the instructions around them.
+constexpr int64_t kWideFrom = 16384;
+template <bool GATED, int GPC, bool ZEROS>
+int launch_for(const Params& p, cudaStream_t st) {
+  auto sized = [&](auto split) {
+    constexpr bool kSplit = decltype(split)::value;
+    if (p.rows > 16) return launch_rows<4, 2, GATED, kSplit, GPC, ZEROS>(p, st);
+    if (p.rows > 8) return launch_rows<2, 2, GATED, kSplit, GPC, ZEROS>(p, st);
+    if constexpr (!GATED)
+      if (gc::ceil_div(p.N, 16) * gc::ceil_div(p.K, kChunk) < kWideFrom) return launch_rows<1, 1, GATED, kSplit, GPC, ZEROS>(p, st);
+    return launch_rows<1, 2, GATED, kSplit, GPC, ZEROS>(p, st);
+  };
+  if constexpr (GATED)
+    if (p.N % 16) return sized(std::true_type{});
+  return sized(std::false_type{});
+}
 template <bool GATED>
 int product(const Weights& w, Params p, cudaStream_t st) {
-  p.codes = w.codes;
-  p.scale = w.scale;
-  p.zero = w.zero;
-  auto sized = [&](auto gpc) {
+  p.w = w.records;
+  auto zeros = [&](auto gpc) {
     constexpr int kGpc = decltype(gpc)::value;
-    if (p.rows <= 8) return launch_rows<1, GATED ? 2 : 1, GATED, kGpc, GATED ? 2 : 4>(p, st);
-    if (p.rows <= 16) return launch_rows<2, 2, GATED, kGpc, 2>(p, st);
-    if (p.rows <= 32) return launch_rows<4, 2, GATED, kGpc, 2>(p, st);
-    return launch_rows<8, 2, GATED, kGpc, 1>(p, st);
+    return w.zeros ? launch_for<GATED, kGpc, true>(p, st) : launch_for<GATED, kGpc, false>(p, st);
   };
-  return w.group == 32    ? sized(std::integral_constant<int, 4>{})
-         : w.group == 64 ? sized(std::integral_constant<int, 2>{})
-                         : sized(std::integral_constant<int, 1>{});
+  return w.group == 32    ? zeros(std::integral_constant<int, 4>{})
+         : w.group == 64 ? zeros(std::integral_constant<int, 2>{})
+                         : zeros(std::integral_constant<int, 1>{});
 }
 // X as the kernel takes it: itself, or a copy in the workspace.
 bool rows_ready(const uint16_t* X, int64_t ldx, int64_t K) { return gc::aligned16(X) && ldx % 8 == 0 && K % 8 == 0; }
@@ -426,19 +516,19 @@ int ready_rows(Params& p, const uint16_t* X, int64_t ldx, int64_t M, int64_t K, 
 int unpack_to(const Weights& w, int64_t K, int64_t N, void* to, cudaStream_t st) {
   const int64_t pieces = N * gc::ceil_div(K, kChunk) * 16;
   int4_unpack_kernel<<<unsigned(std::min<int64_t>(gc::ceil_div(pieces, 256), gc::kNumSMs * 32)), 256, 0, st>>>(
-      w.codes, w.scale, w.zero, int(K), int(N), kChunk / w.group, static_cast<uint16_t*>(to), up8(K));
+      w.records, w.zeros, int(K), int(N), w.gpc(), static_cast<uint16_t*>(to), up8(K));
   return gc::check_launch("int4_unpack_kernel");
 }
 size_t unpacked_bytes(int64_t K, int64_t N) { return align256(size_t(N) * up8(K) * 2); }
 
 bool sizes_ok(int64_t M, int64_t K, int64_t N) {
-  const int64_t top = (int64_t(1) << 30) - 512;  // coordinates are 32-bit, and so is the way from a block's codes to the next one's
+  const int64_t top = (int64_t(1) << 30) - 512;  // coordinates are 32-bit
   return M <= top && K <= top / 8 && N <= top;
 }
 int weights_ok(const Weights& w, const char* what) {
   GC_REQUIRE(w.group == 32 || w.group == 64 || w.group == 128, "%s: a group is 32, 64 or 128 inputs", what);
-  GC_REQUIRE(w.codes && w.scale, "%s: null pointer", what);
-  GC_REQUIRE(gc::aligned16(w.codes) && gc::aligned16(w.scale) && gc::aligned16(w.zero), "%s: weights must be 16-byte aligned", what);
+  GC_REQUIRE(w.records, "%s: null pointer", what);
+  GC_REQUIRE(gc::aligned16(w.records), "%s: weights must be 16-byte aligned", what);
   return GC_OK;
 }
 int zeros(uint16_t* Y, int64_t ldy, int64_t M, int64_t N, cudaStream_t st, const char* what) {
@@ -457,9 +547,8 @@ size_t gc_linear_int4_workspace_bytes(int64_t M, int64_t K, int64_t N) {
   return unpacked_bytes(K, N) + gc::ffn::rows_workspace(M, K, N);
 }
 
-int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes, const uint16_t* scale, const uint8_t* zero, int group,
-                        int64_t M, int64_t K, int64_t N, uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes,
-                        void* stream) {
+int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* W, int group, int zero_points, int64_t M, int64_t K, int64_t N,
+                        uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   GC_REQUIRE(M >= 0 && K >= 0 && N >= 0, "gc_linear_int4_bf16: negative size");
   GC_REQUIRE(ldx >= K && ldy >= N, "gc_linear_int4_bf16: leading dimension below the row length");
   if (!sizes_ok(M, K, N)) return gc::fail(GC_ERR_UNSUPPORTED, "gc_linear_int4_bf16: rows or outputs beyond 2^30, or inputs beyond 2^27");
@@ -468,7 +557,7 @@ int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes, co
   GC_REQUIRE(Y, "gc_linear_int4_bf16: null pointer");
   if (K == 0) return zeros(Y, ldy, M, N, st, "gc_linear_int4_bf16");
   GC_REQUIRE(X, "gc_linear_int4_bf16: null pointer");
-  const Weights w{codes, scale, zero, group};
+  const Weights w{W, group, zero_points != 0};
   int rc = weights_ok(w, "gc_linear_int4_bf16");
   if (rc != GC_OK) return rc;
   if (!workspace || workspace_bytes < gc_linear_int4_workspace_bytes(M, K, N))
@@ -496,10 +585,9 @@ size_t gc_gated_ffn_int4_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_
   return unpacked_bytes(D, 2 * H) + unpacked_bytes(H, O) + gc::ffn::block_workspace(M, D, H, O);
 }
 
-int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes_in, const uint16_t* scale_in, const uint8_t* zero_in,
-                           int group_in, const uint8_t* codes_out, const uint16_t* scale_out, const uint8_t* zero_out, int group_out,
-                           int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace,
-                           size_t workspace_bytes, void* stream) {
+int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, int group_in, int zero_points_in, const uint8_t* Wout,
+                           int group_out, int zero_points_out, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y,
+                           int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   GC_REQUIRE(M >= 0 && D >= 0 && H >= 0 && O >= 0, "gc_gated_ffn_int4_bf16: negative size");
   GC_REQUIRE(act >= GC_ACT_SILU && act <= GC_ACT_RELU, "gc_gated_ffn_int4_bf16: unknown activation");
   GC_REQUIRE(ldx >= D && ldy >= O, "gc_gated_ffn_int4_bf16: leading dimension below the row length");
@@ -509,7 +597,7 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes_
   GC_REQUIRE(Y, "gc_gated_ffn_int4_bf16: null pointer");
   if (D == 0 || H == 0) return zeros(Y, ldy, M, O, st, "gc_gated_ffn_int4_bf16");
   GC_REQUIRE(X, "gc_gated_ffn_int4_bf16: null pointer");
-  const Weights in{codes_in, scale_in, zero_in, group_in}, out{codes_out, scale_out, zero_out, group_out};
+  const Weights in{Win, group_in, zero_points_in != 0}, out{Wout, group_out, zero_points_out != 0};
   int rc = weights_ok(in, "gc_gated_ffn_int4_bf16");
   if (rc == GC_OK) rc = weights_ok(out, "gc_gated_ffn_int4_bf16");
   if (rc != GC_OK) return rc;
@@ -525,8 +613,8 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes_
     p.rows = p.out_rows = int(M);
     p.K = int(D); p.N = int(H);
     p.act = act;
-    p.next = codes_out;
-    p.next_bytes = gc::ceil_div(O, 16) * gc::ceil_div(H, kChunk) * kTile;
+    p.next = Wout;
+    p.next_bytes = out.bytes(H, O);
     rc = product<true>(in, p, st);
     if (rc != GC_OK) return rc;
     Params q{};

@@ -15,15 +15,13 @@ _CHUNK = 128  # inputs whose codes lie together
 class Int4Weight(torch.nn.Module):
     """A weight matrix [in, out] of 4-bit codes: ``(code - zero) * scale`` with a bfloat16 scale, and a zero point of 0 to 15 (8 where
     there is none), for every ``group`` inputs of an output.  Made by ``quantize_weight_int4`` or, of codes that exist, by
-    ``from_codes``; ``dequantize`` gives the values back.  Its buffers are in the order in which the kernels read them."""
+    ``from_codes``; ``dequantize`` gives the values back.  Its buffer is in the order in which the kernels read it."""
 
-    def __init__(self, codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor], in_features: int,
-                 out_features: int, group: int):
+    def __init__(self, records: torch.Tensor, zero_points: bool, in_features: int, out_features: int, group: int):
         super().__init__()
-        self.in_features, self.out_features, self.group = in_features, out_features, group
-        self.register_buffer("codes", codes)  # uint8 [out / 16, in / 128, 1024]
-        self.register_buffer("scale", scale)  # bfloat16 [out / 16, in / 128, 16, 128 / group]
-        self.register_buffer("zero", zero)    # uint8 like scale, or None
+        self.zero_points, self.in_features, self.out_features, self.group = zero_points, in_features, out_features, group
+        # uint8 [out / 16, in / 128, record]: codes [16, 64], scales [16, 128 / group] of 2 bytes, zero points [16, 128 / group] of one
+        self.register_buffer("records", records)
 
     @staticmethod
     def from_codes(codes: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None, *, group: int) -> "Int4Weight":
@@ -53,27 +51,31 @@ class Int4Weight(torch.nn.Module):
         def laid(t):
             s = t.new_zeros(blocks * 16, chunks * per)
             s[:n, :groups] = t.t()
-            return s.view(blocks, 16, chunks, per).transpose(1, 2).contiguous()
+            return s.view(blocks, 16, chunks, per).transpose(1, 2).contiguous().view(blocks, chunks, 16 * per).view(torch.uint8)
 
-        return Int4Weight(q.contiguous(), laid(scale), None if zero is None else laid(zero), k, n, group)
+        parts = [q, laid(scale)] + ([] if zero is None else [laid(zero)])
+        return Int4Weight(torch.cat(parts, 2).contiguous(), zero is not None, k, n, group)
 
     def dequantize(self) -> torch.Tensor:
         """The weights' values, float32 [in, out]."""
-        blocks, chunks = self.codes.shape[:2]
-        q = torch.stack((self.codes & 15, self.codes >> 4), -1).view(blocks, chunks, 2, 8, 4, 4, 2, 4)
+        blocks, chunks = self.records.shape[:2]
+        per = _CHUNK // self.group
+        codes, scale, zero = self.records.split((1024, 32 * per, 16 * per if self.zero_points else 0), 2)
+        q = torch.stack((codes & 15, codes >> 4), -1).view(blocks, chunks, 2, 8, 4, 4, 2, 4)
         q = q.permute(0, 2, 3, 1, 5, 4, 7, 6).reshape(blocks * 16, chunks * _CHUNK)
 
         def flat(t):
-            return t.transpose(1, 2).reshape(blocks * 16, chunks * _CHUNK // self.group).repeat_interleave(self.group, 1).float()
+            t = t.reshape(blocks, chunks, 16, per).transpose(1, 2).reshape(blocks * 16, chunks * per)
+            return t.repeat_interleave(self.group, 1).float()
 
-        w = (q.float() - (8.0 if self.zero is None else flat(self.zero))) * flat(self.scale)
+        w = (q.float() - (flat(zero) if self.zero_points else 8.0)) * flat(scale.contiguous().view(torch.bfloat16))
         return w[:self.out_features, :self.in_features].t().contiguous()
 
     def _parts(self):
-        return self.codes, self.scale, self.zero, self.group, self.in_features, self.out_features
+        return self.records, self.zero_points, self.group, self.in_features, self.out_features
 
     def extra_repr(self) -> str:
-        return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, zero_points={self.zero is not None}"
+        return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}, zero_points={self.zero_points}"
 
 
 def quantize_weight_int4(w: torch.Tensor, group: int = 64, zero_points: bool = False) -> Int4Weight:
@@ -109,8 +111,8 @@ class _TracedLinear(torch.autograd.Function):
     """The product inside torch.jit.trace (see gcn._TracedConv)."""
 
     @staticmethod
-    def forward(ctx, x, codes, scale, zero, group, k, n):
-        return _lib.host.linear_int4_forward(x, codes, scale, zero, group, k, n)
+    def forward(ctx, x, *call):
+        return _lib.host.linear_int4_forward(x, *call)
 
     @staticmethod
     def backward(ctx, dy):
@@ -132,7 +134,7 @@ class _TracedBlock(torch.autograd.Function):
 def linear_int4(x: torch.Tensor, w: Int4Weight) -> torch.Tensor:
     """``x @ w``: ``x`` is bfloat16 [rows, in], the result bfloat16 [rows, out], sums are float32.
 
-    Up to 64 rows the weights' values enter unrounded, and only the result's rounding shows.  For more rows they are rounded to
+    Up to 32 rows the weights' values enter unrounded, and only the result's rounding shows.  For more rows they are rounded to
     bfloat16 on their way to the tensor cores, which adds as much again (2.4e-3 instead of 1.7e-3, relative, root mean square)."""
     y = _lib.host.linear_int4(x, *w._parts())
     return y if y is not None else _TracedLinear.apply(x, *w._parts())
@@ -142,7 +144,7 @@ def gated_ffn_int4(x: torch.Tensor, w_in: Int4Weight, w_out: Int4Weight, activat
     """``gated_ffn`` for serving with both weights in 4 bits: ``(act(x @ Wg) * (x @ Wu)) @ w_out`` with ``w_in = [Wg | Wu]``; ``x``
     and the result are bfloat16.
 
-    Up to 32 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
+    Up to 16 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
     rounded to bfloat16 (4e-3 instead of 1.7e-3, relative, root mean square; the hidden row up to 64 rows not)."""
     act = _act(activation)
     y = _lib.host.gated_ffn_int4(x, *w_in._parts(), *w_out._parts(), act)

@@ -564,25 +564,24 @@ int gc_grouped_linear_backward_bf16(const uint16_t* dY, int64_t lddy, const uint
 /*
  * Products with weights of 4 bits, for serving: Y (M x N, bf16) = X (M x K, bf16) W with
  *   W[k, n] = (code - zero) * scale
- * of an input's group of 32, 64 or 128 (`group`) and an output: codes and zero points 0 to 15 (zero null: 8), scales bf16.  Laid out,
- * 16-byte aligned, for ceil(N / 16) blocks of 16 outputs and, within one, ceil(K / 128) chunks of 128 inputs (what lies beyond N and K
- * may be anything, scales there finite):
- *   codes  1024 bytes per block and chunk, 64 per output: inputs 32 j + 8 t to 32 j + 8 t + 7 in the 32-bit word 4 t + j, of which
- *          inputs 0, 2, 4, 6 are the four codes of the lower half from the lowest bits up, and 1, 3, 5, 7 those of the upper half
- *   scale, zero   [block][chunk][16 outputs][128 / group], zero in bytes
- * Up to 64 rows weights are not rounded; above, they are unpacked into bf16 in the workspace.
+ * of an input's group of 32, 64 or 128 (`group`) and an output: codes and zero points 0 to 15 (8 where there are none), scales bf16.  W is
+ * laid out in records, 16-byte aligned, one for every block of 16 outputs and, within it, every chunk of 128 inputs:
+ *   codes   64 bytes per output: inputs 32 j + 8 t to 32 j + 8 t + 7 of the chunk in the 32-bit word 4 t + j, of which inputs 0, 2, 4, 6
+ *           are the four codes of the lower half from the lowest bits up, and 1, 3, 5, 7 those of the upper half
+ *   scales  [16 outputs][128 / group]
+ *   zero points, where there are any (zero_points != 0): [16 outputs][128 / group], a byte each
+ * What lies beyond N and K may be anything; scales there are finite.  Up to 32 rows weights are not rounded; above, they are unpacked
+ * into bf16 in the workspace.
  */
 size_t gc_linear_int4_workspace_bytes(int64_t M, int64_t K, int64_t N);
-int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes, const uint16_t* scale, const uint8_t* zero, int group,
-                        int64_t M, int64_t K, int64_t N, uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes,
-                        void* stream);
+int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* W, int group, int zero_points, int64_t M, int64_t K, int64_t N,
+                        uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* The gated feed-forward block (see gc_gated_ffn_forward_bf16) with both weights so: Win has D inputs and 2H outputs, [Wg | Wu], Wout H
- * and O.  Up to 32 rows nothing is rounded on the way but Y. */
+ * and O.  Up to 16 rows nothing is rounded on the way but Y. */
 size_t gc_gated_ffn_int4_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O);
-int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* codes_in, const uint16_t* scale_in, const uint8_t* zero_in,
-                           int group_in, const uint8_t* codes_out, const uint16_t* scale_out, const uint8_t* zero_out, int group_out,
-                           int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace,
-                           size_t workspace_bytes, void* stream);
+int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, int group_in, int zero_points_in, const uint8_t* Wout,
+                           int group_out, int zero_points_out, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y,
+                           int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- adjacency construction (reference tests/gcn/graphcuda_impl.py:27-38) - */
 

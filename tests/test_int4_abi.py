@@ -10,20 +10,20 @@ M, K, N = 70, 200, 33
 D, H, O = 40, 24, 16
 
 
-def _linear(x=16, ldx=K, codes=16, scale=16, zero=None, group=64, m=M, k=K, n=N, y=16, ldy=N, ws=16, wsb=None):
+def _linear(x=16, ldx=K, w=16, group=64, zeros=0, m=M, k=K, n=N, y=16, ldy=N, ws=16, wsb=None):
     need = L().gc_linear_int4_workspace_bytes(M, K, N)
-    return L().gc_linear_int4_bf16(x, ldx, codes, scale, zero, group, m, k, n, y, ldy, ws, need if wsb is None else wsb, None)
+    return L().gc_linear_int4_bf16(x, ldx, w, group, zeros, m, k, n, y, ldy, ws, need if wsb is None else wsb, None)
 
 
-def _block(x=16, ldx=D, ci=16, si=16, zi=None, gi=64, co=16, so=16, zo=None, go=128, m=M, d=D, h=H, o=O, act=0, y=16, ldy=O, ws=16,
+def _block(x=16, ldx=D, wi=16, gi=64, zi=0, wo=16, go=128, zo=1, m=M, d=D, h=H, o=O, act=0, y=16, ldy=O, ws=16,
            wsb=None):
     need = L().gc_gated_ffn_int4_workspace_bytes(M, D, H, O)
-    return L().gc_gated_ffn_int4_bf16(x, ldx, ci, si, zi, gi, co, so, zo, go, m, d, h, o, act, y, ldy, ws, need if wsb is None else wsb, None)
+    return L().gc_gated_ffn_int4_bf16(x, ldx, wi, gi, zi, wo, go, zo, m, d, h, o, act, y, ldy, ws, need if wsb is None else wsb, None)
 
 
 def test_what_the_product_refuses():
-    for bad in (dict(m=-1), dict(k=-1), dict(n=-1), dict(ldx=K - 1), dict(ldy=N - 1), dict(x=None), dict(y=None), dict(codes=None),
-                dict(scale=None), dict(group=16), dict(group=256), dict(group=0), dict(codes=8), dict(scale=8), dict(zero=4), dict(ws=24)):
+    for bad in (dict(m=-1), dict(k=-1), dict(n=-1), dict(ldx=K - 1), dict(ldy=N - 1), dict(x=None), dict(y=None), dict(w=None),
+                dict(group=16), dict(group=256), dict(group=0), dict(w=8), dict(ws=24)):
         assert _linear(**bad) == -1, bad
     assert _linear(m=1 << 30) == -2 and _linear(k=1 << 27, ldx=1 << 27) == -2
     assert _linear(ws=None) == -4 and _linear(wsb=L().gc_linear_int4_workspace_bytes(M, K, N) - 1) == -4
@@ -31,8 +31,8 @@ def test_what_the_product_refuses():
 
 
 def test_what_the_block_refuses():
-    for bad in (dict(m=-1), dict(d=-1), dict(h=-1), dict(o=-1), dict(ldx=D - 1), dict(ldy=O - 1), dict(x=None), dict(y=None), dict(ci=None),
-                dict(so=None), dict(gi=1), dict(go=1), dict(co=8), dict(zi=8), dict(act=3), dict(act=-1), dict(ws=24)):
+    for bad in (dict(m=-1), dict(d=-1), dict(h=-1), dict(o=-1), dict(ldx=D - 1), dict(ldy=O - 1), dict(x=None), dict(y=None), dict(wi=None),
+                dict(wo=None), dict(gi=1), dict(go=1), dict(wi=8), dict(wo=8), dict(act=3), dict(act=-1), dict(ws=24)):
         assert _block(**bad) == -1, bad
     assert _block(m=1 << 30) == -2 and _block(h=1 << 29) == -2
     assert _block(ws=None) == -4 and _block(wsb=L().gc_gated_ffn_int4_workspace_bytes(M, D, H, O) - 1) == -4
@@ -42,7 +42,7 @@ def test_what_the_block_refuses():
 def test_queries():
     for q in (lambda m: L().gc_linear_int4_workspace_bytes(m, K, N), lambda m: L().gc_gated_ffn_int4_workspace_bytes(m, D, H, O)):
         assert q(0) == q(-1) == q(1 << 30) == 0 and q(1000) >= q(65) > 0
-    assert L().gc_linear_int4_workspace_bytes(64, K, N) < 2 * K * N + 64 * 2 * K  # weights are not unpacked for so few rows
+    assert L().gc_linear_int4_workspace_bytes(32, K, N) < 2 * K * N  # weights are not unpacked for so few rows
 
 
 @pytest.mark.parametrize("k,n,group", [(1, 1, 32), (130, 20, 32), (200, 33, 64), (128, 16, 128), (300, 70, 128), (0, 5, 32), (7, 0, 64)])
@@ -61,10 +61,13 @@ def test_layout_and_back(k, n, group, zeros):
     for kk, nn in ((0, 0), (k - 1, n - 1), (k // 2, n // 3)):  # the layout that the C interface documents
         c = kk % 128
         at = nn % 16 * 64 + (c % 32 // 8 * 4 + c // 32) * 4
-        word = int.from_bytes(bytes(w.codes[nn // 16, kk // 128, at:at + 4].tolist()), "little")
+        record = w.records[nn // 16, kk // 128]
+        word = int.from_bytes(bytes(record[at:at + 4].tolist()), "little")
         e = c % 8
         assert word >> (4 * (e // 2 + e % 2 * 4)) & 15 == int(codes[kk, nn])
-        assert w.scale[nn // 16, kk // 128, nn % 16, c // group] == scale[kk // group, nn]
+        of = nn % 16 * (128 // group) + c // group
+        assert record[1024:1024 + 32 * (128 // group)].clone().view(torch.bfloat16)[of] == scale[kk // group, nn]
+        assert not zeros or record[1024 + 32 * (128 // group) + of] == zero[kk // group, nn]
 
 
 def test_refused_codes():
@@ -121,7 +124,8 @@ def test_cpu_tensors_are_refused():
 
 def test_state_and_moves():
     w = gc.quantize_weight_int4(torch.randn(100, 40), 32, True)
-    assert set(w.state_dict()) == {"codes", "scale", "zero"}
+    assert set(w.state_dict()) == {"records"}
+    w.half(), w.float()  # of no concern to bytes
     other = gc.quantize_weight_int4(torch.randn(100, 40), 32, True)
     other.load_state_dict(w.state_dict())
     assert torch.equal(other.dequantize(), w.dequantize())
