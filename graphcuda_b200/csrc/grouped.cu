@@ -3,9 +3,10 @@
 //   forward    Y[r] = X[r] W[g]              for rows r of group g, offsets[g] <= r < offsets[g + 1]
 //   backward   dX[r] = dY[r] W[g]^T,  dW[g] = X_g^T dY_g
 //
-// Groups are as large as they are: the offsets lie on the device, and nothing here asks the host for them.  One persistent kernel;
-// every warp of it walks the groups in the same order, 32 at a time (a scan over their tiles), as far as its next tile is.  Tiles
-// begin at a group's first row, wherever that is.  A tile's rows beyond the group's end are multiplied like the others -- rows of a
+// Groups are as large as they are: the offsets lie on the device, and nothing here asks the host for them.  One persistent kernel, in
+// which one warp of a CTA walks the groups, 32 at a time (a scan over their tiles), as far as the CTA's next tile is, and hands tiles
+// to the other warps through a ring in shared memory.  (With every warp walking for itself the MMA issuer spent 3300 clocks on it
+// where neighbouring tiles lie in different groups: half of the time at K = 256.)  Tiles begin at a group's first row, wherever that is.  A tile's rows beyond the group's end are multiplied like the others -- rows of a
 // product do not mix -- and not stored: blocks of 32 rows that are the group's own leave by TMA, the one that it ends in row by
 // row.  In dW the rows are what is summed over, and none of the next group's may come in (zeros would not keep out its
 // infinities): a first launch copies what a group has beyond whole blocks of 64 rows into blocks filled up with zeros, from
@@ -15,8 +16,8 @@
 // them into parts of `part` rows, whose fp32 sums a last launch adds in their order: for parallelism where a weight has few tiles, and
 // because a chain of additions in the tensor core truncates (16,384 rows: 1e-4 relative, below the result's rounding).
 //
-// CTA = 20 warps, as in the gated block's kernel: TMA producers of A and of B, MMA issuer, TMEM allocator, 16 epilogue warps on the
-// 32 x 32 blocks of a tile in turn; two accumulators; CTAs in pairs on 256 x 256 where there are rows for it.  Waits are bounded
+// CTA = 20 warps, as in the gated block's kernel: TMA producers of A and of B, MMA issuer, the warp that deals tiles, 16 epilogue warps
+// on the 32 x 32 blocks of a tile in turn; two accumulators; CTAs in pairs on 256 x 256 where there are rows for it.  Waits are bounded
 // as there.
 //
 // Rows of no group (before the first offset, behind the last) get zeros.  Offsets that are no offsets (outside the rows, or
@@ -110,6 +111,15 @@ __device__ __forceinline__ Group before_all(const Params& p) {
   return {-1, first, first, 0, 0};
 }
 
+// A tile as one warp deals it to the others.
+struct __align__(16) Tile {
+  int row, col;        // of the product, where the CTA's half begins
+  int row_end, group;  // the group's last row, or the weight's; of the last tile, which is none, the last group's
+  int from, blocks;    // dW: first row that is summed over; k-blocks, below zero for the last
+  int over, part;      // dW: rows of the last k-block, where that is not whole; number of the part, below zero where it is the only one
+};
+constexpr int kDealt = 4;
+
 template <int MODE, int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
@@ -129,58 +139,52 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
   auto bar_empty = [&](int s) { return bars + 8 * (S + s); };
   auto bar_tfull = [&](int b) { return bars + 8 * (2 * S + b); };
   auto bar_tempty = [&](int b) { return bars + 8 * (2 * S + 2 + b); };
+  auto bar_dealt = [&](int i) { return bars + 8 * (2 * S + 4 + i); };
+  auto bar_taken = [&](int i) { return bars + 8 * (2 * S + 4 + kDealt + i); };
+  static_assert(8 * (2 * S + 4 + 2 * kDealt) <= 512, "room for the barriers");
+  __shared__ Tile dealt[kDealt];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int tiles_n = (p.n + BN - 1) / BN;
   const int weight_tiles = (p.m + TM - 1) / TM * tiles_n;  // dW
-  auto count = [&](int rows) {
-    if (MODE == kWeights) return max(1, (rows + p.part - 1) / p.part) * weight_tiles;
-    return (rows + TM - 1) / TM * tiles_n;
-  };
   // This CTA's (or pair's) items are every units-th.  Of a part: groups of 8 rows of tiles, so that tiles that run at one time
   // are a square of the product.
-  struct Tile {
-    Group in;
-    int item, t;       // t: which of this CTA's
-    int m, n;          // of the product
-    int from, blocks;  // dW: first row that is summed over; k-blocks
-    int over;          // dW: rows of the last k-block, where that is not whole
-    int part, parts;
-  };
-  constexpr int kSquare = 8;
-  auto find = [&](Tile& x) {
-    if (!seek(p, x.in, x.item, count)) return false;
-    int i = x.item - x.in.first;
-    const int tiles_m = MODE == kWeights ? (p.m + TM - 1) / TM : (x.in.end - x.in.start + TM - 1) / TM;
+  Group in = before_all(p);
+  int item = unit;
+  auto find = [&](Tile& x) {  // by a whole warp
+    constexpr int kSquare = 8;
+    const bool there = seek(p, in, item, [&](int rows) {
+      if (MODE == kWeights) return max(1, (rows + p.part - 1) / p.part) * weight_tiles;
+      return (rows + TM - 1) / TM * tiles_n;
+    });
+    x.group = in.g;
+    x.row_end = MODE == kWeights && there ? p.m : in.end;
+    x.blocks = -1;
+    if (!there) return false;
+    int i = item - in.first;
+    const int tiles_m = MODE == kWeights ? (p.m + TM - 1) / TM : (in.end - in.start + TM - 1) / TM;
     if (MODE == kWeights) {
-      x.part = i / weight_tiles;
-      x.parts = x.in.count / weight_tiles;
-      i -= x.part * weight_tiles;
-      x.from = x.in.start + x.part * p.part;
-      const int rows = min(p.part, x.in.end - x.from);
+      const int part = i / weight_tiles;
+      i -= part * weight_tiles;
+      x.from = in.start + part * p.part;
+      const int rows = min(p.part, in.end - x.from);
       x.blocks = (rows + KE - 1) / KE;
       x.over = rows % KE;
+      x.part = in.count > weight_tiles ? in.first / weight_tiles + part : -1;
     } else {
       x.blocks = (p.K + KE - 1) / KE;
     }
     const int g = i / (kSquare * tiles_n), r = i - g * (kSquare * tiles_n), high = min(kSquare, tiles_m - g * kSquare);
-    x.n = r / high;
-    x.m = g * kSquare + r - x.n * high;
+    const int n = r / high;
+    x.row = (MODE == kWeights ? 0 : in.start) + (g * kSquare + r - n * high) * TM + int(rank) * BM;
+    x.col = n * BN;
+    item += units;
     return true;
   };
-  auto first_tile = [&](Tile& x) {
-    x.in = before_all(p);
-    x.item = unit;
-    x.t = 0;
-    return find(x);
-  };
-  auto next = [&](Tile& x) {
-    x.item += units;
-    ++x.t;
-    return find(x);
-  };
+  Tile ahead;
+  if (warp == 2) find(ahead);  // while the barriers are made and TMEM is allocated
 
   if (threadIdx.x == 0) {
     abort_s = 0;
@@ -192,6 +196,10 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       mbar_init(bar_tfull(b), 1);
       mbar_init(bar_tempty(b), kEpiWarps * (PAIR ? 2 : 1));
     }
+    for (int i = 0; i < kDealt; ++i) {
+      mbar_init(bar_dealt(i), 1);
+      mbar_init(bar_taken(i), 2 + kEpiWarps + (rank == 0));
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();
   }
@@ -199,14 +207,37 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     __syncthreads();
     cluster_sync_all();  // both CTAs' barriers exist before either is signalled
   }
-  if (warp == 2) tmem_alloc<PAIR>(smem_u32(&tmem_base_s), C_::kTmemCols);
+  if (warp == 1) tmem_alloc<PAIR>(smem_u32(&tmem_base_s), C_::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
   volatile int* abort_p = &abort_s;
+  // The t-th tile, for one lane or a whole warp; false when there is none.
+  auto take = [&](int t, Tile& x, bool all) {
+    const int i = t % kDealt;
+    bool ok = wait(bar_dealt(i), (t / kDealt) & 1u, abort_p);
+    if (all) ok = __all_sync(kAll, ok);
+    if (!ok) return false;
+    x = dealt[i];
+    if (all) __syncwarp();
+    if (!all || lane == 0) mbar_arrive(bar_taken(i));
+    return x.blocks >= 0;
+  };
 
-  if (warp == 0 || warp == 3) {
+  if (warp == 2) {
+    // ------------------------------------------------------------ deals the tiles
+    for (int t = 0;; ++t) {
+      const int i = t % kDealt;
+      if (!__all_sync(kAll, wait(bar_taken(i), ((t / kDealt) & 1u) ^ 1u, abort_p))) break;
+      if (lane == 0) {
+        dealt[i] = ahead;
+        mbar_arrive(bar_dealt(i));
+      }
+      if (ahead.blocks < 0) break;
+      find(ahead);
+    }
+  } else if ((warp == 0 || warp == 3) && lane == 0) {
     // ------------------------------------------------------------ TMA producers: A, B
     const bool is_a = warp == 0;
     auto expect = [&](uint32_t bar, uint32_t bytes) {  // a pair's copies are all counted at the leader
@@ -223,76 +254,68 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     };
     uint32_t s = 0, phase = 0, issued = 0;
     Tile x;
-    for (bool more = first_tile(x); more; more = next(x)) {
-      bool ok = true;
-      if (lane == 0) {
-        const int m0 = (MODE == kWeights ? 0 : x.in.start) + x.m * TM + int(rank) * BM, n0 = x.n * BN + int(rank) * BNC;
-        for (int kb = 0; kb < x.blocks; ++kb) {
-          if (!wait(bar_empty(s), phase ^ 1u, abort_p)) { ok = false; break; }
-          const uint32_t bar = bar_full(s);
-          const bool tail = MODE == kWeights && x.over && kb == x.blocks - 1;
-          const int row = tail ? x.in.g * KE : x.from + kb * KE;  // dW
-          if (is_a) {
-            expect(bar, p.a_bytes);
-            if (A_MN) {
+    bool ok = true;
+    for (int t = 0; ok && take(t, x, false); ++t) {
+      const int n0 = x.col + int(rank) * BNC;
+      for (int kb = 0; kb < x.blocks; ++kb) {
+        if (!wait(bar_empty(s), phase ^ 1u, abort_p)) { ok = false; break; }
+        const uint32_t bar = bar_full(s);
+        const bool tail = MODE == kWeights && x.over && kb == x.blocks - 1;
+        const int row = tail ? x.group * KE : x.from + kb * KE;  // dW
+        if (is_a) {
+          expect(bar, p.a_bytes);
+          if (A_MN) {
 #pragma unroll
-              for (int c = 0; c < BM / 64; ++c) load(sA(s) + c * (64 * 128), tail ? &maps.a_tail : &maps.a, m0 + c * 64, row, bar);
-            } else {
-              load(sA(s), &maps.a, kb * KE, m0, bar);
-            }
+            for (int c = 0; c < BM / 64; ++c) load(sA(s) + c * (64 * 128), tail ? &maps.a_tail : &maps.a, x.row + c * 64, row, bar);
           } else {
-            expect(bar, C_::kBBytes);
-            if (MODE == kBack) {
-              load_weight(sB(s), kb * KE, n0, x.in.g, bar);
-            } else {
+            load(sA(s), &maps.a, kb * KE, x.row, bar);
+          }
+        } else {
+          expect(bar, C_::kBBytes);
+          if (MODE == kBack) {
+            load_weight(sB(s), kb * KE, n0, x.group, bar);
+          } else {
 #pragma unroll
-              for (int c = 0; c < BNC / 64; ++c) {
-                if (MODE == kForward) load_weight(sB(s) + c * (64 * 128), n0 + c * 64, kb * KE, x.in.g, bar);
-                else load(sB(s) + c * (64 * 128), tail ? &maps.b_tail : &maps.b, n0 + c * 64, row, bar);
-              }
+            for (int c = 0; c < BNC / 64; ++c) {
+              if (MODE == kForward) load_weight(sB(s) + c * (64 * 128), n0 + c * 64, kb * KE, x.group, bar);
+              else load(sB(s) + c * (64 * 128), tail ? &maps.b_tail : &maps.b, n0 + c * 64, row, bar);
             }
           }
-          ++issued;
-          if (++s == uint32_t(S)) s = 0, phase ^= 1u;
         }
+        ++issued;
+        if (++s == uint32_t(S)) s = 0, phase ^= 1u;
       }
-      if (!__shfl_sync(kAll, int(ok), 0)) break;
     }
-    if (lane == 0 && (!PAIR || rank == 0))  // every copy issued must have landed before the CTA may exit
+    if (!PAIR || rank == 0)  // every copy issued must have landed before the CTA may exit
       for (uint32_t j = 0; j < issued && j < uint32_t(S); ++j) {
         if (s == 0) phase ^= 1u;
         s = s == 0 ? S - 1 : s - 1;
         drain(bar_full(s), phase);
       }
-  } else if (warp == 1) {
+  } else if (warp == 1 && lane == 0 && rank == 0) {
     // ------------------------------------------------------------ MMA issuer
-    if (rank == 0) {
-      constexpr uint32_t idesc = make_idesc(TM, BN, A_MN, B_MN, false);
-      constexpr uint32_t kAStep = A_MN ? 16 * 128 : 32, kBStep = B_MN ? 16 * 128 : 32;  // bytes per MMA
-      const uint64_t da0 = operand_desc(sA(0), A_MN), db0 = operand_desc(sB(0), B_MN);
-      uint32_t s = 0, phase = 0;
-      Tile x;
-      for (bool more = first_tile(x); more; more = next(x)) {
-        bool ok = true;
-        if (lane == 0) {
-          const int b = x.t & 1;
-          ok = wait(bar_tempty(b), ((x.t >> 1) & 1u) ^ 1u, abort_p);
-          tc_fence_after();
-          const uint32_t d_tmem = tmem_base + uint32_t(b * BN);
-          for (int kb = 0; ok && kb < x.blocks; ++kb) {
-            if (!wait(bar_full(s), phase, abort_p)) { ok = false; break; }
-            tc_fence_after();
-            const uint64_t da = da0 + s * (C_::kStageBytes >> 4), db = db0 + s * (C_::kStageBytes >> 4);
+    constexpr uint32_t idesc = make_idesc(TM, BN, A_MN, B_MN, false);
+    constexpr uint32_t kAStep = A_MN ? 16 * 128 : 32, kBStep = B_MN ? 16 * 128 : 32;  // bytes per MMA
+    const uint64_t da0 = operand_desc(sA(0), A_MN), db0 = operand_desc(sB(0), B_MN);
+    uint32_t s = 0, phase = 0;
+    Tile x;
+    bool ok = true;
+    for (int t = 0; ok && take(t, x, false); ++t) {
+      const int b = t & 1;
+      if (!wait(bar_tempty(b), ((t >> 1) & 1u) ^ 1u, abort_p)) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + uint32_t(b * BN);
+      for (int kb = 0; kb < x.blocks; ++kb) {
+        if (!wait(bar_full(s), phase, abort_p)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t da = da0 + s * (C_::kStageBytes >> 4), db = db0 + s * (C_::kStageBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma<PAIR, false>(d_tmem, da + ((k * kAStep) >> 4), db + ((k * kBStep) >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
-            umma_commit<PAIR>(bar_empty(s));  // frees the stage once these MMAs have read it
-            if (++s == uint32_t(S)) s = 0, phase ^= 1u;
-          }
-          if (ok) umma_commit<PAIR>(bar_tfull(b));
-        }
-        if (!__shfl_sync(kAll, int(ok), 0)) break;
+        for (int k = 0; k < 4; ++k)
+          umma<PAIR, false>(d_tmem, da + ((k * kAStep) >> 4), db + ((k * kBStep) >> 4), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+        umma_commit<PAIR>(bar_empty(s));  // frees the stage once these MMAs have read it
+        if (++s == uint32_t(S)) s = 0, phase ^= 1u;
       }
+      if (ok) umma_commit<PAIR>(bar_tfull(b));
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
@@ -310,10 +333,10 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       return buf;
     };
     Tile x;
-    bool more = first_tile(x);
-    for (; more; more = next(x)) {
-      const int b = x.t & 1, n0 = x.n * BN;
-      if (!__all_sync(kAll, wait(bar_tfull(b), (x.t >> 1) & 1u, abort_p))) break;
+    x.blocks = 0;
+    for (int t = 0; take(t, x, true); ++t) {
+      const int b = t & 1;
+      if (!__all_sync(kAll, wait(bar_tfull(b), (t >> 1) & 1u, abort_p))) break;
       tc_fence_after();
       bool held = true;
       auto release = [&]() {  // the accumulator goes back as soon as the warp's last chunk is in registers
@@ -325,11 +348,10 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         }
         held = false;
       };
-      const int row0 = (MODE == kWeights ? 0 : x.in.start) + x.m * TM + int(rank) * BM + q * 32;  // of the product
-      const int rows = min(32, (MODE == kWeights ? p.m : x.in.end) - row0);
+      const int row0 = x.row + q * 32, rows = min(32, x.row_end - row0);  // of the product
       const uint32_t taddr = tmem_base + (uint32_t(q * 32) << 16) + uint32_t(b * BN);
       for (int c = grp; c < BN / 32 && rows > 0; c += kEpiGroups) {
-        const int col = n0 + c * 32;
+        const int col = x.col + c * 32;
         if (col >= p.n) break;
         uint32_t acc[32];
         tmem_ld32(taddr + uint32_t(c * 32), acc);
@@ -339,9 +361,8 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[i] = 0;
         }
-        if (MODE == kWeights && x.parts > 1) {
-          // fp32 parts, 16 columns to a tile; a part's number is that of its first item among all parts
-          const int part = x.in.first / weight_tiles + x.part;
+        if (MODE == kWeights && x.part >= 0) {
+          // fp32 parts, 16 columns to a tile
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const uint32_t bo = acquire();
@@ -353,7 +374,7 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (col + half * 16 < pitch) tma_store_3d(&maps.out_parts, tiles + bo, col + half * 16, row0, part);
+              if (col + half * 16 < pitch) tma_store_3d(&maps.out_parts, tiles + bo, col + half * 16, row0, x.part);
               store_commit();
             }
           }
@@ -370,14 +391,14 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (MODE == kWeights) tma_store_3d(&maps.out, tiles + bo, col, row0, x.in.g);
+              if (MODE == kWeights) tma_store_3d(&maps.out, tiles + bo, col, row0, x.group);
               else tma_store_2d(&maps.out, tiles + bo, col, row0);
               store_commit();
             }
           } else {
             // rows of an odd pitch, or the last of a group: a row at a time, a column per lane
             __syncwarp();
-            bf16* to = p.C + (MODE == kWeights ? int64_t(x.in.g) * p.m + row0 : int64_t(row0)) * p.ldc + col + lane;
+            bf16* to = p.C + (MODE == kWeights ? int64_t(x.group) * p.m + row0 : int64_t(row0)) * p.ldc + col + lane;
             if (col + lane < p.n)
               for (int r = 0; r < rows; ++r) to[r * p.ldc] = __ushort_as_bfloat16(load_column(tiles + bo, r, lane));
             if (lane == 0) store_commit();  // nothing: the tiles' turns are counted in groups of stores
@@ -387,12 +408,12 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       }
       if (held) release();
     }
-    if (MODE != kWeights && !more) {  // rows of no group
-      const int head = clamped(p, 0), spare = p.rows - x.in.end;
+    if (MODE != kWeights && x.blocks < 0) {  // all tiles are done; rows of no group
+      const int head = clamped(p, 0), spare = p.rows - x.row_end;
       const int64_t total = int64_t(head + spare) * p.n, step = int64_t(gridDim.x) * kEpiWarps * 32;
       for (int64_t i = (int64_t(blockIdx.x) * kEpiWarps + warp - 4) * 32 + lane; i < total; i += step) {
         const int64_t r = i / p.n;
-        p.C[(r < head ? r : x.in.end + r - head) * p.ldc + (i - r * p.n)] = __ushort_as_bfloat16(0);
+        p.C[(r < head ? r : x.row_end + r - head) * p.ldc + (i - r * p.n)] = __ushort_as_bfloat16(0);
       }
     }
     if (lane == 0) store_wait_all();  // shared memory is read until then
@@ -403,7 +424,7 @@ grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
   __syncthreads();
   if (PAIR) cluster_sync_all();  // the peer's MMAs read this CTA's shared memory and write its TMEM until here
   tc_fence_after();
-  if (warp == 2) tmem_dealloc<PAIR>(tmem_base, C_::kTmemCols);
+  if (warp == 1) tmem_dealloc<PAIR>(tmem_base, C_::kTmemCols);
   if (threadIdx.x == 0 && abort_s) atomicExch(p.word, 1);
 }
 
@@ -483,7 +504,7 @@ grouped_sum_kernel(const __grid_constant__ Params p) {
   const float* from = p.parts + b.parts_before * size;
   for (int64_t i = int64_t(blockIdx.y) * 256 + threadIdx.x; i < quads; i += int64_t(gridDim.y) * 256) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int z = 0; z < parts; ++z) {
       const float4 v = __ldcs(reinterpret_cast<const float4*>(from + z * size) + i);
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
@@ -519,13 +540,15 @@ Shape shape_of_weights(int64_t m, int64_t n) {
   if (m > 128 && n > 128) return {256, true};
   return {n > 64 ? 128 : 64, false};
 }
-// Rows of a part of dW: two parts' tiles per SM (or pair) if all groups were one, but at least 4 k-blocks, and at most kChain rows,
-// beyond which truncation would show.
+// Rows of a part of dW.  Few tiles: so many that the parts' tiles, one more per group than the rows alone would make, fill the GPU once
+// (8 groups of 169,343 rows, 256 x 256: 36 us; with half as many rows in a part, whose last round is nearly empty, 44 and twice the
+// sums).  Else half of an SM's share of the work, so that large groups spread.  At least 4 k-blocks, and at most kChain rows, beyond which
+// truncation would show.
 constexpr int64_t kChain = 16384;
-int64_t part_rows(int64_t M, int64_t m, int64_t n, const Shape& s) {
+int64_t part_rows(int64_t M, int64_t m, int64_t n, int64_t G, const Shape& s) {
   const int64_t tiles = gc::ceil_div(m, s.pair ? 256 : BM) * gc::ceil_div(n, s.bn), units = s.pair ? gc::kNumSMs / 2 : gc::kNumSMs;
-  const int64_t rows = gc::ceil_div(M * tiles, 2 * units);
-  return std::min(kChain, std::max<int64_t>(4 * KE, gc::ceil_div(rows, KE) * KE));
+  const int64_t share = units > 4 * G * tiles ? units - G * tiles : 2 * units;
+  return std::min(kChain, std::max<int64_t>(4 * KE, gc::ceil_div(gc::ceil_div(M * tiles, share), KE) * KE));
 }
 int64_t parts_most(int64_t M, int64_t G, int64_t part) { return M / part + G; }  // that exist, at most
 
@@ -585,7 +608,7 @@ int rows_product(const Matrix& A, const Matrix& w, const int32_t* offsets, int64
 }
 
 size_t weights_workspace(int64_t M, int64_t K, int64_t N, int64_t G) {
-  const int64_t part = part_rows(M, K, N, shape_of_weights(K, N));
+  const int64_t part = part_rows(M, K, N, G, shape_of_weights(K, N));
   const size_t parts = M > part ? align256(size_t(parts_most(M, G, part)) * size_t(K) * size_t((N + 3) / 4 * 4) * 4) : 0;
   return align256(size_t(G) * KE * up8(K) * 2) + align256(size_t(G) * KE * up8(N) * 2) + parts;
 }
@@ -597,7 +620,7 @@ int weights_product(const Matrix& x, const Matrix& dy, const int32_t* offsets, i
   p.offsets = offsets;
   p.groups = int(G); p.rows = int(M);
   p.m = int(K); p.n = int(N);
-  p.part = int(part_rows(M, K, N, s));
+  p.part = int(part_rows(M, K, N, G, s));
   p.C = C; p.ldc = N;
   p.tma_store = N % 8 == 0 && gc::aligned16(C);
   p.a_bytes = BM * 128;
