@@ -83,10 +83,11 @@ SIGNATURES = {
     "gc_gated_ffn_int4_bf16": (_int, [_void, _i64, _void, _int, _int, _void, _int, _int, _i64, _i64, _i64, _i64, _int, _void, _i64, _void,
                                       _size, _void]),
     "gc_distill_workspace_bytes": (_size, [_i64, _i64]),
+    "gc_distill_one_pass": (_int, [_void, _int, _i64, _i64, _i64, _i64, _i64]),
     "gc_distill_forward": (_int, [_void, _int, _i64, _void, _int, _i64, _void, _int, _i64, _void, _i64, _i64, _i64, C.c_float,
-                                  C.c_float, _f32p, _f32p, _void, _size, _void]),
+                                  C.c_float, _f32p, _f32p, _void, _i64, _i64, _void, _size, _void]),
     "gc_distill_backward": (_int, [_void, _int, _i64, _void, _int, _i64, _void, _int, _i64, _f32p, _i64, _i64, _i64, C.c_float,
-                                   C.c_float, _f32p, _void, _i64, _i64, _void]),
+                                   C.c_float, _f32p, _void, _i64, _i64, _int, _void]),
     "gc_logsoftmax_nll_backward_pad_f32": (_int, [_f32p, _i64, _i64p, _void, _i64, _i64, C.c_float, _f32p, _f32p,
                                                   _i64, _void, _void]),
     "gc_argmax_accuracy_masks_f32": (_int, [_f32p, _i64, _i64, _i64, _i64p, _void, _int, _i64p, _i64p, _void]),

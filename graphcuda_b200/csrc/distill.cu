@@ -9,11 +9,17 @@
 // come from one exponential each, and nothing but dZ is written.  Sums and statistics are fp32.  With u = (z - max) log2(e) / T the
 // subtraction comes before the product, so that a row filled with the type's lowest value does not overflow.
 //
-// G threads take a row: 8 up to 256 classes (a row is few vectors, and what a row costs beside them is shared by fewer), a warp up to
+// With a gradient to be asked for, rows of some thousands of classes are read once in all (one_pass): a CTA streams rows through a ring of
+// segments in shared memory; one half of its threads goes over a row's segments as they arrive for its statistics, the other
+// over the same segments again for dZ, giving them back to the copies of the next row.  That is dZ for g = 1, which is what a loss that is differentiated by
+// itself has; the backward call looks at g and, where it is another, computes dZ from the logits as it does for other rows.
+//
+// Otherwise G threads take a row: 8 up to 256 classes (a row is few vectors, and what a row costs beside them is shared by fewer), a warp up to
 // 4096, a CTA of 512 above; with fewer rows than SMs a CTA takes a part of a row (kParts) and another launch puts the parts
 // together.  Rows may start anywhere: what lies before the first and behind the last 16-byte vector is read by itself.
 #include "common.cuh"
 #include "ffn_internal.cuh"
+#include "tiles.cuh"
 
 #include <cuda_bf16.h>
 
@@ -321,13 +327,299 @@ __device__ __forceinline__ T rounded(float v) {
   else return __float2bfloat16_rn(v);
 }
 
+// g (q - p) of a logit.  Where the maximum times a is a number the exponent is one multiply-add, (z a - zm a - zl), as in the vectors.
+__device__ __forceinline__ bool product_is_finite(float m, float a) { return fabsf(m * a) < 1e38f; }
+struct Gradient {
+  float zm, zl, a, g;
+  __device__ __forceinline__ float operator()(float z, float p) const {
+    const float e = product_is_finite(zm, a) ? fmaf(z, a, -zm * a - zl) : (z - zm) * a - zl;
+    return g * (exp2_approx(e) - p);
+  }
+};
+// The probabilities of a class's entries: an index may stand in the list more than once.  kp: a multiple of 4.
+__device__ __forceinline__ float sum_at(int c, const int* cls, const float* prob, int kp) {
+  float sum = 0.f;
+  for (int i = 0; i < kp; i += 4) {
+    const int4 ci = *reinterpret_cast<const int4*>(cls + i);
+    const float4 pi = *reinterpret_cast<const float4*>(prob + i);
+    sum += (ci.x == c ? pi.x : 0.f) + (ci.y == c ? pi.y : 0.f) + (ci.z == c ? pi.z : 0.f) + (ci.w == c ? pi.w : 0.f);
+  }
+  return sum;
+}
+
+// ------------------------------------------------------------------ both in one pass
+constexpr int64_t kOnePassFrom = 8192;  // bytes of a row
+constexpr int kLong = 480, kShort = 128;  // threads for long and short rows
+template <int THREADS>
+struct Ring {
+  static constexpr int kBytes = THREADS * 32;  // of a segment: two vectors per thread
+  static constexpr int kVectors = THREADS * 2;
+  static constexpr int kSegments = THREADS == kLong ? 14 : 13;
+  static constexpr int kMostBytes = (kSegments - 1) * kBytes;  // of a row
+};
+// Entries' classes, logits (later probabilities) and the student's logits at them, of a row.
+constexpr int kListWords = 3;
+constexpr int kOnePassList = 256;  // entries of a list
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+template <int BARRIER, int THREADS>
+__device__ __forceinline__ void sync_threads() { asm volatile("bar.sync %0, %1;" ::"n"(BARRIER), "n"(THREADS) : "memory"); }
+
+// THREADS that make a row's statistics, as many that make the gradient of the row before, and a warp whose first lane fetches.
+// Persistent over rows.  (With the same threads doing one after the other the exponentials of a row waited for its sums: 285 us for 4096 x
+// 65,536 in bf16.)
+template <class T, int THREADS>
+__global__ void __launch_bounds__(2 * THREADS + 32)
+distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ stats, float* __restrict__ partials, float g,
+                        T* __restrict__ dz, int64_t lddz, int pad, int* __restrict__ word) {
+  using namespace gc::tc;
+  constexpr int kBytes = Ring<THREADS>::kBytes, kVectors = Ring<THREADS>::kVectors, kWarps = THREADS / 32, N = Vec<T>::N;
+  constexpr int kSegments = Ring<THREADS>::kSegments;
+  extern __shared__ __align__(128) uint8_t smem[];  // the ring; the lists of two rows: classes, logits (then probabilities), the student's logits
+  __shared__ __align__(8) uint64_t bars[2 * kSegments + 4];
+  __shared__ float sh[2][kWarps][4];
+  __shared__ float info[2][4];  // of two rows: the student's maximum and logarithm of its sum; whether the row counts
+  __shared__ int abort_s;
+  const uint32_t ring = smem_u32(smem);
+  auto full = [&](int i) { return smem_u32(&bars[i]); };
+  auto empty = [&](int i) { return smem_u32(&bars[kSegments + i]); };
+  auto ready = [&](int i) { return smem_u32(&bars[2 * kSegments + i]); };
+  auto taken = [&](int i) { return smem_u32(&bars[2 * kSegments + 2 + i]); };
+  const int kp = (p.k + 3) / 4 * 4;
+  auto classes = [&](int i) { return reinterpret_cast<int*>(smem + kSegments * kBytes) + i * kListWords * kp; };
+  auto probs = [&](int i) { return reinterpret_cast<float*>(classes(i) + kp); };
+  auto at_entries = [&](int i) { return probs(i) + kp; };
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    for (int i = 0; i < kSegments; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), kWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(ready(i), 1);
+      mbar_init(taken(i), kWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();
+  }
+  __syncthreads();
+  volatile int* abort_p = &abort_s;
+  const int rank = threadIdx.x % THREADS, lane = threadIdx.x % 32;
+  int slot = 0, rows = 0;  // rows: of those that are chosen
+  uint32_t phase = 0;
+  auto advance = [&]() {
+    if (++slot == kSegments) slot = 0, phase ^= 1u;
+  };
+  bool ok = true;
+
+  if (threadIdx.x >= 2 * THREADS) {
+    // ------------------------------------------------------------ fetches
+    if (lane == 0) {
+      uint32_t issued = 0;
+      for (int64_t r = blockIdx.x; ok && r < p.M; r += gridDim.x) {
+        if (p.mask && !p.mask[r]) continue;
+        const T* z = static_cast<const T*>(p.z) + r * p.ldz;
+        const int head = before_vectors(z, p.C), vectors = (p.C - head) / N;
+        for (int v = 0; v < vectors; v += kVectors) {
+          if (!gc::tiles::wait(empty(slot), phase ^ 1u, abort_p)) { ok = false; break; }
+          const uint32_t bytes = min(kVectors, vectors - v) * 16;
+          mbar_expect_tx(full(slot), bytes);
+          bulk_load(ring + slot * kBytes, z + head + int64_t(v) * N, bytes, full(slot));
+          advance();
+          ++issued;
+        }
+      }
+      for (uint32_t j = 0; j < issued && j < uint32_t(kSegments); ++j) {  // what was issued lands before the CTA exits
+        if (slot == 0) phase ^= 1u;
+        slot = slot == 0 ? kSegments - 1 : slot - 1;
+        gc::tiles::drain(full(slot), phase);
+      }
+    }
+  } else if (threadIdx.x < THREADS) {
+    // ------------------------------------------------------------ statistics
+    const int warp = rank / 32;
+    float loss = 0.f;
+    int turn = 0;
+    auto reduce = [&](float (&v)[4], auto f) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = f(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
+      turn ^= 1;  // the other place's readers have come past a barrier since
+      if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sh[turn][warp][i] = v[i];
+      sync_threads<1, THREADS>();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = sh[turn][0][i];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = f(v[i], sh[turn][w][i]);
+    };
+    for (int64_t r = blockIdx.x; r < p.M; r += gridDim.x) {
+      if (p.mask && !p.mask[r]) {
+        if (rank == 0) stats[r] = {0.f, 0.f, 0.f, INFINITY};
+        continue;
+      }
+      const T* z = static_cast<const T*>(p.z) + r * p.ldz;
+      const int head = before_vectors(z, p.C), vectors = (p.C - head) / N, tail = head + vectors * N;
+      const int buf = rows & 1;
+      int* cls = classes(buf);
+      float *prob = probs(buf), *at_entry = at_entries(buf);
+      if (ok) ok = gc::tiles::wait(taken(buf), ((rows >> 1) & 1u) ^ 1u, abort_p);
+      // the list, while the row arrives
+      Running x;
+      float tm = -INFINITY;
+      bool any = false;
+      for (int j = rank; j < kp; j += THREADS) {
+        Entry e{0.f, -1};
+        if (j < p.k) e = entry(p, r, j);
+        cls[j] = e.c;
+        prob[j] = e.t;
+        if (e.c >= 0) {
+          at_entry[j] = as_float(z[e.c]);
+          tm = fmaxf(tm, e.t), any = true;
+        }
+      }
+      const float ends[2] = {rank < head ? as_float(z[rank]) : -INFINITY, rank < p.C - tail ? as_float(z[tail + rank]) : -INFINITY};
+      for (int v = 0; v < vectors; v += kVectors) {
+        if (ok) ok = gc::tiles::wait(full(slot), phase, abort_p);
+        const uint4* seg = reinterpret_cast<const uint4*>(smem + slot * kBytes);
+        uint4 w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) w[u] = v + rank + u * THREADS < vectors ? seg[rank + u * THREADS] : nothing<T>();
+        x.raise(fmaxf(vec_max<T>(w[0]), vec_max<T>(w[1])), p.a);
+        const F2 scale = both(p.a);
+        F2 sum = both(0.f);
+        if (product_is_finite(x.base(), p.a)) {
+          const F2 base = both(-x.base() * p.a);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            F2 f[Vec<T>::P];
+            unpack<T>(w[u], f);
+#pragma unroll
+            for (int e = 0; e < Vec<T>::P; ++e) sum = sum + each(fma2(f[e], scale, base), [](float t) { return exp2_approx(t); });
+          }
+        } else {
+          const F2 base = both(-x.base());
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            F2 f[Vec<T>::P];
+            unpack<T>(w[u], f);
+#pragma unroll
+            for (int e = 0; e < Vec<T>::P; ++e) sum = sum + each((f[e] + base) * scale, [](float t) { return exp2_approx(t); });
+          }
+        }
+        float a, b;
+        sum.get(a, b);
+        x.s += a + b;
+        advance();
+      }
+      x.raise(fmaxf(ends[0], ends[1]), p.a);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x.s += exp2_approx((ends[i] - x.base()) * p.a);
+      float top[4] = {x.m, tm, any ? 1.f : 0.f, 0.f};
+      reduce(top, [](float a, float b) { return fmaxf(a, b); });
+      const bool counts = top[2] > 0.f;
+      const float zm = top[0];
+      tm = top[1];
+      float sums[4] = {x.m == -INFINITY ? x.s : x.s * exp2_approx((x.m - zm) * p.a), 0.f, 0.f, 0.f};
+      for (int j = rank; counts && j < p.k; j += THREADS) {
+        if (cls[j] < 0) continue;
+        const float w = exp2_approx((prob[j] - tm) * p.a);
+        sums[1] += w;
+        if (!(w == 0.f)) sums[2] += w * (((prob[j] - tm) - (at_entry[j] - zm)) * p.a);
+      }
+      reduce(sums, [](float a, float b) { return a + b; });
+      const float zl = log2_approx(sums[0]), tl = log2_approx(sums[1]);
+      for (int j = rank; counts && j < p.k; j += THREADS) prob[j] = exp2_approx((prob[j] - tm) * p.a - tl);
+      if (rank == 0) {
+        stats[r] = counts ? Stats{zm, zl, tm, tl} : Stats{0.f, 0.f, 0.f, INFINITY};
+        if (counts) loss += kLn2 * (sums[2] / sums[1] - tl + zl);
+        info[buf][0] = zm, info[buf][1] = zl, info[buf][2] = counts ? 1.f : 0.f;
+      }
+      sync_threads<1, THREADS>();  // all of the list is written
+      if (rank == 0) mbar_arrive(ready(buf));
+      ++rows;
+    }
+    if (rank == 0) partials[blockIdx.x] = loss;
+  } else {
+    // ------------------------------------------------------------ gradient
+    for (int64_t r = blockIdx.x; r < p.M; r += gridDim.x) {
+      const T* z = static_cast<const T*>(p.z) + r * p.ldz;
+      T* d = dz + r * lddz;
+      const int head = before_vectors(z, p.C), vectors = (p.C - head) / N, tail = head + vectors * N;
+      uint4* to = reinterpret_cast<uint4*>(d + head);
+      if (rank < pad) d[p.C + rank] = rounded<T>(0.f);
+      const bool chosen = !p.mask || p.mask[r];
+      const int buf = rows & 1;
+      if (chosen && ok) ok = gc::tiles::wait(ready(buf), (rows >> 1) & 1u, abort_p);
+      const float zm = info[buf][0], zl = info[buf][1];
+      const bool counts = chosen && info[buf][2] > 0.f;
+      if (!counts) {
+        if (rank < head) d[rank] = rounded<T>(0.f);
+        if (rank < p.C - tail) d[tail + rank] = rounded<T>(0.f);
+        for (int i = rank; i < vectors; i += THREADS) to[i] = make_uint4(0, 0, 0, 0);
+        if (!chosen) continue;
+      }
+      const bool plain = product_is_finite(zm, p.a);
+      const F2 a = both(p.a), gg = both(g), c = both(-zm * p.a - zl), m = both(-zm), l = both(-zl);
+      for (int v = 0; v < vectors; v += kVectors) {
+        if (ok) ok = gc::tiles::wait(full(slot), phase, abort_p);
+        const uint4* seg = reinterpret_cast<const uint4*>(smem + slot * kBytes);
+        uint4 w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) w[u] = seg[rank + u * THREADS];  // (in a last segment's rest: what a row before left)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(slot));
+        advance();
+        if (!counts) continue;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = v + rank + u * THREADS;
+          F2 f[Vec<T>::P];
+          unpack<T>(w[u], f);
+          if (plain) {
+#pragma unroll
+            for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e], a, c), [](float t) { return exp2_approx(t); }) * gg;
+          } else {
+#pragma unroll
+            for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e] + m, a, l), [](float t) { return exp2_approx(t); }) * gg;
+          }
+          if (i < vectors) to[i] = pack<T>(f);
+        }
+      }
+      if (counts) {
+        const Gradient one{zm, zl, p.a, g};
+        if (rank < head) d[rank] = rounded<T>(one(as_float(z[rank]), 0.f));
+        if (rank < p.C - tail) d[tail + rank] = rounded<T>(one(as_float(z[tail + rank]), 0.f));
+        sync_threads<2, THREADS>();  // the columns that the entries write again
+        const int* cls = classes(buf);
+        const float* at_entry = at_entries(buf);
+        for (int j = rank; j < p.k; j += THREADS)
+          if (cls[j] >= 0) d[cls[j]] = rounded<T>(one(at_entry[j], sum_at(cls[j], cls, probs(buf), kp)));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(taken(buf));
+      ++rows;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && abort_s) atomicExch(word, 1);
+}
+
 // G threads per row, or per part of one (G = kWide).  Rows are taken from the last to the first: the forward pass, which has mostly
 // just run, left the last ones in the L2.  `pad`: columns of zeros behind a row of dZ.
 template <class T, int G>
 __global__ void __launch_bounds__(G > 32 ? G : 256)
 distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restrict__ stats, const float* __restrict__ grad, float factor,
-                        T* __restrict__ dz, int64_t lddz, int pad) {
+                        T* __restrict__ dz, int64_t lddz, int pad, bool has_one) {
   constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G, U = G == 8 ? 2 : 4;
+  if (has_one && __ldg(grad) == 1.f) return;  // dZ holds that gradient
   extern __shared__ __align__(16) uint8_t lists[];  // of each of the CTA's rows: the entries' classes, then their probabilities
   const int rank = threadIdx.x % G, kp = (p.k + 3) / 4 * 4;
   int* cls = reinterpret_cast<int*>(lists) + (threadIdx.x / G) * 2 * kp;
@@ -354,15 +646,16 @@ distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restri
         cls[j] = e.c;
         prob[j] = e.c < 0 ? 0.f : exp2_approx((e.t - st.tm) * p.a - st.tl);
       }
-    auto one = [&](float v) { return g * exp2_approx((v - st.zm) * p.a - st.zl); };
+    const Gradient one{st.zm, st.zl, p.a, g};
     const int head = before_vectors(d, n);
     const bool vectors_fit = (reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(d)) % 16 == 0;
     const int vectors = vectors_fit ? (n - head) / Vec<T>::N : 0, tail = vectors_fit ? head + vectors * Vec<T>::N : head;
-    if (rank < head) d[rank] = rounded<T>(counts ? one(as_float(z[rank])) : 0.f);
-    for (int c = tail + rank; c < n; c += G) d[c] = rounded<T>(counts ? one(as_float(z[c])) : 0.f);
+    if (rank < head) d[rank] = rounded<T>(counts ? one(as_float(z[rank]), 0.f) : 0.f);
+    for (int c = tail + rank; c < n; c += G) d[c] = rounded<T>(counts ? one(as_float(z[c]), 0.f) : 0.f);
     const uint4* v = reinterpret_cast<const uint4*>(z + head);
     uint4* to = reinterpret_cast<uint4*>(d + head);
-    const F2 m = both(-st.zm), a = both(p.a), l = both(-st.zl), gg = both(g);
+    const bool plain = product_is_finite(st.zm, p.a);
+    const F2 m = both(-st.zm), a = both(p.a), l = both(-st.zl), gg = both(g), c = both(-st.zm * p.a - st.zl);
     for (int i = rank; i < vectors; i += G * U) {
       uint4 w[U];
 #pragma unroll
@@ -371,8 +664,13 @@ distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restri
       for (int u = 0; u < U; ++u) {
         F2 f[Vec<T>::P];
         unpack<T>(w[u], f);
+        if (plain) {
 #pragma unroll
-        for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e] + m, a, l), [](float x) { return exp2_approx(x); }) * gg;
+          for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e], a, c), [](float x) { return exp2_approx(x); }) * gg;
+        } else {
+#pragma unroll
+          for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e] + m, a, l), [](float x) { return exp2_approx(x); }) * gg;
+        }
         if (i + u * G < vectors) __stcs(to + i + u * G, counts ? pack<T>(f) : make_uint4(0, 0, 0, 0));
       }
     }
@@ -381,19 +679,22 @@ distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restri
     for (int j = rank; j < p.k; j += G) {
       const int c = cls[j];
       if (c < from || c >= from + n) continue;
-      float sum = 0.f;  // an index may stand in the list more than once: all of its entries write the same
-      for (int i = 0; i < kp; i += 4) {
-        const int4 ci = *reinterpret_cast<const int4*>(cls + i);
-        const float4 pi = *reinterpret_cast<const float4*>(prob + i);
-        sum += (ci.x == c ? pi.x : 0.f) + (ci.y == c ? pi.y : 0.f) + (ci.z == c ? pi.z : 0.f) + (ci.w == c ? pi.w : 0.f);
-      }
-      d[c - from] = rounded<T>(g * (exp2_approx((as_float(z[c - from]) - st.zm) * p.a - st.zl) - sum));
+      // all of an index's entries write the same
+      d[c - from] = rounded<T>(one(as_float(z[c - from]), sum_at(c, cls, prob, kp)));
     }
   }
 }
 
 // ------------------------------------------------------------------ host
 int threads_per_row(int64_t C, int64_t k) { return C > 4096 ? kWide : C <= 256 && k <= kShortList ? 8 : 32; }
+// Whether one pass makes statistics and gradient: rows that both start as far behind a 16-byte boundary, enough of them, and of a length
+// that keeps the CTA's barriers small beside it.  Returns the CTA's computing threads, or 0.
+int one_pass_threads(const void* Z, int type, int64_t ldz, const void* dZ, int64_t lddz, int64_t M, int64_t C, int64_t k) {
+  const int64_t size = type == GC_TYPE_F32 ? 4 : 2, bytes = C * size;
+  const bool same = (reinterpret_cast<uintptr_t>(Z) - reinterpret_cast<uintptr_t>(dZ)) % 16 == 0 && (ldz - lddz) * size % 16 == 0;
+  if (!same || M < gc::kNumSMs || k > kOnePassList) return 0;
+  return bytes < kOnePassFrom || bytes > Ring<kLong>::kMostBytes ? 0 : bytes <= Ring<kShort>::kMostBytes ? kShort : kLong;
+}
 // Rows above 8192 columns of which there are fewer than SMs are cut, into parts of 4096 or more.
 int parts_of(int64_t M, int64_t C) {
   if (M >= gc::kNumSMs || C <= 8192) return 1;
@@ -440,14 +741,21 @@ size_t gc_distill_workspace_bytes(int64_t M, int64_t C) {
   return size_t(kBlocks) * sizeof(float) + (parts_of(M, C) > 1 ? size_t(M) * kMaxParts * sizeof(float2) : 0);
 }
 
+int gc_distill_one_pass(const void* Z, int type, int64_t ldz, int64_t lddz, int64_t M, int64_t C, int64_t k) {
+  return (type == GC_TYPE_F32 || type == GC_TYPE_BF16) && M >= 0 && C >= 1 && k >= 0 && one_pass_threads(Z, type, ldz, nullptr, lddz, M, C, k) != 0;
+}
+
 int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
                        int index_bits, int64_t ldi, const uint8_t* row_mask, int64_t M, int64_t C, int64_t k, float temperature,
-                       float scale, float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+                       float scale, float* loss, float* stats, void* dZ, int64_t lddz, int64_t pad, void* workspace,
+                       size_t workspace_bytes, void* stream) {
   Problem p;
-  const int rc = fill(p, "gc_distill_forward", Z, type, ldz, top, top_type, ldt, index, index_bits, ldi, M, C, k, temperature);
+  int rc = fill(p, "gc_distill_forward", Z, type, ldz, top, top_type, ldt, index, index_bits, ldi, M, C, k, temperature);
   if (rc != GC_OK) return rc;
   GC_REQUIRE(loss && (M == 0 || stats), "gc_distill_forward: null pointer");
   GC_REQUIRE(gc::aligned16(stats), "gc_distill_forward: the statistics must be 16-byte aligned");
+  GC_REQUIRE(!dZ || (pad >= 0 && pad < 8 && lddz >= C + pad), "gc_distill_forward: leading dimension below the row length");
+  GC_REQUIRE(!dZ || one_pass_threads(Z, type, ldz, dZ, lddz, M, C, k), "gc_distill_forward: no gradient for rows like these");
   const cudaStream_t st = gc::as_stream(stream);
   if (M == 0) {
     const cudaError_t e = cudaMemsetAsync(loss, 0, sizeof(float), st);
@@ -460,6 +768,31 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
   float* partials = static_cast<float*>(workspace);
   float2* parts = p.parts > 1 ? reinterpret_cast<float2*>(partials + kBlocks) : nullptr;
   const int G = parts ? 32 : threads_per_row(C, k);
+  const int whole = dZ ? one_pass_threads(Z, type, ldz, dZ, lddz, M, C, k) : 0;
+  if (whole) {
+    int* word = nullptr;
+    rc = gc::tiles::error_word(&word);
+    if (rc != GC_OK) return rc;
+    const int smem = (whole == kLong ? Ring<kLong>::kSegments : Ring<kShort>::kSegments) * whole * 32 + 2 * kListWords * int((k + 3) / 4 * 4) * 4;
+    const unsigned ctas = unsigned(std::min<int64_t>(M, gc::kNumSMs * (whole == kLong ? 1 : std::min(4, 222 * 1024 / (smem + 2048)))));
+    with_type(type, [&](auto t) {
+      using T = decltype(t);
+      auto run = [&](auto threads) {
+        constexpr int kThreads = decltype(threads)::value;
+        auto kern = distill_one_pass_kernel<T, kThreads>;
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) rc = gc::fail(GC_ERR_CUDA, "gc_distill_forward: %s", cudaGetErrorString(e));
+        else
+          kern<<<ctas, 2 * kThreads + 32, smem, st>>>(p, reinterpret_cast<Stats*>(stats), partials, scale * temperature, static_cast<T*>(dZ), lddz,
+                                                  int(pad), word);
+      };
+      if (whole == kLong) run(std::integral_constant<int, kLong>{});
+      else run(std::integral_constant<int, kShort>{});
+    });
+    if (rc != GC_OK) return rc;
+    distill_sum_kernel<<<1, 256, 0, st>>>(partials, int(ctas), scale * temperature * temperature, loss);
+    return gc::check_launch("gc_distill_forward", 2);
+  }
   const unsigned grid = grid_of(M, G);
   with_type(type, [&](auto t) {
     using T = decltype(t);
@@ -475,7 +808,7 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
 
 int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
                         int index_bits, int64_t ldi, const float* stats, int64_t M, int64_t C, int64_t k, float temperature,
-                        float scale, const float* grad_loss, void* dZ, int64_t lddz, int64_t pad, void* stream) {
+                        float scale, const float* grad_loss, void* dZ, int64_t lddz, int64_t pad, int dz_made, void* stream) {
   Problem p;
   const int rc = fill(p, "gc_distill_backward", Z, type, ldz, top, top_type, ldt, index, index_bits, ldi, M, C, k, temperature);
   if (rc != GC_OK) return rc;
@@ -486,7 +819,8 @@ int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, i
   const int G = threads_per_row(C, k);
   const int rows = G > 32 ? 1 : 256 / G, kp = int((k + 3) / 4 * 4);
   const size_t smem = size_t(rows) * 2 * kp * 4;
-  const unsigned grid = unsigned(std::min<int64_t>(gc::ceil_div(M * p.parts, rows), int64_t(1) << 30));
+  // where dZ is mostly there already, as many CTAs as run at one time
+  const unsigned grid = unsigned(std::min<int64_t>(gc::ceil_div(M * p.parts, rows), dz_made ? gc::kNumSMs * 4 : int64_t(1) << 30));
   int bad = GC_OK;
   with_type(type, [&](auto t) {
     using T = decltype(t);
@@ -499,7 +833,7 @@ int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, i
       }
       if (bad == GC_OK)
         kern<<<grid, kG > 32 ? kG : 256, smem, gc::as_stream(stream)>>>(p, reinterpret_cast<const Stats*>(stats), grad_loss,
-                                                                         scale * temperature, static_cast<T*>(dZ), lddz, int(pad));
+                                                                         scale * temperature, static_cast<T*>(dZ), lddz, int(pad), dz_made != 0);
     });
   });
   return bad != GC_OK ? bad : gc::check_launch("gc_distill_backward");

@@ -273,10 +273,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   }, NoGil());
   m.def("distill_forward", [](const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
                               double scale) {
-    const DistillForward f = distill_forward(Z, top, index, row_mask, temperature, scale);
+    const DistillForward f = distill_forward(Z, top, index, row_mask, temperature, scale, false);
     return std::make_tuple(f.loss, std::vector<Tensor>{f.Z, f.top, f.index, f.stats});
   }, NoGil());
-  m.def("distill_backward", &distill_backward, NoGil());
+  m.def("distill_backward", [](const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats,
+                               double temperature, double scale) {
+    return distill_backward(grad, Z, top, index, stats, Tensor(), temperature, scale);
+  }, NoGil());
   m.def("argmax_accuracy", [](const Tensor& logits, const OptTensor& labels, const std::optional<std::vector<Tensor>>& masks,
                               bool want_pred) -> std::optional<std::pair<Tensor, Tensor>> {
     if (torch::jit::tracer::isTracing()) return std::nullopt;

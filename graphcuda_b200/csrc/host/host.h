@@ -49,7 +49,7 @@ inline bool f32_on(const Tensor& t, const at::Device& dev) {
   X(gc_rms_norm_forward) X(gc_rms_norm_backward_workspace_bytes) X(gc_rms_norm_backward) X(gc_adamw_step)           \
   X(gc_adamw_moments_f32) X(gc_gated_ffn_saved_bytes) X(gc_gated_ffn_workspace_bytes)                              \
   X(gc_gated_ffn_forward_bf16) X(gc_gated_ffn_backward_bf16) X(gc_gated_ffn_e4m3_workspace_bytes)                   \
-  X(gc_gated_ffn_forward_e4m3) X(gc_distill_workspace_bytes) X(gc_distill_forward) X(gc_distill_backward)             \
+  X(gc_gated_ffn_forward_e4m3) X(gc_distill_workspace_bytes) X(gc_distill_one_pass) X(gc_distill_forward) X(gc_distill_backward)             \
   X(gc_grouped_linear_workspace_bytes) X(gc_grouped_linear_forward_bf16) X(gc_grouped_linear_backward_bf16)         \
   X(gc_linear_int4_workspace_bytes) X(gc_linear_int4_bf16) X(gc_gated_ffn_int4_workspace_bytes) X(gc_gated_ffn_int4_bf16)
 struct Abi {
@@ -201,10 +201,11 @@ Tensor nll_loss(const Tensor& Z, const Tensor& labels, const OptTensor& row_mask
 // The distillation loss, and what its backward pass needs.
 struct DistillForward {
   Tensor loss, Z, top, index, stats;  // as the kernels took them
+  Tensor dz;                          // where asked for, and made in the same pass: the buffer of the gradient for a loss's gradient of 1
 };
 DistillForward distill_forward(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
-                               double scale);
-Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats,
+                               double scale, bool want_gradient);
+Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats, const Tensor& dz,
                         double temperature, double scale);
 Tensor distill_loss(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
                     double scale);

@@ -104,10 +104,24 @@ namespace {
 bool f32_or_bf16(const Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
 int type_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? GC_TYPE_F32 : GC_TYPE_BF16; }
 int bits_of(const Tensor& index) { return index.scalar_type() == at::kLong ? 64 : 32; }
+// The gradient's buffer.  Its rows start as many bytes behind a 16-byte boundary as the logits' own, so that both go in vectors.  Where
+// the logits are a view of a matrix padded to 16-byte rows (an odd class count), its `pad` columns become zero, so that the layer below
+// can aggregate it without re-padding a copy (as in nll_backward).
+struct GradientRows {
+  int64_t ld, pad;
+};
+GradientRows gradient_rows(const Tensor& Z) {
+  const int64_t C = Z.size(1), ldz = ld_of(Z), vec = 16 / Z.element_size();
+  GradientRows g{C + (ldz - C) % vec, 0};
+  if (Z.size(0) > 1 && C < g.ld && ldz == g.ld && g.ld % 4 == 0 && g.ld <= C + 3 && Z.scalar_type() == at::kFloat &&
+      reinterpret_cast<uintptr_t>(Z.data_ptr()) % 16 == 0)
+    g.pad = g.ld - C;
+  return g;
+}
 }  // namespace
 
 DistillForward distill_forward(const Tensor& Zin, const Tensor& top, const Tensor& index, const OptTensor& row_mask,
-                               double temperature, double scale) {
+                               double temperature, double scale, bool want_gradient) {
   require(Zin.dim() == 2 && Zin.is_cuda() && f32_or_bf16(Zin), "distill_loss: logits must be a float32 or bfloat16 CUDA matrix");
   const at::Device dev = Zin.device();
   const int64_t M = Zin.size(0), C = Zin.size(1);
@@ -134,37 +148,36 @@ DistillForward distill_forward(const Tensor& Zin, const Tensor& top, const Tenso
   const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
   f.stats = at::empty({M, 4}, f32);
   f.loss = at::empty({}, f32);
+  GradientRows rows{C, 0};
+  if (want_gradient) {
+    rows = gradient_rows(f.Z);
+    if (abi.gc_distill_one_pass(f.Z.const_data_ptr(), type_of(f.Z), ld_of(f.Z), rows.ld, M, C, top.size(1)))
+      f.dz = at::empty({M, rows.ld}, f.Z.options());
+  }
   const Scratch ws = scratch(kSpmm, abi.gc_distill_workspace_bytes(M, C), dev);
   check(abi.gc_distill_forward(f.Z.const_data_ptr(), type_of(f.Z), ld_of(f.Z), f.top.const_data_ptr(), type_of(f.top), ld_of(f.top),
                                f.index.const_data_ptr(), bits_of(f.index), ld_of(f.index),
                                mask8.defined() ? static_cast<const uint8_t*>(mask8.data_ptr()) : nullptr, M, C, top.size(1),
-                               float(temperature), float(scale), f.loss.data_ptr<float>(), f.stats.data_ptr<float>(), ws.ptr,
-                               ws.bytes, stream_of(dev)),
+                               float(temperature), float(scale), f.loss.data_ptr<float>(), f.stats.data_ptr<float>(),
+                               f.dz.defined() ? f.dz.data_ptr() : nullptr, rows.ld, rows.pad, ws.ptr, ws.bytes, stream_of(dev)),
         "gc_distill_forward");
   return f;
 }
 
-Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats,
+// dz: the buffer that the forward pass has filled, or undefined
+Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats, const Tensor& dz,
                         double temperature, double scale) {
-  const int64_t M = Z.size(0), C = Z.size(1), ldz = ld_of(Z);
+  const int64_t M = Z.size(0), C = Z.size(1);
   const at::Device dev = Z.device();
   const c10::cuda::CUDAGuard guard(dev);
-  // Rows of the gradient start as many bytes behind a 16-byte boundary as the logits' own, so that both go in vectors.  Where the
-  // logits are a view of a matrix padded to 16-byte rows (an odd class count), its pad columns become zero, so that the layer below
-  // can aggregate it without re-padding a copy (as in nll_backward).
-  const int64_t vec = 16 / Z.element_size(), lddz = std::max<int64_t>(C, 1) + (ldz - C) % vec;
-  Tensor buf = at::empty({M, lddz}, Z.options());
-  int64_t pad = 0;
-  if (M > 1 && C < lddz && ldz == lddz && lddz % 4 == 0 && lddz <= C + 3 && Z.scalar_type() == at::kFloat &&
-      reinterpret_cast<uintptr_t>(Z.data_ptr()) % 16 == 0) {
-    pad = lddz - C;
-    register_zero_padded(buf);
-  }
-  const Tensor dZ = lddz == C ? buf : buf.narrow(1, 0, C);
+  const GradientRows rows = gradient_rows(Z);
+  const Tensor buf = dz.defined() ? dz : at::empty({M, rows.ld}, Z.options());
+  if (rows.pad) register_zero_padded(buf);
+  const Tensor dZ = rows.ld == C ? buf : buf.narrow(1, 0, C);
   const Tensor g = grad.to(at::kFloat).contiguous();
-  check(abi.gc_distill_backward(Z.const_data_ptr(), type_of(Z), ldz, top.const_data_ptr(), type_of(top), ld_of(top),
+  check(abi.gc_distill_backward(Z.const_data_ptr(), type_of(Z), ld_of(Z), top.const_data_ptr(), type_of(top), ld_of(top),
                                 index.const_data_ptr(), bits_of(index), ld_of(index), stats.const_data_ptr<float>(), M, C, top.size(1),
-                                float(temperature), float(scale), g.const_data_ptr<float>(), buf.data_ptr(), lddz, pad,
+                                float(temperature), float(scale), g.const_data_ptr<float>(), buf.data_ptr(), rows.ld, rows.pad, dz.defined(),
                                 stream_of(dev)),
         "gc_distill_backward");
   return dZ;
@@ -174,16 +187,24 @@ namespace {
 struct DistillFunction : torch::autograd::Function<DistillFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& Z, const Tensor& top, const Tensor& index,
                         const OptTensor& row_mask, double temperature, double scale) {
-    const DistillForward f = distill_forward(Z, top, index, row_mask, temperature, scale);
+    const DistillForward f = distill_forward(Z, top, index, row_mask, temperature, scale, true);
     ctx->save_for_backward({f.Z, f.top, f.index, f.stats});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["scale"] = scale;
+    if (f.dz.defined()) ctx->saved_data["dz"] = f.dz;
     return f.loss;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     once("distill_loss");
     const auto saved = ctx->get_saved_variables();
-    return {distill_backward(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["temperature"].toDouble(),
+    // handed out once: whoever differentiates the same graph again may have changed it by then, and gets a buffer of its own
+    Tensor dz;
+    const auto made = ctx->saved_data.find("dz");
+    if (made != ctx->saved_data.end()) {
+      dz = made->second.toTensor();
+      ctx->saved_data.erase(made);
+    }
+    return {distill_backward(grads[0], saved[0], saved[1], saved[2], saved[3], dz, ctx->saved_data["temperature"].toDouble(),
                              ctx->saved_data["scale"].toDouble()),
             Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
@@ -192,7 +213,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
 
 Tensor distill_loss(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
                     double scale) {
-  if (!recorded({&Z, &top})) return distill_forward(Z, top, index, row_mask, temperature, scale).loss;
+  if (!recorded({&Z, &top})) return distill_forward(Z, top, index, row_mask, temperature, scale, false).loss;
   return DistillFunction::apply(Z, top, index, row_mask, temperature, scale);
 }
 

@@ -400,14 +400,18 @@ int gc_logsoftmax_nll_backward_pad_f32(const float* Z, int64_t ldz, const int64_
  *   type, top_type: GC_TYPE_F32 or GC_TYPE_BF16 (dZ has Z's).  index_bits: 64 or 32.  k: at most 1024.
  *   stats: M x 4 floats, 16-byte aligned, which the backward call reads.  loss, grad_loss: one device float each.
  *   pad: columns behind a row of dZ that are its own and become zero (less than 8).
+ * Where gc_distill_one_pass (a 16-byte aligned dZ assumed) is not 0, one pass over the logits can do both: a forward call that is given
+ * dZ writes it, for grad_loss = 1.  Then the backward call gets the same dZ with dz_made = 1, and leaves it as it is where grad_loss is 1.
  */
+int gc_distill_one_pass(const void* Z, int type, int64_t ldz, int64_t lddz, int64_t M, int64_t C, int64_t k);
 size_t gc_distill_workspace_bytes(int64_t M, int64_t C);
 int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
                        int index_bits, int64_t ldi, const uint8_t* row_mask, int64_t M, int64_t C, int64_t k, float temperature,
-                       float scale, float* loss, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+                       float scale, float* loss, float* stats, void* dZ, int64_t lddz, int64_t pad, void* workspace,
+                       size_t workspace_bytes, void* stream);
 int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
                         int index_bits, int64_t ldi, const float* stats, int64_t M, int64_t C, int64_t k, float temperature,
-                        float scale, const float* grad_loss, void* dZ, int64_t lddz, int64_t pad, void* stream);
+                        float scale, const float* grad_loss, void* dZ, int64_t lddz, int64_t pad, int dz_made, void* stream);
 
 /*
  * Evaluation tail of the reference's script (tests/gcn/graphcuda_impl.py:63-68:

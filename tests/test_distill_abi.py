@@ -10,14 +10,14 @@ L = _lib.lib
 
 
 def _forward(z=16, zt=0, ldz=C, t=16, tt=0, ldt=K, i=16, bits=64, ldi=K, mask=None, m=M, c=C, k=K, temp=1.0, scale=1.0, loss=16,
-             stats=16, ws=16, wsb=None):
-    return L().gc_distill_forward(z, zt, ldz, t, tt, ldt, i, bits, ldi, mask, m, c, k, temp, scale, loss, stats, ws,
+             stats=16, dz=None, lddz=C, pad=0, ws=16, wsb=None):
+    return L().gc_distill_forward(z, zt, ldz, t, tt, ldt, i, bits, ldi, mask, m, c, k, temp, scale, loss, stats, dz, lddz, pad, ws,
                                   L().gc_distill_workspace_bytes(M, C) if wsb is None else wsb, None)
 
 
 def _backward(z=16, zt=0, ldz=C, t=16, tt=0, ldt=K, i=16, bits=64, ldi=K, stats=16, m=M, c=C, k=K, temp=1.0, scale=1.0, g=16, dz=16,
-              lddz=C, pad=0):
-    return L().gc_distill_backward(z, zt, ldz, t, tt, ldt, i, bits, ldi, stats, m, c, k, temp, scale, g, dz, lddz, pad, None)
+              lddz=C, pad=0, made=0):
+    return L().gc_distill_backward(z, zt, ldz, t, tt, ldt, i, bits, ldi, stats, m, c, k, temp, scale, g, dz, lddz, pad, made, None)
 
 
 @pytest.mark.parametrize("call", [_forward, _backward])
@@ -32,6 +32,8 @@ def test_what_both_refuse(call):
 
 def test_forward_arguments():
     assert _forward(loss=None) == -1
+    assert _forward(dz=16, lddz=C - 1) == -1 and _forward(dz=16, pad=8, lddz=C + 8) == -1
+    assert _forward(dz=16) == -1 and b"rows like these" in L().gc_last_error()
     assert _forward(ws=None) == -4 and _forward(wsb=L().gc_distill_workspace_bytes(M, C) - 1) == -4 and _forward(ws=24) == -1
     assert L().gc_distill_workspace_bytes(-1, C) == L().gc_distill_workspace_bytes(M, 0) == 0
     assert L().gc_distill_workspace_bytes(4, 100_000) > L().gc_distill_workspace_bytes(4, 100)
@@ -41,6 +43,18 @@ def test_backward_arguments():
     assert _backward(g=None) == -1 and _backward(dz=None) == -1 and _backward(lddz=C - 1) == -1
     assert _backward(pad=-1) == -1 and _backward(pad=8, lddz=C + 8) == -1 and _backward(pad=2, lddz=C + 1) == -1
     assert _backward(m=0, z=None, t=None, i=None, stats=None, dz=None, g=None) == 0
+
+
+def test_which_rows_go_in_one_pass():
+    def one(z, t, ldz, lddz, m, c, k=8):
+        return L().gc_distill_one_pass(z, t, ldz, lddz, m, c, k)
+
+    assert one(16, 0, 8192, 8192, 1000, 8192) and one(16, 1, 90_001, 90_001, 1000, 90_001)
+    assert not one(16, 0, 47, 47, 100_000, 47)       # short rows
+    assert not one(16, 0, 50_000, 50_000, 1000, 50_000) and not one(16, 1, 100_000, 100_000, 1000, 100_000)  # longer than the ring
+    assert not one(16, 0, 8192, 8192, 100, 8192)     # few rows
+    assert not one(20, 0, 8192, 8192, 1000, 8192) and not one(16, 0, 8193, 8192, 1000, 8192)  # the rows lie differently
+    assert not one(16, 2, 8192, 8192, 1000, 8192) and not one(16, 0, 8192, 8192, 1000, 8192, 257)
 
 
 def test_cpu_tensors_are_refused():
