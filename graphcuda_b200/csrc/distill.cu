@@ -15,8 +15,8 @@
 // itself has; the backward call looks at g and, where it is another, computes dZ from the logits as it does for other rows.
 //
 // Otherwise G threads take a row: 8 up to 256 classes (a row is few vectors, and what a row costs beside them is shared by fewer), a warp up to
-// 4096, a CTA of 512 above; with fewer rows than SMs a CTA takes a part of a row (kParts) and another launch puts the parts
-// together.  Rows may start anywhere: what lies before the first and behind the last 16-byte vector is read by itself.
+// 4096, a CTA of 128 threads up to 12,288, of 256 above (forward: 20,000 x 8192 in bf16 88 us with 128 threads, 102 with 256, 237 with 512; 4096 x
+// 65,536 99, 92, 109); with fewer rows than SMs a CTA takes a part of a row and another launch puts the parts together.  Rows may start anywhere: what lies before the first and behind the last 16-byte vector is read by itself.
 #include "common.cuh"
 #include "ffn_internal.cuh"
 #include "tiles.cuh"
@@ -36,7 +36,9 @@ using gc::ffn::fma2;
 constexpr int kBlocks = gc::kNumSMs * 8;  // partial sums of the loss
 constexpr int kMaxParts = 16;             // of a row
 constexpr int kMaxList = 1024;            // entries of a list
-constexpr int kWide = 512;                // threads of a CTA that takes a row, or a part of one
+constexpr int kWide = 256, kMid = 128;    // threads of a CTA that takes a row
+constexpr int kPart = 512;                // of one that takes a part of a row
+constexpr int64_t kMidTo = 12288;         // classes up to which kMid threads take a row
 constexpr int kShortList = 32;            // entries up to which 8 threads take a row
 constexpr float kLn2 = 0.69314718055994531f, kLog2e = 1.4426950408889634f;
 
@@ -58,29 +60,34 @@ __device__ __forceinline__ float log2_approx(float x) {
 }
 
 // ------------------------------------------------------------------ groups of threads
-// Reductions over the G threads of a row; all of them get the result.  For a CTA `sh` holds a word per warp.
-template <int G, class F>
-__device__ __forceinline__ float over_group(float v, float* sh, F&& f) {
+// Reductions over the G threads of a row, of several values at once; all threads get the results.  For a CTA `sh` holds so many words per
+// warp.
+template <int G, int N, class F>
+__device__ __forceinline__ void over_group(float (&v)[N], float* sh, F&& f) {
 #pragma unroll
-  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = f(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
   if constexpr (G > 32) {
     __syncthreads();  // the words' last readers are done
-    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = sh[0];
+    if (threadIdx.x % 32 == 0)
 #pragma unroll
-    for (int w = 1; w < G / 32; ++w) v = f(v, sh[w]);
+      for (int i = 0; i < N; ++i) sh[threadIdx.x / 32 * N + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = sh[i];
+#pragma unroll
+    for (int w = 1; w < G / 32; ++w)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = f(v[i], sh[w * N + i]);
   }
-  return v;
 }
-template <int G>
-__device__ __forceinline__ float group_max(float v, float* sh) {
-  return over_group<G>(v, sh, [](float a, float b) { return fmaxf(a, b); });
-}
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float* sh) {
-  return over_group<G>(v, sh, [](float a, float b) { return a + b; });
-}
+struct Larger {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Sum {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
 template <int G>
 __device__ __forceinline__ void group_sync() {
   if constexpr (G > 32) __syncthreads();
@@ -179,13 +186,9 @@ __device__ __forceinline__ Running scan(const T* __restrict__ z, int n, int rank
   for (int i = 0; i < 2; ++i) r.s += exp2_approx((ends[i] - r.base()) * a);
   return r;
 }
-// The group's threads together.
-template <int G>
-__device__ __forceinline__ Running combined(Running r, float a, float* sh) {
-  Running all;
-  all.m = group_max<G>(r.m, sh);
-  all.s = group_sum<G>(r.m == -INFINITY ? r.s : r.s * exp2_approx((r.m - all.m) * a), sh);
-  return all;
+// What a thread's sum is where the maximum is `top`.
+__device__ __forceinline__ float rescaled(const Running& r, float top, float a) {
+  return r.m == -INFINITY ? r.s : r.s * exp2_approx((r.m - top) * a);
 }
 
 // ------------------------------------------------------------------ lists
@@ -193,15 +196,22 @@ struct Entry {
   float t;
   int c;  // below zero: none
 };
-__device__ __forceinline__ Entry entry(const Problem& p, int64_t r, int j) {
-  const int64_t at = r * p.ldi + j;
-  const int64_t c = p.index64 ? __ldg(static_cast<const int64_t*>(p.index) + at) : __ldg(static_cast<const int32_t*>(p.index) + at);
-  const int64_t ta = r * p.ldt + j;
-  Entry e;
+// As it was loaded, so that the loads can go out long before anything looks at it.
+struct Loaded {
+  int64_t c;
+  float t;
+};
+__device__ __forceinline__ Loaded load_entry(const Problem& p, int64_t r, int j) {
+  const int64_t at = r * p.ldi + j, ta = r * p.ldt + j;
+  Loaded e;
+  e.c = p.index64 ? __ldg(static_cast<const int64_t*>(p.index) + at) : __ldg(static_cast<const int32_t*>(p.index) + at);
   e.t = p.top16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.top)[ta]) : __ldg(static_cast<const float*>(p.top) + ta);
-  e.c = c >= 0 && c < p.C && e.t != -INFINITY ? int(c) : -1;
   return e;
 }
+__device__ __forceinline__ Entry looked_at(const Problem& p, const Loaded& e) {
+  return {e.t, e.c >= 0 && e.c < p.C && e.t != -INFINITY ? int(e.c) : -1};
+}
+__device__ __forceinline__ Entry entry(const Problem& p, int64_t r, int j) { return looked_at(p, load_entry(p, r, j)); }
 
 // Of a row: the student's maximum and the logarithm (base 2) of its sum, and the teacher's.  A row that does not count has +inf
 // for the last, which no other has.
@@ -214,14 +224,18 @@ __device__ __host__ __forceinline__ int part_columns(int C, int parts) { return 
 
 // Part `blockIdx.x` of row `blockIdx.y`.
 template <class T>
-__global__ void __launch_bounds__(kWide)
+__global__ void __launch_bounds__(kPart)
 distill_part_kernel(const __grid_constant__ Problem p, float2* __restrict__ out) {
-  __shared__ float sh[kWide / 32];
+  __shared__ float sh[kPart / 32];
   const int64_t r = blockIdx.y;
   if (p.mask && !p.mask[r]) return;
   const int width = part_columns(p.C, p.parts), from = min(p.C, int(blockIdx.x) * width), n = min(width, p.C - from);
-  const Running x = combined<kWide>(scan<T, kWide>(static_cast<const T*>(p.z) + r * p.ldz + from, n, threadIdx.x, p.a), p.a, sh);
-  if (threadIdx.x == 0) out[r * p.parts + blockIdx.x] = make_float2(x.m, x.s);
+  const Running x = scan<T, kPart>(static_cast<const T*>(p.z) + r * p.ldz + from, n, threadIdx.x, p.a);
+  float top[1] = {x.m};
+  over_group<kPart>(top, sh, Larger{});
+  float sum[1] = {rescaled(x, top[0], p.a)};
+  over_group<kPart>(sum, sh, Sum{});
+  if (threadIdx.x == 0) out[r * p.parts + blockIdx.x] = make_float2(top[0], sum[0]);
 }
 
 // G threads per row; the block's sum of losses goes to partials.  from_parts: what the kernel above left, or null.
@@ -230,29 +244,22 @@ __global__ void __launch_bounds__(G > 32 ? G : 256)
 distill_forward_kernel(const __grid_constant__ Problem p, const float2* __restrict__ from_parts, Stats* __restrict__ stats,
                        float* __restrict__ partials) {
   constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G;  // rows of a CTA at a time
-  __shared__ float sh[32];
+  __shared__ float sh[3 * 32];
   const int rank = threadIdx.x % G;
   float loss = 0.f;
   for (int64_t r0 = int64_t(blockIdx.x) * R; r0 < p.M; r0 += int64_t(gridDim.x) * R) {  // the same for all of a CTA
     const int64_t mine = r0 + threadIdx.x / G, r = min(mine, p.M - 1);
     const bool chosen = mine < p.M && (!p.mask || p.mask[r]);
     const T* z = static_cast<const T*>(p.z) + r * p.ldz;
-    // the list: its largest logit
-    float tm = -INFINITY;
-    bool any = false;
-    for (int j = rank; chosen && j < p.k; j += G) {
-      const Entry e = entry(p, r, j);
-      if (e.c >= 0) tm = fmaxf(tm, e.t), any = true;
-    }
-    tm = group_max<G>(tm, sh);
-    any = group_max<G>(any ? 1.f : 0.f, sh) > 0.f;
-    const bool counts = chosen && any;
-    if (G > 32 && !counts) {
+    if (G > 32 && !chosen) {
       if (threadIdx.x == 0) stats[r] = {0.f, 0.f, 0.f, INFINITY};
       continue;
     }
+    // the thread's first entry is on its way while the row is read
+    Loaded own{-1, 0.f};
+    if (chosen && rank < p.k) own = load_entry(p, r, rank);
     Running x;
-    if (counts) {
+    if (chosen) {
       if (from_parts) {
         for (int i = rank; i < p.parts; i += G) {
           const float2 part = from_parts[r * p.parts + i];
@@ -263,26 +270,42 @@ distill_forward_kernel(const __grid_constant__ Problem p, const float2* __restri
         x = scan<T, G>(z, p.C, rank, p.a);
       }
     }
-    x = combined<G>(x, p.a, sh);
-    // sum of the list's exponentials, and of their products with what the logarithms differ by
-    float s = 0.f, d = 0.f;
-    for (int j = rank; counts && j < p.k; j += G) {
+    const Entry mine_first = looked_at(p, own);
+    const float at_first = mine_first.c >= 0 ? as_float(z[mine_first.c]) : 0.f;
+    // the maxima; whether the list has entries
+    float top[3] = {x.m, mine_first.c >= 0 ? mine_first.t : -INFINITY, mine_first.c >= 0 ? 1.f : 0.f};
+    for (int j = rank + G; chosen && j < p.k; j += G) {
       const Entry e = entry(p, r, j);
-      if (e.c < 0) continue;
-      const float w = exp2_approx((e.t - tm) * p.a);
-      s += w;
-      if (!(w == 0.f)) d += w * (((e.t - tm) - (as_float(z[e.c]) - x.m)) * p.a);
+      if (e.c >= 0) top[1] = fmaxf(top[1], e.t), top[2] = 1.f;
     }
-    s = group_sum<G>(s, sh);
-    d = group_sum<G>(d, sh);
+    over_group<G>(top, sh, Larger{});
+    const float zm = top[0], tm = top[1];
+    const bool counts = chosen && top[2] > 0.f;
+    // the sums: of the row's exponentials, of the list's, and of the list's times what the logarithms differ by
+    float sum[3] = {rescaled(x, zm, p.a), 0.f, 0.f};
+    auto add = [&](const Entry& e, float at) {
+      if (e.c < 0) return;
+      const float w = exp2_approx((e.t - tm) * p.a);
+      sum[1] += w;
+      if (!(w == 0.f)) sum[2] += w * (((e.t - tm) - (at - zm)) * p.a);
+    };
+    if (counts) {
+      add(mine_first, at_first);
+      for (int j = rank + G; j < p.k; j += G) {
+        const Entry e = entry(p, r, j);
+        add(e, e.c >= 0 ? as_float(z[e.c]) : 0.f);
+      }
+    }
+    over_group<G>(sum, sh, Sum{});
     if (rank == 0 && mine < p.M) {
-      const Stats st = {x.m, log2_approx(x.s), tm, counts ? log2_approx(s) : INFINITY};
+      const Stats st = {zm, log2_approx(sum[0]), tm, counts ? log2_approx(sum[1]) : INFINITY};
       stats[r] = counts ? st : Stats{0.f, 0.f, 0.f, INFINITY};
-      if (counts) loss += kLn2 * (d / s - st.tl + st.zl);
+      if (counts) loss += kLn2 * (sum[2] / sum[1] - st.tl + st.zl);
     }
   }
-  loss = over_group<(G > 32 ? G : 256)>(loss, sh, [](float a, float b) { return a + b; });
-  if (threadIdx.x == 0) partials[blockIdx.x] = loss;
+  float all[1] = {loss};
+  over_group<(G > 32 ? G : 256)>(all, sh, Sum{});
+  if (threadIdx.x == 0) partials[blockIdx.x] = all[0];
 }
 
 __global__ void __launch_bounds__(256)
@@ -348,14 +371,14 @@ __device__ __forceinline__ float sum_at(int c, const int* cls, const float* prob
 }
 
 // ------------------------------------------------------------------ both in one pass
-constexpr int64_t kOnePassFrom = 8192;  // bytes of a row
-constexpr int kLong = 480, kShort = 128;  // threads for long and short rows
+constexpr int64_t kOnePassFrom = 8192;  // bytes; rows that are longer (30,000 x 4096 in bf16: 161 us, 143 in two passes; 20,000 x 8192: 184 and 412)
+constexpr int kLong = 352, kShort = 64;  // threads of either half, for long and short rows
+constexpr int kSegments = 10;            // of a ring
+constexpr int kEach = 4;                 // vectors per thread of a segment
 template <int THREADS>
 struct Ring {
-  static constexpr int kBytes = THREADS * 32;  // of a segment: two vectors per thread
-  static constexpr int kVectors = THREADS * 2;
-  static constexpr int kSegments = THREADS == kLong ? 14 : 13;
-  static constexpr int kMostBytes = (kSegments - 1) * kBytes;  // of a row
+  static constexpr int kVectors = THREADS * kEach, kBytes = kVectors * 16;  // of a segment
+  static constexpr int kMostBytes = (kSegments - 1) * kBytes;               // of a row
 };
 // Entries' classes, logits (later probabilities) and the student's logits at them, of a row.
 constexpr int kListWords = 3;
@@ -368,26 +391,28 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 template <int BARRIER, int THREADS>
 __device__ __forceinline__ void sync_threads() { asm volatile("bar.sync %0, %1;" ::"n"(BARRIER), "n"(THREADS) : "memory"); }
 
-// THREADS that make a row's statistics, as many that make the gradient of the row before, and a warp whose first lane fetches.
-// Persistent over rows.  (With the same threads doing one after the other the exponentials of a row waited for its sums: 285 us for 4096 x
-// 65,536 in bf16.)
+// THREADS that make a row's statistics, as many that make the gradient of the row before, a warp whose first lane fetches segments, and
+// one that fetches lists a row ahead (two loads after each other, which the row's threads would wait for).  Persistent over rows.  (4096 x 65,536 in bf16, forward and backward: 212 us, 5.1 TB/s
+// of the bytes that cannot be avoided; 285 with the same threads doing one after the other, whose exponentials of a row wait for its
+// sums; 231 with 256 threads and 13 segments of 16 KB, 220 with 384 and 9.  What is left is issue slots: 16 instructions per logit,
+// the special function unit half busy.)
 template <class T, int THREADS>
-__global__ void __launch_bounds__(2 * THREADS + 32)
+__global__ void __launch_bounds__(2 * THREADS + 64)
 distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ stats, float* __restrict__ partials, float g,
                         T* __restrict__ dz, int64_t lddz, int pad, int* __restrict__ word) {
   using namespace gc::tc;
   constexpr int kBytes = Ring<THREADS>::kBytes, kVectors = Ring<THREADS>::kVectors, kWarps = THREADS / 32, N = Vec<T>::N;
-  constexpr int kSegments = Ring<THREADS>::kSegments;
   extern __shared__ __align__(128) uint8_t smem[];  // the ring; the lists of two rows: classes, logits (then probabilities), the student's logits
-  __shared__ __align__(8) uint64_t bars[2 * kSegments + 4];
+  __shared__ __align__(8) uint64_t bars[2 * kSegments + 6];
   __shared__ float sh[2][kWarps][4];
-  __shared__ float info[2][4];  // of two rows: the student's maximum and logarithm of its sum; whether the row counts
+  __shared__ float info[2][4];  // of two rows: the student's maximum and logarithm of its sum; whether the row counts; the list's largest logit
   __shared__ int abort_s;
   const uint32_t ring = smem_u32(smem);
   auto full = [&](int i) { return smem_u32(&bars[i]); };
   auto empty = [&](int i) { return smem_u32(&bars[kSegments + i]); };
   auto ready = [&](int i) { return smem_u32(&bars[2 * kSegments + i]); };
   auto taken = [&](int i) { return smem_u32(&bars[2 * kSegments + 2 + i]); };
+  auto listed = [&](int i) { return smem_u32(&bars[2 * kSegments + 4 + i]); };
   const int kp = (p.k + 3) / 4 * 4;
   auto classes = [&](int i) { return reinterpret_cast<int*>(smem + kSegments * kBytes) + i * kListWords * kp; };
   auto probs = [&](int i) { return reinterpret_cast<float*>(classes(i) + kp); };
@@ -400,6 +425,7 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(ready(i), 1);
+      mbar_init(listed(i), 1);
       mbar_init(taken(i), kWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -415,7 +441,39 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
   };
   bool ok = true;
 
-  if (threadIdx.x >= 2 * THREADS) {
+  if (threadIdx.x >= 2 * THREADS + 32) {
+    // ------------------------------------------------------------ fetches lists
+    constexpr int kEntries = kOnePassList / 32;  // of a lane
+    for (int64_t r = blockIdx.x; r < p.M; r += gridDim.x) {
+      if (p.mask && !p.mask[r]) continue;
+      const T* z = static_cast<const T*>(p.z) + r * p.ldz;
+      const int buf = rows & 1;
+      Entry e[kEntries];
+      float at[kEntries], tm = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kEntries; ++i) e[i] = i * 32 + lane < p.k ? entry(p, r, i * 32 + lane) : Entry{0.f, -1};
+#pragma unroll
+      for (int i = 0; i < kEntries; ++i) at[i] = e[i].c >= 0 ? as_float(z[e[i].c]) : 0.f;
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < kEntries; ++i)
+        if (e[i].c >= 0) tm = fmaxf(tm, e[i].t), any = true;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+      any = __any_sync(0xffffffffu, any);
+      if (ok) ok = gc::tiles::wait(taken(buf), ((rows >> 1) & 1u) ^ 1u, abort_p);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kEntries; ++i) {
+        const int j = i * 32 + lane;
+        if (j < kp) classes(buf)[j] = e[i].c, probs(buf)[j] = e[i].t, at_entries(buf)[j] = at[i];
+      }
+      if (lane == 0) info[buf][2] = any ? 1.f : 0.f, info[buf][3] = tm;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(listed(buf));
+      ++rows;
+    }
+  } else if (threadIdx.x >= 2 * THREADS) {
     // ------------------------------------------------------------ fetches
     if (lane == 0) {
       uint32_t issued = 0;
@@ -443,22 +501,23 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
     const int warp = rank / 32;
     float loss = 0.f;
     int turn = 0;
-    auto reduce = [&](float (&v)[4], auto f) {
+    auto reduce = [&](auto& v, auto f) {
+      constexpr int n = sizeof(v) / sizeof(float);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = f(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
+        for (int i = 0; i < n; ++i) v[i] = f(v[i], __shfl_xor_sync(0xffffffffu, v[i], o));
       turn ^= 1;  // the other place's readers have come past a barrier since
       if (lane == 0)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sh[turn][warp][i] = v[i];
+        for (int i = 0; i < n; ++i) sh[turn][warp][i] = v[i];
       sync_threads<1, THREADS>();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = sh[turn][0][i];
+      for (int i = 0; i < n; ++i) v[i] = sh[turn][0][i];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = f(v[i], sh[turn][w][i]);
+        for (int i = 0; i < n; ++i) v[i] = f(v[i], sh[turn][w][i]);
     };
     for (int64_t r = blockIdx.x; r < p.M; r += gridDim.x) {
       if (p.mask && !p.mask[r]) {
@@ -468,37 +527,24 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
       const T* z = static_cast<const T*>(p.z) + r * p.ldz;
       const int head = before_vectors(z, p.C), vectors = (p.C - head) / N, tail = head + vectors * N;
       const int buf = rows & 1;
-      int* cls = classes(buf);
-      float *prob = probs(buf), *at_entry = at_entries(buf);
-      if (ok) ok = gc::tiles::wait(taken(buf), ((rows >> 1) & 1u) ^ 1u, abort_p);
-      // the list, while the row arrives
+      const int* cls = classes(buf);
+      float* prob = probs(buf);
+      const float* at_entry = at_entries(buf);
       Running x;
-      float tm = -INFINITY;
-      bool any = false;
-      for (int j = rank; j < kp; j += THREADS) {
-        Entry e{0.f, -1};
-        if (j < p.k) e = entry(p, r, j);
-        cls[j] = e.c;
-        prob[j] = e.t;
-        if (e.c >= 0) {
-          at_entry[j] = as_float(z[e.c]);
-          tm = fmaxf(tm, e.t), any = true;
-        }
-      }
       const float ends[2] = {rank < head ? as_float(z[rank]) : -INFINITY, rank < p.C - tail ? as_float(z[tail + rank]) : -INFINITY};
       for (int v = 0; v < vectors; v += kVectors) {
         if (ok) ok = gc::tiles::wait(full(slot), phase, abort_p);
         const uint4* seg = reinterpret_cast<const uint4*>(smem + slot * kBytes);
-        uint4 w[2];
+        uint4 w[kEach];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) w[u] = v + rank + u * THREADS < vectors ? seg[rank + u * THREADS] : nothing<T>();
-        x.raise(fmaxf(vec_max<T>(w[0]), vec_max<T>(w[1])), p.a);
+        for (int u = 0; u < kEach; ++u) w[u] = v + rank + u * THREADS < vectors ? seg[rank + u * THREADS] : nothing<T>();
+        x.raise(fmaxf(fmaxf(vec_max<T>(w[0]), vec_max<T>(w[1])), fmaxf(vec_max<T>(w[2]), vec_max<T>(w[3]))), p.a);
         const F2 scale = both(p.a);
         F2 sum = both(0.f);
         if (product_is_finite(x.base(), p.a)) {
           const F2 base = both(-x.base() * p.a);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int u = 0; u < kEach; ++u) {
             F2 f[Vec<T>::P];
             unpack<T>(w[u], f);
 #pragma unroll
@@ -507,7 +553,7 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
         } else {
           const F2 base = both(-x.base());
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int u = 0; u < kEach; ++u) {
             F2 f[Vec<T>::P];
             unpack<T>(w[u], f);
 #pragma unroll
@@ -522,12 +568,12 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
       x.raise(fmaxf(ends[0], ends[1]), p.a);
 #pragma unroll
       for (int i = 0; i < 2; ++i) x.s += exp2_approx((ends[i] - x.base()) * p.a);
-      float top[4] = {x.m, tm, any ? 1.f : 0.f, 0.f};
+      float top[1] = {x.m};
       reduce(top, [](float a, float b) { return fmaxf(a, b); });
-      const bool counts = top[2] > 0.f;
-      const float zm = top[0];
-      tm = top[1];
-      float sums[4] = {x.m == -INFINITY ? x.s : x.s * exp2_approx((x.m - zm) * p.a), 0.f, 0.f, 0.f};
+      if (ok) ok = gc::tiles::wait(listed(buf), (rows >> 1) & 1u, abort_p);
+      const bool counts = info[buf][2] > 0.f;
+      const float zm = top[0], tm = info[buf][3];
+      float sums[3] = {x.m == -INFINITY ? x.s : x.s * exp2_approx((x.m - zm) * p.a), 0.f, 0.f};
       for (int j = rank; counts && j < p.k; j += THREADS) {
         if (cls[j] < 0) continue;
         const float w = exp2_approx((prob[j] - tm) * p.a);
@@ -540,7 +586,7 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
       if (rank == 0) {
         stats[r] = counts ? Stats{zm, zl, tm, tl} : Stats{0.f, 0.f, 0.f, INFINITY};
         if (counts) loss += kLn2 * (sums[2] / sums[1] - tl + zl);
-        info[buf][0] = zm, info[buf][1] = zl, info[buf][2] = counts ? 1.f : 0.f;
+        info[buf][0] = zm, info[buf][1] = zl;
       }
       sync_threads<1, THREADS>();  // all of the list is written
       if (rank == 0) mbar_arrive(ready(buf));
@@ -571,15 +617,15 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
       for (int v = 0; v < vectors; v += kVectors) {
         if (ok) ok = gc::tiles::wait(full(slot), phase, abort_p);
         const uint4* seg = reinterpret_cast<const uint4*>(smem + slot * kBytes);
-        uint4 w[2];
+        uint4 w[kEach];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) w[u] = seg[rank + u * THREADS];  // (in a last segment's rest: what a row before left)
+        for (int u = 0; u < kEach; ++u) w[u] = seg[rank + u * THREADS];  // (in a last segment's rest: what a row before left)
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(slot));
         advance();
         if (!counts) continue;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < kEach; ++u) {
           const int i = v + rank + u * THREADS;
           F2 f[Vec<T>::P];
           unpack<T>(w[u], f);
@@ -612,7 +658,7 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
   if (threadIdx.x == 0 && abort_s) atomicExch(word, 1);
 }
 
-// G threads per row, or per part of one (G = kWide).  Rows are taken from the last to the first: the forward pass, which has mostly
+// G threads per row, or per part of one.  Rows are taken from the last to the first: the forward pass, which has mostly
 // just run, left the last ones in the L2.  `pad`: columns of zeros behind a row of dZ.
 template <class T, int G>
 __global__ void __launch_bounds__(G > 32 ? G : 256)
@@ -686,14 +732,14 @@ distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restri
 }
 
 // ------------------------------------------------------------------ host
-int threads_per_row(int64_t C, int64_t k) { return C > 4096 ? kWide : C <= 256 && k <= kShortList ? 8 : 32; }
+int threads_per_row(int64_t C, int64_t k) { return C > kMidTo ? kWide : C > 4096 ? kMid : C <= 256 && k <= kShortList ? 8 : 32; }
 // Whether one pass makes statistics and gradient: rows that both start as far behind a 16-byte boundary, enough of them, and of a length
 // that keeps the CTA's barriers small beside it.  Returns the CTA's computing threads, or 0.
 int one_pass_threads(const void* Z, int type, int64_t ldz, const void* dZ, int64_t lddz, int64_t M, int64_t C, int64_t k) {
   const int64_t size = type == GC_TYPE_F32 ? 4 : 2, bytes = C * size;
   const bool same = (reinterpret_cast<uintptr_t>(Z) - reinterpret_cast<uintptr_t>(dZ)) % 16 == 0 && (ldz - lddz) * size % 16 == 0;
   if (!same || M < gc::kNumSMs || k > kOnePassList) return 0;
-  return bytes < kOnePassFrom || bytes > Ring<kLong>::kMostBytes ? 0 : bytes <= Ring<kShort>::kMostBytes ? kShort : kLong;
+  return bytes <= kOnePassFrom || bytes > Ring<kLong>::kMostBytes ? 0 : bytes <= Ring<kShort>::kMostBytes ? kShort : kLong;
 }
 // Rows above 8192 columns of which there are fewer than SMs are cut, into parts of 4096 or more.
 int parts_of(int64_t M, int64_t C) {
@@ -721,9 +767,10 @@ int fill(Problem& p, const char* what, const void* Z, int type, int64_t ldz, con
   return GC_OK;
 }
 template <class F>
-void with_group(int G, F&& f) {
+void with_group(int G, bool parts, F&& f) {
   if (G == 8) f(std::integral_constant<int, 8>{});
   else if (G == 32) f(std::integral_constant<int, 32>{});
+  else if (G == kMid && !parts) f(std::integral_constant<int, kMid>{});
   else f(std::integral_constant<int, kWide>{});
 }
 template <class F>
@@ -773,7 +820,7 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
     int* word = nullptr;
     rc = gc::tiles::error_word(&word);
     if (rc != GC_OK) return rc;
-    const int smem = (whole == kLong ? Ring<kLong>::kSegments : Ring<kShort>::kSegments) * whole * 32 + 2 * kListWords * int((k + 3) / 4 * 4) * 4;
+    const int smem = kSegments * whole * kEach * 16 + 2 * kListWords * int((k + 3) / 4 * 4) * 4;
     const unsigned ctas = unsigned(std::min<int64_t>(M, gc::kNumSMs * (whole == kLong ? 1 : std::min(4, 222 * 1024 / (smem + 2048)))));
     with_type(type, [&](auto t) {
       using T = decltype(t);
@@ -783,7 +830,7 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) rc = gc::fail(GC_ERR_CUDA, "gc_distill_forward: %s", cudaGetErrorString(e));
         else
-          kern<<<ctas, 2 * kThreads + 32, smem, st>>>(p, reinterpret_cast<Stats*>(stats), partials, scale * temperature, static_cast<T*>(dZ), lddz,
+          kern<<<ctas, 2 * kThreads + 64, smem, st>>>(p, reinterpret_cast<Stats*>(stats), partials, scale * temperature, static_cast<T*>(dZ), lddz,
                                                   int(pad), word);
       };
       if (whole == kLong) run(std::integral_constant<int, kLong>{});
@@ -796,8 +843,8 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
   const unsigned grid = grid_of(M, G);
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    if (parts) distill_part_kernel<T><<<dim3(unsigned(p.parts), unsigned(M)), kWide, 0, st>>>(p, parts);
-    with_group(G, [&](auto gt) {
+    if (parts) distill_part_kernel<T><<<dim3(unsigned(p.parts), unsigned(M)), kPart, 0, st>>>(p, parts);
+    with_group(G, p.parts > 1, [&](auto gt) {
       constexpr int kG = decltype(gt)::value;
       distill_forward_kernel<T, kG><<<grid, kG > 32 ? kG : 256, 0, st>>>(p, parts, reinterpret_cast<Stats*>(stats), partials);
     });
@@ -816,7 +863,7 @@ int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, i
   if (M == 0) return GC_OK;
   GC_REQUIRE(stats && grad_loss && dZ, "gc_distill_backward: null pointer");
   GC_REQUIRE(gc::aligned16(stats), "gc_distill_backward: the statistics must be 16-byte aligned");
-  const int G = threads_per_row(C, k);
+  const int G = p.parts > 1 ? kWide : threads_per_row(C, k);
   const int rows = G > 32 ? 1 : 256 / G, kp = int((k + 3) / 4 * 4);
   const size_t smem = size_t(rows) * 2 * kp * 4;
   // where dZ is mostly there already, as many CTAs as run at one time
@@ -824,7 +871,7 @@ int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, i
   int bad = GC_OK;
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    with_group(G, [&](auto gt) {
+    with_group(G, p.parts > 1, [&](auto gt) {
       constexpr int kG = decltype(gt)::value;
       auto kern = distill_backward_kernel<T, kG>;
       if (smem > 48 * 1024) {

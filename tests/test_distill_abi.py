@@ -51,7 +51,7 @@ def test_which_rows_go_in_one_pass():
 
     assert one(16, 0, 8192, 8192, 1000, 8192) and one(16, 1, 90_001, 90_001, 1000, 90_001)
     assert not one(16, 0, 47, 47, 100_000, 47)       # short rows
-    assert not one(16, 0, 50_000, 50_000, 1000, 50_000) and not one(16, 1, 100_000, 100_000, 1000, 100_000)  # longer than the ring
+    assert not one(16, 0, 50_689, 50_689, 1000, 50_689) and not one(16, 1, 101_377, 101_377, 1000, 101_377)  # longer than the ring
     assert not one(16, 0, 8192, 8192, 100, 8192)     # few rows
     assert not one(20, 0, 8192, 8192, 1000, 8192) and not one(16, 0, 8193, 8192, 1000, 8192)  # the rows lie differently
     assert not one(16, 2, 8192, 8192, 1000, 8192) and not one(16, 0, 8192, 8192, 1000, 8192, 257)

@@ -70,7 +70,7 @@ SIZES = [(1, 1, 1), (1, 2, 1), (3, 2, 2), (5, 7, 3), (33, 47, 8), (100, 256, 32)
          (130, 31, 31), (3, 4096, 64), (5, 4097, 1024), (2, 200_001, 50), (1, 8193, 7), (147, 12_345, 10), (149, 12_345, 10),
          (300, 5000, 10), (2708, 7, 3),
          # one pass: in rings of short segments and of long ones, rows of whole segments and not, up to the ring's length
-         (148, 4096, 5), (700, 4099, 40), (601, 12_288, 3), (200, 24_576, 100), (149, 24_577, 256), (310, 49_920, 64), (150, 99_840, 12), (150, 99_841, 12)]
+         (148, 4096, 5), (700, 4099, 40), (601, 12_288, 3), (200, 18_432, 100), (149, 18_433, 256), (310, 50_688, 64), (150, 101_376, 12), (150, 101_377, 12)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
