@@ -38,7 +38,7 @@ SOURCES = [
     "gcn_layer.cu",
     "graph_build.cu",
     "loss.cu", "distill.cu", "optim.cu",
-    "norm.cu", "adamw.cu", "ffn.cu", "ffn_rows.cu", "int4.cu", "grouped.cu",
+    "norm.cu", "adamw.cu", "ffn.cu", "ffn_rows.cu", "int4.cu", "int4_tiles.cu", "grouped.cu",
 ]
 
 HOSTSRC = os.path.join(CSRC, "host")

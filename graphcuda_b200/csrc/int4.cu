@@ -2,8 +2,8 @@
 //
 //   W[k, n] = (code[k, n] - zero[k / group, n]) * scale[k / group, n]      codes 0 to 15, zero 8 where none is given, scale bf16
 //
-// Up to 32 rows (16 in the block) every code is read once and the time is that of reading them.  A warp turns 16 outputs x 32 inputs of codes into
-// the bf16 operand of mma.sync -- code - zero is a whole number below 16 and exact there -- multiplies it by up to 32 rows of X, and
+// Up to 16 rows (8 in the block) every code is read once and the time is that of reading them.  A warp turns 16 outputs x 32 inputs of codes into
+// the bf16 operand of mma.sync -- code - zero is a whole number below 16 and exact there -- multiplies it by up to 16 rows of X, and
 // adds the fp32 sums of a group times its scale to the outputs' fp32 sums: no weight is ever rounded.  (The 5th-generation tensor
 // core takes its operands from shared memory and TMEM, through which every unpacked weight would have to go first; a
 // product that waits for memory gains nothing from its rate.)
@@ -16,129 +16,24 @@
 // two launches goes as two bf16 numbers, hi and lo, in twice the rows of X; the second launch starts while the first runs, and its
 // first codes are in registers when it has ended.
 //
-// More rows than that: the weights are unpacked once into bf16 in the workspace (rounded: 2^-9 at most, as an operand of the tensor
-// cores has to be), 2.5 bytes of traffic per weight, and the tensor-core product of the gated block runs on them.
-#include "common.cuh"
-#include "ffn_internal.cuh"
-#include "tiles.cuh"
-
-#include <cuda_bf16.h>
+// One row of 8192 x 32,768 takes 38.8 us, 3.67 TB/s of codes and scales; of 2048 x 8192, whose floor is 1.4 us, 5.2, which are launch,
+// first fetch and the cluster's sum; 16 rows of 16,384 x 8192 with zero points 34.1 (floor 11.9), bound by unpacking: 151 instructions a warp
+// for 2048 codes at one row.  Loads into registers instead of rings took 10.2 and 89.5 us for the last two.
+//
+// Up to 128 rows (64 in the block): int4_tiles.cu.  More than that: the weights are unpacked once into bf16 in the workspace (rounded: 2^-9
+// at most, as an operand of the tensor cores has to be), 2.5 bytes of traffic per weight, and the tensor-core product of the gated block
+// runs on them.
+#include "int4_internal.cuh"
 
 #include <algorithm>
 
 namespace {
 
-using namespace gc::ffn;
-using namespace gc::tc;
-using gc::tiles::align256;
-using gc::tiles::drain;
-using gc::tiles::up8;
-using bf16 = __nv_bfloat16;
+using namespace gc::int4;
+using gc::int4::unpack;
 
 constexpr int kMostThreads = 256;
-constexpr int kChunk = 128;       // inputs of a chunk
-constexpr int kMostColumns = 32;  // rows of X (of hi and lo: twice) that a launch takes
-
-__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float peer_load(const float* p, uint32_t rank) {
-  uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(p)), there;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-  return v;
-}
-// c = A B, or c + A B.
-template <bool FIRST>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  float d[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) d[i] = FIRST ? 0.f : c[i];
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
-}
-// Waits for a copy, a bounded time (tries of a microsecond at most); the same answer for all of a warp.
-__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
-  uint32_t tries = 1u << 21;
-  bool done;
-  do {
-    uint32_t now;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(now)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    done = now != 0;
-  } while (!done && --tries);
-  return __all_sync(0xFFFFFFFFu, done);
-}
-// Eight codes as four pairs of bf16 numbers less their zero points; 0x4300 is 128 and its last bits count ones, and `zero` is a pair of
-// -(128 + zero point).  (A multiply-add, by one: a subtraction would go to the pipe of the shifts and masks, which is the busy one.)
-__device__ __forceinline__ void unpack(uint32_t w, __nv_bfloat162 zero, uint32_t (&o)[4]) {
-  const __nv_bfloat162 one = __float2bfloat162_rn(1.f);
-  uint32_t mask;
-  asm("mov.b32 %0, 0x000F000F;" : "=r"(mask));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t t;  // (w >> 4 i & mask) | 128s, in one instruction but for the shift: the mask waits in a register
-    asm("lop3.b32 %0, %1, %2, 0x43004300, 0xEA;" : "=r"(t) : "r"(w >> (4 * i)), "r"(mask));
-    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&t), one, zero);
-    o[i] = *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-__device__ __forceinline__ __nv_bfloat162 zero_pair(uint32_t zeros, int byte) {
-  const uint32_t t = __byte_perm(zeros, 0xC3u, 0x4040u + 0x0101u * byte);
-  return *reinterpret_cast<const __nv_bfloat162*>(&t);
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ uint4 shared_16(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 shared_8(uint32_t at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t shared_4(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t shared_2(uint32_t at) {
-  uint16_t v;
-  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t shared_1(uint32_t at) {
-  uint16_t v;
-  asm volatile("{\n\t.reg .u8 b;\n\tld.shared.u8 b, [%1];\n\tcvt.u16.u8 %0, b;\n\t}" : "=h"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float gated(float g, float u, int act) {
-  float a = 0.f, unused;
-  with_activation(act, [&](auto t) {
-    F2 slope;
-    activate<decltype(t)::value>(F2(g, g), slope).get(a, unused);
-  });
-  return a * u;
-}
-
-// A record: 64 bytes of codes for each of 16 outputs, their scales, their zero points.
-constexpr int kScales = 16 * 64;
 constexpr int kRun = 2;  // records that are fetched, waited for and given back together: of a block of outputs they follow each other
-__host__ __device__ constexpr int zeros_at(int gpc) { return kScales + 16 * gpc * 2; }
-__host__ __device__ constexpr int record_bytes(int gpc, bool zeros) { return zeros_at(gpc) + (zeros ? 16 * gpc : 0); }
 
 struct Params {
   const uint16_t* x;  // rows in 16-byte accesses, zeros up to the next multiple of 8 inputs
@@ -159,7 +54,7 @@ struct Params {
 // NT: 8 rows of X each.  MT: blocks of 16 outputs that a CTA takes at a time (GATED: the same ones of G and of U, whose outputs lie in two
 // blocks where SPLIT).  GPC: groups in a record.  ZEROS: whether records have zero points.
 template <int NT, int MT, bool GATED, bool SPLIT, int GPC, bool ZEROS>
-__global__ void __launch_bounds__(kMostThreads, NT == 1 ? (MT == 1 ? 3 : 2) : NT == 2 ? 2 : 1)
+__global__ void __launch_bounds__(kMostThreads, NT == 1 && MT == 1 ? 3 : 2)
 int4_rows_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) uint8_t shared[];  // sums of two turns, [warp][MT * 16][NT * 8]; barriers; rings
   constexpr int kCols = NT * 8, kOuts = MT * 16, kBlocks = 4 / GPC;  // kBlocks: 32s of inputs in a group
@@ -422,18 +317,11 @@ int4_unpack_kernel(const uint8_t* __restrict__ records, int zeros, int K, int N,
 }
 
 // ------------------------------------------------------------------ host
-struct Weights {
-  const uint8_t* records;
-  int group, zeros;
-  int gpc() const { return kChunk / group; }
-  int64_t bytes(int64_t K, int64_t N) const { return gc::ceil_div(N, 16) * gc::ceil_div(K, kChunk) * record_bytes(gpc(), zeros); }
-};
-
 template <int NT, int MT, bool GATED, bool SPLIT, int GPC, bool ZEROS>
 int launch_rows(Params p, cudaStream_t st) {
   const int64_t blocks = gc::ceil_div(p.N, GATED ? 16 : 16 * MT);
   const int runs = int(gc::ceil_div(gc::ceil_div(p.K, kChunk), kRun));
-  const int warps = runs >= 16 ? 8 : 4, per_sm = NT == 1 && MT == 1 ? 24 : NT <= 2 ? 16 : 8;
+  const int warps = runs >= 16 ? 8 : 4, per_sm = NT == 1 && MT == 1 ? 24 : 16;
   // All warps at once: outputs beyond those follow in the same CTAs.
   const int64_t slots = per_sm / warps * gc::kNumSMs;
   p.ctas = 1;
@@ -444,7 +332,7 @@ int launch_rows(Params p, cudaStream_t st) {
   const int64_t mine = gc::ceil_div(runs, p.ctas * warps) * gc::ceil_div(blocks, ctas);
   const int sums = 2 * warps * MT * 16 * NT * 8 * int(sizeof(float));
   const int room = (220 * 1024 / (per_sm / warps) - 1024 - 256 - sums) / warps;
-  static_assert((220 * 1024 / (NT == 1 && MT == 1 ? 6 : NT <= 2 ? 4 : 2) - 1280) / 4 - 2 * MT * 16 * NT * 8 * 4 >= kPlace + 8, "room for a place");
+  static_assert((220 * 1024 / (NT == 1 && MT == 1 ? 6 : 4) - 1280) / 4 - 2 * MT * 16 * NT * 8 * 4 >= kPlace + 8, "room for a place");
   p.ring = int(std::min<int64_t>({mine, 16, room / (kPlace + 8)}));
   const int smem = sums + (warps * p.ring * 8 + 127) / 128 * 128 + warps * p.ring * kPlace;
   auto kern = int4_rows_kernel<NT, MT, GATED, SPLIT, GPC, ZEROS>;
@@ -478,7 +366,6 @@ template <bool GATED, int GPC, bool ZEROS>
 int launch_for(const Params& p, cudaStream_t st) {
   auto sized = [&](auto split) {
     constexpr bool kSplit = decltype(split)::value;
-    if (p.rows > 16) return launch_rows<4, 2, GATED, kSplit, GPC, ZEROS>(p, st);
     if (p.rows > 8) return launch_rows<2, 2, GATED, kSplit, GPC, ZEROS>(p, st);
     if constexpr (!GATED)
       if (gc::ceil_div(p.N, 16) * gc::ceil_div(p.K, kChunk) < kWideFrom) return launch_rows<1, 1, GATED, kSplit, GPC, ZEROS>(p, st);
@@ -535,7 +422,7 @@ int zeros(uint16_t* Y, int64_t ldy, int64_t M, int64_t N, cudaStream_t st, const
   const cudaError_t e = cudaMemset2DAsync(Y, size_t(ldy) * 2, 0, size_t(N) * 2, size_t(M), st);
   return e == cudaSuccess ? GC_OK : gc::fail(GC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
-constexpr int64_t kLinearRows = kMostColumns, kBlockRows = kMostColumns / 2;
+constexpr int64_t kLinearRows = 16, kBlockRows = 8;  // in the block the hidden rows are twice as many
 
 }  // namespace
 
@@ -544,6 +431,7 @@ extern "C" {
 size_t gc_linear_int4_workspace_bytes(int64_t M, int64_t K, int64_t N) {
   if (M <= 0 || K <= 0 || N <= 0 || !sizes_ok(M, K, N)) return 0;
   if (M <= kLinearRows) return rows_bytes(M, K);
+  if (M <= kLinearTileRows) return linear_tiles_workspace(M, K, N);
   return unpacked_bytes(K, N) + gc::ffn::rows_workspace(M, K, N);
 }
 
@@ -573,6 +461,7 @@ int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* W, int gr
     p.K = int(K); p.N = int(N);
     return product<false>(w, p, st);
   }
+  if (M <= kLinearTileRows) return linear_tiles(X, ldx, w, M, K, N, Y, ldy, workspace, st);
   rc = unpack_to(w, K, N, workspace, st);
   if (rc != GC_OK) return rc;
   return gc::ffn::rows_times(X, ldx, static_cast<const uint16_t*>(workspace), up8(K), M, K, N, Y, ldy,
@@ -582,6 +471,7 @@ int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* W, int gr
 size_t gc_gated_ffn_int4_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O) {
   if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, std::max(D, H), O) || !sizes_ok(2 * H, 0, 0)) return 0;
   if (M <= kBlockRows) return rows_bytes(M, D) + rows_bytes(2 * M, H);
+  if (M <= kBlockTileRows) return block_tiles_workspace(M, D, H, O);
   return unpacked_bytes(D, 2 * H) + unpacked_bytes(H, O) + gc::ffn::block_workspace(M, D, H, O);
 }
 
@@ -625,6 +515,7 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, i
     q.wait = 1;
     return product<false>(out, q, st);
   }
+  if (M <= kBlockTileRows) return block_tiles(X, ldx, in, out, M, D, H, O, act, Y, ldy, workspace, st);
   uint16_t* w_in = reinterpret_cast<uint16_t*>(ws);
   uint16_t* w_out = reinterpret_cast<uint16_t*>(ws + unpacked_bytes(D, 2 * H));
   ws += unpacked_bytes(D, 2 * H) + unpacked_bytes(H, O);

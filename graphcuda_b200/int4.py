@@ -134,7 +134,7 @@ class _TracedBlock(torch.autograd.Function):
 def linear_int4(x: torch.Tensor, w: Int4Weight) -> torch.Tensor:
     """``x @ w``: ``x`` is bfloat16 [rows, in], the result bfloat16 [rows, out], sums are float32.
 
-    Up to 32 rows the weights' values enter unrounded, and only the result's rounding shows.  For more rows they are rounded to
+    Up to 128 rows the weights' values enter unrounded, and only the result's rounding shows.  For more rows they are rounded to
     bfloat16 on their way to the tensor cores, which adds as much again (2.4e-3 instead of 1.7e-3, relative, root mean square)."""
     y = _lib.host.linear_int4(x, *w._parts())
     return y if y is not None else _TracedLinear.apply(x, *w._parts())
@@ -144,8 +144,8 @@ def gated_ffn_int4(x: torch.Tensor, w_in: Int4Weight, w_out: Int4Weight, activat
     """``gated_ffn`` for serving with both weights in 4 bits: ``(act(x @ Wg) * (x @ Wu)) @ w_out`` with ``w_in = [Wg | Wu]``; ``x``
     and the result are bfloat16.
 
-    Up to 16 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
-    rounded to bfloat16 (4e-3 instead of 1.7e-3, relative, root mean square; the hidden row up to 64 rows not)."""
+    Up to 64 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
+    rounded to bfloat16 (4e-3 instead of 1.7e-3, relative, root mean square)."""
     act = _act(activation)
     y = _lib.host.gated_ffn_int4(x, *w_in._parts(), *w_out._parts(), act)
     return y if y is not None else _TracedBlock.apply(x, *w_in._parts(), *w_out._parts(), act)

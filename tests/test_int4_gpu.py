@@ -1,7 +1,7 @@
 """Products with weights of 4 bits against their formulas in 64 bits.
 
 Tolerances.  Sums are fp32, of which the tensor core's chain and the groups' together have at most in / 32 + 32 terms, each off by 2^-23
-of the sum of magnitudes.  The result's own rounding is half a step of bf16, 2^-8 of it.  Above 32 rows (16 in the block) a weight's rounding
+of the sum of magnitudes.  The result's own rounding is half a step of bf16, 2^-8 of it.  Above 128 rows (64 in the block) a weight's rounding
 is another 2^-8 of it at worst; in the block those of both weights and of the hidden row."""
 import pytest
 import torch
@@ -36,12 +36,12 @@ def check_linear(x, w):
     got = gc.linear_int4(x, w)
     assert got.shape == (x.size(0), w.out_features) and got.dtype == torch.bfloat16
     X, W = x.double(), w.dequantize().double()
-    slack = (X.abs() @ W.abs()) * ((w.in_features / 32 + 32) * 2.0 ** -23 + (HALF if x.size(0) > 32 else 0))
+    slack = (X.abs() @ W.abs()) * ((w.in_features / 32 + 32) * 2.0 ** -23 + (HALF if x.size(0) > 128 else 0))
     near(got, X @ W, slack + 1e-30)
     return got
 
 
-ROWS = [1, 2, 3, 8, 9, 16, 17, 32, 33, 64, 65, 200]
+ROWS = [1, 2, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 96, 97, 128, 129]
 
 
 @pytest.mark.parametrize("m", ROWS)
@@ -54,7 +54,7 @@ def test_linear(m, k, n):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("zeros", [False, True])
 def test_wide_layers(group, zeros):
-    for m, k, n in ((1, 2048, 8192), (5, 8192, 2050), (16, 16_384, 1024), (40, 1024, 9000), (1, 64, 40_000)):
+    for m, k, n in ((1, 2048, 8192), (5, 8192, 2050), (16, 16_384, 1024), (40, 1024, 9000), (120, 4096, 700), (1, 64, 40_000)):
         check_linear(rows(m, k), weight(k, n, group, zeros))
 
 
@@ -63,7 +63,7 @@ def test_zero_points_are_exact_however_large_the_inputs():
     w = gc.Int4Weight.from_codes(torch.full((256, 32), 11, dtype=torch.uint8, device=DEV),
                                  torch.ones(4, 32, dtype=torch.bfloat16, device=DEV),
                                  torch.full((4, 32), 11, dtype=torch.uint8, device=DEV), group=64)
-    for m in (1, 20, 100):
+    for m in (1, 20, 100, 300):
         x = rows(m, 256) * 1e30
         assert not gc.linear_int4(x, w).any()
 
@@ -84,8 +84,8 @@ def check_block(x, w_in, w_out, act):
     G, U = (X @ Wi).split(h, 1)
     a, slope = act64(act, G)
     hidden = a * U
-    many = m > 16
-    # of the first product, the activation (1e-5 of its input), the hidden row (16 bits, or a step of bf16 above 64 rows), the second
+    many = m > 64
+    # of the first product, the activation (1e-5 of its input), the hidden row (16 bits, or a step of bf16), the second
     first = (X.abs() @ Wi.abs()) * ((w_in.in_features / 32 + 32) * 2.0 ** -23 + (HALF if many else 0))
     eg, eu = first.split(h, 1)
     # slopes of the activations are below 1.13, and near g the one at g moves by at most 1.1 times the distance
@@ -117,16 +117,16 @@ def test_errors_on_average():
     one = HALF / 3 ** 0.5
     x, w = rows(2000, 512), weight(512, 256)
     want = x.double() @ w.dequantize().double()
-    assert rms(gc.linear_int4(x[:32], w), want[:32]) <= one and rms(gc.linear_int4(x, w), want) <= one * 2 ** 0.5
+    assert rms(gc.linear_int4(x[:128], w), want[:128]) <= one and rms(gc.linear_int4(x, w), want) <= one * 2 ** 0.5
     wi, wo = weight(512, 1024, 32), weight(512, 200, 32, seed=1)
-    for m, n in ((16, 1), (2000, 6.25)):  # result; and both halves of the first weight (1.5 for the slope), the second's, the hidden row's
+    for m, n in ((64, 1), (2000, 6.25)):  # result; and both halves of the first weight (1.5 for the slope), the second's, the hidden row's
         assert rms(*check_block(x[:m], wi, wo, "silu")) <= one * n ** 0.5
 
 
 def test_strides_and_alignment():
     for k in (48, 200, 333):
         w, wi, wo = weight(k, 40), weight(k, 48), weight(24, 30)
-        for m in (1, 6, 20, 90):
+        for m in (1, 6, 20, 90, 250):
             wide = torch.full((m, k + 9), torch.nan, device=DEV, dtype=torch.bfloat16)
             for off in (0, 1, 8, 9):
                 wide[:] = torch.nan
@@ -140,7 +140,7 @@ def test_strides_and_alignment():
 
 def test_what_is_no_number_stays_in_its_row():
     w, wi, wo = weight(200, 40, zeros=True), weight(200, 96), weight(48, 24)
-    for m in (3, 12, 100):
+    for m in (3, 12, 100, 250):
         x = rows(m, 200)
         fine_l, fine_b = gc.linear_int4(x, w), gc.gated_ffn_int4(x, wi, wo)
         for bad in (float("nan"), float("inf")):
@@ -156,7 +156,7 @@ def test_nothing_to_do():
     w = weight(64, 24)
     assert gc.linear_int4(rows(0, 64), w).shape == (0, 24)
     assert gc.linear_int4(rows(3, 64), weight(64, 0)).shape == (3, 0)
-    for m in (3, 100):
+    for m in (3, 20, 300):
         none = gc.linear_int4(rows(m, 0), weight(0, 24))
         assert none.shape == (m, 24) and not none.any()
         assert not gc.gated_ffn_int4(rows(m, 0), weight(0, 48), weight(24, 8)).any()
@@ -166,7 +166,7 @@ def test_nothing_to_do():
 
 def test_same_bits_every_time_and_in_any_company():
     w, wi, wo = weight(3000, 700), weight(3000, 1000), weight(500, 260)
-    for m in (1, 8, 64, 300):
+    for m in (1, 8, 64, 100, 300):
         x = rows(m, 3000)
         for f in (lambda t: gc.linear_int4(t, w), lambda t: gc.gated_ffn_int4(t, wi, wo)):
             first = f(x)
@@ -197,7 +197,7 @@ def test_refusals():
         gc.gated_ffn_int4(x.clone().requires_grad_(), w, weight(24, 8))
 
 
-@pytest.mark.parametrize("m", [1, 20, 100])
+@pytest.mark.parametrize("m", [1, 20, 100, 300])
 def test_recorded_in_a_graph_and_on_another_stream(m):
     x, w, wi, wo = rows(m, 1000), weight(1000, 300), weight(1000, 512), weight(256, 130)
     calls = (lambda t: gc.linear_int4(t, w), lambda t: gc.gated_ffn_int4(t, wi, wo))
