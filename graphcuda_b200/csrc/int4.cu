@@ -360,7 +360,8 @@ int launch_rows(Params p, cudaStream_t st) {
   cudaLaunchKernelEx(&cfg, kern, p);
   return gc::check_launch("int4_rows_kernel");
 }
-// Records from which on a warp takes two blocks of outputs at a time, with half of the instructions around them.
+// Records from which on a warp takes two blocks of outputs at a time, with half of the instructions around them: a row of 4096 x 8192 takes
+// 8.3 us so and 9.0 with one block, 8192 x 32,768 38.1 and 39.9; 2048 x 8192 5.6 and 5.1, for it is short of warps.
 constexpr int64_t kWideFrom = 16384;
 template <bool GATED, int GPC, bool ZEROS>
 int launch_for(const Params& p, cudaStream_t st) {

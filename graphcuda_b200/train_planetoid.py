@@ -10,7 +10,9 @@ launch, test() is GCN.evaluate (fused argmax / accuracy counts), and ``--graph``
 one CUDA graph.  ``--optimizer adam`` gives the Adam lr 0.01 configuration this library is benchmarked on.
 
 Beyond the script, a deep model: ``--layers 8 --hidden 64 --optimizer adamw [--state-bits 8] [--serve]`` trains
-models.ResidualGCN (norms, gated feed-forward blocks) with FusedAdamW; ``--serve`` evaluates it in 8 bits at the end.
+models.ResidualGCN (norms, gated feed-forward blocks) with FusedAdamW; ``--serve`` evaluates it in 8 bits at the end, or in
+4 with ``--serve-bits 4``.  ``--distill 16`` then trains a 2-layer GCN of that width on the answers of the trained model, for
+every vertex and without labels (distill_loss), with Adam and as many epochs.
 """
 from __future__ import annotations
 
@@ -33,7 +35,10 @@ def main(argv=None) -> dict:
     ap.add_argument("--lr", type=float, default=None,
                     help="default: 1 for sgd (the script's value), 0.01 for adam, 0.003 for adamw")
     ap.add_argument("--state-bits", type=int, choices=[8, 32], default=32, help="of the moments that adamw keeps")
-    ap.add_argument("--serve", action="store_true", help="with --layers: evaluate in 8 bits at the end")
+    ap.add_argument("--serve", action="store_true", help="with --layers: evaluate in few bits at the end")
+    ap.add_argument("--serve-bits", type=int, choices=[8, 4], default=8, help="of the feed-forward weights with --serve")
+    ap.add_argument("--distill", type=int, default=None, metavar="HIDDEN", help="train a 2-layer GCN on the model's answers at the end")
+    ap.add_argument("--temperature", type=float, default=2.0, help="of the answers with --distill")
     ap.add_argument("--seed", type=int, default=None)
     ap.add_argument("--graph", action="store_true", help="record the train step once and replay it as a CUDA graph")
     ap.add_argument("--precision", default=None)
@@ -79,7 +84,7 @@ def main(argv=None) -> dict:
         opt.step()
         return loss
 
-    def test():
+    def test(model=model):
         model.eval()
         _, counts = model.evaluate(data.x, adj, data.y, masks)
         c = counts.cpu()
@@ -112,13 +117,38 @@ def main(argv=None) -> dict:
               f"Train Acc: {accs[0]:.4f} | Val Acc: {accs[1]:.4f} | Test Acc: {accs[2]:.4f}")
     if args.serve:
         model.eval()
-        _, counts = model.for_serving().evaluate(data.x, adj, data.y, masks)
-        served = [int(a) / max(int(b), 1) for a, b in counts.cpu()]
-        print(f"Served in 8 bits | Train Acc: {served[0]:.4f} | Val Acc: {served[1]:.4f} | Test Acc: {served[2]:.4f}")
+        served = test(model.for_serving(args.serve_bits))
+        print(f"Served in {args.serve_bits} bits | Train Acc: {served[0]:.4f} | Val Acc: {served[1]:.4f} | Test Acc: {served[2]:.4f}")
         history.append(dict(epoch=args.epochs, served=True, train=served[0], val=served[1], test=served[2]))
+    if args.distill is not None:
+        history += _distill(model.eval(), args, data, adj, device, test)
     print(f"\nTotal training time for {args.epochs} epochs: {total:.4f} seconds")
     print(f"Average time per epoch (train): {total / max(args.epochs, 1):.6f} seconds")
     return dict(history=history, seconds=total)
+
+
+def _distill(teacher, args, data, adj, device, test) -> list:
+    import graphcuda_b200 as gc
+    from graphcuda_b200.models import GCN
+
+    with torch.no_grad():
+        top, index = teacher(data.x, adj, log_softmax=False).topk(min(data.num_classes, 1024))
+    student = GCN([data.num_node_features, args.distill, data.num_classes], precision=args.precision).to(device)
+    opt = gc.FusedAdam(student.parameters(), lr=0.01)
+    lines = []
+    for epoch in range(1, args.epochs + 1):
+        student.train()
+        opt.zero_grad(set_to_none=True)
+        loss = gc.distill_loss(student(data.x, adj, log_softmax=False), top, index, temperature=args.temperature)
+        loss.backward()
+        opt.step()
+        loss_value = loss.item()
+        ops.check_gemm_flag(data.x.device)
+        accs = test(student)
+        lines.append(dict(epoch=epoch, distilled=True, loss=loss_value, train=accs[0], val=accs[1], test=accs[2]))
+        print(f"Distilled epoch {epoch:03d} | Loss: {loss_value:.4f} | "
+              f"Train Acc: {accs[0]:.4f} | Val Acc: {accs[1]:.4f} | Test Acc: {accs[2]:.4f}")
+    return lines
 
 
 if __name__ == "__main__":
