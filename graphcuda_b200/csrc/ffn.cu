@@ -98,6 +98,9 @@ struct Params {
   int8_t* exps;     // G's and U's exponents, [2][ceil(N / 32)][M] (Gated: null where G and U are not stored)
   const float* sa;  // e4m3: scales of A's rows and B's columns
   const float* sb;
+  const int* ea;  // H16: exponents of A's rows, B's columns, and (Gated) of the rows that are stored
+  const int* eb;
+  const int* eh;
   bf16* C;  // Plain: the output, for rows that TMA cannot store; else what the rounding of A, or of dG | dU, left; or null
   int64_t ldc;
   int tma_store, parts;  // parts: Plain stores fp32 parts
@@ -171,6 +174,18 @@ __device__ __forceinline__ F2 unpack_fp16(uint32_t w, F2 scale) {
   return F2(f.x, f.y) * scale;
 }
 
+__device__ __forceinline__ uint32_t pack2_fp16(F2 a) {
+  float x, y;
+  a.get(x, y);
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }  // of two, -126 to 127
+// A float times 2^e, in two steps: e may be -252 to 254.
+__device__ __forceinline__ uint32_t times_power(uint32_t v, int e) {
+  return __float_as_uint(__uint_as_float(v) * power(e / 2) * power(e - e / 2));
+}
+
 // Where a column of the product goes (see Params); one that is dropped goes beyond the last.
 __device__ __forceinline__ int out_column(int n, int gap_from, int gap) {
   return n < gap_from ? n : n < gap_from + gap ? 0x7FFFFFFF : n - gap;
@@ -186,8 +201,8 @@ struct Maps {
 
 // A_MN / B_MN: the operand is MN-major.  F8: e4m3 operands (K-major).  PAIR: two CTAs of a cluster work on a tile of 256 rows,
 // each with its 128 rows of A and half of B's (Gated: rank 0 has G's columns, rank 1 U's).  RES: see Cfg.  LO: what roundings left is
-// stored too.
-template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES, bool LO>
+// stored too.  H16: operands are fp16 numbers, rows of A and columns of B times powers of two, and so is what Gated stores.
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES, bool LO, bool H16>
 __global__ void __launch_bounds__(kThreads, 1)
 ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C_ = Cfg<KIND, BN, F8, PAIR, RES>;
@@ -196,6 +211,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
   constexpr int TM = PAIR ? 2 * BM : BM;
   constexpr int NT = KIND == kGated ? BN / 2 : BN;  // output columns of a tile
   static_assert(!F8 || (!A_MN && !B_MN && KIND == kGated), "e4m3 operands are K-major");
+  static_assert(!H16 || (!F8 && !A_MN && !B_MN && KIND != kGatedBack && !LO), "fp16 operands are K-major");
   static_assert(!RES || (!A_MN && KIND != kPlain), "A is held K-major, for short products");
   const uint32_t rank = PAIR ? cluster_rank() : 0;
   const int unit = PAIR ? int(blockIdx.x / 2) : int(blockIdx.x), units = PAIR ? int(gridDim.x / 2) : int(gridDim.x);
@@ -373,7 +389,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = make_idesc(TM, BN, A_MN, B_MN, F8);
+      constexpr uint32_t idesc = make_idesc(TM, BN, A_MN, B_MN, F8 || H16);
       constexpr uint32_t kAStep = A_MN ? 16 * 128 : 32, kBStep = B_MN ? 16 * 128 : 32;  // bytes per MMA
       const uint64_t da0 = operand_desc(RES ? sHeld(0) : sA(0), A_MN), db0 = operand_desc(sB(0), B_MN);
       uint32_t s = 0, phase = 0, rows = 0;
@@ -479,6 +495,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
         tmem_ld_wait();
         if (c + kEpiGroups >= NT / 32 || n0 + (c + kEpiGroups) * 32 >= p.N) release();
       };
+      const int ea = H16 ? __ldg(p.ea + min(row, p.M - 1)) : 0;
       for (int c = grp; c < NT / 32; c += kEpiGroups) {
         const int col = n0 + c * 32;
         if (col >= p.N || row0 >= p.M) break;
@@ -540,6 +557,19 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
         } else if constexpr (KIND == kGated) {
           const float sa = F8 ? p.sa[min(row, p.M - 1)] : 1.f;
           const uint32_t scales = staging + C_::kStaging - C_::kScaleBytes + (warp - 4) * 256;
+          float fg = 1.f, fu = 1.f;  // H16
+          int eg = 0, eu = 0;
+          bool alike = true;
+          if (H16) {
+            const int n = min(col + lane, p.N - 1), eh = __ldg(p.eh + min(row, p.M - 1));
+            eg = __ldg(p.eb + n), eu = __ldg(p.eb + p.b_up + n);
+            // |G| stays below 2^96, so that what U times 2^-eh loses below 2^-126 is nothing beside 2^-24, the last bit of what is stored
+            const int sg = ea + eg, su = ea + eu - eh;
+            const int eg0 = __shfl_sync(0xFFFFFFFFu, eg, 0), eu0 = __shfl_sync(0xFFFFFFFFu, eu, 0);
+            alike = __all_sync(0xFFFFFFFFu, eg == eg0 && eu == eu0 && -126 <= sg && sg <= 40 && -126 <= su && su <= 127);
+            if (alike) fg = power(sg), fu = power(su);
+            else fu = power(-eh);
+          }
           if (F8) {
             const int n = min(col + lane, p.N - 1);
             asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + 4 * lane), "f"(__ldg(p.sb + n)) : "memory");
@@ -549,7 +579,14 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           tmem_ld32(acc_at, g);
           tmem_ld32(acc_at + uint32_t(NT), u);
           loaded(c);
-          if (!F8 && p.exps) {
+          if (H16 && !alike) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              g[i] = times_power(g[i], ea + __shfl_sync(0xFFFFFFFFu, eg, i));
+              u[i] = times_power(u[i], ea + __shfl_sync(0xFFFFFFFFu, eu, i));
+            }
+          }
+          if (!F8 && !H16 && p.exps) {
             const int64_t at = int64_t(col / 32) * p.M + row;
             if (col + 32 > p.N) {  // what lies beyond has no say in the exponents
 #pragma unroll
@@ -583,8 +620,9 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
                 const int i = j * 8 + 2 * e;
                 F2 vg(g[i], g[i + 1]), vu(u[i], u[i + 1]), unused;
                 if (F8) vg = vg * (both(sa) * sg[e]), vu = vu * (both(sa) * su[e]);
+                if (H16) vg = vg * both(fg), vu = vu * both(fu);
                 const F2 a = activate<decltype(act)::value>(vg, unused) * vu;
-                w[e] = pack2(a);
+                w[e] = H16 ? pack2_fp16(a) : pack2(a);
                 if (LO) rest[e] = pack_rest(a, w[e]);
               }
               if (LO && row < p.M && col + 8 * j < p.N)
@@ -595,8 +633,21 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           put(&maps.out, bo, col, row0);
         } else {
           uint32_t acc[32];
+          int eb = 0;
+          if (H16) eb = __ldg(p.eb + min(col + lane, p.N - 1));
           tmem_ld32(acc_at, acc);
           loaded(c);
+          if (H16) {
+            const int e = ea + eb;
+            const int eb0 = __shfl_sync(0xFFFFFFFFu, eb, 0);
+            if (__all_sync(0xFFFFFFFFu, eb == eb0 && -126 <= e && e <= 127)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) acc[i] = __float_as_uint(__uint_as_float(acc[i]) * power(e));
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) acc[i] = times_power(acc[i], ea + __shfl_sync(0xFFFFFFFFu, eb, i));
+            }
+          }
           if (p.parts) {
             // fp32 parts, 16 columns to a tile
 #pragma unroll
@@ -725,10 +776,10 @@ size_t plain_workspace(int64_t M, int64_t N, int64_t K, int64_t halves = 1) {
   return s.splits > 1 || halves > 1 ? align256(size_t(s.splits) * size_t(M) * size_t(part_pitch(N)) * 4) : 0;
 }
 
-template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES, bool LO = false>
+template <int KIND, int BN, bool A_MN, bool B_MN, bool F8, bool PAIR, bool RES, bool LO = false, bool H16 = false>
 int launch_kernel(const Maps& maps, const Params& p, cudaStream_t st) {
   using C_ = Cfg<KIND, BN, F8, PAIR, RES>;
-  auto kern = ffn_kernel<KIND, BN, A_MN, B_MN, F8, PAIR, RES, LO>;
+  auto kern = ffn_kernel<KIND, BN, A_MN, B_MN, F8, PAIR, RES, LO, H16>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C_::kSmemBytes);
   if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   constexpr int kCtas = PAIR ? 2 : 1;
@@ -769,6 +820,17 @@ int launch_tile(const Tile& t, const Maps& maps, const Params& p, cudaStream_t s
   return width(std::false_type{});
 }
 
+template <int KIND>
+int launch_tile_fp16(const Tile& t, const Maps& maps, const Params& p, cudaStream_t st) {
+  if constexpr (KIND == kGated) {
+    if (t.pair && gc::ceil_div(p.K, 64) <= kResident) return launch_kernel<KIND, 256, false, false, false, true, true, false, true>(maps, p, st);
+  }
+  if (t.pair) return launch_kernel<KIND, 256, false, false, false, true, false, false, true>(maps, p, st);
+  if constexpr (KIND != kGated)
+    if (t.bn == 64) return launch_kernel<KIND, 64, false, false, false, false, false, false, true>(maps, p, st);
+  return launch_kernel<KIND, 128, false, false, false, false, false, false, true>(maps, p, st);
+}
+
 // The maps of the operands.  A and B: matrices as they lie; K-major ones have K in their rows.
 int operand_maps(Maps& maps, Params& p, const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int b_rows) {
   const int ke = 128 / A.size;  // K elements of a stage
@@ -781,9 +843,11 @@ int operand_maps(Maps& maps, Params& p, const Matrix& A, bool a_mn, const Matrix
   return rc;
 }
 
-// C (M x N, bf16) = A B, fp32 sums; `halves`: A has that many times M rows, and M apart are added.
+// C (M x N, bf16) = A B, fp32 sums; `halves`: A has that many times M rows, and M apart are added.  ea, eb: operands are fp16, with
+// exponents.
 int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int64_t N, int64_t K, bf16* C, int64_t ldc,
-          int64_t gap_from, int64_t gap, void* workspace, cudaStream_t st, int64_t halves = 1) {
+          int64_t gap_from, int64_t gap, void* workspace, cudaStream_t st, int64_t halves = 1, const int* ea = nullptr,
+          const int* eb = nullptr) {
   if (M == 0 || N == 0) return GC_OK;
   const int64_t out_rows = M;
   M *= halves;
@@ -795,6 +859,7 @@ int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int
   p.gap_from = gap ? int(gap_from) : int(N);
   p.gap = int(gap);
   p.c_cols = int(N - 2 * gap);  // [G | U] with the pads behind both
+  p.ea = ea; p.eb = eb;
   p.splits = s.splits; p.kb_per_split = s.per;
   p.parts = s.splits > 1 || halves > 1;
   p.tma_store = gap == 0 && ldc % 8 == 0 && gc::aligned16(C);
@@ -804,7 +869,8 @@ int plain(const Matrix& A, bool a_mn, const Matrix& B, bool b_mn, int64_t M, int
   if (rc == GC_OK && p.parts) rc = make_map(&maps.out, Matrix{workspace, M, N, pitch, 4}, 16, 32, s.splits);
   else if (rc == GC_OK && p.tma_store) rc = make_map(&maps.out, Matrix{C, M, N, ldc, 2}, 32, 32);
   if (rc != GC_OK) return rc;
-  if (a_mn) rc = launch_tile<kPlain, true, true, false>(s.tile, maps, p, st);
+  if (ea) rc = launch_tile_fp16<kPlain>(s.tile, maps, p, st);
+  else if (a_mn) rc = launch_tile<kPlain, true, true, false>(s.tile, maps, p, st);
   else if (b_mn) rc = launch_tile<kPlain, false, true, false>(s.tile, maps, p, st);
   else rc = launch_tile<kPlain, false, false, false>(s.tile, maps, p, st);
   if (rc != GC_OK || !p.parts) return rc;
@@ -894,36 +960,25 @@ int rows_times(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, i
   return plain(x, false, Matrix{W, N, K, ldw, 2}, false, M, N, K, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
 }
 
-size_t block_workspace(int64_t M, int64_t D, int64_t H, int64_t O) {
-  const int64_t halves = stack(M);
-  return align256(size_t(M) * up8(D) * 2) + hidden_bytes(M, up8(H)) + plain_workspace(M, O, H, halves);
-}
-int block_times(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin, const uint16_t* Wout, int64_t ldwout, int64_t M,
-                int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace, cudaStream_t st) {
-  char* ws = static_cast<char*>(workspace);
-  Matrix x{X, M, D, ldx, 2};
-  Copies copies{};
-  make_readable(x, ws, copies);
-  int rc = run_copies(copies, st);
-  if (rc != GC_OK) return rc;
-  const int64_t hp = up8(H), halves = stack(M);
-  uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);
-  ws += hidden_bytes(M, hp);
+size_t block_fp16_workspace(int64_t M, int64_t, int64_t H, int64_t O) { return align256(size_t(M) * up8(H) * 2) + plain_workspace(M, O, H); }
+int block_fp16(const BlockFp16& b, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace,
+               cudaStream_t st) {
+  const int64_t hp = up8(H);
+  uint16_t* hidden = static_cast<uint16_t*>(workspace);
   const Tile t = pick_tile(kGated, M, H, 1);
   Maps maps;
   Params p{};
   p.M = int(M); p.N = int(H); p.K = int(D);
   p.b_up = int(H);  // rows of Win: no alignment to keep
   p.act = act;
-  p.C = halves > 1 ? reinterpret_cast<bf16*>(hidden) + M * hp : nullptr;
-  p.ldc = hp;
-  rc = error_word(&p.word);
-  if (rc == GC_OK) rc = operand_maps(maps, p, x, false, Matrix{Win, 2 * H, D, ldwin, 2}, false, t.bn / 2);
+  p.ea = b.ex; p.eb = b.ein; p.eh = b.eh;
+  int rc = error_word(&p.word);
+  if (rc == GC_OK) rc = operand_maps(maps, p, Matrix{b.x, M, D, up8(D), 2}, false, Matrix{b.w_in, 2 * H, D, up8(D), 2}, false, t.bn / 2);
   if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 32, 32);
-  if (rc == GC_OK) rc = launch_tile<kGated, false, false, false>(t, maps, p, st);
+  if (rc == GC_OK) rc = launch_tile_fp16<kGated>(t, maps, p, st);
   if (rc != GC_OK) return rc;
-  return plain(Matrix{hidden, halves * M, H, hp, 2}, false, Matrix{Wout, O, H, ldwout, 2}, false, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0,
-               0, ws, st, halves);
+  return plain(Matrix{hidden, M, H, hp, 2}, false, Matrix{b.w_out, O, H, hp, 2}, false, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0,
+               static_cast<char*>(workspace) + align256(size_t(M) * hp * 2), st, 1, b.eh, b.eout);
 }
 
 }  // namespace ffn

@@ -134,14 +134,21 @@ struct Rows {
 };
 int forward_few_rows(const Rows& r, bool e4m3, cudaStream_t st);
 
-// On the tensor cores, with weights whose inputs run along their rows (16-byte aligned ones): Y (M x N) = X W^T with W N x K, and the
-// block with Win 2H x D and Wout O x H.  All bf16; X and Y may lie as they like.
+// On the tensor cores, with weights whose inputs run along their rows (16-byte aligned ones): Y (M x N) = X W^T with W N x K, all
+// bf16; X and Y may lie as they like.
 size_t rows_workspace(int64_t M, int64_t K, int64_t N);
 int rows_times(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, int64_t M, int64_t K, int64_t N, uint16_t* Y,
                int64_t ldy, void* workspace, cudaStream_t st);
-size_t block_workspace(int64_t M, int64_t D, int64_t H, int64_t O);
-int block_times(const uint16_t* X, int64_t ldx, const uint16_t* Win, int64_t ldwin, const uint16_t* Wout, int64_t ldwout, int64_t M,
-                int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace, cudaStream_t st);
+// The block with fp16 operands that are so times powers of two (exponents -126 to 127): X row by row, the weights output by output, and
+// the hidden row, whose exponents have to bring it below 2^16.  X is M x D, Win 2H x D, Wout O x H, all of them in rows that
+// are a multiple of 8 long; Y is bf16.
+struct BlockFp16 {
+  const uint16_t *x, *w_in, *w_out;
+  const int *ex, *eh, *ein, *eout;  // value = stored * 2^exponent
+};
+size_t block_fp16_workspace(int64_t M, int64_t D, int64_t H, int64_t O);
+int block_fp16(const BlockFp16& b, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace,
+               cudaStream_t st);
 
 }  // namespace ffn
 }  // namespace gc

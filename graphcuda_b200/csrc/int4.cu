@@ -20,10 +20,16 @@
 // first fetch and the cluster's sum; 16 rows of 16,384 x 8192 with zero points 34.1 (floor 11.9), bound by unpacking: 151 instructions a warp
 // for 2048 codes at one row.  Loads into registers instead of rings took 10.2 and 89.5 us for the last two.
 //
-// Up to 128 rows (64 in the block): int4_tiles.cu.  More than that: the weights are unpacked once into bf16 in the workspace (rounded: 2^-9
-// at most, as an operand of the tensor cores has to be), 2.5 bytes of traffic per weight, and the tensor-core product of the gated block
-// runs on them.
+// Up to 128 rows (64 in the block): int4_tiles.cu.  More than that: the weights are unpacked once into the workspace, 2.5 bytes of traffic per
+// weight, and the tensor-core products of the gated block run on them.  For Y = X W they are bf16 (rounded: 2^-9 of a weight at most, as
+// much as the result's own rounding).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-12,
+// with a power of two per output, row of X and hidden row that keeps fp16's range from mattering; X is copied into fp16, exactly.  A
+// hidden row's power comes from a bound, |x|^2 |w|^2, beside which 2^-24 is the last bit that is kept: less than fp32 sums keep of G and U.
+// 169,343 rows through 256, 1024 and 256 take 283 us (bf16 took 243, with twice the error of a plain form in fp32): 40 for X, 6 for
+// the weights, 158 for the first product and 79 for the second.
 #include "int4_internal.cuh"
+
+#include <cuda_fp16.h>
 
 #include <algorithm>
 
@@ -316,6 +322,155 @@ int4_unpack_kernel(const uint8_t* __restrict__ records, int zeros, int K, int N,
   }
 }
 
+// The exponent whose power of two brings numbers up to `most` below 2^14, and half of that at least; not so small that a power is no fp32
+// number.
+__device__ __forceinline__ int fp16_exponent(float most) { return max(int(__float_as_uint(most) >> 23) - 127 - 13, -100); }
+
+// Weights as fp16, every output's times a power of two, an output's inputs in a row.  A CTA takes a part of 16 outputs' chunks.  Exponents
+// are multiples of 16: the outputs of a layer mostly share one, which the products' epilogues apply in a multiplication, and the largest weight
+// is 2^-2 at least, of which the last bit of fp16 is 2^-22.
+struct ToFp16 {
+  const uint8_t* records;
+  uint16_t* w;
+  int* exps;
+  int* largest;  // of 16 outputs, a power of two's exponent: every weight is below it
+  int64_t ldw;
+  int zeros, K, N, gpc, parts;
+};
+__device__ __forceinline__ int common_exponent(int e) { return min((e + 111) / 16 * 16 - 96, 115); }  // from -100 to 115: one as large at least
+__global__ void __launch_bounds__(256)
+int4_unpack_fp16_kernel(const ToFp16 first, const ToFp16 second, int ctas_of_first) {
+  __shared__ uint32_t most_s[16];
+  const bool is_first = int(blockIdx.x) < ctas_of_first;
+  const ToFp16& p = is_first ? first : second;
+  const int cta = is_first ? blockIdx.x : blockIdx.x - ctas_of_first, block = cta / p.parts, part = cta % p.parts;
+  const int zeros = p.zeros, K = p.K, N = p.N, gpc = p.gpc;
+  const int chunks = (K + kChunk - 1) / kChunk, size = record_bytes(gpc, zeros != 0);
+  const uint8_t* r = p.records + int64_t(block) * chunks * size;
+  if (threadIdx.x < 16) most_s[threadIdx.x] = 0;
+  __syncthreads();
+  const int out = threadIdx.x / 16, piece = threadIdx.x % 16, j = piece / 4, t = piece % 4;  // output, of 16; 8 inputs of a chunk
+  const bool exists = block * 16 + out < N;
+  uint32_t most = 0;  // as a float's bits
+  for (int c = piece; c < chunks && exists; c += 16)
+    for (int g = 0; g < gpc && c * kChunk + g * (kChunk / gpc) < K; ++g)
+      most = max(most, gc::ffn::finite_bits(uint32_t(__ldg(reinterpret_cast<const uint16_t*>(r + int64_t(c) * size + kScales) + out * gpc + g)) << 16));
+  atomicMax(&most_s[out], most);
+  __syncthreads();
+  const int e = common_exponent(fp16_exponent(__uint_as_float(most_s[out]) * 15.f));  // codes less zero points: -15 to 15
+  const float f = __uint_as_float(uint32_t(127 - e) << 23);
+  if (part == 0 && piece == 0) {
+    if (exists) p.exps[block * 16 + out] = e;
+    if (out == 0) {
+      uint32_t all = 0;
+      for (int i = 0; i < 16; ++i) all = max(all, most_s[i]);
+      p.largest[block] = fp16_exponent(__uint_as_float(all) * 15.f) + 14;
+    }
+  }
+  const int from = int(int64_t(chunks) * part / p.parts), to = int(int64_t(chunks) * (part + 1) / p.parts);
+  for (int c = from; c < to; ++c) {
+    const int k = c * kChunk + piece * 8;
+    if (k >= K || !exists) continue;
+    const uint8_t* at = r + int64_t(c) * size;
+    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(at + out * 64 + t * 16) + j);
+    const int group = out * gpc + j * gpc / 4;
+    const float s = __uint_as_float(uint32_t(__ldg(reinterpret_cast<const uint16_t*>(at + kScales) + group)) << 16) * f;
+    uint32_t o[4];
+    unpack(word, zero_pair(zeros ? __ldg(at + zeros_at(gpc) + group) : 8, 0), o);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const __half2 v = __floats2half2_rn(s * __uint_as_float(o[q] << 16), s * __uint_as_float(o[q] & 0xFFFF0000u));
+      o[q] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    *reinterpret_cast<uint4*>(p.w + (int64_t(block) * 16 + out) * p.ldw + k) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// X as fp16, every row times a power of two, zeros up to a multiple of 8; a warp per row.  eh: for the block's hidden row, of which |x| and the
+// weights' largest powers (`blocks` of them) give a bound: |act(G)| <= |G|, |G|, |U| <= |x| |w| <= |x| sqrt(K) 2^largest.
+__global__ void __launch_bounds__(256)
+int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K, int vec, const int* __restrict__ largest, int blocks,
+                      uint16_t* __restrict__ out, int64_t ldo, int* __restrict__ exps, int* __restrict__ eh) {
+  __shared__ int most_s[8];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int top = -1000;
+  for (int i = threadIdx.x; i < blocks; i += 256) top = max(top, __ldg(largest + i));
+  top = __reduce_max_sync(0xFFFFFFFFu, top);
+  if (lane == 0) most_s[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, most_s[i]);
+  const int log_k = 32 - __clz(K);  // 2^log_k > K
+  const int64_t step = int64_t(gridDim.x) * 8;
+  uint4 following = make_uint4(0, 0, 0, 0);  // the first 256 inputs of a row are on their way while the one before is written
+  for (int64_t m = int64_t(blockIdx.x) * 8 + warp - step; m < M; m += step) {
+    auto load_of = [&](const uint16_t* row, int k) {
+      if (vec && k + 8 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+      uint32_t w[4] = {};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k + e < K) w[e / 2] |= uint32_t(row[k + e]) << (e % 2 * 16);
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto load = [&](int k) { return load_of(x + m * ldx, k); };
+    const uint4 first = following;
+    if (m + step < M && lane * 8 < K) following = load_of(x + (m + step) * ldx, lane * 8);
+    if (m < 0) continue;
+    __nv_bfloat162 tops = __float2bfloat162_rn(0.f);
+    for (int k = lane * 8; k < K; k += 256) {
+      const uint4 v = k < 256 ? first : load(k);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // a NaN is passed over
+        const uint32_t a = w[q] & 0x7FFF7FFFu;
+        tops = __hmax2(tops, *reinterpret_cast<const __nv_bfloat162*>(&a));
+      }
+    }
+    const uint32_t both_tops = *reinterpret_cast<const uint32_t*>(&tops);
+    uint32_t most = __reduce_max_sync(0xFFFFFFFFu, max(both_tops << 16, both_tops & 0xFFFF0000u));
+    if (most == 0x7F800000u) {  // an infinity has no say in its row's exponent either
+      most = 0;
+      for (int k = lane * 8; k < K; k += 256) {
+        const uint4 v = load(k);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) most = max(most, max(gc::ffn::finite_bits(w[q] << 16), gc::ffn::finite_bits(w[q] & 0xFFFF0000u)));
+      }
+      most = __reduce_max_sync(0xFFFFFFFFu, most);
+    }
+    const int e = fp16_exponent(__uint_as_float(most));
+    const F2 f = gc::ffn::both(__uint_as_float(uint32_t(127 - e) << 23));
+    F2 squares2(0.f, 0.f);
+    for (int k = lane * 8; k < K; k += 256) {
+      const uint4 v = k < 256 ? first : load(k);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      uint32_t o[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const F2 v2 = F2(w[q] << 16, w[q] & 0xFFFF0000u) * f;
+        squares2 = gc::ffn::fma2(v2, v2, squares2);
+        float a, b;
+        v2.get(a, b);
+        const __half2 h = __floats2half2_rn(a, b);
+        o[q] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      *reinterpret_cast<uint4*>(out + m * ldo + k) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    float squares, odd;
+    squares2.get(squares, odd);
+    squares += odd;
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) squares += __shfl_xor_sync(0xFFFFFFFFu, squares, d);
+    if (lane == 0) {
+      exps[m] = e;
+      if (!isfinite(squares)) squares = 0x1p28f * float(K);  // of what is finite: below 2^14 each
+      // squares < 2^log2s; the hidden row stays below 2^15
+      const int log2s = int(__float_as_uint(squares) >> 23) - 127 + 1;
+      eh[m] = squares > 0.f ? min(max(2 * e + log2s + log_k + 2 * top - 15, -100), 112) : 0;
+    }
+  }
+}
+
 // ------------------------------------------------------------------ host
 template <int NT, int MT, bool GATED, bool SPLIT, int GPC, bool ZEROS>
 int launch_rows(Params p, cudaStream_t st) {
@@ -407,7 +562,37 @@ int unpack_to(const Weights& w, int64_t K, int64_t N, void* to, cudaStream_t st)
       w.records, w.zeros, int(K), int(N), w.gpc(), static_cast<uint16_t*>(to), up8(K));
   return gc::check_launch("int4_unpack_kernel");
 }
+ToFp16 to_fp16(const Weights& w, int64_t K, int64_t N, uint16_t* to, int* exps, int* largest) {
+  const int64_t parts = std::min(gc::ceil_div(K, kChunk), gc::ceil_div(gc::kNumSMs * 8, gc::ceil_div(N, 16)));
+  return ToFp16{w.records, to, exps, largest, up8(K), w.zeros, int(K), int(N), w.gpc(), int(parts)};
+}
 size_t unpacked_bytes(int64_t K, int64_t N) { return align256(size_t(N) * up8(K) * 2); }
+
+// The block's operands in the workspace, and what follows them.
+struct Unpacked {
+  uint16_t *x, *w_in, *w_out;
+  int *ex, *eh, *ein, *eout, *largest;
+  void* rest;
+  size_t bytes;
+};
+Unpacked unpacked_block(char* ws, int64_t M, int64_t D, int64_t H, int64_t O) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char* p = ws ? ws + at : nullptr;
+    at += align256(bytes);
+    return static_cast<void*>(p);
+  };
+  auto ints = [&](int64_t n) { return static_cast<int*>(take(size_t(n) * 4)); };
+  Unpacked u;
+  u.x = static_cast<uint16_t*>(take(size_t(M) * up8(D) * 2));
+  u.w_in = static_cast<uint16_t*>(take(unpacked_bytes(D, 2 * H)));
+  u.w_out = static_cast<uint16_t*>(take(unpacked_bytes(H, O)));
+  u.ex = ints(M), u.eh = ints(M), u.ein = ints(2 * H), u.eout = ints(O);
+  u.largest = ints(gc::ceil_div(2 * H, 16) + gc::ceil_div(O, 16));
+  u.rest = ws ? ws + at : nullptr;
+  u.bytes = at;
+  return u;
+}
 
 bool sizes_ok(int64_t M, int64_t K, int64_t N) {
   const int64_t top = (int64_t(1) << 30) - 512;  // coordinates are 32-bit
@@ -473,7 +658,7 @@ size_t gc_gated_ffn_int4_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_
   if (M <= 0 || D <= 0 || H <= 0 || O <= 0 || !sizes_ok(M, std::max(D, H), O) || !sizes_ok(2 * H, 0, 0)) return 0;
   if (M <= kBlockRows) return rows_bytes(M, D) + rows_bytes(2 * M, H);
   if (M <= kBlockTileRows) return block_tiles_workspace(M, D, H, O);
-  return unpacked_bytes(D, 2 * H) + unpacked_bytes(H, O) + gc::ffn::block_workspace(M, D, H, O);
+  return unpacked_block(nullptr, M, D, H, O).bytes + gc::ffn::block_fp16_workspace(M, D, H, O);
 }
 
 int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, int group_in, int zero_points_in, const uint8_t* Wout,
@@ -517,13 +702,17 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, i
     return product<false>(out, q, st);
   }
   if (M <= kBlockTileRows) return block_tiles(X, ldx, in, out, M, D, H, O, act, Y, ldy, workspace, st);
-  uint16_t* w_in = reinterpret_cast<uint16_t*>(ws);
-  uint16_t* w_out = reinterpret_cast<uint16_t*>(ws + unpacked_bytes(D, 2 * H));
-  ws += unpacked_bytes(D, 2 * H) + unpacked_bytes(H, O);
-  rc = unpack_to(in, D, 2 * H, w_in, st);
-  if (rc == GC_OK) rc = unpack_to(out, H, O, w_out, st);
+  const Unpacked u = unpacked_block(ws, M, D, H, O);
+  const ToFp16 a = to_fp16(in, D, 2 * H, u.w_in, u.ein, u.largest), b = to_fp16(out, H, O, u.w_out, u.eout, u.largest + gc::ceil_div(2 * H, 16));
+  const int64_t ctas = gc::ceil_div(2 * H, 16) * a.parts;
+  int4_unpack_fp16_kernel<<<unsigned(ctas + gc::ceil_div(O, 16) * b.parts), 256, 0, st>>>(a, b, int(ctas));
+  rc = gc::check_launch("int4_unpack_fp16_kernel");
   if (rc != GC_OK) return rc;
-  return gc::ffn::block_times(X, ldx, w_in, up8(D), w_out, up8(H), M, D, H, O, act, Y, ldy, ws, st);
+  int4_rows_fp16_kernel<<<unsigned(std::min<int64_t>(gc::ceil_div(M, 8), gc::kNumSMs * 8)), 256, 0, st>>>(
+      X, ldx, int(M), int(D), gc::aligned16(X) && ldx % 8 == 0, u.largest, int(gc::ceil_div(2 * H, 16)), u.x, up8(D), u.ex, u.eh);
+  rc = gc::check_launch("int4_rows_fp16_kernel");
+  if (rc != GC_OK) return rc;
+  return gc::ffn::block_fp16(gc::ffn::BlockFp16{u.x, u.w_in, u.w_out, u.ex, u.eh, u.ein, u.eout}, M, D, H, O, act, Y, ldy, u.rest, st);
 }
 
 }  // extern "C"

@@ -145,7 +145,7 @@ def gated_ffn_int4(x: torch.Tensor, w_in: Int4Weight, w_out: Int4Weight, activat
     and the result are bfloat16.
 
     Up to 64 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
-    rounded to bfloat16 (4e-3 instead of 1.7e-3, relative, root mean square)."""
+    rounded to 11 bits, an eighth of the result's own rounding."""
     act = _act(activation)
     y = _lib.host.gated_ffn_int4(x, *w_in._parts(), *w_out._parts(), act)
     return y if y is not None else _TracedBlock.apply(x, *w_in._parts(), *w_out._parts(), act)

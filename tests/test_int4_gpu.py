@@ -1,8 +1,9 @@
 """Products with weights of 4 bits against their formulas in 64 bits.
 
 Tolerances.  Sums are fp32, of which the tensor core's chain and the groups' together have at most in / 32 + 32 terms, each off by 2^-23
-of the sum of magnitudes.  The result's own rounding is half a step of bf16, 2^-8 of it.  Above 128 rows (64 in the block) a weight's rounding
-is another 2^-8 of it at worst; in the block those of both weights and of the hidden row."""
+of the sum of magnitudes.  The result's own rounding is half a step of bf16, 2^-8 of it.  Above 128 rows a weight's rounding
+is another 2^-8 of it at worst; in the block above 64 rows those of both weights and of the hidden row, to fp16, are 2^-11, and what
+fp16 cannot hold of a hidden row beside its bound."""
 import pytest
 import torch
 
@@ -84,14 +85,18 @@ def check_block(x, w_in, w_out, act):
     G, U = (X @ Wi).split(h, 1)
     a, slope = act64(act, G)
     hidden = a * U
-    many = m > 64
-    # of the first product, the activation (1e-5 of its input), the hidden row (16 bits, or a step of bf16), the second
-    first = (X.abs() @ Wi.abs()) * ((w_in.in_features / 32 + 32) * 2.0 ** -23 + (HALF if many else 0))
+    many = 2.0 ** -11 if m > 64 else 0
+    # of the first product, the activation (1e-5 of its input), the hidden row (16 bits, or a step of fp16), the second
+    first = (X.abs() @ Wi.abs()) * ((w_in.in_features / 32 + 32) * 2.0 ** -23 + many)
     eg, eu = first.split(h, 1)
     # slopes of the activations are below 1.13, and near g the one at g moves by at most 1.1 times the distance
     dh = (slope.abs() + 1.1 * eg) * eg * U.abs() + a.abs() * eu + eg * eu * 1.13 + 1e-5 * G.abs() * U.abs()
-    dh += (hidden.abs() + dh) * (HALF if m > 64 else 2.0 ** -16)
-    second = (hidden.abs() @ Wo.abs()) * ((h / 32 + 32) * 2.0 ** -23 + (HALF if many else 0))
+    dh += (hidden.abs() + dh) * (many or 2.0 ** -16)
+    if many:  # half of fp16's smallest number, 2^-25, where 2^15 stands for the bound: |x|^2 D w^2 in powers of two, 15 steps of the largest scale for w
+        dh += 2.0 ** -31 * X.square().sum(1, keepdim=True) * w_in.in_features * Wi.abs().max() ** 2
+        # the bound is 2^-85 at least, so that 2^-24 of fp16 stands for 2^-124; the hidden row's own range, fp32's, ends at 2^-126
+        dh += 2.0 ** -124
+    second = (hidden.abs() @ Wo.abs()) * ((h / 32 + 32) * 2.0 ** -23 + many)
     near(got, hidden @ Wo, second + dh @ Wo.abs() * (1 + HALF) + 1e-30)
     return got, hidden @ Wo
 
@@ -119,7 +124,7 @@ def test_errors_on_average():
     want = x.double() @ w.dequantize().double()
     assert rms(gc.linear_int4(x[:128], w), want[:128]) <= one and rms(gc.linear_int4(x, w), want) <= one * 2 ** 0.5
     wi, wo = weight(512, 1024, 32), weight(512, 200, 32, seed=1)
-    for m, n in ((64, 1), (2000, 6.25)):  # result; and both halves of the first weight (1.5 for the slope), the second's, the hidden row's
+    for m, n in ((64, 1), (2000, 1.09)):  # result; and both halves of the first weight (1.5 for the slope), the second's, the hidden row's, an eighth each
         assert rms(*check_block(x[:m], wi, wo, "silu")) <= one * n ** 0.5
 
 
@@ -254,3 +259,15 @@ def test_a_model_served_in_4_bits():
     assert float((got - want).norm() / want.norm()) <= 2e-2
     pred, counts = served.evaluate(x, adj, torch.zeros(n, dtype=torch.int64, device=DEV))
     assert torch.equal(pred, got.argmax(1)) and int(counts[0, 1]) == n
+
+
+@pytest.mark.parametrize("x_size,in_size,out_size", [(1e-30, 1.0, 1.0), (1e18, 1e-18, 1.0), (1e-20, 1e12, 1e25), (1e10, 1e-25, 1e20), (1e30, 1e-25, 1e-5)])
+def test_block_over_the_range_of_its_types(x_size, in_size, out_size):
+    # rows, outputs and groups of very different sizes: many rows go through fp16 with exponents of their own
+    torch.manual_seed(5)
+    def sized(k, n, size):
+        codes = torch.randint(0, 16, (k, n), dtype=torch.uint8, device=DEV)
+        scale = size * 2.0 ** torch.randint(-6, 7, (1, n), device=DEV) * (0.5 + torch.rand(k // 32, n, device=DEV))
+        return gc.Int4Weight.from_codes(codes, scale.bfloat16(), torch.randint(0, 16, scale.shape, dtype=torch.uint8, device=DEV), group=32)
+    x = (torch.randn(150, 96, device=DEV) * x_size * 2.0 ** torch.randint(-20, 1, (150, 1), device=DEV)).bfloat16()
+    check_block(x, sized(96, 2 * 64, in_size), sized(64, 40, out_size), "relu")
