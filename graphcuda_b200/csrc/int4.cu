@@ -17,12 +17,13 @@
 // first codes are in registers when it has ended.
 //
 // One row of 8192 x 32,768 takes 38.8 us, 3.67 TB/s of codes and scales; of 2048 x 8192, whose floor is 1.4 us, 5.2, which are launch,
-// first fetch and the cluster's sum; 16 rows of 16,384 x 8192 with zero points 34.1 (floor 11.9), bound by unpacking: 151 instructions a warp
-// for 2048 codes at one row.  Loads into registers instead of rings took 10.2 and 89.5 us for the last two.
+// first fetch and the cluster's sum; 16 rows of 16,384 x 8192 with zero points 34.1 (floor 11.9), where unpacking (151 instructions a warp for
+// 2048 codes at one row) takes half of the issue slots and warps wait for X, twice as many bytes from the L2 as codes; the next chunk's X in
+// registers ahead spills (47.6).  Loads into registers instead of rings took 10.2 and 89.5 us for the last two.
 //
 // Up to 128 rows (64 in the block): int4_tiles.cu.  More than that: the weights are unpacked once into the workspace, 2.5 bytes of traffic per
-// weight, and the tensor-core products of the gated block run on them.  For Y = X W they are bf16 (rounded: 2^-9 of a weight at most, as
-// much as the result's own rounding).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-12,
+// weight, and the tensor-core products of the gated block run on them.  For Y = X W they are bf16 (rounded: 2^-8 of a weight at most, as
+// much as the result's own rounding).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-11,
 // with a power of two per output, row of X and hidden row that keeps fp16's range from mattering; X is copied into fp16, exactly.  A
 // hidden row's power comes from a bound, |x|^2 |w|^2, beside which 2^-24 is the last bit that is kept: less than fp32 sums keep of G and U.
 // 169,343 rows through 256, 1024 and 256 take 283 us (bf16 took 243, with twice the error of a plain form in fp32): 40 for X, 6 for
@@ -133,7 +134,6 @@ int4_rows_kernel(const __grid_constant__ Params p) {
     if (all || c * kChunk + j * 32 + t * 8 < p.K) return __ldg(reinterpret_cast<const uint4*>(x_at[n] + c * kChunk + j * 32));
     return make_uint4(0, 0, 0, 0);
   };
-  constexpr bool kWhole = NT <= 2;  // X of a chunk at once
 
   if (GATED) {
     let_next_begin();
@@ -160,19 +160,17 @@ int4_rows_kernel(const __grid_constant__ Params p) {
         const int c = c0 + u;
         if (u > 0 && c >= chunks) break;
         const bool all = (c + 1) * kChunk <= p.K;
-        uint4 xs[NT][kWhole ? 4 : 1];
-        if constexpr (kWhole) {
-          if (all) {
+        uint4 xs[NT][4];
+        if (all) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) xs[n][j] = fetch_x(n, c, j, true);
-          } else {
+            for (int j = 0; j < 4; ++j) xs[n][j] = fetch_x(n, c, j, true);
+        } else {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) xs[n][j] = fetch_x(n, c, j, false);
-          }
+            for (int j = 0; j < 4; ++j) xs[n][j] = fetch_x(n, c, j, false);
         }
         if (u == 0 && ok) ok = arrived(bar, parity);
         uint4 codes[MT][2];
@@ -193,10 +191,6 @@ int4_rows_kernel(const __grid_constant__ Params p) {
           }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // 32 inputs
-          if constexpr (!kWhole)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) xs[n][0] = fetch_x(n, c, j, all);
-          auto x = [&](int n) { return xs[n][kWhole ? j : 0]; };
           uint32_t a[MT][2][4];
 #pragma unroll
           for (int m = 0; m < MT; ++m)
@@ -206,9 +200,10 @@ int4_rows_kernel(const __grid_constant__ Params p) {
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              if (j % kBlocks == 0) mma<true>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x(n).x, x(n).y);
-              else mma<false>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x(n).x, x(n).y);
-              mma<false>(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], x(n).z, x(n).w);
+              const uint4 x = xs[n][j];
+              if (j % kBlocks == 0) mma<true>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x.x, x.y);
+              else mma<false>(acc[m][n], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], x.x, x.y);
+              mma<false>(acc[m][n], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], x.z, x.w);
             }
           if (j % kBlocks == kBlocks - 1) {
 #pragma unroll
