@@ -46,7 +46,7 @@ struct Cfg {
   static constexpr int kStages = std::min(8, (227 * 1024 - 1024 - 512 - kStaging) / kStageBytes);
   static constexpr int kSmemBytes = kStages * kStageBytes + kStaging + 512 /*barriers*/ + 1024 /*alignment*/;
   static constexpr uint32_t kTmemCols = 2 * BN;
-  static_assert(kSmemBytes <= 227 * 1024 && kStages >= 2 && kTmemCols <= 512, "budget");
+  static_assert(kSmemBytes <= 227 * 1024 && kStages >= 2 && kTmemCols <= 512, "shared memory and TMEM");
 };
 
 struct Params {

@@ -41,20 +41,24 @@ class Int4Weight(torch.nn.Module):
             if what is not None and what.numel() and int(what.max()) > 15:
                 raise RuntimeError("Int4Weight: codes and zero points are 0 to 15")
         blocks, chunks, per = -(-n // 16), -(-k // _CHUNK), _CHUNK // group
-        q = codes.new_zeros(blocks * 16, chunks * _CHUNK)
-        q[:n, :k] = codes.t()
-        # outputs: block, half, row; inputs: chunk, 32s, lane, and the four codes of either half of a lane's word
-        q = q.view(blocks, 2, 8, chunks, 4, 4, 4, 2)
-        q = q.permute(0, 3, 1, 2, 5, 4, 7, 6).reshape(blocks, chunks, 16, 4, 4, 8)
-        q = (q[..., 0::2] | q[..., 1::2] << 4).reshape(blocks, chunks, 1024)
+        if k % _CHUNK or n % 16:
+            codes = torch.nn.functional.pad(codes, (0, blocks * 16 - n, 0, chunks * _CHUNK - k))
+        # inputs: chunk, 32s, lane, and the four codes of either half of a lane's word, two to a byte; outputs: block, row
+        q = codes.reshape(chunks, 4, 4, 2, 2, 2, blocks, 16)
+        q = q[:, :, :, :, 0] | q[:, :, :, :, 1] << 4
+        records = codes.new_empty(blocks, chunks, 1024 + 16 * per * (2 if zero is None else 3))
+        records[..., :1024].view(blocks, chunks, 16, 4, 4, 2, 2).copy_(q.permute(5, 0, 6, 2, 1, 4, 3))
 
-        def laid(t):
+        def lay(t, at):
             s = t.new_zeros(blocks * 16, chunks * per)
             s[:n, :groups] = t.t()
-            return s.view(blocks, 16, chunks, per).transpose(1, 2).contiguous().view(blocks, chunks, 16 * per).view(torch.uint8)
+            s = s.view(blocks, 16, chunks, per).transpose(1, 2).contiguous().view(blocks, chunks, 16 * per).view(torch.uint8)
+            records[..., at:at + s.size(2)] = s
 
-        parts = [q, laid(scale)] + ([] if zero is None else [laid(zero)])
-        return Int4Weight(torch.cat(parts, 2).contiguous(), zero is not None, k, n, group)
+        lay(scale, 1024)
+        if zero is not None:
+            lay(zero, 1024 + 32 * per)
+        return Int4Weight(records, zero is not None, k, n, group)
 
     def dequantize(self) -> torch.Tensor:
         """The weights' values, float32 [in, out]."""
