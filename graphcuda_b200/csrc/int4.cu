@@ -26,8 +26,8 @@
 // much as the result's own rounding).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-11,
 // with a power of two per output, row of X and hidden row that keeps fp16's range from mattering; X is copied into fp16, exactly.  A
 // hidden row's power comes from a bound, |x|^2 |w|^2, beside which 2^-24 is the last bit that is kept: less than fp32 sums keep of G and U.
-// 169,343 rows through 256, 1024 and 256 take 283 us (bf16 took 243, with twice the error of a plain form in fp32): 40 for X, 6 for
-// the weights, 158 for the first product and 79 for the second.
+// 169,343 rows through 256, 1024 and 256 take 275 us (bf16 took 243, with twice the error of a plain form in fp32): 34 for X, 6 for
+// the weights, 150 for the first product and 77 for the second.
 #include "int4_internal.cuh"
 
 #include <cuda_fp16.h>
@@ -382,7 +382,11 @@ int4_unpack_fp16_kernel(const ToFp16 first, const ToFp16 second, int ctas_of_fir
 }
 
 // X as fp16, every row times a power of two, zeros up to a multiple of 8; a warp per row.  eh: for the block's hidden row, of which |x| and the
-// weights' largest powers (`blocks` of them) give a bound: |act(G)| <= |G|, |G|, |U| <= |x| |w| <= |x| sqrt(K) 2^largest.
+// weights' largest powers (`blocks` of them) give a bound: |act(G)| <= |G|, |G|, |U| <= |x| |w| <= |x| sqrt(K) 2^largest.  (|x|^2 in its turn
+// is taken for 32 times the largest of the lanes' sums of squares, one instruction instead of ten.)
+// SHORT: rows of up to 256 inputs in 16-byte accesses, each a load and a store.  169,343 rows of 256 take 34 us so, and 40 with the loops
+// that other rows need.
+template <bool SHORT>
 __global__ void __launch_bounds__(256)
 int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K, int vec, const int* __restrict__ largest, int blocks,
                       uint16_t* __restrict__ out, int64_t ldo, int* __restrict__ exps, int* __restrict__ eh) {
@@ -400,7 +404,7 @@ int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
   uint4 following = make_uint4(0, 0, 0, 0);  // the first 256 inputs of a row are on their way while the one before is written
   for (int64_t m = int64_t(blockIdx.x) * 8 + warp - step; m < M; m += step) {
     auto load_of = [&](const uint16_t* row, int k) {
-      if (vec && k + 8 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+      if (SHORT || (vec && k + 8 <= K)) return __ldg(reinterpret_cast<const uint4*>(row + k));
       uint32_t w[4] = {};
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -412,8 +416,8 @@ int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
     if (m + step < M && lane * 8 < K) following = load_of(x + (m + step) * ldx, lane * 8);
     if (m < 0) continue;
     __nv_bfloat162 tops = __float2bfloat162_rn(0.f);
-    for (int k = lane * 8; k < K; k += 256) {
-      const uint4 v = k < 256 ? first : load(k);
+    for (int k = lane * 8; k < K; k += SHORT ? 1 << 30 : 256) {
+      const uint4 v = SHORT || k < 256 ? first : load(k);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {  // a NaN is passed over
@@ -436,8 +440,8 @@ int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
     const int e = fp16_exponent(__uint_as_float(most));
     const F2 f = gc::ffn::both(__uint_as_float(uint32_t(127 - e) << 23));
     F2 squares2(0.f, 0.f);
-    for (int k = lane * 8; k < K; k += 256) {
-      const uint4 v = k < 256 ? first : load(k);
+    for (int k = lane * 8; k < K; k += SHORT ? 1 << 30 : 256) {
+      const uint4 v = SHORT || k < 256 ? first : load(k);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       uint32_t o[4];
 #pragma unroll
@@ -454,11 +458,11 @@ int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
     float squares, odd;
     squares2.get(squares, odd);
     squares += odd;
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) squares += __shfl_xor_sync(0xFFFFFFFFu, squares, d);
+    const bool finite = squares < INFINITY;  // which a NaN is not either
+    squares = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, finite ? __float_as_uint(squares) : 0x7F800000u));
     if (lane == 0) {
       exps[m] = e;
-      if (!isfinite(squares)) squares = 0x1p28f * float(K);  // of what is finite: below 2^14 each
+      squares = squares < INFINITY ? 32.f * squares : 0x1p28f * float(K);  // of what is finite: below 2^14 each
       // squares < 2^log2s; the hidden row stays below 2^15
       const int log2s = int(__float_as_uint(squares) >> 23) - 127 + 1;
       eh[m] = squares > 0.f ? min(max(2 * e + log2s + log_k + 2 * top - 15, -100), 112) : 0;
@@ -703,8 +707,10 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, i
   int4_unpack_fp16_kernel<<<unsigned(ctas + gc::ceil_div(O, 16) * b.parts), 256, 0, st>>>(a, b, int(ctas));
   rc = gc::check_launch("int4_unpack_fp16_kernel");
   if (rc != GC_OK) return rc;
-  int4_rows_fp16_kernel<<<unsigned(std::min<int64_t>(gc::ceil_div(M, 8), gc::kNumSMs * 8)), 256, 0, st>>>(
-      X, ldx, int(M), int(D), gc::aligned16(X) && ldx % 8 == 0, u.largest, int(gc::ceil_div(2 * H, 16)), u.x, up8(D), u.ex, u.eh);
+  const bool vec = gc::aligned16(X) && ldx % 8 == 0;
+  auto rows = vec && D <= 256 && D % 8 == 0 ? int4_rows_fp16_kernel<true> : int4_rows_fp16_kernel<false>;
+  rows<<<unsigned(std::min<int64_t>(gc::ceil_div(M, 8), gc::kNumSMs * 8)), 256, 0, st>>>(
+      X, ldx, int(M), int(D), vec, u.largest, int(gc::ceil_div(2 * H, 16)), u.x, up8(D), u.ex, u.eh);
   rc = gc::check_launch("int4_rows_fp16_kernel");
   if (rc != GC_OK) return rc;
   return gc::ffn::block_fp16(gc::ffn::BlockFp16{u.x, u.w_in, u.w_out, u.ex, u.eh, u.ein, u.eout}, M, D, H, O, act, Y, ldy, u.rest, st);

@@ -92,8 +92,8 @@ def check_block(x, w_in, w_out, act):
     # slopes of the activations are below 1.13, and near g the one at g moves by at most 1.1 times the distance
     dh = (slope.abs() + 1.1 * eg) * eg * U.abs() + a.abs() * eu + eg * eu * 1.13 + 1e-5 * G.abs() * U.abs()
     dh += (hidden.abs() + dh) * (many or 2.0 ** -16)
-    if many:  # half of fp16's smallest number, 2^-25, where 2^15 stands for the bound: |x|^2 D w^2 in powers of two, 15 steps of the largest scale for w
-        dh += 2.0 ** -31 * X.square().sum(1, keepdim=True) * w_in.in_features * Wi.abs().max() ** 2
+    if many:  # half of fp16's smallest number, 2^-25, where 2^15 stands for the bound: |x|^2 D w^2 in powers of two (x by up to 32 more), 15 steps of the largest scale for w
+        dh += 2.0 ** -26 * X.square().sum(1, keepdim=True) * w_in.in_features * Wi.abs().max() ** 2
         # the bound is 2^-85 at least, so that 2^-24 of fp16 stands for 2^-124; the hidden row's own range, fp32's, ends at 2^-126
         dh += 2.0 ** -124
     second = (hidden.abs() @ Wo.abs()) * ((h / 32 + 32) * 2.0 ** -23 + many)
