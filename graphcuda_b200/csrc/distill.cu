@@ -12,7 +12,8 @@
 // With a gradient to be asked for, rows of some thousands of classes are read once in all (one_pass): a CTA streams rows through a ring of
 // segments in shared memory; one half of its threads goes over a row's segments as they arrive for its statistics, the other
 // over the same segments again for dZ, giving them back to the copies of the next row.  That is dZ for g = 1, which is what a loss that is differentiated by
-// itself has; the backward call looks at g and, where it is another, computes dZ from the logits as it does for other rows.
+// itself has; the backward call looks at g and, where it is another, computes dZ from the logits as it does for other rows.  Rows that a warp
+// or less takes get their gradient in the forward launch too, from logits that are still in the caches.
 //
 // Otherwise G threads take a row: 8 up to 256 classes (a row is few vectors, and what a row costs beside them is shared by fewer), a warp up to
 // 4096, a CTA of 128 threads up to 12,288, of 256 above (forward: 20,000 x 8192 in bf16 88 us with 128 threads, 102 with 256, 237 with 512; 4096 x
@@ -238,76 +239,6 @@ distill_part_kernel(const __grid_constant__ Problem p, float2* __restrict__ out)
   if (threadIdx.x == 0) out[r * p.parts + blockIdx.x] = make_float2(top[0], sum[0]);
 }
 
-// G threads per row; the block's sum of losses goes to partials.  from_parts: what the kernel above left, or null.
-template <class T, int G>
-__global__ void __launch_bounds__(G > 32 ? G : 256)
-distill_forward_kernel(const __grid_constant__ Problem p, const float2* __restrict__ from_parts, Stats* __restrict__ stats,
-                       float* __restrict__ partials) {
-  constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G;  // rows of a CTA at a time
-  __shared__ float sh[3 * 32];
-  const int rank = threadIdx.x % G;
-  float loss = 0.f;
-  for (int64_t r0 = int64_t(blockIdx.x) * R; r0 < p.M; r0 += int64_t(gridDim.x) * R) {  // the same for all of a CTA
-    const int64_t mine = r0 + threadIdx.x / G, r = min(mine, p.M - 1);
-    const bool chosen = mine < p.M && (!p.mask || p.mask[r]);
-    const T* z = static_cast<const T*>(p.z) + r * p.ldz;
-    if (G > 32 && !chosen) {
-      if (threadIdx.x == 0) stats[r] = {0.f, 0.f, 0.f, INFINITY};
-      continue;
-    }
-    // the thread's first entry is on its way while the row is read
-    Loaded own{-1, 0.f};
-    if (chosen && rank < p.k) own = load_entry(p, r, rank);
-    Running x;
-    if (chosen) {
-      if (from_parts) {
-        for (int i = rank; i < p.parts; i += G) {
-          const float2 part = from_parts[r * p.parts + i];
-          x.raise(part.x, p.a);
-          x.s += part.x == -INFINITY ? part.y : part.y * exp2_approx((part.x - x.m) * p.a);
-        }
-      } else {
-        x = scan<T, G>(z, p.C, rank, p.a);
-      }
-    }
-    const Entry mine_first = looked_at(p, own);
-    const float at_first = mine_first.c >= 0 ? as_float(z[mine_first.c]) : 0.f;
-    // the maxima; whether the list has entries
-    float top[3] = {x.m, mine_first.c >= 0 ? mine_first.t : -INFINITY, mine_first.c >= 0 ? 1.f : 0.f};
-    for (int j = rank + G; chosen && j < p.k; j += G) {
-      const Entry e = entry(p, r, j);
-      if (e.c >= 0) top[1] = fmaxf(top[1], e.t), top[2] = 1.f;
-    }
-    over_group<G>(top, sh, Larger{});
-    const float zm = top[0], tm = top[1];
-    const bool counts = chosen && top[2] > 0.f;
-    // the sums: of the row's exponentials, of the list's, and of the list's times what the logarithms differ by
-    float sum[3] = {rescaled(x, zm, p.a), 0.f, 0.f};
-    auto add = [&](const Entry& e, float at) {
-      if (e.c < 0) return;
-      const float w = exp2_approx((e.t - tm) * p.a);
-      sum[1] += w;
-      if (!(w == 0.f)) sum[2] += w * (((e.t - tm) - (at - zm)) * p.a);
-    };
-    if (counts) {
-      add(mine_first, at_first);
-      for (int j = rank + G; j < p.k; j += G) {
-        const Entry e = entry(p, r, j);
-        add(e, e.c >= 0 ? as_float(z[e.c]) : 0.f);
-      }
-    }
-    over_group<G>(sum, sh, Sum{});
-    if (rank == 0 && mine < p.M) {
-      const Stats st = {zm, log2_approx(sum[0]), tm, counts ? log2_approx(sum[1]) : INFINITY};
-      stats[r] = counts ? st : Stats{0.f, 0.f, 0.f, INFINITY};
-      if (counts) loss += kLn2 * (sum[2] / sum[1] - st.tl + st.zl);
-    }
-  }
-  float all[1] = {loss};
-  over_group<(G > 32 ? G : 256)>(all, sh, Sum{});
-  if (threadIdx.x == 0) partials[blockIdx.x] = all[0];
-}
-
 __global__ void __launch_bounds__(256)
 distill_sum_kernel(const float* __restrict__ partials, int n, float scale, float* __restrict__ loss) {
   __shared__ double sh[256];
@@ -368,6 +299,140 @@ __device__ __forceinline__ float sum_at(int c, const int* cls, const float* prob
     sum += (ci.x == c ? pi.x : 0.f) + (ci.y == c ? pi.y : 0.f) + (ci.z == c ? pi.z : 0.f) + (ci.w == c ? pi.w : 0.f);
   }
   return sum;
+}
+
+// n columns of a row's gradient, from column `from` on, by G threads: z and d point at the first.  `cls`, `prob`: room for the list.  pad:
+// columns of zeros behind them.
+template <class T, int G>
+__device__ __forceinline__ void gradient_of_row(const Problem& p, int64_t r, const T* z, T* d, int from, int n, int pad, const Stats& st, float g,
+                                                int rank, int* cls, float* prob) {
+  constexpr int U = G == 8 ? 2 : 4;
+  const int kp = (p.k + 3) / 4 * 4;
+  const bool counts = !(st.tl == INFINITY);
+  if (rank < pad) d[n + rank] = rounded<T>(0.f);
+  if (counts)
+    for (int j = rank; j < kp; j += G) {
+      Entry e{0.f, -1};
+      if (j < p.k) e = entry(p, r, j);
+      cls[j] = e.c;
+      prob[j] = e.c < 0 ? 0.f : exp2_approx((e.t - st.tm) * p.a - st.tl);
+    }
+  const Gradient one{st.zm, st.zl, p.a, g};
+  const int head = before_vectors(d, n);
+  const bool vectors_fit = (reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(d)) % 16 == 0;
+  const int vectors = vectors_fit ? (n - head) / Vec<T>::N : 0, tail = vectors_fit ? head + vectors * Vec<T>::N : head;
+  if (rank < head) d[rank] = rounded<T>(counts ? one(as_float(z[rank]), 0.f) : 0.f);
+  for (int c = tail + rank; c < n; c += G) d[c] = rounded<T>(counts ? one(as_float(z[c]), 0.f) : 0.f);
+  const uint4* v = reinterpret_cast<const uint4*>(z + head);
+  uint4* to = reinterpret_cast<uint4*>(d + head);
+  const bool plain = product_is_finite(st.zm, p.a);
+  const F2 m = both(-st.zm), a = both(p.a), l = both(-st.zl), gg = both(g), c = both(-st.zm * p.a - st.zl);
+  for (int i = rank; i < vectors; i += G * U) {
+    uint4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = counts && i + u * G < vectors ? __ldg(v + i + u * G) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      F2 f[Vec<T>::P];
+      unpack<T>(w[u], f);
+      if (plain) {
+#pragma unroll
+        for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e], a, c), [](float x) { return exp2_approx(x); }) * gg;
+      } else {
+#pragma unroll
+        for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e] + m, a, l), [](float x) { return exp2_approx(x); }) * gg;
+      }
+      if (i + u * G < vectors) __stcs(to + i + u * G, counts ? pack<T>(f) : make_uint4(0, 0, 0, 0));
+    }
+  }
+  group_sync<G>();  // the lists, and the columns that the entries below write again
+  if (!counts) return;
+  for (int j = rank; j < p.k; j += G) {
+    const int c = cls[j];
+    if (c < from || c >= from + n) continue;
+    // all of an index's entries write the same
+    d[c - from] = rounded<T>(one(as_float(z[c - from]), sum_at(c, cls, prob, kp)));
+  }
+}
+
+// G threads per row; the block's sum of losses goes to partials.  from_parts: what distill_part_kernel left, or null.  GRADIENT: the
+// row's gradient too, for a loss that is differentiated by itself.
+template <class T, int G, bool GRADIENT>
+__global__ void __launch_bounds__(G > 32 ? G : 256)
+distill_forward_kernel(const __grid_constant__ Problem p, const float2* __restrict__ from_parts, Stats* __restrict__ stats,
+                       float* __restrict__ partials, float factor, T* __restrict__ dz, int64_t lddz, int pad) {
+  constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G;  // rows of a CTA at a time
+  __shared__ float sh[3 * 32];
+  extern __shared__ __align__(16) uint8_t lists[];  // GRADIENT: see distill_backward_kernel
+  const int rank = threadIdx.x % G;
+  float loss = 0.f;
+  for (int64_t r0 = int64_t(blockIdx.x) * R; r0 < p.M; r0 += int64_t(gridDim.x) * R) {  // the same for all of a CTA
+    const int64_t mine = r0 + threadIdx.x / G, r = min(mine, p.M - 1);
+    const bool chosen = mine < p.M && (!p.mask || p.mask[r]);
+    const T* z = static_cast<const T*>(p.z) + r * p.ldz;
+    if (G > 32 && !chosen) {
+      if (threadIdx.x == 0) stats[r] = {0.f, 0.f, 0.f, INFINITY};
+      continue;
+    }
+    // the thread's first entry is on its way while the row is read
+    Loaded own{-1, 0.f};
+    if (chosen && rank < p.k) own = load_entry(p, r, rank);
+    Running x;
+    if (chosen) {
+      if (from_parts) {
+        for (int i = rank; i < p.parts; i += G) {
+          const float2 part = from_parts[r * p.parts + i];
+          x.raise(part.x, p.a);
+          x.s += part.x == -INFINITY ? part.y : part.y * exp2_approx((part.x - x.m) * p.a);
+        }
+      } else {
+        x = scan<T, G>(z, p.C, rank, p.a);
+      }
+    }
+    const Entry mine_first = looked_at(p, own);
+    const float at_first = mine_first.c >= 0 ? as_float(z[mine_first.c]) : 0.f;
+    // the maxima; whether the list has entries
+    float top[3] = {x.m, mine_first.c >= 0 ? mine_first.t : -INFINITY, mine_first.c >= 0 ? 1.f : 0.f};
+    for (int j = rank + G; chosen && j < p.k; j += G) {
+      const Entry e = entry(p, r, j);
+      if (e.c >= 0) top[1] = fmaxf(top[1], e.t), top[2] = 1.f;
+    }
+    over_group<G>(top, sh, Larger{});
+    const float zm = top[0], tm = top[1];
+    const bool counts = chosen && top[2] > 0.f;
+    // the sums: of the row's exponentials, of the list's, and of the list's times what the logarithms differ by
+    float sum[3] = {rescaled(x, zm, p.a), 0.f, 0.f};
+    auto add = [&](const Entry& e, float at) {
+      if (e.c < 0) return;
+      const float w = exp2_approx((e.t - tm) * p.a);
+      sum[1] += w;
+      if (!(w == 0.f)) sum[2] += w * (((e.t - tm) - (at - zm)) * p.a);
+    };
+    if (counts) {
+      add(mine_first, at_first);
+      for (int j = rank + G; j < p.k; j += G) {
+        const Entry e = entry(p, r, j);
+        add(e, e.c >= 0 ? as_float(z[e.c]) : 0.f);
+      }
+    }
+    over_group<G>(sum, sh, Sum{});
+    const Stats st = counts ? Stats{zm, log2_approx(sum[0]), tm, log2_approx(sum[1])} : Stats{0.f, 0.f, 0.f, INFINITY};
+    if (rank == 0 && mine < p.M) {
+      stats[r] = st;
+      if (counts) loss += kLn2 * (sum[2] / sum[1] - st.tl + st.zl);
+    }
+    if constexpr (GRADIENT) {
+      if (mine < p.M) {
+        const int kp = (p.k + 3) / 4 * 4;
+        int* cls = reinterpret_cast<int*>(lists) + (threadIdx.x / G) * 2 * kp;
+        gradient_of_row<T, G>(p, r, z, dz + r * lddz, 0, p.C, pad, st, factor, rank, cls, reinterpret_cast<float*>(cls + kp));
+      }
+      group_sync<G>();  // the lists are read
+    }
+  }
+  float all[1] = {loss};
+  over_group<(G > 32 ? G : 256)>(all, sh, Sum{});
+  if (threadIdx.x == 0) partials[blockIdx.x] = all[0];
 }
 
 // ------------------------------------------------------------------ both in one pass
@@ -664,7 +729,7 @@ template <class T, int G>
 __global__ void __launch_bounds__(G > 32 ? G : 256)
 distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restrict__ stats, const float* __restrict__ grad, float factor,
                         T* __restrict__ dz, int64_t lddz, int pad, bool has_one) {
-  constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G, U = G == 8 ? 2 : 4;
+  constexpr int kThreads = G > 32 ? G : 256, R = kThreads / G;
   if (has_one && __ldg(grad) == 1.f) return;  // dZ holds that gradient
   extern __shared__ __align__(16) uint8_t lists[];  // of each of the CTA's rows: the entries' classes, then their probabilities
   const int rank = threadIdx.x % G, kp = (p.k + 3) / 4 * 4;
@@ -682,52 +747,7 @@ distill_backward_kernel(const __grid_constant__ Problem p, const Stats* __restri
     const bool last = int(item - r * p.parts) == p.parts - 1;
     const T* z = static_cast<const T*>(p.z) + r * p.ldz + from;
     T* d = dz + r * lddz + from;
-    const Stats st = stats[r];
-    const bool counts = !(st.tl == INFINITY);
-    if (last && rank < pad) dz[r * lddz + p.C + rank] = rounded<T>(0.f);
-    if (counts)
-      for (int j = rank; j < kp; j += G) {
-        Entry e{0.f, -1};
-        if (j < p.k) e = entry(p, r, j);
-        cls[j] = e.c;
-        prob[j] = e.c < 0 ? 0.f : exp2_approx((e.t - st.tm) * p.a - st.tl);
-      }
-    const Gradient one{st.zm, st.zl, p.a, g};
-    const int head = before_vectors(d, n);
-    const bool vectors_fit = (reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(d)) % 16 == 0;
-    const int vectors = vectors_fit ? (n - head) / Vec<T>::N : 0, tail = vectors_fit ? head + vectors * Vec<T>::N : head;
-    if (rank < head) d[rank] = rounded<T>(counts ? one(as_float(z[rank]), 0.f) : 0.f);
-    for (int c = tail + rank; c < n; c += G) d[c] = rounded<T>(counts ? one(as_float(z[c]), 0.f) : 0.f);
-    const uint4* v = reinterpret_cast<const uint4*>(z + head);
-    uint4* to = reinterpret_cast<uint4*>(d + head);
-    const bool plain = product_is_finite(st.zm, p.a);
-    const F2 m = both(-st.zm), a = both(p.a), l = both(-st.zl), gg = both(g), c = both(-st.zm * p.a - st.zl);
-    for (int i = rank; i < vectors; i += G * U) {
-      uint4 w[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = counts && i + u * G < vectors ? __ldg(v + i + u * G) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        F2 f[Vec<T>::P];
-        unpack<T>(w[u], f);
-        if (plain) {
-#pragma unroll
-          for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e], a, c), [](float x) { return exp2_approx(x); }) * gg;
-        } else {
-#pragma unroll
-          for (int e = 0; e < Vec<T>::P; ++e) f[e] = each(fma2(f[e] + m, a, l), [](float x) { return exp2_approx(x); }) * gg;
-        }
-        if (i + u * G < vectors) __stcs(to + i + u * G, counts ? pack<T>(f) : make_uint4(0, 0, 0, 0));
-      }
-    }
-    group_sync<G>();  // the lists, and the columns that the entries below write again
-    if (!counts) continue;
-    for (int j = rank; j < p.k; j += G) {
-      const int c = cls[j];
-      if (c < from || c >= from + n) continue;
-      // all of an index's entries write the same
-      d[c - from] = rounded<T>(one(as_float(z[c - from]), sum_at(c, cls, prob, kp)));
-    }
+    gradient_of_row<T, G>(p, r, z, d, from, n, last ? pad : 0, stats[r], g, rank, cls, prob);
   }
 }
 
@@ -740,6 +760,12 @@ int one_pass_threads(const void* Z, int type, int64_t ldz, const void* dZ, int64
   const bool same = (reinterpret_cast<uintptr_t>(Z) - reinterpret_cast<uintptr_t>(dZ)) % 16 == 0 && (ldz - lddz) * size % 16 == 0;
   if (!same || M < gc::kNumSMs || k > kOnePassList) return 0;
   return bytes <= kOnePassFrom || bytes > Ring<kLong>::kMostBytes ? 0 : bytes <= Ring<kShort>::kMostBytes ? kShort : kLong;
+}
+// Whether a forward call makes the gradient: in one pass, or where a warp or less takes a row, which is still near when the row's
+// statistics are there.  169,343 x 47 in fp32: 41 us in all, 52 with a launch of its own for the gradient; 60,000 x 1000 in bf16 87 and 102, in
+// fp32 127 and 142; 20,000 x 4096 in bf16 96 and 111, in fp32 175 and 175.
+bool makes_gradient(const void* Z, int type, int64_t ldz, const void* dZ, int64_t lddz, int64_t M, int64_t C, int64_t k) {
+  return one_pass_threads(Z, type, ldz, dZ, lddz, M, C, k) || threads_per_row(C, k) <= 32;
 }
 // Rows above 8192 columns of which there are fewer than SMs are cut, into parts of 4096 or more.
 int parts_of(int64_t M, int64_t C) {
@@ -791,7 +817,8 @@ size_t gc_distill_workspace_bytes(int64_t M, int64_t C) {
 }
 
 int gc_distill_one_pass(const void* Z, int type, int64_t ldz, int64_t lddz, int64_t M, int64_t C, int64_t k) {
-  return (type == GC_TYPE_F32 || type == GC_TYPE_BF16) && M >= 0 && C >= 1 && k >= 0 && one_pass_threads(Z, type, ldz, nullptr, lddz, M, C, k) != 0;
+  return (type == GC_TYPE_F32 || type == GC_TYPE_BF16) && M >= 0 && C >= 1 && k >= 0 && k <= kMaxList &&
+         makes_gradient(Z, type, ldz, nullptr, lddz, M, C, k);
 }
 
 int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, int top_type, int64_t ldt, const void* index,
@@ -804,7 +831,7 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
   GC_REQUIRE(loss && (M == 0 || stats), "gc_distill_forward: null pointer");
   GC_REQUIRE(gc::aligned16(stats), "gc_distill_forward: the statistics must be 16-byte aligned");
   GC_REQUIRE(!dZ || (pad >= 0 && pad < 8 && lddz >= C + pad), "gc_distill_forward: leading dimension below the row length");
-  GC_REQUIRE(!dZ || one_pass_threads(Z, type, ldz, dZ, lddz, M, C, k), "gc_distill_forward: no gradient for rows like these");
+  GC_REQUIRE(!dZ || makes_gradient(Z, type, ldz, dZ, lddz, M, C, k), "gc_distill_forward: no gradient for rows like these");
   const cudaStream_t st = gc::as_stream(stream);
   if (M == 0) {
     const cudaError_t e = cudaMemsetAsync(loss, 0, sizeof(float), st);
@@ -848,9 +875,21 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
     if (parts) distill_part_kernel<T><<<dim3(unsigned(p.parts), unsigned(M)), kPart, 0, st>>>(p, parts);
     with_group(G, p.parts > 1, [&](auto gt) {
       constexpr int kG = decltype(gt)::value;
-      distill_forward_kernel<T, kG><<<grid, kG > 32 ? kG : 256, 0, st>>>(p, parts, reinterpret_cast<Stats*>(stats), partials);
+      Stats* const to = reinterpret_cast<Stats*>(stats);
+      if constexpr (kG <= 32) {
+        if (dZ) {
+          const int smem = 256 / kG * 2 * int((k + 3) / 4 * 4) * 4;
+          auto kern = distill_forward_kernel<T, kG, true>;
+          const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+          if (e != cudaSuccess) rc = gc::fail(GC_ERR_CUDA, "gc_distill_forward: %s", cudaGetErrorString(e));
+          else kern<<<grid, 256, smem, st>>>(p, parts, to, partials, scale * temperature, static_cast<T*>(dZ), lddz, int(pad));
+          return;
+        }
+      }
+      distill_forward_kernel<T, kG, false><<<grid, kG > 32 ? kG : 256, 0, st>>>(p, parts, to, partials, 0.f, nullptr, 0, 0);
     });
   });
+  if (rc != GC_OK) return rc;
   distill_sum_kernel<<<1, 256, 0, st>>>(partials, int(grid), scale * temperature * temperature, loss);
   return gc::check_launch("gc_distill_forward", parts ? 3 : 2);
 }

@@ -400,7 +400,7 @@ int gc_logsoftmax_nll_backward_pad_f32(const float* Z, int64_t ldz, const int64_
  *   type, top_type: GC_TYPE_F32 or GC_TYPE_BF16 (dZ has Z's).  index_bits: 64 or 32.  k: at most 1024.
  *   stats: M x 4 floats, 16-byte aligned, which the backward call reads.  loss, grad_loss: one device float each.
  *   pad: columns behind a row of dZ that are its own and become zero (less than 8).
- * Where gc_distill_one_pass (a 16-byte aligned dZ assumed) is not 0, one pass over the logits can do both: a forward call that is given
+ * Where gc_distill_one_pass (a 16-byte aligned dZ assumed) is not 0, one launch can do both: a forward call that is given
  * dZ writes it, for grad_loss = 1.  Then the backward call gets the same dZ with dz_made = 1, and leaves it as it is where grad_loss is 1.
  */
 int gc_distill_one_pass(const void* Z, int type, int64_t ldz, int64_t lddz, int64_t M, int64_t C, int64_t k);

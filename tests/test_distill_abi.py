@@ -33,7 +33,7 @@ def test_what_both_refuse(call):
 def test_forward_arguments():
     assert _forward(loss=None) == -1
     assert _forward(dz=16, lddz=C - 1) == -1 and _forward(dz=16, pad=8, lddz=C + 8) == -1
-    assert _forward(dz=16) == -1 and b"rows like these" in L().gc_last_error()
+    assert _forward(dz=16, c=5000, ldz=5000, lddz=5000) == -1 and b"rows like these" in L().gc_last_error()
     assert _forward(ws=None) == -4 and _forward(wsb=L().gc_distill_workspace_bytes(M, C) - 1) == -4 and _forward(ws=24) == -1
     assert L().gc_distill_workspace_bytes(-1, C) == L().gc_distill_workspace_bytes(M, 0) == 0
     assert L().gc_distill_workspace_bytes(4, 100_000) > L().gc_distill_workspace_bytes(4, 100)
@@ -50,7 +50,8 @@ def test_which_rows_go_in_one_pass():
         return L().gc_distill_one_pass(z, t, ldz, lddz, m, c, k)
 
     assert one(16, 0, 8192, 8192, 1000, 8192) and one(16, 1, 90_001, 90_001, 1000, 90_001)
-    assert not one(16, 0, 47, 47, 100_000, 47)       # short rows
+    assert one(16, 0, 47, 47, 100_000, 47) and one(20, 0, 4099, 4096, 3, 4096, 1024)  # short rows, wherever they lie
+    assert not one(16, 1, 4097, 4097, 10_000, 4097, 300)  # neither short nor with a short list
     assert not one(16, 0, 50_689, 50_689, 1000, 50_689) and not one(16, 1, 101_377, 101_377, 1000, 101_377)  # longer than the ring
     assert not one(16, 0, 8192, 8192, 100, 8192)     # few rows
     assert not one(20, 0, 8192, 8192, 1000, 8192) and not one(16, 0, 8193, 8192, 1000, 8192)  # the rows lie differently
