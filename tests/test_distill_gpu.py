@@ -217,9 +217,10 @@ def test_default_scale_and_nothing_to_do():
         assert float(loss) == 0 and dx.shape == x.shape and not dx.any()
 
 
-def test_a_gradient_that_is_not_one_and_gradients_of_their_own():
-    """Rows of one pass have their gradient before the loss's is known; what is handed out is changed by no later backward pass."""
-    logits, top, index = make(200, 9000, 20)
+@pytest.mark.parametrize("M,C,k", [(200, 9000, 20), (300, 47, 8), (300, 47, 40), (70, 1000, 200), (9, 4096, 1000)])
+def test_a_gradient_that_is_not_one_and_gradients_of_their_own(M, C, k):
+    """Rows may have their gradient before the loss's is known; what is handed out is changed by no later backward pass."""
+    logits, top, index = make(M, C, k, distinct=C != 1000)
     x = logits.detach().requires_grad_()
     loss = gc.distill_loss(x, top, index, None, 2.0)
     first = torch.autograd.grad(loss, x, retain_graph=True)[0]
@@ -235,9 +236,9 @@ def test_a_gradient_that_is_not_one_and_gradients_of_their_own():
     assert float((half.grad - 0.5 * kept).abs().max()) <= float(kept.abs().max()) * 2.0 ** -22
 
 
-@pytest.mark.parametrize("M,C", [(500, 20_000), (200, 60_000)])
-def test_same_bits_every_time_and_backward_twice(M, C):
-    logits, top, index = make(M, C, 30, dtype=torch.bfloat16)
+@pytest.mark.parametrize("M,C,k", [(500, 20_000, 30), (200, 60_000, 30), (1000, 47, 8), (300, 1000, 300), (60, 6000, 600)])
+def test_same_bits_every_time_and_backward_twice(M, C, k):
+    logits, top, index = make(M, C, k, dtype=torch.bfloat16, distinct=k < 100)
     x = logits.detach().requires_grad_()
     losses, grads = [], []
     for _ in range(3):
