@@ -528,13 +528,17 @@ struct Shape {
   int bn;
   bool pair;
 };
-// Rows times weights.  Pairs on 256 x 256 where groups have rows for it on average and every pair gets a tile; else 128 columns, or 64
-// where that gives each SM a tile (few rows: bound by reading the weights).
+// Rows times weights: pairs on 256 x 256, 128 columns or 64, whichever takes least of (rounds of tiles over the SMs) x (rows of A and of B
+// that a CTA loads for a k-block), with groups taken to be equally large.  4096 rows of 8 groups, 1024 -> 1024: 64 pairs' tiles in one round 13.6
+// us, 64 columns in four 26; 600 of 2, 4096 -> 4096: 29 and 65; a row to each of 8, 4096 -> 4096: 128 columns in two rounds 50, 64 in four 84.
 Shape shape_of_rows(int64_t M, int64_t n, int64_t G) {
-  const int64_t with_rows = std::min(G, M);
-  if (n > 128 && M >= 256 * with_rows && gc::ceil_div(M, 256) * gc::ceil_div(n, 256) >= gc::kNumSMs / 2) return {256, true};
-  const int64_t tiles = std::max(gc::ceil_div(M, BM), with_rows) * gc::ceil_div(n, 128);
-  return {n > 64 && tiles >= 2 * gc::kNumSMs ? 128 : 64, false};
+  const int64_t with_rows = std::min(G, M), rows = gc::ceil_div(M, with_rows), a = std::min<int64_t>(BM, M);
+  auto cost = [&](int64_t bm, int64_t bn, int64_t units, int64_t loads) {
+    return gc::ceil_div(with_rows * gc::ceil_div(rows, bm) * gc::ceil_div(n, bn), units) * (a + loads);
+  };
+  const int64_t pair = cost(256, 256, gc::kNumSMs / 2, 128), wide = cost(BM, 128, gc::kNumSMs, 128), narrow = cost(BM, 64, gc::kNumSMs, 64);
+  if (n > 128 && rows > BM && pair <= std::min(wide, narrow)) return {256, true};
+  return {n > 64 && wide <= narrow ? 128 : 64, false};
 }
 Shape shape_of_weights(int64_t m, int64_t n) {
   if (m > 128 && n > 128) return {256, true};
