@@ -546,13 +546,27 @@ Shape shape_of_weights(int64_t m, int64_t n) {
 }
 // Rows of a part of dW.  Few tiles: so many that the parts' tiles, one more per group than the rows alone would make, fill the GPU once
 // (8 groups of 169,343 rows, 256 x 256: 36 us; with half as many rows in a part, whose last round is nearly empty, 44 and twice the
-// sums).  Else half of an SM's share of the work, so that large groups spread.  At least 4 k-blocks, and at most kChain rows, beyond which
-// truncation would show.
+// sums).  More: the number of parts of an average group that takes least, where a part's fp32 sums cost as much as kSums rows to write and
+// add, and the launch that adds as half of that; a group that stays whole may be a quarter
+// larger, or half an SM's share of the work (4096 rows of 8 groups, 1024 x 1024: 19 us, 41 where every part is such a share; 60,000 of 8 102 and
+// 144; 20,000 of 8, 512 x 512, 27 and 38).  At least 4 k-blocks, and at most kChain rows, beyond which truncation would show.
 constexpr int64_t kChain = 16384;
+constexpr int64_t kSums = 1280;
 int64_t part_rows(int64_t M, int64_t m, int64_t n, int64_t G, const Shape& s) {
   const int64_t tiles = gc::ceil_div(m, s.pair ? 256 : BM) * gc::ceil_div(n, s.bn), units = s.pair ? gc::kNumSMs / 2 : gc::kNumSMs;
-  const int64_t share = units > 4 * G * tiles ? units - G * tiles : 2 * units;
-  return std::min(kChain, std::max<int64_t>(4 * KE, gc::ceil_div(gc::ceil_div(M * tiles, share), KE) * KE));
+  const int64_t groups = std::min(G, M), rows = gc::ceil_div(M, groups), all = groups * tiles;
+  int64_t part;
+  if (units > 4 * all) {
+    part = gc::ceil_div(M * tiles, units - all);
+  } else {
+    int64_t parts = 1, least = gc::ceil_div(all, units) * (rows + kSums / 4);
+    for (int64_t i = 2; i <= 8; ++i) {
+      const int64_t cost = gc::ceil_div(all * i, units) * (gc::ceil_div(rows, i) + kSums) + kSums / 2;
+      if (cost < least) least = cost, parts = i;
+    }
+    part = parts > 1 ? gc::ceil_div(rows, parts) : std::max({rows + rows / 4, kSums, gc::ceil_div(M * tiles, 2 * units)});
+  }
+  return std::min(kChain, std::max<int64_t>(4 * KE, gc::ceil_div(part, KE) * KE));
 }
 int64_t parts_most(int64_t M, int64_t G, int64_t part) { return M / part + G; }  // that exist, at most
 
