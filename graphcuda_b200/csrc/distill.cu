@@ -11,13 +11,14 @@
 //
 // With a gradient to be asked for, rows of some thousands of classes are read once in all (one_pass): a CTA streams rows through a ring of
 // segments in shared memory; one half of its threads goes over a row's segments as they arrive for its statistics, the other
-// over the same segments again for dZ, giving them back to the copies of the next row.  That is dZ for g = 1, which is what a loss that is differentiated by
-// itself has; the backward call looks at g and, where it is another, computes dZ from the logits as it does for other rows.  Rows that a warp
+// over the same segments again for dZ, giving them back to the copies of the next row.  That is dZ for g = 1, which is what a loss that is
+// differentiated by itself has; the backward call looks at g and, where it is another, computes dZ from the logits as it does for other rows.  Rows that a warp
 // or less takes get their gradient in the forward launch too, from logits that are still in the caches.
 //
 // Otherwise G threads take a row: 8 up to 256 classes (a row is few vectors, and what a row costs beside them is shared by fewer), a warp up to
 // 4096, a CTA of 128 threads up to 12,288, of 256 above (forward: 20,000 x 8192 in bf16 88 us with 128 threads, 102 with 256, 237 with 512; 4096 x
-// 65,536 99, 92, 109); with fewer rows than SMs a CTA takes a part of a row and another launch puts the parts together.  Rows may start anywhere: what lies before the first and behind the last 16-byte vector is read by itself.
+// 65,536 99, 92, 109); with fewer rows than SMs a CTA takes a part of a row and another launch puts the parts together.  Rows may start
+// anywhere: what lies before the first and behind the last 16-byte vector is read by itself.
 #include "common.cuh"
 #include "ffn_internal.cuh"
 #include "tiles.cuh"

@@ -74,6 +74,13 @@ def test_step(sizes, k, n):
     check(*inputs(sizes, k, n))
 
 
+@pytest.mark.parametrize("sizes,k,n", [([2600] * 20, 256, 256), ([2000, 0, 4500, 2603] * 5, 200, 256), ([700] * 30 + [9000], 264, 250),
+                                       ([40] * 70, 512, 512), ([1300, 500], 1024, 1024), ([130, 3], 2048, 1024)])
+def test_parts_and_tiles_of_all_sorts(sizes, k, n):
+    """Groups cut into parts and groups left whole, tiles of each shape."""
+    check(*inputs(sizes, k, n))
+
+
 @pytest.mark.parametrize("before,behind", [(0, 9), (3, 0), (70, 300)])
 @pytest.mark.parametrize("k,n", [(64, 128), (47, 100), (256, 512)])
 def test_rows_of_no_group(before, behind, k, n):
