@@ -7,7 +7,8 @@
 // An entry whose index is no class, or whose logit is -inf, is none; a row without entries does not count.  The logits are read
 // once forward (a running maximum and sum) and once backward, where the row's four statistics are at hand; probabilities
 // come from one exponential each, and nothing but dZ is written.  Sums and statistics are fp32.  With u = (z - max) log2(e) / T the
-// subtraction comes before the product, so that a row filled with the type's lowest value does not overflow.
+// subtraction comes before the product, so that neither a row filled with the type's lowest value overflows nor one far from zero loses the
+// difference to rounding; where the maximum lies near zero (see near_zero) dZ, and one_pass's sums, take one multiply-add for both.
 //
 // With a gradient to be asked for, rows of some thousands of classes are read once in all (one_pass): a CTA streams rows through a ring of
 // segments in shared memory; one half of its threads goes over a row's segments as they arrive for its statistics, the other
@@ -282,12 +283,14 @@ __device__ __forceinline__ T rounded(float v) {
   else return __float2bfloat16_rn(v);
 }
 
-// g (q - p) of a logit.  Where the maximum times a is a number the exponent is one multiply-add, (z a - zm a - zl), as in the vectors.
-__device__ __forceinline__ bool product_is_finite(float m, float a) { return fabsf(m * a) < 1e38f; }
+// g (q - p) of a logit.  Where the maximum lies near zero the exponent is one multiply-add, z a + (-zm a - zl), as in the vectors: the rounding
+// of that sum, half a step of numbers below 64, stays below 2^-19.  It grows with the maximum (at -1e9, a mask's value, it is 64 or so),
+// so that other rows subtract first, which is exact beside the difference.
+__device__ __forceinline__ bool near_zero(float m, float a) { return fabsf(m * a) < 32.f; }
 struct Gradient {
   float zm, zl, a, g;
   __device__ __forceinline__ float operator()(float z, float p) const {
-    const float e = product_is_finite(zm, a) ? fmaf(z, a, -zm * a - zl) : (z - zm) * a - zl;
+    const float e = near_zero(zm, a) ? fmaf(z, a, -zm * a - zl) : (z - zm) * a - zl;
     return g * (exp2_approx(e) - p);
   }
 };
@@ -352,7 +355,7 @@ __device__ __forceinline__ void gradient_of_row(const Problem& p, int64_t r, con
   for (int c = tail + rank; c < n; c += G) d[c] = rounded<T>(counts ? one(as_float(z[c]), 0.f) : 0.f);
   const uint4* v = reinterpret_cast<const uint4*>(z + head);
   uint4* to = reinterpret_cast<uint4*>(d + head);
-  const bool plain = product_is_finite(st.zm, p.a);
+  const bool plain = near_zero(st.zm, p.a);
   const F2 m = both(-st.zm), a = both(p.a), l = both(-st.zl), gg = both(g), c = both(-st.zm * p.a - st.zl);
   for (int i = rank; i < vectors; i += G * U) {
     uint4 w[U];
@@ -633,7 +636,7 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
         x.raise(fmaxf(fmaxf(vec_max<T>(w[0]), vec_max<T>(w[1])), fmaxf(vec_max<T>(w[2]), vec_max<T>(w[3]))), p.a);
         const F2 scale = both(p.a);
         F2 sum = both(0.f);
-        if (product_is_finite(x.base(), p.a)) {
+        if (near_zero(x.base(), p.a)) {
           const F2 base = both(-x.base() * p.a);
 #pragma unroll
           for (int u = 0; u < kEach; ++u) {
@@ -704,7 +707,7 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
         for (int i = rank; i < vectors; i += THREADS) to[i] = make_uint4(0, 0, 0, 0);
         if (!chosen) continue;
       }
-      const bool plain = product_is_finite(zm, p.a);
+      const bool plain = near_zero(zm, p.a);
       const F2 a = both(p.a), gg = both(g), c = both(-zm * p.a - zl), m = both(-zm), l = both(-zl);
       for (int v = 0; v < vectors; v += kVectors) {
         if (ok) ok = gc::tiles::wait(full(slot), phase, abort_p);
