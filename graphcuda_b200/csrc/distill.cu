@@ -738,11 +738,18 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
         const Gradient one{zm, zl, p.a, g};
         if (rank < head) d[rank] = rounded<T>(one(as_float(z[rank]), 0.f));
         if (rank < p.C - tail) d[tail + rank] = rounded<T>(one(as_float(z[tail + rank]), 0.f));
-        sync_threads<2, THREADS>();  // the columns that the entries write again
+      }
+      // The columns that the entries write again.  (Of every row that is chosen: when a wait has run out, lists change under their readers and
+      // not all threads find the same `counts`, but all come here; and what they then find for a class may be anything.)
+      sync_threads<2, THREADS>();
+      if (counts) {
+        const Gradient one{zm, zl, p.a, g};
         const int* cls = classes(buf);
         const float* at_entry = at_entries(buf);
-        for (int j = rank; j < p.k; j += THREADS)
-          if (cls[j] >= 0) d[cls[j]] = rounded<T>(one(at_entry[j], sum_at(cls[j], cls, probs(buf), kp)));
+        for (int j = rank; j < p.k; j += THREADS) {
+          const int at = cls[j];
+          if (uint32_t(at) < uint32_t(p.C)) d[at] = rounded<T>(one(at_entry[j], sum_at(at, cls, probs(buf), kp)));
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(taken(buf));
