@@ -830,6 +830,15 @@ int fill(Problem& p, const char* what, const void* Z, int type, int64_t ldz, con
               kLog2e / temperature};
   return GC_OK;
 }
+// Shared memory of a launch: the ring and two rows' lists; the lists of a CTA's rows.
+constexpr int one_pass_bytes(int threads, int k) { return kSegments * threads * kEach * 16 + 2 * kListWords * ((k + 3) / 4 * 4) * 4; }
+constexpr int list_bytes(int G, int k) { return (G > 32 ? 1 : 256 / G) * list_words(k) * 4; }
+// The attribute belongs to all threads of the process: a call sets it to the longest list's, so that a launch that another thread has
+// just allowed stays allowed.
+template <class Kernel>
+cudaError_t allow_lists(Kernel kern, int G, int smem) {
+  return smem > 47 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, list_bytes(G, kMaxList)) : cudaSuccess;
+}
 template <class F>
 void with_group(int G, bool parts, F&& f) {
   if (G == 8) f(std::integral_constant<int, 8>{});
@@ -885,14 +894,14 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
     int* word = nullptr;
     rc = gc::tiles::error_word(&word);
     if (rc != GC_OK) return rc;
-    const int smem = kSegments * whole * kEach * 16 + 2 * kListWords * int((k + 3) / 4 * 4) * 4;
+    const int smem = one_pass_bytes(whole, int(k));
     const unsigned ctas = unsigned(std::min<int64_t>(M, gc::kNumSMs * (whole == kLong ? 1 : std::min(4, 222 * 1024 / (smem + 2048)))));
     with_type(type, [&](auto t) {
       using T = decltype(t);
       auto run = [&](auto threads) {
         constexpr int kThreads = decltype(threads)::value;
         auto kern = distill_one_pass_kernel<T, kThreads>;
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, one_pass_bytes(kThreads, kOnePassList));
         if (e != cudaSuccess) rc = gc::fail(GC_ERR_CUDA, "gc_distill_forward: %s", cudaGetErrorString(e));
         else
           kern<<<ctas, 2 * kThreads + 64, smem, st>>>(p, reinterpret_cast<Stats*>(stats), partials, scale * temperature, static_cast<T*>(dZ), lddz,
@@ -914,9 +923,9 @@ int gc_distill_forward(const void* Z, int type, int64_t ldz, const void* top, in
       Stats* const to = reinterpret_cast<Stats*>(stats);
       if constexpr (kG <= 32) {
         if (dZ) {
-          const int smem = 256 / kG * list_words(int(k)) * 4;
+          const int smem = list_bytes(kG, int(k));
           auto kern = distill_forward_kernel<T, kG, true>;
-          const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+          const cudaError_t e = allow_lists(kern, kG, smem);
           if (e != cudaSuccess) rc = gc::fail(GC_ERR_CUDA, "gc_distill_forward: %s", cudaGetErrorString(e));
           else kern<<<grid, 256, smem, st>>>(p, parts, to, partials, scale * temperature, static_cast<T*>(dZ), lddz, int(pad));
           return;
@@ -942,7 +951,7 @@ int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, i
   GC_REQUIRE(gc::aligned16(stats), "gc_distill_backward: the statistics must be 16-byte aligned");
   const int G = p.parts > 1 ? kWide : threads_per_row(C, k);
   const int rows = G > 32 ? 1 : 256 / G;
-  const size_t smem = size_t(rows) * list_words(int(k)) * 4;
+  const int smem = list_bytes(G, int(k));
   // where dZ is mostly there already, as many CTAs as run at one time
   const unsigned grid = unsigned(std::min<int64_t>(gc::ceil_div(M * p.parts, rows), dz_made ? gc::kNumSMs * 4 : int64_t(1) << 30));
   int bad = GC_OK;
@@ -951,11 +960,9 @@ int gc_distill_backward(const void* Z, int type, int64_t ldz, const void* top, i
     with_group(G, p.parts > 1, [&](auto gt) {
       constexpr int kG = decltype(gt)::value;
       auto kern = distill_backward_kernel<T, kG>;
-      if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-        if (e != cudaSuccess) bad = gc::fail(GC_ERR_CUDA, "gc_distill_backward: %s", cudaGetErrorString(e));
-      }
-      if (bad == GC_OK)
+      const cudaError_t e = allow_lists(kern, kG, smem);
+      if (e != cudaSuccess) bad = gc::fail(GC_ERR_CUDA, "gc_distill_backward: %s", cudaGetErrorString(e));
+      else
         kern<<<grid, kG > 32 ? kG : 256, smem, gc::as_stream(stream)>>>(p, reinterpret_cast<const Stats*>(stats), grad_loss,
                                                                          scale * temperature, static_cast<T*>(dZ), lddz, int(pad), dz_made != 0);
     });

@@ -475,9 +475,10 @@ template <int NT, int MT, bool GATED, bool SPLIT, int GPC, bool ZEROS>
 int launch_rows(Params p, cudaStream_t st) {
   const int64_t blocks = gc::ceil_div(p.N, GATED ? 16 : 16 * MT);
   const int runs = int(gc::ceil_div(gc::ceil_div(p.K, kChunk), kRun));
-  const int warps = runs >= 16 ? 8 : 4, per_sm = NT == 1 && MT == 1 ? 24 : 16;
+  constexpr int kPerSm = NT == 1 && MT == 1 ? 24 : 16;  // warps
+  const int warps = runs >= 16 ? 8 : 4;
   // All warps at once: outputs beyond those follow in the same CTAs.
-  const int64_t slots = per_sm / warps * gc::kNumSMs;
+  const int64_t slots = kPerSm / warps * gc::kNumSMs;
   p.ctas = 1;
   while (p.ctas < 8 && blocks * 2 * p.ctas <= slots && 2 * p.ctas * warps <= runs) p.ctas *= 2;
   const int64_t ctas = std::min(blocks, slots);
@@ -485,12 +486,15 @@ int launch_rows(Params p, cudaStream_t st) {
   constexpr int kPlace = (SPLIT ? 3 : MT) * kRun * record_bytes(GPC, ZEROS);
   const int64_t mine = gc::ceil_div(runs, p.ctas * warps) * gc::ceil_div(blocks, ctas);
   const int sums = 2 * warps * MT * 16 * NT * 8 * int(sizeof(float));
-  const int room = (220 * 1024 / (per_sm / warps) - 1024 - 256 - sums) / warps;
-  static_assert((220 * 1024 / (NT == 1 && MT == 1 ? 6 : 4) - 1280) / 4 - 2 * MT * 16 * NT * 8 * 4 >= kPlace + 8, "room for a place");
+  const int room = (220 * 1024 / (kPerSm / warps) - 1024 - 256 - sums) / warps;
+  static_assert((220 * 1024 / (kPerSm / 4) - 1280) / 4 - 2 * MT * 16 * NT * 8 * 4 >= kPlace + 8, "room for a place");
   p.ring = int(std::min<int64_t>({mine, 16, room / (kPlace + 8)}));
   const int smem = sums + (warps * p.ring * 8 + 127) / 128 * 128 + warps * p.ring * kPlace;
   auto kern = int4_rows_kernel<NT, MT, GATED, SPLIT, GPC, ZEROS>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // what any call of this form may take: the attribute is every thread's of the process, and one that calls with less must not lower it
+  // between another's two calls
+  constexpr int kMostBytes = 220 * 1024 / (kPerSm / 8) - 1024;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostBytes);
   if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   const int rc = gc::tiles::error_word(&p.word);
   if (rc != GC_OK) return rc;

@@ -361,7 +361,7 @@ int launch(Params p, int64_t z, cudaStream_t st) {
   p.stages = int(std::min<int64_t>({gc::ceil_div(chunks, p.ctas), 8, kRoom / S_::kStage}));
   const int smem = 128 + std::max(p.stages * S_::kStage, S_::kSums);
   auto kern = int4_tiles_kernel<NT, MT, GATED, SPLIT, GPC, ZEROS>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 + kRoom);  // any call's: see int4.cu
   if (e != cudaSuccess) return gc::fail(GC_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   const int rc = gc::tiles::error_word(&p.word);
   if (rc != GC_OK) return rc;
