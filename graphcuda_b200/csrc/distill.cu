@@ -707,6 +707,11 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
         for (int i = rank; i < vectors; i += THREADS) to[i] = make_uint4(0, 0, 0, 0);
         if (!chosen) continue;
       }
+      const Gradient one{zm, zl, p.a, g};
+      if (counts) {
+        if (rank < head) d[rank] = rounded<T>(one(as_float(z[rank]), 0.f));
+        if (rank < p.C - tail) d[tail + rank] = rounded<T>(one(as_float(z[tail + rank]), 0.f));
+      }
       const bool plain = near_zero(zm, p.a);
       const F2 a = both(p.a), gg = both(g), c = both(-zm * p.a - zl), m = both(-zm), l = both(-zl);
       for (int v = 0; v < vectors; v += kVectors) {
@@ -734,16 +739,10 @@ distill_one_pass_kernel(const __grid_constant__ Problem p, Stats* __restrict__ s
           if (i < vectors) to[i] = pack<T>(f);
         }
       }
-      if (counts) {
-        const Gradient one{zm, zl, p.a, g};
-        if (rank < head) d[rank] = rounded<T>(one(as_float(z[rank]), 0.f));
-        if (rank < p.C - tail) d[tail + rank] = rounded<T>(one(as_float(z[tail + rank]), 0.f));
-      }
       // The columns that the entries write again.  (Of every row that is chosen: when a wait has run out, lists change under their readers and
       // not all threads find the same `counts`, but all come here; and what they then find for a class may be anything.)
       sync_threads<2, THREADS>();
       if (counts) {
-        const Gradient one{zm, zl, p.a, g};
         const int* cls = classes(buf);
         const float* at_entry = at_entries(buf);
         for (int j = rank; j < p.k; j += THREADS) {
