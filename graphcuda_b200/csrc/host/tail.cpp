@@ -184,6 +184,14 @@ Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, 
 }
 
 namespace {
+// Which capture the current stream takes part in; 0: none.
+int64_t recording(const at::Device& dev) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream_of(dev)), &status, &id);
+  if (e != cudaSuccess) raise(std::string("cudaStreamGetCaptureInfo: ") + cudaGetErrorString(e));
+  return status == cudaStreamCaptureStatusActive ? int64_t(id) : 0;
+}
 struct DistillFunction : torch::autograd::Function<DistillFunction> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& Z, const Tensor& top, const Tensor& index,
                         const OptTensor& row_mask, double temperature, double scale) {
@@ -191,16 +199,20 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
     ctx->save_for_backward({f.Z, f.top, f.index, f.stats});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["scale"] = scale;
-    if (f.dz.defined()) ctx->saved_data["dz"] = f.dz;
+    if (f.dz.defined()) {
+      ctx->saved_data["dz"] = f.dz;
+      ctx->saved_data["recording"] = recording(Z.device());
+    }
     return f.loss;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     once("distill_loss");
     const auto saved = ctx->get_saved_variables();
-    // handed out once: whoever differentiates the same graph again may have changed it by then, and gets a buffer of its own
+    // Handed out once: whoever differentiates the same graph again may have changed it by then, and gets a buffer of its own.  And only
+    // within the recording that has filled it, or outside of all: replayed by itself, a backward pass has to write what it returns.
     Tensor dz;
     const auto made = ctx->saved_data.find("dz");
-    if (made != ctx->saved_data.end()) {
+    if (made != ctx->saved_data.end() && ctx->saved_data["recording"].toInt() == recording(saved[0].device())) {
       dz = made->second.toTensor();
       ctx->saved_data.erase(made);
     }
