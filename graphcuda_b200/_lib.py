@@ -74,6 +74,7 @@ SIGNATURES = {
     "gc_logsoftmax_nll_backward_f32": (_int, [_f32p, _i64, _i64p, _void, _i64, _i64, C.c_float, _f32p, _f32p, _i64,
                                               _void, _void]),
     "gc_grouped_linear_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _int]),
+    "gc_grouped_linear_workspace_bytes_for": (_size, [_void, _i64, _void, _i64, _void, _i64, _i64, _i64, _i64, _i64, _int, _int]),
     "gc_grouped_linear_forward_bf16": (_int, [_void, _i64, _void, _i64, _i32p, _i64, _i64, _i64, _i64, _void, _i64, _void, _size, _void]),
     "gc_grouped_linear_backward_bf16": (_int, [_void, _i64, _void, _i64, _void, _i64, _i32p, _i64, _i64, _i64, _i64, _void, _i64, _void,
                                                _void, _size, _void]),

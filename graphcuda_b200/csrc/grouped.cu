@@ -670,6 +670,28 @@ int weights_product(const Matrix& x, const Matrix& dy, const int32_t* offsets, i
   return gc::check_launch("grouped_sum_kernel");
 }
 
+// A call's operands, of which it copies those that cannot be read in place.
+struct Operands {
+  Matrix dy, x, w;
+  bool needs_dy, needs_x, needs_w;
+};
+Operands operands(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, int64_t M, int64_t K,
+                  int64_t N, int64_t G, bool backward, bool dx, bool dw) {
+  return {Matrix{dY, M, N, lddy, 2}, Matrix{X, M, K, ldx, 2}, Matrix{W, G * K, N, ldw, 2}, backward, !backward || dw, !backward || dx};
+}
+// Up to here room for every copy is asked for whatever the operands are, so that a buffer that is kept does not change its size with them.
+constexpr size_t kSmallWorkspace = size_t(1) << 20;
+size_t workspace_of(const Operands& o, int64_t M, int64_t K, int64_t N, int64_t G, bool backward, bool dw) {
+  const size_t all = gc_grouped_linear_workspace_bytes(M, K, N, G, backward);
+  if (all <= kSmallWorkspace) return all;
+  size_t b = 256;  // a workspace there is
+  if (o.needs_dy) b += copy_bytes(o.dy);
+  if (o.needs_x) b += copy_bytes(o.x);
+  if (o.needs_w) b += copy_bytes(o.w);
+  if (dw) b += weights_workspace(M, K, N, G);
+  return std::min(all, b);
+}
+
 int check_sizes(const char* what, int64_t M, int64_t K, int64_t N, int64_t G, int64_t ldw, const int32_t* offsets) {
   GC_REQUIRE(M >= 0 && K >= 0 && N >= 0 && G >= 0, "%s: negative size", what);
   GC_REQUIRE(ldw >= N, "%s: leading dimension below the row length", what);
@@ -695,6 +717,13 @@ size_t gc_grouped_linear_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_
   return backward ? x + dy + w + weights_workspace(M, K, N, G) : x + w;
 }
 
+size_t gc_grouped_linear_workspace_bytes_for(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw,
+                                             int64_t M, int64_t K, int64_t N, int64_t G, int dx, int dw) {
+  if (M <= 0 || K <= 0 || N <= 0 || G <= 0) return 0;
+  const bool backward = dx || dw;
+  return workspace_of(operands(dY, lddy, X, ldx, W, ldw, M, K, N, G, backward, dx, dw), M, K, N, G, backward, dw);
+}
+
 int gc_grouped_linear_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, const int32_t* offsets, int64_t M,
                                    int64_t K, int64_t N, int64_t G, uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes,
                                    void* stream) {
@@ -707,17 +736,17 @@ int gc_grouped_linear_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_
   GC_REQUIRE(Y, "%s: null pointer", what);
   if (K == 0 || G == 0) return zero(Y, ldy, M, N, st, what);
   GC_REQUIRE(X && W, "%s: null pointer", what);
-  if (!workspace || workspace_bytes < gc_grouped_linear_workspace_bytes(M, K, N, G, 0))
+  Operands o = operands(nullptr, 0, X, ldx, W, ldw, M, K, N, G, false, false, false);
+  if (!workspace || workspace_bytes < workspace_of(o, M, K, N, G, false, false))
     return gc::fail(GC_ERR_WORKSPACE, "%s: workspace missing or smaller than its query says", what);
   GC_REQUIRE(gc::aligned16(workspace), "%s: workspace must be 16-byte aligned", what);
   char* ws = static_cast<char*>(workspace);
-  Matrix x{X, M, K, ldx, 2}, w{W, G * K, N, ldw, 2};
   Copies copies{};
-  make_readable(x, ws, copies);
-  make_readable(w, ws, copies);
+  make_readable(o.x, ws, copies);
+  make_readable(o.w, ws, copies);
   rc = run_copies(copies, st);
   if (rc != GC_OK) return rc;
-  return rows_product<kForward>(x, w, offsets, M, K, N, G, reinterpret_cast<bf16*>(Y), ldy, st);
+  return rows_product<kForward>(o.x, o.w, offsets, M, K, N, G, reinterpret_cast<bf16*>(Y), ldy, st);
 }
 
 int gc_grouped_linear_backward_bf16(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw,
@@ -734,18 +763,18 @@ int gc_grouped_linear_backward_bf16(const uint16_t* dY, int64_t lddy, const uint
   }
   if (!dX && !dW) return GC_OK;
   GC_REQUIRE(dY && X && W, "%s: null pointer", what);
-  if (!workspace || workspace_bytes < gc_grouped_linear_workspace_bytes(M, K, N, G, 1))
+  Operands o = operands(dY, lddy, X, ldx, W, ldw, M, K, N, G, true, dX, dW);
+  if (!workspace || workspace_bytes < workspace_of(o, M, K, N, G, true, dW))
     return gc::fail(GC_ERR_WORKSPACE, "%s: workspace missing or smaller than its query says", what);
   GC_REQUIRE(gc::aligned16(workspace), "%s: workspace must be 16-byte aligned", what);
   char* ws = static_cast<char*>(workspace);
-  Matrix dy{dY, M, N, lddy, 2}, x{X, M, K, ldx, 2}, w{W, G * K, N, ldw, 2};
   Copies copies{};
-  make_readable(dy, ws, copies);
-  if (dW) make_readable(x, ws, copies);
-  if (dX) make_readable(w, ws, copies);
+  make_readable(o.dy, ws, copies);
+  if (o.needs_x) make_readable(o.x, ws, copies);
+  if (o.needs_w) make_readable(o.w, ws, copies);
   rc = run_copies(copies, st);
-  if (rc == GC_OK && dX) rc = rows_product<kBack>(dy, w, offsets, M, N, K, G, reinterpret_cast<bf16*>(dX), lddx, st);
-  if (rc == GC_OK && dW) rc = weights_product(x, dy, offsets, M, K, N, G, reinterpret_cast<bf16*>(dW), ws, st);
+  if (rc == GC_OK && dX) rc = rows_product<kBack>(o.dy, o.w, offsets, M, N, K, G, reinterpret_cast<bf16*>(dX), lddx, st);
+  if (rc == GC_OK && dW) rc = weights_product(o.x, o.dy, offsets, M, K, N, G, reinterpret_cast<bf16*>(dW), ws, st);
   return rc;
 }
 

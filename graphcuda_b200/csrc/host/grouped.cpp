@@ -30,7 +30,8 @@ GroupedForward grouped_linear_forward(const Tensor& x, const Tensor& w, const Te
   f.offsets = offsets.contiguous();
   const int64_t M = x.size(0), K = x.size(1), G = w.size(0), N = w.size(2);
   f.y = at::empty({M, N}, x.options());
-  const Scratch ws = product_workspace(abi.gc_grouped_linear_workspace_bytes(M, K, N, G, 0), dev);
+  const Scratch ws = product_workspace(abi.gc_grouped_linear_workspace_bytes_for(nullptr, 0, bits(f.x), ld_of(f.x), bits(f.w),
+                                                                                     std::max<int64_t>(f.w.stride(1), N), M, K, N, G, 0, 0), dev);
   check(abi.gc_grouped_linear_forward_bf16(bits(f.x), ld_of(f.x), bits(f.w), std::max<int64_t>(f.w.stride(1), N),
                                            f.offsets.const_data_ptr<int32_t>(), M, K, N, G, bits_mut(f.y), std::max<int64_t>(N, 1),
                                            ws.ptr, ws.bytes, stream_of(dev)),
@@ -47,7 +48,9 @@ std::pair<Tensor, Tensor> grouped_linear_backward(const Tensor& dy_in, const Ten
   Tensor dx, dw;
   if (need_dx) dx = at::empty({M, K}, x.options());
   if (need_dw) dw = at::empty({G, K, N}, x.options());
-  const Scratch ws = product_workspace(abi.gc_grouped_linear_workspace_bytes(M, K, N, G, 1), dev);
+  const Scratch ws = product_workspace(abi.gc_grouped_linear_workspace_bytes_for(bits(dy), ld_of(dy), bits(x), ld_of(x), bits(w),
+                                                                                     std::max<int64_t>(w.stride(1), N), M, K, N, G, need_dx,
+                                                                                     need_dw), dev);
   check(abi.gc_grouped_linear_backward_bf16(bits(dy), ld_of(dy), bits(x), ld_of(x), bits(w), std::max<int64_t>(w.stride(1), N),
                                             offsets.const_data_ptr<int32_t>(), M, K, N, G, need_dx ? bits_mut(dx) : nullptr,
                                             std::max<int64_t>(K, 1), need_dw ? bits_mut(dw) : nullptr, ws.ptr, ws.bytes, stream_of(dev)),

@@ -50,7 +50,7 @@ inline bool f32_on(const Tensor& t, const at::Device& dev) {
   X(gc_adamw_moments_f32) X(gc_gated_ffn_saved_bytes) X(gc_gated_ffn_workspace_bytes)                              \
   X(gc_gated_ffn_forward_bf16) X(gc_gated_ffn_backward_bf16) X(gc_gated_ffn_e4m3_workspace_bytes)                   \
   X(gc_gated_ffn_forward_e4m3) X(gc_distill_workspace_bytes) X(gc_distill_one_pass) X(gc_distill_forward) X(gc_distill_backward)             \
-  X(gc_grouped_linear_workspace_bytes) X(gc_grouped_linear_forward_bf16) X(gc_grouped_linear_backward_bf16)         \
+  X(gc_grouped_linear_workspace_bytes_for) X(gc_grouped_linear_forward_bf16) X(gc_grouped_linear_backward_bf16)         \
   X(gc_linear_int4_workspace_bytes) X(gc_linear_int4_bf16) X(gc_gated_ffn_int4_workspace_bytes) X(gc_gated_ffn_int4_bf16)
 struct Abi {
 #define X(name) decltype(&::name) name = nullptr;

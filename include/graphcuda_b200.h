@@ -558,6 +558,11 @@ int gc_gated_ffn_forward_e4m3(const uint8_t* X8, int64_t ldx, const float* x_sca
  *   backward   dX[r] = dY[r] W[g]^T and dW[g] = X_g^T dY_g (dW contiguous; either may be null)
  */
 size_t gc_grouped_linear_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int backward);
+/* What one call needs.  The query above answers for any operands, and counts a copy of each, the weights of all groups among them; this one
+ * counts only those that cannot be read in place (16-byte aligned, rows a multiple of 8 elements apart), and where it says less, so
+ * much is enough.  Forward: dx and dw 0, dY unused; backward: which of dX and dW will be asked for. */
+size_t gc_grouped_linear_workspace_bytes_for(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw,
+                                             int64_t M, int64_t K, int64_t N, int64_t G, int dx, int dw);
 int gc_grouped_linear_forward_bf16(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, const int32_t* offsets, int64_t M,
                                    int64_t K, int64_t N, int64_t G, uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes,
                                    void* stream);
