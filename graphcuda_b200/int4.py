@@ -107,7 +107,7 @@ def quantize_weight_int4(w: torch.Tensor, group: int = 64, zero_points: bool = F
         scale = (t.abs().amax(1) / 7.5).bfloat16()
         step = torch.where(scale > 0, scale, 1.0).float()
         zero = torch.full_like(step, 8)
-    codes = (t / step[:, None] + zero[:, None]).round().clamp(0, 15).to(torch.uint8).view(-1, n)[:k]
+    codes = (t / step[:, None] + zero[:, None]).round().clamp(0, 15).to(torch.uint8).view(groups * group, n)[:k]
     return Int4Weight.from_codes(codes, scale, zero.to(torch.uint8) if zero_points else None, group=group)
 
 
