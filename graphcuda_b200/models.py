@@ -118,6 +118,8 @@ def _frozen(module: torch.nn.Module) -> torch.nn.Module:
 class ServedBlock(ResidualBlock):
     """``ResidualBlock`` with its feed-forward block in 8 or 4 bits: weights of their own, those that the block had."""
 
+    bits = 8  # what blocks have that were pickled when there was no choice
+
     def __init__(self, block: ResidualBlock, bits: int = 8):
         torch.nn.Module.__init__(self)
         self.norm_conv, self.conv, self.norm_ffn = (_frozen(m) for m in (block.norm_conv, block.conv, block.norm_ffn))
@@ -136,6 +138,8 @@ class ServedResidualGCN(ResidualGCN):
     """``ResidualGCN`` for inference.  ``bits=8``: the norm in front of a feed-forward block writes 8 bits and a scale per row, which
     the block multiplies with weights laid out in 8 bits once.  ``bits=4``: both weights of every feed-forward block have 4 bits.
     All of its weights are copies: the source may train on, or go."""
+
+    bits = 8  # as in ServedBlock
 
     def __init__(self, model: ResidualGCN, bits: int = 8):
         torch.nn.Module.__init__(self)
