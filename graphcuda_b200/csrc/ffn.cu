@@ -558,7 +558,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           const float sa = F8 ? p.sa[min(row, p.M - 1)] : 1.f;
           const uint32_t scales = staging + C_::kStaging - C_::kScaleBytes + (warp - 4) * 256;
           float fg = 1.f, fu = 1.f;  // H16
-          int eg = 0, eu = 0;
+          int eg = 0, eu = 0, up = 0;
           bool alike = true;
           if (H16) {
             const int n = min(col + lane, p.N - 1), eh = __ldg(p.eh + min(row, p.M - 1));
@@ -568,7 +568,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
             const int eg0 = __shfl_sync(0xFFFFFFFFu, eg, 0), eu0 = __shfl_sync(0xFFFFFFFFu, eu, 0);
             alike = __all_sync(0xFFFFFFFFu, eg == eg0 && eu == eu0 && -126 <= sg && sg <= 40 && -126 <= su && su <= 127);
             if (alike) fg = power(sg), fu = power(su);
-            else fu = power(-eh);
+            up = ea - eh;
           }
           if (F8) {
             const int n = min(col + lane, p.N - 1);
@@ -583,7 +583,8 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               g[i] = times_power(g[i], ea + __shfl_sync(0xFFFFFFFFu, eg, i));
-              u[i] = times_power(u[i], ea + __shfl_sync(0xFFFFFFFFu, eu, i));
+              // (an accumulator lies between 2^-48 and 2^56: beyond these ends it comes to infinity or to nothing either way)
+              u[i] = times_power(u[i], min(max(up + __shfl_sync(0xFFFFFFFFu, eu, i), -252), 254));
             }
           }
           if (!F8 && !H16 && p.exps) {

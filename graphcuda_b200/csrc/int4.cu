@@ -24,10 +24,12 @@
 // Up to 128 rows (64 in the block): int4_tiles.cu.  More than that: the weights are unpacked once into the workspace, 2.5 bytes of traffic per
 // weight, and the tensor-core products of the gated block run on them.  For Y = X W they are bf16 (rounded: 2^-8 of a weight at most, as
 // much as the result's own rounding).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-11,
-// with a power of two per output, row of X and hidden row that keeps fp16's range from mattering; X is copied into fp16, exactly.  A
-// hidden row's power comes from a bound, |x|^2 |w|^2, beside which 2^-24 is the last bit that is kept: less than fp32 sums keep of G and U.
-// 169,343 rows through 256, 1024 and 256 take 275 us (bf16 took 243, with twice the error of a plain form in fp32): 34 for X, 6 for
-// the weights, 150 for the first product and 77 for the second.
+// with a power of two per output, row of X, hidden row and hidden column that keeps fp16's range from mattering; X is copied into fp16, exactly
+// down to 2^-28 of a row's largest.  The powers of hidden rows and columns come from a bound, |x|^2 |Wg| |Wu| with a column's own norms
+// (see column_shift), of which 2^-32 at least is the last bit that is kept; fp32 sums of G and U keep no more.  (With one power per
+// row, from the largest weight of all columns, one column of 64 times the others' size left those an error of 4e-3, and one of 256
+// times 5e-2.)  169,343 rows through 256, 1024 and 256 take 277 us (bf16 took 243, with twice the error of a plain form in fp32): 36 for X,
+// 6 for the weights, 150 for the first product and 77 for the second.
 #include "int4_internal.cuh"
 
 #include <cuda_fp16.h>
@@ -328,17 +330,59 @@ struct ToFp16 {
   const uint8_t* records;
   uint16_t* w;
   int* exps;
-  int* largest;  // of 16 outputs, a power of two's exponent: every weight is below it
   int64_t ldw;
   int zeros, K, N, gpc, parts;
 };
+// The block's hidden columns, as the first weight's outputs say: G's are the first H of them, U's follow.
+struct Columns {
+  int* norms;   // of an output, the exponent of a power of two that its weights, as a vector, are shorter than
+  int2* range;  // the largest and the smallest norm of 16 outputs
+  int* eup;     // U's exponents, which take up what a column is stored larger by
+  int H;
+};
+constexpr int kNoNorm = -(1 << 20);  // of zeros
 __device__ __forceinline__ int common_exponent(int e) { return min((e + 111) / 16 * 16 - 96, 115); }  // from -100 to 115: one as large at least
-__global__ void __launch_bounds__(256)
-int4_unpack_fp16_kernel(const ToFp16 first, const ToFp16 second, int ctas_of_first) {
+
+// A column whose bound, the product of its two norms, lies below the largest is stored larger, times 2^7 or 2^14, and the second weight's
+// rows of it are smaller for it: a bound comes to 2^8 or more, and the largest column has no say in the others' rounding, as long as they lie
+// above 2^-21 of it.  (Below, a bit is lost for every power of two; a larger shift would leave values of 2^112 and above no place beside
+// a row's exponent of 126.)  In steps of 7, so that the columns of a layer mostly share one, for which the first product's epilogue has a short form.
+__device__ __forceinline__ int column_shift(const Columns& c, int k, int top) {
+  const int bound = __ldg(c.norms + k) + __ldg(c.norms + c.H + k);
+  return bound > kNoNorm / 2 ? min((top - bound) / 7 * 7, 14) : 0;
+}
+struct Bounds {
+  int g, u;    // the largest norms of either half
+  bool mixed;  // whether columns may differ in how they are stored
+};
+__device__ __forceinline__ Bounds bounds_of(const Columns& c) {  // by a whole CTA of 256 threads
+  __shared__ int found[8][4];
+  int v[4] = {kNoNorm, kNoNorm, kNoNorm, kNoNorm};  // the largest, and less the smallest, of G's and of U's
+  for (int i = threadIdx.x; i * 16 < 2 * c.H; i += 256) {  // a block on the border is of both halves
+    const int2 r = __ldg(c.range + i);
+    if (i * 16 < c.H) v[0] = max(v[0], r.x), v[1] = max(v[1], -r.y);
+    if (i * 16 + 16 > c.H) v[2] = max(v[2], r.x), v[3] = max(v[3], -r.y);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    v[q] = __reduce_max_sync(0xFFFFFFFFu, v[q]);
+    if (threadIdx.x % 32 == 0) found[threadIdx.x / 32][q] = v[q];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = max(v[q], found[i][q]);
+  return {v[0], v[2], v[0] + v[1] + v[2] + v[3] >= 7};
+}
+
+// FIRST: the weight of G and U, whose norms go to `columns`; otherwise the second one, whose inputs are the columns.
+template <bool FIRST>
+__device__ __forceinline__ void unpack_fp16(const ToFp16& p, int cta, const Columns& columns, bool mixed, int top) {
   __shared__ uint32_t most_s[16];
-  const bool is_first = int(blockIdx.x) < ctas_of_first;
-  const ToFp16& p = is_first ? first : second;
-  const int cta = is_first ? blockIdx.x : blockIdx.x - ctas_of_first, block = cta / p.parts, part = cta % p.parts;
+  __shared__ int norms_s[16];
+  __shared__ __align__(8) uint8_t shift_s[kChunk];
+  const int block = cta / p.parts, part = cta % p.parts;
   const int zeros = p.zeros, K = p.K, N = p.N, gpc = p.gpc;
   const int chunks = (K + kChunk - 1) / kChunk, size = record_bytes(gpc, zeros != 0);
   const uint8_t* r = p.records + int64_t(block) * chunks * size;
@@ -347,23 +391,48 @@ int4_unpack_fp16_kernel(const ToFp16 first, const ToFp16 second, int ctas_of_fir
   const int out = threadIdx.x / 16, piece = threadIdx.x % 16, j = piece / 4, t = piece % 4;  // output, of 16; 8 inputs of a chunk
   const bool exists = block * 16 + out < N;
   uint32_t most = 0;  // as a float's bits
+  double squares = 0.;
   for (int c = piece; c < chunks && exists; c += 16)
-    for (int g = 0; g < gpc && c * kChunk + g * (kChunk / gpc) < K; ++g)
-      most = max(most, gc::ffn::finite_bits(uint32_t(__ldg(reinterpret_cast<const uint16_t*>(r + int64_t(c) * size + kScales) + out * gpc + g)) << 16));
+    for (int g = 0; g < gpc && c * kChunk + g * (kChunk / gpc) < K; ++g) {
+      const uint32_t bits = gc::ffn::finite_bits(uint32_t(__ldg(reinterpret_cast<const uint16_t*>(r + int64_t(c) * size + kScales) + out * gpc + g)) << 16);
+      most = max(most, bits);
+      if (FIRST && part == 0) {
+        const double s = __uint_as_float(bits);
+        squares += s * s * min(kChunk / gpc, K - c * kChunk - g * (kChunk / gpc));
+      }
+    }
   atomicMax(&most_s[out], most);
+  if (FIRST && part == 0) {
+    squares *= zeros ? 225. : 64.;  // codes less zero points: -15 to 15, or -8 to 7
+    for (int o = 8; o > 0; o >>= 1) squares += __shfl_xor_sync(0xFFFFFFFFu, squares, o);
+    const int above = int(__double_as_longlong(squares) >> 52) - 1022;  // squares < 2^above
+    const int norm = squares > 0. ? (above + 1) >> 1 : kNoNorm;
+    if (piece == 0) {
+      norms_s[out] = norm;
+      if (exists) columns.norms[block * 16 + out] = norm;
+    }
+  }
   __syncthreads();
-  const int e = common_exponent(fp16_exponent(__uint_as_float(most_s[out]) * 15.f));  // codes less zero points: -15 to 15
+  // (where inputs are divided by as much as 2^14, outputs' exponents are their own, so that what is divided keeps fp16's 11 bits)
+  const int own = fp16_exponent(__uint_as_float(most_s[out]) * 15.f), e = mixed ? own : common_exponent(own);
   const float f = __uint_as_float(uint32_t(127 - e) << 23);
   if (part == 0 && piece == 0) {
     if (exists) p.exps[block * 16 + out] = e;
-    if (out == 0) {
-      uint32_t all = 0;
-      for (int i = 0; i < 16; ++i) all = max(all, most_s[i]);
-      p.largest[block] = fp16_exponent(__uint_as_float(all) * 15.f) + 14;
+    if (FIRST && out == 0) {
+      int2 range = make_int2(kNoNorm, -kNoNorm);
+      for (int i = 0; i < 16; ++i)
+        if (norms_s[i] != kNoNorm) range.x = max(range.x, norms_s[i]), range.y = min(range.y, norms_s[i]);
+      columns.range[block] = range;
     }
   }
   const int from = int(int64_t(chunks) * part / p.parts), to = int(int64_t(chunks) * (part + 1) / p.parts);
   for (int c = from; c < to; ++c) {
+    if (mixed) {  // the same for all of the CTA
+      __syncthreads();
+      const int k = c * kChunk + threadIdx.x;
+      if (threadIdx.x < kChunk) shift_s[threadIdx.x] = k < K ? uint8_t(column_shift(columns, k, top)) : 0;
+      __syncthreads();
+    }
     const int k = c * kChunk + piece * 8;
     if (k >= K || !exists) continue;
     const uint8_t* at = r + int64_t(c) * size;
@@ -374,33 +443,43 @@ int4_unpack_fp16_kernel(const ToFp16 first, const ToFp16 second, int ctas_of_fir
     unpack(word, zero_pair(zeros ? __ldg(at + zeros_at(gpc) + group) : 8, 0), o);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const __half2 v = __floats2half2_rn(s * __uint_as_float(o[q] << 16), s * __uint_as_float(o[q] & 0xFFFF0000u));
+      float a = s * __uint_as_float(o[q] << 16), b = s * __uint_as_float(o[q] & 0xFFFF0000u);
+      if (mixed) {
+        a *= __uint_as_float((127u - shift_s[piece * 8 + 2 * q]) << 23);
+        b *= __uint_as_float((127u - shift_s[piece * 8 + 2 * q + 1]) << 23);
+      }
+      const __half2 v = __floats2half2_rn(a, b);
       o[q] = *reinterpret_cast<const uint32_t*>(&v);
     }
     *reinterpret_cast<uint4*>(p.w + (int64_t(block) * 16 + out) * p.ldw + k) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
+__global__ void __launch_bounds__(256)
+int4_unpack_fp16_kernel(const ToFp16 p, const Columns columns) {
+  unpack_fp16<true>(p, blockIdx.x, columns, false, 0);
+}
 
-// X as fp16, every row times a power of two, zeros up to a multiple of 8; a warp per row.  eh: for the block's hidden row, of which |x| and the
-// weights' largest powers (`blocks` of them) give a bound: |act(G)| <= |G|, |G|, |U| <= |x| |w| <= |x| sqrt(K) 2^largest.  (|x|^2 in its turn
-// is taken for 32 times the largest of the lanes' sums of squares, one instruction instead of ten.)
+// What follows from the columns: U's exponents, the second weight, and X as fp16, every row times a power of two, zeros up to a multiple of
+// 8.  eh: for the block's hidden row, of which |x| and the largest norms of G's and of U's outputs give a bound, |act(G) U| <= |G| |U| <=
+// |x|^2 |Wg| |Wu|, that comes to 2^15.  The first `row_ctas` CTAs take rows, a warp each; then 256 columns to a CTA; then the weight.
 // SHORT: rows of up to 256 inputs in 16-byte accesses, each a load and a store.  169,343 rows of 256 take 34 us so, and 40 with the loops
 // that other rows need.
 template <bool SHORT>
 __global__ void __launch_bounds__(256)
-int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K, int vec, const int* __restrict__ largest, int blocks,
-                      uint16_t* __restrict__ out, int64_t ldo, int* __restrict__ exps, int* __restrict__ eh) {
-  __shared__ int most_s[8];
+int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K, int vec, const Columns columns, const ToFp16 second,
+                      int row_ctas, int column_ctas, uint16_t* __restrict__ out, int64_t ldo, int* __restrict__ exps, int* __restrict__ eh) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  int top = -1000;
-  for (int i = threadIdx.x; i < blocks; i += 256) top = max(top, __ldg(largest + i));
-  top = __reduce_max_sync(0xFFFFFFFFu, top);
-  if (lane == 0) most_s[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, most_s[i]);
+  const Bounds most_of = bounds_of(columns);
+  const int behind = int(blockIdx.x) - row_ctas;
+  if (behind >= column_ctas) return unpack_fp16<false>(second, behind - column_ctas, columns, most_of.mixed, most_of.g + most_of.u);
+  if (behind >= 0) {
+    const int k = behind * 256 + threadIdx.x;
+    if (most_of.mixed && k < columns.H) columns.eup[k] += column_shift(columns, k, most_of.g + most_of.u);
+    return;
+  }
   const int log_k = 32 - __clz(K);  // 2^log_k > K
-  const int64_t step = int64_t(gridDim.x) * 8;
+  const float unit = __uint_as_float(uint32_t(130 - log_k) << 23);  // sums of squares in 2^(log_k - 3): what is finite stays below 2^14 each
+  const int64_t step = int64_t(row_ctas) * 8;
   uint4 following = make_uint4(0, 0, 0, 0);  // the first 256 inputs of a row are on their way while the one before is written
   for (int64_t m = int64_t(blockIdx.x) * 8 + warp - step; m < M; m += step) {
     auto load_of = [&](const uint16_t* row, int k) {
@@ -459,13 +538,14 @@ int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
     squares2.get(squares, odd);
     squares += odd;
     const bool finite = squares < INFINITY;  // which a NaN is not either
-    squares = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, finite ? __float_as_uint(squares) : 0x7F800000u));
+    uint32_t sum = __reduce_add_sync(0xFFFFFFFFu, finite ? __float2uint_ru(squares * unit) : 0u);
+    if (!__all_sync(0xFFFFFFFFu, finite)) sum = 1u << 31;
     if (lane == 0) {
       exps[m] = e;
-      squares = squares < INFINITY ? 32.f * squares : 0x1p28f * float(K);  // of what is finite: below 2^14 each
-      // squares < 2^log2s; the hidden row stays below 2^15
-      const int log2s = int(__float_as_uint(squares) >> 23) - 127 + 1;
-      eh[m] = squares > 0.f ? min(max(2 * e + log2s + log_k + 2 * top - 15, -100), 112) : 0;
+      const int row = 2 * e + 32 - __clz(sum) + log_k - 3;  // |x|^2 < 2^row
+      // (U times 2^-eh has to be a number by itself: where G is below 2^-97, the row is stored smaller than it could be)
+      const int h = max(row + most_of.g + most_of.u - 15, max(((row + 1) >> 1) + most_of.u - 112, -100));
+      eh[m] = sum > 0 && most_of.g > kNoNorm / 2 && most_of.u > kNoNorm / 2 ? min(h, 126) : 0;
     }
   }
 }
@@ -565,16 +645,18 @@ int unpack_to(const Weights& w, int64_t K, int64_t N, void* to, cudaStream_t st)
       w.records, w.zeros, int(K), int(N), w.gpc(), static_cast<uint16_t*>(to), up8(K));
   return gc::check_launch("int4_unpack_kernel");
 }
-ToFp16 to_fp16(const Weights& w, int64_t K, int64_t N, uint16_t* to, int* exps, int* largest) {
+ToFp16 to_fp16(const Weights& w, int64_t K, int64_t N, uint16_t* to, int* exps) {
   const int64_t parts = std::min(gc::ceil_div(K, kChunk), gc::ceil_div(gc::kNumSMs * 8, gc::ceil_div(N, 16)));
-  return ToFp16{w.records, to, exps, largest, up8(K), w.zeros, int(K), int(N), w.gpc(), int(parts)};
+  return ToFp16{w.records, to, exps, up8(K), w.zeros, int(K), int(N), w.gpc(), int(parts)};
 }
+int64_t ctas_of(const ToFp16& p) { return gc::ceil_div(p.N, 16) * p.parts; }
 size_t unpacked_bytes(int64_t K, int64_t N) { return align256(size_t(N) * up8(K) * 2); }
 
 // The block's operands in the workspace, and what follows them.
 struct Unpacked {
   uint16_t *x, *w_in, *w_out;
-  int *ex, *eh, *ein, *eout, *largest;
+  int *ex, *eh, *ein, *eout, *norms;
+  int2* range;
   void* rest;
   size_t bytes;
 };
@@ -591,7 +673,8 @@ Unpacked unpacked_block(char* ws, int64_t M, int64_t D, int64_t H, int64_t O) {
   u.w_in = static_cast<uint16_t*>(take(unpacked_bytes(D, 2 * H)));
   u.w_out = static_cast<uint16_t*>(take(unpacked_bytes(H, O)));
   u.ex = ints(M), u.eh = ints(M), u.ein = ints(2 * H), u.eout = ints(O);
-  u.largest = ints(gc::ceil_div(2 * H, 16) + gc::ceil_div(O, 16));
+  u.norms = ints(2 * H);
+  u.range = static_cast<int2*>(take(size_t(gc::ceil_div(2 * H, 16)) * sizeof(int2)));
   u.rest = ws ? ws + at : nullptr;
   u.bytes = at;
   return u;
@@ -706,15 +789,16 @@ int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, i
   }
   if (M <= kBlockTileRows) return block_tiles(X, ldx, in, out, M, D, H, O, act, Y, ldy, workspace, st);
   const Unpacked u = unpacked_block(ws, M, D, H, O);
-  const ToFp16 a = to_fp16(in, D, 2 * H, u.w_in, u.ein, u.largest), b = to_fp16(out, H, O, u.w_out, u.eout, u.largest + gc::ceil_div(2 * H, 16));
-  const int64_t ctas = gc::ceil_div(2 * H, 16) * a.parts;
-  int4_unpack_fp16_kernel<<<unsigned(ctas + gc::ceil_div(O, 16) * b.parts), 256, 0, st>>>(a, b, int(ctas));
+  const ToFp16 first = to_fp16(in, D, 2 * H, u.w_in, u.ein), second = to_fp16(out, H, O, u.w_out, u.eout);
+  const Columns columns{u.norms, u.range, u.ein + H, int(H)};
+  int4_unpack_fp16_kernel<<<unsigned(ctas_of(first)), 256, 0, st>>>(first, columns);
   rc = gc::check_launch("int4_unpack_fp16_kernel");
   if (rc != GC_OK) return rc;
   const bool vec = gc::aligned16(X) && ldx % 8 == 0;
   auto rows = vec && D <= 256 && D % 8 == 0 ? int4_rows_fp16_kernel<true> : int4_rows_fp16_kernel<false>;
-  rows<<<unsigned(std::min<int64_t>(gc::ceil_div(M, 8), gc::kNumSMs * 8)), 256, 0, st>>>(
-      X, ldx, int(M), int(D), vec, u.largest, int(gc::ceil_div(2 * H, 16)), u.x, up8(D), u.ex, u.eh);
+  const int row_ctas = int(std::min<int64_t>(gc::ceil_div(M, 8), gc::kNumSMs * 8)), column_ctas = int(gc::ceil_div(H, 256));
+  rows<<<unsigned(row_ctas + column_ctas + ctas_of(second)), 256, 0, st>>>(X, ldx, int(M), int(D), vec, columns, second, row_ctas, column_ctas, u.x,
+                                                                           up8(D), u.ex, u.eh);
   rc = gc::check_launch("int4_rows_fp16_kernel");
   if (rc != GC_OK) return rc;
   return gc::ffn::block_fp16(gc::ffn::BlockFp16{u.x, u.w_in, u.w_out, u.ex, u.eh, u.ein, u.eout}, M, D, H, O, act, Y, ldy, u.rest, st);

@@ -149,7 +149,8 @@ def gated_ffn_int4(x: torch.Tensor, w_in: Int4Weight, w_out: Int4Weight, activat
     and the result are bfloat16.
 
     Up to 64 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
-    rounded to 11 bits, an eighth of the result's own rounding."""
+    rounded to 11 bits, an eighth of the result's own rounding, by powers of two per row and per hidden column: columns of unlike
+    size keep theirs while the norms of their weights, multiplied, differ by less than 2^21."""
     act = _act(activation)
     y = _lib.host.gated_ffn_int4(x, *w_in._parts(), *w_out._parts(), act)
     return y if y is not None else _TracedBlock.apply(x, *w_in._parts(), *w_out._parts(), act)
