@@ -61,6 +61,19 @@ def test_columns_over_a_wide_range_that_the_second_weight_evens_out(m):
         assert error(rows(m, D), gc.quantize_weight_int4(wi, 64), gc.quantize_weight_int4(wo, 32), act) <= ALLOWED
 
 
+@pytest.mark.parametrize("m", [64, 65, 300])
+@pytest.mark.parametrize("power", [0, 3, 6, 9, 12])
+def test_large_groups_that_meet_zeros(m, power):
+    """Weights of inputs, and of hidden columns, that are zero: the others keep their bits beside them."""
+    wi, wo, x = normal(512, 2 * 64, 12), normal(64, 32, 13), rows(m, 512)
+    wi[:32] *= 300
+    x[:, :32] = 0
+    wi[:, :32] = 0  # of G: so these hidden columns are zero
+    wo *= 2.0 ** power  # (wherever that lies among the steps of outputs' exponents)
+    wo[:32] *= 2.0 ** 14
+    assert error(x, gc.quantize_weight_int4(wi, 32), gc.quantize_weight_int4(wo, 32), "silu") <= ALLOWED
+
+
 def test_columns_of_zeros_and_a_weight_of_zeros():
     wi, wo = normal(256, 2 * 96, 8), normal(96, 40, 9)
     wi[:, :40] = 0
