@@ -278,7 +278,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   }, NoGil());
   m.def("distill_backward", [](const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats,
                                double temperature, double scale) {
-    return distill_backward(grad, Z, top, index, stats, Tensor(), temperature, scale);
+    return distill_backward(grad, Z, top, index, stats, Tensor(), 0, temperature, scale);
   }, NoGil());
   m.def("argmax_accuracy", [](const Tensor& logits, const OptTensor& labels, const std::optional<std::vector<Tensor>>& masks,
                               bool want_pred) -> std::optional<std::pair<Tensor, Tensor>> {

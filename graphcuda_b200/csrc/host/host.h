@@ -202,11 +202,12 @@ Tensor nll_loss(const Tensor& Z, const Tensor& labels, const OptTensor& row_mask
 struct DistillForward {
   Tensor loss, Z, top, index, stats;  // as the kernels took them
   Tensor dz;                          // where asked for, and made in the same pass: the buffer of the gradient for a loss's gradient of 1
+  int64_t pad = 0;                    // columns of zeros in it
 };
 DistillForward distill_forward(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
                                double scale, bool want_gradient);
 Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats, const Tensor& dz,
-                        double temperature, double scale);
+                        int64_t dz_pad, double temperature, double scale);
 Tensor distill_loss(const Tensor& Z, const Tensor& top, const Tensor& index, const OptTensor& row_mask, double temperature,
                     double scale);
 std::pair<Tensor, Tensor> argmax_accuracy(const Tensor& logits, const OptTensor& labels,

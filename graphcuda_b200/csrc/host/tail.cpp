@@ -151,6 +151,7 @@ DistillForward distill_forward(const Tensor& Zin, const Tensor& top, const Tenso
   GradientRows rows{C, 0};
   if (want_gradient) {
     rows = gradient_rows(f.Z);
+    f.pad = rows.pad;
     if (abi.gc_distill_one_pass(f.Z.const_data_ptr(), type_of(f.Z), ld_of(f.Z), rows.ld, M, C, top.size(1)))
       f.dz = at::empty({M, rows.ld}, f.Z.options());
   }
@@ -164,13 +165,13 @@ DistillForward distill_forward(const Tensor& Zin, const Tensor& top, const Tenso
   return f;
 }
 
-// dz: the buffer that the forward pass has filled, or undefined
+// dz: the buffer that the forward pass has filled, or undefined; its rows are as they were then (a hook may give Z back with other strides)
 Tensor distill_backward(const Tensor& grad, const Tensor& Z, const Tensor& top, const Tensor& index, const Tensor& stats, const Tensor& dz,
-                        double temperature, double scale) {
+                        int64_t dz_pad, double temperature, double scale) {
   const int64_t M = Z.size(0), C = Z.size(1);
   const at::Device dev = Z.device();
   const c10::cuda::CUDAGuard guard(dev);
-  const GradientRows rows = gradient_rows(Z);
+  const GradientRows rows = dz.defined() ? GradientRows{dz.size(1), dz_pad} : gradient_rows(Z);
   const Tensor buf = dz.defined() ? dz : at::empty({M, rows.ld}, Z.options());
   if (rows.pad) register_zero_padded(buf);
   const Tensor dZ = rows.ld == C ? buf : buf.narrow(1, 0, C);
@@ -201,6 +202,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
     ctx->saved_data["scale"] = scale;
     if (f.dz.defined()) {
       ctx->saved_data["dz"] = f.dz;
+      ctx->saved_data["pad"] = f.pad;
       ctx->saved_data["recording"] = recording(Z.device());
     }
     return f.loss;
@@ -211,12 +213,14 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
     // Handed out once: whoever differentiates the same graph again may have changed it by then, and gets a buffer of its own.  And only
     // within the recording that has filled it, or outside of all: replayed by itself, a backward pass has to write what it returns.
     Tensor dz;
+    int64_t pad = 0;
     const auto made = ctx->saved_data.find("dz");
     if (made != ctx->saved_data.end() && ctx->saved_data["recording"].toInt() == recording(saved[0].device())) {
       dz = made->second.toTensor();
+      pad = ctx->saved_data["pad"].toInt();
       ctx->saved_data.erase(made);
     }
-    return {distill_backward(grads[0], saved[0], saved[1], saved[2], saved[3], dz, ctx->saved_data["temperature"].toDouble(),
+    return {distill_backward(grads[0], saved[0], saved[1], saved[2], saved[3], dz, pad, ctx->saved_data["temperature"].toDouble(),
                              ctx->saved_data["scale"].toDouble()),
             Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
