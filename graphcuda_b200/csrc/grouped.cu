@@ -681,14 +681,18 @@ Operands operands(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t l
 }
 // Up to here room for every copy is asked for whatever the operands are, so that a buffer that is kept does not change its size with them.
 constexpr size_t kSmallWorkspace = size_t(1) << 20;
+size_t workspace_of_all(int64_t M, int64_t K, int64_t N, int64_t G, bool backward, size_t weights) {
+  const size_t x = align256(size_t(M) * up8(K) * 2), dy = align256(size_t(M) * up8(N) * 2), w = align256(size_t(G) * K * up8(N) * 2);
+  return backward ? x + dy + w + weights : x + w;
+}
 size_t workspace_of(const Operands& o, int64_t M, int64_t K, int64_t N, int64_t G, bool backward, bool dw) {
-  const size_t all = gc_grouped_linear_workspace_bytes(M, K, N, G, backward);
+  const size_t weights = backward ? weights_workspace(M, K, N, G) : 0, all = workspace_of_all(M, K, N, G, backward, weights);
   if (all <= kSmallWorkspace) return all;
   size_t b = 256;  // a workspace there is
   if (o.needs_dy) b += copy_bytes(o.dy);
   if (o.needs_x) b += copy_bytes(o.x);
   if (o.needs_w) b += copy_bytes(o.w);
-  if (dw) b += weights_workspace(M, K, N, G);
+  if (dw) b += weights;
   return std::min(all, b);
 }
 
@@ -713,8 +717,7 @@ extern "C" {
 size_t gc_grouped_linear_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t G, int backward) {
   if (M <= 0 || K <= 0 || N <= 0 || G <= 0) return 0;
   // copies of every operand, should none be readable in place
-  const size_t x = align256(size_t(M) * up8(K) * 2), dy = align256(size_t(M) * up8(N) * 2), w = align256(size_t(G) * K * up8(N) * 2);
-  return backward ? x + dy + w + weights_workspace(M, K, N, G) : x + w;
+  return workspace_of_all(M, K, N, G, backward, backward ? weights_workspace(M, K, N, G) : 0);
 }
 
 size_t gc_grouped_linear_workspace_bytes_for(const uint16_t* dY, int64_t lddy, const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw,

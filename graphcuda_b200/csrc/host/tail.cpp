@@ -198,30 +198,24 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
                         const OptTensor& row_mask, double temperature, double scale) {
     const DistillForward f = distill_forward(Z, top, index, row_mask, temperature, scale, true);
     ctx->save_for_backward({f.Z, f.top, f.index, f.stats});
-    ctx->saved_data["temperature"] = temperature;
-    ctx->saved_data["scale"] = scale;
-    if (f.dz.defined()) {
-      ctx->saved_data["dz"] = f.dz;
-      ctx->saved_data["pad"] = f.pad;
-      ctx->saved_data["recording"] = recording(Z.device());
-    }
+    const int64_t where = f.dz.defined() ? recording(Z.device()) : 0;
+    ctx->saved_data["call"] = std::vector<double>{temperature, scale, double(f.pad), double(where)};
+    if (f.dz.defined()) ctx->saved_data["dz"] = f.dz;
     return f.loss;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     once("distill_loss");
     const auto saved = ctx->get_saved_variables();
+    const std::vector<double> call = ctx->saved_data["call"].toDoubleVector();
     // Handed out once: whoever differentiates the same graph again may have changed it by then, and gets a buffer of its own.  And only
     // within the recording that has filled it, or outside of all: replayed by itself, a backward pass has to write what it returns.
     Tensor dz;
-    int64_t pad = 0;
     const auto made = ctx->saved_data.find("dz");
-    if (made != ctx->saved_data.end() && ctx->saved_data["recording"].toInt() == recording(saved[0].device())) {
+    if (made != ctx->saved_data.end() && int64_t(call[3]) == recording(saved[0].device())) {
       dz = made->second.toTensor();
-      pad = ctx->saved_data["pad"].toInt();
       ctx->saved_data.erase(made);
     }
-    return {distill_backward(grads[0], saved[0], saved[1], saved[2], saved[3], dz, pad, ctx->saved_data["temperature"].toDouble(),
-                             ctx->saved_data["scale"].toDouble()),
+    return {distill_backward(grads[0], saved[0], saved[1], saved[2], saved[3], dz, int64_t(call[2]), call[0], call[1]),
             Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
