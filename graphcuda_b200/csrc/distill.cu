@@ -479,10 +479,6 @@ struct Ring {
 constexpr int kListWords = 3;
 constexpr int kOnePassList = 256;  // entries of a list
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
 template <int BARRIER, int THREADS>
 __device__ __forceinline__ void sync_threads() { asm volatile("bar.sync %0, %1;" ::"n"(BARRIER), "n"(THREADS) : "memory"); }
 

@@ -77,10 +77,6 @@ __device__ __forceinline__ __nv_bfloat162 zero_pair(uint32_t zeros, int byte) {
   const uint32_t t = __byte_perm(zeros, 0xC3u, 0x4040u + 0x0101u * byte);
   return *reinterpret_cast<const __nv_bfloat162*>(&t);
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
 __device__ __forceinline__ uint4 shared_16(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
