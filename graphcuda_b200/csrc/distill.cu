@@ -483,7 +483,7 @@ template <int BARRIER, int THREADS>
 __device__ __forceinline__ void sync_threads() { asm volatile("bar.sync %0, %1;" ::"n"(BARRIER), "n"(THREADS) : "memory"); }
 
 // THREADS that make a row's statistics, as many that make the gradient of the row before, a warp whose first lane fetches segments, and
-// one that fetches lists a row ahead (two loads after each other, which the row's threads would wait for).  Persistent over rows.  (4096 x 65,536 in bf16, forward and backward: 212 us, 5.1 TB/s
+// one that fetches lists a row ahead (two loads after each other, which the row's threads would wait for).  Persistent over rows.  (4096 x 65,536 in bf16, forward and backward: 217 us, 5.0 TB/s
 // of the bytes that cannot be avoided; 285 with the same threads doing one after the other, whose exponentials of a row wait for its
 // sums; 231 with 256 threads and 13 segments of 16 KB, 220 with 384 and 9.  What is left is issue slots: 16 instructions per logit,
 // the special function unit half busy.)

@@ -23,7 +23,8 @@
 //
 // Up to 128 rows (64 in the block): int4_tiles.cu.  More than that: the weights are unpacked once into the workspace, 2.5 bytes of traffic per
 // weight, and the tensor-core products of the gated block run on them.  For Y = X W they are bf16 (rounded: 2^-8 of a weight at most, as
-// much as the result's own rounding).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-11,
+// much as the result's own rounding; fp16 as in the block would need X's copy too, 35 us beside 34 for all of 169,343 rows through 256 and
+// 256).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-11,
 // with a power of two per output, row of X, hidden row and hidden column that keeps fp16's range from mattering; X is copied into fp16, exactly
 // down to 2^-28 of a row's largest.  The powers of hidden rows and columns come from a bound, |x|^2 |Wg| |Wu| with a column's own norms
 // (see column_shift), of which 2^-32 at least is the last bit that is kept; fp32 sums of G and U keep no more.  (With one power per

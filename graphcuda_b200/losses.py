@@ -82,7 +82,12 @@ def distill_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_index: torc
     outside [0, classes) (-1, where a row has fewer) or whose logit is -inf is none; a row without entries, or that
     ``row_mask`` (bool or uint8) leaves out, adds nothing and gets a gradient of zeros.  ``scale`` defaults to 1 / (number of rows
     that ``row_mask`` selects), as in ``log_softmax_nll_loss``.  The factor temperature**2 keeps the gradient's size (it
-    has one 1 / temperature of the student's and one of the teacher's slope).  The teacher has no gradient."""
+    has one 1 / temperature of the student's and one of the teacher's slope).  The teacher has no gradient.
+
+    Where a gradient may be asked for, short rows and rows of some thousands of classes get it in the forward pass, for a loss that is
+    differentiated by itself; it takes as much memory as the logits from then on.  A backward pass whose gradient of the loss is not 1
+    computes it once more.  So a weight beside other losses belongs in ``scale``: ``distill_loss(..., scale=0.5 / n) + other``,
+    not ``0.5 * distill_loss(...) + other``."""
     if scale is None:
         cnt = int(row_mask.sum().item()) if row_mask is not None else logits.size(0)
         scale = 1.0 / max(cnt, 1)
