@@ -95,10 +95,11 @@ struct Params {
   int a_bytes;  // of a k-block of A that are loaded: fewer than a tile's where M is below its rows
   int b_up;     // Gated: where U's columns start in B
   int act;
-  int8_t* exps;     // G's and U's exponents, [2][ceil(N / 32)][M] (Gated: null where G and U are not stored)
+  int8_t* exps;     // G's and U's exponents, [2][ceil(N / 32)][M] (Gated: null where G and U are not stored; H16: steps, see level_step, [ceil(N / 32)][step_pitch])
+  int64_t step_pitch;
   const float* sa;  // e4m3: scales of A's rows and B's columns
   const float* sb;
-  const int* ea;  // H16: exponents of A's rows, B's columns, and (Gated) of the rows that are stored
+  const int* ea;  // H16: exponents of A's rows, B's columns, and (Gated) of the rows that are stored, before their steps
   const int* eb;
   const int* eh;
   bf16* C;  // Plain: the output, for rows that TMA cannot store; else what the rounding of A, or of dG | dU, left; or null
@@ -181,6 +182,14 @@ __device__ __forceinline__ uint32_t pack2_fp16(F2 a) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float power(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }  // of two, -126 to 127
+// H16: how many steps of 2^8 above a row's exponent 32 of its values lie, the largest of them `most` (a float's bits) times the exponent's
+// power, so that it comes to less than 2^15 and to 1 at least (or to what fp32 numbers can be).
+constexpr int kNoStep = -128;  // they are zeros
+__device__ __forceinline__ int level_step(uint32_t most, int exponent) {
+  if (most == 0) return kNoStep;
+  const int e = int(most >> 23) - 127;  // 2^e <= most < 2^(e + 1), or below 2^-126
+  return e > 14 ? (e - 14 + 7) / 8 : e < 0 ? -min((7 - e) / 8, (exponent + 126) / 8) : 0;
+}
 // A float times 2^e, in two steps: e may be -252 to 254.
 __device__ __forceinline__ uint32_t times_power(uint32_t v, int e) {
   return __float_as_uint(__uint_as_float(v) * power(e / 2) * power(e - e / 2));
@@ -608,6 +617,7 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
           const uint32_t bo = acquire();
           if (F8) __syncwarp();  // the scales are written
           with_activation(p.act, [&](auto act) {
+            F2 squares = both(0.f);  // H16: of what is stored
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t w[4], rest[4];
@@ -624,11 +634,44 @@ ffn_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) 
                 if (H16) vg = vg * both(fg), vu = vu * both(fu);
                 const F2 a = activate<decltype(act)::value>(vg, unused) * vu;
                 w[e] = H16 ? pack2_fp16(a) : pack2(a);
+                if (H16) squares = fma2(a, a, squares);
                 if (LO) rest[e] = pack_rest(a, w[e]);
               }
               if (LO && row < p.M && col + 8 * j < p.N)
                 *reinterpret_cast<uint4*>(p.C + row * p.ldc + col + 8 * j) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
               store_unit(lane_at + bo, j, w[0], w[1], w[2], w[3]);
+            }
+            if constexpr (H16) {
+              // Where the largest of the 32 is not between 2^-1 and 2^15, as the sum of their squares tells, the row's exponent is not theirs: they
+              // take one of their own, so many steps of 2^8 away, and ffn_level_kernel brings the row together.
+              float sum, odd;
+              squares.get(sum, odd);
+              sum += odd;
+              const bool away = row < p.M && !(sum >= 8.f && sum < 0x1p30f);
+              int step = 0;
+              if (__any_sync(0xFFFFFFFFu, away)) {
+                uint32_t most = 0;
+                auto value = [&](int i) {
+                  F2 unused;
+                  return activate<decltype(act)::value>(F2(g[i], g[i + 1]) * both(fg), unused) * (F2(u[i], u[i + 1]) * both(fu));
+                };
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                  float a, b;
+                  value(i).get(a, b);
+                  most = max(most, max(finite_bits(__float_as_uint(a)), finite_bits(__float_as_uint(b))));
+                }
+                if (away) step = level_step(most, __ldg(p.eh + row));
+                const F2 half = both(power(step == kNoStep ? 0 : -4 * step));  // 2^(-8 step) in two factors
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  uint32_t w[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) w[e] = pack2_fp16(value(j * 8 + 2 * e) * half * half);
+                  store_unit(lane_at + bo, j, w[0], w[1], w[2], w[3]);
+                }
+              }
+              if (row < p.step_pitch) p.exps[int64_t(col / 32) * p.step_pitch + row] = int8_t(step);  // (0 behind the last row)
             }
           });
           put(&maps.out, bo, col, row0);
@@ -728,6 +771,55 @@ ffn_sum_kernel(const float* __restrict__ parts, int splits, int M, int pitch, bf
         const int c = out_column(n + e, gap_from, gap);
         if (c < c_cols) C[m * ldc + c] = __float2bfloat16_rn(v[e]);
       }
+    }
+  }
+}
+
+// H16: brings the chunks of 32 columns of a hidden row to one exponent, that of the largest: what lies below is divided, in place.  Mostly
+// all have the same, and only the steps are read: 16 rows of a chunk at a time, every 32nd chunk by a thread.
+constexpr int kLevelRows = 128, kLevelAlign = 16;  // rows of a CTA; of a row of steps
+__global__ void __launch_bounds__(256)
+ffn_level_kernel(const int8_t* __restrict__ steps, int64_t pitch, const int* __restrict__ exponents, int M, int columns, uint16_t* __restrict__ hidden,
+                 int64_t ld, int* __restrict__ out) {
+  const int chunks = (columns + 31) / 32;
+  const int64_t row0 = int64_t(blockIdx.x) * kLevelRows, mine = row0 + threadIdx.x % 8 * 16;
+  bool differ = false;
+  if (mine < M) {
+    const uint4* at = reinterpret_cast<const uint4*>(steps + mine);
+    const uint4 first = __ldg(at);
+#pragma unroll 4
+    for (int c = threadIdx.x / 8; c < chunks; c += 32) {
+      const uint4 v = __ldg(at + c * (pitch / 16));
+      differ |= v.x != first.x || v.y != first.y || v.z != first.z || v.w != first.w;
+    }
+  }
+  differ = __syncthreads_or(differ);
+  // two threads for a row
+  __shared__ int found[2][kLevelRows];
+  const int i = threadIdx.x % kLevelRows, half = threadIdx.x / kLevelRows;
+  const int64_t row = row0 + i;
+  int top = kNoStep;
+#pragma unroll 8
+  for (int c = half; c < (row >= M ? 0 : differ ? chunks : 1); c += 2) top = max(top, int(__ldg(steps + c * pitch + row)));
+  found[half][i] = top;
+  __syncthreads();
+  top = max(top, found[1 - half][i]);
+  if (row >= M) return;
+  if (half == 0) out[row] = __ldg(exponents + row) + (top == kNoStep ? 0 : 8 * top);
+  for (int c = half; differ && c < chunks; c += 2) {
+    const int s = __ldg(steps + c * pitch + row);
+    if (s == kNoStep || s == top) continue;
+    const float f = power(max(-8 * (top - s), -64));  // (below 2^-40 nothing is left of what fp16 holds)
+    uint4* at = reinterpret_cast<uint4*>(hidden + row * ld + c * 32);
+    for (int q = 0; q < 4 && c * 32 + q * 8 < ld; ++q) {
+      uint4 v = at[q];
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        w[e] = pack2_fp16(F2(a.x * f, a.y * f));
+      }
+      at[q] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
@@ -961,11 +1053,23 @@ int rows_times(const uint16_t* X, int64_t ldx, const uint16_t* W, int64_t ldw, i
   return plain(x, false, Matrix{W, N, K, ldw, 2}, false, M, N, K, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st);
 }
 
-size_t block_fp16_workspace(int64_t M, int64_t, int64_t H, int64_t O) { return align256(size_t(M) * up8(H) * 2) + plain_workspace(M, O, H); }
+// The hidden row, its steps, and its exponents in the end.
+size_t hidden_fp16_bytes(int64_t M, int64_t H) { return align256(size_t(M) * up8(H) * 2); }
+int64_t step_pitch(int64_t M) { return (M + kLevelAlign - 1) / kLevelAlign * kLevelAlign; }
+size_t steps_bytes(int64_t M, int64_t H) { return align256(size_t(step_pitch(M)) * size_t((H + 31) / 32)); }
+size_t block_fp16_workspace(int64_t M, int64_t, int64_t H, int64_t O) {
+  return hidden_fp16_bytes(M, H) + steps_bytes(M, H) + align256(size_t(M) * 4) + plain_workspace(M, O, H);
+}
 int block_fp16(const BlockFp16& b, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y, int64_t ldy, void* workspace,
                cudaStream_t st) {
   const int64_t hp = up8(H);
-  uint16_t* hidden = static_cast<uint16_t*>(workspace);
+  char* ws = static_cast<char*>(workspace);
+  uint16_t* hidden = reinterpret_cast<uint16_t*>(ws);
+  ws += hidden_fp16_bytes(M, H);
+  int8_t* steps = reinterpret_cast<int8_t*>(ws);
+  ws += steps_bytes(M, H);
+  int* exponents = reinterpret_cast<int*>(ws);
+  ws += align256(size_t(M) * 4);
   const Tile t = pick_tile(kGated, M, H, 1);
   Maps maps;
   Params p{};
@@ -973,13 +1077,18 @@ int block_fp16(const BlockFp16& b, int64_t M, int64_t D, int64_t H, int64_t O, i
   p.b_up = int(H);  // rows of Win: no alignment to keep
   p.act = act;
   p.ea = b.ex; p.eb = b.ein; p.eh = b.eh;
+  p.exps = steps;
+  p.step_pitch = step_pitch(M);
   int rc = error_word(&p.word);
   if (rc == GC_OK) rc = operand_maps(maps, p, Matrix{b.x, M, D, up8(D), 2}, false, Matrix{b.w_in, 2 * H, D, up8(D), 2}, false, t.bn / 2);
   if (rc == GC_OK) rc = make_map(&maps.out, Matrix{hidden, M, H, hp, 2}, 32, 32);
   if (rc == GC_OK) rc = launch_tile_fp16<kGated>(t, maps, p, st);
   if (rc != GC_OK) return rc;
-  return plain(Matrix{hidden, M, H, hp, 2}, false, Matrix{b.w_out, O, H, hp, 2}, false, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0,
-               static_cast<char*>(workspace) + align256(size_t(M) * hp * 2), st, 1, b.eh, b.eout);
+  ffn_level_kernel<<<unsigned(gc::ceil_div(M, kLevelRows)), 256, 0, st>>>(steps, p.step_pitch, b.eh, int(M), int(H), hidden, hp, exponents);
+  rc = gc::check_launch("ffn_level_kernel");
+  if (rc != GC_OK) return rc;
+  return plain(Matrix{hidden, M, H, hp, 2}, false, Matrix{b.w_out, O, H, hp, 2}, false, M, O, H, reinterpret_cast<bf16*>(Y), ldy, 0, 0, ws, st, 1,
+               exponents, b.eout);
 }
 
 }  // namespace ffn

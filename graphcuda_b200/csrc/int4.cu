@@ -26,11 +26,14 @@
 // much as the result's own rounding; fp16 as in the block would need X's copy too, 35 us beside 34 for all of 169,343 rows through 256 and
 // 256).  In the block, where two weights and the hidden row would be rounded so, they are fp16, 2^-11,
 // with a power of two per output, row of X, hidden row and hidden column that keeps fp16's range from mattering; X is copied into fp16, exactly
-// down to 2^-28 of a row's largest.  The powers of hidden rows and columns come from a bound, |x|^2 |Wg| |Wu| with a column's own norms
-// (see column_shift), of which 2^-32 at least is the last bit that is kept; fp32 sums of G and U keep no more.  (With one power per
-// row, from the largest weight of all columns, one column of 64 times the others' size left those an error of 4e-3, and one of 256
-// times 5e-2.)  169,343 rows through 256, 1024 and 256 take 277 us (bf16 took 243, with twice the error of a plain form in fp32): 36 for X,
-// 6 for the weights, 150 for the first product and 77 for the second.
+// down to 2^-28 of a row's largest.  A hidden row's power is what its largest value asks for, whatever that is: the one that it starts with
+// is a guess from norms, 32 columns that do not fit it take another, and a launch after the first product brings a row's columns to the
+// largest's (ffn_level_kernel).  So its values have their 11 bits down to 2^-14 of the largest, and large columns are taken down first, see
+// column_shift.  (With a power from a bound,
+// |x|^2 and the weights' norms, nothing was left of them where channels of X differ by thousands and the weights even that out: it lies
+// that far above.)  169,343 rows through 256, 1024 and 256 take 290 us (280
+// with the bound; bf16 took 243, with twice the error of a plain form in fp32): 36 for X and the second weight, 6 for the first, 155 for the first
+// product, 6 to bring rows together and 77 for the second product.
 #include "int4_internal.cuh"
 
 #include <cuda_fp16.h>
@@ -325,8 +328,9 @@ int4_unpack_kernel(const uint8_t* __restrict__ records, int zeros, int K, int N,
 __device__ __forceinline__ int fp16_exponent(float most) { return max(int(__float_as_uint(most) >> 23) - 127 - 13, -100); }
 
 // Weights as fp16, every output's times a power of two, an output's inputs in a row.  A CTA takes a part of 16 outputs' chunks.  Exponents
-// are multiples of 16: the outputs of a layer mostly share one, which the products' epilogues apply in a multiplication, and the largest weight
-// is 2^-2 at least, of which the last bit of fp16 is 2^-22.
+// are multiples of 16, which brings the largest weight to 2^-2 at least: the outputs of a layer mostly share one, which the products'
+// epilogues apply in a multiplication.  An output whose smallest group would come below fp16's normal numbers so has one of its own, which brings
+// the largest to 2^13 (groups 2^-20 of the largest, whose inputs make up for it, left an error of up to 3e-2 otherwise).
 struct ToFp16 {
   const uint8_t* records;
   uint16_t* w;
@@ -338,19 +342,20 @@ struct ToFp16 {
 struct Columns {
   int* norms;   // of an output, the exponent of a power of two that its weights, as a vector, are shorter than
   int2* range;  // the largest and the smallest norm of 16 outputs
-  int* eup;     // U's exponents, which take up what a column is stored larger by
+  int* eup;     // U's exponents, which take up what a column is divided by
   int H;
 };
 constexpr int kNoNorm = -(1 << 20);  // of zeros
 __device__ __forceinline__ int common_exponent(int e) { return min((e + 111) / 16 * 16 - 96, 115); }  // from -100 to 115: one as large at least
 
-// A column whose bound, the product of its two norms, lies below the largest is stored larger, times 2^7 or 2^14, and the second weight's
-// rows of it are smaller for it: a bound comes to 2^8 or more, and the largest column has no say in the others' rounding, as long as they lie
-// above 2^-21 of it.  (Below, a bit is lost for every power of two; a larger shift would leave values of 2^112 and above no place beside
-// a row's exponent of 126.)  In steps of 7, so that the columns of a layer mostly share one, for which the first product's epilogue has a short form.
+// Columns by the product of their two norms: where these differ, the largest columns are divided by 2^14, those below 2^-7 of the largest
+// by 2^7, those below 2^-14 not, and the second weight's rows of them are multiplied by that: a large column has so much less of a say in the
+// others' rounding.  In steps of 7, so that the columns of a layer mostly share one, for which the first product's epilogue has a short form; two
+// of them, for which fp16's range has room in the second weight.
+constexpr int kMostShift = 14;
 __device__ __forceinline__ int column_shift(const Columns& c, int k, int top) {
   const int bound = __ldg(c.norms + k) + __ldg(c.norms + c.H + k);
-  return bound > kNoNorm / 2 ? min((top - bound) / 7 * 7, 14) : 0;
+  return bound > kNoNorm / 2 ? max(kMostShift - (top - bound) / 7 * 7, 0) : 0;
 }
 struct Bounds {
   int g, u;    // the largest norms of either half
@@ -380,29 +385,31 @@ __device__ __forceinline__ Bounds bounds_of(const Columns& c) {  // by a whole C
 // FIRST: the weight of G and U, whose norms go to `columns`; otherwise the second one, whose inputs are the columns.
 template <bool FIRST>
 __device__ __forceinline__ void unpack_fp16(const ToFp16& p, int cta, const Columns& columns, bool mixed, int top) {
-  __shared__ uint32_t most_s[16];
+  __shared__ uint32_t most_s[16], least_s[16];
   __shared__ int norms_s[16];
   __shared__ __align__(8) uint8_t shift_s[kChunk];
   const int block = cta / p.parts, part = cta % p.parts;
   const int zeros = p.zeros, K = p.K, N = p.N, gpc = p.gpc;
   const int chunks = (K + kChunk - 1) / kChunk, size = record_bytes(gpc, zeros != 0);
   const uint8_t* r = p.records + int64_t(block) * chunks * size;
-  if (threadIdx.x < 16) most_s[threadIdx.x] = 0;
+  if (threadIdx.x < 16) most_s[threadIdx.x] = 0, least_s[threadIdx.x] = 0x7F800000u;
   __syncthreads();
   const int out = threadIdx.x / 16, piece = threadIdx.x % 16, j = piece / 4, t = piece % 4;  // output, of 16; 8 inputs of a chunk
   const bool exists = block * 16 + out < N;
-  uint32_t most = 0;  // as a float's bits
+  uint32_t most = 0, least = 0x7F800000u;  // as a float's bits
   double squares = 0.;
   for (int c = piece; c < chunks && exists; c += 16)
     for (int g = 0; g < gpc && c * kChunk + g * (kChunk / gpc) < K; ++g) {
       const uint32_t bits = gc::ffn::finite_bits(uint32_t(__ldg(reinterpret_cast<const uint16_t*>(r + int64_t(c) * size + kScales) + out * gpc + g)) << 16);
       most = max(most, bits);
+      if (bits) least = min(least, bits);
       if (FIRST && part == 0) {
         const double s = __uint_as_float(bits);
         squares += s * s * min(kChunk / gpc, K - c * kChunk - g * (kChunk / gpc));
       }
     }
   atomicMax(&most_s[out], most);
+  atomicMin(&least_s[out], least);
   if (FIRST && part == 0) {
     squares *= zeros ? 225. : 64.;  // codes less zero points: -15 to 15, or -8 to 7
     for (int o = 8; o > 0; o >>= 1) squares += __shfl_xor_sync(0xFFFFFFFFu, squares, o);
@@ -414,8 +421,9 @@ __device__ __forceinline__ void unpack_fp16(const ToFp16& p, int cta, const Colu
     }
   }
   __syncthreads();
-  // (where inputs are divided by as much as 2^14, outputs' exponents are their own, so that what is divided keeps fp16's 11 bits)
-  const int own = fp16_exponent(__uint_as_float(most_s[out]) * 15.f), e = mixed ? own : common_exponent(own);
+  // (where inputs are multiplied by as much as 2^14, outputs' exponents are their own, so that the other inputs keep fp16's 11 bits)
+  const int own = fp16_exponent(__uint_as_float(most_s[out]) * 15.f), common = common_exponent(own);
+  const int e = mixed ? min(own + kMostShift, 126) : int(least_s[out] >> 23) - 127 - common < -14 ? own : common;
   const float f = __uint_as_float(uint32_t(127 - e) << 23);
   if (part == 0 && piece == 0) {
     if (exists) p.exps[block * 16 + out] = e;
@@ -446,8 +454,8 @@ __device__ __forceinline__ void unpack_fp16(const ToFp16& p, int cta, const Colu
     for (int q = 0; q < 4; ++q) {
       float a = s * __uint_as_float(o[q] << 16), b = s * __uint_as_float(o[q] & 0xFFFF0000u);
       if (mixed) {
-        a *= __uint_as_float((127u - shift_s[piece * 8 + 2 * q]) << 23);
-        b *= __uint_as_float((127u - shift_s[piece * 8 + 2 * q + 1]) << 23);
+        a *= __uint_as_float((127u + shift_s[piece * 8 + 2 * q]) << 23);
+        b *= __uint_as_float((127u + shift_s[piece * 8 + 2 * q + 1]) << 23);
       }
       const __half2 v = __floats2half2_rn(a, b);
       o[q] = *reinterpret_cast<const uint32_t*>(&v);
@@ -461,8 +469,10 @@ int4_unpack_fp16_kernel(const ToFp16 p, const Columns columns) {
 }
 
 // What follows from the columns: U's exponents, the second weight, and X as fp16, every row times a power of two, zeros up to a multiple of
-// 8.  eh: for the block's hidden row, of which |x| and the largest norms of G's and of U's outputs give a bound, |act(G) U| <= |G| |U| <=
-// |x|^2 |Wg| |Wu|, that comes to 2^15.  The first `row_ctas` CTAs take rows, a warp each; then 256 columns to a CTA; then the weight.
+// 8.  The first `row_ctas` CTAs take rows, a warp each; then 256 columns to a CTA; then the weight.
+// eh: where the hidden row's values are to lie, from |x| and the largest norms of G's and of U's outputs.  |act(G) U| is at most |x|^2
+// |Wg| |Wu| and mostly, as sums of products that do not know of each other, a K-th of that or less: the largest of 32 such come to some 2^5.
+// (Where they do not, the first product's epilogue sees it and takes another exponent.)
 // SHORT: rows of up to 256 inputs in 16-byte accesses, each a load and a store.  169,343 rows of 256 take 34 us so, and 40 with the loops
 // that other rows need.
 template <bool SHORT>
@@ -475,7 +485,7 @@ int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
   if (behind >= column_ctas) return unpack_fp16<false>(second, behind - column_ctas, columns, most_of.mixed, most_of.g + most_of.u);
   if (behind >= 0) {
     const int k = behind * 256 + threadIdx.x;
-    if (most_of.mixed && k < columns.H) columns.eup[k] += column_shift(columns, k, most_of.g + most_of.u);
+    if (most_of.mixed && k < columns.H) columns.eup[k] -= column_shift(columns, k, most_of.g + most_of.u);
     return;
   }
   const int log_k = 32 - __clz(K);  // 2^log_k > K
@@ -544,8 +554,9 @@ int4_rows_fp16_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
     if (lane == 0) {
       exps[m] = e;
       const int row = 2 * e + 32 - __clz(sum) + log_k - 3;  // |x|^2 < 2^row
-      // (U times 2^-eh has to be a number by itself: where G is below 2^-97, the row is stored smaller than it could be)
-      const int h = max(row + most_of.g + most_of.u - 15, max(((row + 1) >> 1) + most_of.u - 112, -100));
+      // (U times 2^-eh has to be a number by itself: the second term, for G below 2^-90 or so)
+      const int bound = row + most_of.g + most_of.u - (most_of.mixed ? kMostShift + 3 : 0);  // (columns are then spread over 7 powers below it)
+      const int h = max(bound - log_k - 10, max(((row + 1) >> 1) + most_of.u - 112, -126));
       eh[m] = sum > 0 && most_of.g > kNoNorm / 2 && most_of.u > kNoNorm / 2 ? min(h, 126) : 0;
     }
   }

@@ -150,9 +150,9 @@ def gated_ffn_int4(x: torch.Tensor, w_in: Int4Weight, w_out: Int4Weight, activat
     and the result are bfloat16.
 
     Up to 64 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
-    rounded to 11 bits, an eighth of the result's own rounding.  They are held in fp16 with powers of two per output, row and hidden
-    column.  A hidden value's come from the bound |x|^2 |Wg| |Wu| with its own column's weights: it keeps the 11 bits down to 2^-22 of
-    that (typical are 1 / inputs; where large weights meet only zeros, or large inputs, it is less), if the bound is above 2^-21 of the largest column's."""
+    rounded to 11 bits, an eighth of the result's own rounding: they are held in fp16 with powers of two per output and row, a hidden row
+    so that it keeps them down to 2^-14 of its largest value (columns whose weights are larger than others' by a factor of up to 2^14 are
+    taken down by it first)."""
     act = _act(activation)
     y = _lib.host.gated_ffn_int4(x, *w_in._parts(), *w_out._parts(), act)
     return y if y is not None else _TracedBlock.apply(x, *w_in._parts(), *w_out._parts(), act)

@@ -1,6 +1,7 @@
 """Gated blocks with 4-bit weights where a few weights or inputs are far larger than the others.
 
-A hidden column's rounding is of its own size: what another column, or an input that few weights take up, comes to has no say in it.  The
+A hidden value's rounding is of its own size, down to 2^-14 of its row's largest: what a bound over the row, an input that few weights
+take up, or a weight that meets zeros would come to has no say in it.  The
 error on average is the documented one (see test_int4_gpu): the result's rounding, 2^-8 / sqrt(3) at most, and above 64 rows an
 eighth of that each for both weights, the hidden row, and once more for the slope."""
 import pytest
@@ -72,6 +73,64 @@ def test_large_groups_that_meet_zeros(m, power):
     wo *= 2.0 ** power  # (wherever that lies among the steps of outputs' exponents)
     wo[:32] *= 2.0 ** 14
     assert error(x, gc.quantize_weight_int4(wi, 32), gc.quantize_weight_int4(wo, 32), "silu") <= ALLOWED
+
+
+@pytest.mark.parametrize("m", [64, 65, 300])
+@pytest.mark.parametrize("d,zeros", [(64, False), (64, True), (512, True), (4096, False), (4096, True)])
+@pytest.mark.parametrize("act", ["silu", "relu"])
+def test_inputs_of_all_sizes_that_the_weights_even_out(m, d, zeros, act):
+    """Channels of the input differ by some thousands, and so do the weights that take them up: what they come to is far below the
+    product of the row's length and the weights'."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    size = torch.exp(2 * torch.randn(d, generator=g, device=DEV))
+    wi, wo = normal(d, 2 * 256, 14), normal(256, 128, 15)
+    wi = wi / size[:, None] * torch.exp(1.5 * torch.randn(2 * 256, generator=g, device=DEV))
+    wo = wo * torch.exp(2 * torch.randn(256, generator=g, device=DEV))[:, None]
+    x = (rows(m, d).float() * size).bfloat16()
+    assert error(x, gc.quantize_weight_int4(wi, 32, zeros), gc.quantize_weight_int4(wo, 32, zeros), act) <= ALLOWED
+
+
+@pytest.mark.parametrize("power", [10, 16, 20])
+@pytest.mark.parametrize("inputs", [32, 2048])
+def test_small_groups_whose_inputs_make_up_for_it(power, inputs):
+    for shift in (0, 5, 10):  # wherever that lies among the steps of outputs' exponents
+        wi, wo, x = normal(D, 2 * 256, 22) * 2.0 ** shift, normal(256, 128, 23), rows(300, D).float()
+        wi[:inputs] *= 2.0 ** -power
+        x[:, :inputs] *= 2.0 ** power
+        assert error(x.bfloat16(), gc.quantize_weight_int4(wi, 32), gc.quantize_weight_int4(wo, 32), "silu") <= ALLOWED
+
+
+@pytest.mark.parametrize("m", [65, 300])
+@pytest.mark.parametrize("times", [300, 4096, 65_536])
+def test_large_weights_of_inputs_that_are_zero(m, times):
+    wi, wo, x = normal(D, 2 * H, 16), normal(H, O, 17), rows(m, D)
+    wi[7] *= times
+    x[:, 7] = 0
+    assert error(x, gc.quantize_weight_int4(wi, 32), gc.quantize_weight_int4(wo, 32), "silu") <= ALLOWED
+
+
+@pytest.mark.parametrize("m", [65, 300])
+@pytest.mark.parametrize("times", [1000.0, 1e5])
+def test_a_large_input_that_no_weight_takes_up(m, times):
+    wi, wo, x = normal(D, 2 * H, 18), normal(H, O, 19), rows(m, D)
+    x[:, 40] = times
+    wi[40] = 0
+    assert error(x, gc.quantize_weight_int4(wi, 32), gc.quantize_weight_int4(wo, 32), "gelu") <= ALLOWED
+
+
+def test_rows_of_all_sizes():
+    """Rows that follow the gate and the other weights closely, rows that hardly meet any, and rows of zeros, side by side."""
+    wi, wo, x = normal(256, 2 * 96, 20), normal(96, 40, 21), rows(200, 256).float()
+    x[1::5] = wi[:, 5] * 1000
+    x[2::5] = wi[:, 96 + 5] * 1e-3
+    x[3::5, 1:] = 0
+    x[4::5] = 0
+    q, o, x = gc.quantize_weight_int4(wi, 32), gc.quantize_weight_int4(wo, 32), x.bfloat16()
+    for first in range(4):
+        got = gc.gated_ffn_int4(x, q, o)[first::5]
+        G, U = (x[first::5].double() @ q.dequantize().double()).split(96, 1)
+        assert rms(got, (act64("silu", G)[0] * U) @ o.dequantize().double()) <= ALLOWED
+    assert not gc.gated_ffn_int4(x, q, o)[4::5].any()
 
 
 def test_columns_of_zeros_and_a_weight_of_zeros():
