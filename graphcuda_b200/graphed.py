@@ -35,7 +35,7 @@ class GraphedTrainStep:
                  row_mask: Optional[torch.Tensor] = None, warmup: int = 3):
         self.model, self.adj, self.optimizer = model, adj, optimizer
         self.X, self.labels, self.row_mask = X, labels, row_mask
-        self.scale = 1.0 / max(int(row_mask.sum().item()) if row_mask is not None else X.size(0), 1)
+        self.scale = 1.0 / max(int(row_mask.count_nonzero()) if row_mask is not None else X.size(0), 1)
         side = torch.cuda.Stream(device=X.device)
         side.wait_stream(torch.cuda.current_stream(X.device))
         with torch.cuda.stream(side):

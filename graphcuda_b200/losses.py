@@ -64,7 +64,7 @@ def log_softmax_nll_loss(logits: torch.Tensor, labels: torch.Tensor, row_mask: O
     count, or for a different normalisation (e.g. 1 / global rows in the
     row-partitioned model)."""
     if scale is None:
-        cnt = int(row_mask.sum().item()) if row_mask is not None else logits.size(0)
+        cnt = int(row_mask.count_nonzero()) if row_mask is not None else logits.size(0)
         scale = 1.0 / max(cnt, 1)
     loss = _lib.host.nll_loss(logits, labels, row_mask, scale)
     return loss if loss is not None else _TracedLoss.apply(logits, labels, row_mask, scale)
@@ -89,7 +89,7 @@ def distill_loss(logits: torch.Tensor, top_logits: torch.Tensor, top_index: torc
     computes it once more.  So a weight beside other losses belongs in ``scale``: ``distill_loss(..., scale=0.5 / n) + other``,
     not ``0.5 * distill_loss(...) + other``."""
     if scale is None:
-        cnt = int(row_mask.sum().item()) if row_mask is not None else logits.size(0)
+        cnt = int(row_mask.count_nonzero()) if row_mask is not None else logits.size(0)
         scale = 1.0 / max(cnt, 1)
     loss = _lib.host.distill_loss(logits, top_logits, top_index, row_mask, temperature, scale)
     if loss is not None:
