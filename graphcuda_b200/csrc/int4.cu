@@ -28,7 +28,7 @@
 // with a power of two per output, row of X, hidden row and hidden column that keeps fp16's range from mattering; X is copied into fp16, exactly
 // down to 2^-28 of a row's largest.  A hidden row's power is what its largest value asks for, whatever that is: the one that it starts with
 // is a guess from norms, 32 columns that do not fit it take another, and a launch after the first product brings a row's columns to the
-// largest's (ffn_level_kernel).  So its values have their 11 bits down to 2^-14 of the largest, and large columns are taken down first, see
+// largest's (ffn_level_kernel).  So its values have their 11 bits down to 2^-13 of the largest, and large columns are taken down first, see
 // column_shift.  (With a power from a bound,
 // |x|^2 and the weights' norms, nothing was left of them where channels of X differ by thousands and the weights even that out: it lies
 // that far above.)  169,343 rows through 256, 1024 and 256 take 290 us (280

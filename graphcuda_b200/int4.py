@@ -152,7 +152,7 @@ def gated_ffn_int4(x: torch.Tensor, w_in: Int4Weight, w_out: Int4Weight, activat
     Up to 64 rows nothing is rounded on the way but the result.  For more rows the weights and the hidden row between the products are
     rounded to 11 bits, an eighth of the result's own rounding: they and ``x`` are held in fp16 with powers of two per output and row.  What
     keeps fewer bits is a value of ``x`` below 2^-28 of its row's largest, a group of weights below 2^-23 of its output's largest, and a
-    hidden value below 2^-14 of its row's largest (columns whose weights are larger than others' by a factor of up to 2^14 are taken down
+    hidden value below 2^-13 of its row's largest (columns whose weights are larger than others' by a factor of up to 2^14 are taken down
     by it first)."""
     act = _act(activation)
     y = _lib.host.gated_ffn_int4(x, *w_in._parts(), *w_out._parts(), act)

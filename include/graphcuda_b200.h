@@ -587,7 +587,7 @@ int gc_linear_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* W, int gr
                         uint16_t* Y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* The gated feed-forward block (see gc_gated_ffn_forward_bf16) with both weights so: Win has D inputs and 2H outputs, [Wg | Wu], Wout H
  * and O.  Up to 64 rows nothing is rounded on the way but Y; above, weights and hidden row to 11 bits (fp16 with exponents per output and row: a
- * hidden value has them down to 2^-14 of the largest of its row, where columns with larger weights are first taken down by up to 2^14). */
+ * hidden value has them down to 2^-13 of the largest of its row, where columns with larger weights are first taken down by up to 2^14). */
 size_t gc_gated_ffn_int4_workspace_bytes(int64_t M, int64_t D, int64_t H, int64_t O);
 int gc_gated_ffn_int4_bf16(const uint16_t* X, int64_t ldx, const uint8_t* Win, int group_in, int zero_points_in, const uint8_t* Wout,
                            int group_out, int zero_points_out, int64_t M, int64_t D, int64_t H, int64_t O, int act, uint16_t* Y,

@@ -1,6 +1,6 @@
 """Gated blocks with 4-bit weights where a few weights or inputs are far larger than the others.
 
-A hidden value's rounding is of its own size, down to 2^-14 of its row's largest: what a bound over the row, an input that few weights
+A hidden value's rounding is of its own size, down to 2^-13 of its row's largest: what a bound over the row, an input that few weights
 take up, or a weight that meets zeros would come to has no say in it.  The
 error on average is the documented one (see test_int4_gpu): the result's rounding, 2^-8 / sqrt(3) at most, and above 64 rows an
 eighth of that each for both weights, the hidden row, and once more for the slope."""
